@@ -416,6 +416,33 @@ int nsw_skip_conv_accumulate(const void* x, const void* inv, const float* w, voi
                              int64_t C_x, int64_t C_inv, int64_t C_out, int64_t H, int64_t W, int64_t frame0,
                              int64_t out_bstride, int x_dtype, int model_dtype, int out_dtype, void* stream);
 
+/* The norms around a residual branch with its gate and residual scale, and
+ * their gradients (no counterpart in the reference, whose blocks are pre-norm
+ * without gates: models/swin_helpers.py:435-459):
+ *   n = branch / sqrt(mean(branch^2) + eps) * post_w   (post_w NULL: n = branch)
+ *   y = alpha * skip + gate * n                        (gate NULL: 1)
+ *   z = y / sqrt(mean(y^2) + eps) * norm_w             (norm_w and z NULL: no z)
+ * branch, skip, y, z [rows, C]; post_w, norm_w [C]; gate [G, C], row r taking
+ * gate row r / (rows / G) (G = 1: one gate for all rows).  All of one dtype,
+ * 16-byte aligned; C a multiple of 8 (bf16) / 4 (fp32), at most 8192 / 4096.
+ * Outputs must not overlap inputs. */
+int nsw_residual_norm(const void* branch, const void* skip, const void* post_w, const void* gate,
+                      const void* norm_w, void* y, void* z, int64_t rows, int64_t C, int64_t G, float alpha,
+                      float eps, int dtype, void* stream);
+
+/* Gradients of nsw_residual_norm from those of y and z (dy may be NULL: zero;
+ * dz and norm_w are given together or both NULL): dbranch and dskip [rows, C],
+ * and where not NULL dpost_w [C], dgate [G, C], dnorm_w [C] (rows == 0: zeros).
+ * Sums over rows in a fixed order.  Workspace (16-byte aligned) of
+ * nsw_residual_norm_backward_workspace_size bytes, 0 for sizes that are
+ * refused. */
+size_t nsw_residual_norm_backward_workspace_size(int64_t rows, int64_t C, int64_t G, int dtype);
+int nsw_residual_norm_backward(const void* dy, const void* dz, const void* branch, const void* skip,
+                               const void* post_w, const void* gate, const void* norm_w, void* dbranch, void* dskip,
+                               void* dpost_w, void* dgate, void* dnorm_w, int64_t rows, int64_t C, int64_t G,
+                               float alpha, float eps, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* HBM stream probe.  No counterpart in the reference: a measurement helper
  * for callers that report kernel rates against what the device sustains
  * (bench.py's achievable peaks).  dst == NULL: reads `bytes` from src with

@@ -1,0 +1,558 @@
+// The norms around a branch of a pre-norm block, with its gate and residual:
+//
+//   n = branch * ro * post_w      ro = 1 / sqrt(mean(branch^2) + eps)   (post_w NULL: n = branch)
+//   y = alpha * skip + gate * n   gate of the row's sample              (gate NULL: 1)
+//   z = y * ry * norm_w           ry = 1 / sqrt(mean(y^2) + eps)        (norm_w NULL: no z)
+//
+// and the gradients of all of it.  Values are held in fp32 from the loads to the
+// stores: z is of the unrounded y.  The backward pass forms y again from branch and
+// skip (the same bytes as reading y, without y's rounding):
+//
+//   t  = dz * norm_w,  d  = dy + ry * (t - yh * mean(t * yh))     yh = y * ry
+//   dskip = alpha * d
+//   s  = d * gate * post_w,  dbranch = ro * (s - oh * mean(s * oh))   oh = branch * ro
+//   S[sample, c] = sum over the sample's rows of d * oh,  Q[c] = sum over rows of dz * yh
+//   dgate = post_w * S,  dpost_w = sum over samples of gate * S,  dnorm_w = Q
+//
+// Bound by HBM: one pass over the rows, each element read and written once.  A
+// workgroup takes a range of one sample's rows, a row at a time on LPR lanes (narrow
+// rows, several to a wave), a wave, or the whole workgroup (wide rows), so that a
+// lane's columns stay the same: the parameters live in registers, and so do the
+// lane's sums for S and Q, which go to a partial row of the workgroup and from there
+// through a second kernel in a fixed order (no atomics: the same bits every time).
+// The next row's loads are issued before the present row's arithmetic.
+#include <algorithm>
+
+#include "nsw_common.h"
+
+namespace nsw {
+
+namespace {
+
+constexpr int NT = 256;   // threads of a workgroup
+
+struct NormArgs {
+  const void *branch, *skip, *post_w, *gate, *norm_w;
+  const void *dy, *dz;
+  void *y, *z, *dbranch, *dskip;
+  float* part;            // [G P][2][C] sums of the workgroups: S, Q
+  int64_t R;              // rows of a sample
+  int64_t per;            // rows of a workgroup
+  int P;                  // workgroups of a sample
+  int C;
+  float alpha, eps;
+};
+
+// LPR lanes hold a row of up to LPR * CH 16-byte pieces; LPR = NT: the workgroup.
+template <typename T, int LPR_, int CH_> struct RowCfg {
+  static constexpr int LPR = LPR_, CH = CH_, VEC = Vec16<T>::N;
+  static constexpr bool WG = LPR_ == NT;
+  static constexpr int RPS = NT / LPR_;              // rows in flight at once
+  static constexpr int WIDTH = LPR_ * CH_ * VEC;     // widest row
+};
+
+template <class CFG>
+struct Lane {
+  int lr, slot;
+  __device__ __forceinline__ Lane() : lr((int)threadIdx.x % CFG::LPR), slot((int)threadIdx.x / CFG::LPR) {}
+  __device__ __forceinline__ int col(int k) const { return (lr + CFG::LPR * k) * CFG::VEC; }
+};
+
+// Sums over the lanes of a row, on each of them.  Workgroup rows: the waves' sums
+// meet in LDS, red[turn & 1]; two turns apart a barrier lies between a buffer's reads
+// and its next writes.
+template <class CFG, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[2][4], int& turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = row16_sum(v[i]);
+    if constexpr (CFG::LPR == 32) v[i] = rows2_sum(v[i]);
+    if constexpr (CFG::LPR >= 64) v[i] = rows4_sum(v[i]);
+  }
+  if constexpr (CFG::WG) {
+    float(*r)[4] = red[turn & 1];
+    ++turn;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i][threadIdx.x >> 6] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (r[i][0] + r[i][1]) + (r[i][2] + r[i][3]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const u32x4& raw, float* out) {
+  if constexpr (sizeof(T) == 2) {
+    const bf16x8 v = __builtin_bit_cast(bf16x8, raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = (float)v[i];
+  } else {
+    const f32x4 v = __builtin_bit_cast(f32x4, raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = v[i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 narrow(const float* in) {
+  if constexpr (sizeof(T) == 2) {
+    bf16x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (bf16)in[i];
+    return __builtin_bit_cast(u32x4, v);
+  } else {
+    return __builtin_bit_cast(u32x4, f32x4{in[0], in[1], in[2], in[3]});
+  }
+}
+
+// The lane's pieces of row `row` (zeros past the row's end).
+template <typename T, class CFG>
+__device__ __forceinline__ void load_row(const void* p, int64_t row, int C, const Lane<CFG>& ln, u32x4 (&raw)[CFG::CH]) {
+#pragma unroll
+  for (int k = 0; k < CFG::CH; ++k) {
+    const int c = ln.col(k);
+    raw[k] = u32x4{0, 0, 0, 0};
+    if (c < C) raw[k] = *reinterpret_cast<const u32x4*>((const T*)p + row * C + c);
+  }
+}
+
+// A parameter's values for the lane's columns (1 where there is none; 0 past the end).
+template <typename T, class CFG>
+__device__ __forceinline__ void load_param(const void* p, int C, const Lane<CFG>& ln, float (&w)[CFG::CH][CFG::VEC]) {
+#pragma unroll
+  for (int k = 0; k < CFG::CH; ++k) {
+    const int c = ln.col(k);
+#pragma unroll
+    for (int e = 0; e < CFG::VEC; ++e) w[k][e] = c < C ? 1.f : 0.f;
+    if (p != nullptr && c < C) load16<T>((const T*)p + c, w[k]);
+  }
+}
+
+template <typename T, class CFG>
+__global__ __launch_bounds__(NT) void residual_norm_kernel(NormArgs a) {
+  constexpr int CH = CFG::CH, VEC = CFG::VEC;
+  __shared__ float red[2][2][4];
+  int turn = 0;
+  const Lane<CFG> ln;
+  const int C = a.C, g = (int)(blockIdx.x / (unsigned)a.P), p = (int)(blockIdx.x % (unsigned)a.P);
+  const int64_t base = g * a.R, r0 = base + p * a.per, r1 = r0 + a.per < base + a.R ? r0 + a.per : base + a.R;
+  const bool post = a.post_w != nullptr, pre = a.norm_w != nullptr;
+  const float inv = 1.f / (float)C;
+  float wg[CH][VEC], wn[CH][VEC];
+  {   // gate * post_w: one factor of the normalised branch
+    float w[CH][VEC];
+    load_param<T, CFG>(a.post_w, C, ln, w);
+    load_param<T, CFG>(a.gate == nullptr ? nullptr : (const T*)a.gate + (int64_t)g * C, C, ln, wg);
+    load_param<T, CFG>(a.norm_w, C, ln, wn);
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) wg[k][e] *= w[k][e];
+  }
+  u32x4 ro_[CH], rx_[CH];
+  auto fetch = [&](int64_t row, u32x4(&o)[CH], u32x4(&x)[CH]) {
+    row = row < r1 ? row : r1 - 1;
+    load_row<T, CFG>(a.branch, row, C, ln, o);
+    load_row<T, CFG>(a.skip, row, C, ln, x);
+  };
+  fetch(r0 + ln.slot, ro_, rx_);
+  for (int64_t r = r0; r < r1; r += CFG::RPS) {
+    const int64_t row = r + ln.slot;
+    u32x4 no_[CH], nx_[CH];
+    fetch(row + CFG::RPS, no_, nx_);
+    float o[CH][VEC], y[CH][VEC];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      widen<T>(ro_[k], o[k]);
+      widen<T>(rx_[k], y[k]);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[0] = fmaf(o[k][e], o[k][e], s[0]);
+    }
+    float ro = 1.f;
+    if (post) {
+      row_sums<CFG>(s, red, turn);
+      ro = 1.f / sqrtf(s[0] * inv + a.eps);
+    }
+    s[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        y[k][e] = fmaf(a.alpha, y[k][e], (o[k][e] * ro) * wg[k][e]);
+        s[0] = fmaf(y[k][e], y[k][e], s[0]);
+      }
+    const bool ok = row < r1;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.y + row * C + ln.col(k)) = narrow<T>(y[k]);
+    if (pre) {
+      row_sums<CFG>(s, red, turn);
+      const float ry = 1.f / sqrtf(s[0] * inv + a.eps);
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) y[k][e] = (y[k][e] * ry) * wn[k][e];
+        if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.z + row * C + ln.col(k)) = narrow<T>(y[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      ro_[k] = no_[k];
+      rx_[k] = nx_[k];
+    }
+  }
+}
+
+// The workgroup's sum of v over the slots of its lanes' columns, into dst [C].
+template <class CFG>
+__device__ __forceinline__ void store_part(float (&v)[CFG::CH][CFG::VEC], float* buf, float* dst, int C, const Lane<CFG>& ln) {
+  if constexpr (CFG::RPS == 1) {
+#pragma unroll
+    for (int k = 0; k < CFG::CH; ++k)
+      if (ln.col(k) < C) {
+#pragma unroll
+        for (int e = 0; e < CFG::VEC; e += 4)
+          *reinterpret_cast<f32x4*>(dst + ln.col(k) + e) = f32x4{v[k][e], v[k][e + 1], v[k][e + 2], v[k][e + 3]};
+      }
+  } else {
+    __syncthreads();   // the buffer's earlier use
+#pragma unroll
+    for (int k = 0; k < CFG::CH; ++k)
+#pragma unroll
+      for (int e = 0; e < CFG::VEC; e += 4)
+        *reinterpret_cast<f32x4*>(buf + ln.slot * CFG::WIDTH + ln.col(k) + e) =
+            f32x4{v[k][e], v[k][e + 1], v[k][e + 2], v[k][e + 3]};
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += NT) {
+      float t = 0.f;
+#pragma unroll
+      for (int s = 0; s < CFG::RPS; ++s) t += buf[s * CFG::WIDTH + c];
+      dst[c] = t;
+    }
+  }
+}
+
+template <typename T, class CFG>
+__global__ __launch_bounds__(NT) void residual_norm_backward_kernel(NormArgs a) {
+  constexpr int CH = CFG::CH, VEC = CFG::VEC;
+  __shared__ float red[2][2][4];
+  __shared__ __attribute__((aligned(16))) float buf[CFG::RPS == 1 ? 4 : CFG::RPS * CFG::WIDTH];
+  int turn = 0;
+  const Lane<CFG> ln;
+  const int C = a.C, g = (int)(blockIdx.x / (unsigned)a.P), p = (int)(blockIdx.x % (unsigned)a.P);
+  const int64_t base = g * a.R, r0 = base + p * a.per, r1 = r0 + a.per < base + a.R ? r0 + a.per : base + a.R;
+  const bool post = a.post_w != nullptr, pre = a.norm_w != nullptr, has_dy = a.dy != nullptr;
+  const float inv = 1.f / (float)C;
+  float wg[CH][VEC], wn[CH][VEC], S[CH][VEC], Q[CH][VEC];
+  {   // gate * post_w: the factor of the normalised branch, and of d on its way back
+    float w[CH][VEC];
+    load_param<T, CFG>(a.post_w, C, ln, w);
+    load_param<T, CFG>(a.gate == nullptr ? nullptr : (const T*)a.gate + (int64_t)g * C, C, ln, wg);
+    load_param<T, CFG>(a.norm_w, C, ln, wn);
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        wg[k][e] *= w[k][e];
+        S[k][e] = 0.f;
+        Q[k][e] = 0.f;
+      }
+  }
+  u32x4 ro_[CH], rx_[CH], ry_[CH], rz_[CH];
+  auto fetch = [&](int64_t row, u32x4(&o)[CH], u32x4(&x)[CH], u32x4(&dy)[CH], u32x4(&dz)[CH]) {
+    row = row < r1 ? row : r1 - 1;
+    load_row<T, CFG>(a.branch, row, C, ln, o);
+    if (pre) load_row<T, CFG>(a.skip, row, C, ln, x);
+    if (has_dy) load_row<T, CFG>(a.dy, row, C, ln, dy);
+    if (pre) load_row<T, CFG>(a.dz, row, C, ln, dz);
+  };
+#pragma unroll
+  for (int k = 0; k < CH; ++k) rx_[k] = ry_[k] = rz_[k] = u32x4{0, 0, 0, 0};
+  if (r0 < r1) fetch(r0 + ln.slot, ro_, rx_, ry_, rz_);
+  for (int64_t r = r0; r < r1; r += CFG::RPS) {
+    const int64_t row = r + ln.slot;
+    const bool ok = row < r1;
+    u32x4 no_[CH], nx_[CH], ny_[CH], nz_[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) nx_[k] = ny_[k] = nz_[k] = u32x4{0, 0, 0, 0};
+    fetch(row + CFG::RPS, no_, nx_, ny_, nz_);
+    float oh[CH][VEC], d[CH][VEC];
+    float s1[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      widen<T>(ro_[k], oh[k]);
+      widen<T>(ry_[k], d[k]);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s1[0] = fmaf(oh[k][e], oh[k][e], s1[0]);
+    }
+    float ro = 1.f;
+    if (post) {
+      row_sums<CFG>(s1, red, turn);
+      ro = 1.f / sqrtf(s1[0] * inv + a.eps);
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) oh[k][e] *= ro;
+    }
+    if (pre) {
+      float y[CH][VEC], dz[CH][VEC];
+      float s2[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        widen<T>(rx_[k], y[k]);
+        widen<T>(rz_[k], dz[k]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          y[k][e] = fmaf(a.alpha, y[k][e], oh[k][e] * wg[k][e]);
+          s2[0] = fmaf(y[k][e], y[k][e], s2[0]);
+          s2[1] = fmaf(dz[k][e] * wn[k][e], y[k][e], s2[1]);
+        }
+      }
+      row_sums<CFG>(s2, red, turn);
+      const float ry = 1.f / sqrtf(s2[0] * inv + a.eps);
+      const float m = (s2[1] * ry) * inv;          // mean(t * yh)
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float yh = y[k][e] * ry;
+          d[k][e] = fmaf(ry, fmaf(-yh, m, dz[k][e] * wn[k][e]), d[k][e]);
+          Q[k][e] = fmaf(ok ? dz[k][e] : 0.f, ok ? yh : 0.f, Q[k][e]);
+        }
+    }
+    float s3[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      float ds[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        ds[e] = a.alpha * d[k][e];
+        S[k][e] = fmaf(ok ? d[k][e] : 0.f, ok ? oh[k][e] : 0.f, S[k][e]);
+        d[k][e] *= wg[k][e];
+        s3[0] = fmaf(d[k][e], oh[k][e], s3[0]);
+      }
+      if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.dskip + row * C + ln.col(k)) = narrow<T>(ds);
+    }
+    if (post) {
+      row_sums<CFG>(s3, red, turn);
+      const float m = s3[0] * inv;
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[k][e] = ro * fmaf(-oh[k][e], m, d[k][e]);
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.dbranch + row * C + ln.col(k)) = narrow<T>(d[k]);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      ro_[k] = no_[k];
+      rx_[k] = nx_[k];
+      ry_[k] = ny_[k];
+      rz_[k] = nz_[k];
+    }
+  }
+  float* dst = a.part + (int64_t)blockIdx.x * 2 * C;
+  store_part<CFG>(S, buf, dst, C, ln);
+  store_part<CFG>(Q, buf, dst + C, C, ln);
+}
+
+// dgate, dpost_w and dnorm_w from the workgroups' partial rows [G P][2][C], 32
+// columns to a workgroup: 8 lanes hold 4 columns each, 32 groups of them take every
+// 32nd partial row and meet in LDS, always in the same order.
+template <typename T>
+__global__ __launch_bounds__(NT) void residual_norm_params_kernel(const float* __restrict__ part, int G, int P, int C,
+                                                                  const T* __restrict__ post_w, const T* __restrict__ gate,
+                                                                  T* __restrict__ dpost, T* __restrict__ dgate,
+                                                                  T* __restrict__ dnorm) {
+  __shared__ __attribute__((aligned(16))) float red[32][36];
+  const int cl = ((int)threadIdx.x & 7) * 4, grp = (int)threadIdx.x >> 3;
+  const int c = (int)blockIdx.x * 32 + cl;
+  const bool in = c < C;
+  // the sum over rows [p0, p1) of partial array h, for the thread's 4 columns where grp == 0
+  auto sum = [&](int64_t p0, int64_t p1, int h) {
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    if (in) {
+#pragma unroll 4
+      for (int64_t p = p0 + grp; p < p1; p += 32) t += *reinterpret_cast<const f32x4*>(part + (p * 2 + h) * C + c);
+    }
+    __syncthreads();
+    *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
+    __syncthreads();
+    if (grp < 4) {
+      t = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += *reinterpret_cast<const f32x4*>(&red[grp * 8 + i][cl]);
+    }
+    __syncthreads();
+    if (grp < 4) *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+      for (int i = 1; i < 4; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
+    }
+    return t;
+  };
+  const bool out = in && grp == 0;
+  if (dpost != nullptr || dgate != nullptr) {
+    float w[4] = {1.f, 1.f, 1.f, 1.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
+    if (post_w != nullptr && in) load4<T>(post_w + c, w);
+    for (int g = 0; g < G; ++g) {
+      const f32x4 s = sum((int64_t)g * P, (int64_t)(g + 1) * P, 0);
+      if (!out) continue;
+      float gt[4] = {1.f, 1.f, 1.f, 1.f}, dg[4];
+      if (gate != nullptr) load4<T>(gate + (int64_t)g * C + c, gt);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dg[e] = w[e] * s[e];
+        dp[e] = fmaf(gt[e], s[e], dp[e]);
+      }
+      if (dgate != nullptr) store4<T>(dgate + (int64_t)g * C + c, dg);
+    }
+    if (dpost != nullptr && out) store4<T>(dpost + c, dp);
+  }
+  if (dnorm != nullptr) {
+    const f32x4 q = sum(0, (int64_t)G * P, 1);
+    const float v[4] = {q[0], q[1], q[2], q[3]};
+    if (out) store4<T>(dnorm + c, v);
+  }
+}
+
+// Workgroups of a sample: enough to fill the chip `per_cu` times over in all, each
+// with at least one turn of rows.
+struct Split {
+  int64_t per;
+  int P;
+};
+inline Split split_rows(int64_t R, int64_t G, int rps, int per_cu) {
+  const int64_t turns = (R + rps - 1) / rps;
+  const int64_t want = std::max<int64_t>(1, (256 * per_cu + G - 1) / G);
+  const int64_t each = std::max<int64_t>(1, (turns + want - 1) / want);
+  return {each * rps, (int)((turns + each - 1) / each)};
+}
+
+constexpr int FWD_PER_CU = 16, BWD_PER_CU = 4;
+
+// f(RowCfg) for the narrowest shape that holds C.
+template <typename T, class F>
+int with_cfg(int64_t C, F f) {
+  if (C <= RowCfg<T, 16, 1>::WIDTH) return f(RowCfg<T, 16, 1>{});
+  if (C <= RowCfg<T, 32, 1>::WIDTH) return f(RowCfg<T, 32, 1>{});
+  if (C <= RowCfg<T, 64, 1>::WIDTH) return f(RowCfg<T, 64, 1>{});
+  if (C <= RowCfg<T, 64, 2>::WIDTH) return f(RowCfg<T, 64, 2>{});
+  if (C <= RowCfg<T, NT, 2>::WIDTH) return f(RowCfg<T, NT, 2>{});
+  return f(RowCfg<T, NT, 4>{});
+}
+
+int check_norm(const char* what, int64_t rows, int64_t C, int64_t G, int dtype, const void* gate) {
+  NSW_CHECK_ARG(dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32, "%s: unknown dtype %d", what, dtype);
+  const int64_t vec = dtype == NSW_DTYPE_BF16 ? 8 : 4;
+  NSW_CHECK_ARG(rows >= 0 && rows < (1LL << 40), "%s: rows=%lld out of range", what, (long long)rows);
+  NSW_CHECK_ARG(C > 0 && C % vec == 0 && C <= vec * 1024, "%s: C=%lld must be a multiple of %lld, at most %lld", what,
+                (long long)C, (long long)vec, (long long)(vec * 1024));
+  NSW_CHECK_ARG(G >= 1 && G <= (1 << 20) && rows % G == 0, "%s: rows=%lld must be a multiple of the gate's rows G=%lld",
+                what, (long long)rows, (long long)G);
+  NSW_CHECK_ARG(gate != nullptr || G == 1, "%s: G=%lld without a gate", what, (long long)G);
+  return NSW_OK;
+}
+
+template <typename T>
+int64_t backward_parts(int64_t rows, int64_t C, int64_t G) {
+  int64_t n = 0;
+  with_cfg<T>(C, [&](auto cfg) {
+    n = (int64_t)split_rows(rows / G, G, decltype(cfg)::RPS, BWD_PER_CU).P * G;
+    return 0;
+  });
+  return n;
+}
+
+template <typename T>
+int launch_forward(NormArgs a, int64_t rows, int64_t G, hipStream_t st) {
+  if (rows == 0) return NSW_OK;
+  return with_cfg<T>(a.C, [&](auto cfg) {
+    using CFG = decltype(cfg);
+    const Split s = split_rows(rows / G, G, CFG::RPS, FWD_PER_CU);
+    a.R = rows / G; a.per = s.per; a.P = s.P;
+    hipLaunchKernelGGL((residual_norm_kernel<T, CFG>), dim3((unsigned)(G * s.P)), dim3(NT), 0, st, a);
+    return check_launch("nsw_residual_norm");
+  });
+}
+
+template <typename T>
+int launch_backward(NormArgs a, int64_t rows, int64_t G, void* dpost, void* dgate, void* dnorm, hipStream_t st) {
+  const char* what = "nsw_residual_norm_backward";
+  int P = 0;
+  int rc = with_cfg<T>(a.C, [&](auto cfg) {
+    using CFG = decltype(cfg);
+    const Split s = split_rows(rows / G, G, CFG::RPS, BWD_PER_CU);
+    a.R = rows / G; a.per = s.per; a.P = P = s.P;
+    if (rows == 0) return (int)NSW_OK;
+    hipLaunchKernelGGL((residual_norm_backward_kernel<T, CFG>), dim3((unsigned)(G * s.P)), dim3(NT), 0, st, a);
+    return check_launch(what);
+  });
+  if (rc || (!dpost && !dgate && !dnorm)) return rc;
+  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 31) / 32)), dim3(NT), 0, st, a.part, (int)G, P,
+                     a.C, (const T*)a.post_w, (const T*)a.gate, (T*)dpost, (T*)dgate, (T*)dnorm);
+  return check_launch(what);
+}
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+
+}  // namespace
+
+}  // namespace nsw
+
+using namespace nsw;
+
+extern "C" int nsw_residual_norm(const void* branch, const void* skip, const void* post_w, const void* gate,
+                                 const void* norm_w, void* y, void* z, int64_t rows, int64_t C, int64_t G, float alpha,
+                                 float eps, int dtype, void* stream) {
+  const char* what = "nsw_residual_norm";
+  if (int rc = check_norm(what, rows, C, G, dtype, gate)) return rc;
+  NSW_CHECK_ARG(rows == 0 || (branch && skip && y), "%s: branch, skip and y are required", what);
+  NSW_CHECK_ARG(rows == 0 || (norm_w != nullptr) == (z != nullptr), "%s: z is written where norm_w is given", what);
+  NSW_CHECK_ARG(aligned16({branch, skip, post_w, gate, norm_w, y, z}), "%s: pointers must be 16-byte aligned", what);
+  NormArgs a{};
+  a.branch = branch; a.skip = skip; a.post_w = post_w; a.gate = gate; a.norm_w = norm_w;
+  a.y = y; a.z = z; a.C = (int)C; a.alpha = alpha; a.eps = eps;
+  return dtype == NSW_DTYPE_BF16 ? launch_forward<bf16>(a, rows, G, (hipStream_t)stream)
+                                 : launch_forward<float>(a, rows, G, (hipStream_t)stream);
+}
+
+extern "C" size_t nsw_residual_norm_backward_workspace_size(int64_t rows, int64_t C, int64_t G, int dtype) {
+  if (check_norm("nsw_residual_norm_backward_workspace_size", rows, C, G, dtype, &rows) != NSW_OK) return 0;
+  const int64_t n = dtype == NSW_DTYPE_BF16 ? backward_parts<bf16>(rows, C, G) : backward_parts<float>(rows, C, G);
+  return (size_t)(std::max<int64_t>(n, 1) * 2 * C) * sizeof(float);
+}
+
+extern "C" int nsw_residual_norm_backward(const void* dy, const void* dz, const void* branch, const void* skip,
+                                          const void* post_w, const void* gate, const void* norm_w, void* dbranch,
+                                          void* dskip, void* dpost_w, void* dgate, void* dnorm_w, int64_t rows, int64_t C,
+                                          int64_t G, float alpha, float eps, int dtype, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  const char* what = "nsw_residual_norm_backward";
+  if (int rc = check_norm(what, rows, C, G, dtype, gate)) return rc;
+  NSW_CHECK_ARG(rows == 0 || (branch && skip && dbranch && dskip), "%s: branch, skip, dbranch and dskip are required", what);
+  NSW_CHECK_ARG(rows == 0 || dy || dz, "%s: dy or dz is required", what);
+  NSW_CHECK_ARG(rows == 0 || (norm_w != nullptr) == (dz != nullptr), "%s: dz and norm_w go together", what);
+  NSW_CHECK_ARG((!dpost_w || post_w) && (!dgate || gate) && (!dnorm_w || norm_w),
+                "%s: a gradient of a parameter that is not given", what);
+  NSW_CHECK_ARG(aligned16({dy, dz, branch, skip, post_w, gate, norm_w, dbranch, dskip, dpost_w, dgate, dnorm_w, workspace}),
+                "%s: pointers must be 16-byte aligned", what);
+  const size_t need = nsw_residual_norm_backward_workspace_size(rows, C, G, dtype);
+  NSW_CHECK_ARG(workspace != nullptr && workspace_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", what, need,
+                workspace ? workspace_bytes : (size_t)0);
+  NormArgs a{};
+  a.branch = branch; a.skip = skip; a.post_w = post_w; a.gate = gate; a.norm_w = norm_w;
+  a.dy = dy; a.dz = dz; a.dbranch = dbranch; a.dskip = dskip; a.part = (float*)workspace;
+  a.C = (int)C; a.alpha = alpha; a.eps = eps;
+  return dtype == NSW_DTYPE_BF16 ? launch_backward<bf16>(a, rows, G, dpost_w, dgate, dnorm_w, (hipStream_t)stream)
+                                 : launch_backward<float>(a, rows, G, dpost_w, dgate, dnorm_w, (hipStream_t)stream);
+}

@@ -104,6 +104,10 @@ SIGNATURES = {
     "nsw_head_unpatchify": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp]),
     "nsw_skip_conv_accumulate": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                         _int, _int, _int, _vp]),
+    "nsw_residual_norm": (_int, [_vp] * 7 + [_i64, _i64, _i64, _f32, _f32, _int, _vp]),
+    "nsw_residual_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
+    "nsw_residual_norm_backward": (_int, [_vp] * 12 + [_i64, _i64, _i64, _f32, _f32, _int, _vp, ctypes.c_size_t,
+                                                       _vp]),
 }
 
 _lib = None

@@ -7,6 +7,7 @@ all arithmetic runs in libnsw's kernels).  Inputs must be contiguous,
 """
 from __future__ import annotations
 
+import contextlib
 import threading
 from typing import Optional, Sequence, Tuple
 
@@ -181,6 +182,91 @@ def rmsnorm_roll_partition(x: torch.Tensor, weight: torch.Tensor, window_size, s
                                            C, ws0, ws1, int(shift_size[0]), int(shift_size[1]),
                                            dtype_code(x), _stream(dev)), "rmsnorm_roll_partition")
     return out
+
+
+def _guard(dev: torch.device):
+    """Makes dev the current device for a launch on its stream."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps):
+    """(device, rows, C, G, eps) of a residual_norm, its arguments checked."""
+    dev = _dev(branch, skip, post_weight, gate, norm_weight)
+    _same_dtype(branch, skip, post_weight, gate, norm_weight)
+    if branch.dim() < 1 or branch.shape != skip.shape:
+        raise ValueError(f"{what}: branch {tuple(branch.shape)} and skip {tuple(skip.shape)} must have one shape")
+    C = branch.shape[-1]
+    if C == 0:
+        raise ValueError(f"{what}: no features")
+    rows = branch.numel() // C
+    for name, t in (("post_weight", post_weight), ("norm_weight", norm_weight)):
+        if t is not None and tuple(t.shape) != (C,):
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({C},)")
+    G = 1
+    if gate is not None:
+        if gate.dim() not in (1, 2) or gate.shape[-1] != C or gate.numel() == 0:
+            raise ValueError(f"{what}: gate has shape {tuple(gate.shape)}, expected ({C},) or (G, {C})")
+        G = gate.numel() // C
+        if rows % G:
+            raise ValueError(f"{what}: {rows} rows are not a multiple of the gate's {G}")
+    return dev, rows, C, G, default_eps(branch.dtype) if eps is None else float(eps)
+
+
+def residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, alpha: float = 1.0,
+                  norm_weight: Optional[torch.Tensor] = None, eps: Optional[float] = None
+                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(y, z): y = alpha * skip + gate * RMSNorm(branch; post_weight) and
+    z = RMSNorm(y; norm_weight), the end of one residual branch and the norm
+    before the next, in one pass.  branch and skip [..., C]; post_weight None:
+    the branch is not normalised; gate [C] (a layer scale) or [G, C], the rows
+    of G equal parts of the batch each under their own gate, None: 1;
+    norm_weight None: z is None.  Statistics, and z's y, in fp32."""
+    dev, rows, C, G, eps = _residual_norm_args("residual_norm", branch, skip, post_weight, gate, norm_weight, eps)
+    y = torch.empty_like(branch)
+    z = None if norm_weight is None else torch.empty_like(branch)
+    with _guard(dev):
+        check(lib().nsw_residual_norm(branch.data_ptr(), skip.data_ptr(), _p(post_weight), _p(gate), _p(norm_weight),
+                                      y.data_ptr(), _p(z), rows, C, G, float(alpha), eps, dtype_code(branch),
+                                      _stream(dev)), "residual_norm")
+    return y, z
+
+
+def residual_norm_backward(dy: Optional[torch.Tensor], dz: Optional[torch.Tensor], branch: torch.Tensor,
+                           skip: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
+                           gate: Optional[torch.Tensor] = None, alpha: float = 1.0,
+                           norm_weight: Optional[torch.Tensor] = None, eps: Optional[float] = None):
+    """(dbranch, dskip, dpost_weight, dgate, dnorm_weight) of residual_norm from
+    the gradients of y and z, None for what was None.  dy or dz may be None
+    (zero)."""
+    what = "residual_norm_backward"
+    dev, rows, C, G, eps = _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps)
+    if dy is None and dz is None:
+        raise ValueError(f"{what}: dy or dz is required")
+    if dz is not None and norm_weight is None:
+        raise ValueError(f"{what}: dz without norm_weight")
+    for t in (dy, dz):
+        if t is not None:
+            if _dev(t) != dev:
+                raise RuntimeError("libnsw op arguments are on different devices")
+            _same_dtype(branch, t)
+            if t.shape != branch.shape:
+                raise ValueError(f"{what}: gradient of shape {tuple(t.shape)}, expected {tuple(branch.shape)}")
+    db, ds = torch.empty_like(branch), torch.empty_like(branch)
+    dp = None if post_weight is None else torch.empty_like(post_weight)
+    dg = None if gate is None else torch.empty_like(gate)
+    # without dz the norm before the next branch has no part in the gradients
+    dn = None if norm_weight is None else torch.zeros_like(norm_weight) if dz is None else torch.empty_like(norm_weight)
+    nw = None if dz is None else norm_weight
+    code = dtype_code(branch)
+    nbytes = int(lib().nsw_residual_norm_backward_workspace_size(rows, C, G, code))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        check(lib().nsw_residual_norm_backward(_p(dy), _p(dz), branch.data_ptr(), skip.data_ptr(), _p(post_weight),
+                                               _p(gate), _p(nw), db.data_ptr(), ds.data_ptr(), _p(dp), _p(dg),
+                                               None if dz is None else _p(dn), rows, C, G, float(alpha), eps, code,
+                                               ws.data_ptr(), nbytes, _stream(dev)), what)
+    return db, ds, dp, dg, dn
 
 
 # -------------------------------------------------------------------- GEMM ---

@@ -46,6 +46,11 @@ extern "C" {
                                     the reference's TE block ("gelu" activation of
                                     te.LayerNormMLP, models/swin_helpers_te.py:318-323) */
 
+/* Activations of nsw_gated_linear. */
+#define NSW_ACT_SILU 0      /* g / (1 + e^-g)           */
+#define NSW_ACT_GELU 1      /* exact-erf GELU           */
+#define NSW_ACT_GELU_TANH 2 /* tanh-form GELU           */
+
 const char* nsw_last_error(void);
 int nsw_version(void);
 
@@ -136,6 +141,35 @@ int nsw_rmsnorm_roll_partition(const void* x, const void* w, float eps, void* xw
  * and residual. */
 int nsw_linear(const void* x, const void* w, const void* bias, const void* residual, void* y,
                int64_t M, int64_t N, int64_t K, int epilogue, int dtype, void* stream);
+
+/* Gated linear (no counterpart in the reference, whose MLP has one
+ * projection: models/mlp.py:80-85): both projections of a gated feed-forward
+ * block, the activation of the gate and the product in one kernel,
+ *   h[M, H] = act(x . w[0:H]^T + bias[0:H]) * (x . w[H:2H]^T + bias[H:2H]),
+ * x [M, K], w [2H, K] the gate's rows stacked over the up projection's, bias
+ * [2H] or NULL, act NSW_ACT_*.  K and alignment as nsw_linear, H a multiple
+ * of 16, w below 2 GiB (x and h may be larger). */
+int nsw_gated_linear(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K,
+                     int act, int dtype, void* stream);
+
+/* Gradients of nsw_gated_linear from that of h [M, H]: where not NULL dx
+ * [M, K], dw [2H, K] and db [2H].  The two projections are formed again from
+ * x and w, so nothing but the inputs is kept from the forward pass.  Sums over
+ * rows in a fixed order.  Workspace (16-byte aligned) of
+ * nsw_gated_linear_backward_workspace_size bytes, 0 for sizes that are
+ * refused. */
+size_t nsw_gated_linear_backward_workspace_size(int64_t M, int64_t H, int64_t K, int dtype);
+int nsw_gated_linear_backward(const void* dh, const void* x, const void* w, const void* bias, void* dx, void* dw,
+                              void* db, int64_t M, int64_t H, int64_t K, int act, int dtype, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* Gradients of nsw_linear without an activation, y = x . w^T (+ bias) (+
+ * residual, whose gradient is dy): where not NULL dx [M, K] = dy . w, dw
+ * [N, K] = dy^T . x and db [N] = dy's column sums.  N and K multiples of 32
+ * (bf16) / 16 (fp32), 16-byte aligned.  Workspace as above. */
+size_t nsw_linear_backward_workspace_size(int64_t M, int64_t N, int64_t K, int dtype);
+int nsw_linear_backward(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
+                        int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* q/k/v projections with their biases and the per-head q/k RMSNorm
  * (models/swin_helpers.py:216-234): qkv[M, 3C] = x[M,C] . wqkv[3C,C]^T + bqkv,

@@ -52,13 +52,14 @@ static int launch_gemm(const void* x, const void* w, void* y, int64_t M, int64_t
   NSW_CHECK_ARG(K % KT == 0, "%s: K=%lld must be a multiple of %d", what, (long long)K, KT);
   NSW_CHECK_ARG(N % 8 == 0, "%s: N=%lld must be a multiple of 8", what, (long long)N);
   NSW_CHECK_ARG(M < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31), "%s: dims too large", what);
-  NSW_CHECK_ARG((uint64_t)M * K * sizeof(T) < (1ULL << 31) && (uint64_t)N * K * sizeof(T) < (1ULL << 31),
+  constexpr bool GATE = EPI == EPI_GATED || EPI == EPI_GATED_GRAD;   // x addressed tile by tile
+  NSW_CHECK_ARG((GATE || (uint64_t)M * K * sizeof(T) < (1ULL << 31)) && (uint64_t)N * K * sizeof(T) < (1ULL << 31),
                 "%s: operands above 2 GiB are not supported (32-bit buffer offsets)", what);
   NSW_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)w % 16) == 0 && ((uintptr_t)y % 16) == 0 &&
                     ((uintptr_t)ea.residual % 16) == 0,
                 "%s: x, w, y and residual must be 16-byte aligned", what);
   EpiArgs eg = ea;
-  if constexpr (EPI == EPI_BIAS_GELU || EPI == EPI_BIAS_GELU_TANH) {
+  if constexpr (EPI == EPI_BIAS_GELU || EPI == EPI_BIAS_GELU_TANH || GATE) {
     // the MLP's first GEMM: tile groups of ~128 tiles (8 row blocks x 16
     // column blocks at config 2, 16 x 8 at config 4: each measured 5% faster
     // than the other height on its shape)
@@ -185,6 +186,39 @@ int gemm_qkv_rowscale(const void* x, const void* wqkv_n, const void* bqkv, const
   return dispatch_gemm<EPI_QKV_HN16, PRE_ROWSCALE>(dtype, x, wqkv_n, qkv, M, 3 * C, C, ea, stream, what);
 }
 
+// h = act(x . w[:H]^T + bias[:H]) * (x . w[H:]^T + bias[H:]); with dh given, y [M, 2H]
+// = the gradients of the two factors' sums instead, and in colsum (if given) their
+// sums over the rows of each wave row of the tiles (gated_grad_parts of them).
+int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M,
+               int64_t H, int64_t K, int act, int dtype, void* stream, const char* what) {
+  NSW_CHECK_ARG(act == NSW_ACT_SILU || act == NSW_ACT_GELU || act == NSW_ACT_GELU_TANH, "%s: unknown activation %d", what,
+                act);
+  NSW_CHECK_ARG(x && w && y, "%s: x, w and y are required", what);
+  NSW_CHECK_ARG(H > 0 && H % 16 == 0, "%s: H=%lld must be a positive multiple of 16", what, (long long)H);
+  NSW_CHECK_ARG(((uintptr_t)bias % 16) == 0, "%s: bias must be 16-byte aligned", what);
+  EpiArgs ea{};
+  ea.bias = bias; ea.residual = dh; ea.act = act; ea.row_sumsq = colsum;
+  if (dh) return dispatch_gemm<EPI_GATED_GRAD>(dtype, x, w, y, M, 2 * H, K, ea, stream, what);
+  return dispatch_gemm<EPI_GATED>(dtype, x, w, y, M, 2 * H, K, ea, stream, what);
+}
+
+// Rows of gemm_gated's colsum.
+int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
+  static_assert(BigTile::WGM == 2 && MidTile::WGM == 2 && SmallTile::WGM == 2 && SmallF32Tile::WGM == 2 &&
+                    SmallTile::BM == SmallF32Tile::BM, "two wave rows to a tile");
+  const EpiArgs ea{};
+  const TileSize t = dtype == NSW_DTYPE_F32 ? pick_tile<float, EPI_GATED_GRAD>(M, 2 * H, K, ea)
+                                            : pick_tile<bf16, EPI_GATED_GRAD>(M, 2 * H, K, ea);
+  const int64_t bm = t == TILE_BIG ? BigTile::BM : t == TILE_MID ? MidTile::BM : SmallTile::BM;
+  return (M + bm - 1) / bm * 2;
+}
+
+// y[M, N] = x . w^T
+int gemm_plain(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream,
+               const char* what) {
+  return dispatch_gemm<EPI_NONE>(dtype, x, w, y, M, N, K, EpiArgs{}, stream, what);
+}
+
 // y[remap(m)] = x[m] . w^T + bias + residual[m], the stored rows' partial
 // sums of squares (one float per 512 bytes of row) into row_sumsq at the
 // same rows where asked.  map_mode 0: remap(m) = m (row_sumsq required); 1:
@@ -245,6 +279,11 @@ extern "C" int nsw_linear(const void* x, const void* w, const void* bias, const 
       return dispatch_gemm<EPI_BIAS_RESIDUAL>(dtype, x, w, y, M, N, K, ea, stream, what);
     default: return set_error(NSW_ERR_INVALID, "%s: unknown epilogue %d", what, epilogue);
   }
+}
+
+extern "C" int nsw_gated_linear(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K,
+                                int act, int dtype, void* stream) {
+  return gemm_gated(x, w, bias, nullptr, h, nullptr, M, H, K, act, dtype, stream, "nsw_gated_linear");
 }
 
 extern "C" int nsw_qkv_projection(const void* x, const void* wqkv, const void* bqkv, const void* qn_w,

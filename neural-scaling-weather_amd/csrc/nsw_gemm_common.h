@@ -20,6 +20,9 @@ enum Epi {
   EPI_TOKEN_RESIDUAL = 14,   // bias, + residual[m], stored at token_of_row(m)
   EPI_UNPATCH = 15,          // no bias; row m (a token) and column c p^2 + dy p + dx go to
                              // pixel (dy, dx) of the token's patch in image plane c
+  EPI_GATED = 17,            // w stacks gate and up rows [2H, K]: y[m, h] = act(g) u, optional bias [2H]
+  EPI_GATED_GRAD = 18,       // the same product formed again: y[M, 2H] = the gradients of g and u from
+                             // that of act(g) u (residual), optional column sums into row_sumsq
   EPI_QKV_HN16 = 16,         // bias, then per-head RMSNorm of the q and k
   EPI_QKV_HN32 = 32,         // columns, for head dims 16 / 32 / 64
   EPI_QKV_HN64 = 64,
@@ -61,6 +64,7 @@ struct EpiArgs {
   void* img;
   int64_t img_bstride;
   int img_C, img_H, img_W, img_p, img_f32;
+  int act;      // EPI_GATED, EPI_GATED_GRAD: NSW_ACT_*
 };
 
 // GELU with the exact-erf form of nn.GELU(): 0.5 v (1 + erf(v / sqrt 2)).
@@ -114,6 +118,42 @@ __device__ __forceinline__ float gelu_tanh(float v) {
   const float z = v * v;
   const float a = v * fmaf(-0.10294324f, z, -2.3022082f);
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a));
+}
+
+// Activation of a gate; `act` is the same for every lane.
+template <typename T>
+__device__ __forceinline__ float gate_act(float g, int act) {
+  if (act == NSW_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+  if (act == NSW_ACT_GELU_TANH) return gelu_tanh(g);
+  return sizeof(T) == 2 ? gelu_erf_bf16(g) : gelu_erf(g);
+}
+
+// Activation a and its derivative d at g.  With s the factor of the activation, a =
+// g s: SiLU s = 1 / (1 + e^-g), d = s (1 + g (1 - s)); tanh form s = 1 / (1 + e^-2u),
+// d = s + 2 g s (1 - s) u'; erf form s = Phi(g), d = s + g phi(g), with Phi(-|g|)
+// by the formula of gelu_erf.
+__device__ __forceinline__ void gate_act_grad(float g, int act, float& a, float& d) {
+  if (act == NSW_ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+    a = g * s;
+    d = fmaf(a, 1.0f - s, s);
+  } else if (act == NSW_ACT_GELU_TANH) {
+    const float z = fminf(g * g, 1e4f);   // s is 0 or 1 long before
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * fmaf(-0.10294324f, z, -2.3022082f)));
+    a = g * s;
+    d = fmaf(a * (1.0f - s), fmaf(0.21406445f, z, 1.5957691f), s);
+  } else {
+    const float m = fabsf(g), u = m * 0.84932180028801907f;
+    const float e = __builtin_amdgcn_exp2f(-(u * u));
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.27273748087922252f, u, 1.0f));
+    float h = fmaf(0.5307027145f, t, -0.7265760135f);
+    h = fmaf(h, t, 0.7107068705f);
+    h = fmaf(h, t, -0.142248368f);
+    h = fmaf(h, t, 0.127414796f);
+    const float c = h * t * e;            // Phi(-|g|)
+    a = fmaf(-c, m, fmaxf(g, 0.0f));
+    d = fmaf(g * 0.3989422804f, e, g < 0.0f ? c : 1.0f - c);
+  }
 }
 
 // Row blocks per tile group of one XCD (tiles come from xcd_remap).

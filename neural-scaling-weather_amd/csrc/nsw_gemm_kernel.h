@@ -127,6 +127,25 @@ __device__ __forceinline__ void mfma_f16(f32x4& acc, const f16x8& a, const f16x8
   acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
 }
 
+// Row of w that tile column r (n0 + r of the packed columns) stands for.  GATE: w
+// holds H = N / 2 gate rows and then H up rows, and every 64 columns of a wave are 32
+// of the gate and the 32 of the up projection that meet them, so that a lane holds
+// both factors of its results.  Columns past the edge repeat a row (never stored).
+template <bool GATE>
+__device__ __forceinline__ int w_source_row(int n0, int r, int N) {
+  if constexpr (GATE) {
+    const int H = N >> 1, c = (n0 >> 1) + (r >> 6) * 32 + (r & 31);
+    return (c < H ? c : H - 1) + ((r & 32) ? H : 0);
+  } else {
+    return n0 + r < N ? n0 + r : N - 1;
+  }
+}
+template <bool GATE>
+__device__ __forceinline__ bool w_row_stored(int n0, int r, int N) {
+  if constexpr (GATE) return (n0 >> 1) + (r >> 6) * 32 + (r & 31) < (N >> 1);
+  else return n0 + r < N;
+}
+
 // Fragment read: 16 bytes of k chunk `chunk` of a stage row.
 __device__ __forceinline__ u32x4 lds_frag(const char* stage, int row, int chunk) {
   const int slot = chunk ^ row_swizzle(row);
@@ -152,7 +171,7 @@ __device__ __forceinline__ u32x4 lds_frag(const char* stage, int row, int chunk)
 // barrier.  The fragments of step k+1 are read during step k, so a slot is
 // free once the barrier at the start of the last step of its stage has
 // passed.  NC = 0: a wave that copies nothing (same barriers).
-template <typename T, int NC>
+template <typename T, int NC, bool GATE>
 __device__ __forceinline__ void mainloop_256(char* smem, const T* __restrict__ X, const T* __restrict__ Wt, int M,
                                              int N, int K, int m0, int n0,
                                              f32x4 (&acc)[BigTile::NB][BigTile::MB], int wave, int lane, int rev,
@@ -178,8 +197,7 @@ __device__ __forceinline__ void mainloop_256(char* smem, const T* __restrict__ X
     const int chunk = (lane % 8) ^ row_swizzle(srow);
     int gx = m0 + srow;
     gx = gx < M ? gx : M - 1;   // rows past the edge re-read the last row (never stored)
-    int gw = n0 + srow;
-    gw = gw < N ? gw : N - 1;
+    const int gw = w_source_row<GATE>(n0, srow, N);
     vx[j] = (uint32_t)gx * rowbytes + chunk * 16;
     vw[j] = (uint32_t)gw * rowbytes + chunk * 16;
   }
@@ -408,7 +426,7 @@ __device__ __forceinline__ void mul_parts4(f32x4 (&acc)[NB][MB], int mb, const S
 // of x (j < CX) or of w; lane i writes row +i/8, 16-byte slot i%8, and loads
 // global chunk slot ^ swizzle(row).  Rows past the edge re-read the last row
 // (never stored).
-template <typename T, class TC> struct StageCopy {
+template <typename T, class TC, bool GATE> struct StageCopy {
   static constexpr int NW = TC::NW;
   static constexpr int CX = TC::BM / 8 / NW, CW = TC::BN / 8 / NW;   // 1 KB copies per wave and stage
   static constexpr int NC = CX + CW;
@@ -427,7 +445,7 @@ template <typename T, class TC> struct StageCopy {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int r = row(j) + lane / 8;
-      const int g = j < CX ? (m0 + r < M ? m0 + r : M - 1) : (n0 + r < N ? n0 + r : N - 1);
+      const int g = j < CX ? (m0 + r < M ? m0 + r : M - 1) : w_source_row<GATE>(n0, r, N);
       v[j] = (uint32_t)g * rowbytes + (uint32_t)((lane % 8) ^ row_swizzle(r)) * 16u;
     }
     cx = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * CX * 1024);
@@ -457,12 +475,12 @@ template <typename T, class TC> struct StageCopy {
 // of stage s a wave waits for its copies of stage s, and past the barrier
 // (every wave's copies have landed, and every wave is done reading stage s -
 // 1) it issues the copies of stage s + NST - 1 into the slot of stage s - 1.
-template <class TC>
+template <class TC, bool GATE>
 __device__ __forceinline__ void mainloop_ring(char* smem, const bf16* __restrict__ X, const bf16* __restrict__ Wt, int M,
                                               int N, int K, int m0, int n0, f32x4 (&acc)[TC::NB][TC::MB], int wave,
                                               int lane) {
   constexpr int NB = TC::NB, MB = TC::MB, NST = TC::NST;
-  using Copy = StageCopy<bf16, TC>;
+  using Copy = StageCopy<bf16, TC, GATE>;
   Copy cp;
   cp.init(smem, X, Wt, M, N, K, m0, n0, wave, lane);
   const int nst = cp.nst;
@@ -578,7 +596,7 @@ __device__ __forceinline__ float split2_rest(float x, float s, bool small) {
 // in one rolled loop: added to the accumulators where they are formed, the
 // accumulators spilled.  2 us a unit of x and 5 us a unit of w of a 256 x 256 tile,
 // a quarter of that for the single small values that need nothing.
-template <class TC>
+template <class TC, bool GATE>
 __device__ __forceinline__ void add_outside(const Split2List& list, const int* sh, char* buf, const float* __restrict__ X,
                                             const float* __restrict__ Wt, int M, int N, int K, int m0, int n0, int end,
                                             float lo, uint32_t small, f32x4 (&acc)[TC::NB][TC::MB], int wave, int lane) {
@@ -608,7 +626,8 @@ __device__ __forceinline__ void add_outside(const Split2List& list, const int* s
     // lane (i, g): k 4g..4g+3 and 16+4g..+3 of row i of a block (the second half
     // of the last stage may lie past K: zero)
     auto load = [&](bool ofx, int b, f32x4 (&v)[2]) {
-      const int g = ofx ? m0 + xw + b * 16 + frow : n0 + ww + b * 16 + frow, rows = ofx ? M : N;
+      int g = ofx ? m0 + xw + b * 16 + frow : n0 + ww + b * 16 + frow, rows = ofx ? M : N;
+      if (GATE && !ofx) g = w_source_row<GATE>(n0, ww + b * 16 + frow, N);
       const float* p = (ofx ? X : Wt) + (int64_t)(g < rows ? g : rows - 1) * K + k + 4 * fg;
       v[0] = *reinterpret_cast<const f32x4*>(p);
       v[1] = k + 16 < K ? *reinterpret_cast<const f32x4*>(p + 16) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -685,13 +704,13 @@ __device__ __forceinline__ void add_outside(const Split2List& list, const int* s
 //
 // A row's scale is set at its first stage that is not zero throughout
 // (split2_scale; until then it is 0).
-template <class TC>
+template <class TC, bool GATE>
 __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, const float* __restrict__ X,
                                                const float* __restrict__ Wt, int M, int N, int K, int m0, int n0,
                                                f32x4 (&acc)[TC::NB][TC::MB], int wave, int lane) {
   constexpr int NB = TC::NB, MB = TC::MB;
   constexpr int BARB = MB > 2 ? MB - 2 : 1;      // row block before which the barrier stands
-  using Copy = StageCopy<float, TC>;
+  using Copy = StageCopy<float, TC, GATE>;
   constexpr int NC = Copy::NC, NU = NC / 2;      // copies, 16-row units to split
   constexpr int NC1 = NC * 3 / 4;                // copies issued past the barrier; the others in the next stage
   constexpr int SPLB = BARB > 2 ? 2 : BARB - 1;  // first row block with splits
@@ -719,7 +738,7 @@ __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, con
       if (sc[u] == 0.f) sc[u] = t;
     }
     const int row = (u < Copy::CX / 2 ? 0 : TC::BM) + cp.row(2 * u);
-    const bool stored = u < Copy::CX / 2 ? m0 + row + urow < M : n0 + row + urow - TC::BM < N;   // not a repeated last row
+    const bool stored = u < Copy::CX / 2 ? m0 + row + urow < M : w_row_stored<GATE>(n0, row + urow - TC::BM, N);   // not a repeated last row
     int count = 0;
     bool large = false;
     auto see = [&](float x) {
@@ -858,7 +877,7 @@ __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, con
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) acc[nb][mb][r] = __builtin_amdgcn_ldexpf(acc[nb][mb][r], e[r] + ex[mb]);
   }
-  add_outside<TC>(list, sh, smem + 4096, X, Wt, M, N, K, m0, n0, s * 32, lo, small, acc, wave, lane);
+  add_outside<TC, GATE>(list, sh, smem + 4096, X, Wt, M, N, K, m0, n0, s * 32, lo, small, acc, wave, lane);
   wg_barrier();        // the exponents are no longer read
   return s;
 }
@@ -871,13 +890,13 @@ __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, con
 // Stages, barrier and copies as mainloop_split2, but the parts do not fit in
 // place, so every wave splits the fragments it reads: w block nb + 1 under the
 // MFMAs of (nb, mb 0), x block mb + 1 under those of block mb.
-template <class TC>
+template <class TC, bool GATE>
 __device__ __forceinline__ void mainloop_split3(char* smem, const float* __restrict__ X, const float* __restrict__ Wt,
                                                 int M, int N, int K, int m0, int n0, f32x4 (&acc)[TC::NB][TC::MB],
                                                 int wave, int lane, int first) {
   constexpr int NB = TC::NB, MB = TC::MB;
   constexpr int BARB = MB > 2 ? MB - 2 : 1;      // row block before which the barrier stands
-  using Copy = StageCopy<float, TC>;
+  using Copy = StageCopy<float, TC, GATE>;
   constexpr int NC = Copy::NC, NC1 = NC / 2;     // copies issued past the barrier / in the next stage
   Copy cp;
   cp.init(smem, X, Wt, M, N, K, m0, n0, wave, lane);
@@ -979,7 +998,7 @@ __device__ __forceinline__ bool any_nonfinite(const f32x4 (&acc)[TC::NB][TC::MB]
 // from global memory; of a wave's 16 x 16 blocks those with such a result, a few at
 // a time through LDS (buf, a KB each; with a loop for every block in the code, the
 // loads could not run ahead).  On finite data no wave does.
-template <class TC>
+template <class TC, bool GATE>
 __device__ __forceinline__ void redo_nonfinite(char* buf, const float* __restrict__ X, const float* __restrict__ Wt, int M,
                                                int N, int K, int mw0, int nw0, f32x4 (&acc)[TC::NB][TC::MB], int wave,
                                                int lane) {
@@ -1001,8 +1020,8 @@ __device__ __forceinline__ void redo_nonfinite(char* buf, const float* __restric
     for (int g = 0; g < G && left != 0; ++g) {
       const int b = __builtin_ctz(left);
       left &= left - 1;
-      const int n = nw0 + b / MB * 16 + frow, m = mw0 + b % MB * 16 + frow;
-      const float* wp = Wt + (int64_t)(n < N ? n : N - 1) * K + 4 * fg;
+      const int n = w_source_row<GATE>(nw0, b / MB * 16 + frow, N), m = mw0 + b % MB * 16 + frow;
+      const float* wp = Wt + (int64_t)n * K + 4 * fg;
       const float* xp = X + (int64_t)(m < M ? m : M - 1) * K + 4 * fg;
       f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
@@ -1096,6 +1115,7 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   constexpr int WGM = TC::WGM, WGN = TC::WGN;
   using S = Stg<T, TC>;
   constexpr int PRM_NW = S::PRM_NW, PRM_RS = S::PRM_RS;
+  constexpr bool GATED = EPI == EPI_GATED, GRAD = EPI == EPI_GATED_GRAD, GATE = GATED || GRAD;
   // the operand ring during the k loop, the output staging area in the
   // epilogue
   __shared__ __attribute__((aligned(1024))) char smem[S::SMEM];
@@ -1117,6 +1137,10 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   const int tin = tile - group * GM * NT;
   const int mt = gm0 + tin % gsz, nt = tin / gsz;
   const int m0 = mt * BM, n0 = nt * BN;
+  // the tile's rows of x; GATE: addressed from the tile's first one, so that x may
+  // be larger than the 32-bit offsets reach
+  const T* Xt = GATE ? X + (int64_t)m0 * K : X;
+  const int Mt = GATE ? (M - m0 < BM ? M - m0 : BM) : M, mt0 = GATE ? 0 : m0;
 
   f32x4 acc[NB][MB];
 #pragma unroll
@@ -1134,20 +1158,20 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   {
     const int lane0 = (int)threadIdx.x & 63;
     if constexpr (is_main256<T, TC>) {
-      if (wave < 4) mainloop_256<T, 8>(smem, X, Wt, M, N, K, m0, n0, acc, wave, lane0, rev, ts[1]);
-      else mainloop_256<T, 0>(smem, X, Wt, M, N, K, m0, n0, acc, wave, lane0, rev, ts[1]);
+      if (wave < 4) mainloop_256<T, 8, GATE>(smem, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0, rev, ts[1]);
+      else mainloop_256<T, 0, GATE>(smem, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0, rev, ts[1]);
     } else if constexpr (sizeof(T) == 2) {
-      mainloop_ring<TC>(smem, X, Wt, M, N, K, m0, n0, acc, wave, lane0);
+      mainloop_ring<TC, GATE>(smem, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
     } else {
       // on two fp16 parts as long as they hold the tile's values, then on three
       // bf16 parts
       int stage = 0;
       if (K >= SPLIT2_MIN_K) {
         __shared__ Split2List list;
-        stage = mainloop_split2<TC>(smem, list, X, Wt, M, N, K, m0, n0, acc, wave, lane0);
+        stage = mainloop_split2<TC, GATE>(smem, list, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
       }
-      mainloop_split3<TC>(smem, X, Wt, M, N, K, m0, n0, acc, wave, lane0, stage);
-      redo_nonfinite<TC>(smem, X, Wt, M, N, K, m0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
+      mainloop_split3<TC, GATE>(smem, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0, stage);
+      redo_nonfinite<TC, GATE>(smem, Xt, Wt, Mt, N, K, mt0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
     }
   }
   NSW_STAMP(ts[2]);
@@ -1180,6 +1204,11 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
     const int n = nw0 + nb * 16 + fg * 4;
 #pragma unroll
     for (int r = 0; r < 4; ++r) bv[nb][r] = 0.f;
+    if constexpr (GATE) {   // optional
+      const int r = nb * 16 + fg * 4;
+      if (bias != nullptr) load4<T>(bias + (w_row_stored<true>(nw0, r, N) ? w_source_row<true>(nw0, r, N) : 0), bv[nb]);
+      continue;
+    }
     if constexpr (EPI != EPI_NONE && EPI != EPI_UNPATCH && !PLDS)
       load4<T>(bias + (n < N ? n : 0), bv[nb]);   // straight-line: one batch
   }
@@ -1233,6 +1262,28 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
     p_rs = 1.0f / sqrtf(ss / (float)K + ea.eps);
   }
 
+  // EPI_GATED_GRAD: the gradients of this lane's results, loaded in one batch, and the
+  // sums of its columns' gradients
+  typedef std::conditional_t<sizeof(T) == 2, bf16x4, f32x4> dh4;
+  dh4 dhv[GRAD ? NB / 2 : 1][GRAD ? MB : 1];
+  float csum[GRAD ? NB : 1][4];
+  if constexpr (GRAD) {
+    const int H = N >> 1;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) csum[nb][r] = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < NB / 2; ++nb) {
+      const int c = (nw0 >> 1) + nb * 16 + fg * 4;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const int m = m0 + wm * WTM + mb * 16 + frow;
+        dhv[nb][mb] = *reinterpret_cast<const dh4*>((const T*)ea.residual + (int64_t)(m < M ? m : M - 1) * H + (c < H ? c : 0));
+      }
+    }
+  }
+
   // PRE_ROWSCALE: the row scales of this lane's rows (from LDS, below)
   float rsr[MB];
 #pragma unroll
@@ -1282,6 +1333,25 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[nb][r] = gelu_tanh(v[nb][r]);
+    } else if constexpr (GATED) {
+#pragma unroll
+      for (int nb = 0; nb < NB / 2; ++nb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[nb][r] = gate_act<T>(v[nb][r], ea.act) * v[nb + NB / 2][r];
+    } else if constexpr (GRAD) {
+      const bool in = m0 + wm * WTM + mb * 16 + frow < M;
+#pragma unroll
+      for (int nb = 0; nb < NB / 2; ++nb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float dh = (float)dhv[nb][mb][r], u = v[nb + NB / 2][r];
+          float a, d;
+          gate_act_grad(v[nb][r], ea.act, a, d);
+          v[nb][r] = dh * u * d;
+          v[nb + NB / 2][r] = dh * a;
+          csum[nb][r] += in ? v[nb][r] : 0.f;
+          csum[nb + NB / 2][r] += in ? v[nb + NB / 2][r] : 0.f;
+        }
     }
   };
 
@@ -1294,7 +1364,8 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   // the staging writes; the loads use clamped addresses (no branches), only
   // the stores are predicated.
   constexpr int VEC = 16 / sizeof(T);                 // elements per 16-byte chunk
-  constexpr int LPR = BN / VEC;                       // lanes per output row
+  constexpr int OBN = GATED ? BN / 2 : BN;            // columns of the output tile
+  constexpr int LPR = OBN / VEC;                      // lanes per output row
   constexpr int RPI = 64 / LPR;                       // rows per copy instruction (1, 2 or 4)
   constexpr int ITER = S::ROWS / NW / RPI;            // copy instructions per wave per pass
   constexpr int BATCH = 8;                            // rows loaded one batch ahead (at most)
@@ -1349,8 +1420,12 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   char* stg = smem;
   const int lrow = lane / LPR;                        // row of this lane within an instruction
   const int col = (lane % LPR) * VEC;                 // first tile column of this lane
-  const int n = n0 + col;
-  const int nc = n < N ? n : 0;                       // clamped column for loads
+  // output column; GATED: of H = N / 2; GRAD: the tile's first half holds the gate's
+  // gradients and its second half the up projection's (columns H ..)
+  const int n = GATED ? (n0 >> 1) + col : GRAD ? (n0 >> 1) + col % (BN / 2) + (col < BN / 2 ? 0 : N >> 1) : n0 + col;
+  const int ldy = GATED ? N >> 1 : N;
+  const bool n_in = GRAD ? (n0 >> 1) + col % (BN / 2) < (N >> 1) : n < ldy;
+  const int nc = n_in ? n : 0;                        // clamped column for loads
   // Phases: with the whole tile staged at once (bf16), staging and copy-out
   // run in NPH phases of MB / NPH row blocks per wave row, and a
   // phase's copy-out (LDS reads, global stores in flight) is followed by
@@ -1429,7 +1504,10 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
           float v[NB][4];
           row_values(mb, v);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) store4<T>(reinterpret_cast<T*>(stg + trow * S::STRIDE) + wn * WTN + nb * 16 + fg * 4, v[nb]);
+          for (int nb = 0; nb < (GATED ? NB / 2 : NB); ++nb) {
+            const int scol = GATE ? wn * (WTN / 2) + nb % (NB / 2) * 16 + nb / (NB / 2) * (BN / 2) : wn * WTN + nb * 16;
+            store4<T>(reinterpret_cast<T*>(stg + trow * S::STRIDE) + scol + fg * 4, v[nb]);
+          }
         }
       }
     };
@@ -1464,7 +1542,7 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       for (int b = 0; b < BAT; ++b) {
         const int qq = (g % NBP) * BAT + b;
         const int m = m0 + tile_row(ph, wave * IPP * RPI + qq * RPI + lrow);
-        const bool ok = m < M && n < N;
+        const bool ok = m < M && n_in;
         float ssq = 0.f;                              // sum of squares of this lane's stored values
         if constexpr (RES) {
           float o[VEC], rv[VEC];
@@ -1498,7 +1576,7 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
           // L2 made these GEMMs 4-5% faster (fc1 504 -> 481 us, bit-identical;
           // the residual epilogues, whose 133 MB outputs the next kernel
           // reads, showed no gain and keep ordinary stores)
-          if (ok) __builtin_nontemporal_store(ov[b], reinterpret_cast<u32x4*>(Y + (int64_t)orow[cur][b] * N + n));
+          if (ok) __builtin_nontemporal_store(ov[b], reinterpret_cast<u32x4*>(Y + (int64_t)orow[cur][b] * ldy + n));
         }
         if constexpr (SUMSQ) {
           // partial sum of squares over 32 lanes (32 * VEC columns, one float
@@ -1538,6 +1616,20 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       }
     }
     if (pass + 1 < S::PASSES) wg_barrier();          // before the next pass overwrites the staging rows
+  }
+  if constexpr (GRAD) {
+    // column sums of the wave's rows: row mt WGM + wm of ea.row_sumsq [.., N]
+    if (ea.row_sumsq != nullptr) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        f32x4 t;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = row16_sum(csum[nb][r]);
+        const int r = nb * 16 + fg * 4;
+        if (frow == 0 && w_row_stored<true>(nw0, r, N))
+          *reinterpret_cast<f32x4*>(ea.row_sumsq + (int64_t)(mt * WGM + wm) * N + w_source_row<true>(nw0, r, N)) = t;
+      }
+    }
   }
 #if NSW_GEMM_STAMPS
   NSW_STAMP(ts[4]);

@@ -71,4 +71,7 @@ int launch_tile(const void* x, const void* w, void* y, int64_t M, int64_t N, int
   F(EPI_QKV_HN8, PRE_ROWSCALE) F(EPI_QKV_HN16, PRE_ROWSCALE) F(EPI_QKV_HN32, PRE_ROWSCALE)                           \
   F(EPI_QKV_HN64, PRE_ROWSCALE)
 
+// The gated products (sources of their own).
+#define NSW_GEMM_GATED_FORMS(F) F(EPI_GATED, PRE_NONE) F(EPI_GATED_GRAD, PRE_NONE)
+
 }  // namespace nsw

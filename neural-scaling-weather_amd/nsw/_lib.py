@@ -24,6 +24,9 @@ NSW_EPI_BIAS = 1
 NSW_EPI_BIAS_GELU = 2
 NSW_EPI_BIAS_RESIDUAL = 3
 NSW_EPI_BIAS_GELU_TANH = 4
+NSW_ACT_SILU = 0
+NSW_ACT_GELU = 1
+NSW_ACT_GELU_TANH = 2
 NSW_METRICS_SCRATCH_BYTES = 1 << 20   # scratch of nsw_weighted_metrics_unnorm_noalloc (per GPU)
 
 _vp = ctypes.c_void_p
@@ -104,6 +107,11 @@ SIGNATURES = {
     "nsw_head_unpatchify": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp]),
     "nsw_skip_conv_accumulate": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                         _int, _int, _int, _vp]),
+    "nsw_gated_linear": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp]),
+    "nsw_gated_linear_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
+    "nsw_gated_linear_backward": (_int, [_vp] * 7 + [_i64, _i64, _i64, _int, _int, _vp, ctypes.c_size_t, _vp]),
+    "nsw_linear_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
+    "nsw_linear_backward": (_int, [_vp] * 6 + [_i64, _i64, _i64, _int, _vp, ctypes.c_size_t, _vp]),
     "nsw_residual_norm": (_int, [_vp] * 7 + [_i64, _i64, _i64, _f32, _f32, _int, _vp]),
     "nsw_residual_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "nsw_residual_norm_backward": (_int, [_vp] * 12 + [_i64, _i64, _i64, _f32, _f32, _int, _vp, ctypes.c_size_t,

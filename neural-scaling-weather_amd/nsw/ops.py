@@ -299,6 +299,96 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     return y
 
 
+_ACTS = {"silu": _lib.NSW_ACT_SILU, "gelu": _lib.NSW_ACT_GELU, "gelu_tanh": _lib.NSW_ACT_GELU_TANH}
+
+
+def _gated_args(what, x, weight, bias, act):
+    """(device, M, H, K, act code) of a gated linear, its arguments checked."""
+    dev = _dev(x, weight, bias)
+    _same_dtype(x, weight, bias)
+    if act not in _ACTS:
+        raise ValueError(f"{what}: act must be one of {sorted(_ACTS)}, got {act!r}")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] % 2:
+        raise ValueError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)}, expected [..., K] and [2H, K]")
+    K, H = x.shape[-1], weight.shape[0] // 2
+    if K == 0 or H == 0:
+        raise ValueError(f"{what}: no features")
+    if bias is not None and tuple(bias.shape) != (2 * H,):
+        raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({2 * H},)")
+    return dev, x.numel() // K, H, K, _ACTS[act]
+
+
+def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 act: str = "silu") -> torch.Tensor:
+    """h [..., H] = act(x Wg^T + bg) * (x Wu^T + bu), both projections, the
+    activation and the product of a gated feed-forward block in one kernel.
+    weight [2H, K] stacks Wg over Wu, bias [2H] bg over bu; act "silu",
+    "gelu" (exact erf) or "gelu_tanh"."""
+    dev, M, H, K, code = _gated_args("gated_linear", x, weight, bias, act)
+    h = torch.empty(x.shape[:-1] + (H,), dtype=x.dtype, device=dev)
+    if M == 0:
+        return h
+    with _guard(dev):
+        check(lib().nsw_gated_linear(x.data_ptr(), weight.data_ptr(), _p(bias), h.data_ptr(), M, H, K, code,
+                                     dtype_code(x), _stream(dev)), "gated_linear")
+    return h
+
+
+def _grads(needs, *ts):
+    """Empty gradients of the tensors that are given and asked for."""
+    return [torch.empty_like(t) if n and t is not None else None for n, t in zip(needs, ts)]
+
+
+def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                          bias: Optional[torch.Tensor] = None, act: str = "silu",
+                          needs: Sequence[bool] = (True, True, True)):
+    """(dx, dweight, dbias) of gated_linear from the gradient of h, None where
+    ``needs`` says so or there is no bias.  The projections are formed again
+    from x and weight."""
+    what = "gated_linear_backward"
+    dev, M, H, K, code = _gated_args(what, x, weight, bias, act)
+    if _dev(dh) != dev:
+        raise RuntimeError("libnsw op arguments are on different devices")
+    _same_dtype(x, dh)
+    if dh.shape != x.shape[:-1] + (H,):
+        raise ValueError(f"{what}: dh has shape {tuple(dh.shape)}, expected {tuple(x.shape[:-1]) + (H,)}")
+    dx, dw, db = _grads(needs, x, weight, bias)
+    if M == 0:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    nbytes = int(lib().nsw_gated_linear_backward_workspace_size(M, H, K, dtype_code(x)))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        check(lib().nsw_gated_linear_backward(dh.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(dx), _p(dw),
+                                              _p(db), M, H, K, code, dtype_code(x), ws.data_ptr(), nbytes,
+                                              _stream(dev)), what)
+    return dx, dw, db
+
+
+def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                    needs: Sequence[bool] = (True, True, True)):
+    """(dx, dweight, dbias) = (dy W, dy^T x, column sums of dy) of linear without
+    an activation, None where ``needs`` says so."""
+    what = "linear_backward"
+    dev = _dev(dy, x, weight)
+    _same_dtype(x, dy, weight)
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or dy.shape != x.shape[:-1] + weight.shape[:1]:
+        raise ValueError(f"{what}: dy {tuple(dy.shape)}, x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    N, K = weight.shape
+    if K == 0 or N == 0:
+        raise ValueError(f"{what}: no features")
+    M = x.numel() // K
+    dx, dw = _grads(needs, x, weight)
+    db = torch.empty(N, dtype=x.dtype, device=dev) if needs[2] else None
+    if M == 0:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    nbytes = int(lib().nsw_linear_backward_workspace_size(M, N, K, dtype_code(x)))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        check(lib().nsw_linear_backward(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(dx), _p(dw), _p(db), M, N, K,
+                                        dtype_code(x), ws.data_ptr(), nbytes, _stream(dev)), what)
+    return dx, dw, db
+
+
 def qkv_projection(x: torch.Tensor, wqkv: torch.Tensor, bqkv: torch.Tensor, qn_w: torch.Tensor,
                    kn_w: torch.Tensor, num_heads: int, eps: Optional[float] = None) -> torch.Tensor:
     """[.., C] -> [.., 3C]: q|k|v = x W^T + b with per-head RMSNorm on q and k."""

@@ -477,6 +477,27 @@ int nsw_residual_norm_backward(const void* dy, const void* dz, const void* branc
                                float alpha, float eps, int dtype, void* workspace, size_t workspace_bytes,
                                void* stream);
 
+/* Block-scaled 8-bit floating point (no counterpart in the reference).
+ * nsw_quantize_fp8: x [R, K] (dtype) -> q [R, Kp] bytes of OCP e4m3 (no
+ * infinity), Kp = K rounded up to a multiple of 128 (the rest zeros), and
+ * scale [ceil(R / rows_per_scale), Kp / 128] bytes of E8M0 (exponent + 127),
+ * one for each block of rows_per_scale (1 or 128) x 128 values: the smallest
+ * power of two (at least 2^-127) that brings the block's largest finite
+ * magnitude to at most 448.  q = round to nearest even of x / scale; what is
+ * not finite becomes NaN.  K a multiple of 8 (bf16) / 4 (fp32), x and q 16-byte
+ * aligned. */
+int nsw_quantize_fp8(const void* x, void* q, void* scale, int64_t R, int64_t K, int rows_per_scale, int dtype,
+                     void* stream);
+
+/* nsw_linear on quantised operands: y [M, N] (dtype) = epi(x . w^T), x given
+ * as xq [M, K], xs [M, K / 128] (rows_per_scale 1) and w as wq [N, K], ws
+ * [ceil(N / 128), K / 128] (rows_per_scale 128).  Sums in fp32, one rounding
+ * to dtype; bias and residual in dtype, epilogues as nsw_linear.  K a multiple
+ * of 128 and at most 16128, N of 8, pointers but the scales' 16-byte aligned. */
+int nsw_linear_fp8(const void* xq, const void* xs, const void* wq, const void* ws, const void* bias,
+                   const void* residual, void* y, int64_t M, int64_t N, int64_t K, int epilogue, int dtype,
+                   void* stream);
+
 /* HBM stream probe.  No counterpart in the reference: a measurement helper
  * for callers that report kernel rates against what the device sustains
  * (bench.py's achievable peaks).  dst == NULL: reads `bytes` from src with

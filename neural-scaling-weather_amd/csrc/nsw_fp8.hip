@@ -1,0 +1,466 @@
+// Products in 8-bit floating point: rows of e4m3 values with one power-of-two scale
+// (E8M0: the exponent + 127 in a byte) for each 1 x 128 block of x and each 128 x 128
+// block of w,
+//   y[m, n] = epilogue(sum over blocks kb of 2^(ex[m, kb] + ew[n / 128, kb]) sum over
+//                      the block's k of xq[m, k] wq[n, k]),
+// and the quantiser that makes them: a block's scale is the smallest power of two that
+// brings its largest finite magnitude to at most 448, e4m3's largest.
+//
+// Powers of two, because gfx950's scaled matrix instructions (v_mfma_scale_f32_*_
+// f8f6f4) apply them inside the product, at the rate of the plain 8-bit ones: no
+// vector instruction touches a partial sum, and scaling adds no rounding.  The
+// hardware's own blocks are 32 k; a block of 128 passes the same scale four times.
+//
+// The 8-bit instructions add in groups of 8 consecutive k: within a group a product
+// keeps only its bits at or above 2^-13 of the largest product's power of two
+// (measured: next to 2^16, 2^3 counts and 2^2 does not, of either sign); groups and the
+// accumulator are added in fp32.  A result is off by at most 7 2^-13 of its sum of
+// magnitudes from that, by 2.4e-4 of itself on normal rows: 1/7 of the rounding to
+// bf16 that follows, and far below e4m3's own 2^-4 a value.  For fp32 results that is
+// too much: there the values are widened to bf16 (exact) for the 16-bit instructions,
+// whose sums are fp32 throughout, and each block's sum is scaled as it is added.
+//
+// The instructions are issued "transposed", as in the 16-bit GEMM: A is the weight
+// fragment, B the activation fragment, so that a lane holds four consecutive output
+// columns of one row.
+#include <algorithm>
+#include <type_traits>
+
+#include "nsw_gemm_common.h"
+
+namespace nsw {
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+constexpr int BLK = 128;                 // values of a block along k
+constexpr int MAX_KB = 126;              // longest rows: 16128 values
+constexpr int QT = 256;                  // threads of the quantisers
+
+// ---------------------------------------------------------------- quantiser ---
+
+// Eight values: load (zeros past the row's end), largest finite magnitude, e4m3 of
+// them under inverse scale inv (a value that is not finite becomes NaN).
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int k, int K, float (&v)[8]) {
+  constexpr int VEC = Vec16<T>::N;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e += VEC)
+    if (k + e < K) load16<T>(row + k + e, v + e);
+}
+__device__ __forceinline__ float top8(const float (&v)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float a = fabsf(v[e]);
+    m = fmaxf(m, a < INFINITY ? a : 0.f);
+  }
+  return m;
+}
+__device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = fabsf(v[e]) < INFINITY ? v[e] * inv : __builtin_nanf("");
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(s[4], s[5], 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(s[6], s[7], hi, true);
+  return uint2{(uint32_t)lo, (uint32_t)hi};
+}
+// E8M0 byte of the smallest 2^e with top <= 448 * 2^e: top = 1.f 2^x and 448 = 1.75
+// 2^8, so e = x - 8, one more where 1.f > 1.75; at least 2^-127 (blocks of zeros, and
+// of values below 2^-118, which round to that scale's grid).
+__device__ __forceinline__ int scale_byte(float top) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, top);
+  const int s = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return s < 0 ? 0 : s;
+}
+__device__ __forceinline__ float inverse_scale(int byte) { return __builtin_bit_cast(float, (uint32_t)(254 - byte) << 23); }
+
+__device__ __forceinline__ float row16_max(float x) {
+  x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false)));
+  x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x124, 0xf, 0xf, false)));
+  x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x122, 0xf, 0xf, false)));
+  x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x121, 0xf, 0xf, false)));
+  return x;
+}
+
+// 1 x 128 blocks, 16 lanes each; block b of the R * Kb is row b / Kb.
+template <typename T>
+__global__ __launch_bounds__(QT) void quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                           uint8_t* __restrict__ scale, uint32_t blocks, int K, int Kb,
+                                                           FastDiv by_kb) {
+  constexpr int U = 4;                                      // blocks in flight per 16 lanes
+  const int l = (int)threadIdx.x & 15;
+  const int64_t b0 = ((int64_t)blockIdx.x * (QT / 16) + (threadIdx.x >> 4)) * U;
+  float v[U][8];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t b = b0 + u < blocks ? (uint32_t)(b0 + u) : blocks - 1, r = by_kb.div(b);
+    load8<T>(x + (int64_t)r * K, (int)(b - r * (uint32_t)Kb) * BLK + l * 8, K, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int s = scale_byte(row16_max(top8(v[u])));
+    const uint2 p = pack8(v[u], inverse_scale(s));
+    if (b0 + u < blocks) {
+      *reinterpret_cast<uint2*>(q + (b0 + u) * BLK + l * 8) = p;
+      if (l == 0) scale[b0 + u] = (uint8_t)s;
+    }
+  }
+}
+
+// 128 x 128 blocks, a workgroup each.
+template <typename T>
+__global__ __launch_bounds__(QT) void quantize_tiles_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                            uint8_t* __restrict__ scale, int64_t R, int K, int Kb) {
+  __shared__ float tops[QT / 16];
+  constexpr int U = 128 / (QT / 16);                        // rows of a thread
+  const int l = (int)threadIdx.x & 15, g = (int)threadIdx.x >> 4;
+  const int kb = (int)blockIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.y * 128 + g;
+  float v[U][8], m = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = r0 + u * (QT / 16);
+    load8<T>(x + (r < R ? r : 0) * K, r < R ? kb * BLK + l * 8 : K, K, v[u]);
+    m = fmaxf(m, top8(v[u]));
+  }
+  m = row16_max(m);
+  if (l == 0) tops[g] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < QT / 16; ++i) m = fmaxf(m, tops[i]);
+  const int s = scale_byte(m);
+  const float inv = inverse_scale(s);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = r0 + u * (QT / 16);
+    if (r < R) *reinterpret_cast<uint2*>(q + (r * Kb + kb) * BLK + l * 8) = pack8(v[u], inv);
+  }
+  if (threadIdx.x == 0) scale[(int64_t)blockIdx.y * Kb + kb] = (uint8_t)s;
+}
+
+// ------------------------------------------------------------------ product ---
+
+struct Fp8Args {
+  const uint8_t *xq, *xs, *wq, *ws;
+  const void *bias, *residual;
+  void* y;
+  int64_t M;
+  int N, K, Kb;      // K = 128 Kb
+};
+
+// Epilogue of one value before the residual.
+template <typename T, int EPI>
+__device__ __forceinline__ float finish(float v, float b) {
+  if constexpr (EPI != EPI_NONE) v += b;
+  if constexpr (EPI == EPI_BIAS_GELU) v = sizeof(T) == 2 ? gelu_erf_bf16(v) : gelu_erf(v);
+  if constexpr (EPI == EPI_BIAS_GELU_TANH) v = gelu_tanh(v);
+  return v;
+}
+
+// 32 e4m3 values as four bf16 fragments (every e4m3 value is a bf16 value).
+__device__ __forceinline__ void widen32(const i32x8& f, bf16x8 (&o)[4]) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * g + h], 1.f, false);
+      const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * g + h], 1.f, true);
+      o[g][4 * h] = lo[0]; o[g][4 * h + 1] = lo[1]; o[g][4 * h + 2] = hi[0]; o[g][4 * h + 3] = hi[1];
+    }
+}
+
+// Between a wave's LDS writes and its reads of what other lanes wrote (LDS accesses
+// of a wave are served in order; only the compiler has to keep them so).
+__device__ __forceinline__ void wave_fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Tile of WGM x WGN wavefronts, each MB x NB blocks of 32 x 32 results; operands in a
+// ring of NST stages of 128 k (one scale block), one barrier a stage as mainloop_ring
+// of the 16-bit GEMM; the tile's scales wait in LDS behind the ring.
+template <int WGM_, int WGN_, int MB_, int NB_, int NST_, int LDS_>
+struct Tile8 {
+  static constexpr int WGM = WGM_, WGN = WGN_, MB = MB_, NB = NB_, NST = NST_, LDS = LDS_, NW = WGM * WGN;
+  static constexpr int WTM = MB * 32, WTN = NB * 32, BM = WGM * WTM, BN = WGN * WTN;
+  static constexpr int SLOT = (BM + BN) * BLK, RING = NST * SLOT;
+  static constexpr int NBLK = (BN + 127) / 128;             // weight scale rows a tile meets
+  static constexpr int MINW = NW * (160 * 1024 / LDS) / 4;
+  static_assert(BN % 128 == 0 || 128 % BN == 0, "weight scales");
+  static_assert(RING + MAX_KB * (BM + NBLK) <= LDS, "the scales of the longest rows fit behind the ring");
+};
+using Mid8 = Tile8<2, 2, 2, 2, 2, 80 * 1024>;               // 128 x 128
+
+template <typename T, int EPI, class TC>
+__global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Args a) {
+  constexpr int MB = TC::MB, NB = TC::NB, NW = TC::NW, NST = TC::NST;
+  __shared__ __attribute__((aligned(1024))) char smem[TC::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int wm = wave / TC::WGN, wn = wave % TC::WGN;
+  const int MT = (int)((a.M + TC::BM - 1) / TC::BM), NT = (a.N + TC::BN - 1) / TC::BN;
+  // XCD x works on a contiguous range of tiles, groups of GM row blocks x all column
+  // blocks, column-major inside, so that its L2 holds both panels
+  constexpr int GM = GROUP_M * 256 / TC::BM;
+  const int tile = xcd_remap(blockIdx.x, MT * NT);
+  const int gm0 = tile / (GM * NT) * GM, gsz = MT - gm0 < GM ? MT - gm0 : GM;
+  const int tin = tile - gm0 * NT;
+  const int64_t m0 = (int64_t)(gm0 + tin % gsz) * TC::BM;
+  const int n0 = tin / gsz * TC::BN;
+  const int rows = a.M - m0 < TC::BM ? (int)(a.M - m0) : TC::BM, cols = a.N - n0 < TC::BN ? a.N - n0 : TC::BN;
+
+  // operand copies: copy j of the wave covers 8 stage rows, lane i row i / 8, 16-byte
+  // slot i % 8, swizzled as the 16-bit GEMM's; rows past the edge repeat the last one
+  constexpr int CX = TC::BM / 8 / NW, CW = TC::BN / 8 / NW, NC = CX + CW;
+  static_assert(CX * NW * 8 == TC::BM && CW * NW * 8 == TC::BN, "copies split evenly over the waves");
+  const u32x4 rx = make_rsrc(a.xq + m0 * a.K, (uint32_t)rows * (uint32_t)a.K);
+  const u32x4 rw = make_rsrc(a.wq + (int64_t)n0 * a.K, (uint32_t)cols * (uint32_t)a.K);
+  uint32_t v[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int r = (j < CX ? wave * CX + j : wave * CW + j - CX) * 8 + lane / 8, end = j < CX ? rows : cols;
+    v[j] = (uint32_t)(r < end ? r : end - 1) * (uint32_t)a.K + (uint32_t)((lane % 8) ^ row_swizzle(r)) * 16u;
+  }
+  const uint32_t lds = (uint32_t)(uintptr_t)smem;
+  auto copy = [&](int s, int slot) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+      dma16(j < CX ? rx : rw,
+            lds + slot * TC::SLOT + (j < CX ? (wave * CX + j) * 1024 : TC::BM * BLK + (wave * CW + j - CX) * 1024), v[j],
+            (uint32_t)s * BLK);
+  };
+  const int nst = a.Kb;
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if (s < nst) copy(s, s);
+  // scales: [Kb][BM] bytes of the rows, then [Kb][NBLK] of the weight blocks
+  uint8_t* xsl = reinterpret_cast<uint8_t*>(smem) + TC::RING;
+  uint8_t* wsl = xsl + a.Kb * TC::BM;
+  for (int r = threadIdx.x; r < TC::BM; r += NW * 64) {
+    const uint8_t* p = a.xs + (m0 + (r < rows ? r : rows - 1)) * a.Kb;
+    for (int kb = 0; kb < a.Kb; ++kb) xsl[kb * TC::BM + r] = p[kb];
+  }
+  for (int i = threadIdx.x; i < a.Kb * TC::NBLK; i += NW * 64) {
+    const int kb = i / TC::NBLK, b = i - kb * TC::NBLK;
+    const int nb = n0 / 128 + b, last = (a.N - 1) / 128;
+    wsl[kb * TC::NBLK + b] = a.ws[(int64_t)(nb < last ? nb : last) * a.Kb + kb];
+  }
+
+  f32x16 acc[NB][MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  const int frow = lane & 31, half = lane >> 5;
+  const int xrow = wm * TC::WTM + frow, wrow = TC::BM + wn * TC::WTN + frow;
+  const int wblk = (n0 % 128 + wn * TC::WTN) / 128;         // the wave's columns lie in one weight block
+  auto frag = [&](const char* st, int row, int t) {
+    i32x8 f;
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(st + row * BLK + ((4 * t + 2 * half) ^ row_swizzle(row)) * 16);
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(st + row * BLK + ((4 * t + 2 * half + 1) ^ row_swizzle(row)) * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (int)lo[e];
+      f[4 + e] = (int)hi[e];
+    }
+    return f;
+  };
+  int slot = 0;
+  for (int s = 0; s < nst; ++s) {
+    if (nst - 1 - s >= NST - 2) wait_copies<(NST - 2) * NC>();
+    else wait_copies<0>();
+    wg_barrier();
+    if (s + NST - 1 < nst) copy(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+    const char* st = smem + slot * TC::SLOT;
+    int sx[MB];
+    const int sw = wsl[s * TC::NBLK + wblk];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) sx[mb] = xsl[s * TC::BM + xrow + mb * 32];
+    if constexpr (sizeof(T) == 4) {
+      f32x16 part[NB][MB];                                  // the block's sums
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) part[i][j][e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        bf16x8 wa[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) widen32(frag(st, wrow + nb * 32, t), wa[nb]);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          bf16x8 xb[4];
+          widen32(frag(st, xrow + mb * 32, t), xb);
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              part[nb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wa[nb][g], xb[g], part[nb][mb], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            acc[nb][mb][e] += __builtin_amdgcn_ldexpf(part[nb][mb][e], sw + sx[mb] - 254);
+    } else
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      i32x8 fa[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) fa[nb] = frag(st, wrow + nb * 32, t);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const i32x8 fb = frag(st, xrow + mb * 32, t);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          acc[nb][mb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[nb], fb, acc[nb][mb], 0, 0, 0, sw, 0, sx[mb]);
+      }
+    }
+    slot = slot + 1 == NST ? 0 : slot + 1;
+  }
+  wg_barrier();                                             // the ring is no longer read
+
+  // Epilogue: lane (frow, half) of block (nb, mb) holds y[mb 32 + frow][nb 32 + 8 q +
+  // 4 half + r] in element 4 q + r.  Each wave stages 32 rows of its columns in an
+  // LDS part of its own and copies them out in whole rows of 16-byte pieces.  With a
+  // residual the staged values stay fp32, so that the sum is rounded once.
+  constexpr bool RES = EPI == EPI_BIAS_RESIDUAL;
+  using ST = std::conditional_t<RES, float, T>;
+  constexpr int STRIDE = TC::WTN * (int)sizeof(ST) + 16, VEC = Vec16<T>::N, LPR = TC::WTN / VEC, RPI = 64 / LPR;
+  static_assert(NW * 32 * STRIDE <= TC::RING, "staging fits in the ring");
+  char* stg = smem + wave * 32 * STRIDE;
+  const int nw = n0 + wn * TC::WTN;
+  const int crow = lane / LPR, ccol = lane % LPR * VEC;
+  const bool cin = nw + ccol < a.N;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int64_t mr = m0 + wm * TC::WTM + mb * 32;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = nb * 32 + 8 * q + 4 * half;
+        float b[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+        if constexpr (EPI != EPI_NONE) load4<T>((const T*)a.bias + (nw + c < a.N ? nw + c : 0), b);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = finish<T, EPI>(acc[nb][mb][4 * q + r], b[r]);
+        store4<ST>(reinterpret_cast<ST*>(stg + frow * STRIDE) + c, o);
+      }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int64_t m = mr + i * RPI + crow;
+      const char* src = stg + (i * RPI + crow) * STRIDE + ccol * (int)sizeof(ST);
+      if (m < a.M && cin) {
+        T* yp = (T*)a.y + m * a.N + nw + ccol;
+        if constexpr (RES) {
+          float o[VEC], rv[VEC];
+          load16<T>((const T*)a.residual + m * a.N + nw + ccol, rv);
+#pragma unroll
+          for (int e = 0; e < VEC; e += 4) load16<float>(reinterpret_cast<const float*>(src) + e, o + e);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] += rv[e];
+          store16<T>(yp, o);
+        } else {
+          *reinterpret_cast<u32x4*>(yp) = *reinterpret_cast<const u32x4*>(src);
+        }
+      }
+    }
+    wave_fence();
+  }
+}
+
+template <typename T, int EPI>
+int launch_fp8(const Fp8Args& a, hipStream_t st, const char* what) {
+  using TC = Mid8;
+  const int64_t tiles = ((a.M + TC::BM - 1) / TC::BM) * ((a.N + TC::BN - 1) / TC::BN);
+  NSW_CHECK_ARG(tiles < (1LL << 31), "%s: too many tiles", what);
+  hipLaunchKernelGGL((linear_fp8_kernel<T, EPI, TC>), dim3((unsigned)tiles), dim3(TC::NW * 64), 0, st, a);
+  return check_launch(what);
+}
+
+template <typename T>
+int dispatch_fp8(const Fp8Args& a, int epilogue, hipStream_t st, const char* what) {
+  switch (epilogue) {
+    case NSW_EPI_NONE: return launch_fp8<T, EPI_NONE>(a, st, what);
+    case NSW_EPI_BIAS: return launch_fp8<T, EPI_BIAS>(a, st, what);
+    case NSW_EPI_BIAS_GELU: return launch_fp8<T, EPI_BIAS_GELU>(a, st, what);
+    case NSW_EPI_BIAS_GELU_TANH: return launch_fp8<T, EPI_BIAS_GELU_TANH>(a, st, what);
+    case NSW_EPI_BIAS_RESIDUAL: return launch_fp8<T, EPI_BIAS_RESIDUAL>(a, st, what);
+    default: return set_error(NSW_ERR_INVALID, "%s: unknown epilogue %d", what, epilogue);
+  }
+}
+
+template <typename T>
+int launch_quantize(const void* x, void* q, void* scale, int64_t R, int64_t K, int rows, hipStream_t st, const char* what) {
+  const int64_t Kb = (K + BLK - 1) / BLK;
+  if (rows == 1) {
+    const int64_t blocks = R * Kb, per = QT / 16 * 4, grid = (blocks + per - 1) / per;
+    NSW_CHECK_ARG(blocks < (1LL << 32), "%s: too many blocks", what);
+    hipLaunchKernelGGL((quantize_rows_kernel<T>), dim3((unsigned)grid), dim3(QT), 0, st, (const T*)x, (uint8_t*)q,
+                       (uint8_t*)scale, (uint32_t)blocks, (int)K, (int)Kb, FastDiv::make((uint32_t)Kb));
+  } else {
+    NSW_CHECK_ARG((R + 127) / 128 < 65536, "%s: too many rows", what);
+    hipLaunchKernelGGL((quantize_tiles_kernel<T>), dim3((unsigned)Kb, (unsigned)((R + 127) / 128)), dim3(QT), 0, st,
+                       (const T*)x, (uint8_t*)q, (uint8_t*)scale, R, (int)K, (int)Kb);
+  }
+  return check_launch(what);
+}
+
+}  // namespace
+
+}  // namespace nsw
+
+using namespace nsw;
+
+extern "C" int nsw_quantize_fp8(const void* x, void* q, void* scale, int64_t R, int64_t K, int rows_per_scale, int dtype,
+                                void* stream) {
+  const char* what = "nsw_quantize_fp8";
+  NSW_CHECK_ARG(dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32, "%s: unknown dtype %d", what, dtype);
+  NSW_CHECK_ARG(rows_per_scale == 1 || rows_per_scale == 128, "%s: a scale for 1 or 128 rows, got %d", what, rows_per_scale);
+  const int64_t vec = dtype == NSW_DTYPE_BF16 ? 8 : 4;
+  NSW_CHECK_ARG(R > 0 && R < (1LL << 40) && K > 0 && K < (1LL << 30) && K % vec == 0,
+                "%s: R=%lld, K=%lld: K must be a positive multiple of %lld", what, (long long)R, (long long)K, (long long)vec);
+  NSW_CHECK_ARG(x && q && scale, "%s: x, q and scale are required", what);
+  NSW_CHECK_ARG((((uintptr_t)x | (uintptr_t)q) % 16) == 0, "%s: x and q must be 16-byte aligned", what);
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == NSW_DTYPE_BF16 ? launch_quantize<bf16>(x, q, scale, R, K, rows_per_scale, st, what)
+                                 : launch_quantize<float>(x, q, scale, R, K, rows_per_scale, st, what);
+}
+
+extern "C" int nsw_linear_fp8(const void* xq, const void* xs, const void* wq, const void* ws, const void* bias,
+                              const void* residual, void* y, int64_t M, int64_t N, int64_t K, int epilogue, int dtype,
+                              void* stream) {
+  const char* what = "nsw_linear_fp8";
+  NSW_CHECK_ARG(dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32, "%s: unknown dtype %d", what, dtype);
+  NSW_CHECK_ARG(M > 0 && M < (1LL << 38) && N > 0 && N < (1LL << 30) && K > 0 && K < (1LL << 30),
+                "%s: M, N, K must be positive", what);
+  NSW_CHECK_ARG(K % BLK == 0, "%s: K=%lld must be a multiple of 128 (rows are padded with zeros)", what, (long long)K);
+  NSW_CHECK_ARG(K <= MAX_KB * BLK, "%s: K=%lld, at most %d", what, (long long)K, MAX_KB * BLK);
+  NSW_CHECK_ARG(N % 8 == 0, "%s: N=%lld must be a multiple of 8", what, (long long)N);
+  NSW_CHECK_ARG(xq && xs && wq && ws && y, "%s: xq, xs, wq, ws and y are required", what);
+  NSW_CHECK_ARG(epilogue == NSW_EPI_NONE || bias, "%s: epilogue %d needs a bias", what, epilogue);
+  NSW_CHECK_ARG(epilogue != NSW_EPI_BIAS_RESIDUAL || residual, "%s: residual epilogue needs a residual", what);
+  NSW_CHECK_ARG((((uintptr_t)xq | (uintptr_t)wq | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)y) % 16) == 0,
+                "%s: xq, wq, bias, residual and y must be 16-byte aligned", what);
+  Fp8Args a{};
+  a.xq = (const uint8_t*)xq; a.xs = (const uint8_t*)xs; a.wq = (const uint8_t*)wq; a.ws = (const uint8_t*)ws;
+  a.bias = bias; a.residual = residual; a.y = y; a.M = M; a.N = (int)N; a.K = (int)K; a.Kb = (int)(K / BLK);
+  return dtype == NSW_DTYPE_BF16 ? dispatch_fp8<bf16>(a, epilogue, (hipStream_t)stream, what)
+                                 : dispatch_fp8<float>(a, epilogue, (hipStream_t)stream, what);
+}

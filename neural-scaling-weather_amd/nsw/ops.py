@@ -389,6 +389,75 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     return dx, dw, db
 
 
+FP8_BLOCK = 128     # values along k under one scale
+
+
+def quantize_fp8(x: torch.Tensor, rows: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of x [..., K]: q float8_e4m3fn [..., Kp], the last dim padded
+    with zeros to a multiple of 128, and a power-of-two scale (float8_e8m0fnu)
+    for each block of ``rows`` x 128 values: rows=1 for activations (scale
+    [..., Kp / 128]), rows=128 for a weight matrix [N, K] (scale
+    [ceil(N / 128), Kp / 128])."""
+    dev = _dev(x)
+    if rows not in (1, FP8_BLOCK):
+        raise ValueError(f"quantize_fp8: rows must be 1 or {FP8_BLOCK}, got {rows}")
+    if x.dim() < 1 or x.shape[-1] == 0 or (rows != 1 and x.dim() != 2):
+        raise ValueError(f"quantize_fp8: x has shape {tuple(x.shape)}, expected [..., K], with rows={FP8_BLOCK} [N, K]")
+    K = x.shape[-1]
+    Kb = (K + FP8_BLOCK - 1) // FP8_BLOCK
+    R = x.numel() // K
+    code = dtype_code(x)
+    q = torch.empty(x.shape[:-1] + (Kb * FP8_BLOCK,), dtype=torch.float8_e4m3fn, device=dev)
+    lead = x.shape[:-1] if rows == 1 else ((R + rows - 1) // rows,)
+    scale = torch.empty(tuple(lead) + (Kb,), dtype=torch.float8_e8m0fnu, device=dev)
+    if R:
+        with _guard(dev):
+            check(lib().nsw_quantize_fp8(x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, rows, code, _stream(dev)),
+                  "quantize_fp8")
+    return q, scale
+
+
+def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+               bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+               epilogue: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """linear of operands from quantize_fp8 (x with rows=1, the weight with
+    rows=128): y [..., N] in ``dtype`` (bfloat16 or float32; bias and residual
+    in it too), the epilogues of linear, sums in fp32."""
+    what = "linear_fp8"
+    dev = _dev(xq, x_scale, wq, w_scale, bias, residual)
+    if dtype not in _DTYPES:
+        raise TypeError(f"{what}: the result is float32 or bfloat16, got {dtype}")
+    for t, want in ((xq, torch.float8_e4m3fn), (wq, torch.float8_e4m3fn), (x_scale, torch.float8_e8m0fnu),
+                    (w_scale, torch.float8_e8m0fnu)):
+        if t.dtype != want:
+            raise TypeError(f"{what}: expected {want}, got {t.dtype}")
+    if xq.dim() < 1 or wq.dim() != 2 or wq.shape[1] != xq.shape[-1] or xq.shape[-1] % FP8_BLOCK or xq.shape[-1] == 0:
+        raise ValueError(f"{what}: xq {tuple(xq.shape)} and wq {tuple(wq.shape)}, expected [..., K] and [N, K] with K a "
+                         f"multiple of {FP8_BLOCK}")
+    N, K = wq.shape
+    Kb = K // FP8_BLOCK
+    if x_scale.shape != xq.shape[:-1] + (Kb,) or tuple(w_scale.shape) != ((N + FP8_BLOCK - 1) // FP8_BLOCK, Kb):
+        raise ValueError(f"{what}: scales {tuple(x_scale.shape)} and {tuple(w_scale.shape)} do not match "
+                         f"{tuple(xq.shape)} and {tuple(wq.shape)}")
+    for t in (bias, residual):
+        if t is not None and t.dtype != dtype:
+            raise TypeError(f"dtype mismatch: {t.dtype} vs {dtype}")
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({N},)")
+    if epilogue is None:
+        epilogue = _lib.NSW_EPI_NONE if bias is None else (
+            _lib.NSW_EPI_BIAS if residual is None else _lib.NSW_EPI_BIAS_RESIDUAL)
+    y = torch.empty(xq.shape[:-1] + (N,), dtype=dtype, device=dev)
+    if residual is not None and residual.shape != y.shape:
+        raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")
+    if y.numel():
+        with _guard(dev):
+            check(lib().nsw_linear_fp8(xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), _p(bias),
+                                       _p(residual), y.data_ptr(), xq.numel() // K, N, K, int(epilogue), _DTYPES[dtype],
+                                       _stream(dev)), what)
+    return y
+
+
 def qkv_projection(x: torch.Tensor, wqkv: torch.Tensor, bqkv: torch.Tensor, qn_w: torch.Tensor,
                    kn_w: torch.Tensor, num_heads: int, eps: Optional[float] = None) -> torch.Tensor:
     """[.., C] -> [.., 3C]: q|k|v = x W^T + b with per-head RMSNorm on q and k."""

@@ -213,10 +213,13 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
   return (M + bm - 1) / bm * 2;
 }
 
-// y[M, N] = x . w^T
-int gemm_plain(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream,
-               const char* what) {
-  return dispatch_gemm<EPI_NONE>(dtype, x, w, y, M, N, K, EpiArgs{}, stream, what);
+// fp32 y[s] [M, N] = x[s] [M, K] . w[s] [N, K]^T for s < batch.
+int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int batch, hipStream_t st,
+                   const char* what) {
+  NSW_CHECK_ARG(batch > 0 && batch < 65536, "%s: too many products", what);
+  EpiArgs ea{};
+  ea.batch = batch;
+  return launch_gemm<float, EPI_BATCH, PRE_NONE>(x, w, y, M, N, K, ea, st, what);
 }
 
 // y[remap(m)] = x[m] . w^T + bias + residual[m], the stored rows' partial

@@ -1139,6 +1139,11 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   const int m0 = mt * BM, n0 = nt * BN;
   // the tile's rows of x; GATE: addressed from the tile's first one, so that x may
   // be larger than the 32-bit offsets reach
+  if constexpr (EPI == EPI_BATCH) {
+    X += (int64_t)blockIdx.y * M * K;
+    Wt += (int64_t)blockIdx.y * N * K;
+    Y += (int64_t)blockIdx.y * M * N;
+  }
   const T* Xt = GATE ? X + (int64_t)m0 * K : X;
   const int Mt = GATE ? (M - m0 < BM ? M - m0 : BM) : M, mt0 = GATE ? 0 : m0;
 
@@ -1209,7 +1214,7 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       if (bias != nullptr) load4<T>(bias + (w_row_stored<true>(nw0, r, N) ? w_source_row<true>(nw0, r, N) : 0), bv[nb]);
       continue;
     }
-    if constexpr (EPI != EPI_NONE && EPI != EPI_UNPATCH && !PLDS)
+    if constexpr (EPI != EPI_NONE && EPI != EPI_UNPATCH && EPI != EPI_BATCH && !PLDS)
       load4<T>(bias + (n < N ? n : 0), bv[nb]);   // straight-line: one batch
   }
 
@@ -1649,7 +1654,7 @@ int launch_tile(const void* x, const void* w, void* y, int64_t M, int64_t N, int
                        hipStream_t st, const char* what) {
   const int64_t tiles = ((M + TC::BM - 1) / TC::BM) * ((N + TC::BN - 1) / TC::BN);
   NSW_CHECK_ARG(tiles < (1LL << 31), "%s: too many tiles", what);
-  hipLaunchKernelGGL((gemm_kernel<T, EPI, PRE, TC>), dim3((unsigned)tiles), dim3(TC::NW * 64), 0, st, (const T*)x,
+  hipLaunchKernelGGL((gemm_kernel<T, EPI, PRE, TC>), dim3((unsigned)tiles, EPI == EPI_BATCH ? (unsigned)ea.batch : 1u), dim3(TC::NW * 64), 0, st, (const T*)x,
                      (const T*)w, (T*)y, (int)M, (int)N, (int)K, ea);
   return check_launch(what);
 }

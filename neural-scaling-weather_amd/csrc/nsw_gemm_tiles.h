@@ -73,5 +73,7 @@ int launch_tile(const void* x, const void* w, void* y, int64_t M, int64_t N, int
 
 // The gated products (sources of their own).
 #define NSW_GEMM_GATED_FORMS(F) F(EPI_GATED, PRE_NONE) F(EPI_GATED_GRAD, PRE_NONE)
+// A batch of fp32 products (the gradients' split contraction).
+#define NSW_GEMM_BATCH_FORMS(F) F(EPI_BATCH, PRE_NONE)
 
 }  // namespace nsw

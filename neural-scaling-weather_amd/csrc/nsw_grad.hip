@@ -1,6 +1,9 @@
 // Gradients of the linear products: dx = dy . w, dw = dy^T . x and db = column sums
 // of dy, for nsw_linear (dy given) and for nsw_gated_linear (dy formed from dh by
-// EPI_GATED_GRAD).
+// EPI_GATED_GRAD).  bf16: grad_product, which reads every operand as it lies.  fp32: the
+// forward GEMM on transposed copies (its operands are split into parts as they pass
+// through LDS, so they cannot be turned there), the batch cut into pieces whose products
+// run side by side and are added in a fixed order.
 #include <algorithm>
 
 #include "nsw_gemm_common.h"
@@ -10,38 +13,54 @@ namespace nsw {
 int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M,
                int64_t H, int64_t K, int act, int dtype, void* stream, const char* what);
 int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype);
-int gemm_plain(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream,
-               const char* what);
+int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int batch, hipStream_t st,
+                   const char* what);
+int grad_product(const void* x, const void* w, void* out, int64_t R, int64_t C, int64_t D, int xt, void* ws, hipStream_t st,
+                 const char* what);
+int64_t grad_product_workspace(int64_t R, int64_t C, int64_t D, int64_t ld);
+int add_parts(const void* part, void* out, int64_t n, int S, int dtype, hipStream_t st, const char* what);
 
 namespace {
 
 constexpr int NT = 256;
 
-// out[c][r] = in[r][c] for in [R, C]; rows R .. Rp of the transpose's columns are
-// zeros.  64 x 64 values through LDS, 16-byte accesses on both sides (C and Rp are
-// multiples of 16 bytes).
-template <typename T>
-__global__ __launch_bounds__(NT) void transpose_kernel(const T* __restrict__ in, T* __restrict__ out, int R, int C, int Rp) {
-  constexpr int V = Vec16<T>::N, L = 64 / V;      // values of a piece, pieces of a tile row
-  __shared__ T t[64][64 + (sizeof(T) == 2 ? 2 : 1)];
-  const int c0 = (int)blockIdx.x * 64, r0 = (int)blockIdx.y * 64;
-  const int pl = (int)threadIdx.x % L, rw = (int)threadIdx.x / L;
-  for (int r = rw; r < 64; r += NT / L) {
-    float v[V];
+// out[s][c][i] = in[s P + i][c] for in [R, C], pieces of P rows (a multiple of 4),
+// zeros where s P + i >= R.  64 x 64 values through LDS, 16-byte accesses on both sides.
+__global__ __launch_bounds__(NT) void transpose_kernel(const float* __restrict__ in, float* __restrict__ out, int64_t R, int C,
+                                                       int P) {
+  __shared__ float t[64][65];
+  const int c0 = (int)blockIdx.x * 64;
+  const int tiles = (P + 63) / 64;                     // of a piece
+  const int64_t s = blockIdx.y / (unsigned)tiles;
+  const int i0 = ((int)blockIdx.y - (int)s * tiles) * 64;
+  const int64_t r0 = s * P + i0;
+  const int pl = ((int)threadIdx.x & 15) * 4, rw = (int)threadIdx.x >> 4;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = 0.f;
-    if (r0 + r < R && c0 + pl * V < C) load16<T>(in + (int64_t)(r0 + r) * C + c0 + pl * V, v);
+  for (int r = rw; r < 64; r += NT / 16) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r0 + r < R && c0 + pl < C) load4<float>(in + (r0 + r) * C + c0 + pl, v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[r][pl * V + e] = from_f32<T>(v[e]);
+    for (int e = 0; e < 4; ++e) t[r][pl + e] = v[e];
   }
   __syncthreads();
-  for (int c = rw; c < 64; c += NT / L) {
-    if (c0 + c >= C || r0 + pl * V >= Rp) continue;
-    float v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = to_f32(t[pl * V + e][c]);
-    store16<T>(out + (int64_t)(c0 + c) * Rp + r0 + pl * V, v);
+  for (int c = rw; c < 64; c += NT / 16) {
+    if (c0 + c >= C || i0 + pl >= P) continue;
+    const float v[4] = {t[pl][c], t[pl + 1][c], t[pl + 2][c], t[pl + 3][c]};
+    store4<float>(out + (s * C + c0 + c) * P + i0 + pl, v);
   }
+}
+
+// out[i] = sum over s of part[s][i], in order; n a multiple of 4.
+template <typename T>
+__global__ __launch_bounds__(NT) void add_parts_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t n, int S) {
+  const int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < S; ++s) a += *reinterpret_cast<const f32x4*>(part + s * n + i);
+  const float v[4] = {a[0], a[1], a[2], a[3]};
+  store4<T>(out + i, v);
 }
 
 // part[b][c] = the sum of rows b per .. of x [R, C]: 32 columns to a workgroup, as
@@ -90,12 +109,11 @@ __global__ __launch_bounds__(NT) void column_sums_kernel(const float* __restrict
   }
 }
 
-template <typename T>
-int transpose(const void* in, void* out, int64_t R, int64_t C, int64_t Rp, hipStream_t st, const char* what) {
-  const int64_t gy = (Rp + 63) / 64;
+int transpose(const void* in, void* out, int64_t R, int64_t C, int64_t S, int64_t P, hipStream_t st, const char* what) {
+  const int64_t gy = S * ((P + 63) / 64);
   NSW_CHECK_ARG(gy < 65536, "%s: too many rows", what);
-  hipLaunchKernelGGL((transpose_kernel<T>), dim3((unsigned)((C + 63) / 64), (unsigned)gy), dim3(NT), 0, st, (const T*)in,
-                     (T*)out, (int)R, (int)C, (int)Rp);
+  hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((C + 63) / 64), (unsigned)gy), dim3(NT), 0, st, (const float*)in,
+                     (float*)out, R, (int)C, (int)P);
   return check_launch(what);
 }
 
@@ -106,48 +124,87 @@ int column_sums(const float* part, void* out, int64_t P, int64_t C, hipStream_t 
 }
 
 int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
-int64_t granule(int dtype) { return dtype == NSW_DTYPE_BF16 ? 32 : 16; }
 int64_t column_part_rows(int64_t M) { return std::max<int64_t>(256, (M + 63) / 64); }
 
-// Workspace: w^T, dy^T and x^T (rows padded to the product's step), partial column sums.
+// fp32: pieces of the batch for dw, enough to fill the chip with 64 x 128 tiles of at
+// least 256 rows' work, and none whose transposed rows pass the GEMM's 2 GiB.
+void split_batch(int64_t M, int64_t N, int64_t K, int64_t& S, int64_t& P) {
+  const int64_t tiles = ((N + 63) / 64) * ((K + 127) / 128);
+  S = std::max<int64_t>(1, std::min<int64_t>({768 / tiles, M / 256, 64}));
+  const int64_t most = ((1LL << 31) - 1) / (std::max(N, K) * 4) / 64 * 64;
+  P = std::min(std::max<int64_t>(most, 64), ((M + S - 1) / S + 63) / 64 * 64);
+  S = (M + P - 1) / P;
+}
+
+// Workspace of the two products and the column sums.
 struct GradSpace {
-  int64_t Mp, wt, dyt, xt, part, bytes;
+  int64_t S = 1, P = 0, wt = 0, dyt = 0, xt = 0, prod = 0, part = 0, bytes = 0;
   GradSpace(int64_t M, int64_t N, int64_t K, int64_t parts, int dtype) {
-    const int64_t es = (int64_t)dtype_size(dtype), g = granule(dtype);
-    Mp = (M + g - 1) / g * g;
-    wt = 0;
-    dyt = wt + align256(N * K * es);
-    xt = dyt + align256(N * Mp * es);
-    part = xt + align256(K * Mp * es);
+    if (dtype == NSW_DTYPE_F32) {
+      split_batch(M, N, K, S, P);
+      wt = 0;                                          // w^T
+      dyt = wt + align256(N * K * 4);                  // dy^T and x^T in pieces
+      xt = dyt + align256(S * N * P * 4);
+      prod = xt + align256(S * K * P * 4);             // their products
+      part = prod + (S > 1 ? align256(S * N * K * 4) : 0);
+    } else {
+      const int64_t a = grad_product_workspace(M, K, N, K), b = grad_product_workspace(N, K, M, std::max(N, K));
+      part = align256(std::max(a, b));
+    }
     bytes = part + align256(parts * N * 4);
   }
 };
 
 bool bad_sizes(int64_t M, int64_t N, int64_t K, int dtype) {
   if (dtype != NSW_DTYPE_BF16 && dtype != NSW_DTYPE_F32) return true;
-  const int64_t g = granule(dtype);
+  const int64_t g = dtype == NSW_DTYPE_BF16 ? 32 : 16;   // one step of the products
   return M <= 0 || N <= 0 || K <= 0 || M >= (1LL << 31) || N >= (1LL << 31) || K >= (1LL << 31) || N % g || K % g;
 }
 
-template <typename T>
-int linear_grads(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t parts, int64_t M,
-                 int64_t N, int64_t K, int dtype, char* ws, hipStream_t st, const char* what) {
-  const GradSpace sp(M, N, K, parts, dtype);
+int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, void* dw, int64_t M, int64_t N, int64_t K,
+                     const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
   int rc = NSW_OK;
   if (dx) {
-    if ((rc = transpose<T>(w, ws + sp.wt, N, K, N, st, what))) return rc;
-    if ((rc = gemm_plain(dy, ws + sp.wt, dx, M, K, N, dtype, st, what))) return rc;
+    if ((rc = transpose(w, ws + sp.wt, N, K, 1, N, st, what))) return rc;
+    // as many rows at a time as the GEMM's 2 GiB hold
+    const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4));
+    for (int64_t m = 0; m < M; m += rows)
+      if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, dx + m * K * 4, std::min(rows, M - m), K, N, 1, st, what))) return rc;
   }
   if (dw) {
-    if ((rc = transpose<T>(dy, ws + sp.dyt, M, N, sp.Mp, st, what))) return rc;
-    if ((rc = transpose<T>(x, ws + sp.xt, M, K, sp.Mp, st, what))) return rc;
-    if ((rc = gemm_plain(ws + sp.dyt, ws + sp.xt, dw, N, K, sp.Mp, dtype, st, what))) return rc;
+    if ((rc = transpose(dy, ws + sp.dyt, M, N, sp.S, sp.P, st, what))) return rc;
+    if ((rc = transpose(x, ws + sp.xt, M, K, sp.S, sp.P, st, what))) return rc;
+    void* out = sp.S > 1 ? ws + sp.prod : dw;
+    if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, (int)sp.S, st, what))) return rc;
+    if (sp.S > 1) rc = add_parts(out, dw, N * K, (int)sp.S, NSW_DTYPE_F32, st, what);
   }
-  if (db) rc = column_sums<T>((const float*)(ws + sp.part), db, parts, N, st, what);
   return rc;
 }
 
+int linear_grads(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t parts, int64_t M,
+                 int64_t N, int64_t K, int dtype, char* ws, hipStream_t st, const char* what) {
+  const GradSpace sp(M, N, K, parts, dtype);
+  const float* part = (const float*)(ws + sp.part);
+  int rc = NSW_OK;
+  if (dtype == NSW_DTYPE_F32) {
+    if ((rc = linear_grads_f32((const char*)dy, x, w, (char*)dx, dw, M, N, K, sp, ws, st, what))) return rc;
+    return db ? column_sums<float>(part, db, parts, N, st, what) : rc;
+  }
+  if (dx && (rc = grad_product(dy, w, dx, M, K, N, 0, ws, st, what))) return rc;
+  if (dw && (rc = grad_product(dy, x, dw, N, K, M, 1, ws, st, what))) return rc;
+  return db ? column_sums<bf16>(part, db, parts, N, st, what) : rc;
+}
+
 }  // namespace
+
+int add_parts(const void* part, void* out, int64_t n, int S, int dtype, hipStream_t st, const char* what) {
+  const dim3 grid((unsigned)((n / 4 + NT - 1) / NT));
+  if (dtype == NSW_DTYPE_BF16)
+    hipLaunchKernelGGL((add_parts_kernel<bf16>), grid, dim3(NT), 0, st, (const float*)part, (bf16*)out, n, S);
+  else
+    hipLaunchKernelGGL((add_parts_kernel<float>), grid, dim3(NT), 0, st, (const float*)part, (float*)out, n, S);
+  return check_launch(what);
+}
 
 }  // namespace nsw
 
@@ -181,8 +238,7 @@ extern "C" int nsw_linear_backward(const void* dy, const void* x, const void* w,
       hipLaunchKernelGGL((column_parts_kernel<float>), grid, dim3(NT), 0, st, (const float*)dy, part, M, (int)N, per);
     if (int rc = check_launch(what)) return rc;
   }
-  if (dtype == NSW_DTYPE_BF16) return linear_grads<bf16>(dy, x, w, dx, dw, db, parts, M, N, K, dtype, ws, st, what);
-  return linear_grads<float>(dy, x, w, dx, dw, db, parts, M, N, K, dtype, ws, st, what);
+  return linear_grads(dy, x, w, dx, dw, db, parts, M, N, K, dtype, ws, st, what);
 }
 
 extern "C" size_t nsw_gated_linear_backward_workspace_size(int64_t M, int64_t H, int64_t K, int dtype) {
@@ -213,6 +269,5 @@ extern "C" int nsw_gated_linear_backward(const void* dh, const void* x, const vo
   int rc = gemm_gated(x, w, bias, dh, dy, db ? (float*)(ws + sp.part) : nullptr, M, H, K, act, dtype, stream, what);
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == NSW_DTYPE_BF16) return linear_grads<bf16>(dy, x, w, dx, dw, db, parts, M, 2 * H, K, dtype, ws, st, what);
-  return linear_grads<float>(dy, x, w, dx, dw, db, parts, M, 2 * H, K, dtype, ws, st, what);
+  return linear_grads(dy, x, w, dx, dw, db, parts, M, 2 * H, K, dtype, ws, st, what);
 }

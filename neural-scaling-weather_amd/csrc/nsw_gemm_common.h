@@ -122,11 +122,11 @@ __device__ __forceinline__ float gelu_tanh(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a));
 }
 
-// Activation of a gate; `act` is the same for every lane.
-template <typename T>
-__device__ __forceinline__ float gate_act(float g, int act) {
-  if (act == NSW_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
-  if (act == NSW_ACT_GELU_TANH) return gelu_tanh(g);
+// Activation of a gate.
+template <typename T, int ACT>
+__device__ __forceinline__ float gate_act(float g) {
+  if constexpr (ACT == NSW_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+  if constexpr (ACT == NSW_ACT_GELU_TANH) return gelu_tanh(g);
   return sizeof(T) == 2 ? gelu_erf_bf16(g) : gelu_erf(g);
 }
 
@@ -134,12 +134,13 @@ __device__ __forceinline__ float gate_act(float g, int act) {
 // g s: SiLU s = 1 / (1 + e^-g), d = s (1 + g (1 - s)); tanh form s = 1 / (1 + e^-2u),
 // d = s + 2 g s (1 - s) u'; erf form s = Phi(g), d = s + g phi(g), with Phi(-|g|)
 // by the formula of gelu_erf.
-__device__ __forceinline__ void gate_act_grad(float g, int act, float& a, float& d) {
-  if (act == NSW_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ void gate_act_grad(float g, float& a, float& d) {
+  if constexpr (ACT == NSW_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
     a = g * s;
     d = fmaf(a, 1.0f - s, s);
-  } else if (act == NSW_ACT_GELU_TANH) {
+  } else if constexpr (ACT == NSW_ACT_GELU_TANH) {
     const float z = fminf(g * g, 1e4f);   // s is 0 or 1 long before
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * fmaf(-0.10294324f, z, -2.3022082f)));
     a = g * s;

@@ -1169,9 +1169,10 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       mainloop_ring<TC, GATE>(smem, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
     } else {
       // on two fp16 parts as long as they hold the tile's values, then on three
-      // bf16 parts
+      // bf16 parts; gradients (EPI_BATCH), products of factors near zero, leave two
+      // parts within a few stages, so they start on three
       int stage = 0;
-      if (K >= SPLIT2_MIN_K) {
+      if (EPI != EPI_BATCH && K >= SPLIT2_MIN_K) {
         __shared__ Split2List list;
         stage = mainloop_split2<TC, GATE>(smem, list, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
       }
@@ -1338,25 +1339,42 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[nb][r] = gelu_tanh(v[nb][r]);
-    } else if constexpr (GATED) {
+    } else if constexpr (GATE) {
+      // the activation chosen once for the row block, not once a value: between
+      // branches the values' exponentials and reciprocals would not overlap
+      auto gate = [&](auto form) {
+        constexpr int ACT = decltype(form)::value;
 #pragma unroll
-      for (int nb = 0; nb < NB / 2; ++nb)
+        for (int nb = 0; nb < NB / 2; ++nb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[nb][r] = gate_act<T>(v[nb][r], ea.act) * v[nb + NB / 2][r];
-    } else if constexpr (GRAD) {
-      const bool in = m0 + wm * WTM + mb * 16 + frow < M;
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (GATED) {
+              v[nb][r] = gate_act<T, ACT>(v[nb][r]) * v[nb + NB / 2][r];
+            } else {
+              const float dh = (float)dhv[nb][mb][r];
+              float a, d;
+              gate_act_grad<ACT>(v[nb][r], a, d);
+              v[nb][r] = dh * v[nb + NB / 2][r] * d;
+              v[nb + NB / 2][r] = dh * a;
+            }
+          }
+      };
+      if (ea.act == NSW_ACT_SILU) gate(std::integral_constant<int, NSW_ACT_SILU>{});
+      else if (ea.act == NSW_ACT_GELU) gate(std::integral_constant<int, NSW_ACT_GELU>{});
+      else gate(std::integral_constant<int, NSW_ACT_GELU_TANH>{});
+      if constexpr (GRAD) {
+        if (m0 + BM > M) {            // rows past the edge repeat the last one
+          const bool in = m0 + wm * WTM + mb * 16 + frow < M;
 #pragma unroll
-      for (int nb = 0; nb < NB / 2; ++nb)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float dh = (float)dhv[nb][mb][r], u = v[nb + NB / 2][r];
-          float a, d;
-          gate_act_grad(v[nb][r], ea.act, a, d);
-          v[nb][r] = dh * u * d;
-          v[nb + NB / 2][r] = dh * a;
-          csum[nb][r] += in ? v[nb][r] : 0.f;
-          csum[nb + NB / 2][r] += in ? v[nb + NB / 2][r] : 0.f;
+            for (int r = 0; r < 4; ++r) v[nb][r] = in ? v[nb][r] : 0.f;
         }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) csum[nb][r] += v[nb][r];
+      }
     }
   };
 

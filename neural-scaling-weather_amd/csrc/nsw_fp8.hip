@@ -199,6 +199,94 @@ struct Tile8 {
 };
 using Mid8 = Tile8<2, 2, 2, 2, 2, 80 * 1024>;               // 128 x 128
 
+// The tile's scales into LDS: [Kb][BM] bytes of its rows, [Kb][NBLK] of its weight blocks.
+template <class TC>
+__device__ __forceinline__ void load_scales(const Fp8Args& a, uint8_t* xsl, uint8_t* wsl, int64_t m0, int n0, int rows) {
+  constexpr int NW = TC::NW;
+  {
+    constexpr int TPR = NW * 64 / TC::BM, U = 8;            // threads of a row, loads in flight
+    static_assert(TPR * TC::BM == NW * 64, "whole threads to a row");
+    const int r = (int)threadIdx.x % TC::BM;
+    const uint8_t* p = a.xs + (m0 + (r < rows ? r : rows - 1)) * a.Kb;
+    for (int k0 = (int)threadIdx.x / TC::BM; k0 < a.Kb; k0 += U * TPR) {
+      uint8_t b[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) b[u] = p[k0 + u * TPR < a.Kb ? k0 + u * TPR : 0];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k0 + u * TPR < a.Kb) xsl[(k0 + u * TPR) * TC::BM + r] = b[u];
+    }
+  }
+  for (int i = threadIdx.x; i < a.Kb * TC::NBLK; i += NW * 64) {
+    const int kb = i / TC::NBLK, b = i - kb * TC::NBLK;
+    const int nb = n0 / 128 + b, last = (a.N - 1) / 128;
+    wsl[kb * TC::NBLK + b] = a.ws[(int64_t)(nb < last ? nb : last) * a.Kb + kb];
+  }
+}
+
+// Epilogue: lane (frow, half) of block (nb, mb) holds y[mb 32 + frow][nb 32 + 8 q + 4
+// half + r] in element 4 q + r.  Each wave stages 32 rows of its columns in an LDS part
+// of its own and copies them out in whole rows of 16-byte pieces.  With a residual the
+// staged values stay fp32, so that the sum is rounded once.
+template <typename T, int EPI, class TC>
+__device__ __forceinline__ void write_out(const Fp8Args& a, char* smem, f32x16 (&acc)[TC::NB][TC::MB], int64_t m0, int n0,
+                                          int wave, int lane) {
+  constexpr int MB = TC::MB, NB = TC::NB, NW = TC::NW;
+  const int wm = wave / TC::WGN, wn = wave % TC::WGN, frow = lane & 31, half = lane >> 5;
+  constexpr bool RES = EPI == EPI_BIAS_RESIDUAL;
+  using ST = std::conditional_t<RES, float, T>;
+  constexpr int STRIDE = TC::WTN * (int)sizeof(ST) + 16, VEC = Vec16<T>::N, LPR = TC::WTN / VEC, RPI = 64 / LPR;
+  static_assert(NW * 32 * STRIDE <= TC::LDS, "staging fits in the LDS");
+  char* stg = smem + wave * 32 * STRIDE;
+  const int nw = n0 + wn * TC::WTN;
+  const int crow = lane / LPR, ccol = lane % LPR * VEC;
+  const bool cin = nw + ccol < a.N;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int64_t mr = m0 + wm * TC::WTM + mb * 32;
+    u32x4 res[RES ? 32 / RPI : 1];
+    if constexpr (RES) {   // in one batch, ahead of the staging
+#pragma unroll
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int64_t m = mr + i * RPI + crow;
+        res[i] = *reinterpret_cast<const u32x4*>((const T*)a.residual + (m < a.M ? m : a.M - 1) * a.N + (cin ? nw + ccol : 0));
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = nb * 32 + 8 * q + 4 * half;
+        float b[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+        if constexpr (EPI != EPI_NONE) load4<T>((const T*)a.bias + (nw + c < a.N ? nw + c : 0), b);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = finish<T, EPI>(acc[nb][mb][4 * q + r], b[r]);
+        store4<ST>(reinterpret_cast<ST*>(stg + frow * STRIDE) + c, o);
+      }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int64_t m = mr + i * RPI + crow;
+      const char* src = stg + (i * RPI + crow) * STRIDE + ccol * (int)sizeof(ST);
+      if (m < a.M && cin) {
+        T* yp = (T*)a.y + m * a.N + nw + ccol;
+        if constexpr (RES) {
+          float o[VEC], rv[VEC];
+          load16<T>(reinterpret_cast<const T*>(&res[i]), rv);
+#pragma unroll
+          for (int e = 0; e < VEC; e += 4) load16<float>(reinterpret_cast<const float*>(src) + e, o + e);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] += rv[e];
+          store16<T>(yp, o);
+        } else {
+          __builtin_nontemporal_store(*reinterpret_cast<const u32x4*>(src), reinterpret_cast<u32x4*>(yp));
+        }
+      }
+    }
+    wave_fence();
+  }
+}
+
 template <typename T, int EPI, class TC>
 __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Args a) {
   constexpr int MB = TC::MB, NB = TC::NB, NW = TC::NW, NST = TC::NST;
@@ -240,18 +328,9 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Ar
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s)
     if (s < nst) copy(s, s);
-  // scales: [Kb][BM] bytes of the rows, then [Kb][NBLK] of the weight blocks
   uint8_t* xsl = reinterpret_cast<uint8_t*>(smem) + TC::RING;
   uint8_t* wsl = xsl + a.Kb * TC::BM;
-  for (int r = threadIdx.x; r < TC::BM; r += NW * 64) {
-    const uint8_t* p = a.xs + (m0 + (r < rows ? r : rows - 1)) * a.Kb;
-    for (int kb = 0; kb < a.Kb; ++kb) xsl[kb * TC::BM + r] = p[kb];
-  }
-  for (int i = threadIdx.x; i < a.Kb * TC::NBLK; i += NW * 64) {
-    const int kb = i / TC::NBLK, b = i - kb * TC::NBLK;
-    const int nb = n0 / 128 + b, last = (a.N - 1) / 128;
-    wsl[kb * TC::NBLK + b] = a.ws[(int64_t)(nb < last ? nb : last) * a.Kb + kb];
-  }
+  load_scales<TC>(a, xsl, wsl, m0, n0, rows);
 
   f32x16 acc[NB][MB];
 #pragma unroll
@@ -335,62 +414,275 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Ar
   }
   wg_barrier();                                             // the ring is no longer read
 
-  // Epilogue: lane (frow, half) of block (nb, mb) holds y[mb 32 + frow][nb 32 + 8 q +
-  // 4 half + r] in element 4 q + r.  Each wave stages 32 rows of its columns in an
-  // LDS part of its own and copies them out in whole rows of 16-byte pieces.  With a
-  // residual the staged values stay fp32, so that the sum is rounded once.
-  constexpr bool RES = EPI == EPI_BIAS_RESIDUAL;
-  using ST = std::conditional_t<RES, float, T>;
-  constexpr int STRIDE = TC::WTN * (int)sizeof(ST) + 16, VEC = Vec16<T>::N, LPR = TC::WTN / VEC, RPI = 64 / LPR;
-  static_assert(NW * 32 * STRIDE <= TC::RING, "staging fits in the ring");
-  char* stg = smem + wave * 32 * STRIDE;
-  const int nw = n0 + wn * TC::WTN;
-  const int crow = lane / LPR, ccol = lane % LPR * VEC;
-  const bool cin = nw + ccol < a.N;
+  write_out<T, EPI, TC>(a, smem, acc, m0, n0, wave, lane);
+}
+
+// The large bf16 products: waves of 64 x 128 results, WGM x 2 of them.  Stages of 64 k
+// (64 bytes of a row) in a ring of NST; the fragments of stage s + 1 are read under the
+// matrix instructions of stage s, the w fragment of an n block into the registers that
+// block has just released.  A stage's one barrier frees the slot of the stage before it
+// for the copies of stage s + NST - 1; the reads of stage s may still be in flight there
+// (waiting for them, the matrix units idled for an LDS latency a stage).
+template <int WGM_, int NST_, int LDS_>
+struct Deep8 {
+  static constexpr int WGM = WGM_, WGN = 2, MB = 2, NB = 4, NST = NST_, NW = WGM * WGN, KS = 64, LDS = LDS_;
+  static constexpr int WTM = MB * 32, WTN = NB * 32, BM = WGM * WTM, BN = WGN * WTN;
+  static constexpr int SLOT = (BM + BN) * KS, RING = NST * SLOT, NBLK = BN / 128;
+  static constexpr int KB = (LDS - RING) / (BM + NBLK);     // longest rows: their scales fit behind the ring
+  static constexpr int MINW = NW * (160 * 1024 / LDS) / 4;
+};
+using Big8 = Deep8<4, 4, 160 * 1024>;                       // 256 x 256, one workgroup a CU
+
+// 16-byte slot of chunk c of a 64-byte stage row: conflict-free fragment reads whether 8
+// lanes share 32 banks or 16 lanes 64.
+__device__ __forceinline__ int swizzle64(int row) { return ((row >> 1) & 3) ^ ((row >> 3) & 1); }
+
+template <typename T, int EPI, class TC>
+__global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_deep_kernel(Fp8Args a) {
+  constexpr int MB = TC::MB, NB = TC::NB, NW = TC::NW, NST = TC::NST;
+  __shared__ __attribute__((aligned(1024))) char smem[TC::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int wm = wave / TC::WGN, wn = wave % TC::WGN;
+  const int MT = (int)((a.M + TC::BM - 1) / TC::BM), NT = (a.N + TC::BN - 1) / TC::BN;
+  constexpr int GM = GROUP_M * 256 / TC::BM;                // tile order as linear_fp8_kernel
+  const int tile = xcd_remap(blockIdx.x, MT * NT);
+  const int gm0 = tile / (GM * NT) * GM, gsz = MT - gm0 < GM ? MT - gm0 : GM;
+  const int tin = tile - gm0 * NT;
+  const int64_t m0 = (int64_t)(gm0 + tin % gsz) * TC::BM;
+  const int n0 = tin / gsz * TC::BN;
+  const int rows = a.M - m0 < TC::BM ? (int)(a.M - m0) : TC::BM, cols = a.N - n0 < TC::BN ? a.N - n0 : TC::BN;
+
+  // copy j of the wave: 16 stage rows, lane i row i / 4, 16-byte slot i % 4
+  constexpr int CX = TC::BM / 16 / NW, CW = TC::BN / 16 / NW, NC = CX + CW;
+  const u32x4 rx = make_rsrc(a.xq + m0 * a.K, (uint32_t)rows * (uint32_t)a.K);
+  const u32x4 rw = make_rsrc(a.wq + (int64_t)n0 * a.K, (uint32_t)cols * (uint32_t)a.K);
+  uint32_t v[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int r = (j < CX ? wave * CX + j : wave * CW + j - CX) * 16 + lane / 4, end = j < CX ? rows : cols;
+    v[j] = (uint32_t)(r < end ? r : end - 1) * (uint32_t)a.K + (uint32_t)((lane % 4) ^ swizzle64(r)) * 16u;
+  }
+  const uint32_t lds = (uint32_t)(uintptr_t)smem;
+  auto copy = [&](int s, int slot, int lo, int hi) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+      if (j >= lo && j < hi)
+        dma16(j < CX ? rx : rw,
+              lds + slot * TC::SLOT + (j < CX ? (wave * CX + j) * 1024 : TC::BM * TC::KS + (wave * CW + j - CX) * 1024), v[j],
+              (uint32_t)s * TC::KS);
+  };
+  const int ns = a.Kb * 2;                                  // stages; past the end the last one again, never used
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) copy(s < ns ? s : ns - 1, s, 0, NC);
+  uint8_t* xsl = reinterpret_cast<uint8_t*>(smem) + TC::RING;
+  uint8_t* wsl = xsl + a.Kb * TC::BM;
+  load_scales<TC>(a, xsl, wsl, m0, n0, rows);
+
+  const int frow = lane & 31, half = lane >> 5, nw = n0 + wn * TC::WTN;
+  f32x16 acc[NB][MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  // lane's offset of a fragment's first chunk in a slot; its second chunk is at ^ 16
+  const uint32_t at = (uint32_t)(frow * TC::KS + ((2 * half) ^ swizzle64(frow)) * 16);
+  const char* xp = smem + wm * TC::WTM * TC::KS;
+  const char* wp = smem + (TC::BM + wn * TC::WTN) * TC::KS;
+  auto frag = [&](const char* p) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(p + at), hi = *reinterpret_cast<const u32x4*>(p + (at ^ 16u));
+    i32x8 f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (int)lo[e];
+      f[4 + e] = (int)hi[e];
+    }
+    return f;
+  };
+  const uint8_t* xsp = xsl + wm * TC::WTM + frow;
+  const uint8_t* wsp = wsl + wn;
+  static_assert(TC::WTN == 128, "a wave's columns are one weight block");
+
+  wait_copies<(NST - 2) * NC>();
+  wg_barrier();
+  i32x8 fa[NB], fb[2][MB];
+  int sx[2][MB], sw[2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) fa[nb] = frag(wp + nb * 32 * TC::KS);
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    const int64_t mr = m0 + wm * TC::WTM + mb * 32;
+    fb[0][mb] = frag(xp + mb * 32 * TC::KS);
+    sx[0][mb] = xsp[mb * 32];
+  }
+  sw[0] = wsp[0];
+  // stage s = s0 + u: slots, register sets and scale sets by constants
+  constexpr int UNR = NST % 4 == 0 ? NST : NST % 2 == 0 ? 2 * NST : 4 * NST;
+  for (int s0 = 0; s0 < ns; s0 += UNR) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int u = 0; u < UNR; ++u) {
+      const int s = s0 + u;
+      if (s < ns) {
+        const int cs = s + NST - 1 < ns ? s + NST - 1 : ns - 1, kn = (s + 1 < ns ? s + 1 : s) >> 1;
+        wait_copies<(NST - 3) * NC>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const char* xn = xp + (u + 1) % NST * TC::SLOT;
+        const char* wn_ = wp + (u + 1) % NST * TC::SLOT;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = nb * 32 + 8 * q + 4 * half;
-        float b[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
-        if constexpr (EPI != EPI_NONE) load4<T>((const T*)a.bias + (nw + c < a.N ? nw + c : 0), b);
+        for (int nb = 0; nb < NB; ++nb) {
+          copy(cs, (u + NST - 1) % NST, nb * NC / NB, (nb + 1) * NC / NB);
+          if (nb < MB) fb[(u + 1) & 1][nb] = frag(xn + nb * 32 * TC::KS);
+          if ((u & 1) == 1 && nb == 0) {                    // the next block's scales
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = finish<T, EPI>(acc[nb][mb][4 * q + r], b[r]);
-        store4<ST>(reinterpret_cast<ST*>(stg + frow * STRIDE) + c, o);
-      }
-    wave_fence();
+            for (int mb = 0; mb < MB; ++mb) sx[((u + 1) >> 1) & 1][mb] = xsp[kn * TC::BM + mb * 32];
+            sw[((u + 1) >> 1) & 1] = wsp[kn * TC::NBLK];
+          }
 #pragma unroll
-    for (int i = 0; i < 32 / RPI; ++i) {
-      const int64_t m = mr + i * RPI + crow;
-      const char* src = stg + (i * RPI + crow) * STRIDE + ccol * (int)sizeof(ST);
-      if (m < a.M && cin) {
-        T* yp = (T*)a.y + m * a.N + nw + ccol;
-        if constexpr (RES) {
-          float o[VEC], rv[VEC];
-          load16<T>((const T*)a.residual + m * a.N + nw + ccol, rv);
-#pragma unroll
-          for (int e = 0; e < VEC; e += 4) load16<float>(reinterpret_cast<const float*>(src) + e, o + e);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) o[e] += rv[e];
-          store16<T>(yp, o);
-        } else {
-          *reinterpret_cast<u32x4*>(yp) = *reinterpret_cast<const u32x4*>(src);
+          for (int mb = 0; mb < MB; ++mb)
+            acc[nb][mb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[nb], fb[u & 1][mb], acc[nb][mb], 0, 0, 0,
+                                                                          sw[(u >> 1) & 1], 0, sx[(u >> 1) & 1][mb]);
+          fa[nb] = frag(wn_ + nb * 32 * TC::KS);
         }
       }
     }
-    wave_fence();
   }
+  wait_copies();                                            // those past the last stage
+  wg_barrier();                                             // the ring is no longer read
+  write_out<T, EPI, TC>(a, smem, acc, m0, n0, wave, lane);
+}
+
+// Few rows: the weights' bytes and the latency count.  A workgroup of eight waves takes
+// 16 columns and 16 MB rows; the waves share out the k blocks (one v_mfma_scale_f32_
+// 16x16x128 or four of the 16-bit ones each), operands straight from global memory (lane
+// (i, g): 32 bytes of row i, so a row's 128-byte line is four lanes' loads), and their
+// sums meet in LDS in a fixed order.
+template <typename T, int EPI, int MB>
+__global__ __launch_bounds__(512) void linear_fp8_rows_kernel(Fp8Args a) {
+  constexpr int NW = 8, U = MB == 4 ? 2 : 4;                // k blocks whose loads are in flight together
+  __shared__ f32x4 red[NW][MB][64];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int i = lane & 15, g = lane >> 4, n0 = (int)blockIdx.x * 16;
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MB);
+  const uint8_t* wp = a.wq + (int64_t)(n0 + i < a.N ? n0 + i : a.N - 1) * a.K + g * 32;
+  const uint8_t* wsp = a.ws + (int64_t)(n0 / 128) * a.Kb;
+  const uint8_t *xp[MB], *xsp[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int64_t m = m0 + mb * 16 + i < a.M ? m0 + mb * 16 + i : a.M - 1;
+    xp[mb] = a.xq + m * a.K + g * 32;
+    xsp[mb] = a.xs + m * a.Kb;
+  }
+  auto load = [&](const uint8_t* p) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(p), hi = *reinterpret_cast<const u32x4*>(p + 16);
+    i32x8 f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (int)lo[e];
+      f[4 + e] = (int)hi[e];
+    }
+    return f;
+  };
+  f32x4 acc[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) acc[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wave; k0 < a.Kb; k0 += U * NW) {
+    i32x8 fw[U], fx[U][MB];
+    int sw[U], sx[U][MB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kb = k0 + u * NW < a.Kb ? k0 + u * NW : k0;
+      fw[u] = load(wp + (int64_t)kb * BLK);
+      sw[u] = wsp[kb];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        fx[u][mb] = load(xp[mb] + (int64_t)kb * BLK);
+        sx[u][mb] = xsp[mb][kb];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u * NW >= a.Kb) break;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+          acc[mb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u], fx[u][mb], acc[mb], 0, 0, 0, sw[u], 0, sx[u][mb]);
+      } else {
+        bf16x8 w4[4], x4[4];
+        widen32(fw[u], w4);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          widen32(fx[u][mb], x4);
+          f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w4[q], x4[q], part, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[mb][e] += __builtin_amdgcn_ldexpf(part[e], sw[u] + sx[u][mb] - 254);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) red[wave][mb][lane] = acc[mb];
+  __syncthreads();
+  // lane (i, g) of block mb holds y[m0 + mb 16 + i][n0 + 4 g + r]
+  if (wave >= MB) return;
+  const int64_t m = m0 + wave * 16 + i;
+  const int n = n0 + 4 * g;
+  if (m >= a.M || n >= a.N) return;
+  f32x4 t = red[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) t += red[w][wave][lane];
+  float b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+  if constexpr (EPI != EPI_NONE) load4<T>((const T*)a.bias + n, b);
+  if constexpr (EPI == EPI_BIAS_RESIDUAL) load4<T>((const T*)a.residual + m * a.N + n, r);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = finish<T, EPI>(t[e], b[e]) + r[e];
+  store4<T>((T*)a.y + m * a.N + n, o);
+}
+
+template <typename T, int EPI, int MB>
+int launch_rows(const Fp8Args& a, hipStream_t st, const char* what) {
+  hipLaunchKernelGGL((linear_fp8_rows_kernel<T, EPI, MB>), dim3((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MB - 1) / (16 * MB))),
+                     dim3(512), 0, st, a);
+  return check_launch(what);
 }
 
 template <typename T, int EPI>
 int launch_fp8(const Fp8Args& a, hipStream_t st, const char* what) {
+  const double kb = a.Kb;
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
+  // Kernel by estimated time (us, fits to measured ones within 15%; bias and GELU, us
+  // few rows / 128 x 128 / 256 x 256):
+  //   1024 -> 4096 bf16   M 64: 5.0 / 9.2 / -    256: 13.2 / 9.4 / -    16384: - / 101 / 99    64800: - / 386 / 349
+  //   4096 -> 1024 bf16   M 64: 14.5 / 23.2 / -  512: 27.0 / 24.1 / -   8192: - / 40 / 48      16384: - / 77 / 68
+  //   1024 -> 4096 fp32   M 64: 5.1 / 14.3 / -   512: 23.8 / 14.8 / -
+  // Few rows: every workgroup reads its weights once more for each 64 rows.
+  const int mr = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  const double few = 2.3 + 0.0015 * kb * (double)tiles(16 * mr, 16);
+  const double mid = sizeof(T) == 2 ? std::max(4.5 + 0.61 * kb, (double)tiles(128, 128) / 512 * (3.9 + 1.085 * kb))
+                                    : std::max(5.5 + 1.0 * kb, (double)tiles(128, 128) / 512 * (4 + 1.9 * kb));
+  if (few < mid && a.M < 16 * 65536 * 4LL) {
+    if (mr == 1) return launch_rows<T, EPI, 1>(a, st, what);
+    if (mr == 2) return launch_rows<T, EPI, 2>(a, st, what);
+    return launch_rows<T, EPI, 4>(a, st, what);
+  }
+  if constexpr (sizeof(T) == 2) {
+    using TC = Big8;
+    static_assert(TC::KB >= MAX_KB, "the longest rows' scales fit");
+    const int64_t n = tiles(TC::BM, TC::BN);
+    if (6 + (double)((n + 255) / 256) * (8.5 + 1.53 * kb) < mid) {
+      NSW_CHECK_ARG(n < (1LL << 31), "%s: too many tiles", what);
+      hipLaunchKernelGGL((linear_fp8_deep_kernel<T, EPI, TC>), dim3((unsigned)n), dim3(TC::NW * 64), 0, st, a);
+      return check_launch(what);
+    }
+  }
   using TC = Mid8;
-  const int64_t tiles = ((a.M + TC::BM - 1) / TC::BM) * ((a.N + TC::BN - 1) / TC::BN);
-  NSW_CHECK_ARG(tiles < (1LL << 31), "%s: too many tiles", what);
-  hipLaunchKernelGGL((linear_fp8_kernel<T, EPI, TC>), dim3((unsigned)tiles), dim3(TC::NW * 64), 0, st, a);
+  const int64_t n = tiles(TC::BM, TC::BN);
+  NSW_CHECK_ARG(n < (1LL << 31), "%s: too many tiles", what);
+  hipLaunchKernelGGL((linear_fp8_kernel<T, EPI, TC>), dim3((unsigned)n), dim3(TC::NW * 64), 0, st, a);
   return check_launch(what);
 }
 

@@ -593,7 +593,8 @@ __global__ __launch_bounds__(512) void linear_fp8_rows_kernel(Fp8Args a) {
     int sw[U], sx[U][MB];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int kb = k0 + u * NW < a.Kb ? k0 + u * NW : k0;
+      const int kb = k0 + u * NW;
+      if (kb >= a.Kb) break;
       fw[u] = load(wp + (int64_t)kb * BLK);
       sw[u] = wsp[kb];
 #pragma unroll

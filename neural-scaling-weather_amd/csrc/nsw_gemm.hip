@@ -84,6 +84,9 @@ static int dispatch_gemm(int dtype, const void* x, const void* w, void* y, int64
 
 
 int check_geom(int64_t B, int64_t T, int64_t H, int64_t W, int64_t ws0, int64_t ws1, const char* what);
+bool gated_few_rows(int64_t M, int64_t H, int64_t K, int dtype);
+int gated_rows(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K, int act, int dtype,
+               hipStream_t st, const char* what);
 
 int gemm_qkv(const void* x, const void* wqkv, const void* bqkv, const void* qn_w, const void* kn_w,
              float eps, void* qkv, int64_t M, int64_t C, int64_t num_heads, int dtype, void* stream) {
@@ -198,6 +201,10 @@ int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, v
   NSW_CHECK_ARG(((uintptr_t)bias % 16) == 0, "%s: bias must be 16-byte aligned", what);
   EpiArgs ea{};
   ea.bias = bias; ea.residual = dh; ea.act = act; ea.row_sumsq = colsum;
+  if (!dh && M > 0 && K > 0 && K % (STEPB / (int64_t)dtype_size(dtype)) == 0 && H < (1LL << 30) && K < (1LL << 31) &&
+      (dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32) && (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y) % 16) == 0 &&
+      gated_few_rows(M, H, K, dtype))
+    return gated_rows(x, w, bias, y, M, H, K, act, dtype, (hipStream_t)stream, what);
   if (dh) return dispatch_gemm<EPI_GATED_GRAD>(dtype, x, w, y, M, 2 * H, K, ea, stream, what);
   return dispatch_gemm<EPI_GATED>(dtype, x, w, y, M, 2 * H, K, ea, stream, what);
 }

@@ -20,7 +20,8 @@
 // lane's columns stay the same: the parameters live in registers, and so do the
 // lane's sums for S and Q, which go to a partial row of the workgroup and from there
 // through a second kernel in a fixed order (no atomics: the same bits every time).
-// The next row's loads are issued before the present row's arithmetic.
+// The next row's loads are issued before the present row's arithmetic.  129600 x 1024
+// bf16: forward 180 us (5.9 TB/s), backward 322 us (4.9 TB/s, the second kernel included).
 #include <algorithm>
 
 #include "nsw_common.h"
@@ -107,6 +108,15 @@ __device__ __forceinline__ u32x4 narrow(const float* in) {
   }
 }
 
+// Results past L2 (1-4% faster: 259200 x 512 forward 183 -> 180 us, 129600 x 1024
+// backward 329 -> 322), but not those of workgroup-wide rows (8000 x 8192 backward 188 ->
+// 196).
+template <typename T, class CFG>
+__device__ __forceinline__ void put(T* p, const u32x4& v) {
+  if constexpr (CFG::WG) *reinterpret_cast<u32x4*>(p) = v;
+  else __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));
+}
+
 // The lane's pieces of row `row` (zeros past the row's end).
 template <typename T, class CFG>
 __device__ __forceinline__ void load_row(const void* p, int64_t row, int C, const Lane<CFG>& ln, u32x4 (&raw)[CFG::CH]) {
@@ -187,7 +197,7 @@ __global__ __launch_bounds__(NT) void residual_norm_kernel(NormArgs a) {
     const bool ok = row < r1;
 #pragma unroll
     for (int k = 0; k < CH; ++k)
-      if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.y + row * C + ln.col(k)) = narrow<T>(y[k]);
+      if (ok && ln.col(k) < C) put<T, CFG>((T*)a.y + row * C + ln.col(k), narrow<T>(y[k]));
     if (pre) {
       row_sums<CFG>(s, red, turn);
       const float ry = 1.f / sqrtf(s[0] * inv + a.eps);
@@ -195,7 +205,7 @@ __global__ __launch_bounds__(NT) void residual_norm_kernel(NormArgs a) {
       for (int k = 0; k < CH; ++k) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) y[k][e] = (y[k][e] * ry) * wn[k][e];
-        if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.z + row * C + ln.col(k)) = narrow<T>(y[k]);
+        if (ok && ln.col(k) < C) put<T, CFG>((T*)a.z + row * C + ln.col(k), narrow<T>(y[k]));
       }
     }
 #pragma unroll
@@ -334,7 +344,7 @@ __global__ __launch_bounds__(NT) void residual_norm_backward_kernel(NormArgs a) 
         d[k][e] *= wg[k][e];
         s3[0] = fmaf(d[k][e], oh[k][e], s3[0]);
       }
-      if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.dskip + row * C + ln.col(k)) = narrow<T>(ds);
+      if (ok && ln.col(k) < C) put<T, CFG>((T*)a.dskip + row * C + ln.col(k), narrow<T>(ds));
     }
     if (post) {
       row_sums<CFG>(s3, red, turn);
@@ -346,7 +356,7 @@ __global__ __launch_bounds__(NT) void residual_norm_backward_kernel(NormArgs a) 
     }
 #pragma unroll
     for (int k = 0; k < CH; ++k)
-      if (ok && ln.col(k) < C) *reinterpret_cast<u32x4*>((T*)a.dbranch + row * C + ln.col(k)) = narrow<T>(d[k]);
+      if (ok && ln.col(k) < C) put<T, CFG>((T*)a.dbranch + row * C + ln.col(k), narrow<T>(d[k]));
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       ro_[k] = no_[k];
@@ -360,39 +370,40 @@ __global__ __launch_bounds__(NT) void residual_norm_backward_kernel(NormArgs a) 
   store_part<CFG>(Q, buf, dst + C, C, ln);
 }
 
-// dgate, dpost_w and dnorm_w from the workgroups' partial rows [G P][2][C], 32
-// columns to a workgroup: 8 lanes hold 4 columns each, 32 groups of them take every
-// 32nd partial row and meet in LDS, always in the same order.
+// dgate, dpost_w and dnorm_w from the workgroups' partial rows [G P][2][C], 16
+// columns to a workgroup: 4 lanes hold 4 columns each, 64 groups of them take every
+// 64th partial row and meet in LDS, always in the same order.
 template <typename T>
 __global__ __launch_bounds__(NT) void residual_norm_params_kernel(const float* __restrict__ part, int G, int P, int C,
                                                                   const T* __restrict__ post_w, const T* __restrict__ gate,
                                                                   T* __restrict__ dpost, T* __restrict__ dgate,
                                                                   T* __restrict__ dnorm) {
-  __shared__ __attribute__((aligned(16))) float red[32][36];
-  const int cl = ((int)threadIdx.x & 7) * 4, grp = (int)threadIdx.x >> 3;
-  const int c = (int)blockIdx.x * 32 + cl;
+  constexpr int NG = NT / 4;
+  __shared__ __attribute__((aligned(16))) float red[NG][20];
+  const int cl = ((int)threadIdx.x & 3) * 4, grp = (int)threadIdx.x >> 2;
+  const int c = (int)blockIdx.x * 16 + cl;
   const bool in = c < C;
   // the sum over rows [p0, p1) of partial array h, for the thread's 4 columns where grp == 0
   auto sum = [&](int64_t p0, int64_t p1, int h) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
     if (in) {
-#pragma unroll 4
-      for (int64_t p = p0 + grp; p < p1; p += 32) t += *reinterpret_cast<const f32x4*>(part + (p * 2 + h) * C + c);
+#pragma unroll 8
+      for (int64_t p = p0 + grp; p < p1; p += NG) t += *reinterpret_cast<const f32x4*>(part + (p * 2 + h) * C + c);
     }
     __syncthreads();
     *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
     __syncthreads();
-    if (grp < 4) {
+    if (grp < 8) {
       t = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t += *reinterpret_cast<const f32x4*>(&red[grp * 8 + i][cl]);
+      for (int i = 0; i < NG / 8; ++i) t += *reinterpret_cast<const f32x4*>(&red[grp * (NG / 8) + i][cl]);
     }
     __syncthreads();
-    if (grp < 4) *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
+    if (grp < 8) *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
     __syncthreads();
     if (grp == 0) {
 #pragma unroll
-      for (int i = 1; i < 4; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
+      for (int i = 1; i < 8; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
     }
     return t;
   };
@@ -434,7 +445,13 @@ inline Split split_rows(int64_t R, int64_t G, int rps, int per_cu) {
   return {each * rps, (int)((turns + each - 1) / each)};
 }
 
-constexpr int FWD_PER_CU = 16, BWD_PER_CU = 4;
+// Workgroups to a compute unit.  Forward: many, so that the last ones to finish are
+// short (259200 x 512 bf16, us: 4 216, 16 208, 32 197, 128 183).  Backward: as many as
+// its registers let run at once, since each leaves partial rows for the second kernel
+// (bf16, us with it: 259200 x 512 2 407, 4 340, 8 340; 129600 x 1024 1 373, 2 328, 4 335).
+constexpr int FWD_PER_CU = 128;
+template <typename T, class CFG>
+constexpr int BWD_PER_CU = CFG::CH == 1 ? 4 : (sizeof(T) == 2 ? 4 : 8) / CFG::CH;
 
 // f(RowCfg) for the narrowest shape that holds C.
 template <typename T, class F>
@@ -463,7 +480,7 @@ template <typename T>
 int64_t backward_parts(int64_t rows, int64_t C, int64_t G) {
   int64_t n = 0;
   with_cfg<T>(C, [&](auto cfg) {
-    n = (int64_t)split_rows(rows / G, G, decltype(cfg)::RPS, BWD_PER_CU).P * G;
+    n = (int64_t)split_rows(rows / G, G, decltype(cfg)::RPS, BWD_PER_CU<T, decltype(cfg)>).P * G;
     return 0;
   });
   return n;
@@ -487,14 +504,14 @@ int launch_backward(NormArgs a, int64_t rows, int64_t G, void* dpost, void* dgat
   int P = 0;
   int rc = with_cfg<T>(a.C, [&](auto cfg) {
     using CFG = decltype(cfg);
-    const Split s = split_rows(rows / G, G, CFG::RPS, BWD_PER_CU);
+    const Split s = split_rows(rows / G, G, CFG::RPS, BWD_PER_CU<T, CFG>);
     a.R = rows / G; a.per = s.per; a.P = P = s.P;
     if (rows == 0) return (int)NSW_OK;
     hipLaunchKernelGGL((residual_norm_backward_kernel<T, CFG>), dim3((unsigned)(G * s.P)), dim3(NT), 0, st, a);
     return check_launch(what);
   });
   if (rc || (!dpost && !dgate && !dnorm)) return rc;
-  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 31) / 32)), dim3(NT), 0, st, a.part, (int)G, P,
+  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 15) / 16)), dim3(NT), 0, st, a.part, (int)G, P,
                      a.C, (const T*)a.post_w, (const T*)a.gate, (T*)dpost, (T*)dgate, (T*)dnorm);
   return check_launch(what);
 }

@@ -7,7 +7,6 @@ all arithmetic runs in libnsw's kernels).  Inputs must be contiguous,
 """
 from __future__ import annotations
 
-import contextlib
 import threading
 from typing import Optional, Sequence, Tuple
 
@@ -52,7 +51,13 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle without a Stream object around it (0.1 us, not 1.9)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev: torch.device):
+    if _raw_stream is not None and dev.index is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
@@ -184,9 +189,15 @@ def rmsnorm_roll_partition(x: torch.Tensor, weight: torch.Tensor, window_size, s
     return out
 
 
-def _guard(dev: torch.device):
-    """Makes dev the current device for a launch on its stream."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _run(what: str, dev: torch.device, fn, *args) -> None:
+    """fn(*args, stream) with dev as the current device, its error raised."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        check(rc, what)
 
 
 def _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps):
@@ -225,10 +236,8 @@ def residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optiona
     dev, rows, C, G, eps = _residual_norm_args("residual_norm", branch, skip, post_weight, gate, norm_weight, eps)
     y = torch.empty_like(branch)
     z = None if norm_weight is None else torch.empty_like(branch)
-    with _guard(dev):
-        check(lib().nsw_residual_norm(branch.data_ptr(), skip.data_ptr(), _p(post_weight), _p(gate), _p(norm_weight),
-                                      y.data_ptr(), _p(z), rows, C, G, float(alpha), eps, dtype_code(branch),
-                                      _stream(dev)), "residual_norm")
+    _run("residual_norm", dev, lib().nsw_residual_norm, branch.data_ptr(), skip.data_ptr(), _p(post_weight), _p(gate),
+         _p(norm_weight), y.data_ptr(), _p(z), rows, C, G, float(alpha), eps, dtype_code(branch))
     return y, z
 
 
@@ -261,11 +270,9 @@ def residual_norm_backward(dy: Optional[torch.Tensor], dz: Optional[torch.Tensor
     code = dtype_code(branch)
     nbytes = int(lib().nsw_residual_norm_backward_workspace_size(rows, C, G, code))
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    with _guard(dev):
-        check(lib().nsw_residual_norm_backward(_p(dy), _p(dz), branch.data_ptr(), skip.data_ptr(), _p(post_weight),
-                                               _p(gate), _p(nw), db.data_ptr(), ds.data_ptr(), _p(dp), _p(dg),
-                                               None if dz is None else _p(dn), rows, C, G, float(alpha), eps, code,
-                                               ws.data_ptr(), nbytes, _stream(dev)), what)
+    _run(what, dev, lib().nsw_residual_norm_backward, _p(dy), _p(dz), branch.data_ptr(), skip.data_ptr(),
+         _p(post_weight), _p(gate), _p(nw), db.data_ptr(), ds.data_ptr(), _p(dp), _p(dg), None if dz is None else _p(dn),
+         rows, C, G, float(alpha), eps, code, ws.data_ptr(), nbytes)
     return db, ds, dp, dg, dn
 
 
@@ -328,9 +335,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     h = torch.empty(x.shape[:-1] + (H,), dtype=x.dtype, device=dev)
     if M == 0:
         return h
-    with _guard(dev):
-        check(lib().nsw_gated_linear(x.data_ptr(), weight.data_ptr(), _p(bias), h.data_ptr(), M, H, K, code,
-                                     dtype_code(x), _stream(dev)), "gated_linear")
+    _run("gated_linear", dev, lib().nsw_gated_linear, x.data_ptr(), weight.data_ptr(), _p(bias), h.data_ptr(), M, H, K,
+         code, dtype_code(x))
     return h
 
 
@@ -357,10 +363,8 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     nbytes = int(lib().nsw_gated_linear_backward_workspace_size(M, H, K, dtype_code(x)))
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    with _guard(dev):
-        check(lib().nsw_gated_linear_backward(dh.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(dx), _p(dw),
-                                              _p(db), M, H, K, code, dtype_code(x), ws.data_ptr(), nbytes,
-                                              _stream(dev)), what)
+    _run(what, dev, lib().nsw_gated_linear_backward, dh.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(dx),
+         _p(dw), _p(db), M, H, K, code, dtype_code(x), ws.data_ptr(), nbytes)
     return dx, dw, db
 
 
@@ -383,9 +387,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     nbytes = int(lib().nsw_linear_backward_workspace_size(M, N, K, dtype_code(x)))
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    with _guard(dev):
-        check(lib().nsw_linear_backward(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(dx), _p(dw), _p(db), M, N, K,
-                                        dtype_code(x), ws.data_ptr(), nbytes, _stream(dev)), what)
+    _run(what, dev, lib().nsw_linear_backward, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(dx), _p(dw), _p(db), M,
+         N, K, dtype_code(x), ws.data_ptr(), nbytes)
     return dx, dw, db
 
 
@@ -411,9 +414,7 @@ def quantize_fp8(x: torch.Tensor, rows: int = 1) -> Tuple[torch.Tensor, torch.Te
     lead = x.shape[:-1] if rows == 1 else ((R + rows - 1) // rows,)
     scale = torch.empty(tuple(lead) + (Kb,), dtype=torch.float8_e8m0fnu, device=dev)
     if R:
-        with _guard(dev):
-            check(lib().nsw_quantize_fp8(x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, rows, code, _stream(dev)),
-                  "quantize_fp8")
+        _run("quantize_fp8", dev, lib().nsw_quantize_fp8, x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, rows, code)
     return q, scale
 
 
@@ -451,10 +452,8 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     if residual is not None and residual.shape != y.shape:
         raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")
     if y.numel():
-        with _guard(dev):
-            check(lib().nsw_linear_fp8(xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), _p(bias),
-                                       _p(residual), y.data_ptr(), xq.numel() // K, N, K, int(epilogue), _DTYPES[dtype],
-                                       _stream(dev)), what)
+        _run(what, dev, lib().nsw_linear_fp8, xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
+             _p(bias), _p(residual), y.data_ptr(), xq.numel() // K, N, K, int(epilogue), _DTYPES[dtype])
     return y
 
 

@@ -13,7 +13,7 @@ import math
 import torch
 from torch import nn
 
-from . import ops, torch_ops
+from . import _lib, ops, torch_ops
 
 def submodule(module, name: str):
     """``module.name`` for a registered submodule, without the failed instance
@@ -115,3 +115,71 @@ class NormLayer(nn.Module):
             w = torch.ones(x.shape[-1], dtype=x.dtype, device=x.device)
         eps = self.norm.eps
         return torch.ops.nsw.rms_norm(x, w, ops.default_eps(x.dtype) if eps is None else float(eps))
+
+
+class ResidualNorm(nn.Module):
+    """The end of one residual branch and the norm before the next, in one pass
+    with gradients (no counterpart in the reference, whose blocks are pre-norm
+    without gates): y = alpha * skip + gate * RMSNorm(branch) and z =
+    RMSNorm(y).
+
+    post_norm    a norm after the branch (``post_norm.norm.weight``)
+    layer_scale  initial value of a learned gate for every channel (``gamma``),
+                 None: no learned gate; a gate given to ``forward`` (of a
+                 condition: [C], or [B, C] for B equal parts of the rows)
+                 multiplies the branch instead
+    alpha        scale of the residual
+    next_norm    the norm before the next branch (``next_norm.norm.weight``);
+                 without it z is None
+    """
+
+    def __init__(self, dim, post_norm=True, layer_scale=None, alpha=1.0, next_norm=True, comm_metadata=None):
+        super().__init__()
+        self.post_norm = NormLayer(dim, norm_type="rms_norm", comm_metadata=comm_metadata) if post_norm else None
+        self.next_norm = NormLayer(dim, norm_type="rms_norm", comm_metadata=comm_metadata) if next_norm else None
+        self.gamma = None if layer_scale is None else nn.Parameter(torch.full((dim,), float(layer_scale)))
+        if self.gamma is not None:
+            self.gamma.comm_metadata = comm_metadata or {"sharded": [None], "shared": [], "reduce": []}
+        self.alpha = float(alpha)
+
+    def forward(self, branch, skip, gate=None):
+        norms = [n.norm for n in (self.post_norm, self.next_norm) if n is not None]
+        eps = {n.eps for n in norms}
+        if len(eps) > 1:
+            raise NotImplementedError("the two norms of a ResidualNorm share eps")
+        if gate is not None and self.gamma is not None:
+            raise ValueError("ResidualNorm: a gate is given and a layer scale is learned")
+        return torch_ops.residual_norm(branch, skip, None if self.post_norm is None else self.post_norm.norm.weight,
+                                       self.gamma if gate is None else gate, self.alpha,
+                                       None if self.next_norm is None else self.next_norm.norm.weight,
+                                       eps.pop() if eps else None)
+
+
+class Fp8Linear(nn.Module):
+    """A linear layer served in 8-bit floating point: the weight is quantised
+    once (e4m3, a power-of-two scale for each 128 x 128 block), the rows in
+    every call (a scale for each 1 x 128 block); forward only.  ``epilogue`` as
+    ``nsw.ops.linear``; the result has the input's dtype."""
+
+    def __init__(self, weight: torch.Tensor, bias=None, epilogue=None):
+        super().__init__()
+        q, scale = torch.ops.nsw.quantize_fp8(weight.detach(), ops.FP8_BLOCK)
+        self.register_buffer("weight", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+        self.epilogue = epilogue
+
+    @classmethod
+    def from_layers(cls, linear: LinearLayer, bias=None, epilogue=None):
+        """Of a LinearLayer and the BiasLayer after it, if any."""
+        return cls(linear.weight, None if bias is None else bias.bias, epilogue)
+
+    def forward(self, x, residual=None):
+        xq, xs = torch.ops.nsw.quantize_fp8(x, 1)
+        epi = self.epilogue
+        if epi is None or residual is not None:
+            epi = _lib.NSW_EPI_NONE if self.bias is None else (
+                _lib.NSW_EPI_BIAS if residual is None else _lib.NSW_EPI_BIAS_RESIDUAL)
+        if residual is not None and epi != _lib.NSW_EPI_BIAS_RESIDUAL:
+            raise NotImplementedError("a residual without a bias is not fused")
+        return torch.ops.nsw.linear_fp8(xq, xs, self.weight, self.weight_scale, self.bias, residual, int(epi), x.dtype)

@@ -10,6 +10,10 @@ and enqueue HIP kernels on the current stream, so they also run under CUDA
 graph capture.  Ops that write into a caller's tensor (``out=``) are not
 registered; their callers keep the ``nsw.ops`` functions.
 
+``linear`` (without GELU), ``gated_linear`` and ``residual_norm`` have
+gradients (``linear_backward``, ``gated_linear_backward``,
+``residual_norm_backward``); the others are forward only.
+
 The block parameters travel as one list in the field order of
 ``nsw_block_params`` (``BLOCK_PARAMS``), None for absent fields; shapes,
 windows and shifts as int lists.
@@ -104,6 +108,183 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], 
 @linear.register_fake
 def _(x, weight, bias, residual, epilogue):
     return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and 16-byte aligned (a gradient may be any view)."""
+    t = t.contiguous()
+    return t.clone() if t.is_cuda and t.data_ptr() % 16 else t
+
+
+def _or_empty(like: torch.Tensor, *ts: Optional[torch.Tensor]) -> Tuple[torch.Tensor, ...]:
+    """ts with an empty tensor in the place of None (custom ops return tensors)."""
+    return tuple(like.new_empty((0,)) if t is None else t for t in ts)
+
+
+@torch.library.custom_op("nsw::linear_backward", mutates_args=())
+def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                    needs: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias) of a linear without an activation; empty ([0]) where ``needs`` is False."""
+    return _or_empty(x, *ops.linear_backward(_dense(dy), _dense(x), _dense(weight), needs=tuple(needs)))
+
+
+@linear_backward.register_fake
+def _(dy, x, weight, needs):
+    return (x.new_empty(x.shape if needs[0] else (0,)), x.new_empty(weight.shape if needs[1] else (0,)),
+            x.new_empty((weight.shape[0],) if needs[2] else (0,)))
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, residual, epilogue = inputs
+    ctx.epilogue = epilogue
+    if epilogue in (_lib.NSW_EPI_NONE, _lib.NSW_EPI_BIAS, _lib.NSW_EPI_BIAS_RESIDUAL):
+        ctx.save_for_backward(x, weight)
+
+
+def _linear_backward(ctx, dy):
+    if ctx.epilogue not in (_lib.NSW_EPI_NONE, _lib.NSW_EPI_BIAS, _lib.NSW_EPI_BIAS_RESIDUAL):
+        raise NotImplementedError("nsw.linear with a GELU epilogue has no gradient (nsw.GatedMLP has)")
+    need = list(ctx.needs_input_grad)
+    x, weight = ctx.saved_tensors
+    needs = [need[0], need[1], need[2]]
+    dx, dw, db = torch.ops.nsw.linear_backward(dy, x, weight, needs) if any(needs) else (None, None, None)
+    return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dy if need[3] else None, None)
+
+
+linear.register_autograd(_linear_backward, setup_context=_linear_setup)
+
+
+@torch.library.custom_op("nsw::gated_linear", mutates_args=())
+def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], act: str) -> torch.Tensor:
+    """act(x Wg^T + bg) * (x Wu^T + bu), weight [2H, K] = Wg over Wu."""
+    return ops.gated_linear(_dense(x), _dense(weight), bias, act=act)
+
+
+@gated_linear.register_fake
+def _(x, weight, bias, act):
+    return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0] // 2,))
+
+
+@torch.library.custom_op("nsw::gated_linear_backward", mutates_args=())
+def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                          act: str, needs: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias) of gated_linear; empty ([0]) where ``needs`` is False or there is no bias."""
+    return _or_empty(x, *ops.gated_linear_backward(_dense(dh), _dense(x), _dense(weight), bias, act=act,
+                                                   needs=tuple(needs)))
+
+
+@gated_linear_backward.register_fake
+def _(dh, x, weight, bias, act, needs):
+    return (x.new_empty(x.shape if needs[0] else (0,)), x.new_empty(weight.shape if needs[1] else (0,)),
+            x.new_empty(bias.shape if needs[2] and bias is not None else (0,)))
+
+
+def _gated_setup(ctx, inputs, output):
+    x, weight, bias, act = inputs
+    ctx.act, ctx.has_bias = act, bias is not None
+    ctx.save_for_backward(x, weight, *([bias] if bias is not None else []))
+
+
+def _gated_backward(ctx, dh):
+    x, weight, *rest = ctx.saved_tensors
+    need = list(ctx.needs_input_grad)
+    dx, dw, db = torch.ops.nsw.gated_linear_backward(dh, x, weight, rest[0] if ctx.has_bias else None, ctx.act,
+                                                     [need[0], need[1], need[2]])
+    return dx if need[0] else None, dw if need[1] else None, db if need[2] and ctx.has_bias else None, None
+
+
+gated_linear.register_autograd(_gated_backward, setup_context=_gated_setup)
+
+
+@torch.library.custom_op("nsw::quantize_fp8", mutates_args=())
+def quantize_fp8(x: torch.Tensor, rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 values, E8M0 scales) of x, a scale for each block of rows (1 or 128) x 128."""
+    return ops.quantize_fp8(_dense(x), rows=rows)
+
+
+@quantize_fp8.register_fake
+def _(x, rows):
+    Kb = (x.shape[-1] + ops.FP8_BLOCK - 1) // ops.FP8_BLOCK
+    lead = tuple(x.shape[:-1]) if rows == 1 else ((x.shape[0] + rows - 1) // rows,)
+    return (x.new_empty(tuple(x.shape[:-1]) + (Kb * ops.FP8_BLOCK,), dtype=torch.float8_e4m3fn),
+            x.new_empty(lead + (Kb,), dtype=torch.float8_e8m0fnu))
+
+
+@torch.library.custom_op("nsw::linear_fp8", mutates_args=())
+def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+               bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], epilogue: int,
+               dtype: torch.dtype) -> torch.Tensor:
+    """nsw.linear on operands from quantize_fp8, the result in dtype."""
+    return ops.linear_fp8(xq.contiguous(), x_scale.contiguous(), wq, w_scale, bias,
+                          None if residual is None else _dense(residual), epilogue=epilogue, dtype=dtype)
+
+
+@linear_fp8.register_fake
+def _(xq, x_scale, wq, w_scale, bias, residual, epilogue, dtype):
+    return xq.new_empty(tuple(xq.shape[:-1]) + (wq.shape[0],), dtype=dtype)
+
+
+@torch.library.custom_op("nsw::residual_norm", mutates_args=())
+def _residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optional[torch.Tensor],
+                   gate: Optional[torch.Tensor], alpha: float, norm_weight: Optional[torch.Tensor],
+                   eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _or_empty(branch, *ops.residual_norm(_dense(branch), _dense(skip), post_weight,
+                                                None if gate is None else _dense(gate), alpha, norm_weight, eps))
+
+
+@_residual_norm.register_fake
+def _(branch, skip, post_weight, gate, alpha, norm_weight, eps):
+    y = torch.empty_like(branch, memory_format=torch.contiguous_format)
+    return y, branch.new_empty((0,)) if norm_weight is None else torch.empty_like(y)
+
+
+@torch.library.custom_op("nsw::residual_norm_backward", mutates_args=())
+def _residual_norm_backward(dy: Optional[torch.Tensor], dz: Optional[torch.Tensor], branch: torch.Tensor,
+                            skip: torch.Tensor, post_weight: Optional[torch.Tensor], gate: Optional[torch.Tensor],
+                            alpha: float, norm_weight: Optional[torch.Tensor], eps: float
+                            ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _or_empty(branch, *ops.residual_norm_backward(
+        None if dy is None else _dense(dy), None if dz is None else _dense(dz), _dense(branch), _dense(skip), post_weight,
+        None if gate is None else _dense(gate), alpha, norm_weight, eps))
+
+
+@_residual_norm_backward.register_fake
+def _(dy, dz, branch, skip, post_weight, gate, alpha, norm_weight, eps):
+    full = lambda t: branch.new_empty((0,) if t is None else t.shape)
+    return full(branch), full(skip), full(post_weight), full(gate), full(norm_weight)
+
+
+def _residual_setup(ctx, inputs, output):
+    branch, skip, post_weight, gate, alpha, norm_weight, eps = inputs
+    ctx.alpha, ctx.eps = alpha, eps
+    ctx.given = [t is not None for t in (post_weight, gate, norm_weight)]
+    ctx.save_for_backward(branch, skip, *[t for t in (post_weight, gate, norm_weight) if t is not None])
+    ctx.set_materialize_grads(False)
+
+
+def _residual_backward(ctx, dy, dz):
+    branch, skip, *rest = ctx.saved_tensors
+    rest = iter(rest)
+    post_weight, gate, norm_weight = (next(rest) if g else None for g in ctx.given)
+    if norm_weight is None:
+        dz = None
+    if dy is None and dz is None:
+        return (None,) * 7
+    db, ds, dp, dg, dn = torch.ops.nsw.residual_norm_backward(dy, dz, branch, skip, post_weight, gate, ctx.alpha,
+                                                              norm_weight, ctx.eps)
+    return (db, ds, dp if ctx.given[0] else None, dg if ctx.given[1] else None, None, dn if ctx.given[2] else None, None)
+
+
+_residual_norm.register_autograd(_residual_backward, setup_context=_residual_setup)
+
+
+def residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, alpha: float = 1.0,
+                  norm_weight: Optional[torch.Tensor] = None, eps: Optional[float] = None):
+    """torch.ops.nsw.residual_norm with ops.residual_norm's defaults: (y, z or None)."""
+    y, z = torch.ops.nsw.residual_norm(branch, skip, post_weight, gate, float(alpha), norm_weight,
+                                       ops.default_eps(branch.dtype) if eps is None else float(eps))
+    return y, None if norm_weight is None else z
 
 
 @torch.library.custom_op("nsw::linear_to_window", mutates_args=())

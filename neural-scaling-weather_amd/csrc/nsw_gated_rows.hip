@@ -1,10 +1,12 @@
-// nsw_gated_linear for few rows: the weights' bytes and the latency count.  A workgroup
+// nsw_gated_linear for few rows, and the gradients of its sums (EPI_GATED_GRAD of the
+// GEMM): the weights' bytes and the latency count.  A workgroup
 // of eight waves takes 16 hidden columns (16 gate and 16 up rows of w) and 16 MB rows of
 // x; the waves share out k in steps of 128 bytes of a row, operands straight from global
 // memory (lane (i, g): 32 bytes of row i, so a row's 128-byte line is four lanes'
 // loads), and their sums meet in LDS in a fixed order.  bf16 on v_mfma_f32_16x16x32_bf16,
 // fp32 on v_mfma_f32_16x16x4_f32: any order of k serves as long as both operands have it.
 #include <algorithm>
+#include <type_traits>
 
 #include "nsw_gemm_common.h"
 
@@ -12,9 +14,10 @@ namespace nsw {
 
 namespace {
 
-template <typename T, int MB>
+template <typename T, int MB, bool GRAD>
 __global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                         const T* __restrict__ bias, T* __restrict__ h, int64_t M, int H,
+                                                         const T* __restrict__ bias, const T* __restrict__ dh,
+                                                         T* __restrict__ y, float* __restrict__ colsum, int64_t M, int H,
                                                          int K, int act) {
   constexpr int NW = 8, STEP = 128 / (int)sizeof(T);        // k of a step
   constexpr int U = MB == 4 ? 2 : 4;                        // steps whose loads are in flight together
@@ -81,11 +84,11 @@ __global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ x
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) red[wave][j][mb][lane] = acc[j][mb];
   __syncthreads();
-  // lane (i, g) of row block mb holds h[m0 + mb 16 + i][n0 + 4 g + r]
+  // lane (i, g) of row block mb holds columns n0 + 4 g + r of row m0 + mb 16 + i
   if (wave >= MB) return;
   const int64_t m = m0 + wave * 16 + i;
   const int n = n0 + 4 * g;
-  if (m >= M) return;
+  if (!GRAD && m >= M) return;                              // GRAD: every lane takes part in the column sums
   f32x4 t[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -93,33 +96,65 @@ __global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ x
 #pragma unroll
     for (int v = 1; v < NW; ++v) t[j] += red[v][j][wave][lane];
   }
-  float b[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, o[4];
+  float b[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, o[2][4], d4[4] = {0.f, 0.f, 0.f, 0.f};
   if (bias != nullptr) {
     load4<T>(bias + n, b[0]);
     load4<T>(bias + H + n, b[1]);
   }
+  if (GRAD && m < M) load4<T>(dh + m * H + n, d4);
+  auto form = [&](auto f) {
+    constexpr int ACT = decltype(f)::value;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float gt = t[0][e] + b[0][e];
-    const float a = act == NSW_ACT_SILU ? gate_act<T, NSW_ACT_SILU>(gt)
-                    : act == NSW_ACT_GELU ? gate_act<T, NSW_ACT_GELU>(gt) : gate_act<T, NSW_ACT_GELU_TANH>(gt);
-    o[e] = a * (t[1][e] + b[1][e]);
+    for (int e = 0; e < 4; ++e) {
+      const float gt = t[0][e] + b[0][e], up = t[1][e] + b[1][e];
+      if constexpr (GRAD) {
+        float a, d;
+        gate_act_grad<ACT>(gt, a, d);
+        o[0][e] = d4[e] * up * d;
+        o[1][e] = d4[e] * a;
+      } else {
+        o[0][e] = gate_act<T, ACT>(gt) * up;
+      }
+    }
+  };
+  if (act == NSW_ACT_SILU) form(std::integral_constant<int, NSW_ACT_SILU>{});
+  else if (act == NSW_ACT_GELU) form(std::integral_constant<int, NSW_ACT_GELU>{});
+  else form(std::integral_constant<int, NSW_ACT_GELU_TANH>{});
+  if constexpr (GRAD) {
+    if (m < M) {
+      store4<T>(y + m * 2 * H + n, o[0]);
+      store4<T>(y + m * 2 * H + H + n, o[1]);
+    }
+    if (colsum != nullptr) {                                // row blockIdx.y MB + wave of [.., 2H]
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f32x4 c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = row16_sum(m < M ? o[j][e] : 0.f);
+        if (i == 0) *reinterpret_cast<f32x4*>(colsum + ((int64_t)blockIdx.y * MB + wave) * 2 * H + j * H + n) = c;
+      }
+    }
+  } else {
+    store4<T>(y + m * H + n, o[0]);
   }
-  store4<T>(h + m * H + n, o);
 }
 
 }  // namespace
 
-template <typename T>
-static int launch_rows(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K, int act,
-                       hipStream_t st, const char* what) {
-  const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+static int row_blocks(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
+
+template <typename T, bool GRAD>
+static int launch_rows(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M,
+                       int64_t H, int64_t K, int act, hipStream_t st, const char* what) {
+  const int mb = row_blocks(M);
   const dim3 grid((unsigned)(H / 16), (unsigned)((M + 16 * mb - 1) / (16 * mb))), block(512);
-  const T *xp = (const T*)x, *wp = (const T*)w, *bp = (const T*)bias;
-  T* hp = (T*)h;
-  if (mb == 1) hipLaunchKernelGGL((gated_rows_kernel<T, 1>), grid, block, 0, st, xp, wp, bp, hp, M, (int)H, (int)K, act);
-  else if (mb == 2) hipLaunchKernelGGL((gated_rows_kernel<T, 2>), grid, block, 0, st, xp, wp, bp, hp, M, (int)H, (int)K, act);
-  else hipLaunchKernelGGL((gated_rows_kernel<T, 4>), grid, block, 0, st, xp, wp, bp, hp, M, (int)H, (int)K, act);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, (const T*)x, (const T*)w, (const T*)bias, (const T*)dh, (T*)y, colsum, M,
+                       (int)H, (int)K, act);
+  };
+  if (mb == 1) go(gated_rows_kernel<T, 1, GRAD>);
+  else if (mb == 2) go(gated_rows_kernel<T, 2, GRAD>);
+  else go(gated_rows_kernel<T, 4, GRAD>);
   return check_launch(what);
 }
 
@@ -137,10 +172,20 @@ bool gated_few_rows(int64_t M, int64_t H, int64_t K, int dtype) {
   return std::max(3 + 0.5 * steps, 3 + (double)wgs * (0.004 + 0.0022 * steps)) < 6.5 + 0.0335 * (double)K;
 }
 
-int gated_rows(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K, int act, int dtype,
-               hipStream_t st, const char* what) {
-  return dtype == NSW_DTYPE_BF16 ? launch_rows<bf16>(x, w, bias, h, M, H, K, act, st, what)
-                                 : launch_rows<float>(x, w, bias, h, M, H, K, act, st, what);
+// Rows of gated_rows' colsum.
+int64_t gated_rows_parts(int64_t M) {
+  const int64_t mb = row_blocks(M);
+  return (M + 16 * mb - 1) / (16 * mb) * mb;
+}
+
+// As gemm_gated (dh and colsum NULL: forward).
+int gated_rows(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M, int64_t H,
+               int64_t K, int act, int dtype, hipStream_t st, const char* what) {
+  if (dtype == NSW_DTYPE_BF16)
+    return dh ? launch_rows<bf16, true>(x, w, bias, dh, y, colsum, M, H, K, act, st, what)
+              : launch_rows<bf16, false>(x, w, bias, dh, y, colsum, M, H, K, act, st, what);
+  return dh ? launch_rows<float, true>(x, w, bias, dh, y, colsum, M, H, K, act, st, what)
+            : launch_rows<float, false>(x, w, bias, dh, y, colsum, M, H, K, act, st, what);
 }
 
 }  // namespace nsw

@@ -85,8 +85,9 @@ static int dispatch_gemm(int dtype, const void* x, const void* w, void* y, int64
 
 int check_geom(int64_t B, int64_t T, int64_t H, int64_t W, int64_t ws0, int64_t ws1, const char* what);
 bool gated_few_rows(int64_t M, int64_t H, int64_t K, int dtype);
-int gated_rows(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K, int act, int dtype,
-               hipStream_t st, const char* what);
+int64_t gated_rows_parts(int64_t M);
+int gated_rows(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M, int64_t H,
+               int64_t K, int act, int dtype, hipStream_t st, const char* what);
 
 int gemm_qkv(const void* x, const void* wqkv, const void* bqkv, const void* qn_w, const void* kn_w,
              float eps, void* qkv, int64_t M, int64_t C, int64_t num_heads, int dtype, void* stream) {
@@ -199,12 +200,17 @@ int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, v
   NSW_CHECK_ARG(x && w && y, "%s: x, w and y are required", what);
   NSW_CHECK_ARG(H > 0 && H % 16 == 0, "%s: H=%lld must be a positive multiple of 16", what, (long long)H);
   NSW_CHECK_ARG(((uintptr_t)bias % 16) == 0, "%s: bias must be 16-byte aligned", what);
+  NSW_CHECK_ARG(dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32, "%s: unknown dtype %d", what, dtype);
+  const int64_t step = STEPB / (int64_t)dtype_size(dtype);
+  NSW_CHECK_ARG(M > 0 && K > 0 && M < (1LL << 31) && H < (1LL << 30) && K < (1LL << 31),
+                "%s: M, H, K must be positive and below 2^31 (2H, too)", what);
+  NSW_CHECK_ARG(K % step == 0, "%s: K=%lld must be a multiple of %lld", what, (long long)K, (long long)step);
+  NSW_CHECK_ARG((((uintptr_t)x | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)y) % 16) == 0,
+                "%s: x, w and the results must be 16-byte aligned", what);
+  if (gated_few_rows(M, H, K, dtype))
+    return gated_rows(x, w, bias, dh, y, colsum, M, H, K, act, dtype, (hipStream_t)stream, what);
   EpiArgs ea{};
   ea.bias = bias; ea.residual = dh; ea.act = act; ea.row_sumsq = colsum;
-  if (!dh && M > 0 && K > 0 && K % (STEPB / (int64_t)dtype_size(dtype)) == 0 && H < (1LL << 30) && K < (1LL << 31) &&
-      (dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32) && (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y) % 16) == 0 &&
-      gated_few_rows(M, H, K, dtype))
-    return gated_rows(x, w, bias, y, M, H, K, act, dtype, (hipStream_t)stream, what);
   if (dh) return dispatch_gemm<EPI_GATED_GRAD>(dtype, x, w, y, M, 2 * H, K, ea, stream, what);
   return dispatch_gemm<EPI_GATED>(dtype, x, w, y, M, 2 * H, K, ea, stream, what);
 }
@@ -213,6 +219,7 @@ int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, v
 int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
   static_assert(BigTile::WGM == 2 && MidTile::WGM == 2 && SmallTile::WGM == 2 && SmallF32Tile::WGM == 2 &&
                     SmallTile::BM == SmallF32Tile::BM, "two wave rows to a tile");
+  if (gated_few_rows(M, H, K, dtype)) return gated_rows_parts(M);
   const EpiArgs ea{};
   const TileSize t = dtype == NSW_DTYPE_F32 ? pick_tile<float, EPI_GATED_GRAD>(M, 2 * H, K, ea)
                                             : pick_tile<bf16, EPI_GATED_GRAD>(M, 2 * H, K, ea);
@@ -220,12 +227,15 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
   return (M + bm - 1) / bm * 2;
 }
 
-// fp32 y[s] [M, N] = x[s] [M, K] . w[s] [N, K]^T for s < batch.
-int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int batch, hipStream_t st,
-                   const char* what) {
+// fp32 y[s] [M, N] = x[s] [M, K] . w[s] [N, K]^T for s < batch: rows ld values apart (a
+// multiple of 4), the products' operands xs and ws values apart, the results one after
+// the other.
+int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t ld, int64_t xs, int64_t ws,
+                   int batch, hipStream_t st, const char* what) {
   NSW_CHECK_ARG(batch > 0 && batch < 65536, "%s: too many products", what);
+  NSW_CHECK_ARG((uint64_t)std::max(M, N) * ld * 4 < (1ULL << 31), "%s: operands above 2 GiB are not supported", what);
   EpiArgs ea{};
-  ea.batch = batch;
+  ea.batch = batch; ea.ld = (int)ld; ea.xs = xs; ea.ws = ws;
   return launch_gemm<float, EPI_BATCH, PRE_NONE>(x, w, y, M, N, K, ea, st, what);
 }
 

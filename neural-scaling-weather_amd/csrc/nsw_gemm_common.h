@@ -23,7 +23,7 @@ enum Epi {
   EPI_GATED = 17,            // w stacks gate and up rows [2H, K]: y[m, h] = act(g) u, optional bias [2H]
   EPI_GATED_GRAD = 18,       // the same product formed again: y[M, 2H] = the gradients of g and u from
                              // that of act(g) u (residual), optional column sums into row_sumsq
-  EPI_BATCH = 19,            // no bias; blockIdx.y products of dense operands, one after the other in memory
+  EPI_BATCH = 19,            // no bias; blockIdx.y products, their operands' rows ea.ld values apart
   EPI_QKV_HN16 = 16,         // bias, then per-head RMSNorm of the q and k
   EPI_QKV_HN32 = 32,         // columns, for head dims 16 / 32 / 64
   EPI_QKV_HN64 = 64,
@@ -66,7 +66,8 @@ struct EpiArgs {
   int64_t img_bstride;
   int img_C, img_H, img_W, img_p, img_f32;
   int act;      // EPI_GATED, EPI_GATED_GRAD: NSW_ACT_*
-  int batch;    // EPI_BATCH: products
+  int batch, ld;  // EPI_BATCH: products, and values between an operand's rows
+  int64_t xs, ws; // EPI_BATCH: values between the products' operands
 };
 
 // GELU with the exact-erf form of nn.GELU(): 0.5 v (1 + erf(v / sqrt 2)).

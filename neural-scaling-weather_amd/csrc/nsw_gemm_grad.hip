@@ -261,8 +261,8 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
 
 }  // namespace
 
-// Parts of the contraction, and the d of one: by estimated time, a stage 0.6 us a round
-// of 256 workgroups, 8 us for a workgroup's start and end, the parts' bytes written and
+// Parts of the contraction, and the d of one: by estimated time, a stage STG us a round
+// of 256 workgroups, FIX us for a workgroup's start and end, the parts' bytes written and
 // read at 4.5 TB/s.
 void grad_split(int64_t R, int64_t C, int64_t D, int64_t ld, int& S, int64_t& per) {
   const int64_t tiles = ((R + GB - 1) / GB) * ((C + GB - 1) / GB), stages = (D + GD - 1) / GD;
@@ -273,8 +273,9 @@ void grad_split(int64_t R, int64_t C, int64_t D, int64_t ld, int& S, int64_t& pe
     // 32-bit offsets inside a part
     if (each * GD * ld * 2 >= (1LL << 31) && s < 64 && s < stages) continue;
     const int64_t parts = (stages + each - 1) / each;
-    double t = (double)((tiles * parts + 255) / 256) * (8 + 0.6 * (double)each);
-    if (parts > 1) t += 5 + (double)(parts * R * C) * 8 / 4.5e6;
+    static const double STG = getenv("NSW_STG") ? atof(getenv("NSW_STG")) : 1.2, FIX = getenv("NSW_FIX") ? atof(getenv("NSW_FIX")) : 5; // EXPERIMENT
+    double t = (double)((tiles * parts + 255) / 256) * (FIX + STG * (double)each);
+    if (parts > 1) t += 3 + (double)(parts * R * C) * 8 / 4.5e6;
     if (S == 0 || t < best) {
       best = t;
       S = (int)parts;

@@ -435,11 +435,11 @@ template <typename T, class TC, bool GATE> struct StageCopy {
   uint32_t v[NC], cx, cw;
   int wave, lane, nk, nst;   // nst: stages; an odd step count leaves half of the last one unused
 
-  __device__ __forceinline__ void init(const char* smem, const T* X, const T* Wt, int M, int N, int K, int m0, int n0,
-                                       int wave_, int lane_) {
+  __device__ __forceinline__ void init(const char* smem, const T* X, const T* Wt, int M, int N, int K, int ld, int m0,
+                                       int n0, int wave_, int lane_) {
     wave = wave_;
     lane = lane_;
-    const uint32_t rowbytes = (uint32_t)K * sizeof(T);
+    const uint32_t rowbytes = (uint32_t)ld * sizeof(T);
     rx = make_rsrc(X, (uint32_t)M * rowbytes);
     rw = make_rsrc(Wt, (uint32_t)N * rowbytes);
 #pragma unroll
@@ -482,7 +482,7 @@ __device__ __forceinline__ void mainloop_ring(char* smem, const bf16* __restrict
   constexpr int NB = TC::NB, MB = TC::MB, NST = TC::NST;
   using Copy = StageCopy<bf16, TC, GATE>;
   Copy cp;
-  cp.init(smem, X, Wt, M, N, K, m0, n0, wave, lane);
+  cp.init(smem, X, Wt, M, N, K, K, m0, n0, wave, lane);
   const int nst = cp.nst;
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s)
@@ -717,7 +717,7 @@ __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, con
   static_assert(TC::NST == 2, "a ring of two slots");
   static_assert(Copy::CX % 2 == 0 && Copy::CW % 2 == 0, "units of 16 rows of one operand");
   Copy cp;
-  cp.init(smem, X, Wt, M, N, K, m0, n0, wave, lane);
+  cp.init(smem, X, Wt, M, N, K, K, m0, n0, wave, lane);
   const int nst = cp.nst;
   const float lo = fmaxf(8.f / (float)K, 0x1p-6f);
   cp.copy(0, 0, 0, NC);
@@ -892,14 +892,14 @@ __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, con
 // MFMAs of (nb, mb 0), x block mb + 1 under those of block mb.
 template <class TC, bool GATE>
 __device__ __forceinline__ void mainloop_split3(char* smem, const float* __restrict__ X, const float* __restrict__ Wt,
-                                                int M, int N, int K, int m0, int n0, f32x4 (&acc)[TC::NB][TC::MB],
-                                                int wave, int lane, int first) {
+                                                int M, int N, int K, int ld, int m0, int n0,
+                                                f32x4 (&acc)[TC::NB][TC::MB], int wave, int lane, int first) {
   constexpr int NB = TC::NB, MB = TC::MB;
   constexpr int BARB = MB > 2 ? MB - 2 : 1;      // row block before which the barrier stands
   using Copy = StageCopy<float, TC, GATE>;
   constexpr int NC = Copy::NC, NC1 = NC / 2;     // copies issued past the barrier / in the next stage
   Copy cp;
-  cp.init(smem, X, Wt, M, N, K, m0, n0, wave, lane);
+  cp.init(smem, X, Wt, M, N, K, ld, m0, n0, wave, lane);
   const int nst = cp.nst;
   if (first >= nst) return;
   cp.copy(first, 0, 0, NC);
@@ -1000,7 +1000,7 @@ __device__ __forceinline__ bool any_nonfinite(const f32x4 (&acc)[TC::NB][TC::MB]
 // loads could not run ahead).  On finite data no wave does.
 template <class TC, bool GATE>
 __device__ __forceinline__ void redo_nonfinite(char* buf, const float* __restrict__ X, const float* __restrict__ Wt, int M,
-                                               int N, int K, int mw0, int nw0, f32x4 (&acc)[TC::NB][TC::MB], int wave,
+                                               int N, int K, int ld, int mw0, int nw0, f32x4 (&acc)[TC::NB][TC::MB], int wave,
                                                int lane) {
   constexpr int NB = TC::NB, MB = TC::MB, G = 4;
   static_assert(TC::NW * G * 1024 <= Stg<float, TC>::SMEM, "LDS layout");
@@ -1021,8 +1021,8 @@ __device__ __forceinline__ void redo_nonfinite(char* buf, const float* __restric
       const int b = __builtin_ctz(left);
       left &= left - 1;
       const int n = w_source_row<GATE>(nw0, b / MB * 16 + frow, N), m = mw0 + b % MB * 16 + frow;
-      const float* wp = Wt + (int64_t)n * K + 4 * fg;
-      const float* xp = X + (int64_t)(m < M ? m : M - 1) * K + 4 * fg;
+      const float* wp = Wt + (int64_t)n * ld + 4 * fg;
+      const float* xp = X + (int64_t)(m < M ? m : M - 1) * ld + 4 * fg;
       f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
       for (int k = 0; k < K; k += 16) {
@@ -1140,10 +1140,11 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   // the tile's rows of x; GATE: addressed from the tile's first one, so that x may
   // be larger than the 32-bit offsets reach
   if constexpr (EPI == EPI_BATCH) {
-    X += (int64_t)blockIdx.y * M * K;
-    Wt += (int64_t)blockIdx.y * N * K;
+    X += (int64_t)blockIdx.y * ea.xs;
+    Wt += (int64_t)blockIdx.y * ea.ws;
     Y += (int64_t)blockIdx.y * M * N;
   }
+  const int ld = EPI == EPI_BATCH ? ea.ld : K;     // values between rows of x and of w
   const T* Xt = GATE ? X + (int64_t)m0 * K : X;
   const int Mt = GATE ? (M - m0 < BM ? M - m0 : BM) : M, mt0 = GATE ? 0 : m0;
 
@@ -1176,8 +1177,8 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
         __shared__ Split2List list;
         stage = mainloop_split2<TC, GATE>(smem, list, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
       }
-      mainloop_split3<TC, GATE>(smem, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0, stage);
-      redo_nonfinite<TC, GATE>(smem, Xt, Wt, Mt, N, K, mt0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
+      mainloop_split3<TC, GATE>(smem, Xt, Wt, Mt, N, K, ld, mt0, n0, acc, wave, lane0, stage);
+      redo_nonfinite<TC, GATE>(smem, Xt, Wt, Mt, N, K, ld, mt0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
     }
   }
   NSW_STAMP(ts[2]);

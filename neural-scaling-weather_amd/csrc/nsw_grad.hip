@@ -13,8 +13,8 @@ namespace nsw {
 int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M,
                int64_t H, int64_t K, int act, int dtype, void* stream, const char* what);
 int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype);
-int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int batch, hipStream_t st,
-                   const char* what);
+int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t ld, int64_t xs, int64_t ws,
+                   int batch, hipStream_t st, const char* what);
 int grad_product(const void* x, const void* w, void* out, int64_t R, int64_t C, int64_t D, int xt, void* ws, hipStream_t st,
                  const char* what);
 int64_t grad_product_workspace(int64_t R, int64_t C, int64_t D, int64_t ld);
@@ -136,17 +136,28 @@ void split_batch(int64_t M, int64_t N, int64_t K, int64_t& S, int64_t& P) {
   S = (M + P - 1) / P;
 }
 
+// fp32: pieces of dx's contraction (N) where its tiles leave compute units idle: equal
+// ones of whole steps (16), at least 64 long.
+int64_t split_contraction(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = ((M + 63) / 64) * ((K + 127) / 128);
+  if (M * N * 4 >= (1LL << 31)) return 1;               // dx's rows go in pieces
+  int64_t S = std::min<int64_t>({768 / tiles, N / 64, 32});
+  while (S > 1 && (N / 16) % S) --S;
+  return std::max<int64_t>(1, S);
+}
+
 // Workspace of the two products and the column sums.
 struct GradSpace {
-  int64_t S = 1, P = 0, wt = 0, dyt = 0, xt = 0, prod = 0, part = 0, bytes = 0;
+  int64_t S = 1, P = 0, Sx = 1, wt = 0, dyt = 0, xt = 0, prod = 0, part = 0, bytes = 0;
   GradSpace(int64_t M, int64_t N, int64_t K, int64_t parts, int dtype) {
     if (dtype == NSW_DTYPE_F32) {
       split_batch(M, N, K, S, P);
+      Sx = split_contraction(M, N, K);
       wt = 0;                                          // w^T
       dyt = wt + align256(N * K * 4);                  // dy^T and x^T in pieces
       xt = dyt + align256(S * N * P * 4);
       prod = xt + align256(S * K * P * 4);             // their products
-      part = prod + (S > 1 ? align256(S * N * K * 4) : 0);
+      part = prod + align256(std::max(S > 1 ? S * N * K * 4 : 0, Sx > 1 ? Sx * M * K * 4 : 0));
     } else {
       const int64_t a = grad_product_workspace(M, K, N, K), b = grad_product_workspace(N, K, M, std::max(N, K));
       part = align256(std::max(a, b));
@@ -167,15 +178,20 @@ int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, voi
   if (dx) {
     if ((rc = transpose(w, ws + sp.wt, N, K, 1, N, st, what))) return rc;
     // as many rows at a time as the GEMM's 2 GiB hold
-    const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4));
+    const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4)), n = N / sp.Sx;
+    char* out = sp.Sx > 1 ? ws + sp.prod : dx;            // Sx > 1 only where M is small: one piece of rows
     for (int64_t m = 0; m < M; m += rows)
-      if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, dx + m * K * 4, std::min(rows, M - m), K, N, 1, st, what))) return rc;
+      if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, out + m * K * 4, std::min(rows, M - m), K, n, N, n, n, (int)sp.Sx,
+                               st, what)))
+        return rc;
+    if (sp.Sx > 1 && (rc = add_parts(out, dx, M * K, (int)sp.Sx, NSW_DTYPE_F32, st, what))) return rc;
   }
   if (dw) {
     if ((rc = transpose(dy, ws + sp.dyt, M, N, sp.S, sp.P, st, what))) return rc;
     if ((rc = transpose(x, ws + sp.xt, M, K, sp.S, sp.P, st, what))) return rc;
     void* out = sp.S > 1 ? ws + sp.prod : dw;
-    if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, (int)sp.S, st, what))) return rc;
+    if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st, what)))
+      return rc;
     if (sp.S > 1) rc = add_parts(out, dw, N * K, (int)sp.S, NSW_DTYPE_F32, st, what);
   }
   return rc;

@@ -26,9 +26,8 @@ int add_parts(const void* part, void* out, int64_t n, int S, int dtype, hipStrea
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
-constexpr int GB = 256;                 // tile rows and columns
-constexpr int GSLOT = 32 * 1024;        // one operand's stage
 constexpr int GD = 64;                  // contraction of a stage
+constexpr int gslot(int gb) { return gb * GD * 2; }   // bytes of one operand's stage, GB x GB tile
 
 struct GradArgs {
   const bf16 *x, *w;
@@ -43,35 +42,36 @@ __device__ __forceinline__ void mfma_b(f32x4& acc, const bf16x8& a, const bf16x8
   acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
 }
 
-// Copies of one operand's stages.  T: as it lies, contraction along the rows: copy j of
-// the wave is stage rows 2 (wave 8 + j) and the next, lane i 16-byte slot i % 32 of the
-// row i / 32.  Not T: 128 bytes of d of 256 rows, as the forward GEMM.  Row d >= D, and
-// what lies past the operand's end, reads as zero (the descriptor's range check); rows r
-// past the edge repeat the last one, columns past the edge are never stored.
-template <bool T> struct OperandCopy {
+// Copies of one operand's stages by four waves, NC of 1 KB each a stage.  T: as it lies,
+// contraction along the rows: a copy is RPC rows of GB columns.  Not T: 128 bytes of d of
+// GB rows, as the forward GEMM.  Row d >= D, and what lies past the operand's end, reads
+// as zero (the descriptor's range check); rows r past the edge repeat the last one,
+// columns past the edge are never stored.
+template <bool T, int GB> struct OperandCopy {
+  static constexpr int NC = gslot(GB) / 4096, RPC = 512 / GB, LPR = 64 / RPC;
+  // T: the swizzle of copy j's rows differs from copy 0's by these bits of f
+  static constexpr int swz(int j) { return GB == 256 ? (j & 1) << 1 | ((j >> 2) & 1) << 2 : ((j >> 1) & 1) << 2; }
+  static constexpr int slot_of(int j) { return GB == 256 ? (j & 1) | (j >> 2) << 1 : (j >> 1) & 1; }
+  static constexpr int NV = T ? (GB == 256 ? 4 : 2) : NC;
   u32x4 rsrc;
-  uint32_t v[T ? 4 : 8];
+  uint32_t v[NV];
   uint32_t ld2;                         // T: bytes of a row
   __device__ __forceinline__ void init(const bf16* p, int64_t ld, int64_t d0, int64_t d1, int c0, int count, int wave,
                                        int lane) {
+    ld2 = (uint32_t)ld * 2u;
     if constexpr (T) {
-      ld2 = (uint32_t)ld * 2u;
       rsrc = make_rsrc(p + d0 * ld + c0, (uint32_t)(((d1 - d0) * ld - c0) * 2));
-      const int kr = wave * 16 + lane / 32, f = (kr & 3) | ((kr >> 3) & 1) << 2;
+      const int kr = wave * (NC * RPC) + lane / LPR, f = (kr & 3) | ((kr >> 3) & 1) << 2;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {     // q = (j & 1) | (j >> 2) << 1
-        const int chunk = (lane % 32) ^ (f << 1) ^ ((q & 1) << 2) ^ ((q >> 1) << 3);
-        v[q] = (uint32_t)kr * ld2 + (uint32_t)chunk * 16u;
-      }
+      for (int j = 0; j < NC; ++j)
+        v[slot_of(j)] = (uint32_t)kr * ld2 + (uint32_t)((lane % LPR) ^ ((f ^ swz(j)) << 1)) * 16u;
     } else {
-      const uint32_t rb = (uint32_t)ld * 2u;
       const int rows = count - c0 < GB ? count - c0 : GB;
       rsrc = make_rsrc(p + (int64_t)c0 * ld + d0, (uint32_t)(((int64_t)rows * ld - d0) * 2));
-      ld2 = rb;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = wave * 64 + j * 8 + lane / 8;
-        v[j] = (uint32_t)(r < rows ? r : rows - 1) * rb + (uint32_t)((lane % 8) ^ row_swizzle(r)) * 16u;
+      for (int j = 0; j < NC; ++j) {
+        const int r = (wave * NC + j) * 8 + lane / 8;
+        v[j] = (uint32_t)(r < rows ? r : rows - 1) * ld2 + (uint32_t)((lane % 8) ^ row_swizzle(r)) * 16u;
       }
     }
   }
@@ -79,7 +79,7 @@ template <bool T> struct OperandCopy {
   // stage's start, always below the descriptor's size: the range check subtracts it
   __device__ __forceinline__ void copy(uint32_t lds, int st, int j) const {
     if constexpr (T)
-      dma16(rsrc, lds + j * 1024, v[(j & 1) | (j >> 2) << 1] + (uint32_t)(2 * j) * ld2, (uint32_t)st * GD * ld2);
+      dma16(rsrc, lds + j * 1024, v[slot_of(j)] + (uint32_t)(RPC * j) * ld2, (uint32_t)st * GD * ld2);
     else
       dma16(rsrc, lds + j * 1024, v[j], (uint32_t)st * (GD * 2));
   }
@@ -87,25 +87,25 @@ template <bool T> struct OperandCopy {
 
 // Fragments of 16 rows (columns).  `at` is the lane's offset in a slot for the wave's
 // first unit; unit n after it is at ^ (n << 5) (T: the unit's bits hold the swizzle) or
-// n 2 KB further, the stage's second half of d 16 KB further or, not T, at chunk ^ 4.
-template <bool T>
+// n 2 KB further, the stage's second half of d 32 rows further or, not T, at chunk ^ 4.
+template <bool T, int GB>
 __device__ __forceinline__ uint32_t frag_at(int unit, int lane) {
   const int i = lane & 15, fg = lane >> 4;
   if constexpr (T) {
     const int f = (i >> 2) | (fg & 1) << 2;
-    return (uint32_t)((fg * 8 + (i >> 2)) * 512 + ((unit ^ f) << 5) + (i & 3) * 8);
+    return (uint32_t)((fg * 8 + (i >> 2)) * (GB * 2) + ((unit ^ f) << 5) + (i & 3) * 8);
   } else {
     return (uint32_t)((unit * 16 + i) * ROWB + (fg ^ row_swizzle(i)) * 16);
   }
 }
-template <bool T>
+template <bool T, int GB>
 __device__ __forceinline__ bf16x8 grad_frag(const char* slot, uint32_t at, int n, int sub) {
   if constexpr (T) {
     typedef __attribute__((address_space(3))) s16x4* lds_ptr;
     typedef __attribute__((address_space(3))) char* lds_char;
-    const lds_char p = (lds_char)slot + (at ^ (uint32_t)(n << 5)) + sub * (32 * 512);
+    const lds_char p = (lds_char)slot + (at ^ (uint32_t)(n << 5)) + sub * (32 * GB * 2);
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * 512));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * GB * 2));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   } else {
     return *reinterpret_cast<const bf16x8*>(slot + (at ^ (sub ? 64u : 0u)) + n * (16 * ROWB));
@@ -116,9 +116,9 @@ __device__ __forceinline__ bf16x8 grad_frag(const char* slot, uint32_t at, int n
 template <bool XT, bool COPY>
 __device__ __forceinline__ void grad_loop(char* smem, const GradArgs& a, int r0, int c0, int64_t d0, int64_t d1,
                                           f32x4 (&acc)[4][8], int wave, int lane) {
-  constexpr int NC = 8, CPG = 4, UNR = 12;
-  OperandCopy<XT> cx;
-  OperandCopy<true> cw;
+  constexpr int GB = 256, GSLOT = gslot(GB), NC = OperandCopy<XT, GB>::NC, CPG = NC / 2, UNR = 12;
+  OperandCopy<XT, GB> cx;
+  OperandCopy<true, GB> cw;
   if constexpr (COPY) {
     cx.init(a.x, a.ldx, d0, d1, r0, a.R, wave, lane);
     cw.init(a.w, a.ldw, d0, d1, c0, a.C, wave, lane);
@@ -143,12 +143,12 @@ __device__ __forceinline__ void grad_loop(char* smem, const GradArgs& a, int r0,
     }
   }
   wg_barrier();
-  uint32_t ax = frag_at<XT>((wave / 4) * 8, lane), aw = frag_at<true>((wave % 4) * 4, lane);
+  uint32_t ax = frag_at<XT, GB>((wave / 4) * 8, lane), aw = frag_at<true, GB>((wave % 4) * 4, lane);
   bf16x8 fa[2][4], fb[2][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) fa[0][i] = grad_frag<true>(smem + NSW_WS(0), aw, i, 0);
+  for (int i = 0; i < 4; ++i) fa[0][i] = grad_frag<true, GB>(smem + NSW_WS(0), aw, i, 0);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) fb[0][i] = grad_frag<XT>(smem + NSW_XS(0), ax, i, 0);
+  for (int i = 0; i < 8; ++i) fb[0][i] = grad_frag<XT, GB>(smem + NSW_XS(0), ax, i, 0);
 #define NSW_GSTEP(U)                                                                                   \
   {                                                                                                    \
     const int k = kt + U;                                                                              \
@@ -175,9 +175,9 @@ __device__ __forceinline__ void grad_loop(char* smem, const GradArgs& a, int r0,
           }                                                                                            \
         }                                                                                              \
         _Pragma("unroll") for (int q = 0; q < 2; ++q)                                                  \
-          fb[((U) + 1) & 1][nb * 2 + q] = grad_frag<XT>(smem + NSW_XS(nsu_), ax, nb * 2 + q, nsub_);        \
+          fb[((U) + 1) & 1][nb * 2 + q] = grad_frag<XT, GB>(smem + NSW_XS(nsu_), ax, nb * 2 + q, nsub_);        \
         _Pragma("unroll") for (int mb = 0; mb < 8; ++mb) mfma_b(acc[nb][mb], fa[(U) & 1][nb], fb[(U) & 1][mb]); \
-        fa[((U) + 1) & 1][nb] = grad_frag<true>(smem + NSW_WS(nsu_), aw, nb, nsub_);                   \
+        fa[((U) + 1) & 1][nb] = grad_frag<true, GB>(smem + NSW_WS(nsu_), aw, nb, nsub_);                   \
         if constexpr (XT) {                                                                            \
           _Pragma("unroll") for (int q = 0; q < 4; ++q) {                                              \
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                         \
@@ -205,37 +205,17 @@ __device__ __forceinline__ void grad_loop(char* smem, const GradArgs& a, int r0,
 #undef NSW_WS
 }
 
-// XT: X's contraction runs along its rows; OT: bf16 (S = 1) or the fp32 parts.
-template <bool XT, typename OT>
-__global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
-  __shared__ __attribute__((aligned(1024))) char smem[5 * GSLOT];
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-  // part-major, inside a part groups of GROUP_M row blocks x all column blocks as the
-  // forward GEMM: the tiles of one XCD walk the same d range over shared panels
-  const int MT = (a.R + GB - 1) / GB, NT = (a.C + GB - 1) / GB;
-  const int id = xcd_remap(blockIdx.x, MT * NT * a.S);
-  const int part = id / (MT * NT), tile = id - part * (MT * NT);
-  const int gm0 = tile / (GROUP_M * NT) * GROUP_M, gsz = MT - gm0 < GROUP_M ? MT - gm0 : GROUP_M, tin = tile - gm0 * NT;
-  const int r0 = (gm0 + tin % gsz) * GB, c0 = tin / gsz * GB;
-  const int64_t d0 = part * a.per, d1 = d0 + a.per < a.D ? d0 + a.per : a.D;
-  f32x4 acc[4][8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (wave < 4) grad_loop<XT, true>(smem, a, r0, c0, d0, d1, acc, wave, lane);
-  else grad_loop<XT, false>(smem, a, r0, c0, d0, d1, acc, wave, lane);
-  NSW_WAIT_VMCNT(0);       // the copies past the last stage
-  wg_barrier();            // the ring is no longer read
-  // lane (frow, fg) of block (nb, mb) holds out[mb 16 + frow][nb 16 + 4 fg + r]: 32 rows
-  // at a time through an LDS part of the wave's own, out in whole 64-column rows
+// A wave's results out: lane (frow, fg) of block (nb, mb) holds out[mb 16 + frow][nb 16 + 4
+// fg + r]; 32 rows at a time through an LDS part of the wave's own, in whole 64-column rows.
+template <typename OT, int MB>
+__device__ __forceinline__ void grad_write_out(char* smem, const f32x4 (&acc)[4][MB], const GradArgs& a, int part, int rw,
+                                               int cw0, int wave, int lane) {
   constexpr int STRIDE = 64 * (int)sizeof(OT) + 16, VEC = 16 / (int)sizeof(OT), LPR = 64 / VEC, RPI = 64 / LPR;
   char* stg = smem + wave * 32 * STRIDE;
-  const int frow = lane & 15, fg = lane >> 4, crow = lane / LPR, ccol = lane % LPR * VEC;
-  const int rw = r0 + (wave / 4) * 128, cw = c0 + (wave % 4) * 64 + ccol;
+  const int frow = lane & 15, fg = lane >> 4, crow = lane / LPR, ccol = lane % LPR * VEC, cw = cw0 + ccol;
   OT* out = (OT*)a.out + (int64_t)part * a.R * a.C;
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
+  for (int h = 0; h < MB / 2; ++h) {
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -259,36 +239,148 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   }
 }
 
-}  // namespace
-
-// Parts of the contraction, and the d of one: by estimated time, a stage STG us a round
-// of 256 workgroups, FIX us for a workgroup's start and end, the parts' bytes written and
-// read at 4.5 TB/s.
-void grad_split(int64_t R, int64_t C, int64_t D, int64_t ld, int& S, int64_t& per) {
-  const int64_t tiles = ((R + GB - 1) / GB) * ((C + GB - 1) / GB), stages = (D + GD - 1) / GD;
-  double best = 0;
-  S = 0;
-  for (int64_t s = 1; s <= 64 && s <= stages; ++s) {
-    const int64_t each = (stages + s - 1) / s;
-    // 32-bit offsets inside a part
-    if (each * GD * ld * 2 >= (1LL << 31) && s < 64 && s < stages) continue;
-    const int64_t parts = (stages + each - 1) / each;
-    static const double STG = getenv("NSW_STG") ? atof(getenv("NSW_STG")) : 1.2, FIX = getenv("NSW_FIX") ? atof(getenv("NSW_FIX")) : 5; // EXPERIMENT
-    double t = (double)((tiles * parts + 255) / 256) * (FIX + STG * (double)each);
-    if (parts > 1) t += 3 + (double)(parts * R * C) * 8 / 4.5e6;
-    if (S == 0 || t < best) {
-      best = t;
-      S = (int)parts;
-      per = each * GD;
-    }
-  }
+// XT: X's contraction runs along its rows; OT: bf16 (S = 1) or the fp32 parts.
+template <bool XT, typename OT>
+__global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
+  constexpr int GB = 256;
+  __shared__ __attribute__((aligned(1024))) char smem[5 * gslot(GB)];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  // part-major, inside a part groups of GROUP_M row blocks x all column blocks as the
+  // forward GEMM: the tiles of one XCD walk the same d range over shared panels
+  const int MT = (a.R + GB - 1) / GB, NT = (a.C + GB - 1) / GB;
+  const int id = xcd_remap(blockIdx.x, MT * NT * a.S);
+  const int part = id / (MT * NT), tile = id - part * (MT * NT);
+  const int gm0 = tile / (GROUP_M * NT) * GROUP_M, gsz = MT - gm0 < GROUP_M ? MT - gm0 : GROUP_M, tin = tile - gm0 * NT;
+  const int r0 = (gm0 + tin % gsz) * GB, c0 = tin / gsz * GB;
+  const int64_t d0 = part * a.per, d1 = d0 + a.per < a.D ? d0 + a.per : a.D;
+  f32x4 acc[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (wave < 4) grad_loop<XT, true>(smem, a, r0, c0, d0, d1, acc, wave, lane);
+  else grad_loop<XT, false>(smem, a, r0, c0, d0, d1, acc, wave, lane);
+  NSW_WAIT_VMCNT(0);       // the copies past the last stage
+  wg_barrier();            // the ring is no longer read
+  grad_write_out<OT, 8>(smem, acc, a, part, r0 + (wave / 4) * 128, c0 + (wave % 4) * 64, wave, lane);
 }
 
+// 128 x 128 results, four waves of 64 x 64, two workgroups a CU: where 256 x 256 leaves
+// compute units idle.  A ring of two stages, one barrier a stage (mainloop_ring of the
+// forward GEMM).
+template <bool XT, typename OT>
+__global__ __launch_bounds__(256, 2) void grad_small_kernel(GradArgs a) {
+  constexpr int GB = 128, GSLOT = gslot(GB);
+  using CX = OperandCopy<XT, GB>;
+  using CW = OperandCopy<true, GB>;
+  constexpr int NC = CX::NC;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * GSLOT];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  constexpr int GM = GROUP_M * 2;                           // tile order as grad_kernel
+  const int MT = (a.R + GB - 1) / GB, NT = (a.C + GB - 1) / GB;
+  const int id = xcd_remap(blockIdx.x, MT * NT * a.S);
+  const int part = id / (MT * NT), tile = id - part * (MT * NT);
+  const int gm0 = tile / (GM * NT) * GM, gsz = MT - gm0 < GM ? MT - gm0 : GM, tin = tile - gm0 * NT;
+  const int r0 = (gm0 + tin % gsz) * GB, c0 = tin / gsz * GB;
+  const int64_t d0 = part * a.per, d1 = d0 + a.per < a.D ? d0 + a.per : a.D;
+  CX cx;
+  CW cw;
+  cx.init(a.x, a.ldx, d0, d1, r0, a.R, wave, lane);
+  cw.init(a.w, a.ldw, d0, d1, c0, a.C, wave, lane);
+  const uint32_t base = (uint32_t)(uintptr_t)smem + wave * (NC * 1024);
+  const int nk = (int)((d1 - d0 + 31) / 32), nst = (nk + 1) / 2;
+  // slot s: x at 2 s GSLOT, w behind it
+  auto copy = [&](int st, int slot) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) cx.copy(base + 2 * slot * GSLOT, st, j);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) cw.copy(base + (2 * slot + 1) * GSLOT, st, j);
+  };
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t ax = frag_at<XT, GB>((wave / 2) * 4, lane), aw = frag_at<true, GB>((wave % 2) * 4, lane);
+  copy(0, 0);
+  for (int st = 0; st < nst; ++st) {
+    wait_copies();
+    wg_barrier();          // stage st has landed, and no wave reads stage st - 1 any more
+    const int slot = st & 1;
+    if (st + 1 < nst) copy(st + 1, slot ^ 1);
+    const char* xs = smem + 2 * slot * GSLOT;
+    const char* ws = xs + GSLOT;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      if (sub == 1 && 2 * st + 1 >= nk) break;              // the unused half of the last stage
+      bf16x8 fa[4];
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) fa[nb] = grad_frag<true, GB>(ws, aw, nb, sub);
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        const bf16x8 fb = grad_frag<XT, GB>(xs, ax, mb, sub);
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) mfma_b(acc[nb][mb], fa[nb], fb);
+      }
+    }
+  }
+  wg_barrier();            // the ring is no longer read
+  grad_write_out<OT, 4>(smem, acc, a, part, r0 + (wave / 2) * 64, c0 + (wave % 2) * 64, wave, lane);
+}
+
+}  // namespace
+
+namespace {
+
+// Tile (256 or 128), parts of the contraction and the d of one, by estimated time: a round
+// of workgroups costs fa + fb us a stage with every slot taken, pa + pb while at most the
+// share f0 of the slots is (between them linear); parts are written and read at 4.5 TB/s
+// and a launch more.  Measured, us, 256 x 256 / 128 x 128 with the parts each is best at:
+//   dx = dy [M, N] . w [N, K]   M 500, N 1024, K 256: 12.2 / 8.2     12961, 2720, 512: 49 / 43
+//                               64800, 1024, 1024: 114 / 138         64800, 8192, 1024: 772 / 1091 (1.4 PFLOP/s)
+//   dw = dy^T . x               M 500, N 1024, K 256: 12.5 / 7.3     2000, 8192, 1024: 40 / 34
+//                               64800, 1024, 1024: 118 / 150         64800, 8192, 1024: 758 / 1148
+struct GradCost {
+  int gb, slots;
+  double fa, fb, pa, pb, f0;
+  double us(double wgs, double stages) const {
+    const double t = wgs / slots, r = (double)(int64_t)t, f = t - r, full = fa + fb * stages, part = pa + pb * stages;
+    return r * full + (f > 0 ? part + std::max(0.0, f - f0) / (1 - f0) * (full - part) : 0);
+  }
+};
+struct GradPlan {
+  int gb = 256, S = 0;
+  int64_t per = 0;
+};
+GradPlan grad_plan(int64_t R, int64_t C, int64_t D, int64_t ld) {
+  constexpr GradCost big{256, 256, 8.5, 1.4, 5.5, 0.96, 0}, small{128, 512, 4.5, 0.97, 3.6, 0.56, 0.4};
+  const int64_t stages = (D + GD - 1) / GD;
+  GradPlan p;
+  double best = 0;
+  for (const GradCost& c : {big, small}) {
+    const int64_t tiles = ((R + c.gb - 1) / c.gb) * ((C + c.gb - 1) / c.gb);
+    for (int64_t s = 1; s <= 64 && s <= stages; ++s) {
+      const int64_t each = (stages + s - 1) / s, parts = (stages + each - 1) / each;
+      // 32-bit offsets inside a part (at the most parts there are, the caller refuses)
+      if (each * GD * ld * 2 >= (1LL << 31) && s < 64 && s < stages) continue;
+      double t = c.us((double)(tiles * parts), (double)each);
+      if (parts > 1) t += 3 + (double)(parts * R * C) * 8 / 4.5e6;
+      if (p.S == 0 || t < best) {
+        best = t;
+        p.gb = c.gb;
+        p.S = (int)parts;
+        p.per = each * GD;
+      }
+    }
+  }
+  return p;
+}
+
+}  // namespace
+
 int64_t grad_product_workspace(int64_t R, int64_t C, int64_t D, int64_t ld) {
-  int S;
-  int64_t per;
-  grad_split(R, C, D, ld, S, per);
-  return S > 1 ? (int64_t)S * R * C * 4 : 0;
+  const GradPlan p = grad_plan(R, C, D, ld);
+  return p.S > 1 ? (int64_t)p.S * R * C * 4 : 0;
 }
 
 // out [R, C] = X . W, X [R, D] (xt 0) or [D, R] (xt 1), W [D, C].
@@ -299,22 +391,22 @@ int grad_product(const void* x, const void* w, void* out, int64_t R, int64_t C, 
   a.ldx = xt ? R : D; a.ldw = C;
   a.R = (int)R; a.C = (int)C; a.D = D;
   const int64_t ld = std::max<int64_t>(C, xt ? R : 0);
-  grad_split(R, C, D, ld, a.S, a.per);
-  NSW_CHECK_ARG(a.per * ld * 2 < (1LL << 31) && (xt || GB * D * 2 < (1LL << 31)), "%s: rows too long (32-bit offsets)", what);
-  const int64_t grid = ((R + GB - 1) / GB) * ((C + GB - 1) / GB) * a.S;
+  const GradPlan p = grad_plan(R, C, D, ld);
+  a.S = p.S; a.per = p.per;
+  NSW_CHECK_ARG(a.per * ld * 2 < (1LL << 31) && (xt || p.gb * D * 2 < (1LL << 31)), "%s: rows too long (32-bit offsets)", what);
+  const int64_t grid = ((R + p.gb - 1) / p.gb) * ((C + p.gb - 1) / p.gb) * a.S;
   NSW_CHECK_ARG(grid < (1LL << 31), "%s: too many tiles", what);
   a.out = a.S > 1 ? ws : out;
-  const dim3 g((unsigned)grid), b(512);
-  if (a.S > 1) {
-    if (xt) hipLaunchKernelGGL((grad_kernel<true, float>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((grad_kernel<false, float>), g, b, 0, st, a);
-    if (int rc = check_launch(what)) return rc;
-    return add_parts(ws, out, R * C, a.S, NSW_DTYPE_BF16, st, what);
-  } else {
-    if (xt) hipLaunchKernelGGL((grad_kernel<true, bf16>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((grad_kernel<false, bf16>), g, b, 0, st, a);
-  }
-  return check_launch(what);
+  auto go = [&](auto big, auto small) {
+    if (p.gb == 256) hipLaunchKernelGGL(big, dim3((unsigned)grid), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL(small, dim3((unsigned)grid), dim3(256), 0, st, a);
+  };
+  if (a.S > 1 && xt) go(grad_kernel<true, float>, grad_small_kernel<true, float>);
+  else if (a.S > 1) go(grad_kernel<false, float>, grad_small_kernel<false, float>);
+  else if (xt) go(grad_kernel<true, bf16>, grad_small_kernel<true, bf16>);
+  else go(grad_kernel<false, bf16>, grad_small_kernel<false, bf16>);
+  if (int rc = check_launch(what)) return rc;
+  return a.S > 1 ? add_parts(ws, out, R * C, a.S, NSW_DTYPE_BF16, st, what) : NSW_OK;
 }
 
 }  // namespace nsw

@@ -189,6 +189,22 @@ def rmsnorm_roll_partition(x: torch.Tensor, weight: torch.Tensor, window_size, s
     return out
 
 
+def _uniform(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The device of ts (the first is given) after the checks of _dev and
+    _same_dtype, which raise what is found."""
+    ref = ts[0]
+    dev, dt = ref.device, ref.dtype
+    for t in ts:
+        if t is not None and (t.dtype != dt or t.device != dev or not t.is_contiguous()):
+            break
+    else:
+        if ref.is_cuda:
+            return dev
+    _dev(*ts)
+    _same_dtype(ref, *ts)
+    return dev
+
+
 def _run(what: str, dev: torch.device, fn, *args) -> None:
     """fn(*args, stream) with dev as the current device, its error raised."""
     if torch.cuda.current_device() == dev.index:
@@ -202,17 +218,18 @@ def _run(what: str, dev: torch.device, fn, *args) -> None:
 
 def _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps):
     """(device, rows, C, G, eps) of a residual_norm, its arguments checked."""
-    dev = _dev(branch, skip, post_weight, gate, norm_weight)
-    _same_dtype(branch, skip, post_weight, gate, norm_weight)
-    if branch.dim() < 1 or branch.shape != skip.shape:
+    dev = _uniform(branch, skip, post_weight, gate, norm_weight)
+    shape = branch.shape
+    if not shape or shape != skip.shape:
         raise ValueError(f"{what}: branch {tuple(branch.shape)} and skip {tuple(skip.shape)} must have one shape")
-    C = branch.shape[-1]
+    C = shape[-1]
     if C == 0:
         raise ValueError(f"{what}: no features")
     rows = branch.numel() // C
-    for name, t in (("post_weight", post_weight), ("norm_weight", norm_weight)):
-        if t is not None and tuple(t.shape) != (C,):
-            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({C},)")
+    if post_weight is not None and post_weight.shape != (C,):
+        raise ValueError(f"{what}: post_weight has shape {tuple(post_weight.shape)}, expected ({C},)")
+    if norm_weight is not None and norm_weight.shape != (C,):
+        raise ValueError(f"{what}: norm_weight has shape {tuple(norm_weight.shape)}, expected ({C},)")
     G = 1
     if gate is not None:
         if gate.dim() not in (1, 2) or gate.shape[-1] != C or gate.numel() == 0:
@@ -311,16 +328,16 @@ _ACTS = {"silu": _lib.NSW_ACT_SILU, "gelu": _lib.NSW_ACT_GELU, "gelu_tanh": _lib
 
 def _gated_args(what, x, weight, bias, act):
     """(device, M, H, K, act code) of a gated linear, its arguments checked."""
-    dev = _dev(x, weight, bias)
-    _same_dtype(x, weight, bias)
+    dev = _uniform(x, weight, bias)
     if act not in _ACTS:
         raise ValueError(f"{what}: act must be one of {sorted(_ACTS)}, got {act!r}")
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] % 2:
+    shape, wshape = x.shape, weight.shape
+    if not shape or len(wshape) != 2 or wshape[1] != shape[-1] or wshape[0] % 2:
         raise ValueError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)}, expected [..., K] and [2H, K]")
-    K, H = x.shape[-1], weight.shape[0] // 2
+    K, H = wshape[1], wshape[0] // 2
     if K == 0 or H == 0:
         raise ValueError(f"{what}: no features")
-    if bias is not None and tuple(bias.shape) != (2 * H,):
+    if bias is not None and bias.shape != (2 * H,):
         raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({2 * H},)")
     return dev, x.numel() // K, H, K, _ACTS[act]
 
@@ -332,7 +349,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     weight [2H, K] stacks Wg over Wu, bias [2H] bg over bu; act "silu",
     "gelu" (exact erf) or "gelu_tanh"."""
     dev, M, H, K, code = _gated_args("gated_linear", x, weight, bias, act)
-    h = torch.empty(x.shape[:-1] + (H,), dtype=x.dtype, device=dev)
+    h = x.new_empty(x.shape[:-1] + (H,))
     if M == 0:
         return h
     _run("gated_linear", dev, lib().nsw_gated_linear, x.data_ptr(), weight.data_ptr(), _p(bias), h.data_ptr(), M, H, K,
@@ -410,9 +427,9 @@ def quantize_fp8(x: torch.Tensor, rows: int = 1) -> Tuple[torch.Tensor, torch.Te
     Kb = (K + FP8_BLOCK - 1) // FP8_BLOCK
     R = x.numel() // K
     code = dtype_code(x)
-    q = torch.empty(x.shape[:-1] + (Kb * FP8_BLOCK,), dtype=torch.float8_e4m3fn, device=dev)
-    lead = x.shape[:-1] if rows == 1 else ((R + rows - 1) // rows,)
-    scale = torch.empty(tuple(lead) + (Kb,), dtype=torch.float8_e8m0fnu, device=dev)
+    lead = x.shape[:-1]
+    q = x.new_empty(lead + (Kb * FP8_BLOCK,), dtype=torch.float8_e4m3fn)
+    scale = x.new_empty((lead if rows == 1 else ((R + rows - 1) // rows,)) + (Kb,), dtype=torch.float8_e8m0fnu)
     if R:
         _run("quantize_fp8", dev, lib().nsw_quantize_fp8, x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, rows, code)
     return q, scale
@@ -428,27 +445,28 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     dev = _dev(xq, x_scale, wq, w_scale, bias, residual)
     if dtype not in _DTYPES:
         raise TypeError(f"{what}: the result is float32 or bfloat16, got {dtype}")
-    for t, want in ((xq, torch.float8_e4m3fn), (wq, torch.float8_e4m3fn), (x_scale, torch.float8_e8m0fnu),
-                    (w_scale, torch.float8_e8m0fnu)):
-        if t.dtype != want:
-            raise TypeError(f"{what}: expected {want}, got {t.dtype}")
-    if xq.dim() < 1 or wq.dim() != 2 or wq.shape[1] != xq.shape[-1] or xq.shape[-1] % FP8_BLOCK or xq.shape[-1] == 0:
+    if (xq.dtype != torch.float8_e4m3fn or wq.dtype != torch.float8_e4m3fn or x_scale.dtype != torch.float8_e8m0fnu
+            or w_scale.dtype != torch.float8_e8m0fnu):
+        raise TypeError(f"{what}: expected float8_e4m3fn values and float8_e8m0fnu scales, got "
+                        f"{xq.dtype}, {x_scale.dtype}, {wq.dtype}, {w_scale.dtype}")
+    shape, wshape = xq.shape, wq.shape
+    if not shape or len(wshape) != 2 or wshape[1] != shape[-1] or wshape[1] % FP8_BLOCK or wshape[1] == 0:
         raise ValueError(f"{what}: xq {tuple(xq.shape)} and wq {tuple(wq.shape)}, expected [..., K] and [N, K] with K a "
                          f"multiple of {FP8_BLOCK}")
-    N, K = wq.shape
+    N, K = wshape
     Kb = K // FP8_BLOCK
-    if x_scale.shape != xq.shape[:-1] + (Kb,) or tuple(w_scale.shape) != ((N + FP8_BLOCK - 1) // FP8_BLOCK, Kb):
+    if x_scale.shape != shape[:-1] + (Kb,) or w_scale.shape != ((N + FP8_BLOCK - 1) // FP8_BLOCK, Kb):
         raise ValueError(f"{what}: scales {tuple(x_scale.shape)} and {tuple(w_scale.shape)} do not match "
                          f"{tuple(xq.shape)} and {tuple(wq.shape)}")
     for t in (bias, residual):
         if t is not None and t.dtype != dtype:
             raise TypeError(f"dtype mismatch: {t.dtype} vs {dtype}")
-    if bias is not None and tuple(bias.shape) != (N,):
+    if bias is not None and bias.shape != (N,):
         raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({N},)")
     if epilogue is None:
         epilogue = _lib.NSW_EPI_NONE if bias is None else (
             _lib.NSW_EPI_BIAS if residual is None else _lib.NSW_EPI_BIAS_RESIDUAL)
-    y = torch.empty(xq.shape[:-1] + (N,), dtype=dtype, device=dev)
+    y = xq.new_empty(shape[:-1] + (N,), dtype=dtype)
     if residual is not None and residual.shape != y.shape:
         raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")
     if y.numel():

@@ -155,7 +155,7 @@ int nsw_gated_linear(const void* x, const void* w, const void* bias, void* h, in
 /* Gradients of nsw_gated_linear from that of h [M, H]: where not NULL dx
  * [M, K], dw [2H, K] and db [2H].  The two projections are formed again from
  * x and w, so nothing but the inputs is kept from the forward pass.  Sums over
- * rows in a fixed order.  Workspace (16-byte aligned) of
+ * rows in a fixed order.  Results must not overlap the inputs.  Workspace (16-byte aligned) of
  * nsw_gated_linear_backward_workspace_size bytes, 0 for sizes that are
  * refused. */
 size_t nsw_gated_linear_backward_workspace_size(int64_t M, int64_t H, int64_t K, int dtype);
@@ -457,7 +457,7 @@ int nsw_skip_conv_accumulate(const void* x, const void* inv, const float* w, voi
  *   y = alpha * skip + gate * n                        (gate NULL: 1)
  *   z = y / sqrt(mean(y^2) + eps) * norm_w             (norm_w and z NULL: no z)
  * branch, skip, y, z [rows, C]; post_w, norm_w [C]; gate [G, C], row r taking
- * gate row r / (rows / G) (G = 1: one gate for all rows).  All of one dtype,
+ * gate row r / (rows / G) (G = 1: one gate for all rows; at most 65536).  All of one dtype,
  * 16-byte aligned; C a multiple of 8 (bf16) / 4 (fp32), at most 8192 / 4096.
  * Outputs must not overlap inputs. */
 int nsw_residual_norm(const void* branch, const void* skip, const void* post_w, const void* gate,

@@ -176,6 +176,11 @@ __device__ __forceinline__ void widen32(const i32x8& f, bf16x8 (&o)[4]) {
     }
 }
 
+// v under the E8M0 scales a and b (255 is NaN, as for the scaled instructions).
+__device__ __forceinline__ float scaled(float v, int a, int b) {
+  return a == 255 || b == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(v, a + b - 254);
+}
+
 // Between a wave's LDS writes and its reads of what other lanes wrote (LDS accesses
 // of a wave are served in order; only the compiler has to keep them so).
 __device__ __forceinline__ void wave_fence() {
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Ar
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            acc[nb][mb][e] += __builtin_amdgcn_ldexpf(part[nb][mb][e], sw + sx[mb] - 254);
+            acc[nb][mb][e] += scaled(part[nb][mb][e], sw, sx[mb]);
     } else
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -620,7 +625,7 @@ __global__ __launch_bounds__(512) void linear_fp8_rows_kernel(Fp8Args a) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w4[q], x4[q], part, 0, 0, 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[mb][e] += __builtin_amdgcn_ldexpf(part[e], sw[u] + sx[u][mb] - 254);
+          for (int e = 0; e < 4; ++e) acc[mb][e] += scaled(part[e], sw[u], sx[u][mb]);
         }
       }
     }

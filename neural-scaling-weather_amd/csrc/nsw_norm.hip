@@ -372,12 +372,17 @@ __global__ __launch_bounds__(NT) void residual_norm_backward_kernel(NormArgs a) 
 
 // dgate, dpost_w and dnorm_w from the workgroups' partial rows [G P][2][C], 16
 // columns to a workgroup: 4 lanes hold 4 columns each, 64 groups of them take every
-// 64th partial row and meet in LDS, always in the same order.
+// 64th partial row and meet in LDS, always in the same order.  Many samples are split
+// over gridDim.y workgroups, which leave their sums in over [gridDim.y][2][C] for
+// residual_norm_split_kernel.
 template <typename T>
 __global__ __launch_bounds__(NT) void residual_norm_params_kernel(const float* __restrict__ part, int G, int P, int C,
                                                                   const T* __restrict__ post_w, const T* __restrict__ gate,
                                                                   T* __restrict__ dpost, T* __restrict__ dgate,
-                                                                  T* __restrict__ dnorm) {
+                                                                  T* __restrict__ dnorm, float* __restrict__ over) {
+  const int per = (G + (int)gridDim.y - 1) / (int)gridDim.y, g0 = (int)blockIdx.y * per, g1 = g0 + per < G ? g0 + per : G;
+  const bool split = gridDim.y > 1;
+  float* mine = over + (int64_t)blockIdx.y * 2 * C;
   constexpr int NG = NT / 4;
   __shared__ __attribute__((aligned(16))) float red[NG][20];
   const int cl = ((int)threadIdx.x & 3) * 4, grp = (int)threadIdx.x >> 2;
@@ -411,7 +416,7 @@ __global__ __launch_bounds__(NT) void residual_norm_params_kernel(const float* _
   if (dpost != nullptr || dgate != nullptr) {
     float w[4] = {1.f, 1.f, 1.f, 1.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
     if (post_w != nullptr && in) load4<T>(post_w + c, w);
-    for (int g = 0; g < G; ++g) {
+    for (int g = g0; g < g1; ++g) {
       const f32x4 s = sum((int64_t)g * P, (int64_t)(g + 1) * P, 0);
       if (!out) continue;
       float gt[4] = {1.f, 1.f, 1.f, 1.f}, dg[4];
@@ -423,14 +428,39 @@ __global__ __launch_bounds__(NT) void residual_norm_params_kernel(const float* _
       }
       if (dgate != nullptr) store4<T>(dgate + (int64_t)g * C + c, dg);
     }
-    if (dpost != nullptr && out) store4<T>(dpost + c, dp);
+    if (dpost != nullptr && out) {
+      if (split) store4<float>(mine + c, dp);
+      else store4<T>(dpost + c, dp);
+    }
   }
   if (dnorm != nullptr) {
-    const f32x4 q = sum(0, (int64_t)G * P, 1);
+    const f32x4 q = sum((int64_t)g0 * P, (int64_t)(g1 > g0 ? g1 : g0) * P, 1);
     const float v[4] = {q[0], q[1], q[2], q[3]};
-    if (out) store4<T>(dnorm + c, v);
+    if (out) {
+      if (split) store4<float>(mine + C + c, v);
+      else store4<T>(dnorm + c, v);
+    }
   }
 }
+
+// dpost_w and dnorm_w from the Y split sums, in order; a lane 4 columns of one of them.
+template <typename T>
+__global__ __launch_bounds__(NT) void residual_norm_split_kernel(const float* __restrict__ over, int Y, int C,
+                                                                 T* __restrict__ dpost, T* __restrict__ dnorm) {
+  const int i = ((int)blockIdx.x * NT + (int)threadIdx.x) * 4;
+  if (i >= 2 * C) return;
+  T* out = i < C ? dpost : dnorm;
+  if (out == nullptr) return;
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int y = 0; y < Y; ++y) t += *reinterpret_cast<const f32x4*>(over + (int64_t)y * 2 * C + i);
+  const float v[4] = {t[0], t[1], t[2], t[3]};
+  store4<T>(out + (i < C ? i : i - C), v);
+}
+
+// Workgroups that share the samples of the parameters' sums: one for few samples (a
+// second launch costs more than their loop), else four samples each, at most 64.
+inline int sample_split(int64_t G) { return G <= 8 ? 1 : (int)std::min<int64_t>(64, (G + 3) / 4); }
 
 // Workgroups of a sample: enough to fill the chip `per_cu` times over in all, each
 // with at least one turn of rows.
@@ -470,7 +500,7 @@ int check_norm(const char* what, int64_t rows, int64_t C, int64_t G, int dtype, 
   NSW_CHECK_ARG(rows >= 0 && rows < (1LL << 40), "%s: rows=%lld out of range", what, (long long)rows);
   NSW_CHECK_ARG(C > 0 && C % vec == 0 && C <= vec * 1024, "%s: C=%lld must be a multiple of %lld, at most %lld", what,
                 (long long)C, (long long)vec, (long long)(vec * 1024));
-  NSW_CHECK_ARG(G >= 1 && G <= (1 << 20) && rows % G == 0, "%s: rows=%lld must be a multiple of the gate's rows G=%lld",
+  NSW_CHECK_ARG(G >= 1 && G <= 65536 && rows % G == 0, "%s: rows=%lld must be a multiple of the gate's rows G=%lld (at most 65536)",
                 what, (long long)rows, (long long)G);
   NSW_CHECK_ARG(gate != nullptr || G == 1, "%s: G=%lld without a gate", what, (long long)G);
   return NSW_OK;
@@ -511,8 +541,14 @@ int launch_backward(NormArgs a, int64_t rows, int64_t G, void* dpost, void* dgat
     return check_launch(what);
   });
   if (rc || (!dpost && !dgate && !dnorm)) return rc;
-  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 15) / 16)), dim3(NT), 0, st, a.part, (int)G, P,
-                     a.C, (const T*)a.post_w, (const T*)a.gate, (T*)dpost, (T*)dgate, (T*)dnorm);
+  const int Y = sample_split(G);
+  float* over = a.part + std::max<int64_t>((int64_t)P * G, 1) * 2 * a.C;
+  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 15) / 16), (unsigned)Y), dim3(NT), 0, st, a.part,
+                     (int)G, P, a.C, (const T*)a.post_w, (const T*)a.gate, (T*)dpost, (T*)dgate, (T*)dnorm, over);
+  rc = check_launch(what);
+  if (rc || Y == 1 || (!dpost && !dnorm)) return rc;
+  hipLaunchKernelGGL((residual_norm_split_kernel<T>), dim3((unsigned)((2 * a.C / 4 + NT - 1) / NT)), dim3(NT), 0, st, over, Y,
+                     a.C, (T*)dpost, (T*)dnorm);
   return check_launch(what);
 }
 
@@ -546,7 +582,8 @@ extern "C" int nsw_residual_norm(const void* branch, const void* skip, const voi
 extern "C" size_t nsw_residual_norm_backward_workspace_size(int64_t rows, int64_t C, int64_t G, int dtype) {
   if (check_norm("nsw_residual_norm_backward_workspace_size", rows, C, G, dtype, &rows) != NSW_OK) return 0;
   const int64_t n = dtype == NSW_DTYPE_BF16 ? backward_parts<bf16>(rows, C, G) : backward_parts<float>(rows, C, G);
-  return (size_t)(std::max<int64_t>(n, 1) * 2 * C) * sizeof(float);
+  const int64_t Y = sample_split(G);
+  return (size_t)((std::max<int64_t>(n, 1) + (Y > 1 ? Y : 0)) * 2 * C) * sizeof(float);
 }
 
 extern "C" int nsw_residual_norm_backward(const void* dy, const void* dz, const void* branch, const void* skip,

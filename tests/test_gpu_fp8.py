@@ -216,3 +216,27 @@ def test_graph_replays_and_another_stream(device, M):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+def test_rows_past_32_bit_offsets(device):
+    """x of more than 2^32 quantised bytes: the last rows are those of a call on them alone, bit for bit."""
+    from nsw import ops
+    M, K, N = 4_300_003, 1024, 264
+    x = torch.empty(M, K, dtype=BF16, device=device)
+    x.random_(-6, 7)
+    wq = ops.quantize_fp8(data(N, K, BF16, 1, False).to(device), rows=128)
+    y = ops.linear_fp8(*ops.quantize_fp8(x), *wq)
+    tail = ops.linear_fp8(*ops.quantize_fp8(x[-2000:].contiguous()), *wq)
+    v, tol = reference(ops.quantize_fp8(x[-2000:].contiguous()), wq, None, None, 0, BF16)
+    check(y[-2000:], v, tol, BF16)
+    check(tail, v, tol, BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M", [5, 700])
+def test_a_scale_that_is_not_a_number(device, dtype, M):
+    from nsw import ops
+    xq, wq, _, _ = operands(device, M, 136, 256, dtype)
+    xq[1].view(torch.uint8)[3, 1] = 255
+    y = ops.linear_fp8(*xq, *wq, dtype=dtype)
+    assert y[3].isnan().all() and not y[:3].isnan().any() and not y[4:].isnan().any()

@@ -230,3 +230,43 @@ def test_gradients_against_differences(device, act):
 
         want = (grads[n].double() * e).sum().item()
         assert abs((f(h) - f(-h)) / (2 * h) - want) < 2e-2 * max(1.0, abs(want)), n
+
+
+@pytest.mark.parametrize("dtype,M,K", [(BF16, 2_200_003, 512), (F32, 1_100_003, 512)])
+def test_rows_past_32_bit_offsets(device, dtype, M, K):
+    """x of more than 2^31 bytes: the last rows within the bounds, dW and db against float64 sums over all rows."""
+    from nsw import ops
+    H = 16
+    g = torch.Generator(device=device).manual_seed(1)
+    x = torch.empty(M, K, dtype=dtype, device=device).normal_(0, 1, generator=g)
+    t = {k: v for k, v in case(device, dtype, 1, K, H, True, seed=2).items()}
+    dh = torch.empty(M, H, dtype=dtype, device=device).normal_(0, 1, generator=g)
+    h = ops.gated_linear(x, t["w"], t["b"], act="silu")
+    dx, dw, db = ops.gated_linear_backward(dh, x, t["w"], t["b"], act="silu")
+    n = 300
+    tail = {"x": x[-n:].contiguous(), "w": t["w"], "b": t["b"], "dh": dh[-n:].contiguous()}
+    want = reference(tail, "silu")
+    check({"h": h[-n:], "dx": dx[-n:]}, {k: want[k] for k in ("h", "dx")}, dtype)
+    r, dw64, db64 = torch.finfo(dtype).eps / 2, 0, 0
+    for m in range(0, M, 100_000):                   # dg and du are rounded once, sums of random signs: r by chance
+        p = x[m:m + 100_000].double() @ t["w"].double().t() + t["b"].double()
+        a, d = act64(p[:, :H], "silu")
+        d64 = dh[m:m + 100_000].double()
+        dp = torch.cat([d64 * p[:, H:] * d, d64 * a], 1)
+        dw64, db64 = dw64 + dp.t() @ x[m:m + 100_000].double(), db64 + dp.sum(0)
+    for got, ref in ((dw, dw64), (db, db64)):
+        assert (got.double() - ref).norm() <= (3 * r + 2e-5) * ref.norm()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(40, 1600, 320), (9, 640, 928), (700, 1600, 320), (1000, 96, 4096), (130, 4096, 64)])
+def test_split_contractions(device, dtype, M, N, K):
+    """Few results and long sums, either way: pieces that are added afterwards."""
+    from nsw import ops
+    g = torch.Generator().manual_seed(M)
+    dy, x = (torch.randn(M, n, generator=g).to(device, dtype) for n in (N, K))
+    w = (torch.randn(N, K, generator=g) * K ** -0.5).to(device, dtype)
+    dx, dw, _ = ops.linear_backward(dy, x, w, needs=(True, True, False))
+    d, xx, ww = dy.double(), x.double(), w.double()
+    check({"dx": dx, "dw": dw}, {"dx": (d @ ww, (d.abs() @ ww.abs()) * (N + 8) * U),
+                                 "dw": (d.t() @ xx, (d.abs().t() @ xx.abs()) * (M + 8) * U)}, dtype)

@@ -217,3 +217,32 @@ def test_gradients_against_differences(device):
         up, down = f(**{**v, n: t[n] + h * e}), f(**{**v, n: t[n] - h * e})
         want = (grads[n].double() * e).sum().item()
         assert abs((up - down) / (2 * h) - want) < 2e-2 * max(1.0, abs(want)), n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G", [8, 9, 300])
+def test_many_samples(device, dtype, G):
+    """Gates of many samples, whose sums are split over workgroups, down to a row each."""
+    for R in (1, 7):
+        t = case(dtype, G, R, 136, True, "sample", True, seed=G)
+        check(run(t, 1.0, 1e-5, device), reference(t, 1.0, 1e-5), dtype)
+
+
+def test_rows_past_32_bit_offsets(device):
+    """More than 2^32 bytes a tensor: the last rows are those of a call on them alone, bit for bit."""
+    from nsw import ops
+    rows, C = 1_100_001, 2048
+    branch = torch.empty(rows, C, dtype=torch.bfloat16, device=device)
+    branch.random_(-3, 4)
+    skip, dy = branch.flip(0), branch.roll(1, 0)
+    w = torch.linspace(0.5, 1.5, C, device=device).to(torch.bfloat16)
+    kw = dict(post_weight=w, norm_weight=w, eps=1e-5)
+    y, z = ops.residual_norm(branch, skip, **kw)
+    db, ds, dp, _, dn = ops.residual_norm_backward(dy, branch, branch, skip, **kw)
+    n = 4099
+    tail = [t[-n:].clone() for t in (branch, skip, dy)]
+    y2, z2 = ops.residual_norm(tail[0], tail[1], **kw)
+    db2, ds2, _, _, _ = ops.residual_norm_backward(tail[2], tail[0], tail[0], tail[1], **kw)
+    for a, b in ((y, y2), (z, z2), (db, db2), (ds, ds2)):
+        assert torch.equal(a[-n:], b)
+    assert dp.isfinite().all() and dn.isfinite().all()

@@ -22,7 +22,7 @@ def backward(rows=4, C=64, G=1, dtype=BF16, gate=P, norm=P, dz=P, dy=P, dgate=P,
     (forward, dict(C=60), b"multiple of 8"), (forward, dict(C=62, dtype=F32), b"multiple of 4"),
     (forward, dict(C=8200), b"at most 8192"), (forward, dict(C=4100, dtype=F32), b"at most 4096"),
     (forward, dict(C=0), b"C=0"), (forward, dict(rows=-1), b"rows"), (forward, dict(rows=5, G=2), b"multiple of the gate"),
-    (forward, dict(G=0), b"G=0"), (forward, dict(G=2, gate=None), b"without a gate"), (forward, dict(dtype=7), b"dtype"),
+    (forward, dict(G=0), b"G=0"), (forward, dict(G=1 << 17, rows=1 << 17), b"at most 65536"), (forward, dict(G=2, gate=None), b"without a gate"), (forward, dict(dtype=7), b"dtype"),
     (forward, dict(norm=None), b"z is written"), (forward, dict(z=None), b"z is written"),
     (forward, dict(branch=None), b"required"), (forward, dict(y=24), b"aligned"),
     (backward, dict(C=60), b"multiple of 8"), (backward, dict(rows=5, G=2), b"multiple of the gate"),

@@ -29,18 +29,22 @@ struct TileCost {
   }
 };
 
+// `us`, if given: the estimate for the tile picked.
 template <typename T, int EPI>
-static TileSize pick_tile(int64_t M, int64_t N, int64_t K, const EpiArgs& ea) {
+static TileSize pick_tile(int64_t M, int64_t N, int64_t K, const EpiArgs& ea, double* us = nullptr) {
   using C = TileChoice<T, EPI>;
   constexpr bool F32 = sizeof(T) == 4;
   if (EPI == EPI_UNPATCH && ea.img_p == 16) return TILE_BIG;   // a patch of one channel is 256 columns
+  if (EPI == EPI_BATCH) M *= ea.batch;                         // side by side
   constexpr TileCost big = F32 ? TileCost{256, 256, 256, 18, .0795, 9.5, .0605, 0} : TileCost{256, 256, 256, 8.5, .0234, 5.5, .015, 0};
   constexpr TileCost mid = F32 ? TileCost{C::Mid::BM, C::Mid::BN, 512, 8, .0537, 6, .0324, .4}
                                : TileCost{C::Mid::BM, C::Mid::BN, 512, 4.5, .0152, 3.6, .0088, .4};
   constexpr TileCost small = F32 ? TileCost{C::Small::BM, C::Small::BN, 768, 5, .051, 4.3, .0252, .3}
                                  : TileCost{C::Small::BM, C::Small::BN, 512, 2.3, .0099, 3.1, .0062, .4};
   const double b = big.us(M, N, K), m = mid.us(M, N, K), s = small.us(M, N, K);
-  if (std::min(m, s) > 0.93 * b) return TILE_BIG;
+  const bool keep = std::min(m, s) > 0.93 * b;
+  if (us) *us = keep ? b : std::min(m, s);
+  if (keep) return TILE_BIG;
   return s < m ? TILE_SMALL : TILE_MID;
 }
 
@@ -227,16 +231,26 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
   return (M + bm - 1) / bm * 2;
 }
 
-// fp32 y[s] [M, N] = x[s] [M, K] . w[s] [N, K]^T for s < batch: rows ld values apart (a
-// multiple of 4), the products' operands xs and ws values apart, the results one after
+// fp32 y[s] [M, N] = x[s] . w[s]^T for s < batch: product s contracts values [s K, (s + 1)
+// K) of kall in all (a multiple of 16; the last may be shorter), rows are ld values apart
+// (a multiple of 4), the products' operands xs and ws values apart, the results one after
 // the other.
-int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t ld, int64_t xs, int64_t ws,
-                   int batch, hipStream_t st, const char* what) {
-  NSW_CHECK_ARG(batch > 0 && batch < 65536, "%s: too many products", what);
+int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t kall, int64_t ld,
+                   int64_t xs, int64_t ws, int batch, hipStream_t st, const char* what) {
+  NSW_CHECK_ARG(batch > 0 && batch < 65536 && kall <= batch * K && kall > (batch - 1) * K && kall % 16 == 0,
+                "%s: %d products of %lld for %lld", what, batch, (long long)K, (long long)kall);
   NSW_CHECK_ARG((uint64_t)std::max(M, N) * ld * 4 < (1ULL << 31), "%s: operands above 2 GiB are not supported", what);
   EpiArgs ea{};
-  ea.batch = batch; ea.ld = (int)ld; ea.xs = xs; ea.ws = ws;
+  ea.batch = batch; ea.ld = (int)ld; ea.xs = xs; ea.ws = ws; ea.kall = kall;
   return launch_gemm<float, EPI_BATCH, PRE_NONE>(x, w, y, M, N, K, ea, st, what);
+}
+// Its estimated time (us).
+double gemm_f32_batch_us(int64_t M, int64_t N, int64_t K, int batch) {
+  EpiArgs ea{};
+  ea.batch = batch;
+  double us = 0;
+  pick_tile<float, EPI_BATCH>(M, N, K, ea, &us);
+  return us;
 }
 
 // y[remap(m)] = x[m] . w^T + bias + residual[m], the stored rows' partial

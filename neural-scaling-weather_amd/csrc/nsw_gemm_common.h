@@ -67,7 +67,7 @@ struct EpiArgs {
   int img_C, img_H, img_W, img_p, img_f32;
   int act;      // EPI_GATED, EPI_GATED_GRAD: NSW_ACT_*
   int batch, ld;  // EPI_BATCH: products, and values between an operand's rows
-  int64_t xs, ws; // EPI_BATCH: values between the products' operands
+  int64_t xs, ws, kall; // EPI_BATCH: values between the products' operands; the contraction of all products
 };
 
 // GELU with the exact-erf form of nn.GELU(): 0.5 v (1 + erf(v / sqrt 2)).

@@ -1143,6 +1143,8 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
     X += (int64_t)blockIdx.y * ea.xs;
     Wt += (int64_t)blockIdx.y * ea.ws;
     Y += (int64_t)blockIdx.y * M * N;
+    const int64_t left = ea.kall - (int64_t)blockIdx.y * K;
+    K = left < K ? (int)left : K;
   }
   const int ld = EPI == EPI_BATCH ? ea.ld : K;     // values between rows of x and of w
   const T* Xt = GATE ? X + (int64_t)m0 * K : X;

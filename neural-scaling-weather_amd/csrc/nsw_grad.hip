@@ -13,8 +13,9 @@ namespace nsw {
 int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M,
                int64_t H, int64_t K, int act, int dtype, void* stream, const char* what);
 int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype);
-int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t ld, int64_t xs, int64_t ws,
-                   int batch, hipStream_t st, const char* what);
+int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t kall, int64_t ld,
+                   int64_t xs, int64_t ws, int batch, hipStream_t st, const char* what);
+double gemm_f32_batch_us(int64_t M, int64_t N, int64_t K, int batch);
 int grad_product(const void* x, const void* w, void* out, int64_t R, int64_t C, int64_t D, int xt, void* ws, hipStream_t st,
                  const char* what);
 int64_t grad_product_workspace(int64_t R, int64_t C, int64_t D, int64_t ld);
@@ -126,33 +127,37 @@ int column_sums(const float* part, void* out, int64_t P, int64_t C, hipStream_t 
 int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 int64_t column_part_rows(int64_t M) { return std::max<int64_t>(256, (M + 63) / 64); }
 
-// fp32: pieces of the batch for dw, enough to fill the chip with 64 x 128 tiles of at
-// least 256 rows' work, and none whose transposed rows pass the GEMM's 2 GiB.
-void split_batch(int64_t M, int64_t N, int64_t K, int64_t& S, int64_t& P) {
-  const int64_t tiles = ((N + 63) / 64) * ((K + 127) / 128);
-  S = std::max<int64_t>(1, std::min<int64_t>({768 / tiles, M / 256, 64}));
-  const int64_t most = ((1LL << 31) - 1) / (std::max(N, K) * 4) / 64 * 64;
-  P = std::min(std::max<int64_t>(most, 64), ((M + S - 1) / S + 63) / 64 * 64);
-  S = (M + P - 1) / P;
-}
-
-// fp32: pieces of dx's contraction (N) where its tiles leave compute units idle: equal
-// ones of whole steps (16), at least 64 long.
-int64_t split_contraction(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = ((M + 63) / 64) * ((K + 127) / 128);
-  if (M * N * 4 >= (1LL << 31)) return 1;               // dx's rows go in pieces
-  int64_t S = std::min<int64_t>({768 / tiles, N / 64, 32});
-  while (S > 1 && (N / 16) % S) --S;
-  return std::max<int64_t>(1, S);
+// fp32: how a contraction of D values is cut for R x C results, pieces of P (a multiple of
+// `step`, at least 64, at most `most`): by estimated time, the pieces' products written
+// and read once more at 4.5 TB/s.
+void split_f32(int64_t R, int64_t C, int64_t D, int64_t step, int64_t most, int64_t& S, int64_t& P) {
+  auto up = [&](int64_t v) { return (v + step - 1) / step * step; };
+  double best = 0;
+  S = 0;
+  for (int64_t s = 1; s <= 64; ++s) {
+    const int64_t p = std::min(most, std::max<int64_t>(up((D + s - 1) / s), up(64)));
+    const int64_t n = (D + p - 1) / p;
+    const double us = gemm_f32_batch_us(R, C, std::min(p, up(D)), (int)std::min<int64_t>(n, 1 << 20)) +
+                      (n > 1 ? 3 + (double)(n * R * C) * 8 / 4.5e6 : 0);
+    if (S == 0 || us < best) {
+      best = us;
+      S = n;
+      P = p;
+    }
+    if (n < s) break;                                   // no more pieces to be had
+  }
 }
 
 // Workspace of the two products and the column sums.
 struct GradSpace {
-  int64_t S = 1, P = 0, Sx = 1, wt = 0, dyt = 0, xt = 0, prod = 0, part = 0, bytes = 0;
+  int64_t S = 1, P = 0, Sx = 1, Px = 0, wt = 0, dyt = 0, xt = 0, prod = 0, part = 0, bytes = 0;
   GradSpace(int64_t M, int64_t N, int64_t K, int64_t parts, int dtype) {
     if (dtype == NSW_DTYPE_F32) {
-      split_batch(M, N, K, S, P);
-      Sx = split_contraction(M, N, K);
+      // dw: none whose transposed rows pass the GEMM's 2 GiB; dx: whole, where its rows
+      // go in pieces for that
+      split_f32(N, K, M, 64, std::max<int64_t>(((1LL << 31) - 1) / (std::max(N, K) * 4) / 64 * 64, 64), S, P);
+      if (M * N * 4 < (1LL << 31)) split_f32(M, K, N, 16, N, Sx, Px);
+      else Px = N;
       wt = 0;                                          // w^T
       dyt = wt + align256(N * K * 4);                  // dy^T and x^T in pieces
       xt = dyt + align256(S * N * P * 4);
@@ -178,11 +183,11 @@ int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, voi
   if (dx) {
     if ((rc = transpose(w, ws + sp.wt, N, K, 1, N, st, what))) return rc;
     // as many rows at a time as the GEMM's 2 GiB hold
-    const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4)), n = N / sp.Sx;
+    const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4));
     char* out = sp.Sx > 1 ? ws + sp.prod : dx;            // Sx > 1 only where M is small: one piece of rows
     for (int64_t m = 0; m < M; m += rows)
-      if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, out + m * K * 4, std::min(rows, M - m), K, n, N, n, n, (int)sp.Sx,
-                               st, what)))
+      if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, out + m * K * 4, std::min(rows, M - m), K, sp.Px, N, N, sp.Px,
+                               sp.Px, (int)sp.Sx, st, what)))
         return rc;
     if (sp.Sx > 1 && (rc = add_parts(out, dx, M * K, (int)sp.Sx, NSW_DTYPE_F32, st, what))) return rc;
   }
@@ -190,7 +195,8 @@ int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, voi
     if ((rc = transpose(dy, ws + sp.dyt, M, N, sp.S, sp.P, st, what))) return rc;
     if ((rc = transpose(x, ws + sp.xt, M, K, sp.S, sp.P, st, what))) return rc;
     void* out = sp.S > 1 ? ws + sp.prod : dw;
-    if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st, what)))
+    if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, sp.S * sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st,
+                             what)))
       return rc;
     if (sp.S > 1) rc = add_parts(out, dw, N * K, (int)sp.S, NSW_DTYPE_F32, st, what);
   }

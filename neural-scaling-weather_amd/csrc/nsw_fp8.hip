@@ -670,7 +670,7 @@ int launch_fp8(const Fp8Args& a, hipStream_t st, const char* what) {
   const double few = 2.3 + 0.0015 * kb * (double)tiles(16 * mr, 16);
   const double mid = sizeof(T) == 2 ? std::max(4.5 + 0.61 * kb, (double)tiles(128, 128) / 512 * (3.9 + 1.085 * kb))
                                     : std::max(5.5 + 1.0 * kb, (double)tiles(128, 128) / 512 * (4 + 1.9 * kb));
-  if (few < mid && a.M < 16 * 65536 * 4LL) {
+  if (few < mid && a.M <= 64 * 65535LL) {              // the grid's y
     if (mr == 1) return launch_rows<T, EPI, 1>(a, st, what);
     if (mr == 2) return launch_rows<T, EPI, 2>(a, st, what);
     return launch_rows<T, EPI, 4>(a, st, what);

@@ -174,12 +174,22 @@ class Fp8Linear(nn.Module):
         """Of a LinearLayer and the BiasLayer after it, if any."""
         return cls(linear.weight, None if bias is None else bias.bias, epilogue)
 
+    def _apply(self, fn, recurse=True):
+        # as bytes: a change of dtype (module.bfloat16()) is for the bias
+        self.weight, self.weight_scale = (t.view(torch.uint8) for t in (self.weight, self.weight_scale))
+        try:
+            return super()._apply(fn, recurse)
+        finally:
+            self.weight, self.weight_scale = self.weight.view(torch.float8_e4m3fn), self.weight_scale.view(torch.float8_e8m0fnu)
+
     def forward(self, x, residual=None):
-        xq, xs = torch.ops.nsw.quantize_fp8(x, 1)
         epi = self.epilogue
+        if residual is not None and epi in (_lib.NSW_EPI_BIAS_GELU, _lib.NSW_EPI_BIAS_GELU_TANH):
+            raise NotImplementedError("a residual after a GELU is not fused")
         if epi is None or residual is not None:
             epi = _lib.NSW_EPI_NONE if self.bias is None else (
                 _lib.NSW_EPI_BIAS if residual is None else _lib.NSW_EPI_BIAS_RESIDUAL)
         if residual is not None and epi != _lib.NSW_EPI_BIAS_RESIDUAL:
             raise NotImplementedError("a residual without a bias is not fused")
+        xq, xs = torch.ops.nsw.quantize_fp8(x, 1)
         return torch.ops.nsw.linear_fp8(xq, xs, self.weight, self.weight_scale, self.bias, residual, int(epi), x.dtype)

@@ -466,6 +466,8 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     if epilogue is None:
         epilogue = _lib.NSW_EPI_NONE if bias is None else (
             _lib.NSW_EPI_BIAS if residual is None else _lib.NSW_EPI_BIAS_RESIDUAL)
+    if (bias is not None and epilogue == _lib.NSW_EPI_NONE) or (residual is not None and epilogue != _lib.NSW_EPI_BIAS_RESIDUAL):
+        raise ValueError(f"{what}: epilogue {int(epilogue)} has no part for the {'bias' if residual is None else 'residual'}")
     y = xq.new_empty(shape[:-1] + (N,), dtype=dtype)
     if residual is not None and residual.shape != y.shape:
         raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")

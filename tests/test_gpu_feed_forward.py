@@ -211,3 +211,31 @@ def test_fp8_linear_refusals(device):
         xq, xs = ops.quantize_fp8(x)
         ops.linear_fp8(xq, xs[:2].contiguous(), q.weight, q.weight_scale, dtype=F32)
     assert q(x).dtype == F32 and q.epilogue is None and _lib.NSW_EPI_NONE == 0
+
+
+def test_fp8_parts_that_an_epilogue_lacks(device):
+    """A bias or residual that the epilogue would leave out is refused, not dropped."""
+    mlp = nsw.MLP(64, 128).to(device=device, dtype=BF16).to_fp8()
+    x = torch.randn(3, 64, device=device).to(BF16)
+    with torch.no_grad():
+        with pytest.raises(NotImplementedError, match="GELU"):
+            mlp.fc1(x, residual=torch.zeros(3, 128, device=device, dtype=BF16))
+        xq, w = ops.quantize_fp8(x), (mlp.fc1.weight, mlp.fc1.weight_scale)
+        r = torch.zeros(3, 128, device=device, dtype=BF16)
+        with pytest.raises(ValueError, match="residual"):
+            ops.linear_fp8(*xq, *w, None, r)
+        with pytest.raises(ValueError, match="residual"):
+            ops.linear_fp8(*xq, *w, mlp.fc1.bias, r, epilogue=_lib.NSW_EPI_BIAS_GELU)
+        with pytest.raises(ValueError, match="bias"):
+            ops.linear_fp8(*xq, *w, mlp.fc1.bias, epilogue=_lib.NSW_EPI_NONE)
+
+
+def test_fp8_module_keeps_its_bytes_under_a_change_of_dtype(device):
+    torch.manual_seed(5)
+    mlp = nsw.MLP(128, 256).to(device=device, dtype=F32).to_fp8()
+    held_ = [t.clone() for t in (mlp.fc1.weight, mlp.fc1.weight_scale)]
+    mlp = mlp.to(BF16)
+    x = torch.randn(5, 128, device=device).to(BF16)
+    assert mlp.fc1.bias.dtype == BF16 and mlp(x).dtype == BF16
+    for t, want in zip((mlp.fc1.weight, mlp.fc1.weight_scale), held_):
+        assert t.dtype == want.dtype and torch.equal(t.view(torch.uint8), want.view(torch.uint8))

@@ -370,77 +370,108 @@ __global__ __launch_bounds__(NT) void residual_norm_backward_kernel(NormArgs a) 
   store_part<CFG>(Q, buf, dst + C, C, ln);
 }
 
-// dgate, dpost_w and dnorm_w from the workgroups' partial rows [G P][2][C], 16
-// columns to a workgroup: 4 lanes hold 4 columns each, 64 groups of them take every
-// 64th partial row and meet in LDS, always in the same order.  Many samples are split
-// over gridDim.y workgroups, which leave their sums in over [gridDim.y][2][C] for
-// residual_norm_split_kernel.
+// Team of a sample's partial rows among the 16-column groups of 4 lanes: all of them
+// where there are more than 16 rows, else 1, 4 or 16 groups of one wave, so that few
+// rows need no barrier and many samples go side by side.
+constexpr int PT = 1024, NG = PT / 4;  // threads of residual_norm_params_kernel, its groups
+__host__ __device__ constexpr int team_of(int P) { return P == 1 ? 1 : P <= 4 ? 4 : P <= 16 ? 16 : NG; }
+
+// dgate and dpost_w (blockIdx.z 0) and dnorm_w (1) from the workgroups' partial rows
+// [G P][2][C], 16 columns to a workgroup: 4 lanes hold 4 columns each, a team takes its
+// rows in turn and adds up, always in the same order.  Many samples are split over
+// gridDim.y workgroups, which leave their sums in over [gridDim.y][2][C] for
+// residual_norm_split_kernel.  Bound by latency: with 64 groups, all of them on each
+// sample and both sums in turn the backward pass of 16199 x 200 fp32 took 24.0 us, 19.8
+// so; of 20000 samples of 2 rows of 256 bf16 491 us, 100 so.
 template <typename T>
-__global__ __launch_bounds__(NT) void residual_norm_params_kernel(const float* __restrict__ part, int G, int P, int C,
+__global__ __launch_bounds__(PT) void residual_norm_params_kernel(const float* __restrict__ part, int G, int P, int C,
                                                                   const T* __restrict__ post_w, const T* __restrict__ gate,
                                                                   T* __restrict__ dpost, T* __restrict__ dgate,
                                                                   T* __restrict__ dnorm, float* __restrict__ over) {
   const int per = (G + (int)gridDim.y - 1) / (int)gridDim.y, g0 = (int)blockIdx.y * per, g1 = g0 + per < G ? g0 + per : G;
   const bool split = gridDim.y > 1;
   float* mine = over + (int64_t)blockIdx.y * 2 * C;
-  constexpr int NG = NT / 4;
-  __shared__ __attribute__((aligned(16))) float red[NG][20];
+  __shared__ __attribute__((aligned(16))) float red[2][PT / 64][16];
+  int turn = 0;
   const int cl = ((int)threadIdx.x & 3) * 4, grp = (int)threadIdx.x >> 2;
   const int c = (int)blockIdx.x * 16 + cl;
   const bool in = c < C;
-  // the sum over rows [p0, p1) of partial array h, for the thread's 4 columns where grp == 0
-  auto sum = [&](int64_t p0, int64_t p1, int h) {
+  // over a team of 4 groups, over the wave's 4 of those, over the waves
+  auto over4 = [](f32x4& t) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = t[e];                                       // not t[e] itself: a bit cast of an element reads element 0
+      x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
+      x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x124, 0xf, 0xf, false));
+      t[e] = x;
+    }
+  };
+  auto over16 = [](f32x4& t) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = rows4_sum(t[e]);
+  };
+  // a buffer is written again two turns later, past the barrier of the turn between
+  auto over_waves = [&](f32x4& t) {
+    float(*r)[16] = red[turn & 1];
+    ++turn;
+    if ((threadIdx.x & 63) < 4) *reinterpret_cast<f32x4*>(&r[threadIdx.x >> 6][cl]) = t;
+    __syncthreads();
+    t = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < PT / 64; ++w) t += *reinterpret_cast<const f32x4*>(&r[w][cl]);
+  };
+  // the sum over rows p0, p0 + step .. below p1 of partial array h
+  auto rows = [&](int64_t p0, int64_t p1, int step, int h) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
     if (in) {
-#pragma unroll 8
-      for (int64_t p = p0 + grp; p < p1; p += NG) t += *reinterpret_cast<const f32x4*>(part + (p * 2 + h) * C + c);
-    }
-    __syncthreads();
-    *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
-    __syncthreads();
-    if (grp < 8) {
-      t = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < NG / 8; ++i) t += *reinterpret_cast<const f32x4*>(&red[grp * (NG / 8) + i][cl]);
-    }
-    __syncthreads();
-    if (grp < 8) *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
-    __syncthreads();
-    if (grp == 0) {
-#pragma unroll
-      for (int i = 1; i < 8; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
+#pragma unroll 4
+      for (int64_t p = p0; p < p1; p += step) t += *reinterpret_cast<const f32x4*>(part + (p * 2 + h) * C + c);
     }
     return t;
   };
-  const bool out = in && grp == 0;
-  if (dpost != nullptr || dgate != nullptr) {
-    float w[4] = {1.f, 1.f, 1.f, 1.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
-    if (post_w != nullptr && in) load4<T>(post_w + c, w);
-    for (int g = g0; g < g1; ++g) {
-      const f32x4 s = sum((int64_t)g * P, (int64_t)(g + 1) * P, 0);
-      if (!out) continue;
-      float gt[4] = {1.f, 1.f, 1.f, 1.f}, dg[4];
-      if (gate != nullptr) load4<T>(gate + (int64_t)g * C + c, gt);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dg[e] = w[e] * s[e];
-        dp[e] = fmaf(gt[e], s[e], dp[e]);
-      }
-      if (dgate != nullptr) store4<T>(dgate + (int64_t)g * C + c, dg);
-    }
-    if (dpost != nullptr && out) {
-      if (split) store4<float>(mine + c, dp);
-      else store4<T>(dpost + c, dp);
-    }
-  }
-  if (dnorm != nullptr) {
-    const f32x4 q = sum((int64_t)g0 * P, (int64_t)(g1 > g0 ? g1 : g0) * P, 1);
+  if (blockIdx.z == 1) {
+    if (dnorm == nullptr) return;
+    f32x4 q = rows((int64_t)g0 * P + grp, (int64_t)(g1 > g0 ? g1 : g0) * P, NG, 1);
+    over4(q);
+    over16(q);
+    over_waves(q);
+    if (grp != 0 || !in) return;
     const float v[4] = {q[0], q[1], q[2], q[3]};
-    if (out) {
-      if (split) store4<float>(mine + C + c, v);
-      else store4<T>(dnorm + c, v);
-    }
+    if (split) store4<float>(mine + C + c, v);
+    else store4<T>(dnorm + c, v);
+    return;
   }
+  if (dpost == nullptr && dgate == nullptr) return;
+  const int team = team_of(P), at = grp % team;
+  float w[4] = {1.f, 1.f, 1.f, 1.f};
+  f32x4 dp = {0.f, 0.f, 0.f, 0.f};
+  if (post_w != nullptr && in) load4<T>(post_w + c, w);
+  for (int gb = g0; gb < g1; gb += NG / team) {
+    const int g = gb + grp / team;
+    f32x4 s = g < g1 ? rows((int64_t)g * P + at, (int64_t)(g + 1) * P, team, 0) : f32x4{0.f, 0.f, 0.f, 0.f};
+    if (team >= 4) over4(s);
+    if (team >= 16) over16(s);
+    if (team == NG) over_waves(s);
+    if (at != 0 || g >= g1 || !in) continue;
+    float gt[4] = {1.f, 1.f, 1.f, 1.f}, dg[4];
+    if (gate != nullptr) load4<T>(gate + (int64_t)g * C + c, gt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dg[e] = w[e] * s[e];
+      dp[e] = fmaf(gt[e], s[e], dp[e]);
+    }
+    if (dgate != nullptr) store4<T>(dgate + (int64_t)g * C + c, dg);
+  }
+  if (dpost == nullptr) return;
+  if (team < NG) {                                          // over the teams; lanes that lead none hold zeros
+    over4(dp);
+    over16(dp);
+    over_waves(dp);
+  }
+  if (grp != 0 || !in) return;
+  const float v[4] = {dp[0], dp[1], dp[2], dp[3]};
+  if (split) store4<float>(mine + c, v);
+  else store4<T>(dpost + c, v);
 }
 
 // dpost_w and dnorm_w from the Y split sums, in order; a lane 4 columns of one of them.
@@ -458,9 +489,14 @@ __global__ __launch_bounds__(NT) void residual_norm_split_kernel(const float* __
   store4<T>(out + (i < C ? i : i - C), v);
 }
 
-// Workgroups that share the samples of the parameters' sums: one for few samples (a
-// second launch costs more than their loop), else four samples each, at most 64.
-inline int sample_split(int64_t G) { return G <= 8 ? 1 : (int)std::min<int64_t>(64, (G + 3) / 4); }
+// Workgroups that share the samples of the parameters' sums: one where the samples go
+// side by side or are at most 3 (bf16 backward, us one / shared: 2 x 1000 x 512 11.5 /
+// 12.1, 3 x 1000 x 512 14.0 / 13.3, 8 x 500 x 256 17.6 / 10.5), else as many as it takes,
+// at most 64.
+inline int sample_split(int64_t G, int P) {
+  const int64_t side = NG / team_of(P);
+  return G <= std::max<int64_t>(3, side) ? 1 : (int)std::min<int64_t>(64, (G + side - 1) / side);
+}
 
 // Workgroups of a sample: enough to fill the chip `per_cu` times over in all, each
 // with at least one turn of rows.
@@ -541,9 +577,9 @@ int launch_backward(NormArgs a, int64_t rows, int64_t G, void* dpost, void* dgat
     return check_launch(what);
   });
   if (rc || (!dpost && !dgate && !dnorm)) return rc;
-  const int Y = sample_split(G);
+  const int Y = sample_split(G, P);
   float* over = a.part + std::max<int64_t>((int64_t)P * G, 1) * 2 * a.C;
-  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 15) / 16), (unsigned)Y), dim3(NT), 0, st, a.part,
+  hipLaunchKernelGGL((residual_norm_params_kernel<T>), dim3((unsigned)((a.C + 15) / 16), (unsigned)Y, 2), dim3(PT), 0, st, a.part,
                      (int)G, P, a.C, (const T*)a.post_w, (const T*)a.gate, (T*)dpost, (T*)dgate, (T*)dnorm, over);
   rc = check_launch(what);
   if (rc || Y == 1 || (!dpost && !dnorm)) return rc;
@@ -582,7 +618,7 @@ extern "C" int nsw_residual_norm(const void* branch, const void* skip, const voi
 extern "C" size_t nsw_residual_norm_backward_workspace_size(int64_t rows, int64_t C, int64_t G, int dtype) {
   if (check_norm("nsw_residual_norm_backward_workspace_size", rows, C, G, dtype, &rows) != NSW_OK) return 0;
   const int64_t n = dtype == NSW_DTYPE_BF16 ? backward_parts<bf16>(rows, C, G) : backward_parts<float>(rows, C, G);
-  const int64_t Y = sample_split(G);
+  const int64_t Y = sample_split(G, (int)(n / G));
   return (size_t)((std::max<int64_t>(n, 1) + (Y > 1 ? Y : 0)) * 2 * C) * sizeof(float);
 }
 

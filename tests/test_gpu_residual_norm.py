@@ -228,6 +228,14 @@ def test_many_samples(device, dtype, G):
         check(run(t, 1.0, 1e-5, device), reference(t, 1.0, 1e-5), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G,R", [(3, 30), (3, 100), (2, 300), (4, 300), (40, 300), (70, 100), (300, 33)])
+def test_sums_of_samples_of_unlike_length(device, dtype, G, R):
+    """Few and many samples whose partial sums are few, some and many."""
+    t = case(dtype, G, R, 136, True, "sample", True, seed=G + R)
+    check(run(t, 1.0, 1e-5, device), reference(t, 1.0, 1e-5), dtype)
+
+
 def test_rows_past_32_bit_offsets(device):
     """More than 2^32 bytes a tensor: the last rows are those of a call on them alone, bit for bit."""
     from nsw import ops

@@ -18,10 +18,9 @@
 
 #include "nsw_gemm_common.h"
 #include "nsw_gemm_tiles.h"
+#include "nsw_grad.h"
 
 namespace nsw {
-
-int add_parts(const void* part, void* out, int64_t n, int S, int dtype, hipStream_t st, const char* what);
 
 namespace {
 
@@ -268,17 +267,16 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
 // 128 x 128 results, four waves of 64 x 64, two workgroups a CU: where 256 x 256 leaves
 // compute units idle.  A ring of two stages, one barrier a stage (mainloop_ring of the
 // forward GEMM).
-template <bool XT, typename OT>
-__global__ __launch_bounds__(256, 2) void grad_small_kernel(GradArgs a) {
+template <bool XT>
+__device__ __forceinline__ void grad_small_tile(char* smem, const GradArgs& a, int bid) {
   constexpr int GB = 128, GSLOT = gslot(GB);
   using CX = OperandCopy<XT, GB>;
   using CW = OperandCopy<true, GB>;
   constexpr int NC = CX::NC;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * GSLOT];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   constexpr int GM = GROUP_M * 2;                           // tile order as grad_kernel
   const int MT = (a.R + GB - 1) / GB, NT = (a.C + GB - 1) / GB;
-  const int id = xcd_remap(blockIdx.x, MT * NT * a.S);
+  const int id = xcd_remap(bid, MT * NT * a.S);
   const int part = id / (MT * NT), tile = id - part * (MT * NT);
   const int gm0 = tile / (GM * NT) * GM, gsz = MT - gm0 < GM ? MT - gm0 : GM, tin = tile - gm0 * NT;
   const int r0 = (gm0 + tin % gsz) * GB, c0 = tin / gsz * GB;
@@ -325,7 +323,29 @@ __global__ __launch_bounds__(256, 2) void grad_small_kernel(GradArgs a) {
     }
   }
   wg_barrier();            // the ring is no longer read
-  grad_write_out<OT, 4>(smem, acc, a, part, r0 + (wave / 2) * 64, c0 + (wave % 2) * 64, wave, lane);
+  const int rw = r0 + (wave / 2) * 64, cw0 = c0 + (wave % 2) * 64;
+  if (a.S > 1) grad_write_out<float, 4>(smem, acc, a, part, rw, cw0, wave, lane);
+  else grad_write_out<bf16, 4>(smem, acc, a, part, rw, cw0, wave, lane);
+}
+
+// Workgroups [0, nw) dw, then nx of dx, then the column sums: products that leave compute
+// units idle run side by side in one launch (M 300, N 1024, K 256: PAIR_US us where the
+// three took SEP_US one after the other).  nw is a multiple of 8, so that a workgroup's
+// place in its product keeps its XCD.
+__global__ __launch_bounds__(256, 2) void grad_small_kernel(GradArgs dw, int nw, GradArgs dx, int nx, ColumnSums sums, int N) {
+  __shared__ __attribute__((aligned(1024))) char smem[4 * gslot(128)];
+  int id = (int)blockIdx.x;
+  auto count = [](const GradArgs& a) { return (a.R + 127) / 128 * ((a.C + 127) / 128) * a.S; };
+  if (id < nw) {
+    if (id < count(dw)) grad_small_tile<true>(smem, dw, id);
+    return;
+  }
+  id -= nw;
+  if (id < nx) {
+    if (id < count(dx)) grad_small_tile<false>(smem, dx, id);
+    return;
+  }
+  column_sums_block<bf16>(sums.part, (bf16*)sums.out, (int)sums.parts, N, id - nx, reinterpret_cast<float(*)[36]>(smem));
 }
 
 }  // namespace
@@ -351,62 +371,92 @@ struct GradCost {
 struct GradPlan {
   int gb = 256, S = 0;
   int64_t per = 0;
+  double us = 0;
 };
+constexpr GradCost BIG_COST{256, 256, 8.5, 1.4, 5.5, 0.96, 0}, SMALL_COST{128, 512, 4.5, 0.97, 3.6, 0.56, 0.4};
+int64_t tiles(int64_t R, int64_t C, int gb) { return ((R + gb - 1) / gb) * ((C + gb - 1) / gb); }
+// A second launch, and the parts through memory.
+double parts_us(int64_t S, int64_t n) { return S > 1 ? 3 + (double)(S * n) * 8 / 4.5e6 : 0; }
+
 GradPlan grad_plan(int64_t R, int64_t C, int64_t D, int64_t ld) {
-  constexpr GradCost big{256, 256, 8.5, 1.4, 5.5, 0.96, 0}, small{128, 512, 4.5, 0.97, 3.6, 0.56, 0.4};
   const int64_t stages = (D + GD - 1) / GD;
   GradPlan p;
-  double best = 0;
-  for (const GradCost& c : {big, small}) {
-    const int64_t tiles = ((R + c.gb - 1) / c.gb) * ((C + c.gb - 1) / c.gb);
+  for (const GradCost& c : {BIG_COST, SMALL_COST}) {
+    const int64_t n = tiles(R, C, c.gb);
     for (int64_t s = 1; s <= 64 && s <= stages; ++s) {
       const int64_t each = (stages + s - 1) / s, parts = (stages + each - 1) / each;
       // 32-bit offsets inside a part (at the most parts there are, the caller refuses)
       if (each * GD * ld * 2 >= (1LL << 31) && s < 64 && s < stages) continue;
-      double t = c.us((double)(tiles * parts), (double)each);
-      if (parts > 1) t += 3 + (double)(parts * R * C) * 8 / 4.5e6;
-      if (p.S == 0 || t < best) {
-        best = t;
-        p.gb = c.gb;
-        p.S = (int)parts;
-        p.per = each * GD;
-      }
+      const double t = c.us((double)(n * parts), (double)each) + parts_us(parts, R * C);
+      if (p.S == 0 || t < p.us) p = GradPlan{c.gb, (int)parts, each * GD, t};
     }
   }
   return p;
 }
 
+// Both products side by side on 128 x 128 tiles, in parts of one length; where that is
+// estimated slower than one after the other (x, w), those are left.
+void pair_plan(int64_t M, int64_t N, int64_t K, GradPlan& x, GradPlan& w) {
+  const int64_t sx = (N + GD - 1) / GD, sw = (M + GD - 1) / GD, nx = tiles(M, K, 128), nw = tiles(N, K, 128);
+  double best = x.us + w.us;
+  for (int64_t each = 2; each < 2 * std::max(sx, sw); each *= 2) {
+    const int64_t ex = std::min(each, sx), ew = std::min(each, sw);
+    const int64_t Sx = (sx + ex - 1) / ex, Sw = (sw + ew - 1) / ew;
+    if (Sx > 64 || Sw > 64 || each * GD * std::max(N, K) * 2 >= (1LL << 31)) continue;
+    const double t = SMALL_COST.us((double)(nx * Sx + nw * Sw), (double)std::max(ex, ew)) +
+                     std::max(parts_us(Sx, M * K), parts_us(Sw, N * K));
+    if (t < best) {
+      best = t;
+      x = GradPlan{128, (int)Sx, ex * GD, t};
+      w = GradPlan{128, (int)Sw, ew * GD, t};
+    }
+  }
+}
+int64_t plan_bytes(const GradPlan& p, int64_t n) { return p.S > 1 ? (p.S * n * 4 + 255) / 256 * 256 : 0; }
+
 }  // namespace
 
-int64_t grad_product_workspace(int64_t R, int64_t C, int64_t D, int64_t ld) {
-  const GradPlan p = grad_plan(R, C, D, ld);
-  return p.S > 1 ? (int64_t)p.S * R * C * 4 : 0;
+int64_t grad_products_workspace(int64_t M, int64_t N, int64_t K) {
+  GradPlan x = grad_plan(M, K, N, K), w = grad_plan(N, K, M, std::max(N, K));
+  const int64_t alone = plan_bytes(x, M * K) + plan_bytes(w, N * K);
+  pair_plan(M, N, K, x, w);
+  return std::max(alone, plan_bytes(x, M * K) + plan_bytes(w, N * K));
 }
 
-// out [R, C] = X . W, X [R, D] (xt 0) or [D, R] (xt 1), W [D, C].
-int grad_product(const void* x, const void* w, void* out, int64_t R, int64_t C, int64_t D, int xt, void* ws, hipStream_t st,
-                 const char* what) {
-  GradArgs a{};
-  a.x = (const bf16*)x; a.w = (const bf16*)w;
-  a.ldx = xt ? R : D; a.ldw = C;
-  a.R = (int)R; a.C = (int)C; a.D = D;
-  const int64_t ld = std::max<int64_t>(C, xt ? R : 0);
-  const GradPlan p = grad_plan(R, C, D, ld);
-  a.S = p.S; a.per = p.per;
-  NSW_CHECK_ARG(a.per * ld * 2 < (1LL << 31) && (xt || p.gb * D * 2 < (1LL << 31)), "%s: rows too long (32-bit offsets)", what);
-  const int64_t grid = ((R + p.gb - 1) / p.gb) * ((C + p.gb - 1) / p.gb) * a.S;
-  NSW_CHECK_ARG(grid < (1LL << 31), "%s: too many tiles", what);
-  a.out = a.S > 1 ? ws : out;
-  auto go = [&](auto big, auto small) {
-    if (p.gb == 256) hipLaunchKernelGGL(big, dim3((unsigned)grid), dim3(512), 0, st, a);
-    else hipLaunchKernelGGL(small, dim3((unsigned)grid), dim3(256), 0, st, a);
-  };
-  if (a.S > 1 && xt) go(grad_kernel<true, float>, grad_small_kernel<true, float>);
-  else if (a.S > 1) go(grad_kernel<false, float>, grad_small_kernel<false, float>);
-  else if (xt) go(grad_kernel<true, bf16>, grad_small_kernel<true, bf16>);
-  else go(grad_kernel<false, bf16>, grad_small_kernel<false, bf16>);
-  if (int rc = check_launch(what)) return rc;
-  return a.S > 1 ? add_parts(ws, out, R * C, a.S, NSW_DTYPE_BF16, st, what) : NSW_OK;
+// dx [M, K] = dy . w and dw [N, K] = dy^T . x, where not NULL, and the column sums.
+int grad_products(const void* dy, const void* x, const void* w, void* dx, void* dw, const ColumnSums& sums, int64_t M, int64_t N,
+                  int64_t K, char* ws, hipStream_t st, const char* what) {
+  GradPlan px, pw;
+  if (dx) px = grad_plan(M, K, N, K);
+  if (dw) pw = grad_plan(N, K, M, std::max(N, K));
+  if (dx && dw) pair_plan(M, N, K, px, pw);
+  GradArgs ax{}, aw{};
+  ax.x = (const bf16*)dy; ax.w = (const bf16*)w; ax.ldx = N; ax.ldw = K;
+  ax.R = (int)M; ax.C = (int)K; ax.D = N; ax.S = px.S; ax.per = px.per;
+  ax.out = px.S > 1 ? ws : dx;
+  aw.x = (const bf16*)dy; aw.w = (const bf16*)x; aw.ldx = N; aw.ldw = K;
+  aw.R = (int)N; aw.C = (int)K; aw.D = M; aw.S = pw.S; aw.per = pw.per;
+  aw.out = pw.S > 1 ? ws + plan_bytes(px, M * K) : dw;
+  NSW_CHECK_ARG(ax.per * K * 2 < (1LL << 31) && (!dx || px.gb * N * 2 < (1LL << 31)) && aw.per * std::max(N, K) * 2 < (1LL << 31),
+                "%s: rows too long (32-bit offsets)", what);
+  const int64_t gx = tiles(M, K, px.gb) * px.S, gw = tiles(N, K, pw.gb) * pw.S, gs = sums.out ? (N + 31) / 32 : 0;
+  NSW_CHECK_ARG(gx + gw + gs < (1LL << 31) - 8, "%s: too many tiles", what);
+  if (dx && px.gb == 256) {
+    if (px.S > 1) hipLaunchKernelGGL((grad_kernel<false, float>), dim3((unsigned)gx), dim3(512), 0, st, ax);
+    else hipLaunchKernelGGL((grad_kernel<false, bf16>), dim3((unsigned)gx), dim3(512), 0, st, ax);
+    if (int rc = check_launch(what)) return rc;
+  }
+  if (dw && pw.gb == 256) {
+    if (pw.S > 1) hipLaunchKernelGGL((grad_kernel<true, float>), dim3((unsigned)gw), dim3(512), 0, st, aw);
+    else hipLaunchKernelGGL((grad_kernel<true, bf16>), dim3((unsigned)gw), dim3(512), 0, st, aw);
+    if (int rc = check_launch(what)) return rc;
+  }
+  const int nx = dx && px.gb == 128 ? (int)gx : 0, nw = dw && pw.gb == 128 ? (int)((gw + 7) / 8 * 8) : 0;
+  if (nx + nw + gs > 0) {
+    hipLaunchKernelGGL(grad_small_kernel, dim3((unsigned)(nx + nw + gs)), dim3(256), 0, st, aw, nw, ax, nx, sums, (int)N);
+    if (int rc = check_launch(what)) return rc;
+  }
+  return add_parts(Parts{ax.out, dx, M * K, px.S}, Parts{aw.out, dw, N * K, pw.S}, NSW_DTYPE_BF16, st, what);
 }
 
 }  // namespace nsw

@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "nsw_gemm_common.h"
+#include "nsw_grad.h"
 
 namespace nsw {
 
@@ -16,10 +17,9 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype);
 int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t kall, int64_t ld,
                    int64_t xs, int64_t ws, int batch, hipStream_t st, const char* what);
 double gemm_f32_batch_us(int64_t M, int64_t N, int64_t K, int batch);
-int grad_product(const void* x, const void* w, void* out, int64_t R, int64_t C, int64_t D, int xt, void* ws, hipStream_t st,
-                 const char* what);
-int64_t grad_product_workspace(int64_t R, int64_t C, int64_t D, int64_t ld);
-int add_parts(const void* part, void* out, int64_t n, int S, int dtype, hipStream_t st, const char* what);
+int grad_products(const void* dy, const void* x, const void* w, void* dx, void* dw, const ColumnSums& sums, int64_t M, int64_t N,
+                  int64_t K, char* ws, hipStream_t st, const char* what);
+int64_t grad_products_workspace(int64_t M, int64_t N, int64_t K);
 
 namespace {
 
@@ -52,16 +52,19 @@ __global__ __launch_bounds__(NT) void transpose_kernel(const float* __restrict__
   }
 }
 
-// out[i] = sum over s of part[s][i], in order; n a multiple of 4.
+// Parts a by the first `na` workgroups, b by the others.
 template <typename T>
-__global__ __launch_bounds__(NT) void add_parts_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t n, int S) {
-  const int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4;
-  if (i >= n) return;
-  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+__global__ __launch_bounds__(NT) void add_parts_kernel(Parts a, unsigned na, Parts b) {
+  const bool first = blockIdx.x < na;
+  const Parts& p = first ? a : b;
+  const int64_t i = ((int64_t)(first ? blockIdx.x : blockIdx.x - na) * NT + threadIdx.x) * 4;
+  if (i >= p.n) return;
+  const float* part = (const float*)p.part + i;
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int s = 0; s < S; ++s) a += *reinterpret_cast<const f32x4*>(part + s * n + i);
-  const float v[4] = {a[0], a[1], a[2], a[3]};
-  store4<T>(out + i, v);
+  for (int s = 0; s < p.S; ++s) t += *reinterpret_cast<const f32x4*>(part + s * p.n);
+  const float v[4] = {t[0], t[1], t[2], t[3]};
+  store4<T>((T*)p.out + i, v);
 }
 
 // part[b][c] = the sum of rows b per .. of x [R, C]: 32 columns to a workgroup, as
@@ -90,24 +93,9 @@ __global__ __launch_bounds__(NT) void column_parts_kernel(const T* __restrict__ 
   }
 }
 
-// out[c] = sum over p of part[p][c], in a fixed order.
-template <typename T>
-__global__ __launch_bounds__(NT) void column_sums_kernel(const float* __restrict__ part, T* __restrict__ out, int P, int C) {
+__global__ __launch_bounds__(NT) void column_sums_kernel(const float* __restrict__ part, float* __restrict__ out, int P, int C) {
   __shared__ __attribute__((aligned(16))) float red[32][36];
-  const int cl = ((int)threadIdx.x & 7) * 4, grp = (int)threadIdx.x >> 3;
-  const int c = (int)blockIdx.x * 32 + cl;
-  f32x4 t = {0.f, 0.f, 0.f, 0.f};
-  if (c < C)
-#pragma unroll 4
-    for (int p = grp; p < P; p += 32) t += *reinterpret_cast<const f32x4*>(part + (int64_t)p * C + c);
-  *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
-  __syncthreads();
-  if (grp == 0 && c < C) {
-#pragma unroll
-    for (int i = 1; i < 32; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
-    const float v[4] = {t[0], t[1], t[2], t[3]};
-    store4<T>(out + c, v);
-  }
+  column_sums_block<float>(part, out, P, C, (int)blockIdx.x, red);
 }
 
 int transpose(const void* in, void* out, int64_t R, int64_t C, int64_t S, int64_t P, hipStream_t st, const char* what) {
@@ -115,12 +103,6 @@ int transpose(const void* in, void* out, int64_t R, int64_t C, int64_t S, int64_
   NSW_CHECK_ARG(gy < 65536, "%s: too many rows", what);
   hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((C + 63) / 64), (unsigned)gy), dim3(NT), 0, st, (const float*)in,
                      (float*)out, R, (int)C, (int)P);
-  return check_launch(what);
-}
-
-template <typename T>
-int column_sums(const float* part, void* out, int64_t P, int64_t C, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL((column_sums_kernel<T>), dim3((unsigned)((C + 31) / 32)), dim3(NT), 0, st, part, (T*)out, (int)P, (int)C);
   return check_launch(what);
 }
 
@@ -164,8 +146,7 @@ struct GradSpace {
       prod = xt + align256(S * K * P * 4);             // their products
       part = prod + align256(std::max(S > 1 ? S * N * K * 4 : 0, Sx > 1 ? Sx * M * K * 4 : 0));
     } else {
-      const int64_t a = grad_product_workspace(M, K, N, K), b = grad_product_workspace(N, K, M, std::max(N, K));
-      part = align256(std::max(a, b));
+      part = grad_products_workspace(M, N, K);
     }
     bytes = part + align256(parts * N * 4);
   }
@@ -175,6 +156,10 @@ bool bad_sizes(int64_t M, int64_t N, int64_t K, int dtype) {
   if (dtype != NSW_DTYPE_BF16 && dtype != NSW_DTYPE_F32) return true;
   const int64_t g = dtype == NSW_DTYPE_BF16 ? 32 : 16;   // one step of the products
   return M <= 0 || N <= 0 || K <= 0 || M >= (1LL << 31) || N >= (1LL << 31) || K >= (1LL << 31) || N % g || K % g;
+}
+
+bool bad_gated_sizes(int64_t M, int64_t H, int64_t K, int dtype) {
+  return H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype);
 }
 
 int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, void* dw, int64_t M, int64_t N, int64_t K,
@@ -189,7 +174,7 @@ int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, voi
       if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, out + m * K * 4, std::min(rows, M - m), K, sp.Px, N, N, sp.Px,
                                sp.Px, (int)sp.Sx, st, what)))
         return rc;
-    if (sp.Sx > 1 && (rc = add_parts(out, dx, M * K, (int)sp.Sx, NSW_DTYPE_F32, st, what))) return rc;
+    if (sp.Sx > 1 && (rc = add_parts(Parts{out, dx, M * K, (int)sp.Sx}, Parts{}, NSW_DTYPE_F32, st, what))) return rc;
   }
   if (dw) {
     if ((rc = transpose(dy, ws + sp.dyt, M, N, sp.S, sp.P, st, what))) return rc;
@@ -198,33 +183,30 @@ int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, voi
     if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, sp.S * sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st,
                              what)))
       return rc;
-    if (sp.S > 1) rc = add_parts(out, dw, N * K, (int)sp.S, NSW_DTYPE_F32, st, what);
+    if (sp.S > 1) rc = add_parts(Parts{out, dw, N * K, (int)sp.S}, Parts{}, NSW_DTYPE_F32, st, what);
   }
   return rc;
 }
 
 int linear_grads(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t parts, int64_t M,
-                 int64_t N, int64_t K, int dtype, char* ws, hipStream_t st, const char* what) {
-  const GradSpace sp(M, N, K, parts, dtype);
-  const float* part = (const float*)(ws + sp.part);
-  int rc = NSW_OK;
-  if (dtype == NSW_DTYPE_F32) {
-    if ((rc = linear_grads_f32((const char*)dy, x, w, (char*)dx, dw, M, N, K, sp, ws, st, what))) return rc;
-    return db ? column_sums<float>(part, db, parts, N, st, what) : rc;
-  }
-  if (dx && (rc = grad_product(dy, w, dx, M, K, N, 0, ws, st, what))) return rc;
-  if (dw && (rc = grad_product(dy, x, dw, N, K, M, 1, ws, st, what))) return rc;
-  return db ? column_sums<bf16>(part, db, parts, N, st, what) : rc;
+                 int64_t N, int64_t K, int dtype, const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
+  const ColumnSums sums{(const float*)(ws + sp.part), db, parts};
+  if (dtype == NSW_DTYPE_BF16) return grad_products(dy, x, w, dx, dw, sums, M, N, K, ws, st, what);
+  if (int rc = linear_grads_f32((const char*)dy, x, w, (char*)dx, dw, M, N, K, sp, ws, st, what)) return rc;
+  if (!db) return NSW_OK;
+  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((N + 31) / 32)), dim3(NT), 0, st, sums.part, (float*)db, (int)parts,
+                     (int)N);
+  return check_launch(what);
 }
 
 }  // namespace
 
-int add_parts(const void* part, void* out, int64_t n, int S, int dtype, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)((n / 4 + NT - 1) / NT));
-  if (dtype == NSW_DTYPE_BF16)
-    hipLaunchKernelGGL((add_parts_kernel<bf16>), grid, dim3(NT), 0, st, (const float*)part, (bf16*)out, n, S);
-  else
-    hipLaunchKernelGGL((add_parts_kernel<float>), grid, dim3(NT), 0, st, (const float*)part, (float*)out, n, S);
+int add_parts(const Parts& a, const Parts& b, int dtype, hipStream_t st, const char* what) {
+  auto blocks = [](const Parts& p) { return p.S > 1 ? (unsigned)((p.n / 4 + NT - 1) / NT) : 0u; };
+  const unsigned na = blocks(a), nb = blocks(b);
+  if (na + nb == 0) return NSW_OK;
+  if (dtype == NSW_DTYPE_BF16) hipLaunchKernelGGL((add_parts_kernel<bf16>), dim3(na + nb), dim3(NT), 0, st, a, na, b);
+  else hipLaunchKernelGGL((add_parts_kernel<float>), dim3(na + nb), dim3(NT), 0, st, a, na, b);
   return check_launch(what);
 }
 
@@ -241,18 +223,19 @@ extern "C" size_t nsw_linear_backward_workspace_size(int64_t M, int64_t N, int64
 extern "C" int nsw_linear_backward(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                                    int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "nsw_linear_backward";
-  const size_t need = nsw_linear_backward_workspace_size(M, N, K, dtype);
-  NSW_CHECK_ARG(need > 0, "%s: M=%lld, N=%lld, K=%lld in dtype %d: N and K must be multiples of 32 (bf16) / 16 (fp32)",
+  NSW_CHECK_ARG(!bad_sizes(M, N, K, dtype), "%s: M=%lld, N=%lld, K=%lld in dtype %d: N and K must be multiples of 32 (bf16) / 16 (fp32)",
                 what, (long long)M, (long long)N, (long long)K, dtype);
   NSW_CHECK_ARG(dy && x && w, "%s: dy, x and w are required", what);
-  NSW_CHECK_ARG(workspace != nullptr && workspace_bytes >= need, "%s: workspace of %zu bytes needed", what, need);
+  const int64_t per = column_part_rows(M), parts = (M + per - 1) / per;
+  const GradSpace sp(M, N, K, parts, dtype);
+  NSW_CHECK_ARG(workspace != nullptr && workspace_bytes >= (size_t)sp.bytes, "%s: workspace of %lld bytes needed", what,
+                (long long)sp.bytes);
   NSW_CHECK_ARG((((uintptr_t)dy | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db |
                   (uintptr_t)workspace) % 16) == 0, "%s: pointers must be 16-byte aligned", what);
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
-  const int64_t per = column_part_rows(M), parts = (M + per - 1) / per;
   if (db) {
-    float* part = (float*)(ws + GradSpace(M, N, K, parts, dtype).part);
+    float* part = (float*)(ws + sp.part);
     const dim3 grid((unsigned)((N + 31) / 32), (unsigned)parts);
     if (dtype == NSW_DTYPE_BF16)
       hipLaunchKernelGGL((column_parts_kernel<bf16>), grid, dim3(NT), 0, st, (const bf16*)dy, part, M, (int)N, per);
@@ -260,11 +243,11 @@ extern "C" int nsw_linear_backward(const void* dy, const void* x, const void* w,
       hipLaunchKernelGGL((column_parts_kernel<float>), grid, dim3(NT), 0, st, (const float*)dy, part, M, (int)N, per);
     if (int rc = check_launch(what)) return rc;
   }
-  return linear_grads(dy, x, w, dx, dw, db, parts, M, N, K, dtype, ws, st, what);
+  return linear_grads(dy, x, w, dx, dw, db, parts, M, N, K, dtype, sp, ws, st, what);
 }
 
 extern "C" size_t nsw_gated_linear_backward_workspace_size(int64_t M, int64_t H, int64_t K, int dtype) {
-  if (H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype)) return 0;
+  if (bad_gated_sizes(M, H, K, dtype)) return 0;
   // dy [M, 2H] first
   return (size_t)(align256(M * 2 * H * (int64_t)dtype_size(dtype)) +
                   GradSpace(M, 2 * H, K, gated_grad_parts(M, H, K, dtype), dtype).bytes);
@@ -274,22 +257,21 @@ extern "C" int nsw_gated_linear_backward(const void* dh, const void* x, const vo
                                          void* db, int64_t M, int64_t H, int64_t K, int act, int dtype, void* workspace,
                                          size_t workspace_bytes, void* stream) {
   const char* what = "nsw_gated_linear_backward";
-  const size_t need = nsw_gated_linear_backward_workspace_size(M, H, K, dtype);
-  NSW_CHECK_ARG(need > 0, "%s: M=%lld, H=%lld, K=%lld in dtype %d: H must be a multiple of 16, K of 32 (bf16) / 16 (fp32)",
+  NSW_CHECK_ARG(!bad_gated_sizes(M, H, K, dtype), "%s: M=%lld, H=%lld, K=%lld in dtype %d: H must be a multiple of 16, K of 32 (bf16) / 16 (fp32)",
                 what, (long long)M, (long long)H, (long long)K, dtype);
   NSW_CHECK_ARG(dh && x && w, "%s: dh, x and w are required", what);
-  NSW_CHECK_ARG(workspace != nullptr && workspace_bytes >= need, "%s: workspace of %zu bytes needed", what, need);
+  const int64_t parts = gated_grad_parts(M, H, K, dtype), dy_bytes = align256(M * 2 * H * (int64_t)dtype_size(dtype));
+  const GradSpace sp(M, 2 * H, K, parts, dtype);
+  NSW_CHECK_ARG(workspace != nullptr && workspace_bytes >= (size_t)(dy_bytes + sp.bytes), "%s: workspace of %lld bytes needed",
+                what, (long long)(dy_bytes + sp.bytes));
   NSW_CHECK_ARG((((uintptr_t)dh | (uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)dx | (uintptr_t)dw |
                   (uintptr_t)db | (uintptr_t)workspace) % 16) == 0, "%s: pointers must be 16-byte aligned", what);
   NSW_CHECK_ARG(act == NSW_ACT_SILU || act == NSW_ACT_GELU || act == NSW_ACT_GELU_TANH, "%s: unknown activation %d", what, act);
   if (!dx && !dw && !db) return NSW_OK;
-  const int64_t parts = gated_grad_parts(M, H, K, dtype);
-  char* ws = (char*)workspace;
-  char* dy = ws;
-  ws += align256(M * 2 * H * (int64_t)dtype_size(dtype));
-  const GradSpace sp(M, 2 * H, K, parts, dtype);
+  char* dy = (char*)workspace;
+  char* ws = dy + dy_bytes;
   int rc = gemm_gated(x, w, bias, dh, dy, db ? (float*)(ws + sp.part) : nullptr, M, H, K, act, dtype, stream, what);
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
-  return linear_grads(dy, x, w, dx, dw, db, parts, M, 2 * H, K, dtype, ws, st, what);
+  return linear_grads(dy, x, w, dx, dw, db, parts, M, 2 * H, K, dtype, sp, ws, st, what);
 }

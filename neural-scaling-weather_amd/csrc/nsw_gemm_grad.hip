@@ -328,24 +328,24 @@ __device__ __forceinline__ void grad_small_tile(char* smem, const GradArgs& a, i
   else grad_write_out<bf16, 4>(smem, acc, a, part, rw, cw0, wave, lane);
 }
 
-// Workgroups [0, nw) dw, then nx of dx, then the column sums: products that leave compute
-// units idle run side by side in one launch (M 300, N 1024, K 256: PAIR_US us where the
-// three took SEP_US one after the other).  nw is a multiple of 8, so that a workgroup's
-// place in its product keeps its XCD.
-__global__ __launch_bounds__(256, 2) void grad_small_kernel(GradArgs dw, int nw, GradArgs dx, int nx, ColumnSums sums, int N) {
+// Workgroups [0, na) the product with the longer parts, nb of the other, then the column
+// sums: products that leave compute units idle run side by side in one launch (gated
+// backward of 300 rows, 256 -> 512: 15.0 us, 20.3 one after the other; 1000, 512 -> 1360:
+// 30 / 42).  na is a multiple of 8, so that a workgroup's place in its product keeps its XCD.
+__global__ __launch_bounds__(256, 2) void grad_small_kernel(GradArgs dw, GradArgs dx, int na, int nb, int dw_first,
+                                                            ColumnSums sums, int N) {
   __shared__ __attribute__((aligned(1024))) char smem[4 * gslot(128)];
   int id = (int)blockIdx.x;
-  auto count = [](const GradArgs& a) { return (a.R + 127) / 128 * ((a.C + 127) / 128) * a.S; };
-  if (id < nw) {
-    if (id < count(dw)) grad_small_tile<true>(smem, dw, id);
+  if (id >= na + nb) {
+    column_sums_block<bf16>(sums.part, (bf16*)sums.out, (int)sums.parts, N, id - na - nb, reinterpret_cast<float(*)[36]>(smem));
     return;
   }
-  id -= nw;
-  if (id < nx) {
-    if (id < count(dx)) grad_small_tile<false>(smem, dx, id);
-    return;
-  }
-  column_sums_block<bf16>(sums.part, (bf16*)sums.out, (int)sums.parts, N, id - nx, reinterpret_cast<float(*)[36]>(smem));
+  const bool is_dw = (id < na) == (dw_first != 0);
+  const GradArgs& a = is_dw ? dw : dx;
+  if (id >= na) id -= na;
+  if (id >= (a.R + 127) / 128 * ((a.C + 127) / 128) * a.S) return;
+  if (is_dw) grad_small_tile<true>(smem, dw, id);
+  else grad_small_tile<false>(smem, dx, id);
 }
 
 }  // namespace
@@ -394,42 +394,60 @@ GradPlan grad_plan(int64_t R, int64_t C, int64_t D, int64_t ld) {
   return p;
 }
 
-// Both products side by side on 128 x 128 tiles, in parts of one length; where that is
-// estimated slower than one after the other (x, w), those are left.
+// Both products side by side on 128 x 128 tiles, each in parts of a length of its own;
+// where that is not estimated 3% faster than one after the other (x, w), those are left.
+// More workgroups than slots: 2 us and 0.8 a stage each, shared out, and 0.35 of the
+// shorter one at the end.  Fits to twelve shapes and all pairs of lengths: what it picks
+// is within 10% of the best pair, 1% at the median.  Measured, us, this / one after the
+// other as before (two launches):
+//   M 12961, N 2720, K 512: 88 / 91   2000, 8192, 1024: 71 / 82   64800, 512, 256: 46 / 57
+//   2000, 1024, 256: 15 / 22          64800, 2048, 512: 281 / 234 (left one after the other)
 void pair_plan(int64_t M, int64_t N, int64_t K, GradPlan& x, GradPlan& w) {
   const int64_t sx = (N + GD - 1) / GD, sw = (M + GD - 1) / GD, nx = tiles(M, K, 128), nw = tiles(N, K, 128);
-  double best = x.us + w.us;
-  for (int64_t each = 2; each < 2 * std::max(sx, sw); each *= 2) {
-    const int64_t ex = std::min(each, sx), ew = std::min(each, sw);
-    const int64_t Sx = (sx + ex - 1) / ex, Sw = (sw + ew - 1) / ew;
-    if (Sx > 64 || Sw > 64 || each * GD * std::max(N, K) * 2 >= (1LL << 31)) continue;
-    const double t = SMALL_COST.us((double)(nx * Sx + nw * Sw), (double)std::max(ex, ew)) +
-                     std::max(parts_us(Sx, M * K), parts_us(Sw, N * K));
-    if (t < best) {
-      best = t;
-      x = GradPlan{128, (int)Sx, ex * GD, t};
-      w = GradPlan{128, (int)Sw, ew * GD, t};
+  const int64_t ld = std::max(N, K);
+  double best = 0.97 * (x.us + w.us);
+  auto next = [](int64_t e, int64_t s) { return e == s ? s + 1 : std::min(s, e & (e - 1) ? e / 3 * 4 : e / 2 * 3); };   // 2 3 4 6 8 .. s
+  for (int64_t ex = std::min<int64_t>(2, sx); ex <= sx; ex = next(ex, sx)) {
+    const int64_t Sx = (sx + ex - 1) / ex;
+    if (Sx > 8 || ex * GD * K * 2 >= (1LL << 31)) continue;
+    const double tx = 2 + 0.8 * (double)ex;
+    for (int64_t ew = std::min<int64_t>(2, sw); ew <= sw; ew = next(ew, sw)) {
+      const int64_t Sw = (sw + ew - 1) / ew;
+      if (Sw > 64 || ew * GD * ld * 2 >= (1LL << 31)) continue;
+      const double tw = 2 + 0.8 * (double)ew, ax = (double)(nx * Sx), aw = (double)(nw * Sw);
+      double t = ax + aw <= SMALL_COST.slots
+                     ? SMALL_COST.us(ax + aw, (double)std::max(ex, ew))
+                     : std::max({(ax * tx + aw * tw) / SMALL_COST.slots + 0.35 * std::min(tx, tw), tx, tw});
+      if (Sx > 1 || Sw > 1) t += 4 + (double)((Sx > 1 ? Sx * M * K : 0) + (Sw > 1 ? Sw * N * K : 0)) * 8 / 6e6;
+      if (t < best) {
+        best = t;
+        x = GradPlan{128, (int)Sx, ex * GD, t};
+        w = GradPlan{128, (int)Sw, ew * GD, t};
+      }
     }
   }
+}
+// The plans of both, whichever is asked for: a gradient's bits do not depend on what else is.
+void plan_products(int64_t M, int64_t N, int64_t K, GradPlan& x, GradPlan& w) {
+  x = grad_plan(M, K, N, K);
+  w = grad_plan(N, K, M, std::max(N, K));
+  pair_plan(M, N, K, x, w);
 }
 int64_t plan_bytes(const GradPlan& p, int64_t n) { return p.S > 1 ? (p.S * n * 4 + 255) / 256 * 256 : 0; }
 
 }  // namespace
 
 int64_t grad_products_workspace(int64_t M, int64_t N, int64_t K) {
-  GradPlan x = grad_plan(M, K, N, K), w = grad_plan(N, K, M, std::max(N, K));
-  const int64_t alone = plan_bytes(x, M * K) + plan_bytes(w, N * K);
-  pair_plan(M, N, K, x, w);
-  return std::max(alone, plan_bytes(x, M * K) + plan_bytes(w, N * K));
+  GradPlan x, w;
+  plan_products(M, N, K, x, w);
+  return plan_bytes(x, M * K) + plan_bytes(w, N * K);
 }
 
 // dx [M, K] = dy . w and dw [N, K] = dy^T . x, where not NULL, and the column sums.
 int grad_products(const void* dy, const void* x, const void* w, void* dx, void* dw, const ColumnSums& sums, int64_t M, int64_t N,
                   int64_t K, char* ws, hipStream_t st, const char* what) {
   GradPlan px, pw;
-  if (dx) px = grad_plan(M, K, N, K);
-  if (dw) pw = grad_plan(N, K, M, std::max(N, K));
-  if (dx && dw) pair_plan(M, N, K, px, pw);
+  plan_products(M, N, K, px, pw);
   GradArgs ax{}, aw{};
   ax.x = (const bf16*)dy; ax.w = (const bf16*)w; ax.ldx = N; ax.ldw = K;
   ax.R = (int)M; ax.C = (int)K; ax.D = N; ax.S = px.S; ax.per = px.per;
@@ -437,9 +455,9 @@ int grad_products(const void* dy, const void* x, const void* w, void* dx, void* 
   aw.x = (const bf16*)dy; aw.w = (const bf16*)x; aw.ldx = N; aw.ldw = K;
   aw.R = (int)N; aw.C = (int)K; aw.D = M; aw.S = pw.S; aw.per = pw.per;
   aw.out = pw.S > 1 ? ws + plan_bytes(px, M * K) : dw;
-  NSW_CHECK_ARG(ax.per * K * 2 < (1LL << 31) && (!dx || px.gb * N * 2 < (1LL << 31)) && aw.per * std::max(N, K) * 2 < (1LL << 31),
-                "%s: rows too long (32-bit offsets)", what);
-  const int64_t gx = tiles(M, K, px.gb) * px.S, gw = tiles(N, K, pw.gb) * pw.S, gs = sums.out ? (N + 31) / 32 : 0;
+  NSW_CHECK_ARG((!dx || (ax.per * K * 2 < (1LL << 31) && px.gb * N * 2 < (1LL << 31))) &&
+                    (!dw || aw.per * std::max(N, K) * 2 < (1LL << 31)), "%s: rows too long (32-bit offsets)", what);
+  const int64_t gx = dx ? tiles(M, K, px.gb) * px.S : 0, gw = dw ? tiles(N, K, pw.gb) * pw.S : 0, gs = sums.out ? (N + 31) / 32 : 0;
   NSW_CHECK_ARG(gx + gw + gs < (1LL << 31) - 8, "%s: too many tiles", what);
   if (dx && px.gb == 256) {
     if (px.S > 1) hipLaunchKernelGGL((grad_kernel<false, float>), dim3((unsigned)gx), dim3(512), 0, st, ax);
@@ -451,12 +469,15 @@ int grad_products(const void* dy, const void* x, const void* w, void* dx, void* 
     else hipLaunchKernelGGL((grad_kernel<true, bf16>), dim3((unsigned)gw), dim3(512), 0, st, aw);
     if (int rc = check_launch(what)) return rc;
   }
-  const int nx = dx && px.gb == 128 ? (int)gx : 0, nw = dw && pw.gb == 128 ? (int)((gw + 7) / 8 * 8) : 0;
+  const int64_t nx = px.gb == 128 ? gx : 0, nw = pw.gb == 128 ? gw : 0;
   if (nx + nw + gs > 0) {
-    hipLaunchKernelGGL(grad_small_kernel, dim3((unsigned)(nx + nw + gs)), dim3(256), 0, st, aw, nw, ax, nx, sums, (int)N);
+    const bool dw_first = pw.per >= px.per;
+    const int64_t na = ((dw_first ? nw : nx) + 7) / 8 * 8, nb = dw_first ? nx : nw;
+    hipLaunchKernelGGL(grad_small_kernel, dim3((unsigned)(na + nb + gs)), dim3(256), 0, st, aw, ax, (int)na, (int)nb,
+                       (int)dw_first, sums, (int)N);
     if (int rc = check_launch(what)) return rc;
   }
-  return add_parts(Parts{ax.out, dx, M * K, px.S}, Parts{aw.out, dw, N * K, pw.S}, NSW_DTYPE_BF16, st, what);
+  return add_parts(Parts{ax.out, dx, M * K, dx ? px.S : 0}, Parts{aw.out, dw, N * K, dw ? pw.S : 0}, NSW_DTYPE_BF16, st, what);
 }
 
 }  // namespace nsw

@@ -39,6 +39,7 @@ struct Parts {
   int64_t n;
   int S;
 };
-int add_parts(const Parts& a, const Parts& b, int dtype, hipStream_t st, const char* what);
+// The last launch of a pass: parts of a and b (none where S < 2) and the column sums [N].
+int finish_grads(const Parts& a, const Parts& b, const ColumnSums& sums, int64_t N, int dtype, hipStream_t st, const char* what);
 
 }  // namespace nsw

@@ -1,9 +1,11 @@
 // Gradients of the linear products: dx = dy . w, dw = dy^T . x and db = column sums
 // of dy, for nsw_linear (dy given) and for nsw_gated_linear (dy formed from dh by
-// EPI_GATED_GRAD).  bf16: grad_product, which reads every operand as it lies.  fp32: the
+// EPI_GATED_GRAD).  bf16: grad_products, which reads every operand as it lies.  fp32: the
 // forward GEMM on transposed copies (its operands are split into parts as they pass
 // through LDS, so they cannot be turned there), the batch cut into pieces whose products
-// run side by side and are added in a fixed order.
+// run side by side and are added in a fixed order.  fp32, 16200 rows, 192 -> 768: 287 us
+// in all, of it 83 for the sums formed again and 93 for each product (104 TFLOP/s of fp32
+// in six bf16 products a value).
 #include <algorithm>
 
 #include "nsw_gemm_common.h"
@@ -25,39 +27,64 @@ namespace {
 
 constexpr int NT = 256;
 
-// out[s][c][i] = in[s P + i][c] for in [R, C], pieces of P rows (a multiple of 4),
+// out[s][c][i] = in[s P + i][c] for in [R, C], S pieces of P rows (a multiple of 4),
 // zeros where s P + i >= R.  64 x 64 values through LDS, 16-byte accesses on both sides.
-__global__ __launch_bounds__(NT) void transpose_kernel(const float* __restrict__ in, float* __restrict__ out, int64_t R, int C,
-                                                       int P) {
+struct Turn {
+  const float* in;
+  float* out;
+  int64_t R, S;
+  int C, P;
+  __host__ __device__ int across() const { return (C + 63) / 64; }          // tiles along C
+  __host__ __device__ int down() const { return (P + 63) / 64; }            // and of a piece
+  __host__ __device__ int64_t blocks() const { return S * across() * down(); }
+};
+
+// Of a, then b, then c (blocks() of each; S = 0: none).
+__global__ __launch_bounds__(NT) void transpose_kernel(Turn a, Turn b, Turn c) {
   __shared__ float t[64][65];
-  const int c0 = (int)blockIdx.x * 64;
-  const int tiles = (P + 63) / 64;                     // of a piece
-  const int64_t s = blockIdx.y / (unsigned)tiles;
-  const int i0 = ((int)blockIdx.y - (int)s * tiles) * 64;
+  int64_t id = blockIdx.x;
+  if (id >= a.blocks()) {
+    id -= a.blocks();
+    a = b;
+    if (id >= b.blocks()) {
+      id -= b.blocks();
+      a = c;
+    }
+  }
+  const uint32_t tile = (uint32_t)id / (uint32_t)a.across();
+  const int c0 = (int)((uint32_t)id - tile * (uint32_t)a.across()) * 64, C = a.C, P = a.P;
+  const int64_t s = tile / (uint32_t)a.down();
+  const int i0 = (int)(tile - (uint32_t)s * (uint32_t)a.down()) * 64;
   const int64_t r0 = s * P + i0;
   const int pl = ((int)threadIdx.x & 15) * 4, rw = (int)threadIdx.x >> 4;
 #pragma unroll
   for (int r = rw; r < 64; r += NT / 16) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r0 + r < R && c0 + pl < C) load4<float>(in + (r0 + r) * C + c0 + pl, v);
+    if (r0 + r < a.R && c0 + pl < C) load4<float>(a.in + (r0 + r) * C + c0 + pl, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) t[r][pl + e] = v[e];
   }
   __syncthreads();
 #pragma unroll
-  for (int c = rw; c < 64; c += NT / 16) {
-    if (c0 + c >= C || i0 + pl >= P) continue;
-    const float v[4] = {t[pl][c], t[pl + 1][c], t[pl + 2][c], t[pl + 3][c]};
-    store4<float>(out + (s * C + c0 + c) * P + i0 + pl, v);
+  for (int c_ = rw; c_ < 64; c_ += NT / 16) {
+    if (c0 + c_ >= C || i0 + pl >= P) continue;
+    const float v[4] = {t[pl][c_], t[pl + 1][c_], t[pl + 2][c_], t[pl + 3][c_]};
+    store4<float>(a.out + (s * C + c0 + c_) * P + i0 + pl, v);
   }
 }
 
-// Parts a by the first `na` workgroups, b by the others.
+// Parts a by the first `na` workgroups, b by the next nb, column sums by the others.
 template <typename T>
-__global__ __launch_bounds__(NT) void add_parts_kernel(Parts a, unsigned na, Parts b) {
-  const bool first = blockIdx.x < na;
+__global__ __launch_bounds__(NT) void finish_kernel(Parts a, unsigned na, Parts b, unsigned nb, ColumnSums sums, int N) {
+  __shared__ __attribute__((aligned(16))) float red[32][36];
+  unsigned id = blockIdx.x;
+  if (id >= na + nb) {
+    column_sums_block<T>(sums.part, (T*)sums.out, (int)sums.parts, N, (int)(id - na - nb), red);
+    return;
+  }
+  const bool first = id < na;
   const Parts& p = first ? a : b;
-  const int64_t i = ((int64_t)(first ? blockIdx.x : blockIdx.x - na) * NT + threadIdx.x) * 4;
+  const int64_t i = ((int64_t)(first ? id : id - na) * NT + threadIdx.x) * 4;
   if (i >= p.n) return;
   const float* part = (const float*)p.part + i;
   f32x4 t = {0.f, 0.f, 0.f, 0.f};
@@ -68,7 +95,7 @@ __global__ __launch_bounds__(NT) void add_parts_kernel(Parts a, unsigned na, Par
 }
 
 // part[b][c] = the sum of rows b per .. of x [R, C]: 32 columns to a workgroup, as
-// column_sums_kernel.
+// column_sums_block.
 template <typename T>
 __global__ __launch_bounds__(NT) void column_parts_kernel(const T* __restrict__ x, float* __restrict__ part, int64_t R, int C,
                                                           int64_t per) {
@@ -91,19 +118,6 @@ __global__ __launch_bounds__(NT) void column_parts_kernel(const T* __restrict__ 
     for (int i = 1; i < 32; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
     *reinterpret_cast<f32x4*>(part + (int64_t)blockIdx.y * C + c) = t;
   }
-}
-
-__global__ __launch_bounds__(NT) void column_sums_kernel(const float* __restrict__ part, float* __restrict__ out, int P, int C) {
-  __shared__ __attribute__((aligned(16))) float red[32][36];
-  column_sums_block<float>(part, out, P, C, (int)blockIdx.x, red);
-}
-
-int transpose(const void* in, void* out, int64_t R, int64_t C, int64_t S, int64_t P, hipStream_t st, const char* what) {
-  const int64_t gy = S * ((P + 63) / 64);
-  NSW_CHECK_ARG(gy < 65536, "%s: too many rows", what);
-  hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((C + 63) / 64), (unsigned)gy), dim3(NT), 0, st, (const float*)in,
-                     (float*)out, R, (int)C, (int)P);
-  return check_launch(what);
 }
 
 int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -132,7 +146,7 @@ void split_f32(int64_t R, int64_t C, int64_t D, int64_t step, int64_t most, int6
 
 // Workspace of the two products and the column sums.
 struct GradSpace {
-  int64_t S = 1, P = 0, Sx = 1, Px = 0, wt = 0, dyt = 0, xt = 0, prod = 0, part = 0, bytes = 0;
+  int64_t S = 1, P = 0, Sx = 1, Px = 0, wt = 0, dyt = 0, xt = 0, prodx = 0, prodw = 0, part = 0, bytes = 0;
   GradSpace(int64_t M, int64_t N, int64_t K, int64_t parts, int dtype) {
     if (dtype == NSW_DTYPE_F32) {
       // dw: none whose transposed rows pass the GEMM's 2 GiB; dx: whole, where its rows
@@ -143,8 +157,9 @@ struct GradSpace {
       wt = 0;                                          // w^T
       dyt = wt + align256(N * K * 4);                  // dy^T and x^T in pieces
       xt = dyt + align256(S * N * P * 4);
-      prod = xt + align256(S * K * P * 4);             // their products
-      part = prod + align256(std::max(S > 1 ? S * N * K * 4 : 0, Sx > 1 ? Sx * M * K * 4 : 0));
+      prodx = xt + align256(S * K * P * 4);            // their products
+      prodw = prodx + align256(Sx > 1 ? Sx * M * K * 4 : 0);
+      part = prodw + align256(S > 1 ? S * N * K * 4 : 0);
     } else {
       part = grad_products_workspace(M, N, K);
     }
@@ -162,51 +177,57 @@ bool bad_gated_sizes(int64_t M, int64_t H, int64_t K, int dtype) {
   return H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype);
 }
 
-int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, void* dw, int64_t M, int64_t N, int64_t K,
-                     const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
-  int rc = NSW_OK;
+// fp32: three launches beside the products, transposes, parts with the column sums (each
+// alone costs its own few us: 16200 rows, 192 -> 768, transposes 6.3 us three times).
+int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, void* dw, const ColumnSums& sums, int64_t M,
+                     int64_t N, int64_t K, const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
+  auto f = [&](int64_t at) { return (float*)(ws + at); };
+  Turn tw{}, ty{}, tx{};
+  if (dx) tw = Turn{(const float*)w, f(sp.wt), N, 1, (int)K, (int)N};
+  if (dw) {
+    ty = Turn{(const float*)dy, f(sp.dyt), M, sp.S, (int)N, (int)sp.P};
+    tx = Turn{(const float*)x, f(sp.xt), M, sp.S, (int)K, (int)sp.P};
+  }
+  const int64_t turns = tw.blocks() + ty.blocks() + tx.blocks();
+  NSW_CHECK_ARG(turns < (1LL << 31), "%s: too many rows", what);
+  if (turns > 0) {
+    hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)turns), dim3(NT), 0, st, tw, ty, tx);
+    if (int rc = check_launch(what)) return rc;
+  }
+  char* px = sp.Sx > 1 ? ws + sp.prodx : dx;              // Sx > 1 only where M is small: one piece of rows
   if (dx) {
-    if ((rc = transpose(w, ws + sp.wt, N, K, 1, N, st, what))) return rc;
     // as many rows at a time as the GEMM's 2 GiB hold
     const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4));
-    char* out = sp.Sx > 1 ? ws + sp.prod : dx;            // Sx > 1 only where M is small: one piece of rows
     for (int64_t m = 0; m < M; m += rows)
-      if ((rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, out + m * K * 4, std::min(rows, M - m), K, sp.Px, N, N, sp.Px,
-                               sp.Px, (int)sp.Sx, st, what)))
+      if (int rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, px + m * K * 4, std::min(rows, M - m), K, sp.Px, N, N, sp.Px,
+                                  sp.Px, (int)sp.Sx, st, what))
         return rc;
-    if (sp.Sx > 1 && (rc = add_parts(Parts{out, dx, M * K, (int)sp.Sx}, Parts{}, NSW_DTYPE_F32, st, what))) return rc;
   }
-  if (dw) {
-    if ((rc = transpose(dy, ws + sp.dyt, M, N, sp.S, sp.P, st, what))) return rc;
-    if ((rc = transpose(x, ws + sp.xt, M, K, sp.S, sp.P, st, what))) return rc;
-    void* out = sp.S > 1 ? ws + sp.prod : dw;
-    if ((rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, out, N, K, sp.P, sp.S * sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st,
-                             what)))
+  void* pw = sp.S > 1 ? ws + sp.prodw : dw;
+  if (dw)
+    if (int rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, pw, N, K, sp.P, sp.S * sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st,
+                                what))
       return rc;
-    if (sp.S > 1) rc = add_parts(Parts{out, dw, N * K, (int)sp.S}, Parts{}, NSW_DTYPE_F32, st, what);
-  }
-  return rc;
+  return finish_grads(Parts{px, dx, M * K, dx ? (int)sp.Sx : 0}, Parts{pw, dw, N * K, dw ? (int)sp.S : 0}, sums, N,
+                      NSW_DTYPE_F32, st, what);
 }
 
 int linear_grads(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t parts, int64_t M,
                  int64_t N, int64_t K, int dtype, const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
   const ColumnSums sums{(const float*)(ws + sp.part), db, parts};
-  if (dtype == NSW_DTYPE_BF16) return grad_products(dy, x, w, dx, dw, sums, M, N, K, ws, st, what);
-  if (int rc = linear_grads_f32((const char*)dy, x, w, (char*)dx, dw, M, N, K, sp, ws, st, what)) return rc;
-  if (!db) return NSW_OK;
-  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((N + 31) / 32)), dim3(NT), 0, st, sums.part, (float*)db, (int)parts,
-                     (int)N);
-  return check_launch(what);
+  return dtype == NSW_DTYPE_BF16 ? grad_products(dy, x, w, dx, dw, sums, M, N, K, ws, st, what)
+                                 : linear_grads_f32((const char*)dy, x, w, (char*)dx, dw, sums, M, N, K, sp, ws, st, what);
 }
 
 }  // namespace
 
-int add_parts(const Parts& a, const Parts& b, int dtype, hipStream_t st, const char* what) {
+int finish_grads(const Parts& a, const Parts& b, const ColumnSums& sums, int64_t N, int dtype, hipStream_t st, const char* what) {
   auto blocks = [](const Parts& p) { return p.S > 1 ? (unsigned)((p.n / 4 + NT - 1) / NT) : 0u; };
-  const unsigned na = blocks(a), nb = blocks(b);
-  if (na + nb == 0) return NSW_OK;
-  if (dtype == NSW_DTYPE_BF16) hipLaunchKernelGGL((add_parts_kernel<bf16>), dim3(na + nb), dim3(NT), 0, st, a, na, b);
-  else hipLaunchKernelGGL((add_parts_kernel<float>), dim3(na + nb), dim3(NT), 0, st, a, na, b);
+  const unsigned na = blocks(a), nb = blocks(b), ns = sums.out ? (unsigned)((N + 31) / 32) : 0u;
+  if (na + nb + ns == 0) return NSW_OK;
+  const dim3 grid(na + nb + ns);
+  if (dtype == NSW_DTYPE_BF16) hipLaunchKernelGGL((finish_kernel<bf16>), grid, dim3(NT), 0, st, a, na, b, nb, sums, (int)N);
+  else hipLaunchKernelGGL((finish_kernel<float>), grid, dim3(NT), 0, st, a, na, b, nb, sums, (int)N);
   return check_launch(what);
 }
 

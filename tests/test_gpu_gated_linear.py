@@ -169,6 +169,25 @@ def test_linear_backward(device, dtype, M, N, K):
     assert one[0] is None and one[2] is None and torch.equal(one[1], dw)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 1024, 32), (1, 4096, 64), (1000, 160, 32), (2000, 4096, 1024), (3000, 4096, 512),
+                                   (8000, 2080, 160), (16200, 4096, 1024)])
+def test_gradients_side_by_side(device, M, N, K):
+    """bf16: dx, dw and db in one launch or after one another, whole or in parts, the longer parts first; and the same bits
+    whichever of them are asked for."""
+    from nsw import ops
+    g = torch.Generator().manual_seed(N)
+    dy, x = (torch.randn(M, n, generator=g).to(device, BF16) for n in (N, K))
+    w = (torch.randn(N, K, generator=g) * K ** -0.5).to(device, BF16)
+    got = dict(zip(("dx", "dw", "db"), ops.linear_backward(dy, x, w)))
+    d, xx, ww = dy.double(), x.double(), w.double()
+    want = {"dx": (d @ ww, (d.abs() @ ww.abs()) * (N + 8) * U), "dw": (d.t() @ xx, (d.abs().t() @ xx.abs()) * (M + 8) * U),
+            "db": (d.sum(0), d.abs().sum(0) * 512 * U)}
+    check(got, want, BF16)
+    for needs in ((True, False, False), (False, True, True), (True, False, True), (False, False, True)):
+        for n, t in zip(got, ops.linear_backward(dy, x, w, needs=needs)):
+            assert t is None or torch.equal(t, got[n]), (needs, n)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_no_rows(device, dtype):
     from nsw import ops

@@ -7,6 +7,7 @@ all arithmetic runs in libnsw's kernels).  Inputs must be contiguous,
 """
 from __future__ import annotations
 
+import functools
 import threading
 from typing import Optional, Sequence, Tuple
 
@@ -51,12 +52,14 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-# the current stream's handle without a Stream object around it (0.1 us, not 1.9)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# the current stream's handle without a Stream object around it (0.1 us, not 1.9), and
+# the current device's index without the check that the GPU is initialised
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream(dev: torch.device):
-    if _raw_stream is not None and dev.index is not None:
+    if dev.index is not None:
         return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -189,36 +192,53 @@ def rmsnorm_roll_partition(x: torch.Tensor, weight: torch.Tensor, window_size, s
     return out
 
 
-def _uniform(*ts: Optional[torch.Tensor]) -> torch.device:
-    """The device of ts (the first is given) after the checks of _dev and
-    _same_dtype, which raise what is found."""
-    ref = ts[0]
-    dev, dt = ref.device, ref.dtype
+def _at(*ts: Optional[torch.Tensor]) -> int:
+    """Index of the device of ts (the first is given) after the checks of _dev, which raises what is found."""
+    at = ts[0].get_device()
     for t in ts:
-        if t is not None and (t.dtype != dt or t.device != dev or not t.is_contiguous()):
+        if t is not None and (t.get_device() != at or not t.is_contiguous()):
             break
     else:
-        if ref.is_cuda:
-            return dev
+        if at >= 0:
+            return at
     _dev(*ts)
-    _same_dtype(ref, *ts)
-    return dev
+    return at
 
 
-def _run(what: str, dev: torch.device, fn, *args) -> None:
-    """fn(*args, stream) with dev as the current device, its error raised."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _stream(dev))
+def _uniform(*ts: Optional[torch.Tensor]) -> int:
+    """_at of ts after _same_dtype, too."""
+    at, dt = ts[0].get_device(), ts[0].dtype
+    for t in ts:
+        if t is not None and (t.dtype is not dt or t.get_device() != at or not t.is_contiguous()):
+            break
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _stream(dev))
+        if at >= 0:
+            return at
+    _dev(*ts)
+    _same_dtype(ts[0], *ts)
+    return at
+
+
+def _run(what: str, at: int, fn, *args) -> None:
+    """fn(*args, stream) with device ``at`` as the current one, its error raised."""
+    if _current_index() == at:
+        rc = fn(*args, _raw_stream(at))
+    else:
+        with torch.cuda.device(at):
+            rc = fn(*args, _raw_stream(at))
     if rc:
         check(rc, what)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(handle, name, *sizes) -> int:
+    """The library's answer for these sizes (0.2 us, not up to 3)."""
+    return int(getattr(handle, name)(*sizes))
+
+
 def _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps):
-    """(device, rows, C, G, eps) of a residual_norm, its arguments checked."""
-    dev = _uniform(branch, skip, post_weight, gate, norm_weight)
+    """(device index, rows, C, G, eps) of a residual_norm, its arguments checked."""
+    at = _uniform(branch, skip, post_weight, gate, norm_weight)
     shape = branch.shape
     if not shape or shape != skip.shape:
         raise ValueError(f"{what}: branch {tuple(branch.shape)} and skip {tuple(skip.shape)} must have one shape")
@@ -237,7 +257,7 @@ def _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps)
         G = gate.numel() // C
         if rows % G:
             raise ValueError(f"{what}: {rows} rows are not a multiple of the gate's {G}")
-    return dev, rows, C, G, default_eps(branch.dtype) if eps is None else float(eps)
+    return at, rows, C, G, default_eps(branch.dtype) if eps is None else float(eps)
 
 
 def residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
@@ -250,10 +270,10 @@ def residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optiona
     the branch is not normalised; gate [C] (a layer scale) or [G, C], the rows
     of G equal parts of the batch each under their own gate, None: 1;
     norm_weight None: z is None.  Statistics, and z's y, in fp32."""
-    dev, rows, C, G, eps = _residual_norm_args("residual_norm", branch, skip, post_weight, gate, norm_weight, eps)
+    at, rows, C, G, eps = _residual_norm_args("residual_norm", branch, skip, post_weight, gate, norm_weight, eps)
     y = torch.empty_like(branch)
     z = None if norm_weight is None else torch.empty_like(branch)
-    _run("residual_norm", dev, lib().nsw_residual_norm, branch.data_ptr(), skip.data_ptr(), _p(post_weight), _p(gate),
+    _run("residual_norm", at, lib().nsw_residual_norm, branch.data_ptr(), skip.data_ptr(), _p(post_weight), _p(gate),
          _p(norm_weight), y.data_ptr(), _p(z), rows, C, G, float(alpha), eps, dtype_code(branch))
     return y, z
 
@@ -266,18 +286,15 @@ def residual_norm_backward(dy: Optional[torch.Tensor], dz: Optional[torch.Tensor
     the gradients of y and z, None for what was None.  dy or dz may be None
     (zero)."""
     what = "residual_norm_backward"
-    dev, rows, C, G, eps = _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps)
+    at, rows, C, G, eps = _residual_norm_args(what, branch, skip, post_weight, gate, norm_weight, eps)
     if dy is None and dz is None:
         raise ValueError(f"{what}: dy or dz is required")
     if dz is not None and norm_weight is None:
         raise ValueError(f"{what}: dz without norm_weight")
+    _uniform(branch, dy, dz)
     for t in (dy, dz):
-        if t is not None:
-            if _dev(t) != dev:
-                raise RuntimeError("libnsw op arguments are on different devices")
-            _same_dtype(branch, t)
-            if t.shape != branch.shape:
-                raise ValueError(f"{what}: gradient of shape {tuple(t.shape)}, expected {tuple(branch.shape)}")
+        if t is not None and t.shape != branch.shape:
+            raise ValueError(f"{what}: gradient of shape {tuple(t.shape)}, expected {tuple(branch.shape)}")
     db, ds = torch.empty_like(branch), torch.empty_like(branch)
     dp = None if post_weight is None else torch.empty_like(post_weight)
     dg = None if gate is None else torch.empty_like(gate)
@@ -285,9 +302,9 @@ def residual_norm_backward(dy: Optional[torch.Tensor], dz: Optional[torch.Tensor
     dn = None if norm_weight is None else torch.zeros_like(norm_weight) if dz is None else torch.empty_like(norm_weight)
     nw = None if dz is None else norm_weight
     code = dtype_code(branch)
-    nbytes = int(lib().nsw_residual_norm_backward_workspace_size(rows, C, G, code))
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    _run(what, dev, lib().nsw_residual_norm_backward, _p(dy), _p(dz), branch.data_ptr(), skip.data_ptr(),
+    nbytes = _workspace_bytes(lib(), "nsw_residual_norm_backward_workspace_size", rows, C, G, code)
+    ws = branch.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run(what, at, lib().nsw_residual_norm_backward, _p(dy), _p(dz), branch.data_ptr(), skip.data_ptr(),
          _p(post_weight), _p(gate), _p(nw), db.data_ptr(), ds.data_ptr(), _p(dp), _p(dg), None if dz is None else _p(dn),
          rows, C, G, float(alpha), eps, code, ws.data_ptr(), nbytes)
     return db, ds, dp, dg, dn
@@ -327,8 +344,8 @@ _ACTS = {"silu": _lib.NSW_ACT_SILU, "gelu": _lib.NSW_ACT_GELU, "gelu_tanh": _lib
 
 
 def _gated_args(what, x, weight, bias, act):
-    """(device, M, H, K, act code) of a gated linear, its arguments checked."""
-    dev = _uniform(x, weight, bias)
+    """(device index, M, H, K, act code) of a gated linear, its arguments checked."""
+    at = _uniform(x, weight, bias)
     if act not in _ACTS:
         raise ValueError(f"{what}: act must be one of {sorted(_ACTS)}, got {act!r}")
     shape, wshape = x.shape, weight.shape
@@ -339,7 +356,7 @@ def _gated_args(what, x, weight, bias, act):
         raise ValueError(f"{what}: no features")
     if bias is not None and bias.shape != (2 * H,):
         raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({2 * H},)")
-    return dev, x.numel() // K, H, K, _ACTS[act]
+    return at, x.numel() // K, H, K, _ACTS[act]
 
 
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -348,11 +365,11 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     activation and the product of a gated feed-forward block in one kernel.
     weight [2H, K] stacks Wg over Wu, bias [2H] bg over bu; act "silu",
     "gelu" (exact erf) or "gelu_tanh"."""
-    dev, M, H, K, code = _gated_args("gated_linear", x, weight, bias, act)
+    at, M, H, K, code = _gated_args("gated_linear", x, weight, bias, act)
     h = x.new_empty(x.shape[:-1] + (H,))
     if M == 0:
         return h
-    _run("gated_linear", dev, lib().nsw_gated_linear, x.data_ptr(), weight.data_ptr(), _p(bias), h.data_ptr(), M, H, K,
+    _run("gated_linear", at, lib().nsw_gated_linear, x.data_ptr(), weight.data_ptr(), _p(bias), h.data_ptr(), M, H, K,
          code, dtype_code(x))
     return h
 
@@ -369,18 +386,16 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     ``needs`` says so or there is no bias.  The projections are formed again
     from x and weight."""
     what = "gated_linear_backward"
-    dev, M, H, K, code = _gated_args(what, x, weight, bias, act)
-    if _dev(dh) != dev:
-        raise RuntimeError("libnsw op arguments are on different devices")
-    _same_dtype(x, dh)
+    at, M, H, K, code = _gated_args(what, x, weight, bias, act)
+    _uniform(x, dh)
     if dh.shape != x.shape[:-1] + (H,):
         raise ValueError(f"{what}: dh has shape {tuple(dh.shape)}, expected {tuple(x.shape[:-1]) + (H,)}")
     dx, dw, db = _grads(needs, x, weight, bias)
     if M == 0:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    nbytes = int(lib().nsw_gated_linear_backward_workspace_size(M, H, K, dtype_code(x)))
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    _run(what, dev, lib().nsw_gated_linear_backward, dh.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(dx),
+    nbytes = _workspace_bytes(lib(), "nsw_gated_linear_backward_workspace_size", M, H, K, dtype_code(x))
+    ws = x.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run(what, at, lib().nsw_gated_linear_backward, dh.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(dx),
          _p(dw), _p(db), M, H, K, code, dtype_code(x), ws.data_ptr(), nbytes)
     return dx, dw, db
 
@@ -390,8 +405,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     """(dx, dweight, dbias) = (dy W, dy^T x, column sums of dy) of linear without
     an activation, None where ``needs`` says so."""
     what = "linear_backward"
-    dev = _dev(dy, x, weight)
-    _same_dtype(x, dy, weight)
+    at = _uniform(x, dy, weight)
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or dy.shape != x.shape[:-1] + weight.shape[:1]:
         raise ValueError(f"{what}: dy {tuple(dy.shape)}, x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     N, K = weight.shape
@@ -399,12 +413,12 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         raise ValueError(f"{what}: no features")
     M = x.numel() // K
     dx, dw = _grads(needs, x, weight)
-    db = torch.empty(N, dtype=x.dtype, device=dev) if needs[2] else None
+    db = x.new_empty(N) if needs[2] else None
     if M == 0:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    nbytes = int(lib().nsw_linear_backward_workspace_size(M, N, K, dtype_code(x)))
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    _run(what, dev, lib().nsw_linear_backward, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(dx), _p(dw), _p(db), M,
+    nbytes = _workspace_bytes(lib(), "nsw_linear_backward_workspace_size", M, N, K, dtype_code(x))
+    ws = x.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run(what, at, lib().nsw_linear_backward, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(dx), _p(dw), _p(db), M,
          N, K, dtype_code(x), ws.data_ptr(), nbytes)
     return dx, dw, db
 
@@ -418,7 +432,7 @@ def quantize_fp8(x: torch.Tensor, rows: int = 1) -> Tuple[torch.Tensor, torch.Te
     for each block of ``rows`` x 128 values: rows=1 for activations (scale
     [..., Kp / 128]), rows=128 for a weight matrix [N, K] (scale
     [ceil(N / 128), Kp / 128])."""
-    dev = _dev(x)
+    at = _at(x)
     if rows not in (1, FP8_BLOCK):
         raise ValueError(f"quantize_fp8: rows must be 1 or {FP8_BLOCK}, got {rows}")
     if x.dim() < 1 or x.shape[-1] == 0 or (rows != 1 and x.dim() != 2):
@@ -431,7 +445,7 @@ def quantize_fp8(x: torch.Tensor, rows: int = 1) -> Tuple[torch.Tensor, torch.Te
     q = x.new_empty(lead + (Kb * FP8_BLOCK,), dtype=torch.float8_e4m3fn)
     scale = x.new_empty((lead if rows == 1 else ((R + rows - 1) // rows,)) + (Kb,), dtype=torch.float8_e8m0fnu)
     if R:
-        _run("quantize_fp8", dev, lib().nsw_quantize_fp8, x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, rows, code)
+        _run("quantize_fp8", at, lib().nsw_quantize_fp8, x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, rows, code)
     return q, scale
 
 
@@ -442,7 +456,7 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     rows=128): y [..., N] in ``dtype`` (bfloat16 or float32; bias and residual
     in it too), the epilogues of linear, sums in fp32."""
     what = "linear_fp8"
-    dev = _dev(xq, x_scale, wq, w_scale, bias, residual)
+    at = _at(xq, x_scale, wq, w_scale, bias, residual)
     if dtype not in _DTYPES:
         raise TypeError(f"{what}: the result is float32 or bfloat16, got {dtype}")
     if (xq.dtype != torch.float8_e4m3fn or wq.dtype != torch.float8_e4m3fn or x_scale.dtype != torch.float8_e8m0fnu
@@ -472,7 +486,7 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     if residual is not None and residual.shape != y.shape:
         raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")
     if y.numel():
-        _run(what, dev, lib().nsw_linear_fp8, xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
+        _run(what, at, lib().nsw_linear_fp8, xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
              _p(bias), _p(residual), y.data_ptr(), xq.numel() // K, N, K, int(epilogue), _DTYPES[dtype])
     return y
 

@@ -111,6 +111,14 @@ def test_large_tiles(device, dtype, M, K, H):
     check(run(t, "silu"), reference(t, "silu"), dtype)
 
 
+@pytest.mark.parametrize("dtype,M,K,H", [(BF16, 4100, 256, 2048), (BF16, 2600, 512, 4096), (BF16, 12961, 512, 1360),
+                                         (F32, 4100, 256, 4096), (F32, 6000, 512, 2048)])
+def test_rows_in_two_launches(device, dtype, M, K, H):
+    """Whole rounds of large tiles, then the rest: few rows (4 of 4100) and many."""
+    t = case(device, dtype, M, K, H, True, seed=9)
+    check(run(t, "gelu_tanh"), reference(t, "gelu_tanh"), dtype)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("needs", [(True, False, False), (False, True, False), (False, False, True)])
 def test_gradients_on_their_own(device, dtype, needs):

@@ -35,7 +35,6 @@ static TileSize pick_tile(int64_t M, int64_t N, int64_t K, const EpiArgs& ea, do
   using C = TileChoice<T, EPI>;
   constexpr bool F32 = sizeof(T) == 4;
   if (EPI == EPI_UNPATCH && ea.img_p == 16) return TILE_BIG;   // a patch of one channel is 256 columns
-  if (EPI == EPI_BATCH) M *= ea.batch;                         // side by side
   constexpr TileCost big = F32 ? TileCost{256, 256, 256, 18, .0795, 9.5, .0605, 0} : TileCost{256, 256, 256, 8.5, .0234, 5.5, .015, 0};
   constexpr TileCost mid = F32 ? TileCost{C::Mid::BM, C::Mid::BN, 512, 8, .0537, 6, .0324, .4}
                                : TileCost{C::Mid::BM, C::Mid::BN, 512, 4.5, .0152, 3.6, .0088, .4};
@@ -273,26 +272,50 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
                : tile_parts(M, H, K, dtype);
 }
 
-// fp32 y[s] [M, N] = x[s] . w[s]^T for s < batch: product s contracts values [s K, (s + 1)
-// K) of kall in all (a multiple of 16; the last may be shorter), rows are ld values apart
-// (a multiple of 4), the products' operands xs and ws values apart, the results one after
-// the other.
-int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t kall, int64_t ld,
-                   int64_t xs, int64_t ws, int batch, hipStream_t st, const char* what) {
-  NSW_CHECK_ARG(batch > 0 && batch < 65536 && kall <= batch * K && kall > (batch - 1) * K && kall % 16 == 0,
-                "%s: %d products of %lld for %lld", what, batch, (long long)K, (long long)kall);
-  NSW_CHECK_ARG((uint64_t)std::max(M, N) * ld * 4 < (1ULL << 31), "%s: operands above 2 GiB are not supported", what);
-  EpiArgs ea{};
-  ea.batch = batch; ea.ld = (int)ld; ea.xs = xs; ea.ws = ws; ea.kall = kall;
-  return launch_gemm<float, EPI_BATCH, PRE_NONE>(x, w, y, M, N, K, ea, st, what);
+// Estimated time (us) of one or two families of fp32 products side by side, and the tile
+// for them.  As pick_tile, with the k loop on three parts from its start (FB_FIT); more
+// workgroups than slots: their times shared out, and 0.35 of the shorter one at the end.
+double gemm_f32_pair_us(const BatchOf& a, const BatchOf& b, int& tile) {
+  constexpr double q = 1.7;
+  constexpr TileCost costs[3] = {{256, 256, 256, 18, .0795 * q, 9.5, .0605 * q, 0},
+                                 {MidTile::BM, MidTile::BN, 512, 8, .0537 * q, 6, .0324 * q, .4},
+                                 {SmallF32Tile::BM, SmallF32Tile::BN, 768, 5, .051 * q, 4.3, .0252 * q, .3}};
+  double best = 0;
+  for (int i = 0; i < 3; ++i) {
+    const TileCost& c = costs[i];
+    auto count = [&](const BatchOf& p) { return (double)(((p.M + c.bm - 1) / c.bm) * ((p.N + c.bn - 1) / c.bn) * p.batch); };
+    const double na = count(a), nb = count(b), ta = c.fa + c.fb * (double)a.K, tb = nb > 0 ? c.fa + c.fb * (double)b.K : ta;
+    const double most = (double)std::max(a.K, nb > 0 ? b.K : 0), f = (na + nb) / c.slots;
+    const double part = c.pa + c.pb * most, full = c.fa + c.fb * most;
+    const double us = f <= 1 ? part + std::max(0.0, f - c.f0) / (1 - c.f0) * (full - part)
+                             : std::max((na * ta + nb * tb) / c.slots + 0.35 * std::min(ta, tb), full);
+    if (i == 0 || us < (tile == TILE_BIG ? 0.93 : 1.0) * best) {
+      best = us;
+      tile = i;
+    }
+  }
+  return best;
 }
-// Its estimated time (us).
-double gemm_f32_batch_us(int64_t M, int64_t N, int64_t K, int batch) {
+
+// fp32: the products of a, and beside them those of b.
+int gemm_f32_pair(const BatchOf& a, const BatchOf& b, int tile, hipStream_t st, const char* what) {
   EpiArgs ea{};
-  ea.batch = batch;
-  double us = 0;
-  pick_tile<float, EPI_BATCH>(M, N, K, ea, &us);
-  return us;
+  int n = 0;
+  for (const BatchOf* p : {&a, &b}) {
+    if (p->batch == 0) continue;
+    NSW_CHECK_ARG(p->batch < 65536 && p->kall <= p->batch * p->K && p->kall > (p->batch - 1) * p->K && p->kall % 16 == 0,
+                  "%s: %lld products of %lld for %lld", what, (long long)p->batch, (long long)p->K, (long long)p->kall);
+    NSW_CHECK_ARG((uint64_t)std::max(p->M, p->N) * p->ld * 4 < (1ULL << 31) && p->M < (1LL << 31) && p->N < (1LL << 31),
+                  "%s: operands above 2 GiB are not supported", what);
+    ea.pair[n++] = *p;
+  }
+  if (n == 0) return NSW_OK;
+  static_assert(TILE_BIG == 0 && TILE_MID == 1 && TILE_SMALL == 2, "costs by tile");
+  switch (tile) {
+    case TILE_BIG: return launch_tile<float, EPI_BATCH, PRE_NONE, BigTile>(a.x, a.w, a.y, 0, 0, 0, ea, st, what);
+    case TILE_MID: return launch_tile<float, EPI_BATCH, PRE_NONE, MidTile>(a.x, a.w, a.y, 0, 0, 0, ea, st, what);
+    default: return launch_tile<float, EPI_BATCH, PRE_NONE, SmallF32Tile>(a.x, a.w, a.y, 0, 0, 0, ea, st, what);
+  }
 }
 
 // y[remap(m)] = x[m] . w^T + bias + residual[m], the stored rows' partial

@@ -23,7 +23,7 @@ enum Epi {
   EPI_GATED = 17,            // w stacks gate and up rows [2H, K]: y[m, h] = act(g) u, optional bias [2H]
   EPI_GATED_GRAD = 18,       // the same product formed again: y[M, 2H] = the gradients of g and u from
                              // that of act(g) u (residual), optional column sums into row_sumsq
-  EPI_BATCH = 19,            // no bias; blockIdx.y products, their operands' rows ea.ld values apart
+  EPI_BATCH = 19,            // no bias; the products of ea.pair instead of the kernel's own operands
   EPI_QKV_HN16 = 16,         // bias, then per-head RMSNorm of the q and k
   EPI_QKV_HN32 = 32,         // columns, for head dims 16 / 32 / 64
   EPI_QKV_HN64 = 64,
@@ -46,6 +46,16 @@ constexpr int qkv_head_dim(int epi) {
          : epi == EPI_QKV_HN4 ? 4 : epi == EPI_QKV_HN8 ? 8 : 0;
 }
 
+// `batch` products y[s] [M, N] = x[s] . w[s]^T (0: none): product s contracts values [s K,
+// (s + 1) K) of kall in all (a multiple of 16; the last may be shorter), rows are ld values
+// apart (a multiple of 4), the products' operands xs and ws values apart, the results one
+// after the other.
+struct BatchOf {
+  const void *x, *w;
+  void* y;
+  int64_t M, N, K, batch, kall, ld, xs, ws;
+};
+
 struct EpiArgs {
   const void* bias;
   const void* residual;
@@ -66,8 +76,7 @@ struct EpiArgs {
   int64_t img_bstride;
   int img_C, img_H, img_W, img_p, img_f32;
   int act;      // EPI_GATED, EPI_GATED_GRAD: NSW_ACT_*
-  int batch, ld;  // EPI_BATCH: products, and values between an operand's rows
-  int64_t xs, ws, kall; // EPI_BATCH: values between the products' operands; the contraction of all products
+  BatchOf pair[2];  // EPI_BATCH
 };
 
 // GELU with the exact-erf form of nn.GELU(): 0.5 v (1 + erf(v / sqrt 2)).

@@ -1123,6 +1123,27 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave / WGN, wn = wave % WGN;
 
+  int bid = (int)blockIdx.x, ld = K;               // values between rows of x and of w
+  if constexpr (EPI == EPI_BATCH) {                // the products of pair[0], then those of pair[1]
+    auto tiles = [](const BatchOf& b) { return ((int)b.M + BM - 1) / BM * (((int)b.N + BN - 1) / BN); };
+    int n = tiles(ea.pair[0]);
+    const bool second = bid >= n * (int)ea.pair[0].batch;
+    const BatchOf& b = ea.pair[second ? 1 : 0];
+    if (second) {
+      bid -= n * (int)ea.pair[0].batch;
+      n = tiles(b);
+    }
+    const int piece = bid / n;
+    bid -= piece * n;
+    M = (int)b.M;
+    N = (int)b.N;
+    ld = (int)b.ld;
+    X = (const T*)b.x + piece * b.xs;
+    Wt = (const T*)b.w + piece * b.ws;
+    Y = (T*)b.y + piece * b.M * b.N;
+    const int64_t left = b.kall - piece * b.K;
+    K = (int)(left < b.K ? left : b.K);
+  }
   const int MT = (M + BM - 1) / BM, NT = (N + BN - 1) / BN;
   // Tiles of one XCD run in groups of GROUP_M row blocks x all column blocks,
   // column-major inside the group, so that the tiles in flight on an XCD
@@ -1130,7 +1151,7 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   // (ea.group_m 256-row blocks when set: 4 for the QKV projection and 16 for
   // proj, each measured 1.5-3% faster there; fc1 is fastest at 8)
   const int GM = (ea.group_m > 0 ? ea.group_m : GROUP_M) * (256 / BM);
-  const int tile = xcd_remap(blockIdx.x, MT * NT);
+  const int tile = xcd_remap(bid, MT * NT);
   const int group = tile / (GM * NT);
   const int gm0 = group * GM;
   const int gsz = MT - gm0 < GM ? MT - gm0 : GM;
@@ -1139,14 +1160,6 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   const int m0 = mt * BM, n0 = nt * BN;
   // the tile's rows of x; GATE: addressed from the tile's first one, so that x may
   // be larger than the 32-bit offsets reach
-  if constexpr (EPI == EPI_BATCH) {
-    X += (int64_t)blockIdx.y * ea.xs;
-    Wt += (int64_t)blockIdx.y * ea.ws;
-    Y += (int64_t)blockIdx.y * M * N;
-    const int64_t left = ea.kall - (int64_t)blockIdx.y * K;
-    K = left < K ? (int)left : K;
-  }
-  const int ld = EPI == EPI_BATCH ? ea.ld : K;     // values between rows of x and of w
   const T* Xt = GATE ? X + (int64_t)m0 * K : X;
   const int Mt = GATE ? (M - m0 < BM ? M - m0 : BM) : M, mt0 = GATE ? 0 : m0;
 
@@ -1673,9 +1686,12 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
 template <typename T, int EPI, int PRE, class TC>
 int launch_tile(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, const EpiArgs& ea,
                        hipStream_t st, const char* what) {
-  const int64_t tiles = ((M + TC::BM - 1) / TC::BM) * ((N + TC::BN - 1) / TC::BN);
+  auto count = [](int64_t m, int64_t n) { return ((m + TC::BM - 1) / TC::BM) * ((n + TC::BN - 1) / TC::BN); };
+  int64_t tiles = count(M, N);
+  if constexpr (EPI == EPI_BATCH)
+    tiles = count(ea.pair[0].M, ea.pair[0].N) * ea.pair[0].batch + count(ea.pair[1].M, ea.pair[1].N) * ea.pair[1].batch;
   NSW_CHECK_ARG(tiles < (1LL << 31), "%s: too many tiles", what);
-  hipLaunchKernelGGL((gemm_kernel<T, EPI, PRE, TC>), dim3((unsigned)tiles, EPI == EPI_BATCH ? (unsigned)ea.batch : 1u), dim3(TC::NW * 64), 0, st, (const T*)x,
+  hipLaunchKernelGGL((gemm_kernel<T, EPI, PRE, TC>), dim3((unsigned)tiles), dim3(TC::NW * 64), 0, st, (const T*)x,
                      (const T*)w, (T*)y, (int)M, (int)N, (int)K, ea);
   return check_launch(what);
 }

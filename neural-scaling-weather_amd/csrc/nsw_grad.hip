@@ -16,9 +16,8 @@ namespace nsw {
 int gemm_gated(const void* x, const void* w, const void* bias, const void* dh, void* y, float* colsum, int64_t M,
                int64_t H, int64_t K, int act, int dtype, void* stream, const char* what);
 int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype);
-int gemm_f32_batch(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t kall, int64_t ld,
-                   int64_t xs, int64_t ws, int batch, hipStream_t st, const char* what);
-double gemm_f32_batch_us(int64_t M, int64_t N, int64_t K, int batch);
+double gemm_f32_pair_us(const BatchOf& a, const BatchOf& b, int& tile);
+int gemm_f32_pair(const BatchOf& a, const BatchOf& b, int tile, hipStream_t st, const char* what);
 int grad_products(const void* dy, const void* x, const void* w, void* dx, void* dw, const ColumnSums& sums, int64_t M, int64_t N,
                   int64_t K, char* ws, hipStream_t st, const char* what);
 int64_t grad_products_workspace(int64_t M, int64_t N, int64_t K);
@@ -123,43 +122,69 @@ __global__ __launch_bounds__(NT) void column_parts_kernel(const T* __restrict__ 
 int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 int64_t column_part_rows(int64_t M) { return std::max<int64_t>(256, (M + 63) / 64); }
 
-// fp32: how a contraction of D values is cut for R x C results, pieces of P (a multiple of
-// `step`, at least 64, at most `most`): by estimated time, the pieces' products written
-// and read once more at 4.5 TB/s.
-void split_f32(int64_t R, int64_t C, int64_t D, int64_t step, int64_t most, int64_t& S, int64_t& P) {
-  auto up = [&](int64_t v) { return (v + step - 1) / step * step; };
-  double best = 0;
-  S = 0;
-  for (int64_t s = 1; s <= 64; ++s) {
-    const int64_t p = std::min(most, std::max<int64_t>(up((D + s - 1) / s), up(64)));
-    const int64_t n = (D + p - 1) / p;
-    const double us = gemm_f32_batch_us(R, C, std::min(p, up(D)), (int)std::min<int64_t>(n, 1 << 20)) +
-                      (n > 1 ? 3 + (double)(n * R * C) * 8 / 4.5e6 : 0);
-    if (S == 0 || us < best) {
-      best = us;
-      S = n;
-      P = p;
+// fp32: how the contractions of dx (N values, pieces of Px) and dw (M rows, pieces of P)
+// are cut, and the tile: by the estimated time of both side by side, whichever is asked
+// for (a gradient's bits do not depend on what else is), the pieces' products written and
+// read once more.  No piece of dw's operands passes the GEMM's 2 GiB; where dy does, dx
+// goes in pieces of rows, by itself.
+struct PlanF32 {
+  int64_t S = 0, P = 0, Sx = 1, Px = 0, rows = 0;      // rows: of dx in one launch
+  int tile = 0, tilex = 0;                             // of both (of dw, where they run apart), of dx apart
+  bool together = true;
+  PlanF32() = default;
+  PlanF32(int64_t M, int64_t N, int64_t K) {
+    auto pieces = [](int64_t D, int64_t step, int64_t most, int64_t s, int64_t& n) {
+      auto up = [&](int64_t v) { return (v + step - 1) / step * step; };
+      const int64_t p = std::min(most, std::max<int64_t>(up((D + s - 1) / s), up(64)));
+      n = (D + p - 1) / p;
+      return p;
+    };
+    const int64_t most = std::max<int64_t>(((1LL << 31) - 1) / (std::max(N, K) * 4) / 64 * 64, 64);
+    rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4));
+    together = rows >= M;
+    Px = N;
+    double best = 0;
+    auto next = [](int64_t s) { return s == 1 ? 2 : s & (s - 1) ? s / 3 * 4 : s / 2 * 3; };   // 1 2 3 4 6 8 12 ..
+    for (int64_t sx = 1; sx <= (together ? 8 : 1); sx = next(sx)) {
+      int64_t nx;
+      const int64_t px = pieces(N, 16, N, sx, nx);
+      if (nx < sx) break;                              // no more pieces to be had
+      const BatchOf bx{nullptr, nullptr, nullptr, M, K, px, together ? nx : 0, N, N, px, px};
+      for (int64_t s = 1; s <= 64; s = next(s)) {
+        int64_t n;
+        const int64_t p = pieces(M, 64, most, s, n);
+        int t;
+        const BatchOf bw{nullptr, nullptr, nullptr, N, K, p, n, n * p, p, N * p, K * p};
+        double us = gemm_f32_pair_us(bw, bx, t);
+        if (n > 1 || nx > 1) us += 4 + (double)((n > 1 ? n * N : 0) + (nx > 1 ? nx * M : 0)) * (double)K * 8 / 6e6;
+        if (S == 0 || us < best) {
+          best = us;
+          S = n;
+          P = p;
+          Sx = nx;
+          Px = px;
+          tile = t;
+        }
+        if (n < s) break;
+      }
     }
-    if (n < s) break;                                   // no more pieces to be had
+    if (!together) gemm_f32_pair_us(BatchOf{nullptr, nullptr, nullptr, rows, K, N, 1, N, N, N, N}, BatchOf{}, tilex);
   }
-}
+};
 
 // Workspace of the two products and the column sums.
 struct GradSpace {
-  int64_t S = 1, P = 0, Sx = 1, Px = 0, wt = 0, dyt = 0, xt = 0, prodx = 0, prodw = 0, part = 0, bytes = 0;
+  PlanF32 f;
+  int64_t wt = 0, dyt = 0, xt = 0, prodx = 0, prodw = 0, part = 0, bytes = 0;
   GradSpace(int64_t M, int64_t N, int64_t K, int64_t parts, int dtype) {
     if (dtype == NSW_DTYPE_F32) {
-      // dw: none whose transposed rows pass the GEMM's 2 GiB; dx: whole, where its rows
-      // go in pieces for that
-      split_f32(N, K, M, 64, std::max<int64_t>(((1LL << 31) - 1) / (std::max(N, K) * 4) / 64 * 64, 64), S, P);
-      if (M * N * 4 < (1LL << 31)) split_f32(M, K, N, 16, N, Sx, Px);
-      else Px = N;
+      f = PlanF32(M, N, K);
       wt = 0;                                          // w^T
       dyt = wt + align256(N * K * 4);                  // dy^T and x^T in pieces
-      xt = dyt + align256(S * N * P * 4);
-      prodx = xt + align256(S * K * P * 4);            // their products
-      prodw = prodx + align256(Sx > 1 ? Sx * M * K * 4 : 0);
-      part = prodw + align256(S > 1 ? S * N * K * 4 : 0);
+      xt = dyt + align256(f.S * N * f.P * 4);
+      prodx = xt + align256(f.S * K * f.P * 4);            // their products
+      prodw = prodx + align256(f.Sx > 1 ? f.Sx * M * K * 4 : 0);
+      part = prodw + align256(f.S > 1 ? f.S * N * K * 4 : 0);
     } else {
       part = grad_products_workspace(M, N, K);
     }
@@ -177,16 +202,17 @@ bool bad_gated_sizes(int64_t M, int64_t H, int64_t K, int dtype) {
   return H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype);
 }
 
-// fp32: three launches beside the products, transposes, parts with the column sums (each
-// alone costs its own few us: 16200 rows, 192 -> 768, transposes 6.3 us three times).
+// fp32: transposes, both products side by side, parts with the column sums (a launch
+// each: alone every one costs its own few us).
 int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, void* dw, const ColumnSums& sums, int64_t M,
                      int64_t N, int64_t K, const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
   auto f = [&](int64_t at) { return (float*)(ws + at); };
+  const PlanF32& p = sp.f;
   Turn tw{}, ty{}, tx{};
   if (dx) tw = Turn{(const float*)w, f(sp.wt), N, 1, (int)K, (int)N};
   if (dw) {
-    ty = Turn{(const float*)dy, f(sp.dyt), M, sp.S, (int)N, (int)sp.P};
-    tx = Turn{(const float*)x, f(sp.xt), M, sp.S, (int)K, (int)sp.P};
+    ty = Turn{(const float*)dy, f(sp.dyt), M, p.S, (int)N, (int)p.P};
+    tx = Turn{(const float*)x, f(sp.xt), M, p.S, (int)K, (int)p.P};
   }
   const int64_t turns = tw.blocks() + ty.blocks() + tx.blocks();
   NSW_CHECK_ARG(turns < (1LL << 31), "%s: too many rows", what);
@@ -194,21 +220,23 @@ int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, voi
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)turns), dim3(NT), 0, st, tw, ty, tx);
     if (int rc = check_launch(what)) return rc;
   }
-  char* px = sp.Sx > 1 ? ws + sp.prodx : dx;              // Sx > 1 only where M is small: one piece of rows
-  if (dx) {
-    // as many rows at a time as the GEMM's 2 GiB hold
-    const int64_t rows = std::max<int64_t>(1, ((1LL << 31) - 1) / (N * 4));
-    for (int64_t m = 0; m < M; m += rows)
-      if (int rc = gemm_f32_batch(dy + m * N * 4, ws + sp.wt, px + m * K * 4, std::min(rows, M - m), K, sp.Px, N, N, sp.Px,
-                                  sp.Px, (int)sp.Sx, st, what))
-        return rc;
+  char* px = p.Sx > 1 ? ws + sp.prodx : dx;
+  void* pw = p.S > 1 ? ws + sp.prodw : dw;
+  BatchOf bx{}, bw{};
+  if (dx) bx = BatchOf{dy, ws + sp.wt, px, M, K, p.Px, p.Sx, N, N, p.Px, p.Px};
+  if (dw) bw = BatchOf{ws + sp.dyt, ws + sp.xt, pw, N, K, p.P, p.S, p.S * p.P, p.P, N * p.P, K * p.P};
+  if (dx && !p.together) {
+    for (int64_t m = 0; m < M; m += p.rows) {
+      bx.x = dy + m * N * 4;
+      bx.y = dx + m * K * 4;
+      bx.M = std::min(p.rows, M - m);
+      if (int rc = gemm_f32_pair(bx, BatchOf{}, p.tilex, st, what)) return rc;
+    }
+    bx.batch = 0;
   }
-  void* pw = sp.S > 1 ? ws + sp.prodw : dw;
-  if (dw)
-    if (int rc = gemm_f32_batch(ws + sp.dyt, ws + sp.xt, pw, N, K, sp.P, sp.S * sp.P, sp.P, N * sp.P, K * sp.P, (int)sp.S, st,
-                                what))
-      return rc;
-  return finish_grads(Parts{px, dx, M * K, dx ? (int)sp.Sx : 0}, Parts{pw, dw, N * K, dw ? (int)sp.S : 0}, sums, N,
+  const bool dw_first = p.P >= p.Px;                       // the longer ones
+  if (int rc = gemm_f32_pair(dw_first ? bw : bx, dw_first ? bx : bw, p.tile, st, what)) return rc;
+  return finish_grads(Parts{px, dx, M * K, dx ? (int)p.Sx : 0}, Parts{pw, dw, N * K, dw ? (int)p.S : 0}, sums, N,
                       NSW_DTYPE_F32, st, what);
 }
 

@@ -3,9 +3,9 @@
 // EPI_GATED_GRAD).  bf16: grad_products, which reads every operand as it lies.  fp32: the
 // forward GEMM on transposed copies (its operands are split into parts as they pass
 // through LDS, so they cannot be turned there), the batch cut into pieces whose products
-// run side by side and are added in a fixed order.  fp32, 16200 rows, 192 -> 768: 287 us
-// in all, of it 83 for the sums formed again and 93 for each product (104 TFLOP/s of fp32
-// in six bf16 products a value).
+// run side by side and are added in a fixed order, beside those of dx.  fp32, 16200 rows,
+// 192 -> 768: 258 us in all, of it 83 for the sums formed again, 39 for the transposes
+// (HBM), 130 for dx and dw together (147 TFLOP/s of fp32 in six bf16 products a value).
 #include <algorithm>
 
 #include "nsw_gemm_common.h"
@@ -145,10 +145,11 @@ struct PlanF32 {
     Px = N;
     double best = 0;
     auto next = [](int64_t s) { return s == 1 ? 2 : s & (s - 1) ? s / 3 * 4 : s / 2 * 3; };   // 1 2 3 4 6 8 12 ..
-    for (int64_t sx = 1; sx <= (together ? 8 : 1); sx = next(sx)) {
+    const int64_t tiles = ((M + 63) / 64) * ((K + 127) / 128);
+    for (int64_t sx = 1; sx <= (together ? 64 : 1); sx = next(sx)) {
       int64_t nx;
       const int64_t px = pieces(N, 16, N, sx, nx);
-      if (nx < sx) break;                              // no more pieces to be had
+      if (nx < sx || (sx > 1 && tiles * sx > 2048)) break;   // no more pieces to be had, or enough
       const BatchOf bx{nullptr, nullptr, nullptr, M, K, px, together ? nx : 0, N, N, px, px};
       for (int64_t s = 1; s <= 64; s = next(s)) {
         int64_t n;

@@ -239,3 +239,43 @@ def test_fp8_module_keeps_its_bytes_under_a_change_of_dtype(device):
     assert mlp.fc1.bias.dtype == BF16 and mlp(x).dtype == BF16
     for t, want in zip((mlp.fc1.weight, mlp.fc1.weight_scale), held_):
         assert t.dtype == want.dtype and torch.equal(t.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_two_streams_and_two_graphs_at_once(device, dtype):
+    """Calls that overlap share nothing: the same bits as one after the other."""
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g).to(device=device, dtype=dtype)
+    w, b, nw = r(2 * 160, 96) * 96 ** -0.5, r(2 * 160), r(96)
+    ins = [(r(700, 96), r(700, 160), r(700, 96), r(4, 96)) for _ in range(2)]
+
+    def step(x, dh, s, gate):
+        h = ops.gated_linear(x, w, b)
+        y, z = ops.residual_norm(x, s, nw, gate, 1.0, nw)
+        return (h, y, z, *ops.gated_linear_backward(dh, x, w, b), *ops.residual_norm_backward(y, z, x, s, nw, gate, 1.0, nw),
+                *ops.quantize_fp8(z))
+
+    same = lambda a, b: all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a, b))
+    want = [step(*i) for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(step(*ins[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(same(o, want[k]) for o in got[k])
+    graphs, outs = [], []
+    for i in ins:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(*i))
+    for _ in range(3):
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        assert all(same(o, w_) for o, w_ in zip(outs, want))
+        step(*ins[0])

@@ -276,9 +276,9 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
 // for them.  As pick_tile, the k loop 1.7 times as long for three parts from its start;
 // more workgroups than slots: their times shared out, and 0.35 of the shorter one at the
 // end.  With the parts planned by it (PlanF32) within 5% of the fastest of all tiles and cuts
-// at seven shapes, us, this / fastest / slowest: M 16200, N 1536, K 192 184 / 177 / 522;
-// 300, 1024, 256 18.8 / 18.9 / 129; 4000, 2048, 512 116 / 115 / 484; 64800, 256, 256 156 /
-// 150 / 564.
+// at seven shapes, us with the operands' transposes, this / fastest / slowest: M 16200, N
+// 1536, K 192 184 / 177 / 522; 300, 1024, 256 18.8 / 18.9 / 129; 4000, 2048, 512 116 / 115 /
+// 484; 64800, 256, 256 156 / 150 / 564.
 double gemm_f32_pair_us(const BatchOf& a, const BatchOf& b, int& tile) {
   constexpr double q = 1.7;
   constexpr TileCost costs[3] = {{256, 256, 256, 18, .0795 * q, 9.5, .0605 * q, 0},
@@ -307,10 +307,11 @@ int gemm_f32_pair(const BatchOf& a, const BatchOf& b, int tile, hipStream_t st, 
   int n = 0;
   for (const BatchOf* p : {&a, &b}) {
     if (p->batch == 0) continue;
-    NSW_CHECK_ARG(p->batch < 65536 && p->kall <= p->batch * p->K && p->kall > (p->batch - 1) * p->K && p->kall % 16 == 0,
+    NSW_CHECK_ARG(p->batch < 65536 && p->kall <= p->batch * p->K && p->kall > (p->batch - 1) * p->K &&
+                      (p->xt || (p->kall % 16 == 0 && p->K % 16 == 0)),
                   "%s: %lld products of %lld for %lld", what, (long long)p->batch, (long long)p->K, (long long)p->kall);
-    NSW_CHECK_ARG((uint64_t)std::max(p->M, p->N) * p->ld * 4 < (1ULL << 31) && p->M < (1LL << 31) && p->N < (1LL << 31),
-                  "%s: operands above 2 GiB are not supported", what);
+    NSW_CHECK_ARG((uint64_t)(p->xt ? p->K : p->M) * p->ldx * 4 < (1ULL << 31) && (uint64_t)p->K * p->ldw * 4 < (1ULL << 31) &&
+                      p->M < (1LL << 31) && p->N < (1LL << 31), "%s: operands above 2 GiB are not supported", what);
     ea.pair[n++] = *p;
   }
   if (n == 0) return NSW_OK;

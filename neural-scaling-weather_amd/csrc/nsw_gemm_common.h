@@ -46,14 +46,16 @@ constexpr int qkv_head_dim(int epi) {
          : epi == EPI_QKV_HN4 ? 4 : epi == EPI_QKV_HN8 ? 8 : 0;
 }
 
-// `batch` products y[s] [M, N] = x[s] . w[s]^T (0: none): product s contracts values [s K,
-// (s + 1) K) of kall in all (a multiple of 16; the last may be shorter), rows are ld values
-// apart (a multiple of 4), the products' operands xs and ws values apart, the results one
-// after the other.
+// `batch` products y[s] [M, N] = X[s] . W[s] (0: none), fp32: product s contracts values [s
+// K, (s + 1) K) of kall in all (the last may be fewer).  W [kall, N] has the contraction
+// along its rows, X [M, kall] or, with xt, [kall, M], too (else K and kall multiples of
+// 16); rows are ldx and ldw values apart (multiples of 4), the products' operands xs and
+// ws, the results lie one after the other.
 struct BatchOf {
   const void *x, *w;
   void* y;
-  int64_t M, N, K, batch, kall, ld, xs, ws;
+  int64_t M, N, K, batch, kall, ldx, ldw, xs, ws;
+  int xt;
 };
 
 struct EpiArgs {

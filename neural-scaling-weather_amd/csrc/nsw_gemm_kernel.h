@@ -471,6 +471,72 @@ template <typename T, class TC, bool GATE> struct StageCopy {
   }
 };
 
+// The same for fp32 operands of the gradients, of which w, and with XT also x, lie with
+// the contraction along their rows ([K][N], [K][M]): a stage of such an operand is its 32
+// rows of the tile's columns as they lie, a copy whole rows or a part of them, the
+// 64-byte units (16 columns) of row k XOR-swizzled with (k >> 2) & 3, so that the four
+// rows that turned_frag reads at once lie in distinct banks.  Rows past K read as zero.
+template <class TC, bool XT> struct TurnedCopy {
+  static constexpr int NW = TC::NW, CX = TC::BM / 8 / NW, CW = TC::BN / 8 / NW, NC = CX + CW;
+  u32x4 rx, rw;
+  uint32_t v[NC], cx, cw, ldx, ldw;      // ldx, ldw: bytes of a row
+  int lane, wave_rows, nk, nst;          // wave_rows: the wave's first row of x in the stage
+
+  // lane's offset in an operand with the contraction along its rows, copy q of BW columns
+  template <int BW> __device__ __forceinline__ uint32_t turned(int q, uint32_t ld) const {
+    constexpr int RPC = 256 / BW, LPR = 64 / RPC;
+    const int k = q * RPC + lane / LPR;
+    return (uint32_t)k * ld + (uint32_t)((lane % LPR) ^ (((k >> 2) & 3) << 2)) * 16u;
+  }
+  __device__ __forceinline__ void init(const char* smem, const float* X, const float* Wt, int M, int K, int ldx_, int ldw_,
+                                       int m0, int n0, int wave, int lane_) {
+    lane = lane_;
+    wave_rows = wave * CX * 8;
+    ldx = (uint32_t)ldx_ * 4u;
+    ldw = (uint32_t)ldw_ * 4u;
+    rx = XT ? make_rsrc(X + m0, (uint32_t)K * ldx - (uint32_t)m0 * 4u) : make_rsrc(X, (uint32_t)M * ldx);
+    rw = make_rsrc(Wt + n0, (uint32_t)K * ldw - (uint32_t)n0 * 4u);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if (j >= CX) v[j] = turned<TC::BN>(wave * CW + j - CX, ldw);
+      else if (XT) v[j] = turned<TC::BM>(wave * CX + j, ldx);
+      else {
+        const int r = (wave * CX + j) * 8 + lane / 8;
+        v[j] = (uint32_t)(m0 + r < M ? m0 + r : M - 1) * ldx + (uint32_t)((lane % 8) ^ row_swizzle(r)) * 16u;
+      }
+    }
+    cx = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * CX * 1024);
+    cw = (uint32_t)(uintptr_t)smem + (uint32_t)(TC::BM * ROWB + wave * CW * 1024);
+    nk = (K + 15) / 16;
+    nst = (nk + 1) / 2;
+  }
+  __device__ __forceinline__ void copy(int s, int slot, int lo, int hi) const {
+    const uint32_t so = (uint32_t)slot * (uint32_t)TC::SLOT;
+    const bool half = (nk & 1) != 0 && s == nst - 1;        // x as it is: see StageCopy
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if (j < lo || j >= hi) continue;
+      if (j >= CX) dma16(rw, cw + (j - CX) * 1024u + so, v[j], (uint32_t)s * 32u * ldw);
+      else if (XT) dma16(rx, cx + j * 1024u + so, v[j], (uint32_t)s * 32u * ldx);
+      else dma16(rx, cx + j * 1024u + so, half && unused(j) ? 0x80000000u : v[j], (uint32_t)s * ROWB);
+    }
+  }
+  __device__ __forceinline__ bool unused(int j) const {
+    return ((lane % 8) ^ row_swizzle(wave_rows + j * 8 + lane / 8)) >= 4;
+  }
+};
+
+// Columns unit * 16 + frow of an operand staged as its rows: values k = 4 fg + e and 16 +
+// 4 fg + e, as lds_frag's chunks fg and 4 + fg of a row.
+template <int BW>
+__device__ __forceinline__ void turned_frag(const char* op, int unit, int frow, int fg, u32x4 (&r)[2]) {
+  const char* p = op + fg * (4 * BW * 4) + ((unit ^ fg) << 6) + frow * 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[h][e] = *reinterpret_cast<const uint32_t*>(p + (16 * h + e) * (BW * 4));
+}
+
 // bf16 main loop with a ring of NST stages, one barrier per stage: at the top
 // of stage s a wave waits for its copies of stage s, and past the barrier
 // (every wave's copies have landed, and every wave is done reading stage s -
@@ -890,16 +956,19 @@ __device__ __forceinline__ int mainloop_split2(char* smem, Split2List& list, con
 // Stages, barrier and copies as mainloop_split2, but the parts do not fit in
 // place, so every wave splits the fragments it reads: w block nb + 1 under the
 // MFMAs of (nb, mb 0), x block mb + 1 under those of block mb.
-template <class TC, bool GATE>
+// WT: w, and with XT also x, lies with the contraction along its rows (TurnedCopy).
+template <class TC, bool GATE, bool XT = false, bool WT = false>
 __device__ __forceinline__ void mainloop_split3(char* smem, const float* __restrict__ X, const float* __restrict__ Wt,
-                                                int M, int N, int K, int ld, int m0, int n0,
+                                                int M, int N, int K, int ldx, int ldw, int m0, int n0,
                                                 f32x4 (&acc)[TC::NB][TC::MB], int wave, int lane, int first) {
+  static_assert(WT || !XT, "x turned where w is");
   constexpr int NB = TC::NB, MB = TC::MB;
   constexpr int BARB = MB > 2 ? MB - 2 : 1;      // row block before which the barrier stands
-  using Copy = StageCopy<float, TC, GATE>;
+  using Copy = std::conditional_t<WT, TurnedCopy<TC, XT>, StageCopy<float, TC, GATE>>;
   constexpr int NC = Copy::NC, NC1 = NC / 2;     // copies issued past the barrier / in the next stage
   Copy cp;
-  cp.init(smem, X, Wt, M, N, K, ld, m0, n0, wave, lane);
+  if constexpr (WT) cp.init(smem, X, Wt, M, K, ldx, ldw, m0, n0, wave, lane);
+  else cp.init(smem, X, Wt, M, N, K, ldx, m0, n0, wave, lane);
   const int nst = cp.nst;
   if (first >= nst) return;
   cp.copy(first, 0, 0, NC);
@@ -913,18 +982,26 @@ __device__ __forceinline__ void mainloop_split3(char* smem, const float* __restr
     r[0] = lds_frag(st, row, fg);
     r[1] = lds_frag(st, row, 4 + fg);
   };
+  auto loadx = [&](const char* st, int row, u32x4 (&r)[2]) {
+    if constexpr (XT) turned_frag<TC::BM>(st, row >> 4, frow, fg, r);
+    else load(st, row, r);
+  };
+  auto loadw = [&](const char* st, int row, u32x4 (&r)[2]) {
+    if constexpr (WT) turned_frag<TC::BN>(st + TC::BM * ROWB, (row - TC::BM) >> 4, frow, fg, r);
+    else load(st, row, r);
+  };
   u32x4 rw_[NB][2], rx_[2][2];
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) load(smem, wrow + nb * 16, rw_[nb]);
-  load(smem, xrow, rx_[0]);
-  load(smem, xrow + 16, rx_[1]);
+  for (int nb = 0; nb < NB; ++nb) loadw(smem, wrow + nb * 16, rw_[nb]);
+  loadx(smem, xrow, rx_[0]);
+  loadx(smem, xrow + 16, rx_[1]);
   Split3 ws[NB], xs = split3(rx_[0][0], rx_[0][1]), w0 = split3(rw_[0][0], rw_[0][1]), xn;
   for (int s = first; s < nst; ++s) {
     const int slot = (s - first) & 1;
     const char* st = smem + slot * TC::SLOT;
     const char* sn = smem + (slot ^ 1) * TC::SLOT;
     const int c1 = s + 1 < nst ? s + 1 : nst - 1, c2 = s + 2 < nst ? s + 2 : nst - 1;
-    if (MB > 2) load(st, xrow + 32, rx_[0]);
+    if (MB > 2) loadx(st, xrow + 32, rx_[0]);
     ws[0] = w0;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -949,16 +1026,16 @@ __device__ __forceinline__ void mainloop_split3(char* smem, const float* __restr
         constexpr int L = MB - BARB;             // row blocks past the barrier
         cp.copy(c2, slot, (mb - BARB) * NC1 / L, (mb - BARB + 1) * NC1 / L);
       }
-      if (mb + 2 < MB) load(st, xrow + (mb + 2) * 16, rx_[mb & 1]);
+      if (mb + 2 < MB) loadx(st, xrow + (mb + 2) * 16, rx_[mb & 1]);
       if (mb == BARB) {
-        load(sn, wrow, rw_[0]);
-        load(sn, xrow, rx_[0]);
-        if (MB == 2) load(sn, xrow + 16, rx_[1]);
+        loadw(sn, wrow, rw_[0]);
+        loadx(sn, xrow, rx_[0]);
+        if (MB == 2) loadx(sn, xrow + 16, rx_[1]);
       }
       if (mb == MB - 1) {
 #pragma unroll
-        for (int nb = 1; nb < NB; ++nb) load(sn, wrow + nb * 16, rw_[nb]);
-        if (MB > 2) load(sn, xrow + 16, rx_[1]);
+        for (int nb = 1; nb < NB; ++nb) loadw(sn, wrow + nb * 16, rw_[nb]);
+        if (MB > 2) loadx(sn, xrow + 16, rx_[1]);
       }
       mul_parts4(acc, mb, ws, xs);
       if (mb + 1 < MB) xn = split3(rx_[(mb + 1) & 1][0], rx_[(mb + 1) & 1][1]);
@@ -998,10 +1075,11 @@ __device__ __forceinline__ bool any_nonfinite(const f32x4 (&acc)[TC::NB][TC::MB]
 // from global memory; of a wave's 16 x 16 blocks those with such a result, a few at
 // a time through LDS (buf, a KB each; with a loop for every block in the code, the
 // loads could not run ahead).  On finite data no wave does.
-template <class TC, bool GATE>
+// WT, XT: operands with the contraction along their rows.
+template <class TC, bool GATE, bool XT = false, bool WT = false>
 __device__ __forceinline__ void redo_nonfinite(char* buf, const float* __restrict__ X, const float* __restrict__ Wt, int M,
-                                               int N, int K, int ld, int mw0, int nw0, f32x4 (&acc)[TC::NB][TC::MB], int wave,
-                                               int lane) {
+                                               int N, int K, int ldx, int ldw, int mw0, int nw0,
+                                               f32x4 (&acc)[TC::NB][TC::MB], int wave, int lane) {
   constexpr int NB = TC::NB, MB = TC::MB, G = 4;
   static_assert(TC::NW * G * 1024 <= Stg<float, TC>::SMEM, "LDS layout");
   if (!any_nonfinite<TC>(acc)) return;
@@ -1021,9 +1099,22 @@ __device__ __forceinline__ void redo_nonfinite(char* buf, const float* __restric
       const int b = __builtin_ctz(left);
       left &= left - 1;
       const int n = w_source_row<GATE>(nw0, b / MB * 16 + frow, N), m = mw0 + b % MB * 16 + frow;
-      const float* wp = Wt + (int64_t)n * ld + 4 * fg;
-      const float* xp = X + (int64_t)(m < M ? m : M - 1) * ld + 4 * fg;
       f32x4 a = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (WT) {
+        const int mc = m < M ? m : M - 1;
+        for (int k = 0; k < K; k += 16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t q = k + 4 * fg + e;
+            const float w = q < K ? Wt[q * ldw + n] : 0.f, x = q < K ? (XT ? X[q * ldx + mc] : X[(int64_t)mc * ldx + q]) : 0.f;
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(w, x, a, 0, 0, 0);
+          }
+        }
+        c[g * 64] = a;
+        continue;
+      }
+      const float* wp = Wt + (int64_t)n * ldw + 4 * fg;
+      const float* xp = X + (int64_t)(m < M ? m : M - 1) * ldx + 4 * fg;
 #pragma unroll 8
       for (int k = 0; k < K; k += 16) {
         const f32x4 w = *reinterpret_cast<const f32x4*>(wp + k);
@@ -1123,7 +1214,8 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave / WGN, wn = wave % WGN;
 
-  int bid = (int)blockIdx.x, ld = K;               // values between rows of x and of w
+  int bid = (int)blockIdx.x, ldx = K, ldw = K;     // values between rows of x and of w
+  bool xt = false;
   if constexpr (EPI == EPI_BATCH) {                // the products of pair[0], then those of pair[1]
     auto tiles = [](const BatchOf& b) { return ((int)b.M + BM - 1) / BM * (((int)b.N + BN - 1) / BN); };
     int n = tiles(ea.pair[0]);
@@ -1137,7 +1229,9 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
     bid -= piece * n;
     M = (int)b.M;
     N = (int)b.N;
-    ld = (int)b.ld;
+    ldx = (int)b.ldx;
+    ldw = (int)b.ldw;
+    xt = b.xt != 0;
     X = (const T*)b.x + piece * b.xs;
     Wt = (const T*)b.w + piece * b.ws;
     Y = (T*)b.y + piece * b.M * b.N;
@@ -1187,13 +1281,23 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void gemm_kernel(const T* __
       // on two fp16 parts as long as they hold the tile's values, then on three
       // bf16 parts; gradients (EPI_BATCH), products of factors near zero, leave two
       // parts within a few stages, so they start on three
-      int stage = 0;
-      if (EPI != EPI_BATCH && K >= SPLIT2_MIN_K) {
-        __shared__ Split2List list;
-        stage = mainloop_split2<TC, GATE>(smem, list, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
+      if constexpr (EPI == EPI_BATCH) {
+        auto turned = [&](auto f) {
+          constexpr bool XT = decltype(f)::value;
+          mainloop_split3<TC, false, XT, true>(smem, X, Wt, M, N, K, ldx, ldw, m0, n0, acc, wave, lane0, 0);
+          redo_nonfinite<TC, false, XT, true>(smem, X, Wt, M, N, K, ldx, ldw, m0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
+        };
+        if (xt) turned(std::true_type{});
+        else turned(std::false_type{});
+      } else {
+        int stage = 0;
+        if (K >= SPLIT2_MIN_K) {
+          __shared__ Split2List list;
+          stage = mainloop_split2<TC, GATE>(smem, list, Xt, Wt, Mt, N, K, mt0, n0, acc, wave, lane0);
+        }
+        mainloop_split3<TC, GATE>(smem, Xt, Wt, Mt, N, K, ldx, ldw, mt0, n0, acc, wave, lane0, stage);
+        redo_nonfinite<TC, GATE>(smem, Xt, Wt, Mt, N, K, ldx, ldw, mt0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
       }
-      mainloop_split3<TC, GATE>(smem, Xt, Wt, Mt, N, K, ld, mt0, n0, acc, wave, lane0, stage);
-      redo_nonfinite<TC, GATE>(smem, Xt, Wt, Mt, N, K, ld, mt0 + wm * WTM, n0 + wn * WTN, acc, wave, lane0);
     }
   }
   NSW_STAMP(ts[2]);

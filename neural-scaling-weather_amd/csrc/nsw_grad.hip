@@ -1,11 +1,10 @@
 // Gradients of the linear products: dx = dy . w, dw = dy^T . x and db = column sums
 // of dy, for nsw_linear (dy given) and for nsw_gated_linear (dy formed from dh by
-// EPI_GATED_GRAD).  bf16: grad_products, which reads every operand as it lies.  fp32: the
-// forward GEMM on transposed copies (its operands are split into parts as they pass
-// through LDS, so they cannot be turned there), the batch cut into pieces whose products
-// run side by side and are added in a fixed order, beside those of dx.  fp32, 16200 rows,
-// 192 -> 768: 258 us in all, of it 83 for the sums formed again, 39 for the transposes
-// (HBM), 130 for dx and dw together (147 TFLOP/s of fp32 in six bf16 products a value).
+// EPI_GATED_GRAD).  Every operand is read as it lies: bf16 by grad_products, fp32 by the
+// forward GEMM's kernel with turned operands (EPI_BATCH), dx and dw side by side in pieces
+// of their contractions, the pieces' products added in a fixed order.  fp32, 16200 rows,
+// 192 -> 768: 227 us in all, of it 83 for the sums formed again and 130 for dx and dw (147
+// TFLOP/s of fp32 in six bf16 products a value); on transposed copies it took 257.
 #include <algorithm>
 
 #include "nsw_gemm_common.h"
@@ -25,52 +24,6 @@ int64_t grad_products_workspace(int64_t M, int64_t N, int64_t K);
 namespace {
 
 constexpr int NT = 256;
-
-// out[s][c][i] = in[s P + i][c] for in [R, C], S pieces of P rows (a multiple of 4),
-// zeros where s P + i >= R.  64 x 64 values through LDS, 16-byte accesses on both sides.
-struct Turn {
-  const float* in;
-  float* out;
-  int64_t R, S;
-  int C, P;
-  __host__ __device__ int across() const { return (C + 63) / 64; }          // tiles along C
-  __host__ __device__ int down() const { return (P + 63) / 64; }            // and of a piece
-  __host__ __device__ int64_t blocks() const { return S * across() * down(); }
-};
-
-// Of a, then b, then c (blocks() of each; S = 0: none).
-__global__ __launch_bounds__(NT) void transpose_kernel(Turn a, Turn b, Turn c) {
-  __shared__ float t[64][65];
-  int64_t id = blockIdx.x;
-  if (id >= a.blocks()) {
-    id -= a.blocks();
-    a = b;
-    if (id >= b.blocks()) {
-      id -= b.blocks();
-      a = c;
-    }
-  }
-  const uint32_t tile = (uint32_t)id / (uint32_t)a.across();
-  const int c0 = (int)((uint32_t)id - tile * (uint32_t)a.across()) * 64, C = a.C, P = a.P;
-  const int64_t s = tile / (uint32_t)a.down();
-  const int i0 = (int)(tile - (uint32_t)s * (uint32_t)a.down()) * 64;
-  const int64_t r0 = s * P + i0;
-  const int pl = ((int)threadIdx.x & 15) * 4, rw = (int)threadIdx.x >> 4;
-#pragma unroll
-  for (int r = rw; r < 64; r += NT / 16) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r0 + r < a.R && c0 + pl < C) load4<float>(a.in + (r0 + r) * C + c0 + pl, v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) t[r][pl + e] = v[e];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int c_ = rw; c_ < 64; c_ += NT / 16) {
-    if (c0 + c_ >= C || i0 + pl >= P) continue;
-    const float v[4] = {t[pl][c_], t[pl + 1][c_], t[pl + 2][c_], t[pl + 3][c_]};
-    store4<float>(a.out + (s * C + c0 + c_) * P + i0 + pl, v);
-  }
-}
 
 // Parts a by the first `na` workgroups, b by the next nb, column sums by the others.
 template <typename T>
@@ -148,14 +101,14 @@ struct PlanF32 {
     const int64_t tiles = ((M + 63) / 64) * ((K + 127) / 128);
     for (int64_t sx = 1; sx <= (together ? 64 : 1); sx = next(sx)) {
       int64_t nx;
-      const int64_t px = pieces(N, 16, N, sx, nx);
+      const int64_t px = pieces(N, 32, N, sx, nx);
       if (nx < sx || (sx > 1 && tiles * sx > 2048)) break;   // no more pieces to be had, or enough
-      const BatchOf bx{nullptr, nullptr, nullptr, M, K, px, together ? nx : 0, N, N, px, px};
+      const BatchOf bx{nullptr, nullptr, nullptr, M, K, px, together ? nx : 0, N, N, K, px, px * K, 0};
       for (int64_t s = 1; s <= 64; s = next(s)) {
         int64_t n;
         const int64_t p = pieces(M, 64, most, s, n);
         int t;
-        const BatchOf bw{nullptr, nullptr, nullptr, N, K, p, n, n * p, p, N * p, K * p};
+        const BatchOf bw{nullptr, nullptr, nullptr, N, K, p, n, M, N, K, p * N, p * K, 1};
         double us = gemm_f32_pair_us(bw, bx, t);
         if (n > 1 || nx > 1) us += 4 + (double)((n > 1 ? n * N : 0) + (nx > 1 ? nx * M : 0)) * (double)K * 8 / 6e6;
         if (S == 0 || us < best) {
@@ -169,21 +122,17 @@ struct PlanF32 {
         if (n < s) break;
       }
     }
-    if (!together) gemm_f32_pair_us(BatchOf{nullptr, nullptr, nullptr, rows, K, N, 1, N, N, N, N}, BatchOf{}, tilex);
+    if (!together) gemm_f32_pair_us(BatchOf{nullptr, nullptr, nullptr, rows, K, N, 1, N, N, K, N, N * K, 0}, BatchOf{}, tilex);
   }
 };
 
 // Workspace of the two products and the column sums.
 struct GradSpace {
   PlanF32 f;
-  int64_t wt = 0, dyt = 0, xt = 0, prodx = 0, prodw = 0, part = 0, bytes = 0;
+  int64_t prodx = 0, prodw = 0, part = 0, bytes = 0;
   GradSpace(int64_t M, int64_t N, int64_t K, int64_t parts, int dtype) {
     if (dtype == NSW_DTYPE_F32) {
       f = PlanF32(M, N, K);
-      wt = 0;                                          // w^T
-      dyt = wt + align256(N * K * 4);                  // dy^T and x^T in pieces
-      xt = dyt + align256(f.S * N * f.P * 4);
-      prodx = xt + align256(f.S * K * f.P * 4);            // their products
       prodw = prodx + align256(f.Sx > 1 ? f.Sx * M * K * 4 : 0);
       part = prodw + align256(f.S > 1 ? f.S * N * K * 4 : 0);
     } else {
@@ -203,29 +152,15 @@ bool bad_gated_sizes(int64_t M, int64_t H, int64_t K, int dtype) {
   return H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype);
 }
 
-// fp32: transposes, both products side by side, parts with the column sums (a launch
-// each: alone every one costs its own few us).
+// fp32: both products side by side, then parts with the column sums.
 int linear_grads_f32(const char* dy, const void* x, const void* w, char* dx, void* dw, const ColumnSums& sums, int64_t M,
                      int64_t N, int64_t K, const GradSpace& sp, char* ws, hipStream_t st, const char* what) {
-  auto f = [&](int64_t at) { return (float*)(ws + at); };
   const PlanF32& p = sp.f;
-  Turn tw{}, ty{}, tx{};
-  if (dx) tw = Turn{(const float*)w, f(sp.wt), N, 1, (int)K, (int)N};
-  if (dw) {
-    ty = Turn{(const float*)dy, f(sp.dyt), M, p.S, (int)N, (int)p.P};
-    tx = Turn{(const float*)x, f(sp.xt), M, p.S, (int)K, (int)p.P};
-  }
-  const int64_t turns = tw.blocks() + ty.blocks() + tx.blocks();
-  NSW_CHECK_ARG(turns < (1LL << 31), "%s: too many rows", what);
-  if (turns > 0) {
-    hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)turns), dim3(NT), 0, st, tw, ty, tx);
-    if (int rc = check_launch(what)) return rc;
-  }
   char* px = p.Sx > 1 ? ws + sp.prodx : dx;
   void* pw = p.S > 1 ? ws + sp.prodw : dw;
   BatchOf bx{}, bw{};
-  if (dx) bx = BatchOf{dy, ws + sp.wt, px, M, K, p.Px, p.Sx, N, N, p.Px, p.Px};
-  if (dw) bw = BatchOf{ws + sp.dyt, ws + sp.xt, pw, N, K, p.P, p.S, p.S * p.P, p.P, N * p.P, K * p.P};
+  if (dx) bx = BatchOf{dy, w, px, M, K, p.Px, p.Sx, N, N, K, p.Px, p.Px * K, 0};
+  if (dw) bw = BatchOf{dy, x, pw, N, K, p.P, p.S, M, N, K, p.P * N, p.P * K, 1};
   if (dx && !p.together) {
     for (int64_t m = 0; m < M; m += p.rows) {
       bx.x = dy + m * N * 4;

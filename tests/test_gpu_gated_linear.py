@@ -177,6 +177,22 @@ def test_linear_backward(device, dtype, M, N, K):
     assert one[0] is None and one[2] is None and torch.equal(one[1], dw)
 
 
+@pytest.mark.parametrize("M,N,K", [(77, 96, 64), (1031, 176, 208), (3, 16, 16)])
+def test_infinite_gradients_in_fp32(device, M, N, K):
+    """An infinity stays in its row of dx and its row of dw, with the signs of what it meets; all else as without it."""
+    from nsw import ops
+    g = torch.Generator().manual_seed(K)
+    dy, x, w = (torch.randn(*s, generator=g).to(device) for s in ((M, N), (M, K), (N, K)))
+    clean = ops.linear_backward(dy, x, w)
+    m, n = M - 1, N - 3
+    dy[m, n] = math.inf
+    dx, dw, db = ops.linear_backward(dy, x, w)
+    assert torch.equal(dx[m], math.inf * w[n]) and torch.equal(dw[n], math.inf * x[m]) and db[n] == math.inf
+    for got, want, i in ((dx, clean[0], m), (dw, clean[1], n), (db, clean[2], n)):
+        keep = torch.arange(got.shape[0], device=device) != i
+        assert torch.equal(got[keep], want[keep])
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 1024, 32), (1, 4096, 64), (1000, 160, 32), (2000, 4096, 1024), (3000, 4096, 512),
                                    (8000, 2080, 160), (16200, 4096, 1024)])
 def test_gradients_side_by_side(device, M, N, K):

@@ -273,17 +273,17 @@ int64_t gated_grad_parts(int64_t M, int64_t H, int64_t K, int dtype) {
 }
 
 // Estimated time (us) of one or two families of fp32 products side by side, and the tile
-// for them.  As pick_tile, the k loop 1.7 times as long for three parts from its start;
+// for them.  As pick_tile, the k loop 1.1 - 1.2 times as long for three parts from its start;
 // more workgroups than slots: their times shared out, and 0.35 of the shorter one at the
-// end.  With the parts planned by it (PlanF32) within 5% of the fastest of all tiles and cuts
-// at seven shapes, us with the operands' transposes, this / fastest / slowest: M 16200, N
-// 1536, K 192 184 / 177 / 522; 300, 1024, 256 18.8 / 18.9 / 129; 4000, 2048, 512 116 / 115 /
-// 484; 64800, 256, 256 156 / 150 / 564.
+// end; 256 x 256 stays unless a smaller tile is estimated 7% faster.  Fits to seven shapes,
+// all tiles and cuts: with the parts planned by it (PlanF32) within 10% of the fastest, 4%
+// at the median.  us, this / fastest / slowest: M 16200, N 1536, K 192 149 / 145 / 528; 300,
+// 1024, 256 14 / 14 / 124; 4000, 2048, 512 107 / 102 / 510; 64800, 256, 256 115 / 107 / 580.
 double gemm_f32_pair_us(const BatchOf& a, const BatchOf& b, int& tile) {
-  constexpr double q = 1.7;
-  constexpr TileCost costs[3] = {{256, 256, 256, 18, .0795 * q, 9.5, .0605 * q, 0},
-                                 {MidTile::BM, MidTile::BN, 512, 8, .0537 * q, 6, .0324 * q, .4},
-                                 {SmallF32Tile::BM, SmallF32Tile::BN, 768, 5, .051 * q, 4.3, .0252 * q, .3}};
+  constexpr double q = 1.1, qp = 1.2;
+  constexpr TileCost costs[3] = {{256, 256, 256, 18, .0795 * q, 9.5, .0605 * qp, 0},
+                                 {MidTile::BM, MidTile::BN, 512, 8, .0537 * q, 6, .0324 * qp, .4},
+                                 {SmallF32Tile::BM, SmallF32Tile::BN, 768, 5, .051 * q, 4.3, .0252 * qp, .3}};
   double best = 0;
   for (int i = 0; i < 3; ++i) {
     const TileCost& c = costs[i];

@@ -110,7 +110,7 @@ struct PlanF32 {
         int t;
         const BatchOf bw{nullptr, nullptr, nullptr, N, K, p, n, M, N, K, p * N, p * K, 1};
         double us = gemm_f32_pair_us(bw, bx, t);
-        if (n > 1 || nx > 1) us += 4 + (double)((n > 1 ? n * N : 0) + (nx > 1 ? nx * M : 0)) * (double)K * 8 / 6e6;
+        if (n > 1 || nx > 1) us += 4 + (double)((n > 1 ? n * N : 0) + (nx > 1 ? nx * M : 0)) * (double)K * 8 / 4e6;
         if (S == 0 || us < best) {
           best = us;
           S = n;

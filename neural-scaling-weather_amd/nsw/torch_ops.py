@@ -12,7 +12,9 @@ registered; their callers keep the ``nsw.ops`` functions.
 
 ``linear`` (without GELU), ``gated_linear`` and ``residual_norm`` have
 gradients (``linear_backward``, ``gated_linear_backward``,
-``residual_norm_backward``); the others are forward only.
+``residual_norm_backward``); the others are forward only, and so are the modules
+that pack their parameters (attention, the blocks, the patch embedding): a
+backward pass to those parameters raises.
 
 The block parameters travel as one list in the field order of
 ``nsw_block_params`` (``BLOCK_PARAMS``), None for absent fields; shapes,
@@ -20,7 +22,7 @@ windows and shifts as int lists.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -106,6 +108,19 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], 
 
 
 @linear.register_fake
+def _(x, weight, bias, residual, epilogue):
+    return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
+
+
+@torch.library.custom_op("nsw::linear_forward", mutates_args=())
+def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                   residual: Optional[torch.Tensor], epilogue: int) -> torch.Tensor:
+    """linear without a gradient: a backward pass that reaches it raises."""
+    return ops.linear(x.contiguous(), weight.contiguous(), bias, None if residual is None else residual.contiguous(),
+                      epilogue=epilogue)
+
+
+@linear_forward.register_fake
 def _(x, weight, bias, residual, epilogue):
     return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
 
@@ -307,12 +322,17 @@ def _(x, weight, bias, residual, image, window_size, shift_size):
 
 
 def linear_epi(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
-               residual: Optional[torch.Tensor] = None, epilogue: Optional[int] = None) -> torch.Tensor:
-    """torch.ops.nsw.linear with ops.linear's default epilogue (none / bias / bias + residual)."""
+               residual: Optional[torch.Tensor] = None, epilogue: Optional[int] = None,
+               left_out: Sequence[Optional[torch.Tensor]] = ()) -> torch.Tensor:
+    """torch.ops.nsw.linear with ops.linear's default epilogue (none / bias / bias + residual).
+    ``left_out``: parameters that the arguments were formed from outside the graph (packed,
+    detached).  Where one of them needs a gradient the product has none, so that a backward
+    pass raises instead of leaving theirs out."""
     if epilogue is None:
         epilogue = _lib.NSW_EPI_NONE if bias is None else (
             _lib.NSW_EPI_BIAS if residual is None else _lib.NSW_EPI_BIAS_RESIDUAL)
-    return torch.ops.nsw.linear(x, weight, bias, residual, int(epilogue))
+    whole = not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in left_out))
+    return (torch.ops.nsw.linear if whole else torch.ops.nsw.linear_forward)(x, weight, bias, residual, int(epilogue))
 
 
 @torch.library.custom_op("nsw::rms_norm", mutates_args=())

@@ -316,6 +316,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None, epilogue: Optional[int] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = epi(x . weight^T): F.linear with an optional fused bias / GELU / residual.
+    An epilogue leaves out what it has no part for (a residual without a bias: NSW_EPI_NONE).
     ``out`` (contiguous, x.shape[:-1] + (N,), x's dtype) receives y if given."""
     dev = _dev(x, weight, bias, residual, out)
     _same_dtype(x, weight, bias, residual, out)

@@ -160,6 +160,9 @@ def _linear_backward(ctx, dy):
     if ctx.epilogue not in (_lib.NSW_EPI_NONE, _lib.NSW_EPI_BIAS, _lib.NSW_EPI_BIAS_RESIDUAL):
         raise NotImplementedError("nsw.linear with a GELU epilogue has no gradient (nsw.GatedMLP has)")
     need = list(ctx.needs_input_grad)
+    if (need[2] and ctx.epilogue == _lib.NSW_EPI_NONE) or (need[3] and ctx.epilogue != _lib.NSW_EPI_BIAS_RESIDUAL):
+        raise ValueError(f"nsw.linear: epilogue {ctx.epilogue} left the {'residual' if need[3] else 'bias'} out, which "
+                         "needs a gradient (a residual takes part with a bias)")
     x, weight = ctx.saved_tensors
     needs = [need[0], need[1], need[2]]
     dx, dw, db = torch.ops.nsw.linear_backward(dy, x, weight, needs) if any(needs) else (None, None, None)

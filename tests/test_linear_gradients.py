@@ -47,3 +47,16 @@ def test_patch_embedding_gives_no_partial_gradients():
         p.requires_grad_(False)
     c.tokens(x, residual=r).sum().backward()
     assert r.grad.shape == r.shape
+
+
+@pytest.mark.parametrize("epilogue,wants", [(0, "bias"), (0, "residual"), (1, "residual"), (None, "residual")])
+def test_no_gradient_of_what_the_epilogue_left_out(epilogue, wants):
+    x, w = meta(5, 64).requires_grad_(), meta(96, 64)
+    b, r = meta(96), meta(5, 96)
+    (b if wants == "bias" else r).requires_grad_()
+    y = torch_ops.linear_epi(x, w, None if epilogue is None else b, r, epilogue)
+    with pytest.raises(ValueError, match=wants):
+        y.sum().backward()
+    b, r = b.detach(), r.detach()                  # present, but asked for nothing: x has its gradient
+    g, = torch.autograd.grad(torch_ops.linear_epi(x, w, None if epilogue is None else b, r, epilogue), x, meta(5, 96))
+    assert g.shape == x.shape

@@ -210,7 +210,7 @@ extern "C" int nsw_linear_backward(const void* dy, const void* x, const void* w,
   const char* what = "nsw_linear_backward";
   NSW_CHECK_ARG(!bad_sizes(M, N, K, dtype), "%s: M=%lld, N=%lld, K=%lld in dtype %d: N and K must be multiples of 32 (bf16) / 16 (fp32)",
                 what, (long long)M, (long long)N, (long long)K, dtype);
-  NSW_CHECK_ARG(dy && x && w, "%s: dy, x and w are required", what);
+  NSW_CHECK_ARG(dy && (x || !dw) && w, "%s: dy, w and, for dw, x are required", what);
   const int64_t per = column_part_rows(M), parts = (M + per - 1) / per;
   const GradSpace sp(M, N, K, parts, dtype);
   NSW_CHECK_ARG(workspace != nullptr && workspace_bytes >= (size_t)sp.bytes, "%s: workspace of %lld bytes needed", what,

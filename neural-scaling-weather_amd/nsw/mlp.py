@@ -60,9 +60,9 @@ class MLP(nn.Module):
         x = x.contiguous()
         h = torch_ops.linear_epi(x, self.fc1.weight, self.bias1.bias, epilogue=self.gelu_epilogue)
         if residual is None:
-            return torch_ops.linear_epi(h, self.fc2.weight, self.bias2.bias, epilogue=_lib.NSW_EPI_BIAS)
+            return torch_ops.linear_epi(h, self.fc2.weight, self.bias2.bias, epilogue=_lib.NSW_EPI_BIAS, left_out=(h,))
         return torch_ops.linear_epi(h, self.fc2.weight, self.bias2.bias, residual=residual,
-                                    epilogue=_lib.NSW_EPI_BIAS_RESIDUAL)
+                                    epilogue=_lib.NSW_EPI_BIAS_RESIDUAL, left_out=(h,))
 
 
 class Fp8MLP(nn.Module):

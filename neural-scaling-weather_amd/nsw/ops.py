@@ -401,26 +401,32 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     return dx, dw, db
 
 
-def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+def linear_backward(dy: torch.Tensor, x: Optional[torch.Tensor], weight: torch.Tensor,
                     needs: Sequence[bool] = (True, True, True)):
     """(dx, dweight, dbias) = (dy W, dy^T x, column sums of dy) of linear without
-    an activation, None where ``needs`` says so."""
+    an activation, None where ``needs`` says so.  x may be None where dweight is
+    not needed."""
     what = "linear_backward"
-    at = _uniform(x, dy, weight)
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or dy.shape != x.shape[:-1] + weight.shape[:1]:
-        raise ValueError(f"{what}: dy {tuple(dy.shape)}, x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    at = _uniform(dy, x, weight)
+    if x is None and needs[1]:
+        raise ValueError(f"{what}: dweight needs x")
+    shape = dy.shape[:-1] + weight.shape[1:]                # of x
+    if dy.dim() < 1 or weight.dim() != 2 or dy.shape[-1] != weight.shape[0] or (x is not None and x.shape != shape):
+        raise ValueError(f"{what}: dy {tuple(dy.shape)}, x {None if x is None else tuple(x.shape)} and weight "
+                         f"{tuple(weight.shape)} do not match")
     N, K = weight.shape
     if K == 0 or N == 0:
         raise ValueError(f"{what}: no features")
-    M = x.numel() // K
-    dx, dw = _grads(needs, x, weight)
-    db = x.new_empty(N) if needs[2] else None
+    M = dy.numel() // N
+    dx = dy.new_empty(shape) if needs[0] else None
+    dw = torch.empty_like(weight) if needs[1] else None
+    db = dy.new_empty(N) if needs[2] else None
     if M == 0:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    nbytes = _workspace_bytes(lib(), "nsw_linear_backward_workspace_size", M, N, K, dtype_code(x))
-    ws = x.new_empty(max(nbytes, 16), dtype=torch.uint8)
-    _run(what, at, lib().nsw_linear_backward, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _p(dx), _p(dw), _p(db), M,
-         N, K, dtype_code(x), ws.data_ptr(), nbytes)
+    nbytes = _workspace_bytes(lib(), "nsw_linear_backward_workspace_size", M, N, K, dtype_code(dy))
+    ws = dy.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run(what, at, lib().nsw_linear_backward, dy.data_ptr(), _p(x), weight.data_ptr(), _p(dx), _p(dw), _p(db), M,
+         N, K, dtype_code(dy), ws.data_ptr(), nbytes)
     return dx, dw, db
 
 

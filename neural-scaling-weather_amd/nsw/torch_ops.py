@@ -125,6 +125,14 @@ def _(x, weight, bias, residual, epilogue):
     return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
 
 
+def _no_gradient(ctx, dy):
+    raise NotImplementedError("nsw.linear_forward: the module's pass is forward only (GELU MLP, attention, patch embedding; "
+                              "nsw.GatedMLP has gradients)")
+
+
+linear_forward.register_autograd(_no_gradient)
+
+
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """t contiguous and 16-byte aligned (a gradient may be any view)."""
     t = t.contiguous()
@@ -137,23 +145,25 @@ def _or_empty(like: torch.Tensor, *ts: Optional[torch.Tensor]) -> Tuple[torch.Te
 
 
 @torch.library.custom_op("nsw::linear_backward", mutates_args=())
-def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+def linear_backward(dy: torch.Tensor, x: Optional[torch.Tensor], weight: torch.Tensor,
                     needs: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dx, dweight, dbias) of a linear without an activation; empty ([0]) where ``needs`` is False."""
-    return _or_empty(x, *ops.linear_backward(_dense(dy), _dense(x), _dense(weight), needs=tuple(needs)))
+    """(dx, dweight, dbias) of a linear without an activation; empty ([0]) where ``needs`` is False.
+    x may be None where dweight is not needed."""
+    return _or_empty(dy, *ops.linear_backward(_dense(dy), None if x is None else _dense(x), _dense(weight),
+                                              needs=tuple(needs)))
 
 
 @linear_backward.register_fake
 def _(dy, x, weight, needs):
-    return (x.new_empty(x.shape if needs[0] else (0,)), x.new_empty(weight.shape if needs[1] else (0,)),
-            x.new_empty((weight.shape[0],) if needs[2] else (0,)))
+    return (dy.new_empty(tuple(dy.shape[:-1]) + (weight.shape[1],) if needs[0] else (0,)),
+            dy.new_empty(weight.shape if needs[1] else (0,)), dy.new_empty((weight.shape[0],) if needs[2] else (0,)))
 
 
 def _linear_setup(ctx, inputs, output):
     x, weight, bias, residual, epilogue = inputs
     ctx.epilogue = epilogue
     if epilogue in (_lib.NSW_EPI_NONE, _lib.NSW_EPI_BIAS, _lib.NSW_EPI_BIAS_RESIDUAL):
-        ctx.save_for_backward(x, weight)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight)   # only dweight reads x
 
 
 def _linear_backward(ctx, dy):

@@ -60,3 +60,44 @@ def test_no_gradient_of_what_the_epilogue_left_out(epilogue, wants):
     b, r = b.detach(), r.detach()                  # present, but asked for nothing: x has its gradient
     g, = torch.autograd.grad(torch_ops.linear_epi(x, w, None if epilogue is None else b, r, epilogue), x, meta(5, 96))
     assert g.shape == x.shape
+
+
+def kept(f):
+    """Shapes of what autograd keeps for a backward pass through f."""
+    shapes = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: shapes.append(tuple(t.shape)) or t, lambda t: t):
+        y = f()
+    assert y.requires_grad
+    return shapes
+
+
+def test_linear_keeps_only_what_a_gradient_reads():
+    x, w, b = meta(7, 64), meta(96, 64), meta(96)
+    assert (7, 64) in kept(lambda: torch_ops.linear_epi(x, w.requires_grad_(), b))
+    w = w.detach()
+    assert (7, 64) not in kept(lambda: torch_ops.linear_epi(x.requires_grad_(), w, b))
+    g, = torch.autograd.grad(torch_ops.linear_epi(x, w, b), x, meta(7, 96))
+    assert g.shape == (7, 64)
+    x, b = x.detach(), b.requires_grad_()
+    assert (7, 64) not in kept(lambda: torch_ops.linear_epi(x, w, b))
+    g, = torch.autograd.grad(torch_ops.linear_epi(x, w, b), b, meta(7, 96))
+    assert g.shape == (96,)
+
+
+def test_gelu_mlp_keeps_no_hidden_rows():
+    m = nsw.MLP(64, 256).to(device="meta", dtype=torch.bfloat16)
+    for r in (None, meta(7, 64)):
+        assert (7, 256) not in kept(lambda: m(meta(7, 64), r))
+        with pytest.raises(NotImplementedError):
+            m(meta(7, 64), r).sum().backward()
+    assert all(p.grad is None for p in m.parameters())
+    for p in (m.fc1.weight, m.bias1.bias):
+        p.requires_grad_(False)
+    m(meta(7, 64)).sum().backward()               # what follows the frozen half
+    assert m.fc2.weight.grad.shape == (64, 256) and m.bias2.bias.grad.shape == (64,)
+
+
+def test_linear_backward_without_x():
+    dy, x, w = meta(2, 3, 96), meta(2, 3, 64), meta(96, 64)
+    dx, dw, db = torch.ops.nsw.linear_backward(dy, None, w, [True, False, True])
+    assert dx.shape == x.shape and dw.shape == (0,) and db.shape == (96,)

@@ -166,8 +166,8 @@ int nsw_gated_linear_backward(const void* dh, const void* x, const void* w, cons
 /* Gradients of nsw_linear without an activation, y = x . w^T (+ bias) (+
  * residual, whose gradient is dy): where not NULL dx [M, K] = dy . w, dw
  * [N, K] = dy^T . x and db [N] = dy's column sums; x may be NULL where dw is.
- * N and K multiples of 32 (bf16) / 16 (fp32), 16-byte aligned, w below 2 GiB.
- * Workspace as above. */
+ * N and K multiples of 32 (bf16) / 16 (fp32; a caller with another N adds columns
+ * of zeros), 16-byte aligned, w below 2 GiB.  Workspace as above. */
 size_t nsw_linear_backward_workspace_size(int64_t M, int64_t N, int64_t K, int dtype);
 int nsw_linear_backward(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                         int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream);

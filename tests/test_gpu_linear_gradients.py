@@ -1,5 +1,5 @@
-"""Gradients of torch.ops.nsw.linear where some operands are frozen: the bits of
-those with everything trained."""
+"""Gradients of torch.ops.nsw.linear: where some operands are frozen, the bits of those
+with everything trained; for every width that the forward pass takes."""
 import pytest
 import torch
 
@@ -48,3 +48,35 @@ def test_gelu_mlp_behind_frozen_parameters(device):
     h = torch_ops.linear_epi(x, m.fc1.weight, m.bias1.bias, epilogue=m.gelu_epilogue)
     _, dw, db = ops.linear_backward(dy, h, m.fc2.weight.detach(), needs=(False, True, True))
     assert torch.equal(m.fc2.weight.grad, dw) and torch.equal(m.bias2.bias.grad, db)
+
+
+@pytest.mark.parametrize("dtype,M,N,K", [(BF16, 1, 8, 32), (BF16, 70, 40, 64), (BF16, 300, 1000, 256), (BF16, 4100, 1112, 160),
+                                         (F32, 1, 8, 16), (F32, 70, 24, 48), (F32, 300, 1000, 256), (F32, 4100, 1112, 176)])
+def test_every_width_of_the_forward_pass(device, dtype, M, N, K):
+    """N a multiple of 8.  Bounds: (terms + 8) 2^-24 of the sums of magnitudes, and one rounding; db in at most 512 steps.
+    A row of dy that is not finite stays a row of dx."""
+    g = torch.Generator().manual_seed(N + K)
+    dy, x, w = (torch.randn(*s, generator=g).to(device=device, dtype=dtype) for s in ((M, N), (M, K), (N, K)))
+    a = [t.clone().requires_grad_() for t in (x, w, dy[0])]
+    y = torch_ops.linear_epi(*a)
+    got = torch.autograd.grad(y, a, dy)
+    d, xx, ww = dy.double(), x.double(), w.double()
+    want = ((d @ ww, d.abs() @ ww.abs() * (N + 8)), (d.t() @ xx, d.abs().t() @ xx.abs() * (M + 8)),
+            (d.sum(0), d.abs().sum(0) * 512))
+    step = torch.finfo(dtype).eps / 2
+    for t, (v, mag) in zip(got, want):
+        assert t.dtype == dtype and t.shape == v.shape and t.is_contiguous()
+        over = (t.double() - v).abs() - (mag * 2.0 ** -24 * (1 + step) + v.abs() * step * (1 + 1e-6))
+        assert (over <= torch.finfo(dtype).tiny).all(), over.max().item()
+    if M > 1:
+        clean = ops.linear_backward(dy, x, w, needs=(True, False, False))[0]
+        dy[M // 2, N - 1] = float("nan")
+        dx = ops.linear_backward(dy, x, w, needs=(True, False, False))[0]
+        keep = torch.arange(M, device=device) != M // 2
+        assert torch.equal(dx[keep], clean[keep]) and dx[M // 2].isnan().all()
+
+
+def test_widths_without_rows(device):
+    dx, dw, db = ops.linear_backward(torch.empty(0, 40, device=device), torch.empty(0, 16, device=device),
+                                     torch.ones(40, 16, device=device))
+    assert dx.shape == (0, 16) and dw.shape == (40, 16) and not dw.any() and db.shape == (40,) and not db.any()

@@ -136,9 +136,8 @@ int nsw_rmsnorm_roll_partition(const void* x, const void* w, float eps, void* xw
 
 /* F.linear + BiasLayer (+ GELU / residual) (models/layer_helpers.py:41-42,71-72,
  * models/mlp.py:80-93): y[M,N] = epi(x[M,K] . w[N,K]^T).  bias / residual may
- * be NULL when the epilogue does not use them.  Requires K % 32 == 0 (bf16) or
- * K % 16 == 0 (f32) (one MFMA step of k), N % 8 == 0, 16-byte aligned x, w, y
- * and residual. */
+ * be NULL when the epilogue does not use them.  Requires K % 16 == 0,
+ * N % 8 == 0, 16-byte aligned x, w, y and residual. */
 int nsw_linear(const void* x, const void* w, const void* bias, const void* residual, void* y,
                int64_t M, int64_t N, int64_t K, int epilogue, int dtype, void* stream);
 
@@ -147,8 +146,8 @@ int nsw_linear(const void* x, const void* w, const void* bias, const void* resid
  * block, the activation of the gate and the product in one kernel,
  *   h[M, H] = act(x . w[0:H]^T + bias[0:H]) * (x . w[H:2H]^T + bias[H:2H]),
  * x [M, K], w [2H, K] the gate's rows stacked over the up projection's, bias
- * [2H] or NULL, act NSW_ACT_*.  K and alignment as nsw_linear, H a multiple
- * of 16, w below 2 GiB (x and h may be larger). */
+ * [2H] or NULL, act NSW_ACT_*.  K a multiple of 32 (bf16) / 16 (fp32), alignment
+ * as nsw_linear, H a multiple of 16, w below 2 GiB (x and h may be larger). */
 int nsw_gated_linear(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K,
                      int act, int dtype, void* stream);
 
@@ -166,8 +165,8 @@ int nsw_gated_linear_backward(const void* dh, const void* x, const void* w, cons
 /* Gradients of nsw_linear without an activation, y = x . w^T (+ bias) (+
  * residual, whose gradient is dy): where not NULL dx [M, K] = dy . w, dw
  * [N, K] = dy^T . x and db [N] = dy's column sums; x may be NULL where dw is.
- * N and K multiples of 32 (bf16) / 16 (fp32; a caller with another N adds columns
- * of zeros), 16-byte aligned, w below 2 GiB.  Workspace as above. */
+ * N a multiple of 32 (bf16) / 16 (fp32; a caller with another N adds columns of
+ * zeros), K of 16, 16-byte aligned, w below 2 GiB.  Workspace as above. */
 size_t nsw_linear_backward_workspace_size(int64_t M, int64_t N, int64_t K, int dtype);
 int nsw_linear_backward(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                         int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream);

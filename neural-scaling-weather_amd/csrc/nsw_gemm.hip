@@ -52,7 +52,11 @@ static int launch_gemm(const void* x, const void* w, void* y, int64_t M, int64_t
                 hipStream_t st, const char* what) {
   constexpr int KT = STEPB / sizeof(T);   // k granule: 32 (bf16) / 16 (f32)
   NSW_CHECK_ARG(M > 0 && N > 0 && K > 0, "%s: M, N, K must be positive", what);
-  NSW_CHECK_ARG(K % KT == 0, "%s: K=%lld must be a multiple of %d", what, (long long)K, KT);
+  constexpr bool TAIL = sizeof(T) == 2 && PRE == PRE_NONE &&
+                        (EPI == EPI_NONE || EPI == EPI_BIAS || EPI == EPI_BIAS_GELU || EPI == EPI_BIAS_GELU_TANH ||
+                         EPI == EPI_BIAS_RESIDUAL);
+  const bool tail = TAIL && K % KT == 16;
+  NSW_CHECK_ARG(K % KT == 0 || tail, "%s: K=%lld must be a multiple of %d", what, (long long)K, TAIL ? 16 : KT);
   NSW_CHECK_ARG(N % 8 == 0, "%s: N=%lld must be a multiple of 8", what, (long long)N);
   NSW_CHECK_ARG(M < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31), "%s: dims too large", what);
   constexpr bool GATE = EPI == EPI_GATED || EPI == EPI_GATED_GRAD;   // x addressed tile by tile
@@ -69,6 +73,12 @@ static int launch_gemm(const void* x, const void* w, void* y, int64_t M, int64_t
     if (eg.group_m == 0) eg.group_m = (int)std::max<int64_t>(8, std::min<int64_t>(32, 128 / ((N + 255) / 256)));
   }
   using C = TileChoice<T, EPI>;
+  if constexpr (TAIL)
+    if (tail) switch (pick_tile<T, EPI>(M, N, K, ea)) {
+      case TILE_BIG: return launch_tile<T, EPI, PRE_KTAIL, BigTile>(x, w, y, M, N, K, eg, st, what);
+      case TILE_MID: return launch_tile<T, EPI, PRE_KTAIL, typename C::Mid>(x, w, y, M, N, K, eg, st, what);
+      default: return launch_tile<T, EPI, PRE_KTAIL, typename C::Small>(x, w, y, M, N, K, eg, st, what);
+    }
   switch (pick_tile<T, EPI>(M, N, K, ea)) {
     case TILE_BIG: return launch_tile<T, EPI, PRE, BigTile>(x, w, y, M, N, K, eg, st, what);
     case TILE_MID: return launch_tile<T, EPI, PRE, typename C::Mid>(x, w, y, M, N, K, eg, st, what);

@@ -7,4 +7,5 @@
 
 namespace nsw {
 NSW_GEMM_FORMS(NSW_GEMM_INSTANCE)
+NSW_GEMM_KTAIL_FORMS(NSW_GEMM_INSTANCE)
 }  // namespace nsw

@@ -39,7 +39,9 @@ enum Epi {
 //                RMSNorm of the rows of x with its weight folded into w
 //                (w[n,k] = W[n,k] * norm_w[k], prepared by the caller), at
 //                one read per row instead of a pass over x.
-enum Pre { PRE_NONE = 0, PRE_ROWSCALE = 3 };
+//   PRE_KTAIL    as PRE_NONE, bf16, K 16 more than whole MFMA steps (an instance of
+//                its own, so that the main loops' registers stay as they are)
+enum Pre { PRE_NONE = 0, PRE_ROWSCALE = 3, PRE_KTAIL = 4 };
 
 constexpr int qkv_head_dim(int epi) {
   return (epi == EPI_QKV_HN16 || epi == EPI_QKV_HN32 || epi == EPI_QKV_HN64) ? epi

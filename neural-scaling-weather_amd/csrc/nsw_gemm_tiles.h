@@ -71,6 +71,11 @@ int launch_tile(const void* x, const void* w, void* y, int64_t M, int64_t N, int
   F(EPI_QKV_HN8, PRE_ROWSCALE) F(EPI_QKV_HN16, PRE_ROWSCALE) F(EPI_QKV_HN32, PRE_ROWSCALE)                           \
   F(EPI_QKV_HN64, PRE_ROWSCALE)
 
+// bf16 products whose K is 16 more than whole MFMA steps (nsw_linear).
+#define NSW_GEMM_KTAIL_FORMS(F)                                                                                      \
+  F(EPI_NONE, PRE_KTAIL) F(EPI_BIAS, PRE_KTAIL) F(EPI_BIAS_GELU, PRE_KTAIL) F(EPI_BIAS_GELU_TANH, PRE_KTAIL)         \
+  F(EPI_BIAS_RESIDUAL, PRE_KTAIL)
+
 // The gated products (sources of their own).
 #define NSW_GEMM_GATED_FORMS(F) F(EPI_GATED, PRE_NONE) F(EPI_GATED_GRAD, PRE_NONE)
 // A batch of fp32 products (the gradients' split contraction).

@@ -144,12 +144,12 @@ struct GradSpace {
 
 bool bad_sizes(int64_t M, int64_t N, int64_t K, int dtype) {
   if (dtype != NSW_DTYPE_BF16 && dtype != NSW_DTYPE_F32) return true;
-  const int64_t g = dtype == NSW_DTYPE_BF16 ? 32 : 16;   // one step of the products
-  return M <= 0 || N <= 0 || K <= 0 || M >= (1LL << 31) || N >= (1LL << 31) || K >= (1LL << 31) || N % g || K % g;
+  const int64_t g = dtype == NSW_DTYPE_BF16 ? 32 : 16;   // one step of dx's contraction
+  return M <= 0 || N <= 0 || K <= 0 || M >= (1LL << 31) || N >= (1LL << 31) || K >= (1LL << 31) || N % g || K % 16;
 }
 
 bool bad_gated_sizes(int64_t M, int64_t H, int64_t K, int dtype) {
-  return H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype);
+  return H <= 0 || H >= (1LL << 30) || H % 16 || bad_sizes(M, 2 * H, K, dtype) || (dtype == NSW_DTYPE_BF16 && K % 32);
 }
 
 // fp32: both products side by side, then parts with the column sums.
@@ -208,7 +208,7 @@ extern "C" size_t nsw_linear_backward_workspace_size(int64_t M, int64_t N, int64
 extern "C" int nsw_linear_backward(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                                    int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "nsw_linear_backward";
-  NSW_CHECK_ARG(!bad_sizes(M, N, K, dtype), "%s: M=%lld, N=%lld, K=%lld in dtype %d: N and K must be multiples of 32 (bf16) / 16 (fp32)",
+  NSW_CHECK_ARG(!bad_sizes(M, N, K, dtype), "%s: M=%lld, N=%lld, K=%lld in dtype %d: N and K must be multiples of 32 and 16 (bf16) / 16 (fp32)",
                 what, (long long)M, (long long)N, (long long)K, dtype);
   NSW_CHECK_ARG(dy && (x || !dw) && w, "%s: dy, w and, for dw, x are required", what);
   const int64_t per = column_part_rows(M), parts = (M + per - 1) / per;

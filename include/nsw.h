@@ -137,7 +137,8 @@ int nsw_rmsnorm_roll_partition(const void* x, const void* w, float eps, void* xw
 /* F.linear + BiasLayer (+ GELU / residual) (models/layer_helpers.py:41-42,71-72,
  * models/mlp.py:80-93): y[M,N] = epi(x[M,K] . w[N,K]^T).  bias / residual may
  * be NULL when the epilogue does not use them.  Requires K % 16 == 0,
- * N % 8 == 0, 16-byte aligned x, w, y and residual. */
+ * N % 8 == 0, 16-byte aligned x, w, y and residual, w below 2 GiB (x and y may
+ * be larger). */
 int nsw_linear(const void* x, const void* w, const void* bias, const void* residual, void* y,
                int64_t M, int64_t N, int64_t K, int epilogue, int dtype, void* stream);
 

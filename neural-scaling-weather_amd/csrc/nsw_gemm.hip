@@ -376,9 +376,8 @@ int gemm_linear_remap(const void* x, const void* w, const void* bias, const void
 
 using namespace nsw;
 
-extern "C" int nsw_linear(const void* x, const void* w, const void* bias, const void* residual, void* y,
-                          int64_t M, int64_t N, int64_t K, int epilogue, int dtype, void* stream) {
-  const char* what = "nsw_linear";
+static int linear_rows(const void* x, const void* w, const void* bias, const void* residual, void* y, int64_t M, int64_t N,
+                       int64_t K, int epilogue, int dtype, void* stream, const char* what) {
   EpiArgs ea{};
   ea.bias = bias; ea.residual = residual;
   if (epilogue != NSW_EPI_NONE) NSW_CHECK_ARG(bias != nullptr, "%s: epilogue %d needs a bias", what, epilogue);
@@ -393,6 +392,23 @@ extern "C" int nsw_linear(const void* x, const void* w, const void* bias, const 
       return dispatch_gemm<EPI_BIAS_RESIDUAL>(dtype, x, w, y, M, N, K, ea, stream, what);
     default: return set_error(NSW_ERR_INVALID, "%s: unknown epilogue %d", what, epilogue);
   }
+}
+
+// x of 2 GiB or more (the buffer offsets' reach) goes in pieces of whole 256-row tiles.
+extern "C" int nsw_linear(const void* x, const void* w, const void* bias, const void* residual, void* y,
+                          int64_t M, int64_t N, int64_t K, int epilogue, int dtype, void* stream) {
+  const char* what = "nsw_linear";
+  const int64_t es = (int64_t)dtype_size(dtype), reach = (1LL << 31) - 1;
+  const int64_t rows = K > 0 && K < (1LL << 31) ? reach / (K * es) / 256 * 256 : 0;
+  if (rows <= 0 || M <= rows || M * K * es <= reach || M >= (1LL << 31))
+    return linear_rows(x, w, bias, residual, y, M, N, K, epilogue, dtype, stream, what);
+  for (int64_t m = 0; m < M; m += rows) {
+    const char* r = residual ? (const char*)residual + m * N * es : nullptr;
+    if (int rc = linear_rows((const char*)x + m * K * es, w, bias, r, (char*)y + m * N * es, std::min(rows, M - m), N, K, epilogue,
+                             dtype, stream, what))
+      return rc;
+  }
+  return NSW_OK;
 }
 
 extern "C" int nsw_gated_linear(const void* x, const void* w, const void* bias, void* h, int64_t M, int64_t H, int64_t K,

@@ -106,3 +106,52 @@ def test_training_step(device, dtype, M, C, H, out):
     want = ops.gated_linear_backward(dh, x.detach(), w1, b1)
     for got, v in zip((x.grad, m.fc1.weight.grad, m.bias1.bias.grad), want):
         assert torch.equal(got, v)
+
+
+@pytest.mark.parametrize("dtype,M,K", [(F32, 150_003, 4096), (BF16, 270_011, 4096), (BF16, 800_009, 1360)])
+@pytest.mark.parametrize("epi", [0, 3])
+def test_rows_of_more_than_2_gib(device, dtype, M, K, epi):
+    """x goes in pieces of rows: those on both sides of a border and the last ones, from float64 sums; with a residual."""
+    N = 40
+    g = torch.Generator(device=device).manual_seed(K)
+    x = torch.empty(M, K, dtype=dtype, device=device).normal_(0, 1, generator=g)
+    w = torch.empty(N, K, device=device).normal_(0, K ** -0.5, generator=g).to(dtype)
+    b, r = torch.randn(N, device=device).to(dtype), torch.randn(M, N, device=device).to(dtype)
+    y = ops.linear(x, w, b if epi else None, r if epi else None)
+    piece = (2 ** 31 - 1) // (K * x.element_size()) // 256 * 256
+    assert 0 < piece < M
+    for rows in (slice(0, 300), slice(piece - 300, piece + 300), slice(M - 300, M)):
+        a = x[rows].double()
+        want, mag = a @ w.double().t(), a.abs() @ w.double().abs().t()
+        before = None
+        if epi:
+            before = want + b.double()
+            want, mag = before + r[rows].double(), mag + b.double().abs() + r[rows].double().abs()
+        close(y[rows], want, mag, K + 2, dtype, before)
+
+
+def test_gated_mlp_with_more_than_2_gib_of_hidden_rows(device):
+    """Forward and backward; the last rows are those of a pass over them alone, within the sums' and the roundings' bounds."""
+    M, C, H = 150_003, 32, 4096
+    torch.manual_seed(0)
+    m = nsw.GatedMLP(C, H).to(device=device, dtype=F32)
+    with torch.no_grad():
+        for t in m.parameters():
+            t.copy_(torch.randn_like(t) * (t.shape[-1] ** -0.5 if t.dim() == 2 else 0.3))
+    x = torch.randn(M, C, device=device).requires_grad_()
+    dy = torch.randn(M, C, device=device)
+    y = m(x)
+    gx, gw = torch.autograd.grad(y, (x, m.fc2.weight), dy)
+    n = 500
+    xt = x.detach()[-n:].clone().requires_grad_()
+    yt = m(xt)
+    gt, = torch.autograd.grad(yt, xt, dy[-n:])
+    # relative 2-norm: sums of at most 4096 terms, two one after the other, 4096 2^-24 = 2.5e-4 each at worst
+    for a, c in ((y[-n:], yt), (gx[-n:], gt)):
+        assert (a - c).norm() <= 1e-3 * c.norm()
+    ref = torch.zeros(C, H, dtype=torch.float64, device=device)
+    w1, b1 = m.fc1.weight.detach().double(), m.bias1.bias.detach().double()
+    for i in range(0, M, 30_000):
+        g, u = (x.detach()[i:i + 30_000].double() @ w1.t() + b1).chunk(2, -1)
+        ref += dy[i:i + 30_000].double().t() @ (g * torch.sigmoid(g) * u)
+    assert (gw.double() - ref).norm() <= 1e-3 * ref.norm()

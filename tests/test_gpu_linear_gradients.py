@@ -80,3 +80,31 @@ def test_widths_without_rows(device):
     dx, dw, db = ops.linear_backward(torch.empty(0, 40, device=device), torch.empty(0, 16, device=device),
                                      torch.ones(40, 16, device=device))
     assert dx.shape == (0, 16) and dw.shape == (40, 16) and not dw.any() and db.shape == (40,) and not db.any()
+
+
+def test_fp32_gradients_of_more_than_2_gib(device):
+    """dy of more than 2^31 bytes: dx goes in pieces of rows (262143 and the rest here) and dw by itself.  dx on both sides of
+    the border and at the end from float64 sums, dw and db from sums over all rows; the same bits each on its own."""
+    M, N, K = 270_011, 2048, 32
+    g = torch.Generator(device=device).manual_seed(4)
+    dy = torch.empty(M, N, device=device).normal_(0, 1, generator=g)
+    x = torch.empty(M, K, device=device).normal_(0, 1, generator=g)
+    w = torch.empty(N, K, device=device).normal_(0, 0.02, generator=g)
+    piece = (2 ** 31 - 1) // (N * 4)
+    assert 0 < piece < M
+    dx, dw, db = ops.linear_backward(dy, x, w)
+    for rows in (slice(0, 300), slice(piece - 300, piece + 300), slice(M - 300, M)):
+        d, ww = dy[rows].double(), w.double()
+        over = (dx[rows].double() - d @ ww).abs() - (d.abs() @ ww.abs()) * (N + 8) * 2.0 ** -24
+        assert (over <= 0).all(), over.max().item()
+    dw64, mag, db64, dmag = 0, 0, 0, 0
+    for m in range(0, M, 50_000):
+        d, xx = dy[m:m + 50_000].double(), x[m:m + 50_000].double()
+        dw64, mag = dw64 + d.t() @ xx, mag + d.abs().t() @ xx.abs()
+        db64, dmag = db64 + d.sum(0), dmag + d.abs().sum(0)
+    assert ((dw.double() - dw64).abs() <= mag * (M + 8) * 2.0 ** -24).all()
+    assert (dw.double() - dw64).norm() <= 2e-5 * dw64.norm()        # by chance the square root of the terms, sqrt(M) 2^-24 = 3e-5 / 2
+    # a column sum is of at most M / 64 + 64 steps one after the other (rows of a part, parts)
+    assert ((db.double() - db64).abs() <= dmag * (M // 64 + 64) * 2.0 ** -24).all()
+    assert torch.equal(ops.linear_backward(dy, x, w, needs=(True, False, False))[0], dx)
+    assert torch.equal(ops.linear_backward(dy, x, w, needs=(False, True, False))[1], dw)

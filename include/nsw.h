@@ -499,6 +499,11 @@ int nsw_linear_fp8(const void* xq, const void* xs, const void* wq, const void* w
                    const void* residual, void* y, int64_t M, int64_t N, int64_t K, int epilogue, int dtype,
                    void* stream);
 
+/* Rows of the results of one workgroup of nsw_linear_fp8 (results in dtype): 16,
+ * 32 or 64 of the kernel for few rows, 128 or 256 of the tiled ones.  Host only;
+ * 0 for sizes or dtypes that are refused. */
+int nsw_linear_fp8_tile_rows(int64_t M, int64_t N, int64_t K, int dtype);
+
 /* HBM stream probe.  No counterpart in the reference: a measurement helper
  * for callers that report kernel rates against what the device sustains
  * (bench.py's achievable peaks).  dst == NULL: reads `bytes` from src with

@@ -663,37 +663,45 @@ int launch_rows(const Fp8Args& a, hipStream_t st, const char* what) {
   return check_launch(what);
 }
 
+int64_t tiles(int64_t M, int64_t N, int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
+
+// Rows of the results of one workgroup: 16, 32 or 64 (the kernel for few rows), 128 or 256.
+// Kernel by estimated time (us, fits to measured ones within 15%; bias and GELU, us
+// few rows / 128 x 128 / 256 x 256):
+//   1024 -> 4096 bf16   M 64: 5.0 / 9.2 / -    256: 13.2 / 9.4 / -    16384: - / 101 / 99    64800: - / 386 / 349
+//   4096 -> 1024 bf16   M 64: 14.5 / 23.2 / -  512: 27.0 / 24.1 / -   8192: - / 40 / 48      16384: - / 77 / 68
+//   1024 -> 4096 fp32   M 64: 5.1 / 14.3 / -   512: 23.8 / 14.8 / -
+// Few rows: every workgroup reads its weights once more for each 64 rows.
+template <typename T>
+int tile_rows(int64_t M, int64_t N, int64_t Kb) {
+  const double kb = (double)Kb;
+  const int mr = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  const double few = 2.3 + 0.0015 * kb * (double)tiles(M, N, 16 * mr, 16);
+  const double mid = sizeof(T) == 2 ? std::max(4.5 + 0.61 * kb, (double)tiles(M, N, 128, 128) / 512 * (3.9 + 1.085 * kb))
+                                    : std::max(5.5 + 1.0 * kb, (double)tiles(M, N, 128, 128) / 512 * (4 + 1.9 * kb));
+  if (few < mid && M <= 64 * 65535LL) return 16 * mr;       // the grid's y
+  if (sizeof(T) == 2 && 6 + (double)((tiles(M, N, Big8::BM, Big8::BN) + 255) / 256) * (8.5 + 1.53 * kb) < mid) return Big8::BM;
+  return Mid8::BM;
+}
+
 template <typename T, int EPI>
 int launch_fp8(const Fp8Args& a, hipStream_t st, const char* what) {
-  const double kb = a.Kb;
-  auto tiles = [&](int64_t bm, int64_t bn) { return ((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
-  // Kernel by estimated time (us, fits to measured ones within 15%; bias and GELU, us
-  // few rows / 128 x 128 / 256 x 256):
-  //   1024 -> 4096 bf16   M 64: 5.0 / 9.2 / -    256: 13.2 / 9.4 / -    16384: - / 101 / 99    64800: - / 386 / 349
-  //   4096 -> 1024 bf16   M 64: 14.5 / 23.2 / -  512: 27.0 / 24.1 / -   8192: - / 40 / 48      16384: - / 77 / 68
-  //   1024 -> 4096 fp32   M 64: 5.1 / 14.3 / -   512: 23.8 / 14.8 / -
-  // Few rows: every workgroup reads its weights once more for each 64 rows.
-  const int mr = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  const double few = 2.3 + 0.0015 * kb * (double)tiles(16 * mr, 16);
-  const double mid = sizeof(T) == 2 ? std::max(4.5 + 0.61 * kb, (double)tiles(128, 128) / 512 * (3.9 + 1.085 * kb))
-                                    : std::max(5.5 + 1.0 * kb, (double)tiles(128, 128) / 512 * (4 + 1.9 * kb));
-  if (few < mid && a.M <= 64 * 65535LL) {              // the grid's y
-    if (mr == 1) return launch_rows<T, EPI, 1>(a, st, what);
-    if (mr == 2) return launch_rows<T, EPI, 2>(a, st, what);
-    return launch_rows<T, EPI, 4>(a, st, what);
-  }
+  const int rows = tile_rows<T>(a.M, a.N, a.Kb);
+  if (rows == 16) return launch_rows<T, EPI, 1>(a, st, what);
+  if (rows == 32) return launch_rows<T, EPI, 2>(a, st, what);
+  if (rows == 64) return launch_rows<T, EPI, 4>(a, st, what);
   if constexpr (sizeof(T) == 2) {
     using TC = Big8;
     static_assert(TC::KB >= MAX_KB, "the longest rows' scales fit");
-    const int64_t n = tiles(TC::BM, TC::BN);
-    if (6 + (double)((n + 255) / 256) * (8.5 + 1.53 * kb) < mid) {
+    if (rows == TC::BM) {
+      const int64_t n = tiles(a.M, a.N, TC::BM, TC::BN);
       NSW_CHECK_ARG(n < (1LL << 31), "%s: too many tiles", what);
       hipLaunchKernelGGL((linear_fp8_deep_kernel<T, EPI, TC>), dim3((unsigned)n), dim3(TC::NW * 64), 0, st, a);
       return check_launch(what);
     }
   }
   using TC = Mid8;
-  const int64_t n = tiles(TC::BM, TC::BN);
+  const int64_t n = tiles(a.M, a.N, TC::BM, TC::BN);
   NSW_CHECK_ARG(n < (1LL << 31), "%s: too many tiles", what);
   hipLaunchKernelGGL((linear_fp8_kernel<T, EPI, TC>), dim3((unsigned)n), dim3(TC::NW * 64), 0, st, a);
   return check_launch(what);
@@ -746,6 +754,11 @@ extern "C" int nsw_quantize_fp8(const void* x, void* q, void* scale, int64_t R, 
   hipStream_t st = (hipStream_t)stream;
   return dtype == NSW_DTYPE_BF16 ? launch_quantize<bf16>(x, q, scale, R, K, rows_per_scale, st, what)
                                  : launch_quantize<float>(x, q, scale, R, K, rows_per_scale, st, what);
+}
+
+extern "C" int nsw_linear_fp8_tile_rows(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (M <= 0 || M >= (1LL << 38) || N <= 0 || N >= (1LL << 30) || N % 8 || K <= 0 || K % BLK || K > MAX_KB * BLK) return 0;
+  return dtype == NSW_DTYPE_BF16 ? tile_rows<bf16>(M, N, K / BLK) : dtype == NSW_DTYPE_F32 ? tile_rows<float>(M, N, K / BLK) : 0;
 }
 
 extern "C" int nsw_linear_fp8(const void* xq, const void* xs, const void* wq, const void* ws, const void* bias,

@@ -113,6 +113,7 @@ SIGNATURES = {
     "nsw_linear_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "nsw_linear_backward": (_int, [_vp] * 6 + [_i64, _i64, _i64, _int, _vp, ctypes.c_size_t, _vp]),
     "nsw_quantize_fp8": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "nsw_linear_fp8_tile_rows": (_int, [_i64, _i64, _i64, _int]),
     "nsw_linear_fp8": (_int, [_vp] * 7 + [_i64, _i64, _i64, _int, _int, _vp]),
     "nsw_residual_norm": (_int, [_vp] * 7 + [_i64, _i64, _i64, _f32, _f32, _int, _vp]),
     "nsw_residual_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),

@@ -336,6 +336,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
     if residual is not None and residual.shape != y.shape:
         raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")
+    if M == 0:
+        return y
     check(lib().nsw_linear(x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), M, N, K,
                            int(epilogue), dtype_code(x), _stream(dev)), "linear")
     return y

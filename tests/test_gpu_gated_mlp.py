@@ -155,3 +155,18 @@ def test_gated_mlp_with_more_than_2_gib_of_hidden_rows(device):
         g, u = (x.detach()[i:i + 30_000].double() @ w1.t() + b1).chunk(2, -1)
         ref += dy[i:i + 30_000].double().t() @ (g * torch.sigmoid(g) * u)
     assert (gw.double() - ref).norm() <= 1e-3 * ref.norm()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_no_rows(device, dtype):
+    """Empty outputs, gradients of zero rows and zeros for the parameters, as from the gated product and the norms."""
+    m = nsw.GatedMLP(64, 48, 40).to(device=device, dtype=dtype)
+    x, r = (torch.empty(2, 0, n, device=device, dtype=dtype).requires_grad_() for n in (64, 40))
+    y = m(x, r)
+    assert y.shape == (2, 0, 40) and y.dtype == dtype
+    y.sum().backward()
+    assert x.grad.shape == x.shape and r.grad.shape == r.shape
+    assert all(p.grad.shape == p.shape and not p.grad.any() for p in m.parameters())
+    with pytest.raises(ValueError, match="residual"):
+        ops.linear(x.detach(), torch.empty(8, 64, device=device, dtype=dtype), torch.empty(8, device=device, dtype=dtype),
+                   torch.empty(1, 8, device=device, dtype=dtype))

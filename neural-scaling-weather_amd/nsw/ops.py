@@ -318,8 +318,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """y = epi(x . weight^T): F.linear with an optional fused bias / GELU / residual.
     An epilogue leaves out what it has no part for (a residual without a bias: NSW_EPI_NONE).
     ``out`` (contiguous, x.shape[:-1] + (N,), x's dtype) receives y if given."""
-    dev = _dev(x, weight, bias, residual, out)
-    _same_dtype(x, weight, bias, residual, out)
+    at = _uniform(x, weight, bias, residual, out)
     K = x.shape[-1]
     N, Kw = weight.shape
     if Kw != K:
@@ -333,13 +332,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
             raise ValueError(f"linear: out has {out.numel()} elements, expected {M * N}")
         y = out.view(x.shape[:-1] + (N,))
     else:
-        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
+        y = x.new_empty(x.shape[:-1] + (N,))
     if residual is not None and residual.shape != y.shape:
         raise ValueError(f"residual shape {tuple(residual.shape)} != output {tuple(y.shape)}")
     if M == 0:
         return y
-    check(lib().nsw_linear(x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), M, N, K,
-                           int(epilogue), dtype_code(x), _stream(dev)), "linear")
+    _run("linear", at, lib().nsw_linear, x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), M, N, K,
+         int(epilogue), dtype_code(x))
     return y
 
 

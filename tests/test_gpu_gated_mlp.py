@@ -1,4 +1,5 @@
 """nsw.GatedMLP at every width that its gated product takes: forward and backward."""
+import contextlib
 import math
 
 import pytest
@@ -170,3 +171,23 @@ def test_no_rows(device, dtype):
     with pytest.raises(ValueError, match="residual"):
         ops.linear(x.detach(), torch.empty(8, 64, device=device, dtype=dtype), torch.empty(8, device=device, dtype=dtype),
                    torch.empty(1, 8, device=device, dtype=dtype))
+
+
+def test_another_current_device(device, monkeypatch):
+    """Every call of the block, forward and backward, makes its tensors' device the current one where another is."""
+    m = nsw.GatedMLP(64, 48).to(device=device, dtype=BF16)
+    x = torch.randn(5, 64, device=device).to(BF16).requires_grad_()
+    want, = torch.autograd.grad(m(x), x, torch.ones(5, 64, device=device, dtype=BF16))
+    entered = []
+
+    @contextlib.contextmanager
+    def enter(index):
+        entered.append(index)
+        yield
+
+    monkeypatch.setattr(ops, "_current_index", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", enter)
+    y = m(x)
+    assert entered == [0, 0]                                      # the gated product, the down projection
+    got, = torch.autograd.grad(y, x, torch.ones(5, 64, device=device, dtype=BF16))
+    assert entered == [0] * 4 and torch.equal(got, want)

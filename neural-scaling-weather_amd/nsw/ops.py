@@ -323,6 +323,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     N, Kw = weight.shape
     if Kw != K:
         raise ValueError(f"linear: x has {K} features, weight expects {Kw}")
+    if bias is not None and bias.numel() != N:
+        raise ValueError(f"linear: bias has {bias.numel()} elements, expected {N}")
     M = x.numel() // K
     if epilogue is None:
         epilogue = _lib.NSW_EPI_NONE if bias is None else (

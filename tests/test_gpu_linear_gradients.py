@@ -108,3 +108,12 @@ def test_fp32_gradients_of_more_than_2_gib(device):
     assert ((db.double() - db64).abs() <= dmag * (M // 64 + 64) * 2.0 ** -24).all()
     assert torch.equal(ops.linear_backward(dy, x, w, needs=(True, False, False))[0], dx)
     assert torch.equal(ops.linear_backward(dy, x, w, needs=(False, True, False))[1], dw)
+
+
+def test_a_bias_of_another_size_is_refused(device):
+    x, w = torch.zeros(3, 64, device=device), torch.zeros(32, 64, device=device)
+    for n in (8, 31, 64):
+        with pytest.raises(ValueError, match="bias"):
+            ops.linear(x, w, torch.zeros(n, device=device))
+        with pytest.raises(ValueError, match="bias"):
+            torch_ops.linear_epi(x, w, torch.zeros(n, device=device))

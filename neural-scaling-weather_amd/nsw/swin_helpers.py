@@ -270,7 +270,10 @@ class Block(nn.Module):
             raise ValueError(f"expected [B, T, {self.feat_size[0]}, {self.feat_size[1]}, C], got {tuple(x.shape)}")
         if x.shape[1] != self.temporal_context_window_size:
             raise ValueError("temporal dim does not match temporal_context_window_size")
-        self.mlp._check_fusable()
+        check = getattr(self.mlp, "_check_fusable", None)
+        if check is None:
+            raise NotImplementedError(f"the fused block runs the GELU MLP (nsw.MLP), not {type(self.mlp).__name__}")
+        check()
 
     @profile(name="shifted_wmha")
     def _shifted_window_attn(self, x: torch.Tensor) -> torch.Tensor:

@@ -117,3 +117,19 @@ def test_a_bias_of_another_size_is_refused(device):
             ops.linear(x, w, torch.zeros(n, device=device))
         with pytest.raises(ValueError, match="bias"):
             torch_ops.linear_epi(x, w, torch.zeros(n, device=device))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 32, 16), (77, 64, 48), (1000, 160, 1008), (40, 1600, 336), (2000, 4096, 1008), (8000, 2080, 176),
+                                   (16200, 4096, 1040), (64800, 1024, 16)])
+def test_bf16_rows_of_half_a_step_more(device, M, N, K):
+    """K 16 more than whole steps of 32, on all kernels of the gradients: the bounds as above."""
+    g = torch.Generator().manual_seed(K)
+    dy, x, w = (torch.randn(*s, generator=g).to(device=device, dtype=BF16) for s in ((M, N), (M, K), (N, K)))
+    got = ops.linear_backward(dy, x, w)
+    d, xx, ww = dy.double(), x.double(), w.double()
+    want = ((d @ ww, d.abs() @ ww.abs() * (N + 8)), (d.t() @ xx, d.abs().t() @ xx.abs() * (M + 8)),
+            (d.sum(0), d.abs().sum(0) * (512 + M // 64)))
+    step = torch.finfo(BF16).eps / 2
+    for t, (v, mag) in zip(got, want):
+        over = (t.double() - v).abs() - (mag * 2.0 ** -24 * (1 + step) + v.abs() * step * (1 + 1e-6))
+        assert (over <= torch.finfo(BF16).tiny).all(), over.max().item()

@@ -388,7 +388,8 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
                           needs: Sequence[bool] = (True, True, True)):
     """(dx, dweight, dbias) of gated_linear from the gradient of h, None where
     ``needs`` says so or there is no bias.  The projections are formed again
-    from x and weight."""
+    from x and weight; their gradients are rounded to x's dtype before the
+    products that give dx and dweight."""
     what = "gated_linear_backward"
     at, M, H, K, code = _gated_args(what, x, weight, bias, act)
     _uniform(x, dh)
@@ -474,7 +475,9 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
                epilogue: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """linear of operands from quantize_fp8 (x with rows=1, the weight with
     rows=128): y [..., N] in ``dtype`` (bfloat16 or float32; bias and residual
-    in it too), the epilogues of linear, sums in fp32."""
+    in it too), the epilogues of linear.  Sums of float32 results in fp32; those
+    of bfloat16 results keep 13 bits within a group of 8 products (at most
+    7 2^-13 of the sum of magnitudes), the groups are added in fp32."""
     what = "linear_fp8"
     at = _at(xq, x_scale, wq, w_scale, bias, residual)
     if dtype not in _DTYPES:

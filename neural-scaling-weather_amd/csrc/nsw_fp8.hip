@@ -90,7 +90,7 @@ __device__ __forceinline__ float row16_max(float x) {
 }
 
 // 1 x 128 blocks, 16 lanes each; block b of the R * Kb is row b / Kb.  Bound by HBM
-// (64800 x 1024 bf16 in 36 us: 5.6 TB/s), with four blocks' loads in flight a lane.
+// (64800 x 1024 bf16 in 34 us: 5.8 TB/s), with four blocks' loads in flight a lane.
 template <typename T>
 __global__ __launch_bounds__(QT) void quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                            uint8_t* __restrict__ scale, uint32_t blocks, int K, int Kb,
@@ -204,7 +204,7 @@ struct Tile8 {
   static_assert(RING + MAX_KB * (BM + NBLK) <= LDS, "the scales of the longest rows fit behind the ring");
 };
 // 128 x 128, two workgroups a CU, so that one's epilogue runs beside the other's main loop
-// (16384 x 4096 -> 1024 bf16 77 us, 1.8 PFLOP/s)
+// (16384 x 4096 -> 1024 bf16 69 us, 2.0 PFLOP/s, with bias and GELU 74)
 using Mid8 = Tile8<2, 2, 2, 2, 2, 80 * 1024>;
 
 // The tile's scales into LDS: [Kb][BM] bytes of its rows, [Kb][NBLK] of its weight blocks.
@@ -431,10 +431,11 @@ __global__ __launch_bounds__(TC::NW * 64, TC::MINW) void linear_fp8_kernel(Fp8Ar
 // block has just released.  A stage's one barrier frees the slot of the stage before it
 // for the copies of stage s + NST - 1; the reads of stage s may still be in flight there,
 // those of stage s - 1 are over, because its matrix instructions have been issued.
-// 8192^3 in 435 us, 2.53 PFLOP/s (the matrix units alone, on random values, 3.8); 64800 x
-// 4096 -> 1024 240 us; 64800 x 1024 -> 4096 312, with bias and GELU 361: there the
-// epilogue is two fifths of a tile's time.  Reads pinned a whole stage ahead, and four
-// waves of 128 x 128 with a third less LDS traffic, measure the same within 2%.
+// 8192^3 in 435 us, 2.53 PFLOP/s, the matrix units busy in 72% of the cycles at a clock of
+// 1.71 GHz (of 2.4); 64800 x 4096 -> 1024 242 us; 64800 x 1024 -> 4096 300, with bias and
+// GELU 363 (matrix units busy in 40%): there the epilogue is two fifths of a tile's time.
+// Reads pinned a whole stage ahead, and four waves of 128 x 128 with a third less LDS
+// traffic, measure the same within 2%.
 template <int WGM_, int NST_, int LDS_>
 struct Deep8 {
   static constexpr int WGM = WGM_, WGN = 2, MB = 2, NB = 4, NST = NST_, NW = WGM * WGN, KS = 64, LDS = LDS_;
@@ -668,9 +669,9 @@ int64_t tiles(int64_t M, int64_t N, int64_t bm, int64_t bn) { return ((M + bm - 
 // Rows of the results of one workgroup: 16, 32 or 64 (the kernel for few rows), 128 or 256.
 // Kernel by estimated time (us, fits to measured ones within 15%; bias and GELU, us
 // few rows / 128 x 128 / 256 x 256):
-//   1024 -> 4096 bf16   M 64: 5.0 / 9.2 / -    256: 13.2 / 9.4 / -    16384: - / 101 / 99    64800: - / 386 / 349
-//   4096 -> 1024 bf16   M 64: 14.5 / 23.2 / -  512: 27.0 / 24.1 / -   8192: - / 40 / 48      16384: - / 77 / 68
-//   1024 -> 4096 fp32   M 64: 5.1 / 14.3 / -   512: 23.8 / 14.8 / -
+//   1024 -> 4096 bf16   M 64: 4.9 / 9.1 / -    256: 14.5 / 9.3 / -    16384: - / 97 / 97     64800: - / 378 / 363
+//   4096 -> 1024 bf16   M 64: 14.5 / 23.1 / -  512: 27.5 / 24.0 / -   8192: - / 39 / 47      16384: - / 74 / 64
+//   1024 -> 4096 fp32   M 64: 5.0 / 15.0 / -   512: 27.9 / 15.4 / -
 // Few rows: every workgroup reads its weights once more for each 64 rows.
 template <typename T>
 int tile_rows(int64_t M, int64_t N, int64_t Kb) {

@@ -14,9 +14,9 @@
 //
 // The contraction of dw is the batch: long, with few results.  It is split S ways over
 // workgroups; the parts (fp32) are added in a fixed order by a second kernel.  Tiles of
-// 256 x 256 run at 1.49 PFLOP/s (64800 x 8192 -> 1024: dx 730 us, dw 730 + 20; the
-// matrix units alone reach 2.16 on such values), bound by the chip's power as the forward
-// GEMM; products too small for that take 128 x 128 and share one launch.
+// 256 x 256 run at 1.48 PFLOP/s (64800 x 8192 -> 1024: dx 731 us, dw 739 + 23), the matrix
+// units busy in 85% of the cycles at a clock of 1.65 GHz (of 2.4), which the chip's power sets
+// as for the forward GEMM; products too small for that take 128 x 128 and share one launch.
 #include <algorithm>
 
 #include "nsw_gemm_common.h"

@@ -3,8 +3,10 @@
 // EPI_GATED_GRAD).  Every operand is read as it lies: bf16 by grad_products, fp32 by the
 // forward GEMM's kernel with turned operands (EPI_BATCH), dx and dw side by side in pieces
 // of their contractions, the pieces' products added in a fixed order.  fp32, 16200 rows,
-// 192 -> 768: 217 us in all, of it 80 for the sums formed again and ~130 for dx and dw (147
-// TFLOP/s of fp32 in six bf16 products a value); on transposed copies it took 257.
+// 192 -> 768, kernels in a loop of passes: 76 us for the sums formed again, 144 for dx and dw
+// (132 TFLOP/s of fp32 in six bf16 products a value; the matrix units busy in two thirds of the
+// cycles, the vector ones, which split the operands, in four fifths), 5 for the parts; on
+// transposed copies dx and dw took 40 more.
 #include <algorithm>
 
 #include "nsw_gemm_common.h"

@@ -21,7 +21,7 @@
 // lane's sums for S and Q, which go to a partial row of the workgroup and from there
 // through a second kernel in a fixed order (no atomics: the same bits every time).
 // The next row's loads are issued before the present row's arithmetic.  129600 x 1024
-// bf16: forward 180 us (5.9 TB/s), backward 316 us (5.0 TB/s, the second kernel included).
+// bf16: forward 178 us (6.0 TB/s), backward 302 + 6 us (5.2 TB/s, the second kernel included).
 #include <algorithm>
 
 #include "nsw_common.h"

@@ -298,6 +298,6 @@ class Block(nn.Module):
                                         self._eps(x.dtype), self.mlp.gelu_tanh)
 
 
-# Names used by north_star / other Swin code bases.
+# Names used by other Swin code bases.
 SwinTransformerBlock = Block
 WindowAttention = WindowMultiHeadAttention

@@ -166,6 +166,7 @@ class Fp8Linear(nn.Module):
         q, scale = torch.ops.nsw.quantize_fp8(weight.detach(), ops.FP8_BLOCK)
         self.register_buffer("weight", q)
         self.register_buffer("weight_scale", scale)
+        self.in_features = weight.shape[1]      # the quantised rows are padded
         self.register_buffer("bias", None if bias is None else bias.detach().clone())
         self.epilogue = epilogue
 
@@ -183,6 +184,8 @@ class Fp8Linear(nn.Module):
             self.weight, self.weight_scale = self.weight.view(torch.float8_e4m3fn), self.weight_scale.view(torch.float8_e8m0fnu)
 
     def forward(self, x, residual=None):
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"Fp8Linear: x has {x.shape[-1]} features, weight expects {self.in_features}")
         epi = self.epilogue
         if residual is not None and epi in (_lib.NSW_EPI_BIAS_GELU, _lib.NSW_EPI_BIAS_GELU_TANH):
             raise NotImplementedError("a residual after a GELU is not fused")

@@ -133,3 +133,23 @@ def test_bf16_rows_of_half_a_step_more(device, M, N, K):
     for t, (v, mag) in zip(got, want):
         over = (t.double() - v).abs() - (mag * 2.0 ** -24 * (1 + step) + v.abs() * step * (1 + 1e-6))
         assert (over <= torch.finfo(BF16).tiny).all(), over.max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(70, 40, 64), (700, 1000, 112)])
+def test_replays_of_padded_gradients(device, dtype, M, N, K):
+    """Widths that go through copies, captured: every replay the eager result, with eager work between."""
+    g = torch.Generator().manual_seed(N)
+    dy, x, w = (torch.randn(*s, generator=g).to(device=device, dtype=dtype) for s in ((M, N), (M, K), (N, K)))
+    want = ops.linear_backward(dy, x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_backward(dy, x, w)
+    for i in range(4):
+        dy.copy_(torch.randn(M, N, generator=g))
+        want = ops.linear_backward(dy, x, w)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -159,7 +159,8 @@ int nsw_gated_linear(const void* x, const void* w, const void* bias, void* h, in
  * x and w, so nothing but the inputs is kept from the forward pass.  Their
  * gradients [M, 2H] are rounded to dtype before the products that give dx and dw
  * (not db): in bf16 the errors of those are 1.4 times that of one rounding at the
- * end (relative 2-norm 2.3e-3 for 1.7e-3).  Sums over rows in a fixed order.  Results must not overlap the inputs.  Workspace (16-byte aligned) of
+ * end (relative 2-norm 2.3e-3 for 1.7e-3).  Sums over rows in a fixed order.
+ * Results must not overlap the inputs.  Workspace (16-byte aligned) of
  * nsw_gated_linear_backward_workspace_size bytes, 0 for sizes that are
  * refused. */
 size_t nsw_gated_linear_backward_workspace_size(int64_t M, int64_t H, int64_t K, int dtype);

@@ -100,7 +100,8 @@ class Conv2DLayer(nn.Module):
                 raise NotImplementedError("a residual without a conv bias is not fused")
             y = torch_ops.linear_epi(pm, wp)
         else:
-            y = torch_ops.linear_epi(pm, wp, b, residual=residual, left_out=(self.conv.weight, self.conv.bias))
+            left_out = (self.conv.weight, self.conv.bias) if torch.is_grad_enabled() else ()
+            y = torch_ops.linear_epi(pm, wp, b, residual=residual, left_out=left_out)
         return y.view(B, T, H // p, W // p, wp.shape[0])
 
     def tokens_windowed(self, x: torch.Tensor, residual: torch.Tensor, window_size, shift_size,

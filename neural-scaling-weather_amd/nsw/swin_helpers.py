@@ -150,10 +150,11 @@ class WindowMultiHeadAttention(nn.Module):
             H, W, ws, sh, T = geometry
             geo = [int(H), int(W), int(ws[0]), int(ws[1]), int(sh[0]), int(sh[1]), int(T)]
         o = torch.ops.nsw.window_attention(qkv, self.num_heads, float(self.scale), mask, geo)
-        return torch_ops.linear_epi(o, self.proj.weight, self.biasproj.bias,
-                                    left_out=(self.q.weight, self.k.weight, self.v.weight, self.biasq.bias,
-                                              self.biask.bias, self.biasv.bias, self.q_norm.norm.weight,
-                                              self.k_norm.norm.weight))
+        left_out = ()
+        if torch.is_grad_enabled():
+            left_out = (self.q.weight, self.k.weight, self.v.weight, self.biasq.bias, self.biask.bias, self.biasv.bias,
+                        self.q_norm.norm.weight, self.k_norm.norm.weight)
+        return torch_ops.linear_epi(o, self.proj.weight, self.biasproj.bias, left_out=left_out)
 
 
 class Block(nn.Module):

@@ -51,6 +51,7 @@ extern "C" {
 #define NSW_ACT_GELU 1      /* exact-erf GELU, as NSW_EPI_BIAS_GELU: within 1.5e-7 |g| (fp32; absolute, so
                                the far negative tail has fewer bits) and 0.15 of half a step (bf16) */
 #define NSW_ACT_GELU_TANH 2 /* tanh-form GELU           */
+#define NSW_ACT_NONE 3      /* g; nsw_group_norm only   */
 
 const char* nsw_last_error(void);
 int nsw_version(void);
@@ -511,6 +512,30 @@ int nsw_linear_fp8(const void* xq, const void* xs, const void* wq, const void* w
  * 32 or 64 of the kernel for few rows, 128 or 256 of the tiled ones.  Host only;
  * 0 for sizes or dtypes that are refused. */
 int nsw_linear_fp8_tile_rows(int64_t M, int64_t N, int64_t K, int dtype);
+
+/* Group norm with an activation, channels last (no counterpart in the reference):
+ * x, y [B, R, C], a group of C / groups neighbouring channels,
+ *   y = act((x - mean) / sqrt(var + eps) * weight + bias)
+ * with the mean and (biased) variance over a sample's R rows and a group's channels;
+ * weight, bias [C], NULL: 1, 0; act NSW_ACT_*.  stats [B, groups, 2] fp32 receives mean
+ * and 1 / sqrt(var + eps).  Statistics of centred values and in fp32, whatever the dtype;
+ * one rounding of y.  x, y, weight, bias of one dtype, 16-byte aligned; C a multiple
+ * of 8 (bf16) / 4 (fp32) and of groups, at most 4096 / 2048; B below 2^20.  y may be x.
+ * Workspace (16-byte aligned) of nsw_group_norm_workspace_size bytes, 0 for sizes
+ * that are refused.  B == 0 or R == 0: nothing is written. */
+size_t nsw_group_norm_workspace_size(int64_t B, int64_t R, int64_t C, int64_t groups, int dtype);
+int nsw_group_norm(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t B, int64_t R,
+                   int64_t C, int64_t groups, float eps, int act, int dtype, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* Gradients of nsw_group_norm from that of y: dx [B, R, C], dweight, dbias [C], each
+ * where not NULL (B == 0 or R == 0: zeros).  stats as nsw_group_norm left them.  Sums
+ * over rows and samples in fp32 and a fixed order.  dx may be dy or x.  Workspace as
+ * above. */
+size_t nsw_group_norm_backward_workspace_size(int64_t B, int64_t R, int64_t C, int64_t groups, int dtype);
+int nsw_group_norm_backward(const void* dy, const void* x, const float* stats, const void* weight, const void* bias,
+                            void* dx, void* dweight, void* dbias, int64_t B, int64_t R, int64_t C, int64_t groups,
+                            int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* HBM stream probe.  No counterpart in the reference: a measurement helper
  * for callers that report kernel rates against what the device sustains

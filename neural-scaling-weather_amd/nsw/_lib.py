@@ -27,6 +27,7 @@ NSW_EPI_BIAS_GELU_TANH = 4
 NSW_ACT_SILU = 0
 NSW_ACT_GELU = 1
 NSW_ACT_GELU_TANH = 2
+NSW_ACT_NONE = 3
 NSW_METRICS_SCRATCH_BYTES = 1 << 20   # scratch of nsw_weighted_metrics_unnorm_noalloc (per GPU)
 
 _vp = ctypes.c_void_p
@@ -119,6 +120,10 @@ SIGNATURES = {
     "nsw_residual_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "nsw_residual_norm_backward": (_int, [_vp] * 12 + [_i64, _i64, _i64, _f32, _f32, _int, _vp, ctypes.c_size_t,
                                                        _vp]),
+    "nsw_group_norm_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _int]),
+    "nsw_group_norm": (_int, [_vp] * 5 + [_i64, _i64, _i64, _i64, _f32, _int, _int, _vp, ctypes.c_size_t, _vp]),
+    "nsw_group_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _int]),
+    "nsw_group_norm_backward": (_int, [_vp] * 8 + [_i64, _i64, _i64, _i64, _int, _int, _vp, ctypes.c_size_t, _vp]),
 }
 
 _lib = None

@@ -155,6 +155,40 @@ class ResidualNorm(nn.Module):
                                        eps.pop() if eps else None)
 
 
+class GroupNorm(nn.Module):
+    """Group norm with an activation, channels last and with gradients (no
+    counterpart in the reference): act(GroupNorm(x) * weight + bias) of x [B, ..., C],
+    the statistics over a sample's rows and a group's channels.  act_layer:
+    None, nn.SiLU or nn.GELU (approximate "none" or "tanh")."""
+
+    def __init__(self, num_groups, num_channels, act_layer=None, eps=1e-5, affine=True, comm_metadata=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f"GroupNorm: {num_channels} channels are not a multiple of {num_groups} groups")
+        self.num_groups, self.num_channels, self.eps = num_groups, num_channels, float(eps)
+        self.act = None if act_layer is None else act_layer()
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+        for p in (self.weight, self.bias):
+            if p is not None:
+                p.comm_metadata = comm_metadata or {"sharded": [None], "shared": [], "reduce": []}
+
+    @property
+    def act_name(self) -> str:
+        if self.act is None:
+            return "none"
+        if isinstance(self.act, nn.SiLU):
+            return "silu"
+        if isinstance(self.act, nn.GELU) and self.act.approximate in ("none", "tanh"):
+            return "gelu" if self.act.approximate == "none" else "gelu_tanh"
+        raise NotImplementedError("libnsw's group norm takes no activation, nn.SiLU or nn.GELU (approximate 'none' or 'tanh')")
+
+    def forward(self, x):
+        if x.shape[-1] != self.num_channels:
+            raise ValueError(f"GroupNorm: x has {x.shape[-1]} channels, expected {self.num_channels}")
+        return torch_ops.group_norm(x, self.num_groups, self.weight, self.bias, self.act_name, self.eps)
+
+
 class Fp8Linear(nn.Module):
     """A linear layer served in 8-bit floating point: the weight is quantised
     once (e4m3, a power-of-two scale for each 128 x 128 block), the rows in

@@ -310,6 +310,70 @@ def residual_norm_backward(dy: Optional[torch.Tensor], dz: Optional[torch.Tensor
     return db, ds, dp, dg, dn
 
 
+_NORM_ACTS = {"none": _lib.NSW_ACT_NONE, "silu": _lib.NSW_ACT_SILU, "gelu": _lib.NSW_ACT_GELU,
+              "gelu_tanh": _lib.NSW_ACT_GELU_TANH}
+
+
+def _group_norm_args(what, x, groups, weight, bias, act):
+    """(device index, B, R, C, act code) of a group norm, its arguments checked."""
+    at = _uniform(x, weight, bias)
+    if act not in _NORM_ACTS:
+        raise ValueError(f"{what}: act must be one of {sorted(_NORM_ACTS)}, got {act!r}")
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"{what}: x has shape {tuple(shape)}, expected [B, ..., C]")
+    B, C = shape[0], shape[-1]
+    if C == 0 or groups < 1 or C % groups:
+        raise ValueError(f"{what}: {C} channels are not a multiple of {groups} groups")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.shape != (C,):
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({C},)")
+    return at, B, x.numel() // (B * C) if B else 0, C, _NORM_ACTS[act]
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               act: str = "none", eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, stats): y = act(GroupNorm(x) * weight + bias) of x [B, ..., C], channels
+    last, the mean and variance over a sample's rows and a group's channels; act "none",
+    "silu", "gelu" (exact erf) or "gelu_tanh".  stats [B, groups, 2] fp32: mean and
+    1 / sqrt(var + eps), for group_norm_backward (zeros where a sample has no rows)."""
+    at, B, R, C, code = _group_norm_args("group_norm", x, groups, weight, bias, act)
+    y = torch.empty_like(x)
+    if B == 0 or R == 0:
+        return y, x.new_zeros((B, groups, 2), dtype=torch.float32)
+    dt = dtype_code(x)
+    stats = x.new_empty((B, groups, 2), dtype=torch.float32)
+    nbytes = _workspace_bytes(lib(), "nsw_group_norm_workspace_size", B, R, C, groups, dt)
+    ws = x.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run("group_norm", at, lib().nsw_group_norm, x.data_ptr(), _p(weight), _p(bias), y.data_ptr(), stats.data_ptr(), B, R, C,
+         groups, float(eps), code, dt, ws.data_ptr(), nbytes)
+    return y, stats
+
+
+def group_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, groups: int,
+                        weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, act: str = "none",
+                        needs: Sequence[bool] = (True, True, True)):
+    """(dx, dweight, dbias) of group_norm from the gradient of y and the forward
+    pass's stats, None where ``needs`` says so or there is no such parameter."""
+    what = "group_norm_backward"
+    at, B, R, C, code = _group_norm_args(what, x, groups, weight, bias, act)
+    _uniform(x, dy)
+    if dy.shape != x.shape:
+        raise ValueError(f"{what}: dy has shape {tuple(dy.shape)}, expected {tuple(x.shape)}")
+    _dev(x, stats)
+    if stats.dtype != torch.float32 or stats.shape != (B, groups, 2):
+        raise ValueError(f"{what}: stats is {stats.dtype} {tuple(stats.shape)}, expected float32 {(B, groups, 2)}")
+    dx, dw, db = _grads(needs, x, weight, bias)
+    if B == 0 or R == 0:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    dt = dtype_code(x)
+    nbytes = _workspace_bytes(lib(), "nsw_group_norm_backward_workspace_size", B, R, C, groups, dt)
+    ws = x.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run(what, at, lib().nsw_group_norm_backward, dy.data_ptr(), x.data_ptr(), stats.data_ptr(), _p(weight), _p(bias),
+         _p(dx), _p(dw), _p(db), B, R, C, groups, code, dt, ws.data_ptr(), nbytes)
+    return dx, dw, db
+
+
 # -------------------------------------------------------------------- GEMM ---
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,

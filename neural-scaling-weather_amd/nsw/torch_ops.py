@@ -315,6 +315,66 @@ def residual_norm(branch: torch.Tensor, skip: torch.Tensor, post_weight: Optiona
     return y, None if norm_weight is None else z
 
 
+@torch.library.custom_op("nsw::group_norm", mutates_args=())
+def _group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], act: str,
+                eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(act(GroupNorm(x) * weight + bias), stats) of x [B, ..., C], channels last."""
+    return ops.group_norm(_dense(x), groups, None if weight is None else _dense(weight),
+                          None if bias is None else _dense(bias), act=act, eps=eps)
+
+
+@_group_norm.register_fake
+def _(x, groups, weight, bias, act, eps):
+    return (torch.empty_like(x, memory_format=torch.contiguous_format),
+            x.new_empty((x.shape[0], groups, 2), dtype=torch.float32))
+
+
+@torch.library.custom_op("nsw::group_norm_backward", mutates_args=())
+def _group_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, groups: int,
+                         weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], act: str,
+                         needs: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias); empty ([0]) where ``needs`` is False or there is no such parameter."""
+    return _or_empty(x, *ops.group_norm_backward(
+        _dense(dy), _dense(x), _dense(stats), groups, None if weight is None else _dense(weight),
+        None if bias is None else _dense(bias), act=act, needs=tuple(needs)))
+
+
+@_group_norm_backward.register_fake
+def _(dy, x, stats, groups, weight, bias, act, needs):
+    return tuple(x.new_empty(t.shape if n and t is not None else (0,)) for n, t in zip(needs, (x, weight, bias)))
+
+
+def _group_norm_setup(ctx, inputs, output):
+    x, groups, weight, bias, act, eps = inputs
+    ctx.groups, ctx.act = groups, act
+    ctx.given = [t is not None for t in (weight, bias)]
+    ctx.save_for_backward(x, output[1], *[t for t in (weight, bias) if t is not None])
+    ctx.set_materialize_grads(False)
+
+
+def _group_norm_grad(ctx, dy, dstats):
+    if dstats is not None:
+        raise NotImplementedError("nsw.group_norm: the statistics have no gradient of their own")
+    if dy is None:
+        return (None,) * 6
+    x, stats, *rest = ctx.saved_tensors
+    rest = iter(rest)
+    weight, bias = (next(rest) if g else None for g in ctx.given)
+    need = [ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3]]
+    got = torch.ops.nsw.group_norm_backward(dy, x, stats, ctx.groups, weight, bias, ctx.act, need)
+    dx, dw, db = (g if n else None for n, g in zip(need, got))
+    return dx, None, dw, db, None, None
+
+
+_group_norm.register_autograd(_group_norm_grad, setup_context=_group_norm_setup)
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               act: str = "none", eps: float = 1e-5) -> torch.Tensor:
+    """torch.ops.nsw.group_norm with ops.group_norm's defaults: y alone."""
+    return torch.ops.nsw.group_norm(x, int(groups), weight, bias, act, float(eps))[0]
+
+
 @torch.library.custom_op("nsw::linear_to_window", mutates_args=())
 def linear_to_window(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, residual: torch.Tensor,
                      image: List[int], window_size: List[int], shift_size: List[int]) -> Tuple[torch.Tensor,

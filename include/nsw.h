@@ -537,6 +537,37 @@ int nsw_group_norm_backward(const void* dy, const void* x, const float* stats, c
                             void* dx, void* dweight, void* dbias, int64_t B, int64_t R, int64_t C, int64_t groups,
                             int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Window attention with a learned position bias (no counterpart in the reference, whose
+ * windows have none): qkv [Bw, L, 3C] -> o [Bw, L, C] as nsw_window_attention, with
+ *   z_ij = scale q_i k_j + table[buckets[r(i, j)], head] + mask_ij,  o_i = softmax_j(z_ij) v_j
+ * A window is T x ws0 x ws1 = L tokens (a sequence: 1 x 1 x L), its displacements
+ *   r(i, j) = ((t_i - t_j + T-1) (2 ws0-1) + (h_i - h_j + ws0-1)) (2 ws1-1) + (w_i - w_j + ws1-1),
+ * R = (2T-1)(2 ws0-1)(2 ws1-1) <= 8192 of them; buckets [R] int32 in [0, num_buckets) (one
+ * outside counts as no bias); table [num_buckets, num_heads] in dtype.  mask [nW_mask,
+ * L, L] fp32 is added (NULL: none; -inf takes a pair out, a row with none left gives zeros), or
+ * the shift (s0, s1) of an image of H x W tokens gives nsw_window_attention's.  stats
+ * [Bw, num_heads, L, 2] fp32 receives each row's maximum of z and log2 of its sum of exp(z -
+ * maximum).  bf16: fp32 logits and sums, probabilities rounded to bf16 for the product
+ * with v.  Head dims 4, 8, 16, 32, 64, 128; C a multiple of 8; qkv, o, stats 16-byte aligned. */
+int nsw_position_attention(const void* qkv, const void* table, const int32_t* buckets, const float* mask,
+                           int64_t nW_mask, void* o, float* stats, int64_t Bw, int64_t L, int64_t C,
+                           int64_t num_heads, float scale, int64_t num_buckets, int64_t T, int64_t ws0, int64_t ws1,
+                           int64_t H, int64_t W, int64_t s0, int64_t s1, int dtype, void* stream);
+
+/* Its gradients from that of o (dout): dqkv [Bw, L, 3C] and, where not NULL, dtable
+ * [num_buckets, num_heads] (Bw == 0: zeros), which sums fp32 values in a fixed order;
+ * o and stats as nsw_position_attention left them.  The workspace (16-byte aligned, of
+ * nsw_position_attention_backward_workspace_size bytes, 0 for sizes that are refused) may be
+ * NULL without dtable.  bf16: p and dz are rounded to bf16 for the products. */
+size_t nsw_position_attention_backward_workspace_size(int64_t Bw, int64_t L, int64_t C, int64_t num_heads, int64_t T,
+                                                      int64_t ws0, int64_t ws1, int dtype);
+int nsw_position_attention_backward(const void* dout, const void* qkv, const void* o, const float* stats,
+                                    const void* table, const int32_t* buckets, const float* mask, int64_t nW_mask,
+                                    void* dqkv, void* dtable, int64_t Bw, int64_t L, int64_t C, int64_t num_heads,
+                                    float scale, int64_t num_buckets, int64_t T, int64_t ws0, int64_t ws1, int64_t H,
+                                    int64_t W, int64_t s0, int64_t s1, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* HBM stream probe.  No counterpart in the reference: a measurement helper
  * for callers that report kernel rates against what the device sustains
  * (bench.py's achievable peaks).  dst == NULL: reads `bytes` from src with

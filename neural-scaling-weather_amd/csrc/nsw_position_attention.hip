@@ -1,0 +1,303 @@
+// Window attention with a learned position bias, forward:
+//
+//   z_ij = scale q_i k_j + table[bucket[r(i, j)], head] + mask_ij,  o_i = softmax_j(z_ij) v_j
+//
+// r(i, j) the displacement between tokens i and j of a window of T x A x W tokens, a
+// difference of two codes (one subtraction; the bias is then one LDS read).  A row whose
+// mask leaves nothing (every z_ij = -inf) gives zeros.
+//
+// A workgroup takes QB 64-query blocks of one (window, head): it steps over 64-key tiles in
+// LDS with the running maximum m and sum of each row, so any length goes.  S^T = K Q^T puts a
+// query on a lane, whose probabilities are then the right operand of O^T = V^T P^T as they
+// lie.  Logits in natural units, exp2((z - m) log2 e): a mask of the lowest float stays
+// finite, and all-lowest rows come out uniform, as in fp32 on the formula.  fp32 statistics
+// and sums; bf16: probabilities (at most 1) are rounded to bf16 for the product with v, their
+// sum is of the unrounded ones.  stats keeps m and log2 of the sum apart, since their sum
+// would lose the second where |m| is large.
+#include <cmath>
+
+#include "nsw_position_attention.h"
+
+namespace nsw {
+
+int check_geom(int64_t B, int64_t T, int64_t H, int64_t W, int64_t ws0, int64_t ws1, const char* what);
+
+namespace posattn {
+
+namespace {
+
+template <typename T, int HD, int QB, bool MASK>
+__global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
+  typedef Dim<T, HD> D;
+  constexpr int KT = 64;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* Ks = (T*)smem;
+  T* Vs = Ks + KT * D::STR;
+  int* kinfo = (int*)(Vs + KT * D::STR);
+  float* rel = (float*)(kinfo + KT);
+
+  const uint32_t b = (uint32_t)xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const uint32_t item = a.dnqc.div(b);
+  const int qc = (int)(b - item * (uint32_t)a.nqc);
+  const int64_t win = a.dheads.div(item);
+  const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
+  const int L = a.L, C = a.C;
+  const int64_t ld = 3 * (int64_t)C;
+  const T* base = (const T*)a.qkv + win * L * ld + head * a.hd;
+  const int wi = (int)(win % a.nW);
+  const bool shifted = !MASK && wi >= a.band0;
+  const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
+  const int q0 = qc * 64 * QB + wave * 16;                 // block i of the wave: q0 + 64 i
+
+  TileCopy<T, HD, KT> kc, vc;
+  kc.load(base + C, ld, L, a.hd);
+  vc.load(base + 2 * C, ld, L, a.hd);
+  typename D::Frag qf[QB][D::NS];
+  int qinfo[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = q0 + 64 * i + fr, qr = q < L ? q : L - 1;
+    qinfo[i] = info_of(a, qr, shifted) + a.off;
+#pragma unroll
+    for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(base + qr * ld, s, fg, a.hd);
+  }
+  load_rel<T>(a, head, rel);
+
+  f32x4 O[QB][D::ND];
+  float m[QB], l[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D::ND; ++d) O[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int k0 = 0; k0 < L; k0 += KT) {
+    if (k0) wg_barrier();                                  // the tile before is read
+    kc.store(Ks);
+    vc.store(Vs);
+    if (tid < KT) kinfo[tid] = info_of(a, k0 + tid, shifted);
+    wg_barrier();
+    const int left = L - k0;                               // keys from k0 on
+    if (left > KT) {
+      kc.load(base + (int64_t)(k0 + KT) * ld + C, ld, left - KT, a.hd);
+      vc.load(base + (int64_t)(k0 + KT) * ld + 2 * C, ld, left - KT, a.hd);
+    }
+    f32x4 S[QB][4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      if (16 * kb < left) {
+        typename D::Frag kf[D::NS];
+#pragma unroll
+        for (int s = 0; s < D::NS; ++s) kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg, HD);
+        const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
+        const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+          f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < D::NS; ++s) t = mma(kf[s], qf[i][s], t);
+          const int q = q0 + 64 * i + fr;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int diff = qinfo[i] - kn[r];
+            float z = fmaf(t[r], a.scale, rel[diff & (MAX_R - 1)]);
+            const int key = k0 + 16 * kb + 4 * fg + r;
+            if constexpr (MASK) {
+              if (q < L && key < L) z += mask[(int64_t)q * L + key];
+            } else if (shifted) {
+              z += ((qinfo[i] - a.off) ^ kn[r]) >> 30 ? -100.f : 0.f;
+            }
+            t[r] = key < L ? z : -INFINITY;
+          }
+          S[i][kb] = t;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < QB; ++i) S[i][kb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      float mx = S[i][0][0];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[i][kb][r]);
+      mx = fmaxf(m[i], rows4_max(mx));
+      const float at = mx == -INFINITY ? 0.f : mx;
+      const float f = __builtin_amdgcn_exp2f((m[i] - at) * LOG2E);
+      m[i] = mx;
+      float t = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f((S[i][kb][r] - at) * LOG2E);
+          S[i][kb][r] = p;
+          t += p;
+        }
+      l[i] = fmaf(l[i], f, t);
+#pragma unroll
+      for (int d = 0; d < D::ND; ++d) O[i][d] *= f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      if (32 * ks < left) {
+        typename D::TFrag vf[D::ND];
+#pragma unroll
+        for (int d = 0; d < D::ND; ++d) vf[d] = col_frag<T, D::STR>(Vs + 32 * ks * D::STR, 16 * d, fr, fg);
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+          const typename D::TFrag pf = pair_frag<T>(S[i][2 * ks], S[i][2 * ks + 1]);
+#pragma unroll
+          for (int d = 0; d < D::ND; ++d) O[i][d] = mma(vf[d], pf, O[i][d]);
+        }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = q0 + 64 * i + fr;
+    const float t = rows4_sum(l[i]);
+    const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;    // an empty row: zeros; NaN stays
+    if (q < L) {
+      T* row = (T*)a.o + (win * L + q) * (int64_t)C + head * a.hd;
+#pragma unroll
+      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(row, 16 * d + 4 * fg, a.hd, O[i][d], inv);
+      if (fg == 0) *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + q) * 2) = f32x2{m[i], __builtin_amdgcn_logf(t)};
+    }
+  }
+}
+
+template <typename T, int HD, int QB>
+int launch_qb(Args a, hipStream_t st) {
+  typedef Dim<T, HD> D;
+  a.nqc = (a.L + 64 * QB - 1) / (64 * QB);
+  a.dnqc = FastDiv::make((uint32_t)a.nqc);
+  const int64_t grid = a.Bw * a.heads * a.nqc;
+  if (grid >= (1LL << 31)) return set_error(NSW_ERR_INVALID, "nsw_position_attention: too large");
+  const size_t lds = (size_t)2 * 64 * D::STR * sizeof(T) + 64 * sizeof(int) + (size_t)a.R * sizeof(float);
+  if (a.mask != nullptr) hipLaunchKernelGGL((forward_kernel<T, HD, QB, true>), dim3((unsigned)grid), dim3(NT), lds, st, a);
+  else hipLaunchKernelGGL((forward_kernel<T, HD, QB, false>), dim3((unsigned)grid), dim3(NT), lds, st, a);
+  return check_launch("nsw_position_attention");
+}
+
+// Query blocks of a wave: as many as the window has, at most 3 (2 where registers end).
+template <typename T, int HD>
+int launch_hd(const Args& a, hipStream_t st) {
+  constexpr int MOST = HD == 128 ? (sizeof(T) == 4 ? 1 : 2) : HD == 64 && sizeof(T) == 4 ? 2 : 3;
+  if (a.L <= 64 || MOST == 1) return launch_qb<T, HD, 1>(a, st);
+  if constexpr (MOST >= 2)
+    if (a.L <= 128 || MOST == 2) return launch_qb<T, HD, 2>(a, st);
+  if constexpr (MOST >= 3) return launch_qb<T, HD, 3>(a, st);
+  return NSW_OK;
+}
+
+template <typename T>
+int launch_t(const Args& a, hipStream_t st) {
+  switch (a.hd) {
+    case 4: case 8: case 16: return launch_hd<T, 16>(a, st);
+    case 32: return launch_hd<T, 32>(a, st);
+    case 64: return launch_hd<T, 64>(a, st);
+    default: return launch_hd<T, 128>(a, st);
+  }
+}
+
+// The arguments of both passes, checked.
+int make_args(Args& a, const char* what, int64_t Bw, int64_t L, int64_t C, int64_t heads, float scale, int64_t nb, int64_t T,
+              int64_t A, int64_t W, const float* mask, int64_t nW, int64_t H_img, int64_t W_img, int64_t s0, int64_t s1, int dtype) {
+  NSW_CHECK_ARG(dtype == NSW_DTYPE_BF16 || dtype == NSW_DTYPE_F32, "%s: unknown dtype %d", what, dtype);
+  NSW_CHECK_ARG(Bw >= 0 && heads > 0 && C > 0 && C % heads == 0 && C % 8 == 0 && C < (1 << 18),
+                "%s: Bw=%lld, C=%lld, heads=%lld (C a multiple of 8 and of heads)", what, (long long)Bw, (long long)C, (long long)heads);
+  const int64_t hd = C / heads;
+  NSW_CHECK_ARG(hd == 4 || hd == 8 || hd == 16 || hd == 32 || hd == 64 || hd == 128, "%s: head_dim=%lld unsupported (4, 8, 16, 32, 64, 128)",
+                what, (long long)hd);
+  NSW_CHECK_ARG(T > 0 && A > 0 && W > 0 && T <= MAX_R && A <= MAX_R && W <= MAX_R && L == T * A * W,
+                "%s: L=%lld is not the %lld x %lld x %lld tokens of a window", what, (long long)L, (long long)T, (long long)A, (long long)W);
+  const int64_t R = (2 * T - 1) * (2 * A - 1) * (2 * W - 1);
+  NSW_CHECK_ARG(R <= MAX_R, "%s: %lld displacements in a window, at most %d", what, (long long)R, MAX_R);
+  NSW_CHECK_ARG(nb > 0 && nb < (1 << 24), "%s: %lld buckets", what, (long long)nb);
+  NSW_CHECK_ARG(std::isfinite(scale), "%s: scale=%g", what, (double)scale);
+  NSW_CHECK_ARG(Bw * L < (1LL << 40) && Bw * heads < (1LL << 31), "%s: too large", what);
+  a.Bw = Bw; a.L = (int)L; a.C = (int)C; a.heads = (int)heads; a.hd = (int)hd; a.R = (int)R; a.nb = (int)nb;
+  a.TW = (int)T; a.A = (int)A; a.W = (int)W; a.scale = scale;
+  a.off = (int)(((T - 1) * (2 * A - 1) + A - 1) * (2 * W - 1) + W - 1);
+  a.dAW = FastDiv::make((uint32_t)(A * W)); a.dW = FastDiv::make((uint32_t)W); a.dheads = FastDiv::make((uint32_t)heads);
+  a.mask = mask; a.nW = 1; a.band0 = 1; a.thr = 0;
+  if (mask) {
+    NSW_CHECK_ARG(nW > 0 && Bw % nW == 0 && nW < (1LL << 31), "%s: Bw=%lld not a multiple of the mask's %lld windows", what,
+                  (long long)Bw, (long long)nW);
+    a.nW = (int)nW; a.band0 = a.nW;
+  } else if (s0 != 0 || s1 != 0) {
+    if (int rc = check_geom(1, T, H_img, W_img, A, W, what)) return rc;
+    NSW_CHECK_ARG(s0 >= 0 && s0 < A && s1 >= 0 && s1 < W, "%s: shift must lie in [0, window)", what);
+    const int64_t across = W_img / W, n = (H_img / A) * across;
+    NSW_CHECK_ARG(Bw % n == 0, "%s: Bw=%lld not a multiple of the image's %lld windows", what, (long long)Bw, (long long)n);
+    a.nW = (int)n; a.band0 = (int)(n - across); a.thr = (int)(A - s0);
+  }
+  return NSW_OK;
+}
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+
+}  // namespace
+
+int launch_forward(Args a, int dtype, hipStream_t st) { return dtype == NSW_DTYPE_BF16 ? launch_t<bf16>(a, st) : launch_t<float>(a, st); }
+
+}  // namespace posattn
+
+}  // namespace nsw
+
+using namespace nsw;
+
+extern "C" int nsw_position_attention(const void* qkv, const void* table, const int32_t* buckets, const float* mask, int64_t nW_mask,
+                                      void* o, float* stats, int64_t Bw, int64_t L, int64_t C, int64_t num_heads, float scale,
+                                      int64_t num_buckets, int64_t T, int64_t ws0, int64_t ws1, int64_t H, int64_t W, int64_t s0,
+                                      int64_t s1, int dtype, void* stream) {
+  const char* what = "nsw_position_attention";
+  posattn::Args a{};
+  if (int rc = posattn::make_args(a, what, Bw, L, C, num_heads, scale, num_buckets, T, ws0, ws1, mask, nW_mask, H, W, s0, s1, dtype))
+    return rc;
+  if (Bw == 0) return NSW_OK;
+  NSW_CHECK_ARG(qkv && table && buckets && o && stats, "%s: qkv, table, buckets, o and stats are required", what);
+  NSW_CHECK_ARG(posattn::aligned16({qkv, o, stats}) && (uintptr_t)mask % 4 == 0 && (uintptr_t)buckets % 4 == 0,
+                "%s: qkv, o and stats must be 16-byte aligned", what);
+  a.qkv = qkv; a.table = table; a.buckets = buckets; a.o = o; a.stats = stats;
+  return posattn::launch_forward(a, dtype, (hipStream_t)stream);
+}
+
+extern "C" size_t nsw_position_attention_backward_workspace_size(int64_t Bw, int64_t L, int64_t C, int64_t num_heads, int64_t T,
+                                                                 int64_t ws0, int64_t ws1, int dtype) {
+  posattn::Args a{};
+  if (posattn::make_args(a, "nsw_position_attention_backward_workspace_size", Bw, L, C, num_heads, 1.f, 1, T, ws0, ws1, nullptr, 0, 0,
+                         0, 0, 0, dtype))
+    return 0;
+  return posattn::backward_workspace(a, dtype);
+}
+
+extern "C" int nsw_position_attention_backward(const void* dout, const void* qkv, const void* o, const float* stats, const void* table,
+                                               const int32_t* buckets, const float* mask, int64_t nW_mask, void* dqkv, void* dtable,
+                                               int64_t Bw, int64_t L, int64_t C, int64_t num_heads, float scale, int64_t num_buckets,
+                                               int64_t T, int64_t ws0, int64_t ws1, int64_t H, int64_t W, int64_t s0, int64_t s1,
+                                               int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "nsw_position_attention_backward";
+  posattn::Args a{};
+  if (int rc = posattn::make_args(a, what, Bw, L, C, num_heads, scale, num_buckets, T, ws0, ws1, mask, nW_mask, H, W, s0, s1, dtype))
+    return rc;
+  NSW_CHECK_ARG(Bw == 0 || (dout && qkv && o && stats && table && buckets && dqkv),
+                "%s: dout, qkv, o, stats, table, buckets and dqkv are required", what);
+  NSW_CHECK_ARG(dtable == nullptr || buckets, "%s: buckets are required", what);
+  NSW_CHECK_ARG(posattn::aligned16({dout, qkv, o, stats, dqkv, workspace}) && (uintptr_t)mask % 4 == 0 && (uintptr_t)buckets % 4 == 0,
+                "%s: dout, qkv, o, stats, dqkv and the workspace must be 16-byte aligned", what);
+  const size_t need = dtable ? posattn::backward_workspace(a, dtype) : 0;
+  NSW_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "%s: workspace of %zu bytes needed, got %zu", what,
+                need, workspace ? workspace_bytes : (size_t)0);
+  a.dout = dout; a.qkv = qkv; a.out = o; a.stats = (float*)stats; a.table = table; a.buckets = buckets; a.dqkv = dqkv;
+  return posattn::launch_backward(a, dtable, (float*)workspace, dtype, (hipStream_t)stream);
+}

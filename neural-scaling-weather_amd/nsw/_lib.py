@@ -120,6 +120,11 @@ SIGNATURES = {
     "nsw_residual_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "nsw_residual_norm_backward": (_int, [_vp] * 12 + [_i64, _i64, _i64, _f32, _f32, _int, _vp, ctypes.c_size_t,
                                                        _vp]),
+    "nsw_position_attention": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _f32] + [_i64] * 8
+                               + [_int, _vp]),
+    "nsw_position_attention_backward_workspace_size": (ctypes.c_size_t, [_i64] * 7 + [_int]),
+    "nsw_position_attention_backward": (_int, [_vp] * 7 + [_i64, _vp, _vp, _i64, _i64, _i64, _i64, _f32] + [_i64] * 8
+                                        + [_int, _vp, ctypes.c_size_t, _vp]),
     "nsw_group_norm_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _int]),
     "nsw_group_norm": (_int, [_vp] * 5 + [_i64, _i64, _i64, _i64, _f32, _int, _int, _vp, ctypes.c_size_t, _vp]),
     "nsw_group_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _int]),

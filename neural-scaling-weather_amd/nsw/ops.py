@@ -630,6 +630,98 @@ def window_attention(qkv: torch.Tensor, num_heads: int, scale: float, mask: Opti
     return o
 
 
+def window_displacements(extent: Sequence[int]) -> int:
+    """Displacements between tokens of a window of T x A x W: (2T-1)(2A-1)(2W-1)."""
+    n = 1
+    for e in extent:
+        n *= 2 * int(e) - 1
+    return n
+
+
+def _position_args(what, qkv, num_heads, table, buckets, extent, mask, geometry):
+    """(device index, Bw, L, C, mask, the sizes of the C entries after the scale) of a position attention."""
+    at = _uniform(qkv, table)
+    _dev(qkv, buckets, mask)
+    if qkv.dim() != 3 or qkv.shape[-1] % 3:
+        raise ValueError(f"{what}: qkv has shape {tuple(qkv.shape)}, expected [Bw, L, 3C]")
+    Bw, L, C = qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3
+    T, A, W = (int(e) for e in extent)
+    if min(T, A, W) < 1 or T * A * W != L:
+        raise ValueError(f"{what}: extent {(T, A, W)} does not hold {L} tokens")
+    if table.dim() != 2 or table.shape[1] != num_heads or table.shape[0] == 0:
+        raise ValueError(f"{what}: table has shape {tuple(table.shape)}, expected [buckets, {num_heads}]")
+    R = window_displacements((T, A, W))
+    if buckets.dtype != torch.int32 or buckets.shape != (R,):
+        raise ValueError(f"{what}: buckets is {buckets.dtype} {tuple(buckets.shape)}, expected int32 ({R},)")
+    if mask is not None and geometry is not None:
+        raise ValueError(f"{what}: a mask or a geometry")
+    nW = 0
+    H = Wi = s0 = s1 = 0
+    if mask is not None:
+        if mask.dtype == torch.bool:
+            mask = torch.zeros(mask.shape, dtype=torch.float32, device=mask.device).masked_fill_(~mask, float("-inf"))
+        elif mask.dtype != torch.float32:
+            mask = mask.float()
+        if mask.dim() != 3 or mask.shape[1:] != (L, L) or mask.shape[0] == 0 or Bw % mask.shape[0]:
+            raise ValueError(f"{what}: mask has shape {tuple(mask.shape)}, expected [nW, {L}, {L}] with nW a divisor of {Bw}")
+        nW = mask.shape[0]
+    elif geometry is not None:
+        H, Wi, ws, (s0, s1), Tg = geometry
+        if (Tg, *ws) != (T, A, W):
+            raise ValueError(f"{what}: geometry of windows {(Tg, *ws)}, extent {(T, A, W)}")
+    return at, Bw, L, C, mask, nW, (table.shape[0], T, A, W, H, Wi, int(s0), int(s1), dtype_code(qkv))
+
+
+def position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: torch.Tensor, buckets: torch.Tensor,
+                       extent: Sequence[int], mask: Optional[torch.Tensor] = None,
+                       geometry: Optional[Tuple[int, int, Tuple[int, int], Tuple[int, int], int]] = None
+                       ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(o, stats): window_attention with a learned position bias, o [Bw, L, C] of qkv [Bw,
+    L, 3C] with the logits scale q k^T + table[buckets[r], head] + mask.  ``extent``
+    (T, A, W) lays out the L tokens of a window (a sequence: (1, 1, L)); r numbers the
+    displacements of a query from a key, ((dt + T-1) (2A-1) + da + A-1) (2W-1) + dw + W-1;
+    buckets [(2T-1)(2A-1)(2W-1)] int32 (at most 8192), table [buckets, num_heads] in
+    qkv's dtype.  ``mask`` [nW, L, L] or ``geometry`` as window_attention; a row whose
+    mask leaves nothing gives zeros.  stats [Bw, num_heads, L, 2] fp32 (row maximum,
+    log2 of the sum of exp(z - maximum)) for position_attention_backward."""
+    what = "position_attention"
+    at, Bw, L, C, mask, nW, sizes = _position_args(what, qkv, num_heads, table, buckets, extent, mask, geometry)
+    o = qkv.new_empty((Bw, L, C))
+    stats = qkv.new_empty((Bw, num_heads, L, 2), dtype=torch.float32)
+    _run(what, at, lib().nsw_position_attention, qkv.data_ptr(), table.data_ptr(), buckets.data_ptr(), _p(mask), nW,
+         o.data_ptr(), stats.data_ptr(), Bw, L, C, num_heads, float(scale), *sizes)
+    return o, stats
+
+
+def position_attention_backward(do: torch.Tensor, qkv: torch.Tensor, o: torch.Tensor, stats: torch.Tensor, num_heads: int,
+                                scale: float, table: torch.Tensor, buckets: torch.Tensor, extent: Sequence[int],
+                                mask: Optional[torch.Tensor] = None, geometry=None,
+                                needs: Sequence[bool] = (True, True)):
+    """(dqkv, dtable) of position_attention from the gradient of o, o itself and stats,
+    None where ``needs`` says so.  The mask has no gradient."""
+    what = "position_attention_backward"
+    at, Bw, L, C, mask, nW, sizes = _position_args(what, qkv, num_heads, table, buckets, extent, mask, geometry)
+    _uniform(qkv, do, o)
+    _dev(qkv, stats)
+    if do.shape != (Bw, L, C) or o.shape != (Bw, L, C):
+        raise ValueError(f"{what}: do {tuple(do.shape)} and o {tuple(o.shape)}, expected {(Bw, L, C)}")
+    if stats.dtype != torch.float32 or stats.shape != (Bw, num_heads, L, 2):
+        raise ValueError(f"{what}: stats is {stats.dtype} {tuple(stats.shape)}, expected float32 {(Bw, num_heads, L, 2)}")
+    if not any(needs):
+        return None, None
+    dqkv = torch.empty_like(qkv)
+    dtable = torch.empty_like(table) if needs[1] else None
+    nbytes, ws = 0, None
+    if needs[1]:
+        nbytes = _workspace_bytes(lib(), "nsw_position_attention_backward_workspace_size", Bw, L, C, num_heads, *sizes[1:4],
+                                  sizes[-1])
+        ws = qkv.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _run(what, at, lib().nsw_position_attention_backward, do.data_ptr(), qkv.data_ptr(), o.data_ptr(), stats.data_ptr(),
+         table.data_ptr(), buckets.data_ptr(), _p(mask), nW, dqkv.data_ptr(), _p(dtable), Bw, L, C, num_heads, float(scale),
+         *sizes, _p(ws), nbytes)
+    return dqkv if needs[0] else None, dtable
+
+
 def proj_reverse_residual(o: torch.Tensor, wproj: torch.Tensor, bproj: torch.Tensor, skip: torch.Tensor,
                           window_size, shift_size) -> torch.Tensor:
     """skip + roll(window_reverse(o W^T + b), +shift) with skip [B,T,H,W,C]."""

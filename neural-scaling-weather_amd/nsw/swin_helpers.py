@@ -15,13 +15,14 @@ checkpoints.  Every forward runs libnsw HIP kernels:
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 
 from . import _lib, ops, torch_ops
-from .layer_helpers import BiasLayer, LinearLayer, NormLayer, parameter, submodule
+from .layer_helpers import BiasLayer, GroupNorm, LinearLayer, NormLayer, parameter, submodule, trunc_normal_
 from .mlp import MLP
 from .profiler_utils import profile
 
@@ -297,6 +298,123 @@ class Block(nn.Module):
         return torch.ops.nsw.swin_block(x, torch_ops.block_param_list(pk), self.num_heads,
                                         [int(v) for v in self.window_size], [int(v) for v in self.shift_size],
                                         self._eps(x.dtype), self.mlp.gelu_tanh)
+
+
+def position_buckets(extent: Tuple[int, int, int], num_buckets: Optional[int] = None,
+                     max_distance: int = 128) -> Tuple[torch.Tensor, int]:
+    """(buckets, their number) for ``torch.ops.nsw.position_attention``: the bucket of
+    each displacement of a window of ``extent`` = (T, A, W) tokens, int32.  Without
+    ``num_buckets`` each displacement has its own.  With it every axis of more than
+    one token has that many (even, at least 4): half for either sign, half of those for
+    the distances 0, 1, 2, ... one by one, the rest in steps that grow with the
+    logarithm of the distance up to ``max_distance``, the last for all beyond."""
+    if num_buckets is not None and (num_buckets < 4 or num_buckets % 2):
+        raise ValueError(f"position_buckets: num_buckets must be even and at least 4, got {num_buckets}")
+    axes, sizes = [], []
+    for n in (int(e) for e in extent):
+        if n < 1:
+            raise ValueError(f"position_buckets: extent {tuple(extent)}")
+        d = torch.arange(-(n - 1), n)
+        if n == 1:
+            axes.append(torch.zeros(1, dtype=torch.long))
+            sizes.append(1)
+        elif num_buckets is None:
+            axes.append(d + n - 1)
+            sizes.append(2 * n - 1)
+        else:
+            half = num_buckets // 2
+            near = max(half // 2, 1)
+            if max_distance <= near:
+                raise ValueError(f"position_buckets: max_distance must exceed {near}, got {max_distance}")
+            far = d.abs()
+            # in float64, with a guard below the borders: near * ratio^(k / steps) falls into bucket k exactly
+            steps = half - near
+            wide = torch.log(far.clamp(min=near).double() / near) / math.log(max_distance / near) * steps
+            wide = near + (wide + 1e-9).long().clamp(max=steps - 1)
+            axes.append(torch.where(far < near, far, wide) + half * (d > 0))
+            sizes.append(num_buckets)
+    t, a, w = axes
+    b = (t[:, None, None] * sizes[1] + a[None, :, None]) * sizes[2] + w[None, None, :]
+    return b.reshape(-1).to(torch.int32), sizes[0] * sizes[1] * sizes[2]
+
+
+class RelativePositionBias(nn.Module):
+    """A learned bias for the displacement between a window's tokens (no counterpart in
+    the reference): ``table`` [buckets, num_heads], read by ``buckets`` (see
+    ``position_buckets``; not part of the state dict)."""
+
+    def __init__(self, num_heads: int, extent: Tuple[int, int, int], num_buckets: Optional[int] = None,
+                 max_distance: int = 128):
+        super().__init__()
+        self.extent = tuple(int(e) for e in extent)
+        buckets, n = position_buckets(self.extent, num_buckets, max_distance)
+        if buckets.numel() > 8192:
+            raise ValueError(f"RelativePositionBias: {buckets.numel()} displacements in a window of {self.extent}, at most 8192")
+        self.register_buffer("buckets", buckets, persistent=False)
+        self.table = nn.Parameter(torch.empty(n, num_heads))
+        self.table.comm_metadata = {"sharded": [None, "tp"], "shared": ["sp1-sp2"], "reduce": ["sp1-sp2"]}
+        trunc_normal_(self.table, std=0.02)
+
+
+class PositionWindowAttention(nn.Module):
+    """Window attention with a learned position bias, with gradients (no counterpart in
+    the reference, whose windows have q/k norms and no bias): proj(softmax(scale q
+    k^T + bias + mask) v) with [q, k, v] = qkv(x) + biasqkv."""
+
+    def __init__(self, dim: int, num_heads: int, window_size: Tuple[int, int], temporal_context_window_size: int = 1,
+                 num_buckets: Optional[int] = None, max_distance: int = 128) -> None:
+        super().__init__()
+        if dim % num_heads:
+            raise ValueError(f"PositionWindowAttention: {dim} features are not a multiple of {num_heads} heads")
+        self.dim, self.num_heads = dim, num_heads
+        self.window_size = tuple(int(w) for w in window_size)
+        self.scale = (dim // num_heads) ** -0.5
+        col = {"sharded": ["tp", None], "shared": ["sp1-sp2"], "reduce": ["sp1-sp2"]}
+        self.qkv = LinearLayer(dim, 3 * dim, comm_metadata=col)
+        self.biasqkv = BiasLayer(3 * dim, comm_metadata={"sharded": ["tp"], "shared": ["sp1-sp2"], "reduce": ["sp1-sp2"]})
+        self.position = RelativePositionBias(num_heads, (temporal_context_window_size, *self.window_size), num_buckets,
+                                             max_distance)
+        self.proj = LinearLayer(dim, dim, comm_metadata={"sharded": [None, "tp"], "shared": ["sp1-sp2"], "reduce": ["sp1-sp2"]})
+        self.biasproj = BiasLayer(dim, comm_metadata={"sharded": [], "shared": ["tp-sp1-sp2"], "reduce": ["sp1-sp2"]})
+
+    def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None, geometry=None) -> torch.Tensor:
+        """x [Bw, L, C]; mask and geometry as ``WindowMultiHeadAttention``."""
+        qkv = torch_ops.linear_epi(x, self.qkv.weight, self.biasqkv.bias)
+        o = torch_ops.position_attention(qkv, self.num_heads, self.scale, self.position.table, self.position.buckets,
+                                         self.position.extent, mask=mask, geometry=None if mask is not None else geometry)
+        return torch_ops.linear_epi(o, self.proj.weight, self.biasproj.bias)
+
+
+class PositionAttentionBranch(nn.Module):
+    """The attention branch of a trained block, x + unroll(attn(partition(roll(norm(x))))),
+    with a group norm (and its activation, if any) and a learned position bias; the
+    geometry and arguments of ``Block``, with gradients (no counterpart in the
+    reference)."""
+
+    def __init__(self, dim, num_heads, feat_size, window_size, temporal_context_window_size=1, shift_size=(0, 0),
+                 num_groups=32, act_layer=None, num_buckets=None, max_distance=128):
+        super().__init__()
+        self.feat_size, self.window_size = tuple(feat_size), tuple(int(w) for w in window_size)
+        self.shift_size = tuple(int(s) for s in shift_size)
+        self.temporal_context_window_size = temporal_context_window_size
+        H, W = self.feat_size
+        if H % self.window_size[0] or W % self.window_size[1]:
+            raise ValueError(f"feat_size {self.feat_size} is not divisible by window {self.window_size}")
+        self.norm = GroupNorm(num_groups, dim, act_layer=act_layer)
+        self.attn = PositionWindowAttention(dim, num_heads, self.window_size, temporal_context_window_size, num_buckets,
+                                            max_distance)
+
+    @profile(name="shifted_wmha")
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x [B, T, H, W, C] -> [B, T, H, W, C]."""
+        if x.dim() != 5 or tuple(x.shape[2:4]) != self.feat_size or x.shape[1] != self.temporal_context_window_size:
+            raise ValueError(f"expected [B, {self.temporal_context_window_size}, {self.feat_size[0]}, {self.feat_size[1]}, C], "
+                             f"got {tuple(x.shape)}")
+        B, T, H, W, C = x.shape
+        ws, sh = list(self.window_size), list(self.shift_size)
+        xw = torch.ops.nsw.roll_window_partition(self.norm(x), ws, sh).view(-1, T * ws[0] * ws[1], C)
+        o = self.attn(xw, geometry=(H, W, self.window_size, self.shift_size, T))
+        return x + torch.ops.nsw.window_reverse_roll(o.view(-1, T, ws[0], ws[1], C), ws, [H, W], sh)
 
 
 # Names used by other Swin code bases.

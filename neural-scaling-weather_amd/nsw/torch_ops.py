@@ -462,6 +462,85 @@ def _(qkv, num_heads, scale, mask, geometry):
     return qkv.new_empty((Bw, L, C3 // 3))
 
 
+def _position_geometry(geometry: List[int]):
+    if len(geometry) == 7:
+        H, W, ws0, ws1, s0, s1, T = geometry
+        return (H, W, (ws0, ws1), (s0, s1), T)
+    if len(geometry) != 0:
+        raise ValueError("position_attention: geometry is [H, W, ws0, ws1, s0, s1, T] or empty")
+    return None
+
+
+@torch.library.custom_op("nsw::position_attention", mutates_args=())
+def _position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: torch.Tensor, buckets: torch.Tensor,
+                        extent: List[int], mask: Optional[torch.Tensor], geometry: List[int]
+                        ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(o, stats): window_attention with a learned position bias; geometry = [H, W, ws0, ws1, s0, s1, T] or []."""
+    return ops.position_attention(_dense(qkv), num_heads, scale, table.contiguous(), buckets.contiguous(), tuple(extent),
+                                  mask=None if mask is None else mask.contiguous(), geometry=_position_geometry(geometry))
+
+
+@_position_attention.register_fake
+def _(qkv, num_heads, scale, table, buckets, extent, mask, geometry):
+    Bw, L, C3 = qkv.shape
+    return qkv.new_empty((Bw, L, C3 // 3)), qkv.new_empty((Bw, num_heads, L, 2), dtype=torch.float32)
+
+
+@torch.library.custom_op("nsw::position_attention_backward", mutates_args=())
+def _position_attention_backward(do: torch.Tensor, qkv: torch.Tensor, o: torch.Tensor, stats: torch.Tensor, num_heads: int,
+                                 scale: float, table: torch.Tensor, buckets: torch.Tensor, extent: List[int],
+                                 mask: Optional[torch.Tensor], geometry: List[int], needs: List[bool]
+                                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dqkv, dtable); empty ([0]) where ``needs`` is False."""
+    return _or_empty(qkv, *ops.position_attention_backward(
+        _dense(do), _dense(qkv), _dense(o), stats.contiguous(), num_heads, scale, table.contiguous(), buckets.contiguous(),
+        tuple(extent), mask=None if mask is None else mask.contiguous(), geometry=_position_geometry(geometry),
+        needs=tuple(needs)))
+
+
+@_position_attention_backward.register_fake
+def _(do, qkv, o, stats, num_heads, scale, table, buckets, extent, mask, geometry, needs):
+    return qkv.new_empty(qkv.shape if needs[0] else (0,)), qkv.new_empty(table.shape if needs[1] else (0,))
+
+
+def _position_setup(ctx, inputs, output):
+    qkv, num_heads, scale, table, buckets, extent, mask, geometry = inputs
+    ctx.rest = (num_heads, scale, list(extent), list(geometry))
+    ctx.masked = mask is not None
+    ctx.save_for_backward(qkv, table, buckets, *output, *([mask] if mask is not None else []))
+    ctx.set_materialize_grads(False)
+
+
+def _position_backward(ctx, do, dstats):
+    if dstats is not None:
+        raise NotImplementedError("nsw.position_attention: the row statistics have no gradient of their own")
+    if ctx.needs_input_grad[6]:
+        raise NotImplementedError("nsw.position_attention: the mask has no gradient (a learned bias is a table's)")
+    if do is None:
+        return (None,) * 8
+    qkv, table, buckets, o, stats, *rest = ctx.saved_tensors
+    num_heads, scale, extent, geometry = ctx.rest
+    need = [ctx.needs_input_grad[0], ctx.needs_input_grad[3]]
+    got = torch.ops.nsw.position_attention_backward(do, qkv, o, stats, num_heads, scale, table, buckets, extent,
+                                                    rest[0] if ctx.masked else None, geometry, need)
+    dqkv, dtable = (g if n else None for n, g in zip(need, got))
+    return dqkv, None, None, dtable, None, None, None, None
+
+
+_position_attention.register_autograd(_position_backward, setup_context=_position_setup)
+
+
+def position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: torch.Tensor, buckets: torch.Tensor,
+                       extent: Sequence[int], mask: Optional[torch.Tensor] = None, geometry=None) -> torch.Tensor:
+    """torch.ops.nsw.position_attention with ops.position_attention's arguments: o alone."""
+    geo = []
+    if geometry is not None:
+        H, W, ws, sh, T = geometry
+        geo = [int(H), int(W), int(ws[0]), int(ws[1]), int(sh[0]), int(sh[1]), int(T)]
+    return torch.ops.nsw.position_attention(qkv, int(num_heads), float(scale), table, buckets, [int(e) for e in extent], mask,
+                                            geo)[0]
+
+
 # ------------------------------------------------------------ window maps ---
 
 @torch.library.custom_op("nsw::window_partition", mutates_args=())
@@ -486,6 +565,28 @@ def _(windows, window_size, img_size):
     H, W = img_size
     B = windows.shape[0] // ((H // window_size[0]) * (W // window_size[1]))
     return windows.new_empty((B, T, H, W, C))
+
+
+def _partition_setup(ctx, inputs, output):
+    x, window_size, *rest = inputs
+    ctx.image = [int(x.shape[2]), int(x.shape[3])]
+    ctx.window, ctx.shift = list(window_size), list(rest[0]) if rest else [0, 0]
+
+
+def _partition_backward(ctx, dw):
+    # a permutation of rows: the other map
+    dx = torch.ops.nsw.window_reverse_roll(dw, ctx.window, ctx.image, ctx.shift)
+    return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
+
+
+def _reverse_setup(ctx, inputs, output):
+    _, window_size, _, *rest = inputs
+    ctx.window, ctx.shift = list(window_size), list(rest[0]) if rest else [0, 0]
+
+
+def _reverse_backward(ctx, dx):
+    dw = torch.ops.nsw.roll_window_partition(dx, ctx.window, ctx.shift)
+    return (dw,) + (None,) * (len(ctx.needs_input_grad) - 1)
 
 
 @torch.library.custom_op("nsw::roll_hw", mutates_args=())
@@ -521,6 +622,12 @@ def _(windows, window_size, img_size, shift_size):
     H, W = img_size
     B = windows.shape[0] // ((H // window_size[0]) * (W // window_size[1]))
     return windows.new_empty((B, T, H, W, C))
+
+
+for _op in (window_partition, roll_window_partition):
+    _op.register_autograd(_partition_backward, setup_context=_partition_setup)
+for _op in (window_reverse, window_reverse_roll):
+    _op.register_autograd(_reverse_backward, setup_context=_reverse_setup)
 
 
 # ----------------------------------------------------------- model layout ---

@@ -14,39 +14,53 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct Args {
   const void *qkv, *table, *dout, *out;
   void *o, *dqkv;
-  float* stats;                     // [Bw, heads, L, 2]: row maximum m, log2 of the row's sum of exp(z - m)
+  float* stats;                     // [Bw, heads, L, 2]: row maximum m of z log2 e, log2 of the row's sum of exp2(z log2 e - m)
   const int* buckets;               // [R]
   const float* mask;                // [nW, L, L] or NULL
-  float* part;                      // [heads, NP nkc, R] partial sums of the bias's gradient, or NULL
+  float* part;                      // [heads, NP, L, L]: dz summed over the windows of a workgroup, or NULL
   int64_t Bw;
   int nW;                           // windows of the mask, or of an image
   int L, C, heads, hd, R, off, nb;
   int TW, A, W;                     // extent of a window (frames are the outermost)
   int nqc;                          // workgroups that share a window's queries (keys in the backward pass)
   int NP;                           // backward: workgroups that share a head's windows
-  int copies, RS;                   // backward: accumulators of the bias's gradient in LDS, floats of each
   int band0, thr;                   // shift mask: first window of the last band (none: nW), its first row of the other class
   float scale;
   FastDiv dAW, dW, dheads, dnqc;
 };
 
-// Code of token p = (t, a, w): displacements are differences of codes.  Increasing in p.
-__device__ __forceinline__ int code_of(const Args& a, int p) {
-  const int t = (int)a.dAW.div((uint32_t)p), r = p - t * a.A * a.W, i = (int)a.dW.div((uint32_t)r);
-  return (t * (2 * a.A - 1) + i) * (2 * a.W - 1) + (r - i * a.W);
-}
-
-// The code with the token's class under the shift mask in bit 30.
+// Code of token p = (t, a, w) (past the window: of its last) in bytes of a float table:
+// displacements are differences of codes.  Bit 30: the token's class under the shift mask.
 __device__ __forceinline__ int info_of(const Args& a, int p, bool shifted) {
   if (p >= a.L) p = a.L - 1;
   const int t = (int)a.dAW.div((uint32_t)p), r = p - t * a.A * a.W, i = (int)a.dW.div((uint32_t)r);
   const int code = (t * (2 * a.A - 1) + i) * (2 * a.W - 1) + (r - i * a.W);
-  return code | (shifted && i >= a.thr ? 1 << 30 : 0);
+  return 4 * code | (shifted && i >= a.thr ? 1 << 30 : 0);
 }
 
-// Index of the displacement of tokens with the infos q and k.  R <= 8192 = 2^13, so
-// that the class bits fall out.
-__device__ __forceinline__ int displacement(const Args& a, int q, int k) { return (q - k + a.off) & (MAX_R - 1); }
+// Four logits in units of log2 e from products s: z_r = s_r zs + rel[q_r - k_r] + mask, q and k the
+// infos with the middle displacement's offset added to q's, rel and the masks times log2 e.
+// SHIFT: -100 between the classes.  R <= 8192 = 2^13, so that their bits fall out of the offset.
+template <bool SHIFT>
+__device__ __forceinline__ void logits(f32x4& s, float zs, const float* rel, const int (&q)[4], const int (&k)[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int d = q[r] - k[r];
+    if constexpr (SHIFT) {
+      s[r] = fmaf(s[r], zs, *reinterpret_cast<const float*>((const char*)rel + (d & (4 * MAX_R - 4))));
+      s[r] += (q[r] ^ k[r]) >> 30 ? -100.f * LOG2E : 0.f;
+    } else {
+      s[r] = fmaf(s[r], zs, *reinterpret_cast<const float*>((const char*)rel + d));
+    }
+  }
+}
+
+// A mask value times log2 e: the lowest floats stay finite, so that a row of them is uniform, as
+// in fp32 on the formula.
+__device__ __forceinline__ float mask_units(float m) {
+  const float v = m * LOG2E;
+  return v == -INFINITY && m != -INFINITY ? -3.402823466e38f : v;
+}
 
 // ------------------------------------------------------------- fragments ---
 // Operands of D += A B with 16 x 16 results: lane (fr = lane % 16, fg = lane / 16) holds
@@ -89,16 +103,19 @@ template <typename T, int HD_> struct Dim {
 };
 
 // 16 bytes of a row of hd values (head dim 4 in bf16: 8 bytes and zeros), zeros past its end.
+// The row begins `off` bytes behind base; 32-bit offsets on one base of the wave leave the
+// lanes one register for an address (a window's rows end below 4 GiB: checked by the host).
 template <typename T, int HD>
-__device__ __forceinline__ u32x4 load_chunk(const T* row, int ch, int hd) {
+__device__ __forceinline__ u32x4 load_chunk(const char* base, uint32_t off, int ch, int hd) {
   constexpr int EPC = 16 / (int)sizeof(T);
+  const char* p = base + (off + 16u * (uint32_t)ch);
   if constexpr (HD > 16) {
-    return *reinterpret_cast<const u32x4*>(row + ch * EPC);
+    return *reinterpret_cast<const u32x4*>(p);
   } else {
-    if ((ch + 1) * EPC <= hd) return *reinterpret_cast<const u32x4*>(row + ch * EPC);
+    if ((ch + 1) * EPC <= hd) return *reinterpret_cast<const u32x4*>(p);
     u32x4 v = {0u, 0u, 0u, 0u};
     if (ch * EPC < hd) {
-      const uint64_t h = *reinterpret_cast<const uint64_t*>(row + ch * EPC);
+      const uint64_t h = *reinterpret_cast<const uint64_t*>(p);
       v[0] = (uint32_t)h;
       v[1] = (uint32_t)(h >> 32);
     }
@@ -106,19 +123,33 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int ch, int hd) {
   }
 }
 
-// Fragment over the head dim, k-step s: bf16 values 32 s + 8 fg .., fp32 (head dim 16) 4 fg ..;
-// of a row in memory or in LDS.
+// Fragment over the head dim, k-step s, of a row in memory: bf16 values 32 s + 8 fg .., fp32 the
+// same or (head dim 16) 4 fg ..
 template <typename T, int HD>
-__device__ __forceinline__ typename Dim<T, HD>::Frag row_frag(const T* row, int s, int fg, int hd) {
+__device__ __forceinline__ typename Dim<T, HD>::Frag row_frag(const char* base, uint32_t off, int s, int fg, int hd) {
+  typedef typename Dim<T, HD>::Frag F;
+  if constexpr (sizeof(T) == 4 && HD >= 32) {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(base + (off + 128u * (uint32_t)s + 32u * (uint32_t)fg));
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(base + (off + 128u * (uint32_t)s + 32u * (uint32_t)fg + 16u));
+    return F{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  } else {
+    return __builtin_bit_cast(F, load_chunk<T, HD>(base, off, 4 * s + fg, hd));
+  }
+}
+
+// The same of a row of a tile in LDS.
+template <typename T, int HD>
+__device__ __forceinline__ typename Dim<T, HD>::Frag row_frag(const T* row, int s, int fg) {
   typedef typename Dim<T, HD>::Frag F;
   if constexpr (sizeof(T) == 2) {
     if constexpr (HD >= 32) return *reinterpret_cast<const F*>(row + 32 * s + 8 * fg);
-    else return __builtin_bit_cast(F, load_chunk<T, HD>(row, fg, hd));
+    const F z = {};
+    return fg < 2 ? *reinterpret_cast<const F*>(row + 8 * fg) : z;
   } else if constexpr (HD >= 32) {
     const f32x4 lo = *reinterpret_cast<const f32x4*>(row + 32 * s + 8 * fg), hi = *reinterpret_cast<const f32x4*>(row + 32 * s + 8 * fg + 4);
     return F{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   } else {
-    return __builtin_bit_cast(F, load_chunk<T, HD>(row, fg, hd));
+    return *reinterpret_cast<const F*>(row + 4 * fg);
   }
 }
 
@@ -162,28 +193,28 @@ __device__ __forceinline__ typename FragOf<T, 8>::type pair_frag(const f32x4& lo
   return f;
 }
 
-// rel[r] = the head's bias of displacement r; buckets that the table does not have: 0.
+// rel[r] = the head's bias of displacement r times log2 e; buckets that the table does not have: 0.
 template <typename T>
 __device__ __forceinline__ void load_rel(const Args& a, int head, float* rel) {
-  for (int r = (int)threadIdx.x; r < a.R; r += NT) {
+  for (int r = (int)threadIdx.x; r < a.R; r += (int)blockDim.x) {
     const int b = a.buckets[r];
-    rel[r] = (unsigned)b < (unsigned)a.nb ? to_f32(((const T*)a.table)[(int64_t)b * a.heads + head]) : 0.f;
+    rel[r] = (unsigned)b < (unsigned)a.nb ? to_f32(((const T*)a.table)[(int64_t)b * a.heads + head]) * LOG2E : 0.f;
   }
 }
 
-// A tile of ROWS rows of HD values from memory (row r at base + r ld, rows from `rows` on
-// zeros) by way of registers: load() and later store() into LDS.
-template <typename T, int HD, int ROWS>
+// A tile of ROWS rows of HD values from memory (row r at base + r ldb bytes, rows from `rows`
+// on zeros) by way of registers: load() and later store() into LDS.
+template <typename T, int HD, int ROWS, int NT = posattn::NT>
 struct TileCopy {
   typedef Dim<T, HD> D;
   static constexpr int N = (ROWS * D::CPR + NT - 1) / NT;
   u32x4 v[N];
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int rows, int hd) {
+  __device__ __forceinline__ void load(const char* base, uint32_t ldb, int rows, int hd) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       const int i = (int)threadIdx.x + NT * c, r = i / D::CPR, ch = i % D::CPR;
       v[c] = u32x4{0u, 0u, 0u, 0u};
-      if (r < rows && (ROWS * D::CPR % NT == 0 || r < ROWS)) v[c] = load_chunk<T, HD>(base + r * ld, ch, hd);
+      if (r < rows && (ROWS * D::CPR % NT == 0 || r < ROWS)) v[c] = load_chunk<T, HD>(base, (uint32_t)r * ldb, ch, hd);
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
@@ -196,11 +227,11 @@ struct TileCopy {
 };
 
 // Dot products of the rows of two tiles held by TileCopy, to dst[row] in LDS.
-template <typename T, int HD, int ROWS>
-__device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS>& x, const TileCopy<T, HD, ROWS>& y, float* dst) {
+template <typename T, int HD, int ROWS, int NT>
+__device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS, NT>& x, const TileCopy<T, HD, ROWS, NT>& y, float* dst) {
   typedef Dim<T, HD> D;
 #pragma unroll
-  for (int c = 0; c < TileCopy<T, HD, ROWS>::N; ++c) {
+  for (int c = 0; c < TileCopy<T, HD, ROWS, NT>::N; ++c) {
     const int i = (int)threadIdx.x + NT * c, r = i / D::CPR, ch = i % D::CPR;
     float s = 0.f;
     if constexpr (sizeof(T) == 2) {
@@ -218,12 +249,12 @@ __device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS>& x, const T
   }
 }
 
-// 4 values of a result to a row of hd values.
+// 4 values of a result to column d of a row of hd values, off bytes behind base.
 template <typename T, int HD>
-__device__ __forceinline__ void store_quad(T* row, int d, int hd, const f32x4& v, float f) {
+__device__ __forceinline__ void store_quad(char* base, uint32_t off, int d, int hd, const f32x4& v, float f) {
   if (HD > 16 || d < hd) {
     const float x[4] = {v[0] * f, v[1] * f, v[2] * f, v[3] * f};
-    store4(row + d, x);
+    store4((T*)(base + (off + (uint32_t)(d * (int)sizeof(T)))), x);
   }
 }
 

@@ -9,11 +9,11 @@
 // A workgroup takes QB 64-query blocks of one (window, head): it steps over 64-key tiles in
 // LDS with the running maximum m and sum of each row, so any length goes.  S^T = K Q^T puts a
 // query on a lane, whose probabilities are then the right operand of O^T = V^T P^T as they
-// lie.  Logits in natural units, exp2((z - m) log2 e): a mask of the lowest float stays
-// finite, and all-lowest rows come out uniform, as in fp32 on the formula.  fp32 statistics
-// and sums; bf16: probabilities (at most 1) are rounded to bf16 for the product with v, their
-// sum is of the unrounded ones.  stats keeps m and log2 of the sum apart, since their sum
-// would lose the second where |m| is large.
+// lie.  Logits in units of log2 e (the factor is in the scale and in the bias's LDS copy), so
+// that a probability is one subtraction and exp2.  fp32 statistics and sums; bf16: probabilities
+// (at most 1) are rounded to bf16 for the product with v, and their sum is of the rounded
+// ones, by a product with ones on the matrix units.  stats keeps m and log2 of the sum apart,
+// since their sum would lose the second where |m| is large.
 #include <cmath>
 
 #include "nsw_position_attention.h"
@@ -43,33 +43,39 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
   const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
   const int L = a.L, C = a.C;
-  const int64_t ld = 3 * (int64_t)C;
-  const T* base = (const T*)a.qkv + win * L * ld + head * a.hd;
+  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
+  const char* base = (const char*)a.qkv + win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T);
   const int wi = (int)(win % a.nW);
   const bool shifted = !MASK && wi >= a.band0;
   const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
   const int q0 = qc * 64 * QB + wave * 16;                 // block i of the wave: q0 + 64 i
 
   TileCopy<T, HD, KT> kc, vc;
-  kc.load(base + C, ld, L, a.hd);
-  vc.load(base + 2 * C, ld, L, a.hd);
+  kc.load(base + ob, ldb, L, a.hd);
+  vc.load(base + 2 * (int64_t)ob, ldb, L, a.hd);
   typename D::Frag qf[QB][D::NS];
   int qinfo[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr, qr = q < L ? q : L - 1;
-    qinfo[i] = info_of(a, qr, shifted) + a.off;
+    qinfo[i] = info_of(a, qr, shifted) + 4 * a.off;
 #pragma unroll
-    for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(base + qr * ld, s, fg, a.hd);
+    for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(base, (uint32_t)qr * ldb, s, fg, a.hd);
   }
   load_rel<T>(a, head, rel);
 
-  f32x4 O[QB][D::ND];
+  const float zs = a.scale * LOG2E;
+  constexpr bool ONES = sizeof(T) == 2;
+  typename D::TFrag ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
+  f32x4 O[QB][D::ND], Z[QB];                               // Z: the rows' sums (ONES)
   float m[QB], l[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
+    Z[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < D::ND; ++d) O[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -82,8 +88,8 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
     wg_barrier();
     const int left = L - k0;                               // keys from k0 on
     if (left > KT) {
-      kc.load(base + (int64_t)(k0 + KT) * ld + C, ld, left - KT, a.hd);
-      vc.load(base + (int64_t)(k0 + KT) * ld + 2 * C, ld, left - KT, a.hd);
+      kc.load(base + (int64_t)(k0 + KT) * ldb + ob, ldb, left - KT, a.hd);
+      vc.load(base + (int64_t)(k0 + KT) * ldb + 2 * (int64_t)ob, ldb, left - KT, a.hd);
     }
     f32x4 S[QB][4];
 #pragma unroll
@@ -91,28 +97,39 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
       if (16 * kb < left) {
         typename D::Frag kf[D::NS];
 #pragma unroll
-        for (int s = 0; s < D::NS; ++s) kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg, HD);
+        for (int s = 0; s < D::NS; ++s) kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg);
         const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
         const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
-          f32x4 t = {0.f, 0.f, 0.f, 0.f};
+          S[i][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int s = 0; s < D::NS; ++s) t = mma(kf[s], qf[i][s], t);
-          const int q = q0 + 64 * i + fr;
+          for (int s = 0; s < D::NS; ++s) S[i][kb] = mma(kf[s], qf[i][s], S[i][kb]);
+        }
+        if (shifted) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int diff = qinfo[i] - kn[r];
-            float z = fmaf(t[r], a.scale, rel[diff & (MAX_R - 1)]);
-            const int key = k0 + 16 * kb + 4 * fg + r;
-            if constexpr (MASK) {
-              if (q < L && key < L) z += mask[(int64_t)q * L + key];
-            } else if (shifted) {
-              z += ((qinfo[i] - a.off) ^ kn[r]) >> 30 ? -100.f : 0.f;
+          for (int i = 0; i < QB; ++i) logits<true>(S[i][kb], zs, rel, {qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn);
+        } else {
+#pragma unroll
+          for (int i = 0; i < QB; ++i) logits<false>(S[i][kb], zs, rel, {qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn);
+        }
+        if constexpr (MASK) {
+#pragma unroll
+          for (int i = 0; i < QB; ++i) {
+            const int q = q0 + 64 * i + fr;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int key = k0 + 16 * kb + 4 * fg + r;
+              if (q < L && key < L) S[i][kb][r] += mask_units(mask[(int64_t)q * L + key]);
             }
-            t[r] = key < L ? z : -INFINITY;
           }
-          S[i][kb] = t;
+        }
+        if (16 * kb + 16 > left) {
+#pragma unroll
+          for (int i = 0; i < QB; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * kb + 4 * fg + r >= left) S[i][kb][r] = -INFINITY;
         }
       } else {
 #pragma unroll
@@ -128,18 +145,19 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[i][kb][r]);
       mx = fmaxf(m[i], rows4_max(mx));
       const float at = mx == -INFINITY ? 0.f : mx;
-      const float f = __builtin_amdgcn_exp2f((m[i] - at) * LOG2E);
+      const float f = __builtin_amdgcn_exp2f(m[i] - at);
       m[i] = mx;
       float t = 0.f;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f((S[i][kb][r] - at) * LOG2E);
+          const float p = __builtin_amdgcn_exp2f(S[i][kb][r] - at);
           S[i][kb][r] = p;
-          t += p;
+          if constexpr (!ONES) t += p;
         }
       l[i] = fmaf(l[i], f, t);
+      Z[i] *= f;
 #pragma unroll
       for (int d = 0; d < D::ND; ++d) O[i][d] *= f;
     }
@@ -154,18 +172,19 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
           const typename D::TFrag pf = pair_frag<T>(S[i][2 * ks], S[i][2 * ks + 1]);
 #pragma unroll
           for (int d = 0; d < D::ND; ++d) O[i][d] = mma(vf[d], pf, O[i][d]);
+          if constexpr (ONES) Z[i] = mma(ones, pf, Z[i]);
         }
       }
   }
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr;
-    const float t = rows4_sum(l[i]);
+    const float t = ONES ? Z[i][0] : rows4_sum(l[i]);
     const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;    // an empty row: zeros; NaN stays
     if (q < L) {
-      T* row = (T*)a.o + (win * L + q) * (int64_t)C + head * a.hd;
+      char* orow = (char*)a.o + win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
 #pragma unroll
-      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(row, 16 * d + 4 * fg, a.hd, O[i][d], inv);
+      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orow, (uint32_t)q * ob, 16 * d + 4 * fg, a.hd, O[i][d], inv);
       if (fg == 0) *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + q) * 2) = f32x2{m[i], __builtin_amdgcn_logf(t)};
     }
   }
@@ -220,7 +239,8 @@ int make_args(Args& a, const char* what, int64_t Bw, int64_t L, int64_t C, int64
   NSW_CHECK_ARG(R <= MAX_R, "%s: %lld displacements in a window, at most %d", what, (long long)R, MAX_R);
   NSW_CHECK_ARG(nb > 0 && nb < (1 << 24), "%s: %lld buckets", what, (long long)nb);
   NSW_CHECK_ARG(std::isfinite(scale), "%s: scale=%g", what, (double)scale);
-  NSW_CHECK_ARG(Bw * L < (1LL << 40) && Bw * heads < (1LL << 31), "%s: too large", what);
+  NSW_CHECK_ARG(Bw * L < (1LL << 40) && Bw * heads < (1LL << 31) && L * 3 * C * (int64_t)dtype_size(dtype) < (1LL << 32),
+                "%s: too large", what);
   a.Bw = Bw; a.L = (int)L; a.C = (int)C; a.heads = (int)heads; a.hd = (int)hd; a.R = (int)R; a.nb = (int)nb;
   a.TW = (int)T; a.A = (int)A; a.W = (int)W; a.scale = scale;
   a.off = (int)(((T - 1) * (2 * A - 1) + A - 1) * (2 * W - 1) + W - 1);

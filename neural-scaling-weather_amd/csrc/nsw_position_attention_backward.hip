@@ -5,20 +5,23 @@
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i dz_ij q_i,  dq_i = scale sum_j dz_ij k_j
 //   dtable[b, head] = sum of dz_ij over the windows and the pairs whose bucket is b
 //
-// keys_kernel: a wave owns KB 16-key blocks of a window (their k and v as fragments in
-// registers, dk and dv in accumulators), the workgroup's four waves step together over 32-query
-// tiles in LDS.  S = Q K^T puts a key on a lane, so that p and dz are the right operands of
-// dv^T = do^T p and dk^T = q^T dz as they lie.  Windows that one workgroup holds (ALL) also
-// form dq there: dz goes through LDS, keys by queries, and a wave takes 16 columns of dq over
-// all keys, k^T in registers: five products a pair, every operand read once.  Longer windows:
-// queries_kernel forms dq with p once more (two products more, no sums across workgroups).
+// Both kernels put a key on a lane (S = Q K^T), so that p and dz are the right operands of
+// dv^T = do^T p and dk^T = q^T dz as they lie.  They take the windows of one head in turn and
+// add dz up over them, pair by pair, so that displacements are looked at once a workgroup and not
+// once a window (float additions in LDS, one for each pair of each window, took 1100 us of
+// 1795 at 400 windows of 9 x 18 and 16 heads of 64).
 //
-// The bias's gradient is added up in LDS over all windows that a workgroup takes, of one head.
-// Each group of 16 lanes has accumulators of its own: within it the keys, so the displacements,
-// differ, and a wave's additions keep their order: no two lanes meet, the same bits in
-// every run.  With many displacements the groups of a wave take turns in one accumulator, with
-// more the waves do.  bias_sum_kernel and bias_table_kernel add the workgroups' sums and
-// those of a bucket, in order.
+// windows_kernel, for windows of up to 16 WAVES tokens: a wave owns 16 keys (k and v in
+// fragments, dk and dv in accumulators), the workgroup steps over 32-query tiles in LDS; dz
+// goes through LDS, keys by queries, to the waves that form dq from it and k: five products
+// a pair, every operand read once.  The sums of dz stay in registers.
+//
+// keys_kernel and queries_kernel, for longer ones: a wave owns KB 16-key blocks, dq comes from a
+// kernel of its own that forms p once more (two products more, no sums across workgroups), the
+// sums of dz are read and written in memory, each by one lane.
+//
+// pairs_kernel adds up the pairs of a displacement, table_kernel the displacements of a
+// bucket: no atomics, the same bits in every run.
 //
 // bf16: p and dz are rounded to bf16 for the products (dtable: not rounded).
 #include <algorithm>
@@ -33,49 +36,243 @@ namespace {
 
 constexpr int QT = 32;              // queries of a tile
 
-// Bytes of LDS of keys_kernel without the accumulators.
-template <typename T, int HD, int KB, bool ALL>
-constexpr size_t tile_bytes() {
-  typedef Dim<T, HD> D;
-  const size_t work = (2 * QT * D::STR + (ALL ? 64 * KB * (QT + 16 / sizeof(T)) : 0)) * sizeof(T);
-  const size_t keys = ALL ? 64 * KB * D::STR * sizeof(T) : 0;      // k of the window, before the steps
-  return (work > keys ? work : keys) + 4 * QT * sizeof(float);
+// Row statistics of a tile's queries as the kernels use them: p = exp2(z - m - l), both in
+// m where no mask can make m large; rows without keys, or past the window, p = 0.
+template <bool MASK>
+__device__ __forceinline__ void put_stats(const f32x2& st, float* mrow, float* lrow) {
+  const bool none = st[0] == -INFINITY;
+  if constexpr (MASK) {
+    *mrow = none ? INFINITY : st[0];
+    *lrow = none ? 0.f : st[1];
+  } else {
+    *mrow = none ? INFINITY : st[0] + st[1];
+  }
 }
 
-template <typename T, int HD, int KB, bool ALL, bool MASK>
-__global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
+// p and dz of four pairs from their products: s = q k, g = do v.
+template <bool MASK>
+__device__ __forceinline__ void weigh(f32x4& s, f32x4& g, const f32x4& m, const f32x4& l, const f32x4& d) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(MASK ? s[r] - m[r] - l[r] : s[r] - m[r]);
+    g[r] = s[r] * (g[r] - d[r]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void put4(T* p, const typename FragOf<T, 8>::type& f, int h) {
+  typedef __attribute__((ext_vector_type(4))) T T4;
+  *reinterpret_cast<T4*>(p) = T4{f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]};
+}
+
+// ------------------------------------------------- windows in a workgroup ---
+
+template <typename T, int HD, int WAVES> struct Windows {
   typedef Dim<T, HD> D;
-  constexpr int ND = D::ND, ZS = QT + 16 / (int)sizeof(T);         // floats or bf16 of a key's dz in LDS
-  constexpr int NKS = 2 * KB;                                      // 32-key steps of the workgroup's keys
-  constexpr int DQ = ALL ? (2 * ND + 3) / 4 : 0;                   // 16 x 16 blocks of dq of a wave
-  constexpr int KD = ALL ? (ND + 3) / 4 : 0;                       // 16-column blocks of k^T of a wave
+  static constexpr int KEYS = 16 * WAVES, STEPS = WAVES / 2;
+  static constexpr int ZS = QT + 16 / (int)sizeof(T);              // values of a key's dz in LDS
+  static constexpr size_t TILES = (size_t)(2 * QT * D::STR + 2 * KEYS * D::STR + KEYS * ZS) * sizeof(T);
+  static constexpr size_t LDS = TILES + 4 * QT * sizeof(float);
+};
+
+template <typename T, int HD, int WAVES, bool MASK>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) {
+  typedef Dim<T, HD> D;
+  typedef Windows<T, HD, WAVES> X;
+  constexpr int N = 64 * WAVES, ND = D::ND;
+  constexpr int TASKS = (2 * ND + WAVES - 1) / WAVES;              // 16 x 16 blocks of a tile's dq of a wave
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* Qs = (T*)smem;
   T* Gs = Qs + QT * D::STR;
-  T* Zs = Gs + QT * D::STR;
-  float* rows = (float*)(smem + tile_bytes<T, HD, KB, ALL>()) - 4 * QT;
-  int* qinfo = (int*)rows;
-  float *mrow = rows + QT, *lrow = rows + 2 * QT, *drow = rows + 3 * QT;
-  float* rel = rows + 4 * QT;
-  float* acc = rel + ((a.R + 3) & ~3);
+  T* Ks = Gs + QT * D::STR;
+  T* Vs = Ks + X::KEYS * D::STR;
+  T* Zs = Vs + X::KEYS * D::STR;
+  int* qinfo = (int*)(smem + X::TILES);
+  float *mrow = (float*)qinfo + QT, *lrow = mrow + QT, *drow = lrow + QT;
+  float* rel = drow + QT;
+
+  const int part = (int)blockIdx.x % a.NP, head = (int)blockIdx.x / a.NP;   // a head's parts side by side
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
+  const int L = a.L, C = a.C;
+  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
+  const int k0 = 16 * wave, key = k0 + fr;
+  const bool keys = k0 < L, bias = a.part != nullptr, alone = L == 1;       // alone: p is 1 whatever z, dz exactly 0
+  const float zs = a.scale * LOG2E;
+  load_rel<T>(a, head, rel);
+  f32x4 sums[2 * X::STEPS];
+#pragma unroll
+  for (int i = 0; i < 2 * X::STEPS; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!keys) {                                                     // dz of no keys: zeros, whatever the step
+    typename D::TFrag z = {};
+#pragma unroll
+    for (int i = 0; i < QT / 16; ++i) put4<T>(Zs + key * X::ZS + 16 * i + 4 * fg, z, 0);
+  }
+
+  for (int64_t win = part; win < a.Bw; win += a.NP) {
+    const int64_t at3 = win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T), at1 = win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
+    const char *base = (const char*)a.qkv + at3, *gbase = (const char*)a.dout + at1, *obase = (const char*)a.out + at1;
+    char* dbase = (char*)a.dqkv + at3;
+    const f32x2* stats = (const f32x2*)a.stats + (win * a.heads + head) * L;
+    const int wi = (int)(win % a.nW);
+    const bool shifted = !MASK && wi >= a.band0;
+    const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
+
+    {
+      TileCopy<T, HD, X::KEYS, N> kc, vc;
+      kc.load(base + ob, ldb, L, a.hd);
+      vc.load(base + 2 * (int64_t)ob, ldb, L, a.hd);
+      wg_barrier();                                                // the window before is done
+      kc.store(Ks);
+      vc.store(Vs);
+    }
+    TileCopy<T, HD, QT, N> qc, gc, oc;
+    f32x2 st;
+    auto load_tile = [&](int q0) {
+      qc.load(base + (int64_t)q0 * ldb, ldb, L - q0, a.hd);
+      gc.load(gbase + (int64_t)q0 * ob, ob, L - q0, a.hd);
+      oc.load(obase + (int64_t)q0 * ob, ob, L - q0, a.hd);
+      if (tid < QT) st = q0 + tid < L ? stats[q0 + tid] : f32x2{-INFINITY, 0.f};
+    };
+    load_tile(0);
+    const int kr = key < L ? key : L - 1;                          // keys past the window: p = 0 below
+    const int kinfo = info_of(a, kr, shifted);
+    const int k4[4] = {kinfo, kinfo, kinfo, kinfo};
+    f32x4 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll 1
+    for (int q0 = 0; q0 < L; q0 += QT) {
+      wg_barrier();                                                // the tile before and its dz are read
+      qc.store(Qs);
+      gc.store(Gs);
+      row_dots(gc, oc, drow);
+      if (tid < QT) {
+        qinfo[tid] = info_of(a, q0 + tid, shifted) + 4 * a.off;
+        put_stats<MASK>(st, mrow + tid, lrow + tid);
+      }
+      wg_barrier();
+      if (q0 + QT < L) load_tile(q0 + QT);
+
+      if (keys) {
+        f32x4 P[2], Z[2];                                          // queries 16 qb + 4 fg + r, key fr
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          P[qb] = Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (q0 + 16 * qb >= L) continue;
+#pragma unroll
+          for (int s = 0; s < D::NS; ++s) {
+            P[qb] = mma(row_frag<T, HD>(Qs + (16 * qb + fr) * D::STR, s, fg), row_frag<T, HD>(Ks + key * D::STR, s, fg), P[qb]);
+            Z[qb] = mma(row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg), row_frag<T, HD>(Vs + key * D::STR, s, fg), Z[qb]);
+          }
+          const int4 qi = *reinterpret_cast<const int4*>(qinfo + 16 * qb + 4 * fg);
+          const int qn[4] = {qi.x, qi.y, qi.z, qi.w};
+          const f32x4 m4 = *reinterpret_cast<const f32x4*>(mrow + 16 * qb + 4 * fg);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(drow + 16 * qb + 4 * fg);
+          const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(lrow + 16 * qb + 4 * fg) : m4;
+          if (shifted) logits<true>(P[qb], zs, rel, qn, k4);
+          else logits<false>(P[qb], zs, rel, qn, k4);
+          if constexpr (MASK) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int q = q0 + 16 * qb + 4 * fg + r;
+              if (q < L) P[qb][r] += mask_units(mask[(int64_t)q * L + kr]);
+            }
+          }
+          if (k0 + 16 > L && key >= L) P[qb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          weigh<MASK>(P[qb], Z[qb], m4, l4, d4);
+          if (alone) Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (bias) {
+          // the step's two sums, by branches: a register's index cannot vary
+#pragma unroll
+          for (int i = 0; i < X::STEPS; ++i)
+            if (q0 == QT * i) {
+              sums[2 * i] += Z[0];
+              sums[2 * i + 1] += Z[1];
+              asm volatile("" : "+v"(sums[2 * i]), "+v"(sums[2 * i + 1]));   // not by selects in every step
+            }
+        }
+        const typename D::TFrag pf = pair_frag<T>(P[0], P[1]), zf = pair_frag<T>(Z[0], Z[1]);
+        put4<T>(Zs + key * X::ZS + 4 * fg, zf, 0);
+        put4<T>(Zs + key * X::ZS + 16 + 4 * fg, zf, 1);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          dv[d] = mma(col_frag<T, D::STR>(Gs, 16 * d, fr, fg), pf, dv[d]);
+          dk[d] = mma(col_frag<T, D::STR>(Qs, 16 * d, fr, fg), zf, dk[d]);
+          if (d % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      wg_barrier();                                                // dz of all keys is there
+#pragma unroll
+      for (int i = 0; i < TASKS; ++i) {
+        const int t = wave + WAVES * i, d = t % ND, qb = t / ND;
+        if (t < 2 * ND && q0 + 16 * qb < L) {
+          f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < WAVES / 2; ++s) {
+            if (32 * s < L)
+              o = mma(col_frag<T, D::STR>(Ks + 32 * s * D::STR, 16 * d, fr, fg),
+                      col_frag<T, X::ZS>(Zs + 32 * s * X::ZS, 16 * qb, fr, fg), o);
+            if (s % 2) __builtin_amdgcn_sched_barrier(0);
+          }
+          const int q = q0 + 16 * qb + fr;
+          if (q < L) store_quad<T, HD>(dbase, (uint32_t)q * ldb, 16 * d + 4 * fg, a.hd, o, a.scale);
+        }
+      }
+    }
+    if (key < L) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        store_quad<T, HD>(dbase + ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dk[d], a.scale);
+        store_quad<T, HD>(dbase + 2 * (int64_t)ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dv[d], 1.f);
+      }
+    }
+  }
+  if (bias && key < L) {
+    float* dst = a.part + (int64_t)blockIdx.x * L * L + key;
+#pragma unroll
+    for (int i = 0; i < 2 * X::STEPS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int q = 16 * i + 4 * fg + r;
+        if (q < L) dst[(int64_t)q * L] = sums[i][r];
+      }
+  }
+}
+
+// ---------------------------------------------------------- longer windows ---
+
+template <typename T, int HD>
+constexpr size_t keys_lds() { return 2 * QT * Dim<T, HD>::STR * sizeof(T) + 4 * QT * sizeof(float); }
+
+template <typename T, int HD, int KB, bool MASK>
+__global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
+  typedef Dim<T, HD> D;
+  constexpr int ND = D::ND;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* Qs = (T*)smem;
+  T* Gs = Qs + QT * D::STR;
+  int* qinfo = (int*)(Gs + QT * D::STR);
+  float *mrow = (float*)qinfo + QT, *lrow = mrow + QT, *drow = lrow + QT;
+  float* rel = drow + QT;
 
   // a head's parts side by side
   const int part = (int)blockIdx.x % a.NP, kc = (int)blockIdx.x / a.NP % a.nqc, head = (int)blockIdx.x / a.NP / a.nqc;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
   const int L = a.L, C = a.C;
-  const int64_t ld = 3 * (int64_t)C;
+  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
   const int kw = kc * 64 * KB + wave * 16 * KB;                    // the wave's first key
-  const bool bias = a.part != nullptr, alone = L == 1;           // one token: p is 1 whatever z, dz exactly 0
+  const bool bias = a.part != nullptr;
+  const float zs = a.scale * LOG2E;
   load_rel<T>(a, head, rel);
-  if (bias)
-    for (int i = tid; i < a.copies * a.RS; i += NT) acc[i] = 0.f;
-  float* mine = acc + (a.copies == 16 ? (wave * 4 + fg) * a.RS : a.copies == 4 ? wave * a.RS : 0);
+  float* sums = a.part + ((int64_t)head * a.NP + part) * L * L + kw + fr;
 
   for (int64_t win = part; win < a.Bw; win += a.NP) {
-    const T* base = (const T*)a.qkv + win * L * ld + head * a.hd;
-    T* dbase = (T*)a.dqkv + win * L * ld + head * a.hd;
-    const T* gbase = (const T*)a.dout + win * L * (int64_t)C + head * a.hd;
-    const T* obase = (const T*)a.out + win * L * (int64_t)C + head * a.hd;
+    const int64_t at3 = win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T), at1 = win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
+    const char *base = (const char*)a.qkv + at3, *gbase = (const char*)a.dout + at1, *obase = (const char*)a.out + at1;
+    char* dbase = (char*)a.dqkv + at3;
     const f32x2* stats = (const f32x2*)a.stats + (win * a.heads + head) * L;
     const int wi = (int)(win % a.nW);
     const bool shifted = !MASK && wi >= a.band0;
@@ -84,54 +281,36 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
     TileCopy<T, HD, QT> qc, gc, oc;
     f32x2 st = {0.f, 0.f};
     auto load_tile = [&](int q0) {
-      qc.load(base + (int64_t)q0 * ld, ld, L - q0, a.hd);
-      gc.load(gbase + (int64_t)q0 * C, C, L - q0, a.hd);
-      oc.load(obase + (int64_t)q0 * C, C, L - q0, a.hd);
+      qc.load(base + (int64_t)q0 * ldb, ldb, L - q0, a.hd);
+      gc.load(gbase + (int64_t)q0 * ob, ob, L - q0, a.hd);
+      oc.load(obase + (int64_t)q0 * ob, ob, L - q0, a.hd);
       if (tid < QT) st = q0 + tid < L ? stats[q0 + tid] : f32x2{-INFINITY, 0.f};
     };
     load_tile(0);
-
     typename D::Frag kf[KB][D::NS], vf[KB][D::NS];
     int kinfo[KB];
     f32x4 dk[KB][ND], dv[KB][ND];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      const int key = kw + 16 * b + fr;
-      kinfo[b] = info_of(a, key, shifted) - a.off;
+      const int key = kw + 16 * b + fr, kr = key < L ? key : L - 1;
+      kinfo[b] = info_of(a, kr, shifted);
 #pragma unroll
       for (int s = 0; s < D::NS; ++s) {
-        typename D::Frag z = {};
-        kf[b][s] = key < L ? row_frag<T, HD>(base + (int64_t)key * ld + C, s, fg, a.hd) : z;
-        vf[b][s] = key < L ? row_frag<T, HD>(base + (int64_t)key * ld + 2 * C, s, fg, a.hd) : z;
+        kf[b][s] = row_frag<T, HD>(base + ob, (uint32_t)kr * ldb, s, fg, a.hd);
+        vf[b][s] = row_frag<T, HD>(base + 2 * (int64_t)ob, (uint32_t)kr * ldb, s, fg, a.hd);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) dk[b][d] = dv[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // k^T of the window, through LDS, for dq
-    typename D::TFrag kt[ALL ? KD : 1][ALL ? NKS : 1];
-    if constexpr (ALL) {
-      wg_barrier();                                                // the steps of the window before are done
-      TileCopy<T, HD, 64 * KB> all;
-      all.load(base + C, ld, L, a.hd);
-      all.store(Qs);
-      wg_barrier();
-#pragma unroll
-      for (int i = 0; i < KD; ++i) {
-        const int d = (wave + 4 * i) % ND;
-#pragma unroll
-        for (int s = 0; s < NKS; ++s) kt[i][s] = col_frag<T, D::STR>(Qs + 32 * s * D::STR, 16 * d, fr, fg);
-      }
-    }
 
     for (int q0 = 0; q0 < L; q0 += QT) {
-      wg_barrier();                                                // the tile before (ALL: and its dz) is read
+      wg_barrier();                                                // the tile before is read
       qc.store(Qs);
       gc.store(Gs);
-      row_dots<T, HD, QT>(gc, oc, drow);
+      row_dots(gc, oc, drow);
       if (tid < QT) {
-        qinfo[tid] = info_of(a, q0 + tid, shifted);
-        mrow[tid] = st[0] == -INFINITY ? INFINITY : st[0];         // an empty row, or none: p = 0
-        lrow[tid] = st[0] == -INFINITY ? 0.f : st[1];
+        qinfo[tid] = info_of(a, q0 + tid, shifted) + 4 * a.off;
+        put_stats<MASK>(st, mrow + tid, lrow + tid);
       }
       wg_barrier();
       if (q0 + QT < L) load_tile(q0 + QT);
@@ -142,98 +321,63 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
         typename D::Frag qf[D::NS], gf[D::NS];
 #pragma unroll
         for (int s = 0; s < D::NS; ++s) {
-          qf[s] = row_frag<T, HD>(Qs + (16 * qb + fr) * D::STR, s, fg, HD);
-          gf[s] = row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg, HD);
+          qf[s] = row_frag<T, HD>(Qs + (16 * qb + fr) * D::STR, s, fg);
+          gf[s] = row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg);
         }
         const int4 qi = *reinterpret_cast<const int4*>(qinfo + 16 * qb + 4 * fg);
         const int qn[4] = {qi.x, qi.y, qi.z, qi.w};
         const f32x4 m4 = *reinterpret_cast<const f32x4*>(mrow + 16 * qb + 4 * fg);
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(lrow + 16 * qb + 4 * fg);
         const f32x4 d4 = *reinterpret_cast<const f32x4*>(drow + 16 * qb + 4 * fg);
+        const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(lrow + 16 * qb + 4 * fg) : m4;
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-          f32x4 s4 = {0.f, 0.f, 0.f, 0.f}, g4 = {0.f, 0.f, 0.f, 0.f};
+          P[qb][b] = Z[qb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (kw + 16 * b >= L) continue;
+          const int key = kw + 16 * b + fr;
+          float* at = sums + (int64_t)(q0 + 16 * qb + 4 * fg) * L + 16 * b;
+          f32x4 old = {0.f, 0.f, 0.f, 0.f};
+          if (bias && win != part && key < L) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (q0 + 16 * qb + 4 * fg + r < L) old[r] = at[(int64_t)r * L];
+          }
 #pragma unroll
           for (int s = 0; s < D::NS; ++s) {
-            s4 = mma(qf[s], kf[b][s], s4);
-            g4 = mma(gf[s], vf[b][s], g4);
+            P[qb][b] = mma(qf[s], kf[b][s], P[qb][b]);
+            Z[qb][b] = mma(gf[s], vf[b][s], Z[qb][b]);
           }
-          const int key = kw + 16 * b + fr;
-          int at[4];
+          const int k4[4] = {kinfo[b], kinfo[b], kinfo[b], kinfo[b]};
+          if (shifted) logits<true>(P[qb][b], zs, rel, qn, k4);
+          else logits<false>(P[qb][b], zs, rel, qn, k4);
+          if constexpr (MASK) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            at[r] = (qn[r] - kinfo[b]) & (MAX_R - 1);
-            float z = fmaf(s4[r], a.scale, rel[at[r]]);
-            if constexpr (MASK) {
+            for (int r = 0; r < 4; ++r) {
               const int q = q0 + 16 * qb + 4 * fg + r;
-              if (q < L && key < L) z += mask[(int64_t)q * L + key];
-            } else if (shifted) {
-              z += (qn[r] ^ (kinfo[b] + a.off)) >> 30 ? -100.f : 0.f;
+              if (q < L) P[qb][b][r] += mask_units(mask[(int64_t)q * L + (key < L ? key : L - 1)]);
             }
-            const float p = key < L ? __builtin_amdgcn_exp2f(fmaf(z - m4[r], LOG2E, -l4[r])) : 0.f;
-            P[qb][b][r] = p;
-            Z[qb][b][r] = alone ? 0.f : p * (g4[r] - d4[r]);
           }
-          if (bias) {
-            // 32-bit LDS additions without a result; the lanes of a group lie at different displacements
-            auto add = [&](int r) { __hip_atomic_fetch_add(mine + at[r], Z[qb][b][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
-            if (a.copies == 16) {
-              if (key < L) {
+          if (kw + 16 * b + 16 > L && key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          weigh<MASK>(P[qb][b], Z[qb][b], m4, l4, d4);
+          if (bias && key < L) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) add(r);
-              }
-            } else if (a.copies == 4) {
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
-                if (fg == g && key < L) {
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) add(r);
-                }
-            } else {
-              for (int w = 0; w < 4; ++w) {
-                if (w == wave) {
-#pragma unroll
-                  for (int g = 0; g < 4; ++g)
-                    if (fg == g && key < L) {
-#pragma unroll
-                      for (int r = 0; r < 4; ++r) add(r);
-                    }
-                }
-                wg_barrier();
-              }
-            }
+            for (int r = 0; r < 4; ++r)
+              if (q0 + 16 * qb + 4 * fg + r < L) at[(int64_t)r * L] = old[r] + Z[qb][b][r];
           }
         }
       }
+      typename D::TFrag pf[KB], zf[KB];
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
-        const typename D::TFrag pf = pair_frag<T>(P[0][b], P[1][b]), zf = pair_frag<T>(Z[0][b], Z[1][b]);
-        if constexpr (ALL) {
-          T* zrow = Zs + (wave * 16 * KB + 16 * b + fr) * ZS + 4 * fg;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            typedef __attribute__((ext_vector_type(4))) T T4;
-            *reinterpret_cast<T4*>(zrow + 16 * h) = T4{zf[4 * h], zf[4 * h + 1], zf[4 * h + 2], zf[4 * h + 3]};
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[b][d] = mma(col_frag<T, D::STR>(Gs, 16 * d, fr, fg), pf, dv[b][d]);
-          dk[b][d] = mma(col_frag<T, D::STR>(Qs, 16 * d, fr, fg), zf, dk[b][d]);
-        }
+        pf[b] = pair_frag<T>(P[0][b], P[1][b]);
+        zf[b] = pair_frag<T>(Z[0][b], Z[1][b]);
       }
-      if constexpr (ALL) {
-        wg_barrier();                                              // dz of all keys is there
 #pragma unroll
-        for (int i = 0; i < DQ; ++i) {
-          const int t = wave + 4 * i, d = t % ND, qb = t / ND;     // ND 1: waves 2 and 3 have none
-          if (t < 2 * ND) {
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int d = 0; d < ND; ++d) {
+        const typename D::TFrag gt = col_frag<T, D::STR>(Gs, 16 * d, fr, fg), qt = col_frag<T, D::STR>(Qs, 16 * d, fr, fg);
 #pragma unroll
-            for (int s = 0; s < NKS; ++s) o = mma(kt[ND > 4 ? i % KD : 0][s], col_frag<T, ZS>(Zs + 32 * s * ZS, 16 * qb, fr, fg), o);
-            const int q = q0 + 16 * qb + fr;
-            if (q < L) store_quad<T, HD>(dbase + (int64_t)q * ld, 16 * d + 4 * fg, a.hd, o, a.scale);
-          }
+        for (int b = 0; b < KB; ++b) {
+          dv[b][d] = mma(gt, pf[b], dv[b][d]);
+          dk[b][d] = mma(qt, zf[b], dk[b][d]);
         }
       }
     }
@@ -241,22 +385,12 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
     for (int b = 0; b < KB; ++b) {
       const int key = kw + 16 * b + fr;
       if (key < L) {
-        T* row = dbase + (int64_t)key * ld;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          store_quad<T, HD>(row + C, 16 * d + 4 * fg, a.hd, dk[b][d], a.scale);
-          store_quad<T, HD>(row + 2 * C, 16 * d + 4 * fg, a.hd, dv[b][d], 1.f);
+          store_quad<T, HD>(dbase + ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dk[b][d], a.scale);
+          store_quad<T, HD>(dbase + 2 * (int64_t)ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dv[b][d], 1.f);
         }
       }
-    }
-  }
-  if (bias) {
-    wg_barrier();
-    float* dst = a.part + (int64_t)blockIdx.x * a.R;
-    for (int r = tid; r < a.R; r += NT) {
-      float t = acc[r];
-      for (int c = 1; c < a.copies; ++c) t += acc[c * a.RS + r];
-      dst[r] = t;
     }
   }
 }
@@ -279,39 +413,39 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
   const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
   const int L = a.L, C = a.C;
-  const int64_t ld = 3 * (int64_t)C;
-  const T* base = (const T*)a.qkv + win * L * ld + head * a.hd;
+  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
+  const int64_t at3 = win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T), at1 = win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
+  const char *base = (const char*)a.qkv + at3, *gbase = (const char*)a.dout + at1, *obase = (const char*)a.out + at1;
+  char* dbase = (char*)a.dqkv + at3;
   const int wi = (int)(win % a.nW);
   const bool shifted = !MASK && wi >= a.band0;
   const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
   const int q0 = qc * 64 * QB + wave * 16;
 
   TileCopy<T, HD, KT> kc, vc;
-  kc.load(base + C, ld, L, a.hd);
-  vc.load(base + 2 * C, ld, L, a.hd);
+  kc.load(base + ob, ldb, L, a.hd);
+  vc.load(base + 2 * (int64_t)ob, ldb, L, a.hd);
   typename D::Frag qf[QB][D::NS], gf[QB][D::NS];
   int qinfo[QB];
-  float m[QB], l2[QB], dots[QB];
+  float m[QB], l2[QB] = {}, dots[QB];
+  const float zs = a.scale * LOG2E;
   f32x4 O[QB][D::ND];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr, qr = q < L ? q : L - 1;
-    qinfo[i] = info_of(a, qr, shifted) + a.off;
-    const T* grow = (const T*)a.dout + (win * L + qr) * (int64_t)C + head * a.hd;
-    const T* orow = (const T*)a.out + (win * L + qr) * (int64_t)C + head * a.hd;
+    qinfo[i] = info_of(a, qr, shifted) + 4 * a.off;
     float t = 0.f;
 #pragma unroll
     for (int s = 0; s < D::NS; ++s) {
-      qf[i][s] = row_frag<T, HD>(base + qr * ld, s, fg, a.hd);
-      gf[i][s] = row_frag<T, HD>(grow, s, fg, a.hd);
-      const typename D::Frag of = row_frag<T, HD>(orow, s, fg, a.hd);
+      qf[i][s] = row_frag<T, HD>(base, (uint32_t)qr * ldb, s, fg, a.hd);
+      gf[i][s] = row_frag<T, HD>(gbase, (uint32_t)qr * ob, s, fg, a.hd);
+      const typename D::Frag of = row_frag<T, HD>(obase, (uint32_t)qr * ob, s, fg, a.hd);
 #pragma unroll
       for (int e = 0; e < D::EL; ++e) t = fmaf((float)gf[i][s][e], (float)of[e], t);
     }
     dots[i] = rows4_sum(t);
     const f32x2 st = ((const f32x2*)a.stats)[(win * a.heads + head) * L + qr];
-    m[i] = st[0] == -INFINITY ? INFINITY : st[0];
-    l2[i] = st[0] == -INFINITY ? 0.f : st[1];
+    put_stats<MASK>(st, &m[i], &l2[i]);
 #pragma unroll
     for (int d = 0; d < D::ND; ++d) O[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -325,8 +459,8 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
     wg_barrier();
     const int left = L - k0;
     if (left > KT) {
-      kc.load(base + (int64_t)(k0 + KT) * ld + C, ld, left - KT, a.hd);
-      vc.load(base + (int64_t)(k0 + KT) * ld + 2 * C, ld, left - KT, a.hd);
+      kc.load(base + (int64_t)(k0 + KT) * ldb + ob, ldb, left - KT, a.hd);
+      vc.load(base + (int64_t)(k0 + KT) * ldb + 2 * (int64_t)ob, ldb, left - KT, a.hd);
     }
     f32x4 Z[QB][2];
 #pragma unroll
@@ -334,8 +468,8 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
       typename D::Frag kf[D::NS], vf[D::NS];
 #pragma unroll
       for (int s = 0; s < D::NS; ++s) {
-        kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg, HD);
-        vf[s] = row_frag<T, HD>(Vs + (16 * kb + fr) * D::STR, s, fg, HD);
+        kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg);
+        vf[s] = row_frag<T, HD>(Vs + (16 * kb + fr) * D::STR, s, fg);
       }
       const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
       const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
@@ -347,19 +481,24 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
           s4 = mma(kf[s], qf[i][s], s4);
           g4 = mma(vf[s], gf[i][s], g4);
         }
-        const int q = q0 + 64 * i + fr;
+        const int qn[4] = {qinfo[i], qinfo[i], qinfo[i], qinfo[i]};
+        if (shifted) logits<true>(s4, zs, rel, qn, kn);
+        else logits<false>(s4, zs, rel, qn, kn);
+        if constexpr (MASK) {
+          const int q = q0 + 64 * i + fr;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float z = fmaf(s4[r], a.scale, rel[(qinfo[i] - kn[r]) & (MAX_R - 1)]);
-          const int key = k0 + 16 * kb + 4 * fg + r;
-          if constexpr (MASK) {
-            if (q < L && key < L) z += mask[(int64_t)q * L + key];
-          } else if (shifted) {
-            z += ((qinfo[i] - a.off) ^ kn[r]) >> 30 ? -100.f : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            const int key = k0 + 16 * kb + 4 * fg + r;
+            if (q < L && key < L) s4[r] += mask_units(mask[(int64_t)q * L + key]);
           }
-          const float p = key < L ? __builtin_amdgcn_exp2f(fmaf(z - m[i], LOG2E, -l2[i])) : 0.f;
-          Z[i][kb][r] = p * (g4[r] - dots[i]);                   // L > 64 here
         }
+        if (16 * kb + 16 > left) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * kb + 4 * fg + r >= left) s4[r] = -INFINITY;
+        }
+        weigh<MASK>(s4, g4, f32x4{m[i], m[i], m[i], m[i]}, f32x4{l2[i], l2[i], l2[i], l2[i]}, f32x4{dots[i], dots[i], dots[i], dots[i]});
+        Z[i][kb] = g4;
       }
     }
     typename D::TFrag kf[D::ND];
@@ -376,41 +515,58 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr;
     if (q < L) {
-      T* row = (T*)a.dqkv + (win * L + q) * ld + head * a.hd;
 #pragma unroll
-      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(row, 16 * d + 4 * fg, a.hd, O[i][d], a.scale);
+      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(dbase, (uint32_t)q * ldb, 16 * d + 4 * fg, a.hd, O[i][d], a.scale);
     }
   }
 }
 
-// sums[h, r] = the head's parts at displacement r, in order.
-__global__ __launch_bounds__(NT) void bias_sum_kernel(const float* __restrict__ part, float* __restrict__ sums, int P, int R) {
-  // 64 displacements to a workgroup, four groups of lanes that take every fourth part
-  __shared__ float red[4][64];
-  const int r = (int)blockIdx.x * 64 + ((int)threadIdx.x & 63), grp = (int)threadIdx.x >> 6;
-  const float* p = part + (int64_t)blockIdx.y * P * R;
-  float t = 0.f;
-  if (r < R)
+// out[h, y, r] = sum over the pairs of displacement r whose query lies in share y of the
+// window, and over the parts: a lane a displacement, neighbours on neighbouring keys.
+__global__ __launch_bounds__(NT) void pairs_kernel(Args a, float* __restrict__ out, int share) {
+  const int r = (int)blockIdx.x * NT + (int)threadIdx.x, h = (int)blockIdx.y, y = (int)blockIdx.z;
+  const int w2 = 2 * a.W - 1, a2 = 2 * a.A - 1;
+  const int dw = r % w2 - (a.W - 1), da = r / w2 % a2 - (a.A - 1), dt = r / w2 / a2 - (a.TW - 1);
+  const int back = (dt * a.A + da) * a.W + dw;             // tokens between query and key
+  const int64_t LL = (int64_t)a.L * a.L;
+  const float* part = a.part + (int64_t)h * a.NP * LL;
+  const int i0 = y * share, i1 = i0 + share < a.L ? i0 + share : a.L;
+  int w = i0 % a.W, i = i0 / a.W % a.A, t = i0 / (a.W * a.A);
+  float s = 0.f;
+  for (int q = i0; q < i1; ++q) {
+    if (r < a.R && (unsigned)(w - dw) < (unsigned)a.W && (unsigned)(i - da) < (unsigned)a.A && (unsigned)(t - dt) < (unsigned)a.TW) {
+      const float* at = part + (int64_t)q * a.L + (q - back);
 #pragma unroll 8
-    for (int i = grp; i < P; i += 4) t += p[(int64_t)i * R + r];
-  red[grp][threadIdx.x & 63] = t;
-  __syncthreads();
-  if (grp == 0 && r < R) sums[(int64_t)blockIdx.y * R + r] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+      for (int p = 0; p < a.NP; ++p) s += at[p * LL];
+    }
+    if (++w == a.W) {
+      w = 0;
+      if (++i == a.A) {
+        i = 0;
+        ++t;
+      }
+    }
+  }
+  if (r < a.R) out[((int64_t)h * gridDim.z + y) * a.R + r] = s;
 }
 
-// dtable[b, h] = sum of sums[h, r] over the displacements of bucket b, ascending: a lane a bucket.
+// dtable[b, h] = sum over the displacements of bucket b, ascending, of their shares' sums: a lane a bucket.
 template <typename T>
-__global__ __launch_bounds__(NT) void bias_table_kernel(const float* __restrict__ sums, const int* __restrict__ buckets,
-                                                        T* __restrict__ dtable, int R, int nb, int heads) {
+__global__ __launch_bounds__(NT) void table_kernel(const float* __restrict__ sums, const int* __restrict__ buckets,
+                                                   T* __restrict__ dtable, int R, int shares, int nb, int heads) {
   __shared__ __attribute__((aligned(16))) float v[1024];
   __shared__ __attribute__((aligned(16))) int at[1024];
   const int b = (int)blockIdx.x * NT + (int)threadIdx.x, h = (int)blockIdx.y;
   float t = 0.f;
-  for (int r0 = 0; r0 < R; r0 += 1024) {
+  for (int r0 = 0; r0 < R && shares; r0 += 1024) {
     __syncthreads();
     for (int i = (int)threadIdx.x; i < 1024; i += NT) {
       const int r = r0 + i;
-      v[i] = r < R ? sums[(int64_t)h * R + r] : 0.f;
+      float s = 0.f;
+      if (r < R)
+#pragma unroll 4
+        for (int y = 0; y < shares; ++y) s += sums[((int64_t)h * shares + y) * R + r];
+      v[i] = s;
       at[i] = r < R ? buckets[r] : -1;
     }
     __syncthreads();
@@ -427,29 +583,38 @@ __global__ __launch_bounds__(NT) void bias_table_kernel(const float* __restrict_
   if (b < nb) dtable[(int64_t)b * heads + h] = from_f32<T>(t);
 }
 
-// Key blocks of a wave in keys_kernel, and whether the workgroup holds the window.
-struct KeysPlan {
-  int KB;
-  bool all;
-};
+// Waves of windows_kernel for windows of L tokens; 0: longer than it takes (twelve waves do
+// not hold the accumulators of 256-byte rows, the LDS not k and v of 128 rows of 512 bytes).
+template <typename T, int HD> constexpr int MOST_WAVES = HD * (int)sizeof(T) >= 512 ? 4 : HD * (int)sizeof(T) >= 256 ? 8 : 12;
 template <typename T, int HD>
-KeysPlan keys_plan(int L) {
-  constexpr int MOST = HD == 128 ? (sizeof(T) == 4 ? 1 : 2) : 3;
-  const int KB = L <= 64 ? 1 : MOST >= 3 && L > 128 ? 3 : MOST >= 2 ? 2 : 1;
-  return {KB, L <= 64 * KB};
+int waves_of(int L) {
+  constexpr int MOST = MOST_WAVES<T, HD>;
+  const int w = L <= 64 ? 4 : L <= 128 ? 8 : 12;
+  return L <= 16 * MOST ? w : 0;
 }
 
-// Accumulators in LDS: one for each 16 lanes, each wave, or the workgroup, within 96 KB.
-void set_copies(Args& a) {
-  a.RS = (a.R + 51) / 64 * 64 + 12;                        // 12 mod 64: the groups' lanes fall in different banks
-  a.copies = 16 * a.RS * 4 <= (96 << 10) ? 16 : 4 * a.RS * 4 <= (96 << 10) ? 4 : 1;
+// 16-key blocks of a wave of keys_kernel.
+template <typename T, int HD> constexpr int KEY_BLOCKS = HD == 128 ? (sizeof(T) == 4 ? 1 : 2) : HD == 64 && sizeof(T) == 4 ? 2 : 3;
+
+// Workgroups that share a head's windows: as many as run at once in all (windows_kernel: four
+// waves to a SIMD or one workgroup to a compute unit; keys_kernel: two workgroups), each with the
+// same number of windows as near as can be.  keys_kernel: at most 2 GiB of sums, too.
+void set_parts(Args& a, int waves, int keys) {
+  a.nqc = waves ? 1 : (a.L + keys - 1) / keys;
+  const int64_t all = waves ? 256 * (16 / waves) : 512;
+  int64_t want = std::max<int64_t>(1, all / ((int64_t)a.heads * a.nqc));
+  if (!waves) want = std::max<int64_t>(1, std::min<int64_t>(want, (2LL << 30) / ((int64_t)a.heads * a.L * a.L * 4)));
+  const int64_t Bw = std::max<int64_t>(a.Bw, 1), each = (Bw + want - 1) / want;
+  a.NP = (int)((Bw + each - 1) / each);
 }
 
-// Workgroups that share a head's windows: about four to a compute unit in all.
-void set_parts(Args& a, int KB) {
-  a.nqc = (a.L + 64 * KB - 1) / (64 * KB);
-  const int64_t want = std::max<int64_t>(1, 1024 / ((int64_t)a.heads * a.nqc));
-  a.NP = (int)std::min<int64_t>(std::max<int64_t>(a.Bw, 1), want);
+// Shares of a window's queries in pairs_kernel: about 512 workgroups in all.
+int share_of(const Args& a, int* shares) {
+  const int64_t others = (int64_t)((a.R + NT - 1) / NT) * a.heads;
+  const int want = (int)std::max<int64_t>(1, std::min<int64_t>({16, a.L, 512 / others}));
+  const int share = (a.L + want - 1) / want;
+  *shares = (a.L + share - 1) / share;
+  return share;
 }
 
 template <typename F>
@@ -465,12 +630,22 @@ int with_kind(int dtype, int hd, F f) {
   return dtype == NSW_DTYPE_BF16 ? by(bf16{}) : by(float{});
 }
 
-template <typename T, int HD, int KB, bool ALL>
+template <typename T, int HD, int WAVES>
+int launch_windows(const Args& a, hipStream_t st) {
+  const size_t lds = Windows<T, HD, WAVES>::LDS + (size_t)a.R * sizeof(float);
+  const dim3 grid((unsigned)(a.NP * a.heads)), block(64 * WAVES);
+  if (a.mask) hipLaunchKernelGGL((windows_kernel<T, HD, WAVES, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((windows_kernel<T, HD, WAVES, false>), grid, block, lds, st, a);
+  return check_launch("nsw_position_attention_backward");
+}
+
+template <typename T, int HD>
 int launch_keys(const Args& a, hipStream_t st) {
-  const size_t lds = tile_bytes<T, HD, KB, ALL>() + (size_t)((a.R + 3) & ~3) * 4 + (a.part ? (size_t)a.copies * a.RS * 4 : 0);
+  constexpr int KB = KEY_BLOCKS<T, HD>;
+  const size_t lds = keys_lds<T, HD>() + (size_t)a.R * sizeof(float);
   const dim3 grid((unsigned)(a.NP * a.nqc * a.heads));
-  if (a.mask) hipLaunchKernelGGL((keys_kernel<T, HD, KB, ALL, true>), grid, dim3(NT), lds, st, a);
-  else hipLaunchKernelGGL((keys_kernel<T, HD, KB, ALL, false>), grid, dim3(NT), lds, st, a);
+  if (a.mask) hipLaunchKernelGGL((keys_kernel<T, HD, KB, true>), grid, dim3(NT), lds, st, a);
+  else hipLaunchKernelGGL((keys_kernel<T, HD, KB, false>), grid, dim3(NT), lds, st, a);
   return check_launch("nsw_position_attention_backward");
 }
 
@@ -493,10 +668,14 @@ int launch_queries(Args a, hipStream_t st) {
 size_t backward_workspace(const Args& a0, int dtype) {
   Args a = a0;
   with_kind(dtype, a.hd, [&](auto t, auto hd) {
-    set_parts(a, keys_plan<decltype(t), decltype(hd)::value>(a.L).KB);
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    set_parts(a, waves_of<T, HD>(a.L), 64 * KEY_BLOCKS<T, HD>);
     return 0;
   });
-  return (size_t)a.heads * ((size_t)a.NP * a.nqc + 1) * a.R * sizeof(float);
+  int shares;
+  share_of(a, &shares);
+  return (size_t)a.heads * ((size_t)shares * a.R + (size_t)a.NP * a.L * a.L) * sizeof(float);
 }
 
 int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream_t st) {
@@ -504,25 +683,30 @@ int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream
   return with_kind(dtype, a.hd, [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    const KeysPlan p = keys_plan<T, HD>(a.L);
-    set_parts(a, p.KB);
-    set_copies(a);
-    float* sums = workspace;                               // [heads, R], then the parts
-    a.part = dtable ? workspace + (size_t)a.heads * a.R : nullptr;
+    const int waves = waves_of<T, HD>(a.L);
+    set_parts(a, waves, 64 * KEY_BLOCKS<T, HD>);
+    int shares;
+    const int share = share_of(a, &shares);
+    float* sums = workspace;                               // [heads, shares, R], then the parts
+    a.part = dtable ? workspace + (size_t)a.heads * shares * a.R : nullptr;
     int rc = NSW_OK;
     if (a.Bw > 0) {
-      if (p.KB == 1) rc = p.all ? launch_keys<T, HD, 1, true>(a, st) : launch_keys<T, HD, 1, false>(a, st);
-      if constexpr (!(HD == 128 && sizeof(T) == 4))
-        if (p.KB == 2) rc = p.all ? launch_keys<T, HD, 2, true>(a, st) : launch_keys<T, HD, 2, false>(a, st);
-      if constexpr (HD != 128)
-        if (p.KB == 3) rc = p.all ? launch_keys<T, HD, 3, true>(a, st) : launch_keys<T, HD, 3, false>(a, st);
-      if (rc == NSW_OK && !p.all) rc = launch_queries<T, HD>(a, st);
+      if (waves == 4) rc = launch_windows<T, HD, 4>(a, st);
+      if constexpr (MOST_WAVES<T, HD> >= 8)
+        if (waves == 8) rc = launch_windows<T, HD, 8>(a, st);
+      if constexpr (MOST_WAVES<T, HD> >= 12)
+        if (waves == 12) rc = launch_windows<T, HD, 12>(a, st);
+      if (waves == 0) {
+        rc = launch_keys<T, HD>(a, st);
+        if (rc == NSW_OK) rc = launch_queries<T, HD>(a, st);
+      }
     }
     if (rc || !dtable) return rc;
-    const int P = a.Bw > 0 ? a.NP * a.nqc : 0;
-    hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((a.R + 63) / 64), (unsigned)a.heads), dim3(NT), 0, st, a.part, sums, P, a.R);
-    hipLaunchKernelGGL((bias_table_kernel<T>), dim3((unsigned)((a.nb + NT - 1) / NT), (unsigned)a.heads), dim3(NT), 0, st, sums,
-                       a.buckets, (T*)dtable, a.R, a.nb, a.heads);
+    if (a.Bw > 0)
+      hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)((a.R + NT - 1) / NT), (unsigned)a.heads, (unsigned)shares), dim3(NT), 0, st, a,
+                         sums, share);
+    hipLaunchKernelGGL((table_kernel<T>), dim3((unsigned)((a.nb + NT - 1) / NT), (unsigned)a.heads), dim3(NT), 0, st, sums,
+                       a.buckets, (T*)dtable, a.R, a.Bw > 0 ? shares : 0, a.nb, a.heads);
     return check_launch(what);
   });
 }

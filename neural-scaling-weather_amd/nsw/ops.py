@@ -682,8 +682,8 @@ def position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: t
     displacements of a query from a key, ((dt + T-1) (2A-1) + da + A-1) (2W-1) + dw + W-1;
     buckets [(2T-1)(2A-1)(2W-1)] int32 (at most 8192), table [buckets, num_heads] in
     qkv's dtype.  ``mask`` [nW, L, L] or ``geometry`` as window_attention; a row whose
-    mask leaves nothing gives zeros.  stats [Bw, num_heads, L, 2] fp32 (row maximum,
-    log2 of the sum of exp(z - maximum)) for position_attention_backward."""
+    mask leaves nothing gives zeros.  stats [Bw, num_heads, L, 2] fp32 (each row's
+    maximum m of z log2(e), log2 of its sum of 2^(z log2(e) - m)) for position_attention_backward."""
     what = "position_attention"
     at, Bw, L, C, mask, nW, sizes = _position_args(what, qkv, num_heads, table, buckets, extent, mask, geometry)
     o = qkv.new_empty((Bw, L, C))

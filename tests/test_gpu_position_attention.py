@@ -195,15 +195,15 @@ def test_boolean_mask(device, dtype, extent):
 @pytest.mark.parametrize("extent,shift,hd", [((1, 9, 18), (4, 9), 64), ((1, 3, 5), (1, 2), 16), ((2, 6, 6), (3, 0), 32),
                                              ((2, 9, 18), (0, 9), 32)])
 def test_shift_mask_from_the_geometry(device, dtype, extent, shift, hd):
-    """The same results as with the mask tensor that the geometry stands for."""
+    """Both forms of the mask within their tolerance of the formula, so of each other within twice that."""
     T, A, W = extent
     H, Wi = 3 * A, 2 * W
     t = case(dtype, 12, extent, 2, hd, seed=7)
     m = nsw.swin_helpers.attention_mask_closed_form(H, Wi, (A, W), shift, T)
     got = run(t, device, geometry=(H, Wi, (A, W), shift, T))
-    check(got, reference(t, m), dtype)
-    check(got, {k: (v.double().cpu(), 1e-6 + 2e-2 * v.abs().double().cpu()) for k, v in run(t, device, mask=m).items()
-                if k != "stats"}, dtype)
+    want = reference(t, m)
+    check(got, want, dtype)
+    check(run(t, device, mask=m), want, dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -235,10 +235,11 @@ def test_statistics(device, dtype):
     got = run(t, device)["stats"].double().cpu()
     q, k, _ = t["qkv"].double().view(2, 35, 3, 2, 32).permute(2, 0, 3, 1, 4)
     z = t["scale"] * q @ k.mT + t["table"].double()[pairs(1, 5, 7)].permute(2, 0, 1)
-    top = z.amax(-1)
+    top = z.amax(-1) * math.log2(math.e)
     assert ((got[..., 0] - top).abs() <= 1e-4 * (1 + top.abs())).all()
-    total = (z - top[..., None]).exp().sum(-1).log2()
-    assert ((got[..., 1] - total).abs() <= 1e-4).all()
+    total = (z * math.log2(math.e) - top[..., None]).exp2().sum(-1).log2()
+    # bf16: the sum of probabilities that are each off by at most 2^-8, log2(1 + 2^-8) < 5.7e-3
+    assert ((got[..., 1] - total).abs() <= (1e-4 if dtype == torch.float32 else 5.8e-3)).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

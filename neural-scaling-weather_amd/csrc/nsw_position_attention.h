@@ -1,6 +1,8 @@
 // Window attention with a learned position bias: what its forward and backward kernels share.
 #pragma once
 
+#include <type_traits>
+
 #include "nsw_common.h"
 
 namespace nsw {
@@ -94,7 +96,7 @@ template <typename T, int HD_> struct Dim {
   static constexpr int HD = HD_;
   static constexpr int EPC = 16 / (int)sizeof(T);          // values of a 16-byte chunk
   static constexpr int CPR = HD / EPC;                     // chunks of a row
-  static constexpr int STR = HD + (sizeof(T) == 2 ? 8 : 4);
+  static constexpr int STR = HD + (sizeof(T) == 4 ? 4 : HD == 16 ? 0 : 16);   // bf16: 8 times an odd number of banks
   static constexpr int NS = HD >= 32 ? HD / 32 : 1;        // k-steps of a product over the head dim
   static constexpr int ND = HD / 16;                       // 16-wide blocks of the head dim
   static constexpr int EL = sizeof(T) == 2 || HD >= 32 ? 8 : 4;
@@ -102,38 +104,49 @@ template <typename T, int HD_> struct Dim {
   typedef typename FragOf<T, 8>::type TFrag;               // over 32 tokens
 };
 
-// 16 bytes of a row of hd values (head dim 4 in bf16: 8 bytes and zeros), zeros past its end.
-// The row begins `off` bytes behind base; 32-bit offsets on one base of the wave leave the
-// lanes one register for an address (a window's rows end below 4 GiB: checked by the host).
+// n rows of a tensor, `ldb` bytes apart, of which this head has `bytes`: a buffer descriptor on
+// a base that is the same for the wave.  A lane's address is one 32-bit offset, what lies behind
+// the last row reads as zeros and is not written (rows of a window end below 2 GiB: checked by
+// the host), so no lane branches around its loads.
+struct Rows {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t ldb;
+  __device__ __forceinline__ Rows(const void* p, uint32_t ldb_, int n, int bytes) : ldb(ldb_) {
+    const uint64_t u = (uint64_t)p;
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32));
+    const int num = __builtin_amdgcn_readfirstlane(n > 0 ? (int)((uint32_t)(n - 1) * ldb + (uint32_t)bytes) : 0);
+    r = __builtin_amdgcn_make_buffer_rsrc((void*)(hi << 32 | lo), 0, num, 0x00020000);
+  }
+};
+constexpr uint32_t NOWHERE = 0xfffffff0u;   // an offset behind every row
+
+// 16 bytes, chunk ch, of a row of hd values, zeros past its end (head dims 4 and 8 among 16).
 template <typename T, int HD>
-__device__ __forceinline__ u32x4 load_chunk(const char* base, uint32_t off, int ch, int hd) {
+__device__ __forceinline__ u32x4 load_chunk(const Rows& x, uint32_t off, int ch, int hd) {
   constexpr int EPC = 16 / (int)sizeof(T);
-  const char* p = base + (off + 16u * (uint32_t)ch);
+  const uint32_t at = off + 16u * (uint32_t)ch;
   if constexpr (HD > 16) {
-    return *reinterpret_cast<const u32x4*>(p);
+    return __builtin_amdgcn_raw_buffer_load_b128(x.r, at, 0, 0);
   } else {
-    if ((ch + 1) * EPC <= hd) return *reinterpret_cast<const u32x4*>(p);
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (ch * EPC < hd) {
-      const uint64_t h = *reinterpret_cast<const uint64_t*>(p);
-      v[0] = (uint32_t)h;
-      v[1] = (uint32_t)(h >> 32);
-    }
-    return v;
+    if (hd >= EPC) return __builtin_amdgcn_raw_buffer_load_b128(x.r, ch * EPC < hd ? at : NOWHERE, 0, 0);
+    typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;      // bf16, head dim 4: 8 bytes
+    const u32x2 h = __builtin_amdgcn_raw_buffer_load_b64(x.r, ch == 0 ? at : NOWHERE, 0, 0);
+    return u32x4{h[0], h[1], 0u, 0u};
   }
 }
 
 // Fragment over the head dim, k-step s, of a row in memory: bf16 values 32 s + 8 fg .., fp32 the
 // same or (head dim 16) 4 fg ..
 template <typename T, int HD>
-__device__ __forceinline__ typename Dim<T, HD>::Frag row_frag(const char* base, uint32_t off, int s, int fg, int hd) {
+__device__ __forceinline__ typename Dim<T, HD>::Frag row_frag(const Rows& x, uint32_t row, int s, int fg, int hd) {
   typedef typename Dim<T, HD>::Frag F;
+  const uint32_t off = row * x.ldb;
   if constexpr (sizeof(T) == 4 && HD >= 32) {
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(base + (off + 128u * (uint32_t)s + 32u * (uint32_t)fg));
-    const f32x4 hi = *reinterpret_cast<const f32x4*>(base + (off + 128u * (uint32_t)s + 32u * (uint32_t)fg + 16u));
+    const f32x4 lo = __builtin_bit_cast(f32x4, load_chunk<T, HD>(x, off, 8 * s + 2 * fg, hd));
+    const f32x4 hi = __builtin_bit_cast(f32x4, load_chunk<T, HD>(x, off, 8 * s + 2 * fg + 1, hd));
     return F{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   } else {
-    return __builtin_bit_cast(F, load_chunk<T, HD>(base, off, 4 * s + fg, hd));
+    return __builtin_bit_cast(F, load_chunk<T, HD>(x, off, 4 * s + fg, hd));
   }
 }
 
@@ -202,25 +215,26 @@ __device__ __forceinline__ void load_rel(const Args& a, int head, float* rel) {
   }
 }
 
-// A tile of ROWS rows of HD values from memory (row r at base + r ldb bytes, rows from `rows`
-// on zeros) by way of registers: load() and later store() into LDS.
+// A tile of ROWS rows of HD values from memory by way of registers: load() and later store()
+// into LDS.  By NT threads, a
+// workgroup's or four waves of a larger one.
 template <typename T, int HD, int ROWS, int NT = posattn::NT>
 struct TileCopy {
   typedef Dim<T, HD> D;
   static constexpr int N = (ROWS * D::CPR + NT - 1) / NT;
   u32x4 v[N];
-  __device__ __forceinline__ void load(const char* base, uint32_t ldb, int rows, int hd) {
+  __device__ __forceinline__ void load(const Rows& x, int hd) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int i = (int)threadIdx.x + NT * c, r = i / D::CPR, ch = i % D::CPR;
+      const int i = (int)threadIdx.x % NT + NT * c, r = i / D::CPR, ch = i % D::CPR;
       v[c] = u32x4{0u, 0u, 0u, 0u};
-      if (r < rows && (ROWS * D::CPR % NT == 0 || r < ROWS)) v[c] = load_chunk<T, HD>(base, (uint32_t)r * ldb, ch, hd);
+      if (ROWS * D::CPR % NT == 0 || r < ROWS) v[c] = load_chunk<T, HD>(x, (uint32_t)r * x.ldb, ch, hd);
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int i = (int)threadIdx.x + NT * c, r = i / D::CPR, ch = i % D::CPR;
+      const int i = (int)threadIdx.x % NT + NT * c, r = i / D::CPR, ch = i % D::CPR;
       if (ROWS * D::CPR % NT == 0 || r < ROWS) *reinterpret_cast<u32x4*>(tile + r * D::STR + ch * D::EPC) = v[c];
     }
   }
@@ -232,7 +246,7 @@ __device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS, NT>& x, con
   typedef Dim<T, HD> D;
 #pragma unroll
   for (int c = 0; c < TileCopy<T, HD, ROWS, NT>::N; ++c) {
-    const int i = (int)threadIdx.x + NT * c, r = i / D::CPR, ch = i % D::CPR;
+    const int i = (int)threadIdx.x % NT + NT * c, r = i / D::CPR, ch = i % D::CPR;
     float s = 0.f;
     if constexpr (sizeof(T) == 2) {
       const bf16x8 u = __builtin_bit_cast(bf16x8, x.v[c]), w = __builtin_bit_cast(bf16x8, y.v[c]);
@@ -243,20 +257,62 @@ __device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS, NT>& x, con
 #pragma unroll
       for (int e = 0; e < 4; ++e) s = fmaf(u[e], w[e], s);
     }
-#pragma unroll
-    for (int off = D::CPR / 2; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+    // the row's lanes: pairs, quads, eights (half rows mirrored), sixteens (rows mirrored), 32
+    auto add = [&](auto ctrl) {
+      s += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, s), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    add(std::integral_constant<int, 0xB1>{});
+    if constexpr (D::CPR >= 4) add(std::integral_constant<int, 0x4E>{});
+    if constexpr (D::CPR >= 8) add(std::integral_constant<int, 0x141>{});
+    if constexpr (D::CPR >= 16) add(std::integral_constant<int, 0x140>{});
+    if constexpr (D::CPR >= 32) s = rows2_sum(s);
     if (ch == 0 && (ROWS * D::CPR % NT == 0 || r < ROWS)) dst[r] = s;
   }
 }
 
-// 4 values of a result to column d of a row of hd values, off bytes behind base.
+// 4 values of a result to column d of a row of hd values.
 template <typename T, int HD>
-__device__ __forceinline__ void store_quad(char* base, uint32_t off, int d, int hd, const f32x4& v, float f) {
-  if (HD > 16 || d < hd) {
-    const float x[4] = {v[0] * f, v[1] * f, v[2] * f, v[3] * f};
-    store4((T*)(base + (off + (uint32_t)(d * (int)sizeof(T)))), x);
+__device__ __forceinline__ void store_quad(const Rows& x, uint32_t row, int d, int hd, const f32x4& v, float f) {
+  const uint32_t at = HD > 16 || d < hd ? row * x.ldb + (uint32_t)(d * (int)sizeof(T)) : NOWHERE;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+    const bf16x4 o = {(bf16)(v[0] * f), (bf16)(v[1] * f), (bf16)(v[2] * f), (bf16)(v[3] * f)};
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, o), x.r, at, 0, 0);
+  } else {
+    const f32x4 o = {v[0] * f, v[1] * f, v[2] * f, v[3] * f};
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), x.r, at, 0, 0);
   }
 }
+
+// Where a window's rows begin in each tensor, for one head.
+struct At {
+  uint32_t ldb, ob;                 // bytes of a row of qkv, of o
+  int64_t q, o;                     // byte offsets
+  int bytes;                        // of a head in a row
+  __device__ __forceinline__ At(const Args& a, int64_t win, int head, int es) {
+    ob = (uint32_t)a.C * (uint32_t)es;
+    ldb = 3u * ob;
+    bytes = a.hd * es;
+    q = win * a.L * (int64_t)ldb + head * bytes;
+    o = win * a.L * (int64_t)ob + head * bytes;
+  }
+  // rows [r0, r0 + n) of part 0 (q), 1 (k), 2 (v) of qkv or its gradient; of o or its gradient
+  __device__ __forceinline__ Rows qkv(const void* p, int part, int r0, int n) const {
+    return Rows((const char*)p + q + (int64_t)r0 * ldb + part * (int64_t)ob, ldb, n, bytes);
+  }
+  __device__ __forceinline__ Rows out(const void* p, int r0, int n) const { return Rows((const char*)p + o + (int64_t)r0 * ob, ob, n, bytes); }
+};
+
+// A window's fp32 matrix [L, L], of a mask or of sums: element (q, k), pairs outside the window
+// nowhere.
+struct Plane {
+  __amdgpu_buffer_rsrc_t r;
+  int L;
+  __device__ __forceinline__ Plane(const float* p, int L_) : L(L_) { r = Rows(p, (uint32_t)L_ * 4u, L_, L_ * 4).r; }
+  __device__ __forceinline__ uint32_t at(int q, int k) const { return k < L ? (uint32_t)(q * L + k) * 4u : NOWHERE; }
+  __device__ __forceinline__ float get(int q, int k) const { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at(q, k), 0, 0)); }
+  __device__ __forceinline__ void put(int q, int k, float v) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, at(q, k), 0, 0); }
+};
 
 int launch_forward(Args a, int dtype, hipStream_t st);
 int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream_t st);

@@ -42,25 +42,25 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
   const int64_t win = a.dheads.div(item);
   const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
-  const int L = a.L, C = a.C;
-  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
-  const char* base = (const char*)a.qkv + win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T);
+  const int L = a.L;
+  const At at(a, win, head, (int)sizeof(T));
   const int wi = (int)(win % a.nW);
   const bool shifted = !MASK && wi >= a.band0;
-  const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
+  const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
   const int q0 = qc * 64 * QB + wave * 16;                 // block i of the wave: q0 + 64 i
 
   TileCopy<T, HD, KT> kc, vc;
-  kc.load(base + ob, ldb, L, a.hd);
-  vc.load(base + 2 * (int64_t)ob, ldb, L, a.hd);
+  kc.load(at.qkv(a.qkv, 1, 0, L), a.hd);
+  vc.load(at.qkv(a.qkv, 2, 0, L), a.hd);
+  const Rows qrows = at.qkv(a.qkv, 0, 0, L);
   typename D::Frag qf[QB][D::NS];
   int qinfo[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 64 * i + fr, qr = q < L ? q : L - 1;
-    qinfo[i] = info_of(a, qr, shifted) + 4 * a.off;
+    const int q = q0 + 64 * i + fr;                        // past the window: zeros
+    qinfo[i] = info_of(a, q, shifted) + 4 * a.off;
 #pragma unroll
-    for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(base, (uint32_t)qr * ldb, s, fg, a.hd);
+    for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(qrows, (uint32_t)q, s, fg, a.hd);
   }
   load_rel<T>(a, head, rel);
 
@@ -87,10 +87,8 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
     if (tid < KT) kinfo[tid] = info_of(a, k0 + tid, shifted);
     wg_barrier();
     const int left = L - k0;                               // keys from k0 on
-    if (left > KT) {
-      kc.load(base + (int64_t)(k0 + KT) * ldb + ob, ldb, left - KT, a.hd);
-      vc.load(base + (int64_t)(k0 + KT) * ldb + 2 * (int64_t)ob, ldb, left - KT, a.hd);
-    }
+    kc.load(at.qkv(a.qkv, 1, k0 + KT, left - KT), a.hd);
+    vc.load(at.qkv(a.qkv, 2, k0 + KT, left - KT), a.hd);
     f32x4 S[QB][4];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -119,8 +117,7 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
             const int q = q0 + 64 * i + fr;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int key = k0 + 16 * kb + 4 * fg + r;
-              if (q < L && key < L) S[i][kb][r] += mask_units(mask[(int64_t)q * L + key]);
+              S[i][kb][r] += mask_units(mask.get(q, k0 + 16 * kb + 4 * fg + r));
             }
           }
         }
@@ -144,15 +141,15 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[i][kb][r]);
       mx = fmaxf(m[i], rows4_max(mx));
-      const float at = mx == -INFINITY ? 0.f : mx;
-      const float f = __builtin_amdgcn_exp2f(m[i] - at);
+      const float to = mx == -INFINITY ? 0.f : mx;
+      const float f = __builtin_amdgcn_exp2f(m[i] - to);
       m[i] = mx;
       float t = 0.f;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(S[i][kb][r] - at);
+          const float p = __builtin_amdgcn_exp2f(S[i][kb][r] - to);
           S[i][kb][r] = p;
           if constexpr (!ONES) t += p;
         }
@@ -176,15 +173,15 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
         }
       }
   }
+  const Rows orows = at.out(a.o, 0, L);
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr;
     const float t = ONES ? Z[i][0] : rows4_sum(l[i]);
     const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;    // an empty row: zeros; NaN stays
-    if (q < L) {
-      char* orow = (char*)a.o + win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
 #pragma unroll
-      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orow, (uint32_t)q * ob, 16 * d + 4 * fg, a.hd, O[i][d], inv);
+    for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orows, (uint32_t)q, 16 * d + 4 * fg, a.hd, O[i][d], inv);
+    if (q < L) {
       if (fg == 0) *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + q) * 2) = f32x2{m[i], __builtin_amdgcn_logf(t)};
     }
   }
@@ -239,7 +236,7 @@ int make_args(Args& a, const char* what, int64_t Bw, int64_t L, int64_t C, int64
   NSW_CHECK_ARG(R <= MAX_R, "%s: %lld displacements in a window, at most %d", what, (long long)R, MAX_R);
   NSW_CHECK_ARG(nb > 0 && nb < (1 << 24), "%s: %lld buckets", what, (long long)nb);
   NSW_CHECK_ARG(std::isfinite(scale), "%s: scale=%g", what, (double)scale);
-  NSW_CHECK_ARG(Bw * L < (1LL << 40) && Bw * heads < (1LL << 31) && L * 3 * C * (int64_t)dtype_size(dtype) < (1LL << 32),
+  NSW_CHECK_ARG(Bw * L < (1LL << 40) && Bw * heads < (1LL << 31) && L * 3 * C * (int64_t)dtype_size(dtype) < (1LL << 31),
                 "%s: too large", what);
   a.Bw = Bw; a.L = (int)L; a.C = (int)C; a.heads = (int)heads; a.hd = (int)hd; a.R = (int)R; a.nb = (int)nb;
   a.TW = (int)T; a.A = (int)A; a.W = (int)W; a.scale = scale;

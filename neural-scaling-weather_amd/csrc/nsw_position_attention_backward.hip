@@ -49,6 +49,15 @@ __device__ __forceinline__ void put_stats(const f32x2& st, float* mrow, float* l
   }
 }
 
+// Statistics of query q0 + i of a window, of n queries from q0 on; none behind them.
+__device__ __forceinline__ f32x2 load_stats(const Args& a, int64_t win, int head, int q0, int n, int i) {
+  typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+  const Rows x(a.stats + ((win * a.heads + head) * a.L + q0) * 2, 8u, a.L - q0, 8);
+  const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(x.r, i < n ? 8u * (uint32_t)i : NOWHERE, 0, 0);
+  const f32x2 st = __builtin_bit_cast(f32x2, v);
+  return i < n ? st : f32x2{-INFINITY, 0.f};
+}
+
 // p and dz of four pairs from their products: s = q k, g = do v.
 template <bool MASK>
 __device__ __forceinline__ void weigh(f32x4& s, f32x4& g, const f32x4& m, const f32x4& l, const f32x4& d) {
@@ -70,9 +79,11 @@ __device__ __forceinline__ void put4(T* p, const typename FragOf<T, 8>::type& f,
 template <typename T, int HD, int WAVES> struct Windows {
   typedef Dim<T, HD> D;
   static constexpr int KEYS = 16 * WAVES, STEPS = WAVES / 2;
-  static constexpr int ZS = QT + 16 / (int)sizeof(T);              // values of a key's dz in LDS
-  static constexpr size_t TILES = (size_t)(2 * QT * D::STR + 2 * KEYS * D::STR + KEYS * ZS) * sizeof(T);
-  static constexpr size_t LDS = TILES + 4 * QT * sizeof(float);
+  static constexpr int ZS = QT + (sizeof(T) == 2 ? 16 : 4);        // values of a key's dz in LDS
+  static constexpr int QG = 2 * QT * D::STR;                       // a tile of q and do
+  static constexpr int ZT = KEYS * ZS;
+  static constexpr size_t TILES = (size_t)(2 * QG + 2 * KEYS * D::STR + 2 * ZT) * sizeof(T);
+  static constexpr size_t LDS = TILES + 2 * 4 * QT * sizeof(float);
 };
 
 template <typename T, int HD, int WAVES, bool MASK>
@@ -82,22 +93,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
   constexpr int N = 64 * WAVES, ND = D::ND;
   constexpr int TASKS = (2 * ND + WAVES - 1) / WAVES;              // 16 x 16 blocks of a tile's dq of a wave
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* Qs = (T*)smem;
-  T* Gs = Qs + QT * D::STR;
-  T* Ks = Gs + QT * D::STR;
+  T* QGs = (T*)smem;                                               // [2][q rows, do rows]
+  T* Ks = QGs + 2 * X::QG;
   T* Vs = Ks + X::KEYS * D::STR;
-  T* Zs = Vs + X::KEYS * D::STR;
-  int* qinfo = (int*)(smem + X::TILES);
-  float *mrow = (float*)qinfo + QT, *lrow = mrow + QT, *drow = lrow + QT;
-  float* rel = drow + QT;
+  T* Zs = Vs + X::KEYS * D::STR;                                   // [2][keys]
+  float* rows = (float*)(smem + X::TILES);                         // [2][infos, m, l, D]
+  float* rel = rows + 2 * 4 * QT;
 
   const int part = (int)blockIdx.x % a.NP, head = (int)blockIdx.x / a.NP;   // a head's parts side by side
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
-  const int L = a.L, C = a.C;
-  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
-  const int k0 = 16 * wave, key = k0 + fr;
-  const bool keys = k0 < L, bias = a.part != nullptr, alone = L == 1;       // alone: p is 1 whatever z, dz exactly 0
+  const int L = a.L, steps = (L + QT - 1) / QT;
+  const int key = 16 * wave + fr;
+  const bool keys = 16 * wave < L, bias = a.part != nullptr, alone = L == 1;   // alone: p is 1 whatever z, dz exactly 0
   const float zs = a.scale * LOG2E;
+  // the waves that bring in a tile's q, and its do and o: the last of them own few keys or none
+  const bool bring_q = wave / 4 == (WAVES == 12 ? 2 : 0), bring_g = wave / 4 == (WAVES == 4 ? 0 : 1);
   load_rel<T>(a, head, rel);
   f32x4 sums[2 * X::STEPS];
 #pragma unroll
@@ -105,98 +115,128 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
   if (!keys) {                                                     // dz of no keys: zeros, whatever the step
     typename D::TFrag z = {};
 #pragma unroll
-    for (int i = 0; i < QT / 16; ++i) put4<T>(Zs + key * X::ZS + 16 * i + 4 * fg, z, 0);
+    for (int i = 0; i < 4; ++i) put4<T>(Zs + i / 2 * X::ZT + key * X::ZS + 16 * (i % 2) + 4 * fg, z, 0);
   }
 
+  // what a window needs first, in registers: k, v and the first tile
+  TileCopy<T, HD, X::KEYS, N> kc, vc;
+  TileCopy<T, HD, QT> qc, gc, oc;
+  f32x2 st;
+  // rows of the window from q0 on, n of them (none: zeros, so that nothing is kept from before)
+  auto load_tile = [&](int64_t win, int q0, int n) {
+    const At at(a, win, head, (int)sizeof(T));
+    qc.load(at.qkv(a.qkv, 0, q0, bring_q ? n : 0), a.hd);
+    gc.load(at.out(a.dout, q0, bring_g ? n : 0), a.hd);
+    oc.load(at.out(a.out, q0, bring_g ? n : 0), a.hd);
+    st = load_stats(a, win, head, q0, tid < QT ? n : 0, tid);
+  };
+  auto load_window = [&](int64_t win) {
+    const int n = win < a.Bw ? L : 0;
+    const At at(a, win, head, (int)sizeof(T));
+    kc.load(at.qkv(a.qkv, 1, 0, n), a.hd);
+    vc.load(at.qkv(a.qkv, 2, 0, n), a.hd);
+    load_tile(win, 0, n);
+  };
+  auto store_tile = [&](int step, bool shifted) {
+    T* q = QGs + (step & 1) * X::QG;
+    float* r = rows + (step & 1) * 4 * QT;
+    if (bring_q) qc.store(q);
+    if (bring_g) {
+      gc.store(q + QT * D::STR);
+      row_dots(gc, oc, r + 3 * QT);
+    }
+    if (tid < QT) {
+      ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + 4 * a.off;
+      put_stats<MASK>(st, r + QT + tid, r + 2 * QT + tid);
+    }
+  };
+
+  load_window(part);
   for (int64_t win = part; win < a.Bw; win += a.NP) {
-    const int64_t at3 = win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T), at1 = win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
-    const char *base = (const char*)a.qkv + at3, *gbase = (const char*)a.dout + at1, *obase = (const char*)a.out + at1;
-    char* dbase = (char*)a.dqkv + at3;
-    const f32x2* stats = (const f32x2*)a.stats + (win * a.heads + head) * L;
+    const At at(a, win, head, (int)sizeof(T));
+    const Rows dq = at.qkv(a.dqkv, 0, 0, L);
     const int wi = (int)(win % a.nW);
     const bool shifted = !MASK && wi >= a.band0;
-    const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
-
-    {
-      TileCopy<T, HD, X::KEYS, N> kc, vc;
-      kc.load(base + ob, ldb, L, a.hd);
-      vc.load(base + 2 * (int64_t)ob, ldb, L, a.hd);
-      wg_barrier();                                                // the window before is done
-      kc.store(Ks);
-      vc.store(Vs);
-    }
-    TileCopy<T, HD, QT, N> qc, gc, oc;
-    f32x2 st;
-    auto load_tile = [&](int q0) {
-      qc.load(base + (int64_t)q0 * ldb, ldb, L - q0, a.hd);
-      gc.load(gbase + (int64_t)q0 * ob, ob, L - q0, a.hd);
-      oc.load(obase + (int64_t)q0 * ob, ob, L - q0, a.hd);
-      if (tid < QT) st = q0 + tid < L ? stats[q0 + tid] : f32x2{-INFINITY, 0.f};
-    };
-    load_tile(0);
-    const int kr = key < L ? key : L - 1;                          // keys past the window: p = 0 below
-    const int kinfo = info_of(a, kr, shifted);
-    const int k4[4] = {kinfo, kinfo, kinfo, kinfo};
+    const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
+    const int kinfo = info_of(a, key, shifted);
+    wg_barrier();                                                  // the window before is done with the LDS
+    kc.store(Ks);
+    vc.store(Vs);
+    store_tile(0, shifted);
+    wg_barrier();
     f32x4 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-#pragma unroll 1
-    for (int q0 = 0; q0 < L; q0 += QT) {
-      wg_barrier();                                                // the tile before and its dz are read
-      qc.store(Qs);
-      gc.store(Gs);
-      row_dots(gc, oc, drow);
-      if (tid < QT) {
-        qinfo[tid] = info_of(a, q0 + tid, shifted) + 4 * a.off;
-        put_stats<MASK>(st, mrow + tid, lrow + tid);
+    // dq of a step's tile, from dz of all keys and k
+    auto queries = [&](int step) {
+      const T* z = Zs + (step & 1) * X::ZT;
+#pragma unroll
+      for (int i = 0; i < TASKS; ++i) {
+        const int t = wave + WAVES * i, d = t % ND, qb = t / ND;
+        if (t < 2 * ND) {
+          f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < WAVES / 2; ++s) {
+            o = mma(col_frag<T, D::STR>(Ks + 32 * s * D::STR, 16 * d, fr, fg), col_frag<T, X::ZS>(z + 32 * s * X::ZS, 16 * qb, fr, fg), o);
+            if (s % 3 == 2) __builtin_amdgcn_sched_barrier(0);
+          }
+          store_quad<T, HD>(dq, (uint32_t)(QT * step + 16 * qb + fr), 16 * d + 4 * fg, a.hd, o, a.scale);
+        }
       }
-      wg_barrier();
-      if (q0 + QT < L) load_tile(q0 + QT);
+    };
 
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      load_tile(win, QT * (step + 1), L - QT * (step + 1));
       if (keys) {
+        const T *Qs = QGs + (step & 1) * X::QG, *Gs = Qs + QT * D::STR;
+        const float* r0 = rows + (step & 1) * 4 * QT;
         f32x4 P[2], Z[2];                                          // queries 16 qb + 4 fg + r, key fr
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          P[qb] = Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (q0 + 16 * qb >= L) continue;
+        for (int qb = 0; qb < 2; ++qb) P[qb] = Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int s = 0; s < D::NS; ++s) {
-            P[qb] = mma(row_frag<T, HD>(Qs + (16 * qb + fr) * D::STR, s, fg), row_frag<T, HD>(Ks + key * D::STR, s, fg), P[qb]);
-            Z[qb] = mma(row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg), row_frag<T, HD>(Vs + key * D::STR, s, fg), Z[qb]);
+        for (int s = 0; s < D::NS; ++s) {
+          const typename D::Frag kf = row_frag<T, HD>(Ks + key * D::STR, s, fg), vf = row_frag<T, HD>(Vs + key * D::STR, s, fg);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) {
+            P[qb] = mma(row_frag<T, HD>(Qs + (16 * qb + fr) * D::STR, s, fg), kf, P[qb]);
+            Z[qb] = mma(row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg), vf, Z[qb]);
           }
-          const int4 qi = *reinterpret_cast<const int4*>(qinfo + 16 * qb + 4 * fg);
+        }
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          const int4 qi = *reinterpret_cast<const int4*>(r0 + 16 * qb + 4 * fg);
           const int qn[4] = {qi.x, qi.y, qi.z, qi.w};
-          const f32x4 m4 = *reinterpret_cast<const f32x4*>(mrow + 16 * qb + 4 * fg);
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(drow + 16 * qb + 4 * fg);
-          const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(lrow + 16 * qb + 4 * fg) : m4;
-          if (shifted) logits<true>(P[qb], zs, rel, qn, k4);
-          else logits<false>(P[qb], zs, rel, qn, k4);
+          const f32x4 m4 = *reinterpret_cast<const f32x4*>(r0 + QT + 16 * qb + 4 * fg);
+          const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg) : m4;
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(r0 + 3 * QT + 16 * qb + 4 * fg);
+          if (shifted) logits<true>(P[qb], zs, rel, qn, {kinfo, kinfo, kinfo, kinfo});
+          else logits<false>(P[qb], zs, rel, qn, {kinfo, kinfo, kinfo, kinfo});
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int q = q0 + 16 * qb + 4 * fg + r;
-              if (q < L) P[qb][r] += mask_units(mask[(int64_t)q * L + kr]);
+              P[qb][r] += mask_units(mask.get(QT * step + 16 * qb + 4 * fg + r, key));
             }
           }
-          if (k0 + 16 > L && key >= L) P[qb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (key >= L) P[qb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           weigh<MASK>(P[qb], Z[qb], m4, l4, d4);
           if (alone) Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-          __builtin_amdgcn_sched_barrier(0);
         }
+        const typename D::TFrag pf = pair_frag<T>(P[0], P[1]), zf = pair_frag<T>(Z[0], Z[1]);
+        T* z = Zs + (step & 1) * X::ZT + key * X::ZS + 4 * fg;
+        put4<T>(z, zf, 0);
+        put4<T>(z + 16, zf, 1);
         if (bias) {
           // the step's two sums, by branches: a register's index cannot vary
 #pragma unroll
           for (int i = 0; i < X::STEPS; ++i)
-            if (q0 == QT * i) {
+            if (step == i) {
               sums[2 * i] += Z[0];
               sums[2 * i + 1] += Z[1];
               asm volatile("" : "+v"(sums[2 * i]), "+v"(sums[2 * i + 1]));   // not by selects in every step
             }
         }
-        const typename D::TFrag pf = pair_frag<T>(P[0], P[1]), zf = pair_frag<T>(Z[0], Z[1]);
-        put4<T>(Zs + key * X::ZS + 4 * fg, zf, 0);
-        put4<T>(Zs + key * X::ZS + 16 + 4 * fg, zf, 1);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           dv[d] = mma(col_frag<T, D::STR>(Gs, 16 * d, fr, fg), pf, dv[d]);
@@ -204,41 +244,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
           if (d % 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      wg_barrier();                                                // dz of all keys is there
-#pragma unroll
-      for (int i = 0; i < TASKS; ++i) {
-        const int t = wave + WAVES * i, d = t % ND, qb = t / ND;
-        if (t < 2 * ND && q0 + 16 * qb < L) {
-          f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < WAVES / 2; ++s) {
-            if (32 * s < L)
-              o = mma(col_frag<T, D::STR>(Ks + 32 * s * D::STR, 16 * d, fr, fg),
-                      col_frag<T, X::ZS>(Zs + 32 * s * X::ZS, 16 * qb, fr, fg), o);
-            if (s % 2) __builtin_amdgcn_sched_barrier(0);
-          }
-          const int q = q0 + 16 * qb + fr;
-          if (q < L) store_quad<T, HD>(dbase, (uint32_t)q * ldb, 16 * d + 4 * fg, a.hd, o, a.scale);
-        }
-      }
+      if (step > 0) queries(step - 1);
+      if (step + 1 < steps) store_tile(step + 1, shifted);
+      wg_barrier();                                                // this step's dz and the next tile are there
     }
-    if (key < L) {
+    load_window(win + a.NP);
+    queries(steps - 1);
+    const Rows dkr = at.qkv(a.dqkv, 1, 0, L), dvr = at.qkv(a.dqkv, 2, 0, L);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        store_quad<T, HD>(dbase + ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dk[d], a.scale);
-        store_quad<T, HD>(dbase + 2 * (int64_t)ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dv[d], 1.f);
-      }
+    for (int d = 0; d < ND; ++d) {
+      store_quad<T, HD>(dkr, (uint32_t)key, 16 * d + 4 * fg, a.hd, dk[d], a.scale);
+      store_quad<T, HD>(dvr, (uint32_t)key, 16 * d + 4 * fg, a.hd, dv[d], 1.f);
     }
   }
-  if (bias && key < L) {
-    float* dst = a.part + (int64_t)blockIdx.x * L * L + key;
+  if (bias) {
+    const Plane dst(a.part + (int64_t)blockIdx.x * L * L, L);
 #pragma unroll
     for (int i = 0; i < 2 * X::STEPS; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int q = 16 * i + 4 * fg + r;
-        if (q < L) dst[(int64_t)q * L] = sums[i][r];
-      }
+      for (int r = 0; r < 4; ++r) dst.put(16 * i + 4 * fg + r, key, sums[i][r]);
   }
 }
 
@@ -261,43 +285,40 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
   // a head's parts side by side
   const int part = (int)blockIdx.x % a.NP, kc = (int)blockIdx.x / a.NP % a.nqc, head = (int)blockIdx.x / a.NP / a.nqc;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
-  const int L = a.L, C = a.C;
-  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
+  const int L = a.L;
   const int kw = kc * 64 * KB + wave * 16 * KB;                    // the wave's first key
   const bool bias = a.part != nullptr;
   const float zs = a.scale * LOG2E;
   load_rel<T>(a, head, rel);
-  float* sums = a.part + ((int64_t)head * a.NP + part) * L * L + kw + fr;
+  const Plane sums(bias ? a.part + ((int64_t)head * a.NP + part) * L * L : nullptr, bias ? L : 0);
 
   for (int64_t win = part; win < a.Bw; win += a.NP) {
-    const int64_t at3 = win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T), at1 = win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
-    const char *base = (const char*)a.qkv + at3, *gbase = (const char*)a.dout + at1, *obase = (const char*)a.out + at1;
-    char* dbase = (char*)a.dqkv + at3;
-    const f32x2* stats = (const f32x2*)a.stats + (win * a.heads + head) * L;
+    const At at(a, win, head, (int)sizeof(T));
     const int wi = (int)(win % a.nW);
     const bool shifted = !MASK && wi >= a.band0;
-    const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
+    const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
 
     TileCopy<T, HD, QT> qc, gc, oc;
-    f32x2 st = {0.f, 0.f};
+    f32x2 st;
     auto load_tile = [&](int q0) {
-      qc.load(base + (int64_t)q0 * ldb, ldb, L - q0, a.hd);
-      gc.load(gbase + (int64_t)q0 * ob, ob, L - q0, a.hd);
-      oc.load(obase + (int64_t)q0 * ob, ob, L - q0, a.hd);
-      if (tid < QT) st = q0 + tid < L ? stats[q0 + tid] : f32x2{-INFINITY, 0.f};
+      qc.load(at.qkv(a.qkv, 0, q0, L - q0), a.hd);
+      gc.load(at.out(a.dout, q0, L - q0), a.hd);
+      oc.load(at.out(a.out, q0, L - q0), a.hd);
+      st = load_stats(a, win, head, q0, tid < QT ? L - q0 : 0, tid);
     };
     load_tile(0);
+    const Rows krows = at.qkv(a.qkv, 1, 0, L), vrows = at.qkv(a.qkv, 2, 0, L);
     typename D::Frag kf[KB][D::NS], vf[KB][D::NS];
     int kinfo[KB];
     f32x4 dk[KB][ND], dv[KB][ND];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      const int key = kw + 16 * b + fr, kr = key < L ? key : L - 1;
-      kinfo[b] = info_of(a, kr, shifted);
+      const int key = kw + 16 * b + fr;                            // past the window: zeros
+      kinfo[b] = info_of(a, key, shifted);
 #pragma unroll
       for (int s = 0; s < D::NS; ++s) {
-        kf[b][s] = row_frag<T, HD>(base + ob, (uint32_t)kr * ldb, s, fg, a.hd);
-        vf[b][s] = row_frag<T, HD>(base + 2 * (int64_t)ob, (uint32_t)kr * ldb, s, fg, a.hd);
+        kf[b][s] = row_frag<T, HD>(krows, (uint32_t)key, s, fg, a.hd);
+        vf[b][s] = row_frag<T, HD>(vrows, (uint32_t)key, s, fg, a.hd);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) dk[b][d] = dv[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -313,7 +334,7 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
         put_stats<MASK>(st, mrow + tid, lrow + tid);
       }
       wg_barrier();
-      if (q0 + QT < L) load_tile(q0 + QT);
+      load_tile(q0 + QT);
 
       f32x4 P[2][KB], Z[2][KB];                                    // queries 16 qb + 4 fg + r, key fr of block b
 #pragma unroll
@@ -334,12 +355,10 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
           P[qb][b] = Z[qb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
           if (kw + 16 * b >= L) continue;
           const int key = kw + 16 * b + fr;
-          float* at = sums + (int64_t)(q0 + 16 * qb + 4 * fg) * L + 16 * b;
           f32x4 old = {0.f, 0.f, 0.f, 0.f};
-          if (bias && win != part && key < L) {
+          if (bias && win != part) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (q0 + 16 * qb + 4 * fg + r < L) old[r] = at[(int64_t)r * L];
+            for (int r = 0; r < 4; ++r) old[r] = sums.get(q0 + 16 * qb + 4 * fg + r, key);
           }
 #pragma unroll
           for (int s = 0; s < D::NS; ++s) {
@@ -352,16 +371,14 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int q = q0 + 16 * qb + 4 * fg + r;
-              if (q < L) P[qb][b][r] += mask_units(mask[(int64_t)q * L + (key < L ? key : L - 1)]);
+              P[qb][b][r] += mask_units(mask.get(q0 + 16 * qb + 4 * fg + r, key));
             }
           }
           if (kw + 16 * b + 16 > L && key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           weigh<MASK>(P[qb][b], Z[qb][b], m4, l4, d4);
-          if (bias && key < L) {
+          if (bias) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (q0 + 16 * qb + 4 * fg + r < L) at[(int64_t)r * L] = old[r] + Z[qb][b][r];
+            for (int r = 0; r < 4; ++r) sums.put(q0 + 16 * qb + 4 * fg + r, key, old[r] + Z[qb][b][r]);
           }
         }
       }
@@ -381,17 +398,14 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
         }
       }
     }
+    const Rows dkr = at.qkv(a.dqkv, 1, 0, L), dvr = at.qkv(a.dqkv, 2, 0, L);
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      const int key = kw + 16 * b + fr;
-      if (key < L) {
+    for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          store_quad<T, HD>(dbase + ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dk[b][d], a.scale);
-          store_quad<T, HD>(dbase + 2 * (int64_t)ob, (uint32_t)key * ldb, 16 * d + 4 * fg, a.hd, dv[b][d], 1.f);
-        }
+      for (int d = 0; d < ND; ++d) {
+        store_quad<T, HD>(dkr, (uint32_t)(kw + 16 * b + fr), 16 * d + 4 * fg, a.hd, dk[b][d], a.scale);
+        store_quad<T, HD>(dvr, (uint32_t)(kw + 16 * b + fr), 16 * d + 4 * fg, a.hd, dv[b][d], 1.f);
       }
-    }
   }
 }
 
@@ -412,19 +426,17 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
   const int64_t win = a.dheads.div(item);
   const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
-  const int L = a.L, C = a.C;
-  const uint32_t ldb = 3u * (uint32_t)C * (uint32_t)sizeof(T), ob = (uint32_t)C * (uint32_t)sizeof(T);   // rows of qkv and of o
-  const int64_t at3 = win * L * (int64_t)ldb + head * a.hd * (int)sizeof(T), at1 = win * L * (int64_t)ob + head * a.hd * (int)sizeof(T);
-  const char *base = (const char*)a.qkv + at3, *gbase = (const char*)a.dout + at1, *obase = (const char*)a.out + at1;
-  char* dbase = (char*)a.dqkv + at3;
+  const int L = a.L;
+  const At at(a, win, head, (int)sizeof(T));
   const int wi = (int)(win % a.nW);
   const bool shifted = !MASK && wi >= a.band0;
-  const float* mask = MASK ? a.mask + (int64_t)wi * L * L : nullptr;
+  const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
   const int q0 = qc * 64 * QB + wave * 16;
 
   TileCopy<T, HD, KT> kc, vc;
-  kc.load(base + ob, ldb, L, a.hd);
-  vc.load(base + 2 * (int64_t)ob, ldb, L, a.hd);
+  kc.load(at.qkv(a.qkv, 1, 0, L), a.hd);
+  vc.load(at.qkv(a.qkv, 2, 0, L), a.hd);
+  const Rows qrows = at.qkv(a.qkv, 0, 0, L), grows = at.out(a.dout, 0, L), orows = at.out(a.out, 0, L);
   typename D::Frag qf[QB][D::NS], gf[QB][D::NS];
   int qinfo[QB];
   float m[QB], l2[QB] = {}, dots[QB];
@@ -432,20 +444,19 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
   f32x4 O[QB][D::ND];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 64 * i + fr, qr = q < L ? q : L - 1;
-    qinfo[i] = info_of(a, qr, shifted) + 4 * a.off;
+    const int q = q0 + 64 * i + fr;                        // past the window: zeros
+    qinfo[i] = info_of(a, q, shifted) + 4 * a.off;
     float t = 0.f;
 #pragma unroll
     for (int s = 0; s < D::NS; ++s) {
-      qf[i][s] = row_frag<T, HD>(base, (uint32_t)qr * ldb, s, fg, a.hd);
-      gf[i][s] = row_frag<T, HD>(gbase, (uint32_t)qr * ob, s, fg, a.hd);
-      const typename D::Frag of = row_frag<T, HD>(obase, (uint32_t)qr * ob, s, fg, a.hd);
+      qf[i][s] = row_frag<T, HD>(qrows, (uint32_t)q, s, fg, a.hd);
+      gf[i][s] = row_frag<T, HD>(grows, (uint32_t)q, s, fg, a.hd);
+      const typename D::Frag of = row_frag<T, HD>(orows, (uint32_t)q, s, fg, a.hd);
 #pragma unroll
       for (int e = 0; e < D::EL; ++e) t = fmaf((float)gf[i][s][e], (float)of[e], t);
     }
     dots[i] = rows4_sum(t);
-    const f32x2 st = ((const f32x2*)a.stats)[(win * a.heads + head) * L + qr];
-    put_stats<MASK>(st, &m[i], &l2[i]);
+    put_stats<MASK>(load_stats(a, win, head, 0, L, q), &m[i], &l2[i]);
 #pragma unroll
     for (int d = 0; d < D::ND; ++d) O[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -458,10 +469,8 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
     if (tid < KT) kinfo[tid] = info_of(a, k0 + tid, shifted);
     wg_barrier();
     const int left = L - k0;
-    if (left > KT) {
-      kc.load(base + (int64_t)(k0 + KT) * ldb + ob, ldb, left - KT, a.hd);
-      vc.load(base + (int64_t)(k0 + KT) * ldb + 2 * (int64_t)ob, ldb, left - KT, a.hd);
-    }
+    kc.load(at.qkv(a.qkv, 1, k0 + KT, left - KT), a.hd);
+    vc.load(at.qkv(a.qkv, 2, k0 + KT, left - KT), a.hd);
     f32x4 Z[QB][2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -485,12 +494,8 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
         if (shifted) logits<true>(s4, zs, rel, qn, kn);
         else logits<false>(s4, zs, rel, qn, kn);
         if constexpr (MASK) {
-          const int q = q0 + 64 * i + fr;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = k0 + 16 * kb + 4 * fg + r;
-            if (q < L && key < L) s4[r] += mask_units(mask[(int64_t)q * L + key]);
-          }
+          for (int r = 0; r < 4; ++r) s4[r] += mask_units(mask.get(q0 + 64 * i + fr, k0 + 16 * kb + 4 * fg + r));
         }
         if (16 * kb + 16 > left) {
 #pragma unroll
@@ -511,14 +516,11 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
       for (int d = 0; d < D::ND; ++d) O[i][d] = mma(kf[d], zf, O[i][d]);
     }
   }
+  const Rows dq = at.qkv(a.dqkv, 0, 0, L);
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 64 * i + fr;
-    if (q < L) {
+  for (int i = 0; i < QB; ++i)
 #pragma unroll
-      for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(dbase, (uint32_t)q * ldb, 16 * d + 4 * fg, a.hd, O[i][d], a.scale);
-    }
-  }
+    for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(dq, (uint32_t)(q0 + 64 * i + fr), 16 * d + 4 * fg, a.hd, O[i][d], a.scale);
 }
 
 // out[h, y, r] = sum over the pairs of displacement r whose query lies in share y of the
@@ -588,9 +590,8 @@ __global__ __launch_bounds__(NT) void table_kernel(const float* __restrict__ sum
 template <typename T, int HD> constexpr int MOST_WAVES = HD * (int)sizeof(T) >= 512 ? 4 : HD * (int)sizeof(T) >= 256 ? 8 : 12;
 template <typename T, int HD>
 int waves_of(int L) {
-  constexpr int MOST = MOST_WAVES<T, HD>;
   const int w = L <= 64 ? 4 : L <= 128 ? 8 : 12;
-  return L <= 16 * MOST ? w : 0;
+  return L <= 192 && w <= MOST_WAVES<T, HD> ? w : 0;
 }
 
 // 16-key blocks of a wave of keys_kernel.
@@ -633,9 +634,9 @@ int with_kind(int dtype, int hd, F f) {
 template <typename T, int HD, int WAVES>
 int launch_windows(const Args& a, hipStream_t st) {
   const size_t lds = Windows<T, HD, WAVES>::LDS + (size_t)a.R * sizeof(float);
-  const dim3 grid((unsigned)(a.NP * a.heads)), block(64 * WAVES);
-  if (a.mask) hipLaunchKernelGGL((windows_kernel<T, HD, WAVES, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((windows_kernel<T, HD, WAVES, false>), grid, block, lds, st, a);
+  const dim3 grid((unsigned)(a.NP * a.heads));
+  if (a.mask) hipLaunchKernelGGL((windows_kernel<T, HD, WAVES, true>), grid, dim3(64 * WAVES), lds, st, a);
+  else hipLaunchKernelGGL((windows_kernel<T, HD, WAVES, false>), grid, dim3(64 * WAVES), lds, st, a);
   return check_launch("nsw_position_attention_backward");
 }
 

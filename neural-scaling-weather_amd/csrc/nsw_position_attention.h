@@ -40,21 +40,32 @@ __device__ __forceinline__ int info_of(const Args& a, int p, bool shifted) {
   return 4 * code | (shifted && i >= a.thr ? 1 << 30 : 0);
 }
 
-// Four logits in units of log2 e from products s: z_r = s_r zs + rel[q_r - k_r] + mask, q and k the
-// infos with the middle displacement's offset added to q's, rel and the masks times log2 e.
-// SHIFT: -100 between the classes.  R <= 8192 = 2^13, so that their bits fall out of the offset.
-template <bool SHIFT>
-__device__ __forceinline__ void logits(f32x4& s, float zs, const float* rel, const int (&q)[4], const int (&k)[4]) {
+// The byte address in LDS of rel, to which the queries' infos are moved together with the middle
+// displacement: a pair's bias then lies at the difference of its two infos.
+__device__ __forceinline__ int rel_base(const Args& a, const float* rel) {
+  return (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const float*)rel + 4 * a.off;
+}
+
+// Biases of four pairs in units of log2 e from the infos of their queries (moved) and keys; with a
+// shift -100 between the classes, whose bits have to be kept out of the address.
+__device__ __forceinline__ f32x4 biases(const int (&q)[4], const int (&k)[4], bool shifted) {
+  typedef __attribute__((address_space(3))) const float* lds_ptr;
+  f32x4 b;
+  if (shifted) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int d = q[r] - k[r];
-    if constexpr (SHIFT) {
-      s[r] = fmaf(s[r], zs, *reinterpret_cast<const float*>((const char*)rel + (d & (4 * MAX_R - 4))));
-      s[r] += (q[r] ^ k[r]) >> 30 ? -100.f * LOG2E : 0.f;
-    } else {
-      s[r] = fmaf(s[r], zs, *reinterpret_cast<const float*>((const char*)rel + d));
-    }
+    for (int r = 0; r < 4; ++r)
+      b[r] = *(lds_ptr)(uintptr_t)((uint32_t)(q[r] - k[r]) & 0x3fffffffu) + ((q[r] ^ k[r]) >> 30 ? -100.f * LOG2E : 0.f);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[r] = *(lds_ptr)(uintptr_t)(uint32_t)(q[r] - k[r]);
   }
+  return b;
+}
+
+// Logits in units of log2 e from products.
+__device__ __forceinline__ void logits(f32x4& s, float zs, const f32x4& bias) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) s[r] = fmaf(s[r], zs, bias[r]);
 }
 
 // A mask value times log2 e: the lowest floats stay finite, so that a row of them is uniform, as

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
   const int qc = (int)(b - item * (uint32_t)a.nqc);
   const int64_t win = a.dheads.div(item);
   const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int L = a.L;
   const At at(a, win, head, (int)sizeof(T));
   const int wi = (int)(win % a.nW);
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr;                        // past the window: zeros
-    qinfo[i] = info_of(a, q, shifted) + 4 * a.off;
+    qinfo[i] = info_of(a, q, shifted) + rel_base(a, rel);
 #pragma unroll
     for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(qrows, (uint32_t)q, s, fg, a.hd);
   }
@@ -98,19 +98,17 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
         for (int s = 0; s < D::NS; ++s) kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg);
         const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
         const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
+        f32x4 bias[QB];
+#pragma unroll
+        for (int i = 0; i < QB; ++i) bias[i] = biases({qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn, shifted);
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
           S[i][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = 0; s < D::NS; ++s) S[i][kb] = mma(kf[s], qf[i][s], S[i][kb]);
         }
-        if (shifted) {
 #pragma unroll
-          for (int i = 0; i < QB; ++i) logits<true>(S[i][kb], zs, rel, {qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn);
-        } else {
-#pragma unroll
-          for (int i = 0; i < QB; ++i) logits<false>(S[i][kb], zs, rel, {qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn);
-        }
+        for (int i = 0; i < QB; ++i) logits(S[i][kb], zs, bias[i]);
         if constexpr (MASK) {
 #pragma unroll
           for (int i = 0; i < QB; ++i) {

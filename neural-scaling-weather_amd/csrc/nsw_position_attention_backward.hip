@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
   float* rel = rows + 2 * 4 * QT;
 
   const int part = (int)blockIdx.x % a.NP, head = (int)blockIdx.x / a.NP;   // a head's parts side by side
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int L = a.L, steps = (L + QT - 1) / QT;
   const int key = 16 * wave + fr;
   const bool keys = 16 * wave < L, bias = a.part != nullptr, alone = L == 1;   // alone: p is 1 whatever z, dz exactly 0
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
       row_dots(gc, oc, r + 3 * QT);
     }
     if (tid < QT) {
-      ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + 4 * a.off;
+      ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + rel_base(a, rel);
       put_stats<MASK>(st, r + QT + tid, r + 2 * QT + tid);
     }
   };
@@ -192,9 +192,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
       if (keys) {
         const T *Qs = QGs + (step & 1) * X::QG, *Gs = Qs + QT * D::STR;
         const float* r0 = rows + (step & 1) * 4 * QT;
-        f32x4 P[2], Z[2];                                          // queries 16 qb + 4 fg + r, key fr
+        f32x4 P[2], Z[2], B[2];                                    // queries 16 qb + 4 fg + r, key fr
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) P[qb] = Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int qb = 0; qb < 2; ++qb) {
+          P[qb] = Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          const int4 qi = *reinterpret_cast<const int4*>(r0 + 16 * qb + 4 * fg);
+          B[qb] = biases({qi.x, qi.y, qi.z, qi.w}, {kinfo, kinfo, kinfo, kinfo}, shifted);
+        }
 #pragma unroll
         for (int s = 0; s < D::NS; ++s) {
           const typename D::Frag kf = row_frag<T, HD>(Ks + key * D::STR, s, fg), vf = row_frag<T, HD>(Vs + key * D::STR, s, fg);
@@ -206,22 +210,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
         }
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-          const int4 qi = *reinterpret_cast<const int4*>(r0 + 16 * qb + 4 * fg);
-          const int qn[4] = {qi.x, qi.y, qi.z, qi.w};
           const f32x4 m4 = *reinterpret_cast<const f32x4*>(r0 + QT + 16 * qb + 4 * fg);
           const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg) : m4;
           const f32x4 d4 = *reinterpret_cast<const f32x4*>(r0 + 3 * QT + 16 * qb + 4 * fg);
-          if (shifted) logits<true>(P[qb], zs, rel, qn, {kinfo, kinfo, kinfo, kinfo});
-          else logits<false>(P[qb], zs, rel, qn, {kinfo, kinfo, kinfo, kinfo});
+          logits(P[qb], zs, B[qb]);
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               P[qb][r] += mask_units(mask.get(QT * step + 16 * qb + 4 * fg + r, key));
             }
           }
-          if (key >= L) P[qb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (16 * wave + 16 > L) {
+            if (key >= L) P[qb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            asm volatile("" : "+v"(P[qb]));                        // a branch of these waves, no selects of all
+          }
           weigh<MASK>(P[qb], Z[qb], m4, l4, d4);
-          if (alone) Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (alone) {
+            Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+            asm volatile("" : "+v"(Z[qb]));
+          }
         }
         const typename D::TFrag pf = pair_frag<T>(P[0], P[1]), zf = pair_frag<T>(Z[0], Z[1]);
         T* z = Zs + (step & 1) * X::ZT + key * X::ZS + 4 * fg;
@@ -284,7 +291,7 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
 
   // a head's parts side by side
   const int part = (int)blockIdx.x % a.NP, kc = (int)blockIdx.x / a.NP % a.nqc, head = (int)blockIdx.x / a.NP / a.nqc;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int L = a.L;
   const int kw = kc * 64 * KB + wave * 16 * KB;                    // the wave's first key
   const bool bias = a.part != nullptr;
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
       gc.store(Gs);
       row_dots(gc, oc, drow);
       if (tid < QT) {
-        qinfo[tid] = info_of(a, q0 + tid, shifted) + 4 * a.off;
+        qinfo[tid] = info_of(a, q0 + tid, shifted) + rel_base(a, rel);
         put_stats<MASK>(st, mrow + tid, lrow + tid);
       }
       wg_barrier();
@@ -346,7 +353,9 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
           gf[s] = row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg);
         }
         const int4 qi = *reinterpret_cast<const int4*>(qinfo + 16 * qb + 4 * fg);
-        const int qn[4] = {qi.x, qi.y, qi.z, qi.w};
+        f32x4 B[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) B[b] = biases({qi.x, qi.y, qi.z, qi.w}, {kinfo[b], kinfo[b], kinfo[b], kinfo[b]}, shifted);
         const f32x4 m4 = *reinterpret_cast<const f32x4*>(mrow + 16 * qb + 4 * fg);
         const f32x4 d4 = *reinterpret_cast<const f32x4*>(drow + 16 * qb + 4 * fg);
         const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(lrow + 16 * qb + 4 * fg) : m4;
@@ -365,16 +374,17 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
             P[qb][b] = mma(qf[s], kf[b][s], P[qb][b]);
             Z[qb][b] = mma(gf[s], vf[b][s], Z[qb][b]);
           }
-          const int k4[4] = {kinfo[b], kinfo[b], kinfo[b], kinfo[b]};
-          if (shifted) logits<true>(P[qb][b], zs, rel, qn, k4);
-          else logits<false>(P[qb][b], zs, rel, qn, k4);
+          logits(P[qb][b], zs, B[b]);
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               P[qb][b][r] += mask_units(mask.get(q0 + 16 * qb + 4 * fg + r, key));
             }
           }
-          if (kw + 16 * b + 16 > L && key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (kw + 16 * b + 16 > L) {
+            if (key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            asm volatile("" : "+v"(P[qb][b]));                     // a branch of these waves, no selects of all
+          }
           weigh<MASK>(P[qb][b], Z[qb][b], m4, l4, d4);
           if (bias) {
 #pragma unroll
@@ -425,7 +435,7 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
   const int qc = (int)(blk - item * (uint32_t)a.nqc);
   const int64_t win = a.dheads.div(item);
   const int head = (int)(item - (uint32_t)win * (uint32_t)a.heads);
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fg = lane >> 4;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int L = a.L;
   const At at(a, win, head, (int)sizeof(T));
   const int wi = (int)(win % a.nW);
@@ -445,7 +455,7 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 64 * i + fr;                        // past the window: zeros
-    qinfo[i] = info_of(a, q, shifted) + 4 * a.off;
+    qinfo[i] = info_of(a, q, shifted) + rel_base(a, rel);
     float t = 0.f;
 #pragma unroll
     for (int s = 0; s < D::NS; ++s) {
@@ -482,6 +492,9 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
       }
       const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
       const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
+      f32x4 bias[QB];
+#pragma unroll
+      for (int i = 0; i < QB; ++i) bias[i] = biases({qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn, shifted);
 #pragma unroll
       for (int i = 0; i < QB; ++i) {
         f32x4 s4 = {0.f, 0.f, 0.f, 0.f}, g4 = {0.f, 0.f, 0.f, 0.f};
@@ -490,9 +503,7 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
           s4 = mma(kf[s], qf[i][s], s4);
           g4 = mma(vf[s], gf[i][s], g4);
         }
-        const int qn[4] = {qinfo[i], qinfo[i], qinfo[i], qinfo[i]};
-        if (shifted) logits<true>(s4, zs, rel, qn, kn);
-        else logits<false>(s4, zs, rel, qn, kn);
+        logits(s4, zs, bias[i]);
         if constexpr (MASK) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) s4[r] += mask_units(mask.get(q0 + 64 * i + fr, k0 + 16 * kb + 4 * fg + r));
@@ -524,65 +535,80 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
 }
 
 // out[h, y, r] = sum over the pairs of displacement r whose query lies in share y of the
-// window, and over the parts: a lane a displacement, neighbours on neighbouring keys.
+// window, and over the parts: a lane a displacement, neighbours on neighbouring keys, eight
+// queries at a time.
 __global__ __launch_bounds__(NT) void pairs_kernel(Args a, float* __restrict__ out, int share) {
+  constexpr int U = 8;
   const int r = (int)blockIdx.x * NT + (int)threadIdx.x, h = (int)blockIdx.y, y = (int)blockIdx.z;
   const int w2 = 2 * a.W - 1, a2 = 2 * a.A - 1;
   const int dw = r % w2 - (a.W - 1), da = r / w2 % a2 - (a.A - 1), dt = r / w2 / a2 - (a.TW - 1);
   const int back = (dt * a.A + da) * a.W + dw;             // tokens between query and key
   const int64_t LL = (int64_t)a.L * a.L;
-  const float* part = a.part + (int64_t)h * a.NP * LL;
   const int i0 = y * share, i1 = i0 + share < a.L ? i0 + share : a.L;
   int w = i0 % a.W, i = i0 / a.W % a.A, t = i0 / (a.W * a.A);
-  float s = 0.f;
-  for (int q = i0; q < i1; ++q) {
-    if (r < a.R && (unsigned)(w - dw) < (unsigned)a.W && (unsigned)(i - da) < (unsigned)a.A && (unsigned)(t - dt) < (unsigned)a.TW) {
-      const float* at = part + (int64_t)q * a.L + (q - back);
-#pragma unroll 8
-      for (int p = 0; p < a.NP; ++p) s += at[p * LL];
-    }
-    if (++w == a.W) {
-      w = 0;
-      if (++i == a.A) {
-        i = 0;
-        ++t;
+  float s[U] = {};
+  for (int q0 = i0; q0 < i1; q0 += U) {
+    uint32_t at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = q0 + u;
+      const bool there = q < i1 && r < a.R && (unsigned)(w - dw) < (unsigned)a.W && (unsigned)(i - da) < (unsigned)a.A &&
+                         (unsigned)(t - dt) < (unsigned)a.TW;
+      at[u] = there ? (uint32_t)(q * a.L + q - back) * 4u : NOWHERE;
+      if (++w == a.W) {
+        w = 0;
+        if (++i == a.A) {
+          i = 0;
+          ++t;
+        }
       }
     }
+    for (int p = 0; p < a.NP; ++p) {
+      const Plane x(a.part + ((int64_t)h * a.NP + p) * LL, a.L);
+#pragma unroll
+      for (int u = 0; u < U; ++u) s[u] += __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(x.r, at[u], 0, 0));
+    }
   }
-  if (r < a.R) out[((int64_t)h * gridDim.z + y) * a.R + r] = s;
+  if (r < a.R) out[((int64_t)h * gridDim.z + y) * a.R + r] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
-// dtable[b, h] = sum over the displacements of bucket b, ascending, of their shares' sums: a lane a bucket.
+// dtable[b, h] = sum over the displacements of bucket b of their shares' sums: a workgroup 64
+// buckets of a head, a wave a sixteenth of the displacements, ascending, the sixteenths in order.
+constexpr int TT = 1024;
 template <typename T>
-__global__ __launch_bounds__(NT) void table_kernel(const float* __restrict__ sums, const int* __restrict__ buckets,
+__global__ __launch_bounds__(TT) void table_kernel(const float* __restrict__ sums, const int* __restrict__ buckets,
                                                    T* __restrict__ dtable, int R, int shares, int nb, int heads) {
-  __shared__ __attribute__((aligned(16))) float v[1024];
-  __shared__ __attribute__((aligned(16))) int at[1024];
-  const int b = (int)blockIdx.x * NT + (int)threadIdx.x, h = (int)blockIdx.y;
-  float t = 0.f;
-  for (int r0 = 0; r0 < R && shares; r0 += 1024) {
-    __syncthreads();
-    for (int i = (int)threadIdx.x; i < 1024; i += NT) {
-      const int r = r0 + i;
-      float s = 0.f;
-      if (r < R)
-#pragma unroll 4
-        for (int y = 0; y < shares; ++y) s += sums[((int64_t)h * shares + y) * R + r];
-      v[i] = s;
-      at[i] = r < R ? buckets[r] : -1;
-    }
-    __syncthreads();
-    const int n = R - r0 < 1024 ? R - r0 : 1024;
-    for (int i = 0; i < n; i += 4) {
-      const int4 k = *reinterpret_cast<const int4*>(at + i);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(v + i);
-      if (k.x == b) t += x[0];
-      if (k.y == b) t += x[1];
-      if (k.z == b) t += x[2];
-      if (k.w == b) t += x[3];
-    }
+  extern __shared__ __attribute__((aligned(16))) float v[];        // [Rp], then their buckets [Rp], Rp a multiple of 64
+  __shared__ float red[TT / 64][64];
+  const int Rp = (R + 63) / 64 * 64;
+  int* at = (int*)(v + Rp);
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, b = (int)blockIdx.x * 64 + lane, h = (int)blockIdx.y;
+  for (int r = (int)threadIdx.x; r < Rp; r += TT) {
+    float s = 0.f;
+    if (r < R)
+#pragma unroll 8
+      for (int y = 0; y < shares; ++y) s += sums[((int64_t)h * shares + y) * R + r];
+    v[r] = s;
+    at[r] = r < R ? buckets[r] : -1;
   }
-  if (b < nb) dtable[(int64_t)b * heads + h] = from_f32<T>(t);
+  __syncthreads();
+  float t[4] = {};
+  for (int r = wave * (Rp / 16); r < (wave + 1) * (Rp / 16); r += 4) {
+    const int4 k = *reinterpret_cast<const int4*>(at + r);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(v + r);
+    t[0] += k.x == b ? x[0] : 0.f;
+    t[1] += k.y == b ? x[1] : 0.f;
+    t[2] += k.z == b ? x[2] : 0.f;
+    t[3] += k.w == b ? x[3] : 0.f;
+  }
+  red[wave][lane] = (t[0] + t[1]) + (t[2] + t[3]);
+  __syncthreads();
+  if (wave == 0 && b < nb) {
+    float s = red[0][lane];
+#pragma unroll
+    for (int i = 1; i < TT / 64; ++i) s += red[i][lane];
+    dtable[(int64_t)b * heads + h] = from_f32<T>(s);
+  }
 }
 
 // Waves of windows_kernel for windows of L tokens; 0: longer than it takes (twelve waves do
@@ -609,11 +635,12 @@ void set_parts(Args& a, int waves, int keys) {
   a.NP = (int)((Bw + each - 1) / each);
 }
 
-// Shares of a window's queries in pairs_kernel: about 512 workgroups in all.
+// Queries of a share of pairs_kernel: a multiple of eight, about 2048 workgroups in all and at most
+// 32 shares.
 int share_of(const Args& a, int* shares) {
   const int64_t others = (int64_t)((a.R + NT - 1) / NT) * a.heads;
-  const int want = (int)std::max<int64_t>(1, std::min<int64_t>({16, a.L, 512 / others}));
-  const int share = (a.L + want - 1) / want;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(32, 2048 / others));
+  const int share = (int)(((a.L + want - 1) / want + 7) / 8 * 8);
   *shares = (a.L + share - 1) / share;
   return share;
 }
@@ -706,8 +733,9 @@ int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream
     if (a.Bw > 0)
       hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)((a.R + NT - 1) / NT), (unsigned)a.heads, (unsigned)shares), dim3(NT), 0, st, a,
                          sums, share);
-    hipLaunchKernelGGL((table_kernel<T>), dim3((unsigned)((a.nb + NT - 1) / NT), (unsigned)a.heads), dim3(NT), 0, st, sums,
-                       a.buckets, (T*)dtable, a.R, a.Bw > 0 ? shares : 0, a.nb, a.heads);
+    const size_t lds = (size_t)((a.R + 63) / 64 * 64) * 8;
+    hipLaunchKernelGGL((table_kernel<T>), dim3((unsigned)((a.nb + 63) / 64), (unsigned)a.heads), dim3(TT), lds, st, sums, a.buckets,
+                       (T*)dtable, a.R, a.Bw > 0 ? shares : 0, a.nb, a.heads);
     return check_launch(what);
   });
 }

@@ -276,23 +276,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
 // ---------------------------------------------------------- longer windows ---
 
 template <typename T, int HD>
-constexpr size_t keys_lds() { return 2 * QT * Dim<T, HD>::STR * sizeof(T) + 4 * QT * sizeof(float); }
+constexpr size_t keys_lds() { return 2 * (2 * QT * Dim<T, HD>::STR * sizeof(T) + 4 * QT * sizeof(float)); }
 
 template <typename T, int HD, int KB, bool MASK>
-__global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
+__global__ __launch_bounds__(NT, 2) void keys_kernel(Args a) {
   typedef Dim<T, HD> D;
-  constexpr int ND = D::ND;
+  constexpr int ND = D::ND, QG = 2 * QT * D::STR;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* Qs = (T*)smem;
-  T* Gs = Qs + QT * D::STR;
-  int* qinfo = (int*)(Gs + QT * D::STR);
-  float *mrow = (float*)qinfo + QT, *lrow = mrow + QT, *drow = lrow + QT;
-  float* rel = drow + QT;
+  T* QGs = (T*)smem;                                               // [2][q rows, do rows]
+  float* rows = (float*)(QGs + 2 * QG);                            // [2][infos, m, l, D]
+  float* rel = rows + 2 * 4 * QT;
 
   // a head's parts side by side
   const int part = (int)blockIdx.x % a.NP, kc = (int)blockIdx.x / a.NP % a.nqc, head = (int)blockIdx.x / a.NP / a.nqc;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
-  const int L = a.L;
+  const int L = a.L, steps = (L + QT - 1) / QT;
   const int kw = kc * 64 * KB + wave * 16 * KB;                    // the wave's first key
   const bool bias = a.part != nullptr;
   const float zs = a.scale * LOG2E;
@@ -313,6 +311,17 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
       oc.load(at.out(a.out, q0, L - q0), a.hd);
       st = load_stats(a, win, head, q0, tid < QT ? L - q0 : 0, tid);
     };
+    auto store_tile = [&](int step) {
+      T* q = QGs + (step & 1) * QG;
+      float* r = rows + (step & 1) * 4 * QT;
+      qc.store(q);
+      gc.store(q + QT * D::STR);
+      row_dots(gc, oc, r + 3 * QT);
+      if (tid < QT) {
+        ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + rel_base(a, rel);
+        put_stats<MASK>(st, r + QT + tid, r + 2 * QT + tid);
+      }
+    };
     load_tile(0);
     const Rows krows = at.qkv(a.qkv, 1, 0, L), vrows = at.qkv(a.qkv, 2, 0, L);
     typename D::Frag kf[KB][D::NS], vf[KB][D::NS];
@@ -330,19 +339,16 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) dk[b][d] = dv[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    wg_barrier();                                                  // the window before is done with the LDS
+    store_tile(0);
+    wg_barrier();
 
-    for (int q0 = 0; q0 < L; q0 += QT) {
-      wg_barrier();                                                // the tile before is read
-      qc.store(Qs);
-      gc.store(Gs);
-      row_dots(gc, oc, drow);
-      if (tid < QT) {
-        qinfo[tid] = info_of(a, q0 + tid, shifted) + rel_base(a, rel);
-        put_stats<MASK>(st, mrow + tid, lrow + tid);
-      }
-      wg_barrier();
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      const int q0 = QT * step;
       load_tile(q0 + QT);
-
+      const T *Qs = QGs + (step & 1) * QG, *Gs = Qs + QT * D::STR;
+      const float* r0 = rows + (step & 1) * 4 * QT;
       f32x4 P[2][KB], Z[2][KB];                                    // queries 16 qb + 4 fg + r, key fr of block b
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
@@ -352,34 +358,40 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
           qf[s] = row_frag<T, HD>(Qs + (16 * qb + fr) * D::STR, s, fg);
           gf[s] = row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg);
         }
-        const int4 qi = *reinterpret_cast<const int4*>(qinfo + 16 * qb + 4 * fg);
-        f32x4 B[KB];
+        const int4 qi = *reinterpret_cast<const int4*>(r0 + 16 * qb + 4 * fg);
+        f32x4 B[KB], old[KB], M[KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) B[b] = biases({qi.x, qi.y, qi.z, qi.w}, {kinfo[b], kinfo[b], kinfo[b], kinfo[b]}, shifted);
-        const f32x4 m4 = *reinterpret_cast<const f32x4*>(mrow + 16 * qb + 4 * fg);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(drow + 16 * qb + 4 * fg);
-        const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(lrow + 16 * qb + 4 * fg) : m4;
+        for (int b = 0; b < KB; ++b) {
+          B[b] = biases({qi.x, qi.y, qi.z, qi.w}, {kinfo[b], kinfo[b], kinfo[b], kinfo[b]}, shifted);
+          if constexpr (MASK) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) M[b][r] = mask.get(q0 + 16 * qb + 4 * fg + r, kw + 16 * b + fr);
+          }
+          old[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (bias && win != part) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) old[b][r] = sums.get(q0 + 16 * qb + 4 * fg + r, kw + 16 * b + fr);
+          }
+        }
+        const f32x4 m4 = *reinterpret_cast<const f32x4*>(r0 + QT + 16 * qb + 4 * fg);
+        const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg) : m4;
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(r0 + 3 * QT + 16 * qb + 4 * fg);
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           P[qb][b] = Z[qb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (kw + 16 * b >= L) continue;
-          const int key = kw + 16 * b + fr;
-          f32x4 old = {0.f, 0.f, 0.f, 0.f};
-          if (bias && win != part) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) old[r] = sums.get(q0 + 16 * qb + 4 * fg + r, key);
-          }
 #pragma unroll
           for (int s = 0; s < D::NS; ++s) {
             P[qb][b] = mma(qf[s], kf[b][s], P[qb][b]);
             Z[qb][b] = mma(gf[s], vf[b][s], Z[qb][b]);
           }
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          const int key = kw + 16 * b + fr;
           logits(P[qb][b], zs, B[b]);
           if constexpr (MASK) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              P[qb][b][r] += mask_units(mask.get(q0 + 16 * qb + 4 * fg + r, key));
-            }
+            for (int r = 0; r < 4; ++r) P[qb][b][r] += mask_units(M[b][r]);
           }
           if (kw + 16 * b + 16 > L) {
             if (key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -388,7 +400,7 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
           weigh<MASK>(P[qb][b], Z[qb][b], m4, l4, d4);
           if (bias) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sums.put(q0 + 16 * qb + 4 * fg + r, key, old[r] + Z[qb][b][r]);
+            for (int r = 0; r < 4; ++r) sums.put(q0 + 16 * qb + 4 * fg + r, key, old[b][r] + Z[qb][b][r]);
           }
         }
       }
@@ -407,6 +419,8 @@ __global__ __launch_bounds__(NT, 1) void keys_kernel(Args a) {
           dk[b][d] = mma(qt, zf[b], dk[b][d]);
         }
       }
+      if (step + 1 < steps) store_tile(step + 1);
+      wg_barrier();                                                // the next tile is there
     }
     const Rows dkr = at.qkv(a.dqkv, 1, 0, L), dvr = at.qkv(a.dqkv, 2, 0, L);
 #pragma unroll
@@ -621,7 +635,7 @@ int waves_of(int L) {
 }
 
 // 16-key blocks of a wave of keys_kernel.
-template <typename T, int HD> constexpr int KEY_BLOCKS = HD == 128 ? (sizeof(T) == 4 ? 1 : 2) : HD == 64 && sizeof(T) == 4 ? 2 : 3;
+template <typename T, int HD> constexpr int KEY_BLOCKS = HD * (int)sizeof(T) >= 256 ? 1 : 2;
 
 // Workgroups that share a head's windows: as many as run at once in all (windows_kernel: four
 // waves to a SIMD or one workgroup to a compute unit; keys_kernel: two workgroups), each with the

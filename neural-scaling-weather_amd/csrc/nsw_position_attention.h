@@ -322,6 +322,8 @@ struct Plane {
   __device__ __forceinline__ Plane(const float* p, int L_) : L(L_) { r = Rows(p, (uint32_t)L_ * 4u, L_, L_ * 4).r; }
   __device__ __forceinline__ uint32_t at(int q, int k) const { return k < L ? (uint32_t)(q * L + k) * 4u : NOWHERE; }
   __device__ __forceinline__ float get(int q, int k) const { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at(q, k), 0, 0)); }
+  // keys k .. k + 3 of query q; what lies past the window is of another row or zero
+  __device__ __forceinline__ f32x4 get4(int q, int k) const { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at(q, k), 0, 0)); }
   __device__ __forceinline__ void put(int q, int k, float v) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, at(q, k), 0, 0); }
 };
 

@@ -6,14 +6,17 @@
 // difference of two codes (one subtraction; the bias is then one LDS read).  A row whose
 // mask leaves nothing (every z_ij = -inf) gives zeros.
 //
-// A workgroup takes QB 64-query blocks of one (window, head): it steps over 64-key tiles in
-// LDS with the running maximum m and sum of each row, so any length goes.  S^T = K Q^T puts a
-// query on a lane, whose probabilities are then the right operand of O^T = V^T P^T as they
-// lie.  Logits in units of log2 e (the factor is in the scale and in the bias's LDS copy), so
+// Windows of up to 192 tokens (fewer with 256-byte rows) go through whole_kernel, whose waves
+// hold a row's logits with all keys; longer ones through forward_kernel, which steps over key
+// tiles with the running maximum m and sum of each row, so any length goes (180 x 360 x 1024 of
+// 9 x 18 windows, bf16: 142 us against 210, of them 105 for the bytes at a copy's rate).
+// S^T = K Q^T puts a query on a lane, whose probabilities are then the right operand of
+// O^T = V^T P^T as they lie.  Logits in units of log2 e (the factor is in the scale and in the bias's LDS copy), so
 // that a probability is one subtraction and exp2.  fp32 statistics and sums; bf16: probabilities
 // (at most 1) are rounded to bf16 for the product with v, and their sum is of the rounded
 // ones, by a product with ones on the matrix units.  stats keeps m and log2 of the sum apart,
 // since their sum would lose the second where |m| is large.
+#include <algorithm>
 #include <cmath>
 
 #include "nsw_position_attention.h"
@@ -26,8 +29,164 @@ namespace posattn {
 
 namespace {
 
-template <typename T, int HD, int QB, bool MASK>
-__global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
+// ------------------------------------------------- windows in a workgroup ---
+
+template <typename T, int HD, int NKB> struct Whole {
+  static constexpr int STEPS = (NKB + 1) / 2, KEYS = 32 * STEPS;   // 32-key steps
+  static constexpr size_t KV = (size_t)2 * KEYS * Dim<T, HD>::STR * sizeof(T);
+  static constexpr int BUFS = 2 * KV <= (128 << 10) ? 2 : 1;
+  static constexpr size_t LDS = BUFS * KV + 2 * KEYS * sizeof(int);
+};
+
+// Windows of up to 16 NKB tokens of one head in turn.  A wave owns 16 queries and holds their
+// logits with all keys, so that a row's maximum is known before its probabilities are formed,
+// and, as the pairs are the same in every window, their biases too.  bf16 without a mask: the
+// products start from the biases divided by the scale (which is positive), and a probability is
+// one multiply-add and exp2: off by an ulp of the row's maximum, far below the rounding of p to
+// bf16.  Otherwise the biases are added as the backward adds them.  k and v lie in LDS, loaded
+// while the window before is computed, in a second buffer where it fits (one barrier a window).
+// Four waves with three blocks of queries each, biases looked up: 185 us where this takes 142.
+template <typename T, int HD, int NKB, bool MASK>
+__global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) {
+  typedef Dim<T, HD> D;
+  typedef Whole<T, HD, NKB> X;
+  constexpr int N = 64 * NKB;
+  constexpr bool START = !MASK && sizeof(T) == 2;                  // the products start from the biases
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* KVs = (T*)smem;                                               // [BUFS][k rows, v rows]
+  int* kinfo = (int*)(smem + X::BUFS * X::KV);                     // [2][KEYS]: without and with the shift's classes
+  float* rel = (float*)(kinfo + 2 * X::KEYS);
+
+  const int part = (int)blockIdx.x % a.NP, head = (int)blockIdx.x / a.NP;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
+  const int L = a.L, query = 16 * wave + fr;
+  const bool queries = 16 * wave < L;
+  const float zs = a.scale * LOG2E, shift = START ? -100.f / a.scale : -100.f * LOG2E;
+
+  TileCopy<T, HD, X::KEYS, N> kc, vc;
+  typename D::Frag qn[D::NS];
+  auto load_window = [&](int64_t win) {
+    const int n = win < a.Bw ? L : 0;
+    const At at(a, win, head, (int)sizeof(T));
+    kc.load(at.qkv(a.qkv, 1, 0, n), a.hd);
+    vc.load(at.qkv(a.qkv, 2, 0, n), a.hd);
+    const Rows q = at.qkv(a.qkv, 0, 0, n);
+#pragma unroll
+    for (int s = 0; s < D::NS; ++s) qn[s] = row_frag<T, HD>(q, (uint32_t)query, s, fg, a.hd);
+  };
+  load_window(part);
+  load_rel<T>(a, head, rel);
+  for (int i = tid; i < X::KEYS; i += N) {
+    kinfo[i] = info_of(a, i, false);
+    kinfo[X::KEYS + i] = info_of(a, i, true);
+  }
+  constexpr bool ONES = sizeof(T) == 2;
+  typename D::TFrag ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
+  wg_barrier();
+  // keys past the window: no weight
+  f32x4 bias[NKB];
+#pragma unroll
+  for (int kb = 0; kb < NKB; ++kb) {
+    const int qi = info_of(a, query, false) + rel_base(a, rel);
+    const int4 k = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
+    bias[kb] = biases({qi, qi, qi, qi}, {k.x, k.y, k.z, k.w}, false);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bias[kb][r] = 16 * kb + 4 * fg + r < L ? (START ? bias[kb][r] / zs : bias[kb][r]) : -INFINITY;
+  }
+
+  int turn = 0;
+  for (int64_t win = part; win < a.Bw; win += a.NP, turn ^= 1) {
+    const int wi = (int)(win % a.nW);
+    const bool shifted = !MASK && wi >= a.band0;
+    const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
+    const At at(a, win, head, (int)sizeof(T));
+    T* Ks = KVs + (X::BUFS == 2 ? turn : 0) * (int)(X::KV / sizeof(T));
+    T* Vs = Ks + X::KEYS * D::STR;
+    if constexpr (X::BUFS == 1) wg_barrier();                      // the window before is read
+    kc.store(Ks);
+    vc.store(Vs);
+    typename D::Frag q[D::NS];
+#pragma unroll
+    for (int s = 0; s < D::NS; ++s) q[s] = qn[s];
+    wg_barrier();                                                  // two buffers: the window two before is read, too
+    load_window(win + a.NP);
+    if (!queries) continue;
+    f32x4 S[NKB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      S[kb] = START ? bias[kb] : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < D::NS; ++s) S[kb] = mma(row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg), q[s], S[kb]);
+    }
+    if constexpr (!START)
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[kb][r] = fmaf(S[kb][r], zs, bias[kb][r]);
+    if constexpr (MASK) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        const f32x4 m4 = mask.get4(query, 16 * kb + 4 * fg);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[kb][r] += mask_units(m4[r]);
+      }
+    } else if (shifted) {
+      const int qc = info_of(a, query, true);
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        const int4 k = *reinterpret_cast<const int4*>(kinfo + X::KEYS + 16 * kb + 4 * fg);
+        const int kn[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[kb][r] += (qc ^ kn[r]) >> 30 ? shift : 0.f;
+      }
+    }
+    float mx = S[0][0];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[kb][r]);
+    mx = rows4_max(mx) * (START ? zs : 1.f);
+    const float to = mx == -INFINITY ? 0.f : -mx;
+    float l = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        S[kb][r] = __builtin_amdgcn_exp2f(START ? fmaf(S[kb][r], zs, to) : S[kb][r] + to);
+        if constexpr (!ONES) l += S[kb][r];
+      }
+    f32x4 O[D::ND], Z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < D::ND; ++d) O[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < X::STEPS; ++ks) {
+      const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+      const typename D::TFrag pf = pair_frag<T>(S[2 * ks], 2 * ks + 1 < NKB ? S[2 * ks + 1 < NKB ? 2 * ks + 1 : 0] : none);
+#pragma unroll
+      for (int d = 0; d < D::ND; ++d) O[d] = mma(col_frag<T, D::STR>(Vs + 32 * ks * D::STR, 16 * d, fr, fg), pf, O[d]);
+      if constexpr (ONES) Z = mma(ones, pf, Z);
+    }
+    const float t = ONES ? Z[0] : rows4_sum(l);
+    const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;      // an empty row: zeros; NaN stays
+    const Rows orows = at.out(a.o, 0, L);
+#pragma unroll
+    for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orows, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], inv);
+    if (query < L && fg == 0)
+      *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + query) * 2) = f32x2{mx, __builtin_amdgcn_logf(t)};
+  }
+}
+
+// ---------------------------------------------------------- longer windows ---
+
+constexpr int WAVES = 8;                                           // of forward_kernel, 16 queries each
+
+// A workgroup takes 128 queries of a (window, head) over 64-key tiles, the next tile in
+// registers meanwhile, two workgroups a compute unit (1999 tokens, 8 heads of 64, bf16: 45 us;
+// 64 queries in four waves 52, four waves of 32 queries 78).
+template <typename T, int HD, bool MASK>
+__global__ __launch_bounds__(64 * WAVES, 2) void forward_kernel(Args a) {
   typedef Dim<T, HD> D;
   constexpr int KT = 64;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -47,21 +206,16 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
   const int wi = (int)(win % a.nW);
   const bool shifted = !MASK && wi >= a.band0;
   const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
-  const int q0 = qc * 64 * QB + wave * 16;                 // block i of the wave: q0 + 64 i
+  const int query = (qc * WAVES + wave) * 16 + fr;         // past the window: zeros
 
-  TileCopy<T, HD, KT> kc, vc;
+  TileCopy<T, HD, KT, 64 * WAVES> kc, vc;
   kc.load(at.qkv(a.qkv, 1, 0, L), a.hd);
   vc.load(at.qkv(a.qkv, 2, 0, L), a.hd);
   const Rows qrows = at.qkv(a.qkv, 0, 0, L);
-  typename D::Frag qf[QB][D::NS];
-  int qinfo[QB];
+  typename D::Frag q[D::NS];
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 64 * i + fr;                        // past the window: zeros
-    qinfo[i] = info_of(a, q, shifted) + rel_base(a, rel);
-#pragma unroll
-    for (int s = 0; s < D::NS; ++s) qf[i][s] = row_frag<T, HD>(qrows, (uint32_t)q, s, fg, a.hd);
-  }
+  for (int s = 0; s < D::NS; ++s) q[s] = row_frag<T, HD>(qrows, (uint32_t)query, s, fg, a.hd);
+  const int qinfo = info_of(a, query, shifted) + rel_base(a, rel);
   load_rel<T>(a, head, rel);
 
   const float zs = a.scale * LOG2E;
@@ -69,16 +223,10 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
   typename D::TFrag ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
-  f32x4 O[QB][D::ND], Z[QB];                               // Z: the rows' sums (ONES)
-  float m[QB], l[QB];
+  f32x4 O[D::ND], Z = {0.f, 0.f, 0.f, 0.f};                // Z: the rows' sums (ONES)
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-    Z[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < D::ND; ++d) O[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < D::ND; ++d) O[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   for (int k0 = 0; k0 < L; k0 += KT) {
     if (k0) wg_barrier();                                  // the tile before is read
@@ -89,124 +237,119 @@ __global__ __launch_bounds__(NT, 2) void forward_kernel(Args a) {
     const int left = L - k0;                               // keys from k0 on
     kc.load(at.qkv(a.qkv, 1, k0 + KT, left - KT), a.hd);
     vc.load(at.qkv(a.qkv, 2, k0 + KT, left - KT), a.hd);
-    f32x4 S[QB][4];
+    // whole tiles without a shift run without branches between the lanes' loads and products
+    auto tile = [&](auto shift, auto tail) {
+      f32x4 S[4];
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      if (16 * kb < left) {
-        typename D::Frag kf[D::NS];
+      for (int kb = 0; kb < 4; ++kb) {
+        if (!decltype(tail)::value || 16 * kb < left) {
+          const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
+          const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
+          const f32x4 bias = biases({qinfo, qinfo, qinfo, qinfo}, kn, decltype(shift)::value);
+          S[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < D::NS; ++s) kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg);
-        const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
-        const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
-        f32x4 bias[QB];
+          for (int s = 0; s < D::NS; ++s) S[kb] = mma(row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg), q[s], S[kb]);
+          logits(S[kb], zs, bias);
+          if constexpr (MASK) {
+            const f32x4 m4 = mask.get4(query, k0 + 16 * kb + 4 * fg);
 #pragma unroll
-        for (int i = 0; i < QB; ++i) bias[i] = biases({qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn, shifted);
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-          S[i][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < D::NS; ++s) S[i][kb] = mma(kf[s], qf[i][s], S[i][kb]);
-        }
-#pragma unroll
-        for (int i = 0; i < QB; ++i) logits(S[i][kb], zs, bias[i]);
-        if constexpr (MASK) {
-#pragma unroll
-          for (int i = 0; i < QB; ++i) {
-            const int q = q0 + 64 * i + fr;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              S[i][kb][r] += mask_units(mask.get(q, k0 + 16 * kb + 4 * fg + r));
-            }
+            for (int r = 0; r < 4; ++r) S[kb][r] += mask_units(m4[r]);
           }
-        }
-        if (16 * kb + 16 > left) {
-#pragma unroll
-          for (int i = 0; i < QB; ++i)
+          if (decltype(tail)::value && 16 * kb + 16 > left) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (16 * kb + 4 * fg + r >= left) S[i][kb][r] = -INFINITY;
+              if (16 * kb + 4 * fg + r >= left) S[kb][r] = -INFINITY;
+          }
+        } else {
+          S[kb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < QB; ++i) S[i][kb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       }
-    }
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-      float mx = S[i][0][0];
+      float mx = S[0][0];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[i][kb][r]);
-      mx = fmaxf(m[i], rows4_max(mx));
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[kb][r]);
+      mx = fmaxf(m, rows4_max(mx));
       const float to = mx == -INFINITY ? 0.f : mx;
-      const float f = __builtin_amdgcn_exp2f(m[i] - to);
-      m[i] = mx;
+      const float f = __builtin_amdgcn_exp2f(m - to);
+      m = mx;
       float t = 0.f;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(S[i][kb][r] - to);
-          S[i][kb][r] = p;
-          if constexpr (!ONES) t += p;
+          S[kb][r] = __builtin_amdgcn_exp2f(S[kb][r] - to);
+          if constexpr (!ONES) t += S[kb][r];
         }
-      l[i] = fmaf(l[i], f, t);
-      Z[i] *= f;
+      l = fmaf(l, f, t);
+      Z *= f;
 #pragma unroll
-      for (int d = 0; d < D::ND; ++d) O[i][d] *= f;
-    }
+      for (int d = 0; d < D::ND; ++d) O[d] *= f;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-      if (32 * ks < left) {
-        typename D::TFrag vf[D::ND];
+      for (int ks = 0; ks < 2; ++ks)
+        if (!decltype(tail)::value || 32 * ks < left) {
+          const typename D::TFrag pf = pair_frag<T>(S[2 * ks], S[2 * ks + 1]);
 #pragma unroll
-        for (int d = 0; d < D::ND; ++d) vf[d] = col_frag<T, D::STR>(Vs + 32 * ks * D::STR, 16 * d, fr, fg);
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-          const typename D::TFrag pf = pair_frag<T>(S[i][2 * ks], S[i][2 * ks + 1]);
-#pragma unroll
-          for (int d = 0; d < D::ND; ++d) O[i][d] = mma(vf[d], pf, O[i][d]);
-          if constexpr (ONES) Z[i] = mma(ones, pf, Z[i]);
+          for (int d = 0; d < D::ND; ++d) O[d] = mma(col_frag<T, D::STR>(Vs + 32 * ks * D::STR, 16 * d, fr, fg), pf, O[d]);
+          if constexpr (ONES) Z = mma(ones, pf, Z);
         }
-      }
+    };
+    if (shifted) tile(std::true_type{}, std::true_type{});
+    else if (left < KT) tile(std::false_type{}, std::true_type{});
+    else tile(std::false_type{}, std::false_type{});
   }
   const Rows orows = at.out(a.o, 0, L);
+  const float t = ONES ? Z[0] : rows4_sum(l);
+  const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;        // an empty row: zeros; NaN stays
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 64 * i + fr;
-    const float t = ONES ? Z[i][0] : rows4_sum(l[i]);
-    const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;    // an empty row: zeros; NaN stays
-#pragma unroll
-    for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orows, (uint32_t)q, 16 * d + 4 * fg, a.hd, O[i][d], inv);
-    if (q < L) {
-      if (fg == 0) *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + q) * 2) = f32x2{m[i], __builtin_amdgcn_logf(t)};
-    }
-  }
+  for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orows, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], inv);
+  if (query < L && fg == 0)
+    *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + query) * 2) = f32x2{m, __builtin_amdgcn_logf(t)};
 }
 
-template <typename T, int HD, int QB>
-int launch_qb(Args a, hipStream_t st) {
+template <typename T, int HD>
+int launch_long(Args a, hipStream_t st) {
   typedef Dim<T, HD> D;
-  a.nqc = (a.L + 64 * QB - 1) / (64 * QB);
+  a.nqc = (a.L + 16 * WAVES - 1) / (16 * WAVES);
   a.dnqc = FastDiv::make((uint32_t)a.nqc);
   const int64_t grid = a.Bw * a.heads * a.nqc;
   if (grid >= (1LL << 31)) return set_error(NSW_ERR_INVALID, "nsw_position_attention: too large");
   const size_t lds = (size_t)2 * 64 * D::STR * sizeof(T) + 64 * sizeof(int) + (size_t)a.R * sizeof(float);
-  if (a.mask != nullptr) hipLaunchKernelGGL((forward_kernel<T, HD, QB, true>), dim3((unsigned)grid), dim3(NT), lds, st, a);
-  else hipLaunchKernelGGL((forward_kernel<T, HD, QB, false>), dim3((unsigned)grid), dim3(NT), lds, st, a);
+  if (a.mask != nullptr) hipLaunchKernelGGL((forward_kernel<T, HD, true>), dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
+  else hipLaunchKernelGGL((forward_kernel<T, HD, false>), dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
   return check_launch("nsw_position_attention");
 }
 
-// Query blocks of a wave: as many as the window has, at most 3 (2 where registers end).
+template <typename T, int HD, int NKB>
+int launch_whole(Args a, hipStream_t st) {
+  typedef Whole<T, HD, NKB> X;
+  const int64_t all = 256 * (16 / NKB);                            // as many as run at once
+  const int64_t want = std::max<int64_t>(1, all / a.heads), each = (a.Bw + want - 1) / want;
+  a.NP = (int)((a.Bw + each - 1) / each);
+  const dim3 grid((unsigned)(a.NP * a.heads)), block(64 * NKB);
+  const size_t lds = X::LDS + (size_t)a.R * sizeof(float);
+  if (a.mask != nullptr) hipLaunchKernelGGL((whole_kernel<T, HD, NKB, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((whole_kernel<T, HD, NKB, false>), grid, block, lds, st, a);
+  return check_launch("nsw_position_attention");
+}
+
+// Longest window of whole_kernel, in blocks of 64 tokens: what the LDS holds of k and v and the
+// registers of twelve waves of a row.
+template <typename T, int HD> constexpr int MOST_WHOLE = HD * (int)sizeof(T) >= 512 ? 1 : HD * (int)sizeof(T) >= 256 ? 2 : 3;
+
 template <typename T, int HD>
 int launch_hd(const Args& a, hipStream_t st) {
-  constexpr int MOST = HD == 128 ? (sizeof(T) == 4 ? 1 : 2) : HD == 64 && sizeof(T) == 4 ? 2 : 3;
-  if (a.L <= 64 || MOST == 1) return launch_qb<T, HD, 1>(a, st);
-  if constexpr (MOST >= 2)
-    if (a.L <= 128 || MOST == 2) return launch_qb<T, HD, 2>(a, st);
-  if constexpr (MOST >= 3) return launch_qb<T, HD, 3>(a, st);
-  return NSW_OK;
+  // whole_kernel may divide the biases by the scale: that neither overflows nor loses them
+  if (sizeof(T) == 4 || a.mask != nullptr || (a.scale >= 1e-6f && a.scale <= 1e6f)) {
+    if (a.L <= 64) return launch_whole<T, HD, 4>(a, st);
+    if constexpr (MOST_WHOLE<T, HD> >= 2)
+      if (a.L <= 128) return launch_whole<T, HD, 8>(a, st);
+    if constexpr (MOST_WHOLE<T, HD> >= 3) {
+      if (a.L <= 176) return launch_whole<T, HD, 11>(a, st);
+      if (a.L <= 192) return launch_whole<T, HD, 12>(a, st);
+    }
+  }
+  return launch_long<T, HD>(a, st);
 }
 
 template <typename T>

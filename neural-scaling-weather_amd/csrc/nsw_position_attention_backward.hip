@@ -433,11 +433,13 @@ __global__ __launch_bounds__(NT, 2) void keys_kernel(Args a) {
   }
 }
 
-// dq of QB 64-query blocks of a (window, head), over 64-key tiles, as forward_kernel.
-template <typename T, int HD, int QB, bool MASK>
-__global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
+constexpr int WQ = 8, QKT = 64;                                    // of queries_kernel: waves of 16 queries, keys of a tile
+
+// dq of 128 queries of a (window, head), over key tiles, as the forward pass.
+template <typename T, int HD, bool MASK>
+__global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void queries_kernel(Args a) {
   typedef Dim<T, HD> D;
-  constexpr int KT = 32;
+  constexpr int KT = QKT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* Ks = (T*)smem;
   T* Vs = Ks + KT * D::STR;
@@ -455,110 +457,101 @@ __global__ __launch_bounds__(NT, 2) void queries_kernel(Args a) {
   const int wi = (int)(win % a.nW);
   const bool shifted = !MASK && wi >= a.band0;
   const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
-  const int q0 = qc * 64 * QB + wave * 16;
+  const int query = (qc * WQ + wave) * 16 + fr;            // past the window: zeros
 
-  TileCopy<T, HD, KT> kc, vc;
+  TileCopy<T, HD, KT, 64 * WQ> kc, vc;
   kc.load(at.qkv(a.qkv, 1, 0, L), a.hd);
   vc.load(at.qkv(a.qkv, 2, 0, L), a.hd);
   const Rows qrows = at.qkv(a.qkv, 0, 0, L), grows = at.out(a.dout, 0, L), orows = at.out(a.out, 0, L);
-  typename D::Frag qf[QB][D::NS], gf[QB][D::NS];
-  int qinfo[QB];
-  float m[QB], l2[QB] = {}, dots[QB];
+  typename D::Frag q[D::NS], g[D::NS];
+  const int qinfo = info_of(a, query, shifted) + rel_base(a, rel);
   const float zs = a.scale * LOG2E;
-  f32x4 O[QB][D::ND];
+  float m, l = 0.f, dot = 0.f;
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 64 * i + fr;                        // past the window: zeros
-    qinfo[i] = info_of(a, q, shifted) + rel_base(a, rel);
-    float t = 0.f;
+  for (int s = 0; s < D::NS; ++s) {
+    q[s] = row_frag<T, HD>(qrows, (uint32_t)query, s, fg, a.hd);
+    g[s] = row_frag<T, HD>(grows, (uint32_t)query, s, fg, a.hd);
+    const typename D::Frag o = row_frag<T, HD>(orows, (uint32_t)query, s, fg, a.hd);
 #pragma unroll
-    for (int s = 0; s < D::NS; ++s) {
-      qf[i][s] = row_frag<T, HD>(qrows, (uint32_t)q, s, fg, a.hd);
-      gf[i][s] = row_frag<T, HD>(grows, (uint32_t)q, s, fg, a.hd);
-      const typename D::Frag of = row_frag<T, HD>(orows, (uint32_t)q, s, fg, a.hd);
-#pragma unroll
-      for (int e = 0; e < D::EL; ++e) t = fmaf((float)gf[i][s][e], (float)of[e], t);
-    }
-    dots[i] = rows4_sum(t);
-    put_stats<MASK>(load_stats(a, win, head, 0, L, q), &m[i], &l2[i]);
-#pragma unroll
-    for (int d = 0; d < D::ND; ++d) O[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < D::EL; ++e) dot = fmaf((float)g[s][e], (float)o[e], dot);
   }
+  dot = rows4_sum(dot);
+  put_stats<MASK>(load_stats(a, win, head, 0, L, query), &m, &l);
+  const f32x4 m4 = {m, m, m, m}, l4 = {l, l, l, l}, d4 = {dot, dot, dot, dot};
+  f32x4 O[D::ND];
+#pragma unroll
+  for (int d = 0; d < D::ND; ++d) O[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   load_rel<T>(a, head, rel);
 
   for (int k0 = 0; k0 < L; k0 += KT) {
-    if (k0) wg_barrier();
+    if (k0) wg_barrier();                                  // the tile before is read
     kc.store(Ks);
     vc.store(Vs);
     if (tid < KT) kinfo[tid] = info_of(a, k0 + tid, shifted);
     wg_barrier();
-    const int left = L - k0;
+    const int left = L - k0;                               // keys from k0 on
     kc.load(at.qkv(a.qkv, 1, k0 + KT, left - KT), a.hd);
     vc.load(at.qkv(a.qkv, 2, k0 + KT, left - KT), a.hd);
-    f32x4 Z[QB][2];
+    auto tile = [&](auto shift, auto tail) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      typename D::Frag kf[D::NS], vf[D::NS];
+      for (int ks = 0; ks < KT / 32; ++ks) {
+        if (decltype(tail)::value && 32 * ks >= left) break;
+        f32x4 Z[2];
 #pragma unroll
-      for (int s = 0; s < D::NS; ++s) {
-        kf[s] = row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg);
-        vf[s] = row_frag<T, HD>(Vs + (16 * kb + fr) * D::STR, s, fg);
+        for (int kb = 0; kb < 2; ++kb) {
+          const int k = 32 * ks + 16 * kb;
+          const int4 ki = *reinterpret_cast<const int4*>(kinfo + k + 4 * fg);
+          const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
+          const f32x4 bias = biases({qinfo, qinfo, qinfo, qinfo}, kn, decltype(shift)::value);
+          f32x4 s4 = {0.f, 0.f, 0.f, 0.f}, g4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < D::NS; ++s) {
+            s4 = mma(row_frag<T, HD>(Ks + (k + fr) * D::STR, s, fg), q[s], s4);
+            g4 = mma(row_frag<T, HD>(Vs + (k + fr) * D::STR, s, fg), g[s], g4);
+          }
+          logits(s4, zs, bias);
+          if constexpr (MASK) {
+            const f32x4 x = mask.get4(query, k0 + k + 4 * fg);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s4[r] += mask_units(x[r]);
+          }
+          if (decltype(tail)::value && k + 16 > left) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (k + 4 * fg + r >= left) s4[r] = -INFINITY;
+          }
+          weigh<MASK>(s4, g4, m4, l4, d4);
+          Z[kb] = g4;
+        }
+        const typename D::TFrag zf = pair_frag<T>(Z[0], Z[1]);
+#pragma unroll
+        for (int d = 0; d < D::ND; ++d) O[d] = mma(col_frag<T, D::STR>(Ks + 32 * ks * D::STR, 16 * d, fr, fg), zf, O[d]);
       }
-      const int4 ki = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
-      const int kn[4] = {ki.x, ki.y, ki.z, ki.w};
-      f32x4 bias[QB];
-#pragma unroll
-      for (int i = 0; i < QB; ++i) bias[i] = biases({qinfo[i], qinfo[i], qinfo[i], qinfo[i]}, kn, shifted);
-#pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        f32x4 s4 = {0.f, 0.f, 0.f, 0.f}, g4 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < D::NS; ++s) {
-          s4 = mma(kf[s], qf[i][s], s4);
-          g4 = mma(vf[s], gf[i][s], g4);
-        }
-        logits(s4, zs, bias[i]);
-        if constexpr (MASK) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s4[r] += mask_units(mask.get(q0 + 64 * i + fr, k0 + 16 * kb + 4 * fg + r));
-        }
-        if (16 * kb + 16 > left) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * kb + 4 * fg + r >= left) s4[r] = -INFINITY;
-        }
-        weigh<MASK>(s4, g4, f32x4{m[i], m[i], m[i], m[i]}, f32x4{l2[i], l2[i], l2[i], l2[i]}, f32x4{dots[i], dots[i], dots[i], dots[i]});
-        Z[i][kb] = g4;
-      }
-    }
-    typename D::TFrag kf[D::ND];
-#pragma unroll
-    for (int d = 0; d < D::ND; ++d) kf[d] = col_frag<T, D::STR>(Ks, 16 * d, fr, fg);
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-      const typename D::TFrag zf = pair_frag<T>(Z[i][0], Z[i][1]);
-#pragma unroll
-      for (int d = 0; d < D::ND; ++d) O[i][d] = mma(kf[d], zf, O[i][d]);
-    }
+    };
+    if (shifted) tile(std::true_type{}, std::true_type{});
+    else if (left < KT) tile(std::false_type{}, std::true_type{});
+    else tile(std::false_type{}, std::false_type{});
   }
   const Rows dq = at.qkv(a.dqkv, 0, 0, L);
 #pragma unroll
-  for (int i = 0; i < QB; ++i)
-#pragma unroll
-    for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(dq, (uint32_t)(q0 + 64 * i + fr), 16 * d + 4 * fg, a.hd, O[i][d], a.scale);
+  for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(dq, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], a.scale);
 }
 
-// out[h, y, r] = sum over the pairs of displacement r whose query lies in share y of the
-// window, and over the parts: a lane a displacement, neighbours on neighbouring keys, eight
-// queries at a time.
-__global__ __launch_bounds__(NT) void pairs_kernel(Args a, float* __restrict__ out, int share) {
+// Work of a workgroup of pairs_kernel: `queries` of a window's queries (a multiple of eight) and
+// `parts` of the parts; `shares` of them, qshares of the queries.
+struct Shares { int queries, parts, qshares, shares; };
+
+// out[h, y, r] = sum over the pairs of displacement r whose query lies in share y's queries, and
+// over its parts: a lane a displacement, neighbours on neighbouring keys, eight queries at a time.
+__global__ __launch_bounds__(NT) void pairs_kernel(Args a, float* __restrict__ out, Shares sh) {
   constexpr int U = 8;
   const int r = (int)blockIdx.x * NT + (int)threadIdx.x, h = (int)blockIdx.y, y = (int)blockIdx.z;
   const int w2 = 2 * a.W - 1, a2 = 2 * a.A - 1;
   const int dw = r % w2 - (a.W - 1), da = r / w2 % a2 - (a.A - 1), dt = r / w2 / a2 - (a.TW - 1);
   const int back = (dt * a.A + da) * a.W + dw;             // tokens between query and key
   const int64_t LL = (int64_t)a.L * a.L;
-  const int i0 = y * share, i1 = i0 + share < a.L ? i0 + share : a.L;
+  const int i0 = y % sh.qshares * sh.queries, i1 = i0 + sh.queries < a.L ? i0 + sh.queries : a.L;
+  const int p0 = y / sh.qshares * sh.parts, p1 = p0 + sh.parts < a.NP ? p0 + sh.parts : a.NP;
   int w = i0 % a.W, i = i0 / a.W % a.A, t = i0 / (a.W * a.A);
   float s[U] = {};
   for (int q0 = i0; q0 < i1; q0 += U) {
@@ -577,7 +570,7 @@ __global__ __launch_bounds__(NT) void pairs_kernel(Args a, float* __restrict__ o
         }
       }
     }
-    for (int p = 0; p < a.NP; ++p) {
+    for (int p = p0; p < p1; ++p) {
       const Plane x(a.part + ((int64_t)h * a.NP + p) * LL, a.L);
 #pragma unroll
       for (int u = 0; u < U; ++u) s[u] += __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(x.r, at[u], 0, 0));
@@ -649,14 +642,18 @@ void set_parts(Args& a, int waves, int keys) {
   a.NP = (int)((Bw + each - 1) / each);
 }
 
-// Queries of a share of pairs_kernel: a multiple of eight, about 2048 workgroups in all and at most
-// 32 shares.
-int share_of(const Args& a, int* shares) {
+// Shares of pairs_kernel: up to 32 of the queries, and, while that is fewer than 1024 workgroups,
+// of the parts, 64 in all (2048 windows of 7x7, two heads, 256 parts: the pass 183 -> 119 us).
+Shares shares_of(const Args& a) {
   const int64_t others = (int64_t)((a.R + NT - 1) / NT) * a.heads;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(32, 2048 / others));
-  const int share = (int)(((a.L + want - 1) / want + 7) / 8 * 8);
-  *shares = (a.L + share - 1) / share;
-  return share;
+  Shares s;
+  s.queries = (int)(((a.L + want - 1) / want + 7) / 8 * 8);
+  s.qshares = (a.L + s.queries - 1) / s.queries;
+  const int64_t more = std::max<int64_t>(1, std::min<int64_t>(64 / s.qshares, 1024 / (others * s.qshares)));
+  s.parts = (int)((a.NP + more - 1) / more);
+  s.shares = s.qshares * ((a.NP + s.parts - 1) / s.parts);
+  return s;
 }
 
 template <typename F>
@@ -694,14 +691,13 @@ int launch_keys(const Args& a, hipStream_t st) {
 template <typename T, int HD>
 int launch_queries(Args a, hipStream_t st) {
   typedef Dim<T, HD> D;
-  constexpr int QB = HD == 128 && sizeof(T) == 4 ? 1 : 2;
-  a.nqc = (a.L + 64 * QB - 1) / (64 * QB);
+  a.nqc = (a.L + 16 * WQ - 1) / (16 * WQ);
   a.dnqc = FastDiv::make((uint32_t)a.nqc);
   const int64_t grid = a.Bw * a.heads * a.nqc;
   if (grid >= (1LL << 31)) return set_error(NSW_ERR_INVALID, "nsw_position_attention_backward: too large");
-  const size_t lds = (size_t)2 * 32 * D::STR * sizeof(T) + 32 * sizeof(int) + (size_t)a.R * sizeof(float);
-  if (a.mask) hipLaunchKernelGGL((queries_kernel<T, HD, QB, true>), dim3((unsigned)grid), dim3(NT), lds, st, a);
-  else hipLaunchKernelGGL((queries_kernel<T, HD, QB, false>), dim3((unsigned)grid), dim3(NT), lds, st, a);
+  const size_t lds = (size_t)QKT * (2 * D::STR * sizeof(T) + sizeof(int)) + (size_t)a.R * sizeof(float);
+  if (a.mask) hipLaunchKernelGGL((queries_kernel<T, HD, true>), dim3((unsigned)grid), dim3(64 * WQ), lds, st, a);
+  else hipLaunchKernelGGL((queries_kernel<T, HD, false>), dim3((unsigned)grid), dim3(64 * WQ), lds, st, a);
   return check_launch("nsw_position_attention_backward");
 }
 
@@ -715,9 +711,7 @@ size_t backward_workspace(const Args& a0, int dtype) {
     set_parts(a, waves_of<T, HD>(a.L), 64 * KEY_BLOCKS<T, HD>);
     return 0;
   });
-  int shares;
-  share_of(a, &shares);
-  return (size_t)a.heads * ((size_t)shares * a.R + (size_t)a.NP * a.L * a.L) * sizeof(float);
+  return (size_t)a.heads * ((size_t)shares_of(a).shares * a.R + (size_t)a.NP * a.L * a.L) * sizeof(float);
 }
 
 int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream_t st) {
@@ -727,10 +721,9 @@ int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream
     constexpr int HD = decltype(hd)::value;
     const int waves = waves_of<T, HD>(a.L);
     set_parts(a, waves, 64 * KEY_BLOCKS<T, HD>);
-    int shares;
-    const int share = share_of(a, &shares);
+    const Shares sh = shares_of(a);
     float* sums = workspace;                               // [heads, shares, R], then the parts
-    a.part = dtable ? workspace + (size_t)a.heads * shares * a.R : nullptr;
+    a.part = dtable ? workspace + (size_t)a.heads * sh.shares * a.R : nullptr;
     int rc = NSW_OK;
     if (a.Bw > 0) {
       if (waves == 4) rc = launch_windows<T, HD, 4>(a, st);
@@ -745,11 +738,11 @@ int launch_backward(Args a, void* dtable, float* workspace, int dtype, hipStream
     }
     if (rc || !dtable) return rc;
     if (a.Bw > 0)
-      hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)((a.R + NT - 1) / NT), (unsigned)a.heads, (unsigned)shares), dim3(NT), 0, st, a,
-                         sums, share);
+      hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)((a.R + NT - 1) / NT), (unsigned)a.heads, (unsigned)sh.shares), dim3(NT), 0, st, a,
+                         sums, sh);
     const size_t lds = (size_t)((a.R + 63) / 64 * 64) * 8;
     hipLaunchKernelGGL((table_kernel<T>), dim3((unsigned)((a.nb + 63) / 64), (unsigned)a.heads), dim3(TT), lds, st, sums, a.buckets,
-                       (T*)dtable, a.R, a.Bw > 0 ? shares : 0, a.nb, a.heads);
+                       (T*)dtable, a.R, a.Bw > 0 ? sh.shares : 0, a.nb, a.heads);
     return check_launch(what);
   });
 }

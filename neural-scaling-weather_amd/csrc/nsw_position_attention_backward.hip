@@ -278,8 +278,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
 template <typename T, int HD>
 constexpr size_t keys_lds() { return 2 * (2 * QT * Dim<T, HD>::STR * sizeof(T) + 4 * QT * sizeof(float)); }
 
+// 512-byte rows: one workgroup a compute unit rather than 129 registers in memory (8 windows of
+// 20 x 25 with 8 heads of 128, fp32: the pass 423 -> 360 us).
 template <typename T, int HD, int KB, bool MASK>
-__global__ __launch_bounds__(NT, 2) void keys_kernel(Args a) {
+__global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_kernel(Args a) {
   typedef Dim<T, HD> D;
   constexpr int ND = D::ND, QG = 2 * QT * D::STR;
   extern __shared__ __attribute__((aligned(16))) char smem[];

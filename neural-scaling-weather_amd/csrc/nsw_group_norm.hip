@@ -31,6 +31,7 @@ namespace {
 
 constexpr int NT = 256;            // threads of a workgroup
 constexpr int64_t SMALL = 96 << 10;
+constexpr int64_t MOST_BLOCKS = 1 << 22;   // of the kernels that loop over groups or columns of all samples: a launch has fewer than 2^32 lanes
 
 struct GnArgs {
   const void *x, *dy, *w, *b;
@@ -199,25 +200,25 @@ __global__ __launch_bounds__(NT) void group_norm_stats_kernel(GnArgs a) {
 
 // (mean, rs) of each sample's groups from the workgroups' pairs, a wave each.
 __global__ __launch_bounds__(NT) void group_norm_join_kernel(GnArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * (NT / 64) + (int)threadIdx.x / 64;
-  if (i >= a.B * a.G) return;
   const int lane = (int)threadIdx.x & 63;
-  const int64_t s = i / a.G;
-  const f32x2* part = (const f32x2*)a.part + s * a.P * a.G + (i - s * a.G);
   auto rows = [&](int p) { return (float)((p + 1) * a.per < a.R ? a.per : a.R - p * a.per); };
-  float t = 0.f;
-  for (int p = lane; p < a.P; p += 64) t = fmaf(rows(p), part[(int64_t)p * a.G][0], t);
-  const float m = wave_sum(t) / (float)a.R;
-  float q = 0.f;
-  for (int p = lane; p < a.P; p += 64) {
-    const f32x2 v = part[(int64_t)p * a.G];
-    const float d = v[0] - m;
-    q += fmaf(rows(p) * (float)a.cpg * d, d, v[1]);
-  }
-  q = wave_sum(q);
-  if (lane == 0) {
-    a.stats[2 * i] = m;
-    a.stats[2 * i + 1] = root_of(q, (float)a.R * (float)a.cpg, a.eps);
+  for (int64_t i = (int64_t)blockIdx.x * (NT / 64) + (int)threadIdx.x / 64; i < a.B * a.G; i += (int64_t)gridDim.x * (NT / 64)) {
+    const int64_t s = i / a.G;
+    const f32x2* part = (const f32x2*)a.part + s * a.P * a.G + (i - s * a.G);
+    float t = 0.f;
+    for (int p = lane; p < a.P; p += 64) t = fmaf(rows(p), part[(int64_t)p * a.G][0], t);
+    const float m = wave_sum(t) / (float)a.R;
+    float q = 0.f;
+    for (int p = lane; p < a.P; p += 64) {
+      const f32x2 v = part[(int64_t)p * a.G];
+      const float d = v[0] - m;
+      q += fmaf(rows(p) * (float)a.cpg * d, d, v[1]);
+    }
+    q = wave_sum(q);
+    if (lane == 0) {
+      a.stats[2 * i] = m;
+      a.stats[2 * i + 1] = root_of(q, (float)a.R * (float)a.cpg, a.eps);
+    }
   }
 }
 
@@ -380,22 +381,31 @@ __global__ __launch_bounds__(NT) void group_norm_sums_kernel(GnArgs a) {
 // sums [B, 2, C] from the workgroups' partial rows.
 __global__ __launch_bounds__(NT) void group_norm_sums_join_kernel(GnArgs a, int blocks) {
   __shared__ __attribute__((aligned(16))) float red[32][36];
-  const int64_t s = (int64_t)blockIdx.x / blocks;
-  column_sums_block<float>(a.part + s * a.P * 2 * a.C, a.sums + s * 2 * a.C, a.P, 2 * a.C, (int)((int64_t)blockIdx.x - s * blocks),
-                           red);
+  for (int64_t i = blockIdx.x; i < a.B * blocks; i += gridDim.x) {
+    const int64_t s = i / blocks;
+    column_sums_block<float>(a.part + s * a.P * 2 * a.C, a.sums + s * 2 * a.C, a.P, 2 * a.C, (int)(i - s * blocks), red);
+    __syncthreads();
+  }
 }
 
-// db and dw from sums, 256 of their 2 C columns to a workgroup.
+// db and dw from sums, 32 of their 2 C columns to a workgroup, every 32nd sample to a lane.
+constexpr int PARAMS = 32;
 template <typename T>
 __device__ __forceinline__ void params_block(const GnArgs& a, int block) {
-  const int c = block * NT + (int)threadIdx.x;
-  if (c >= 2 * a.C) return;
+  __shared__ __attribute__((aligned(16))) float red[32][PARAMS + 4];
+  const int cl = ((int)threadIdx.x & 7) * 4, grp = (int)threadIdx.x >> 3, c = block * PARAMS + cl;
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
+  if (c < 2 * a.C)
+#pragma unroll 4
+    for (int64_t s = grp; s < a.B; s += 32) t += *reinterpret_cast<const f32x4*>(a.sums + s * 2 * a.C + c);
+  *reinterpret_cast<f32x4*>(&red[grp][cl]) = t;
+  __syncthreads();
   T* out = (T*)(c < a.C ? a.db : a.dw);
-  if (out == nullptr) return;
-  float t = 0.f;
-#pragma unroll 8
-  for (int64_t s = 0; s < a.B; ++s) t += a.sums[s * 2 * a.C + c];
-  out[c < a.C ? c : c - a.C] = from_f32<T>(t);
+  if (grp != 0 || c >= 2 * a.C || out == nullptr) return;
+#pragma unroll
+  for (int i = 1; i < 32; ++i) t += *reinterpret_cast<const f32x4*>(&red[i][cl]);
+  const float v[4] = {t[0], t[1], t[2], t[3]};
+  store4<T>(out + (c < a.C ? c : c - a.C), v);
 }
 
 template <typename T>
@@ -465,7 +475,7 @@ __device__ __forceinline__ void gradient_rows(const GnArgs& a, const T* x, const
   in_pairs<T, CPT, 1>(x, dy, r, r1, a, at, body);
 }
 
-// The first workgroups, 256 columns each, form the parameters' gradients, the rest dx.
+// The first workgroups form the parameters' gradients, the rest dx.
 template <typename T, int CPT, int ACT>
 __global__ __launch_bounds__(NT) void group_norm_gradient_kernel(GnArgs a, int params) {
   extern __shared__ float lds[];
@@ -612,7 +622,7 @@ extern "C" int nsw_group_norm(const void* x, const void* weight, const void* bia
     set(a, ps);
     if (ps.P > 1) {
       hipLaunchKernelGGL((group_norm_stats_kernel<T, CPT>), dim3((unsigned)(B * ps.P)), dim3(NT), slots_lds(a), st, a);
-      hipLaunchKernelGGL(group_norm_join_kernel, dim3((unsigned)((B * groups + 3) / 4)), dim3(NT), 0, st, a);
+      hipLaunchKernelGGL(group_norm_join_kernel, dim3((unsigned)std::min<int64_t>((B * groups + 3) / 4, MOST_BLOCKS)), dim3(NT), 0, st, a);
       set(a, pa);
     }
     return with_act(act, [&](auto ac) {
@@ -653,7 +663,7 @@ extern "C" int nsw_group_norm_backward(const void* dy, const void* x, const floa
   a.sums = (float*)workspace;
   a.part = a.sums + std::max<int64_t>(B, 1) * 2 * C;
   hipStream_t st = (hipStream_t)stream;
-  const int params = dweight || dbias ? (int)((2 * C + NT - 1) / NT) : 0;
+  const int params = dweight || dbias ? (int)((2 * C + PARAMS - 1) / PARAMS) : 0;
   return with_cols(dtype, C, [&](auto t, auto cpt) {
     using T = decltype(t);
     constexpr int CPT = decltype(cpt)::value;
@@ -673,7 +683,7 @@ extern "C" int nsw_group_norm_backward(const void* dy, const void* x, const floa
       }
       const int blocks = (int)((2 * C + 31) / 32);
       hipLaunchKernelGGL((group_norm_sums_kernel<T, CPT, ACT>), dim3((unsigned)(B * ps.P)), dim3(NT), slots_lds(a), st, a);
-      hipLaunchKernelGGL(group_norm_sums_join_kernel, dim3((unsigned)(B * blocks)), dim3(NT), 0, st, a, blocks);
+      hipLaunchKernelGGL(group_norm_sums_join_kernel, dim3((unsigned)std::min<int64_t>(B * blocks, MOST_BLOCKS)), dim3(NT), 0, st, a, blocks);
       set(a, pa);
       if (dx == nullptr)
         hipLaunchKernelGGL((group_norm_params_kernel<T>), dim3((unsigned)params), dim3(NT), 0, st, a);

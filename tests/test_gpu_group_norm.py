@@ -258,6 +258,34 @@ def test_more_than_32_bits_of_bytes(device):
     assert (err <= want.abs() * 2 ** -8 + 4 * K * U * (1 + want.abs())).all(), err.max()
 
 
+def test_many_large_samples(device):
+    """More groups and columns in all than one launch joins: the first, a middle and the last sample, and the
+    parameters' gradients, sums of all of them."""
+    B, R, C, groups, eps = 16400, 13, 4096, 2048, 1e-5
+    g = torch.Generator(device=device).manual_seed(5)
+    x = torch.empty(B, R, C, dtype=torch.bfloat16, device=device).normal_(generator=g)
+    dy = torch.empty_like(x).normal_(generator=g)
+    w = torch.empty(C, dtype=torch.bfloat16, device=device).normal_(1.0, 0.2, generator=g)
+    b = torch.empty_like(w).normal_(generator=g)
+    y, stats = ops.group_norm(x, groups, w, b, eps=eps)
+    dx, dw, db = ops.group_norm_backward(dy, x, stats, groups, w, b)
+    for i in (0, 8201, B - 1):
+        t = {"x": x[i:i + 1].cpu(), "dy": dy[i:i + 1].cpu(), "weight": w.cpu(), "bias": b.cpu()}
+        want = reference(t, groups, "none", eps)
+        check({"y": y[i:i + 1], "dx": dx[i:i + 1]}, {k: want[k] for k in ("y", "dx")}, torch.bfloat16)
+    sums = torch.zeros(4, C, dtype=torch.float64, device=device)
+    for i in range(0, B, 1000):
+        v = x[i:i + 1000].double().view(-1, R, groups, C // groups)
+        var, mean = torch.var_mean(v, (1, 3), correction=0, keepdim=True)
+        xh = ((v - mean) * (var + eps).rsqrt()).view(-1, R, C)
+        d = dy[i:i + 1000].double()
+        sums += torch.stack([x_.sum((0, 1)) for x_ in (d, d.abs(), d * xh, (d * xh).abs())])
+    for got, v, mag in ((db, sums[0], sums[1]), (dw, sums[2], sums[3] + sums[1])):
+        # xh is off by h of reference(), at most 4 K u a term here, the sums by K u
+        err = (got.double() - v).abs() - (v.abs() * 2 ** -8 + 5 * K * U * mag * (1 + 2 ** -8))
+        assert (err <= 0).all(), err.max()
+
+
 # ------------------------------------------------- autograd, modules, graphs ---
 
 def module(dtype, device, seed=1):

@@ -548,7 +548,9 @@ int nsw_group_norm_backward(const void* dy, const void* x, const float* stats, c
  * the shift (s0, s1) of an image of H x W tokens gives nsw_window_attention's.  stats
  * [Bw, num_heads, L, 2] fp32 receives each row's maximum m of z log2(e) and log2 of its sum of
  * 2^(z log2(e) - m).  bf16: fp32 logits and sums, probabilities rounded to bf16 for the
- * product with v and their sum.  Head dims 4, 8, 16, 32, 64, 128; C a multiple of 8; qkv, o, stats 16-byte aligned. */
+ * product with v and their sum.  Head dims 4, 8, 16, 32, 64, 128; C a multiple of 8 below 2^18;
+ * a window's rows of qkv below 2 GiB; Bw * num_heads below 2^31, and times ceil(L / 128) below
+ * 2^23 where L > 64; qkv, o, stats 16-byte aligned. */
 int nsw_position_attention(const void* qkv, const void* table, const int32_t* buckets, const float* mask,
                            int64_t nW_mask, void* o, float* stats, int64_t Bw, int64_t L, int64_t C,
                            int64_t num_heads, float scale, int64_t num_buckets, int64_t T, int64_t ws0, int64_t ws1,

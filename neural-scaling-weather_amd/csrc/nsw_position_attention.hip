@@ -181,6 +181,7 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
 // ---------------------------------------------------------- longer windows ---
 
 constexpr int WAVES = 8;                                           // of forward_kernel, 16 queries each
+constexpr int64_t MOST_BLOCKS = 1 << 23;                           // a launch has fewer than 2^32 lanes
 
 // A workgroup takes 128 queries of a (window, head) over 64-key tiles, the next tile in
 // registers meanwhile, two workgroups a compute unit (1999 tokens, 8 heads of 64, bf16: 45 us;
@@ -313,7 +314,7 @@ int launch_long(Args a, hipStream_t st) {
   a.nqc = (a.L + 16 * WAVES - 1) / (16 * WAVES);
   a.dnqc = FastDiv::make((uint32_t)a.nqc);
   const int64_t grid = a.Bw * a.heads * a.nqc;
-  if (grid >= (1LL << 31)) return set_error(NSW_ERR_INVALID, "nsw_position_attention: too large");
+  if (grid >= MOST_BLOCKS) return set_error(NSW_ERR_INVALID, "nsw_position_attention: too large");
   const size_t lds = (size_t)2 * 64 * D::STR * sizeof(T) + 64 * sizeof(int) + (size_t)a.R * sizeof(float);
   if (a.mask != nullptr) hipLaunchKernelGGL((forward_kernel<T, HD, true>), dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
   else hipLaunchKernelGGL((forward_kernel<T, HD, false>), dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
@@ -377,7 +378,8 @@ int make_args(Args& a, const char* what, int64_t Bw, int64_t L, int64_t C, int64
   NSW_CHECK_ARG(R <= MAX_R, "%s: %lld displacements in a window, at most %d", what, (long long)R, MAX_R);
   NSW_CHECK_ARG(nb > 0 && nb < (1 << 24), "%s: %lld buckets", what, (long long)nb);
   NSW_CHECK_ARG(std::isfinite(scale), "%s: scale=%g", what, (double)scale);
-  NSW_CHECK_ARG(Bw * L < (1LL << 40) && Bw * heads < (1LL << 31) && L * 3 * C * (int64_t)dtype_size(dtype) < (1LL << 31),
+  NSW_CHECK_ARG(Bw < (1LL << 31) && Bw * heads < (1LL << 31) && (L <= 64 || Bw * heads * ((L + 127) / 128) < MOST_BLOCKS) &&
+                    L * 3 * C * (int64_t)dtype_size(dtype) < (1LL << 31),
                 "%s: too large", what);
   a.Bw = Bw; a.L = (int)L; a.C = (int)C; a.heads = (int)heads; a.hd = (int)hd; a.R = (int)R; a.nb = (int)nb;
   a.TW = (int)T; a.A = (int)A; a.W = (int)W; a.scale = scale;

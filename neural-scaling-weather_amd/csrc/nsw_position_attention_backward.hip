@@ -696,7 +696,6 @@ int launch_queries(Args a, hipStream_t st) {
   a.nqc = (a.L + 16 * WQ - 1) / (16 * WQ);
   a.dnqc = FastDiv::make((uint32_t)a.nqc);
   const int64_t grid = a.Bw * a.heads * a.nqc;
-  if (grid >= (1LL << 31)) return set_error(NSW_ERR_INVALID, "nsw_position_attention_backward: too large");
   const size_t lds = (size_t)QKT * (2 * D::STR * sizeof(T) + sizeof(int)) + (size_t)a.R * sizeof(float);
   if (a.mask) hipLaunchKernelGGL((queries_kernel<T, HD, true>), dim3((unsigned)grid), dim3(64 * WQ), lds, st, a);
   else hipLaunchKernelGGL((queries_kernel<T, HD, false>), dim3((unsigned)grid), dim3(64 * WQ), lds, st, a);

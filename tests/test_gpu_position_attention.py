@@ -53,7 +53,7 @@ def reference(t, mask=None):
     idx = pairs(*t["extent"])
     bias = rel[idx].permute(2, 0, 1)
     z = t["scale"] * q @ k.mT + bias
-    e = (hd + 6) * U * (t["scale"] * q.abs() @ k.abs().mT + bias.abs())
+    e = (hd + 6) * U * (abs(t["scale"]) * q.abs() @ k.abs().mT + bias.abs())
     if mask is not None:
         m = mask.repeat(Bw // mask.shape[0], 1, 1)[:, None]
         z = (z.float() + m).double()
@@ -127,6 +127,17 @@ def test_head_dims(device, dtype, hd, extent):
                                     (3, 6, 9), (1, 1, 257), (5, 1, 7), (4, 4, 1), (1, 40, 2)])
 def test_extents(device, dtype, extent):
     t = case(dtype, 2, extent, 2, 32, seed=math.prod(extent))
+    check(run(t, device), reference(t), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extent", [(1, 5, 6), (1, 9, 18), (1, 1, 200)])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-8, 1e-6, 1e6, 1e8])
+def test_scales(device, dtype, extent, scale):
+    t = case(dtype, 3, extent, 2, 64, seed=12)
+    if abs(scale) >= 1e6:
+        t["qkv"][..., :128] /= 4 * scale
+    t["scale"] = scale
     check(run(t, device), reference(t), dtype)
 
 

@@ -48,6 +48,13 @@ def test_refusals(call, kw, says):
     assert says in _lib.lib().nsw_last_error(), _lib.lib().nsw_last_error()
 
 
+@pytest.mark.parametrize("call", [forward, backward])
+@pytest.mark.parametrize("kw", [dict(Bw=1 << 31), dict(Bw=1 << 30), dict(Bw=1 << 22, A=5, W=14), dict(C=1 << 18, heads=1 << 11),
+                                dict(C=131072, heads=1024, A=1, W=4096)])
+def test_sizes_past_a_launch_are_refused(call, kw):
+    assert call(**kw) == _lib.NSW_ERR_INVALID
+
+
 @pytest.mark.parametrize("kw", [dict(ws=None), dict(nbytes=64), dict(ws=8)])
 def test_workspace_refusals(kw):
     assert backward(**kw) == _lib.NSW_ERR_INVALID and (b"workspace" in _lib.lib().nsw_last_error())

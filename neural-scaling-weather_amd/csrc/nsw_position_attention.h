@@ -16,7 +16,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct Args {
   const void *qkv, *table, *dout, *out;
   void *o, *dqkv;
-  float* stats;                     // [Bw, heads, L, 2]: row maximum m of z log2 e, log2 of the row's sum of exp2(z log2 e - m)
+  float* stats;                     // [Bw, heads, L, ns]: row maximum m of z log2 e, log2 of the row's sum of exp2(z log2 e - m), lost bits
+  int ns;
   const int* buckets;               // [R]
   const float* mask;                // [nW, L, L] or NULL
   float* part;                      // [heads, NP, L, L]: dz summed over the windows of a workgroup, or NULL
@@ -251,9 +252,46 @@ struct TileCopy {
   }
 };
 
-// Dot products of the rows of two tiles held by TileCopy, to dst[row] in LDS.
+// D = do o of the gradients cancels against do v, and the rounding of o to bf16 would be most of
+// its error (dtable 2.5e-3 off where its own rounding is 1.7e-3).  The forward pass therefore
+// leaves, behind a row's statistics, what each value of o lost, in sixteenths of a step and 4
+// bits: a quarter of o's bytes.  A step is 2^16 of fp32's pattern, whatever the exponent: the
+// difference of the two patterns is rounded to 2^12, -7 .. 6 of it are written as 1 .. 14, so that
+// no word of them is a float's NaN, and none zero, which is what lies past a window's rows.
+__device__ __forceinline__ uint32_t lost_of(float x) {
+  const int d = __builtin_bit_cast(int, x) - __builtin_bit_cast(int, (float)(bf16)x) + 0x8800;
+  return (uint32_t)(d < 0x1000 ? 0x1000 : d > 0xefff ? 0xefff : d) >> 12;
+}
+// the value from its bf16 and the e-th 4 bits of a word
+__device__ __forceinline__ float found(float b, uint32_t bits, int e) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, b) - 0x8000u + ((bits >> 4 * e & 15u) << 12));
+}
+__device__ __forceinline__ uint32_t lost_word(const Rows& stats, uint32_t at) {
+  const uint32_t v = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(stats.r, at, 0, 0);
+  return v ? v : 0x88888888u;
+}
+
+// The lost bits that belong to a TileCopy of o: a word to 8 values.
+template <typename T, int HD, int ROWS, int NT = posattn::NT>
+struct Lost {
+  typedef Dim<T, HD> D;
+  static constexpr int N = sizeof(T) == 2 ? TileCopy<T, HD, ROWS, NT>::N : 0;
+  uint32_t v[N > 0 ? N : 1];
+  __device__ __forceinline__ void load(const Rows& stats, int hd) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int i = (int)threadIdx.x % NT + NT * c, r = i / D::CPR, ch = i % D::CPR;
+      const uint32_t at = (HD > 16 || 8 * ch < hd) && (ROWS * D::CPR % NT == 0 || r < ROWS) ? (uint32_t)r * stats.ldb + 8u + 4u * ch : NOWHERE;
+      v[c] = lost_word(stats, at);
+    }
+  }
+};
+
+// Dot products of the rows of two tiles held by TileCopy, of the second with its lost bits, to
+// dst[row] in LDS.
 template <typename T, int HD, int ROWS, int NT>
-__device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS, NT>& x, const TileCopy<T, HD, ROWS, NT>& y, float* dst) {
+__device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS, NT>& x, const TileCopy<T, HD, ROWS, NT>& y,
+                                         const Lost<T, HD, ROWS, NT>& lost, float* dst) {
   typedef Dim<T, HD> D;
 #pragma unroll
   for (int c = 0; c < TileCopy<T, HD, ROWS, NT>::N; ++c) {
@@ -262,7 +300,7 @@ __device__ __forceinline__ void row_dots(const TileCopy<T, HD, ROWS, NT>& x, con
     if constexpr (sizeof(T) == 2) {
       const bf16x8 u = __builtin_bit_cast(bf16x8, x.v[c]), w = __builtin_bit_cast(bf16x8, y.v[c]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf((float)u[e], (float)w[e], s);
+      for (int e = 0; e < 8; ++e) s = fmaf((float)u[e], found((float)w[e], lost.v[c], e), s);
     } else {
       const f32x4 u = __builtin_bit_cast(f32x4, x.v[c]), w = __builtin_bit_cast(f32x4, y.v[c]);
 #pragma unroll
@@ -295,6 +333,16 @@ __device__ __forceinline__ void store_quad(const Rows& x, uint32_t row, int d, i
   }
 }
 
+// What 4 values v f of a result lost in store_quad, to the row's statistics.
+template <typename T, int HD>
+__device__ __forceinline__ void store_lost(const Rows& stats, uint32_t row, int d, int hd, const f32x4& v, float f) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t b = lost_of(v[0] * f) | lost_of(v[1] * f) << 4 | lost_of(v[2] * f) << 8 | lost_of(v[3] * f) << 12;
+    const uint32_t at = HD > 16 || d < (hd + 7) / 8 * 8 ? row * stats.ldb + 8u + (uint32_t)(d / 2) : NOWHERE;
+    __builtin_amdgcn_raw_buffer_store_b16((unsigned short)b, stats.r, at, 0, 0);
+  }
+}
+
 // Where a window's rows begin in each tensor, for one head.
 struct At {
   uint32_t ldb, ob;                 // bytes of a row of qkv, of o
@@ -310,6 +358,10 @@ struct At {
   // rows [r0, r0 + n) of part 0 (q), 1 (k), 2 (v) of qkv or its gradient; of o or its gradient
   __device__ __forceinline__ Rows qkv(const void* p, int part, int r0, int n) const {
     return Rows((const char*)p + q + (int64_t)r0 * ldb + part * (int64_t)ob, ldb, n, bytes);
+  }
+  // rows [r0, r0 + n) of the statistics
+  __device__ __forceinline__ static Rows stats(const Args& a, int64_t win, int head, int r0, int n) {
+    return Rows(a.stats + ((win * a.heads + head) * a.L + r0) * a.ns, 4u * (uint32_t)a.ns, n, 4 * a.ns);
   }
   __device__ __forceinline__ Rows out(const void* p, int r0, int n) const { return Rows((const char*)p + o + (int64_t)r0 * ob, ob, n, bytes); }
 };

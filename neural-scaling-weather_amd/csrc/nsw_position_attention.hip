@@ -14,8 +14,8 @@
 // O^T = V^T P^T as they lie.  Logits in units of log2 e (the factor is in the scale and in the bias's LDS copy), so
 // that a probability is one subtraction and exp2.  fp32 statistics and sums; bf16: probabilities
 // (at most 1) are rounded to bf16 for the product with v, and their sum is of the rounded
-// ones, by a product with ones on the matrix units.  stats keeps m and log2 of the sum apart,
-// since their sum would lose the second where |m| is large.
+// ones, by a product with ones on the matrix units (the gradients' sum, in stats, is not).  stats
+// keeps m and log2 of the sum apart, since their sum would lose the second where |m| is large.
 #include <algorithm>
 #include <cmath>
 
@@ -28,6 +28,13 @@ int check_geom(int64_t B, int64_t T, int64_t H, int64_t W, int64_t ws0, int64_t 
 namespace posattn {
 
 namespace {
+
+// A row's maximum and log2 of its sum.
+__device__ __forceinline__ void store_stats(const Rows& stats, uint32_t at, float m, float t) {
+  typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+  const f32x2 v = {m, __builtin_amdgcn_logf(t)};
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), stats.r, at, 0, 0);
+}
 
 // ------------------------------------------------- windows in a workgroup ---
 
@@ -155,7 +162,7 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         S[kb][r] = __builtin_amdgcn_exp2f(START ? fmaf(S[kb][r], zs, to) : S[kb][r] + to);
-        if constexpr (!ONES) l += S[kb][r];
+        l += S[kb][r];
       }
     f32x4 O[D::ND], Z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -168,13 +175,15 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
       for (int d = 0; d < D::ND; ++d) O[d] = mma(col_frag<T, D::STR>(Vs + 32 * ks * D::STR, 16 * d, fr, fg), pf, O[d]);
       if constexpr (ONES) Z = mma(ones, pf, Z);
     }
-    const float t = ONES ? Z[0] : rows4_sum(l);
+    const float sum = rows4_sum(l), t = ONES ? Z[0] : sum;
     const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;      // an empty row: zeros; NaN stays
     const Rows orows = at.out(a.o, 0, L);
 #pragma unroll
     for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orows, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], inv);
-    if (query < L && fg == 0)
-      *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + query) * 2) = f32x2{mx, __builtin_amdgcn_logf(t)};
+    const Rows srows = At::stats(a, win, head, 0, L);
+#pragma unroll
+    for (int d = 0; d < D::ND; ++d) store_lost<T, HD>(srows, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], inv);
+    store_stats(srows, fg == 0 ? (uint32_t)query * srows.ldb : NOWHERE, mx, sum);
   }
 }
 
@@ -280,7 +289,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void forward_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           S[kb][r] = __builtin_amdgcn_exp2f(S[kb][r] - to);
-          if constexpr (!ONES) t += S[kb][r];
+          t += S[kb][r];
         }
       l = fmaf(l, f, t);
       Z *= f;
@@ -300,12 +309,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void forward_kernel(Args a) {
     else tile(std::false_type{}, std::false_type{});
   }
   const Rows orows = at.out(a.o, 0, L);
-  const float t = ONES ? Z[0] : rows4_sum(l);
+  const float sum = rows4_sum(l), t = ONES ? Z[0] : sum;
   const float inv = t > 0.f ? 1.f / t : t == 0.f ? 0.f : t;        // an empty row: zeros; NaN stays
 #pragma unroll
   for (int d = 0; d < D::ND; ++d) store_quad<T, HD>(orows, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], inv);
-  if (query < L && fg == 0)
-    *reinterpret_cast<f32x2*>(a.stats + (((win * a.heads + head) * L) + query) * 2) = f32x2{m, __builtin_amdgcn_logf(t)};
+  const Rows srows = At::stats(a, win, head, 0, L);
+#pragma unroll
+  for (int d = 0; d < D::ND; ++d) store_lost<T, HD>(srows, (uint32_t)query, 16 * d + 4 * fg, a.hd, O[d], inv);
+  store_stats(srows, fg == 0 ? (uint32_t)query * srows.ldb : NOWHERE, m, sum);
 }
 
 template <typename T, int HD>
@@ -383,6 +394,7 @@ int make_args(Args& a, const char* what, int64_t Bw, int64_t L, int64_t C, int64
                 "%s: too large", what);
   a.Bw = Bw; a.L = (int)L; a.C = (int)C; a.heads = (int)heads; a.hd = (int)hd; a.R = (int)R; a.nb = (int)nb;
   a.TW = (int)T; a.A = (int)A; a.W = (int)W; a.scale = scale;
+  a.ns = dtype == NSW_DTYPE_BF16 ? 2 + (int)((hd + 7) / 8) : 2;
   a.off = (int)(((T - 1) * (2 * A - 1) + A - 1) * (2 * W - 1) + W - 1);
   a.dAW = FastDiv::make((uint32_t)(A * W)); a.dW = FastDiv::make((uint32_t)W); a.dheads = FastDiv::make((uint32_t)heads);
   a.mask = mask; a.nW = 1; a.band0 = 1; a.thr = 0;

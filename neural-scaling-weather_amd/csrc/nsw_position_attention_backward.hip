@@ -52,8 +52,8 @@ __device__ __forceinline__ void put_stats(const f32x2& st, float* mrow, float* l
 // Statistics of query q0 + i of a window, of n queries from q0 on; none behind them.
 __device__ __forceinline__ f32x2 load_stats(const Args& a, int64_t win, int head, int q0, int n, int i) {
   typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
-  const Rows x(a.stats + ((win * a.heads + head) * a.L + q0) * 2, 8u, a.L - q0, 8);
-  const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(x.r, i < n ? 8u * (uint32_t)i : NOWHERE, 0, 0);
+  const Rows x = At::stats(a, win, head, q0, a.L - q0);
+  const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(x.r, i < n ? (uint32_t)i * x.ldb : NOWHERE, 0, 0);
   const f32x2 st = __builtin_bit_cast(f32x2, v);
   return i < n ? st : f32x2{-INFINITY, 0.f};
 }
@@ -121,6 +121,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
   // what a window needs first, in registers: k, v and the first tile
   TileCopy<T, HD, X::KEYS, N> kc, vc;
   TileCopy<T, HD, QT> qc, gc, oc;
+  Lost<T, HD, QT> lost;
   f32x2 st;
   // rows of the window from q0 on, n of them (none: zeros, so that nothing is kept from before)
   auto load_tile = [&](int64_t win, int q0, int n) {
@@ -128,6 +129,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
     qc.load(at.qkv(a.qkv, 0, q0, bring_q ? n : 0), a.hd);
     gc.load(at.out(a.dout, q0, bring_g ? n : 0), a.hd);
     oc.load(at.out(a.out, q0, bring_g ? n : 0), a.hd);
+    lost.load(At::stats(a, win, head, q0, bring_g ? n : 0), a.hd);
     st = load_stats(a, win, head, q0, tid < QT ? n : 0, tid);
   };
   auto load_window = [&](int64_t win) {
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
     if (bring_q) qc.store(q);
     if (bring_g) {
       gc.store(q + QT * D::STR);
-      row_dots(gc, oc, r + 3 * QT);
+      row_dots(gc, oc, lost, r + 3 * QT);
     }
     if (tid < QT) {
       ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + rel_base(a, rel);
@@ -306,11 +308,13 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
     const Plane mask(MASK ? a.mask + (int64_t)wi * L * L : nullptr, MASK ? L : 0);
 
     TileCopy<T, HD, QT> qc, gc, oc;
+    Lost<T, HD, QT> lost;
     f32x2 st;
     auto load_tile = [&](int q0) {
       qc.load(at.qkv(a.qkv, 0, q0, L - q0), a.hd);
       gc.load(at.out(a.dout, q0, L - q0), a.hd);
       oc.load(at.out(a.out, q0, L - q0), a.hd);
+      lost.load(At::stats(a, win, head, q0, L - q0), a.hd);
       st = load_stats(a, win, head, q0, tid < QT ? L - q0 : 0, tid);
     };
     auto store_tile = [&](int step) {
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
       float* r = rows + (step & 1) * 4 * QT;
       qc.store(q);
       gc.store(q + QT * D::STR);
-      row_dots(gc, oc, r + 3 * QT);
+      row_dots(gc, oc, lost, r + 3 * QT);
       if (tid < QT) {
         ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + rel_base(a, rel);
         put_stats<MASK>(st, r + QT + tid, r + 2 * QT + tid);
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
   TileCopy<T, HD, KT, 64 * WQ> kc, vc;
   kc.load(at.qkv(a.qkv, 1, 0, L), a.hd);
   vc.load(at.qkv(a.qkv, 2, 0, L), a.hd);
-  const Rows qrows = at.qkv(a.qkv, 0, 0, L), grows = at.out(a.dout, 0, L), orows = at.out(a.out, 0, L);
+  const Rows qrows = at.qkv(a.qkv, 0, 0, L), grows = at.out(a.dout, 0, L), orows = at.out(a.out, 0, L), srows = At::stats(a, win, head, 0, L);
   typename D::Frag q[D::NS], g[D::NS];
   const int qinfo = info_of(a, query, shifted) + rel_base(a, rel);
   const float zs = a.scale * LOG2E;
@@ -474,8 +478,16 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
     q[s] = row_frag<T, HD>(qrows, (uint32_t)query, s, fg, a.hd);
     g[s] = row_frag<T, HD>(grows, (uint32_t)query, s, fg, a.hd);
     const typename D::Frag o = row_frag<T, HD>(orows, (uint32_t)query, s, fg, a.hd);
+    if constexpr (sizeof(T) == 2) {
+      const int ch = 4 * s + fg;
+      const uint32_t at = HD > 16 || 8 * ch < a.hd ? (uint32_t)query * srows.ldb + 8u + 4u * ch : NOWHERE;
+      const uint32_t bits = lost_word(srows, at);
 #pragma unroll
-    for (int e = 0; e < D::EL; ++e) dot = fmaf((float)g[s][e], (float)o[e], dot);
+      for (int e = 0; e < D::EL; ++e) dot = fmaf((float)g[s][e], found((float)o[e], bits, e), dot);
+    } else {
+#pragma unroll
+      for (int e = 0; e < D::EL; ++e) dot = fmaf(g[s][e], o[e], dot);
+    }
   }
   dot = rows4_sum(dot);
   put_stats<MASK>(load_stats(a, win, head, 0, L, query), &m, &l);

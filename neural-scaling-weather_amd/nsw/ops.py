@@ -672,6 +672,11 @@ def _position_args(what, qkv, num_heads, table, buckets, extent, mask, geometry)
     return at, Bw, L, C, mask, nW, (table.shape[0], T, A, W, H, Wi, int(s0), int(s1), dtype_code(qkv))
 
 
+def position_stats_width(qkv: torch.Tensor, num_heads: int) -> int:
+    """Floats of a row of position_attention's stats."""
+    return 2 + (qkv.shape[-1] // 3 // max(num_heads, 1) + 7) // 8 if qkv.dtype == torch.bfloat16 else 2
+
+
 def position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: torch.Tensor, buckets: torch.Tensor,
                        extent: Sequence[int], mask: Optional[torch.Tensor] = None,
                        geometry: Optional[Tuple[int, int, Tuple[int, int], Tuple[int, int], int]] = None
@@ -682,12 +687,14 @@ def position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: t
     displacements of a query from a key, ((dt + T-1) (2A-1) + da + A-1) (2W-1) + dw + W-1;
     buckets [(2T-1)(2A-1)(2W-1)] int32 (at most 8192), table [buckets, num_heads] in
     qkv's dtype.  ``mask`` [nW, L, L] or ``geometry`` as window_attention; a row whose
-    mask leaves nothing gives zeros.  stats [Bw, num_heads, L, 2] fp32 (each row's
-    maximum m of z log2(e), log2 of its sum of 2^(z log2(e) - m)) for position_attention_backward."""
+    mask leaves nothing gives zeros (k and v have to be finite also where they are masked, as
+    for the formula).  stats [Bw, num_heads, L, position_stats_width] fp32 for
+    position_attention_backward: each row's maximum m of z log2(e), log2 of its sum of
+    2^(z log2(e) - m); bf16: then the bits that o's rounding lost."""
     what = "position_attention"
     at, Bw, L, C, mask, nW, sizes = _position_args(what, qkv, num_heads, table, buckets, extent, mask, geometry)
     o = qkv.new_empty((Bw, L, C))
-    stats = qkv.new_empty((Bw, num_heads, L, 2), dtype=torch.float32)
+    stats = qkv.new_empty((Bw, num_heads, L, position_stats_width(qkv, num_heads)), dtype=torch.float32)
     _run(what, at, lib().nsw_position_attention, qkv.data_ptr(), table.data_ptr(), buckets.data_ptr(), _p(mask), nW,
          o.data_ptr(), stats.data_ptr(), Bw, L, C, num_heads, float(scale), *sizes)
     return o, stats
@@ -705,8 +712,9 @@ def position_attention_backward(do: torch.Tensor, qkv: torch.Tensor, o: torch.Te
     _dev(qkv, stats)
     if do.shape != (Bw, L, C) or o.shape != (Bw, L, C):
         raise ValueError(f"{what}: do {tuple(do.shape)} and o {tuple(o.shape)}, expected {(Bw, L, C)}")
-    if stats.dtype != torch.float32 or stats.shape != (Bw, num_heads, L, 2):
-        raise ValueError(f"{what}: stats is {stats.dtype} {tuple(stats.shape)}, expected float32 {(Bw, num_heads, L, 2)}")
+    rows = (Bw, num_heads, L, position_stats_width(qkv, num_heads))
+    if stats.dtype != torch.float32 or stats.shape != rows:
+        raise ValueError(f"{what}: stats is {stats.dtype} {tuple(stats.shape)}, expected float32 {rows}")
     if not any(needs):
         return None, None
     dqkv = torch.empty_like(qkv)

@@ -483,7 +483,8 @@ def _position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: 
 @_position_attention.register_fake
 def _(qkv, num_heads, scale, table, buckets, extent, mask, geometry):
     Bw, L, C3 = qkv.shape
-    return qkv.new_empty((Bw, L, C3 // 3)), qkv.new_empty((Bw, num_heads, L, 2), dtype=torch.float32)
+    return (qkv.new_empty((Bw, L, C3 // 3)),
+            qkv.new_empty((Bw, num_heads, L, ops.position_stats_width(qkv, num_heads)), dtype=torch.float32))
 
 
 @torch.library.custom_op("nsw::position_attention_backward", mutates_args=())

@@ -142,7 +142,7 @@ def test_shapes_without_a_gpu():
         qkv, table = torch.empty(4, 15, 192, dtype=torch.bfloat16), torch.empty(45, 2, dtype=torch.bfloat16)
         b = torch.empty(45, dtype=torch.int32)
         o, stats = n.position_attention(qkv, 2, 0.2, table, b, [1, 3, 5], None, [])
-        assert o.shape == (4, 15, 64) and o.dtype == qkv.dtype and stats.shape == (4, 2, 15, 2) and stats.dtype == torch.float32
+        assert o.shape == (4, 15, 64) and o.dtype == qkv.dtype and stats.shape == (4, 2, 15, 2 + 4) and stats.dtype == torch.float32
         dqkv, dtable = n.position_attention_backward(o, qkv, o, stats, 2, 0.2, table, b, [1, 3, 5], None, [], [True, False])
         assert dqkv.shape == qkv.shape and dtable.shape == (0,)
         x = torch.empty(2, 1, 6, 10, 8, requires_grad=True)

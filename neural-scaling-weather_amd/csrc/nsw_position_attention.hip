@@ -9,10 +9,11 @@
 // Windows of up to 192 tokens (fewer with 256-byte rows) go through whole_kernel, whose waves
 // hold a row's logits with all keys; longer ones through forward_kernel, which steps over key
 // tiles with the running maximum m and sum of each row, so any length goes (180 x 360 x 1024 of
-// 9 x 18 windows, bf16: 142 us against 210, of them 105 for the bytes at a copy's rate).
+// 9 x 18 windows, bf16: 142 us against 210 when this was chosen, 105 for the bytes at a copy's
+// rate; 155 with the lost bits in the statistics).
 // S^T = K Q^T puts a query on a lane, whose probabilities are then the right operand of
-// O^T = V^T P^T as they lie.  Logits in units of log2 e (the factor is in the scale and in the bias's LDS copy), so
-// that a probability is one subtraction and exp2.  fp32 statistics and sums; bf16: probabilities
+// O^T = V^T P^T as they lie.  Logits in units of log2 e (the factor is in the scale and in the
+// bias's LDS copy), so that a probability is one subtraction and exp2.  fp32 statistics and sums; bf16: probabilities
 // (at most 1) are rounded to bf16 for the product with v, and their sum is of the rounded
 // ones, by a product with ones on the matrix units (the gradients' sum, in stats, is not).  stats
 // keeps m and log2 of the sum apart, since their sum would lose the second where |m| is large.
@@ -52,7 +53,9 @@ template <typename T, int HD, int NKB> struct Whole {
 // one multiply-add and exp2: off by an ulp of the row's maximum, far below the rounding of p to
 // bf16.  Otherwise the biases are added as the backward adds them.  k and v lie in LDS, loaded
 // while the window before is computed, in a second buffer where it fits (one barrier a window).
-// Four waves with three blocks of queries each, biases looked up: 185 us where this takes 142.
+// Four waves with three blocks of queries each, biases looked up: 185 us where this took 142.
+// 6,400 windows of 162 tokens and one head in 155 us: 572 MB at 3.7 TB/s (a copy: 5.1), vector
+// instructions 53 us of issue, matrix units 24, three waves a SIMD.
 template <typename T, int HD, int NKB, bool MASK>
 __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) {
   typedef Dim<T, HD> D;
@@ -193,8 +196,9 @@ constexpr int WAVES = 8;                                           // of forward
 constexpr int64_t MOST_BLOCKS = 1 << 23;                           // a launch has fewer than 2^32 lanes
 
 // A workgroup takes 128 queries of a (window, head) over 64-key tiles, the next tile in
-// registers meanwhile, two workgroups a compute unit (1999 tokens, 8 heads of 64, bf16: 45 us;
-// 64 queries in four waves 52, four waves of 32 queries 78).
+// registers meanwhile, two workgroups a compute unit (2 x 1999 tokens, 8 heads of 64, bf16: 45 us
+// where four waves of 32 queries took 78; 55 with the unrounded sums and lost bits, 0.3 PFLOP/s,
+// bound by vector instructions: a bias, a logit, a maximum, exp2 and a sum for each pair).
 template <typename T, int HD, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, 2) void forward_kernel(Args a) {
   typedef Dim<T, HD> D;

@@ -86,6 +86,10 @@ template <typename T, int HD, int WAVES> struct Windows {
   static constexpr size_t LDS = TILES + 2 * 4 * QT * sizeof(float);
 };
 
+// 180 x 360 x 1024 of 9 x 18 windows, 16 heads, bf16: 470-490 us, 1.3 GB at 2.8 TB/s, five
+// products at 0.22 PFLOP/s.  One workgroup of twelve waves a compute unit; vector instructions
+// 115 us of issue, matrix units 56, the rest LDS reads (with conflicts of the transposing reads)
+// and the barrier of each 32-query step.
 template <typename T, int HD, int WAVES, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) {
   typedef Dim<T, HD> D;
@@ -280,6 +284,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
 template <typename T, int HD>
 constexpr size_t keys_lds() { return 2 * (2 * QT * Dim<T, HD>::STR * sizeof(T) + 4 * QT * sizeof(float)); }
 
+// dk, dv and the sums of dz of 64 KB keys of a head, its windows in turn, over 32-query tiles in two
+// buffers; two workgroups a compute unit (two frames of 90 x 180 x 512, 8 heads, with a mask, bf16:
+// 848 us with one, 262 with two; 2 x 1999 tokens 158).  Bound by vector instructions and, with
+// few keys a window, by the reading and writing of the sums.
 // 512-byte rows: one workgroup a compute unit rather than 129 registers in memory (8 windows of
 // 20 x 25 with 8 heads of 128, fp32: the pass 423 -> 360 us).
 template <typename T, int HD, int KB, bool MASK>
@@ -441,7 +449,8 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
 
 constexpr int WQ = 8, QKT = 64;                                    // of queries_kernel: waves of 16 queries, keys of a tile
 
-// dq of 128 queries of a (window, head), over key tiles, as the forward pass.
+// dq of 128 queries of a (window, head), over key tiles, as the forward pass (two frames of 90 x 180
+// x 512, bf16: 138 us where four waves of 32 queries took 158; 2 x 1999 tokens 54 against 69).
 template <typename T, int HD, bool MASK>
 __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void queries_kernel(Args a) {
   typedef Dim<T, HD> D;
@@ -556,7 +565,8 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
 struct Shares { int queries, parts, qshares, shares; };
 
 // out[h, y, r] = sum over the pairs of displacement r whose query lies in share y's queries, and
-// over its parts: a lane a displacement, neighbours on neighbouring keys, eight queries at a time.
+// over its parts: a lane a displacement, neighbours on neighbouring keys, eight queries at a time
+// (2 x 1999 tokens, 8 heads: 256 MB in 69 us; sixteen at a time measured the same).
 __global__ __launch_bounds__(NT) void pairs_kernel(Args a, float* __restrict__ out, Shares sh) {
   constexpr int U = 8;
   const int r = (int)blockIdx.x * NT + (int)threadIdx.x, h = (int)blockIdx.y, y = (int)blockIdx.z;
@@ -657,7 +667,7 @@ void set_parts(Args& a, int waves, int keys) {
 }
 
 // Shares of pairs_kernel: up to 32 of the queries, and, while that is fewer than 1024 workgroups,
-// of the parts, 64 in all (2048 windows of 7x7, two heads, 256 parts: the pass 183 -> 119 us).
+// of the parts, 64 in all (2048 windows of 7x7, four heads, 256 parts: the pass 183 -> 119 us).
 Shares shares_of(const Args& a) {
   const int64_t others = (int64_t)((a.R + NT - 1) / NT) * a.heads;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(32, 2048 / others));

@@ -18,7 +18,7 @@
 //
 // Large samples: workgroups leave partial sums, a second kernel joins them, a third
 // reads x again, in the opposite order of rows, so that the rows read last are still in
-// the cache.  Samples of at most SMALL bytes: one workgroup each, one launch.
+// the cache.  Small samples: one workgroup each, one launch.
 #include <algorithm>
 #include <cmath>
 
@@ -30,7 +30,6 @@ namespace nsw {
 namespace {
 
 constexpr int NT = 256;            // threads of a workgroup
-constexpr int64_t SMALL = 96 << 10;
 constexpr int64_t MOST_BLOCKS = 1 << 22;   // of the kernels that loop over groups or columns of all samples: a launch has fewer than 2^32 lanes
 
 struct GnArgs {
@@ -520,16 +519,23 @@ struct Plan {
   int64_t per;
 };
 
+// Bytes of a sample up to which one workgroup takes it: more of them where there are workgroups
+// for all compute units.  One workgroup against several, us of the forward and the backward pass, bf16,
+// C = 192: one sample of 48 KB 12.4 + 15.6 and 15.5 + 14.8, of 96 KB 15.8 + 23.4 and 15.7 + 15.0; 128 of 96 KB
+// 17.8 + 26.9 and 21.4 + 24.4, of 192 KB 29.8 + 52.6 and 26.4 + 36.2; 256 of 192 KB 33 + 56 and 37 + 57.
+int64_t small_of(int64_t B) { return (B >= 256 ? 192 : B >= 128 ? 96 : 64) << 10; }
+
 Plan plan(int64_t B, int64_t R, int64_t C, int dtype, int per_cu) {
   const int64_t es = (int64_t)dtype_size(dtype), CV = C * es / 16;
   const int RL = (int)std::max<int64_t>(1, NT / CV);
-  if (R * C * es <= SMALL) return {RL, 1, R};
+  if (R * C * es <= small_of(B)) return {RL, 1, R};
   const int64_t turns = (R + 8 * RL - 1) / (8 * RL);
   const int64_t want = std::max<int64_t>(2, (256 * per_cu + B - 1) / B);
   const int64_t each = std::max<int64_t>(1, (turns + want - 1) / want);
   return {RL, (int)((turns + each - 1) / each), each * 8 * RL};
 }
 
+// Workgroups a compute unit: few where each leaves sums to be joined, many where it only writes rows.
 constexpr int STATS_PER_CU = 2, APPLY_PER_CU = 16;
 
 GnArgs common(int64_t B, int64_t R, int64_t C, int64_t G, int dtype, float eps) {

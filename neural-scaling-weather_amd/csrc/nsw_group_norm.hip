@@ -66,12 +66,6 @@ struct Place {
   __device__ __forceinline__ int col(int k) const { return (cv0 + NT * k) * VEC; }
 };
 
-template <int ACT>
-__device__ __forceinline__ float act_of(float n) {
-  if constexpr (ACT == NSW_ACT_NONE) return n;
-  else return gate_act<float, ACT>(n);
-}
-
 // act of a result that is rounded to T
 template <typename T, int ACT>
 __device__ __forceinline__ float act_for(float n) {

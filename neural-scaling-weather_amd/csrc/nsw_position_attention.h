@@ -26,7 +26,7 @@ struct Args {
   int L, C, heads, hd, R, off, nb;
   int TW, A, W;                     // extent of a window (frames are the outermost)
   int nqc;                          // workgroups that share a window's queries (keys in the backward pass)
-  int NP;                           // backward: workgroups that share a head's windows
+  int NP;                           // workgroups that share a head's windows
   int band0, thr;                   // shift mask: first window of the last band (none: nW), its first row of the other class
   float scale;
   FastDiv dAW, dW, dheads, dnqc;
@@ -228,8 +228,7 @@ __device__ __forceinline__ void load_rel(const Args& a, int head, float* rel) {
 }
 
 // A tile of ROWS rows of HD values from memory by way of registers: load() and later store()
-// into LDS.  By NT threads, a
-// workgroup's or four waves of a larger one.
+// into LDS, by NT threads, a workgroup's or four waves of a larger one.
 template <typename T, int HD, int ROWS, int NT = posattn::NT>
 struct TileCopy {
   typedef Dim<T, HD> D;
@@ -253,7 +252,7 @@ struct TileCopy {
 };
 
 // D = do o of the gradients cancels against do v, and the rounding of o to bf16 would be most of
-// its error (dtable 2.5e-3 off where its own rounding is 1.7e-3).  The forward pass therefore
+// dz's error (dtable 2.5e-3 off where its own rounding is 1.7e-3).  The forward pass therefore
 // leaves, behind a row's statistics, what each value of o lost, in sixteenths of a step and 4
 // bits: a quarter of o's bytes.  A step is 2^16 of fp32's pattern, whatever the exponent: the
 // difference of the two patterns is rounded to 2^12, -7 .. 6 of it are written as 1 .. 14, so that

@@ -48,20 +48,21 @@ template <typename T, int HD, int NKB> struct Whole {
 
 // Windows of up to 16 NKB tokens of one head in turn.  A wave owns 16 queries and holds their
 // logits with all keys, so that a row's maximum is known before its probabilities are formed,
-// and, as the pairs are the same in every window, their biases too.  bf16 without a mask: the
-// products start from the biases divided by the scale (which is positive), and a probability is
-// one multiply-add and exp2: off by an ulp of the row's maximum, far below the rounding of p to
-// bf16.  Otherwise the biases are added as the backward adds them.  k and v lie in LDS, loaded
+// and, as the pairs are the same in every window, their biases too.  Logits are whole before the
+// maximum is taken from them, so that the difference at the maximum is exactly 0 however large
+// a bias is (products that start from the biases over the scale, a probability one multiply-add:
+// infinite or 0 at biases of 1e10, and no faster, 154 us against 155).  k and v lie in LDS, loaded
 // while the window before is computed, in a second buffer where it fits (one barrier a window).
 // Four waves with three blocks of queries each, biases looked up: 185 us where this took 142.
 // 6,400 windows of 162 tokens and one head in 155 us: 572 MB at 3.7 TB/s (a copy: 5.1), vector
-// instructions 53 us of issue, matrix units 24, three waves a SIMD.
+// instructions 53 us of issue, matrix units 24, three waves a SIMD.  (The shift is added to whole
+// logits: added to the biases, two sets of them live at once, and the registers that go to
+// memory make it 275 us.)
 template <typename T, int HD, int NKB, bool MASK>
 __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) {
   typedef Dim<T, HD> D;
   typedef Whole<T, HD, NKB> X;
   constexpr int N = 64 * NKB;
-  constexpr bool START = !MASK && sizeof(T) == 2;                  // the products start from the biases
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* KVs = (T*)smem;                                               // [BUFS][k rows, v rows]
   int* kinfo = (int*)(smem + X::BUFS * X::KV);                     // [2][KEYS]: without and with the shift's classes
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int L = a.L, query = 16 * wave + fr;
   const bool queries = 16 * wave < L;
-  const float zs = a.scale * LOG2E, shift = START ? -100.f / a.scale : -100.f * LOG2E;
+  const float zs = a.scale * LOG2E;
 
   TileCopy<T, HD, X::KEYS, N> kc, vc;
   typename D::Frag qn[D::NS];
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
     const int4 k = *reinterpret_cast<const int4*>(kinfo + 16 * kb + 4 * fg);
     bias[kb] = biases({qi, qi, qi, qi}, {k.x, k.y, k.z, k.w}, false);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) bias[kb][r] = 16 * kb + 4 * fg + r < L ? (START ? bias[kb][r] / zs : bias[kb][r]) : -INFINITY;
+    for (int r = 0; r < 4; ++r) bias[kb][r] = 16 * kb + 4 * fg + r < L ? bias[kb][r] : -INFINITY;
   }
 
   int turn = 0;
@@ -126,15 +127,21 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
     f32x4 S[NKB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) {
-      S[kb] = START ? bias[kb] : f32x4{0.f, 0.f, 0.f, 0.f};
+      S[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < D::NS; ++s) S[kb] = mma(row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg), q[s], S[kb]);
+      logits(S[kb], zs, bias[kb]);
     }
-    if constexpr (!START)
+    if (shifted) {
+      const int qc = info_of(a, query, true);
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
+      for (int kb = 0; kb < NKB; ++kb) {
+        const int4 k = *reinterpret_cast<const int4*>(kinfo + X::KEYS + 16 * kb + 4 * fg);
+        const int kn[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[kb][r] = fmaf(S[kb][r], zs, bias[kb][r]);
+        for (int r = 0; r < 4; ++r) S[kb][r] += ((qc ^ kn[r]) >> 30 ? -100.f * LOG2E : 0.f);
+      }
+    }
     if constexpr (MASK) {
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
@@ -142,29 +149,20 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[kb][r] += mask_units(m4[r]);
       }
-    } else if (shifted) {
-      const int qc = info_of(a, query, true);
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        const int4 k = *reinterpret_cast<const int4*>(kinfo + X::KEYS + 16 * kb + 4 * fg);
-        const int kn[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[kb][r] += (qc ^ kn[r]) >> 30 ? shift : 0.f;
-      }
     }
     float mx = S[0][0];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) mx = fmaxf(mx, S[kb][r]);
-    mx = rows4_max(mx) * (START ? zs : 1.f);
-    const float to = mx == -INFINITY ? 0.f : -mx;
+    mx = rows4_max(mx);
+    const float to = mx == -INFINITY ? 0.f : mx;
     float l = 0.f;
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        S[kb][r] = __builtin_amdgcn_exp2f(START ? fmaf(S[kb][r], zs, to) : S[kb][r] + to);
+        S[kb][r] = __builtin_amdgcn_exp2f(S[kb][r] - to);
         l += S[kb][r];
       }
     f32x4 O[D::ND], Z = {0.f, 0.f, 0.f, 0.f};
@@ -355,15 +353,12 @@ template <typename T, int HD> constexpr int MOST_WHOLE = HD * (int)sizeof(T) >= 
 
 template <typename T, int HD>
 int launch_hd(const Args& a, hipStream_t st) {
-  // whole_kernel may divide the biases by the scale: that neither overflows nor loses them
-  if (sizeof(T) == 4 || a.mask != nullptr || (a.scale >= 1e-6f && a.scale <= 1e6f)) {
-    if (a.L <= 64) return launch_whole<T, HD, 4>(a, st);
-    if constexpr (MOST_WHOLE<T, HD> >= 2)
-      if (a.L <= 128) return launch_whole<T, HD, 8>(a, st);
-    if constexpr (MOST_WHOLE<T, HD> >= 3) {
-      if (a.L <= 176) return launch_whole<T, HD, 11>(a, st);
-      if (a.L <= 192) return launch_whole<T, HD, 12>(a, st);
-    }
+  if (a.L <= 64) return launch_whole<T, HD, 4>(a, st);
+  if constexpr (MOST_WHOLE<T, HD> >= 2)
+    if (a.L <= 128) return launch_whole<T, HD, 8>(a, st);
+  if constexpr (MOST_WHOLE<T, HD> >= 3) {
+    if (a.L <= 176) return launch_whole<T, HD, 11>(a, st);
+    if (a.L <= 192) return launch_whole<T, HD, 12>(a, st);
   }
   return launch_long<T, HD>(a, st);
 }

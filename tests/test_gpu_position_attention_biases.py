@@ -1,0 +1,74 @@
+"""nsw.ops.position_attention with table entries far from zero, as a table holds them for
+displacements that take no part, against the formula in float64 on logits rounded to fp32 as
+fp32 forms them (half an fp32 step at 1e8 and beyond is larger than the products here, a sixteenth
+of a case's, so that a row of such entries alone is uniform).
+
+Tolerances: those of test_gpu_position_attention, a logit's error e without the far
+entry's share.  Entries of one far value cancel exactly in the difference to the row's maximum
+where the row has no other, and have p = 0 exactly where it has (the next logit is more than
+200 away)."""
+import math
+
+import pytest
+import torch
+
+import nsw
+from nsw import ops
+
+from test_gpu_position_attention import DTYPES, U, case, check, pairs, run
+
+pytestmark = pytest.mark.gpu
+
+
+def far_case(dtype, Bw, extent, heads, hd, far, which, seed=20):
+    """A case whose table is `far` at every displacement ("all"), or where the query is not behind the key
+    ("causal": the first token's row has nothing else)."""
+    t = case(dtype, Bw, extent, heads, hd, seed=seed)
+    middle = t["table"].shape[0] // 2
+    t["qkv"][..., :2 * heads * hd] *= 0.25
+    t["table"][:None if which == "all" else middle + 1] = far
+    return t
+
+
+def reference(t, far):
+    """{name: (value, tolerance before the last rounding)} in float64, and the row's maximum and log2 of its sum."""
+    dtype, heads = t["qkv"].dtype, t["heads"]
+    h = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    far = t["table"].new_tensor(far).double()
+    Bw, L, C3 = t["qkv"].shape
+    hd = C3 // 3 // heads
+    q, k, v = t["qkv"].double().view(Bw, L, 3, heads, hd).permute(2, 0, 3, 1, 4)
+    rel = t["table"].double()[t["buckets"].long()]
+    idx = pairs(*t["extent"])
+    bias = rel[idx].permute(2, 0, 1)
+    z = (t["scale"] * q @ k.mT + bias).float().double()
+    e = (hd + 6) * U * (abs(t["scale"]) * q.abs() @ k.abs().mT + torch.where(bias == far, 0.0, bias.abs()))
+    top = z.amax(-1, keepdim=True)
+    p = (z - top).exp()
+    total = p.sum(-1, keepdim=True)
+    p = p / total
+    far_off = torch.where(p > 0, z - top, 0.0).abs()
+    f = 2 * (e + e.amax(-1, keepdim=True)) + 8 * U * (1 + far_off) + (L + 8) * U
+    flat = lambda x: x.transpose(1, 2).reshape(Bw, L, -1)
+    out = {"o": (flat(p @ v), flat((p * (f + h + L * U)) @ v.abs()))}
+    return out, top[..., 0] * math.log2(math.e), total[..., 0].log2(), f.amax(-1)
+
+
+FAR = [-1e8, -1e10, -1e30, -1e38, 1e10, 1e30]
+EXTENTS = [(1, 1, 1), (1, 3, 5), (1, 1, 70), (1, 9, 18), (1, 12, 16), (2, 9, 18)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extent", EXTENTS)
+@pytest.mark.parametrize("which", ["all", "causal"])
+@pytest.mark.parametrize("far", FAR)
+def test_forward(device, dtype, extent, which, far):
+    """A row of far entries alone is a mean of v, neither zeros nor NaN."""
+    for hd in (32, 64):
+        t = far_case(dtype, 3, extent, 2, hd, far, which)
+        got = run(t, device)
+        want, top, total, f = reference(t, far)
+        check(got, want, dtype)
+        stats = got["stats"].double().cpu()
+        assert ((stats[..., 0] - top).abs() <= 8 * U * top.abs() + f).all()
+        assert ((stats[..., 1] - total).abs() <= 2 * f + 4 * U * total).all()

@@ -36,17 +36,13 @@ namespace {
 
 constexpr int QT = 32;              // queries of a tile
 
-// Row statistics of a tile's queries as the kernels use them: p = exp2(z - m - l), both in
-// m where no mask can make m large; rows without keys, or past the window, p = 0.
-template <bool MASK>
+// Row statistics of a tile's queries as the kernels use them: p = exp2(z - m - l), not of one
+// sum m + l, which would lose l where a mask or a bias makes |m| large; rows without keys, or
+// past the window, p = 0.
 __device__ __forceinline__ void put_stats(const f32x2& st, float* mrow, float* lrow) {
   const bool none = st[0] == -INFINITY;
-  if constexpr (MASK) {
-    *mrow = none ? INFINITY : st[0];
-    *lrow = none ? 0.f : st[1];
-  } else {
-    *mrow = none ? INFINITY : st[0] + st[1];
-  }
+  *mrow = none ? INFINITY : st[0];
+  *lrow = none ? 0.f : st[1];
 }
 
 // Statistics of query q0 + i of a window, of n queries from q0 on; none behind them.
@@ -59,11 +55,10 @@ __device__ __forceinline__ f32x2 load_stats(const Args& a, int64_t win, int head
 }
 
 // p and dz of four pairs from their products: s = q k, g = do v.
-template <bool MASK>
 __device__ __forceinline__ void weigh(f32x4& s, f32x4& g, const f32x4& m, const f32x4& l, const f32x4& d) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    s[r] = __builtin_amdgcn_exp2f(MASK ? s[r] - m[r] - l[r] : s[r] - m[r]);
+    s[r] = __builtin_amdgcn_exp2f(s[r] - m[r] - l[r]);
     g[r] = s[r] * (g[r] - d[r]);
   }
 }
@@ -153,7 +148,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
     }
     if (tid < QT) {
       ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + rel_base(a, rel);
-      put_stats<MASK>(st, r + QT + tid, r + 2 * QT + tid);
+      put_stats(st, r + QT + tid, r + 2 * QT + tid);
     }
   };
 
@@ -217,7 +212,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
           const f32x4 m4 = *reinterpret_cast<const f32x4*>(r0 + QT + 16 * qb + 4 * fg);
-          const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg) : m4;
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg);
           const f32x4 d4 = *reinterpret_cast<const f32x4*>(r0 + 3 * QT + 16 * qb + 4 * fg);
           logits(P[qb], zs, B[qb]);
           if constexpr (MASK) {
@@ -230,7 +225,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
             if (key >= L) P[qb] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             asm volatile("" : "+v"(P[qb]));                        // a branch of these waves, no selects of all
           }
-          weigh<MASK>(P[qb], Z[qb], m4, l4, d4);
+          weigh(P[qb], Z[qb], m4, l4, d4);
           if (alone) {
             Z[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
             asm volatile("" : "+v"(Z[qb]));
@@ -333,7 +328,7 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
       row_dots(gc, oc, lost, r + 3 * QT);
       if (tid < QT) {
         ((int*)r)[tid] = info_of(a, QT * step + tid, shifted) + rel_base(a, rel);
-        put_stats<MASK>(st, r + QT + tid, r + 2 * QT + tid);
+        put_stats(st, r + QT + tid, r + 2 * QT + tid);
       }
     };
     load_tile(0);
@@ -388,7 +383,7 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
           }
         }
         const f32x4 m4 = *reinterpret_cast<const f32x4*>(r0 + QT + 16 * qb + 4 * fg);
-        const f32x4 l4 = MASK ? *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg) : m4;
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg);
         const f32x4 d4 = *reinterpret_cast<const f32x4*>(r0 + 3 * QT + 16 * qb + 4 * fg);
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
@@ -411,7 +406,7 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
             if (key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             asm volatile("" : "+v"(P[qb][b]));                     // a branch of these waves, no selects of all
           }
-          weigh<MASK>(P[qb][b], Z[qb][b], m4, l4, d4);
+          weigh(P[qb][b], Z[qb][b], m4, l4, d4);
           if (bias) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sums.put(q0 + 16 * qb + 4 * fg + r, key, old[b][r] + Z[qb][b][r]);
@@ -481,7 +476,7 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
   typename D::Frag q[D::NS], g[D::NS];
   const int qinfo = info_of(a, query, shifted) + rel_base(a, rel);
   const float zs = a.scale * LOG2E;
-  float m, l = 0.f, dot = 0.f;
+  float m, l, dot = 0.f;
 #pragma unroll
   for (int s = 0; s < D::NS; ++s) {
     q[s] = row_frag<T, HD>(qrows, (uint32_t)query, s, fg, a.hd);
@@ -499,7 +494,7 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
     }
   }
   dot = rows4_sum(dot);
-  put_stats<MASK>(load_stats(a, win, head, 0, L, query), &m, &l);
+  put_stats(load_stats(a, win, head, 0, L, query), &m, &l);
   const f32x4 m4 = {m, m, m, m}, l4 = {l, l, l, l}, d4 = {dot, dot, dot, dot};
   f32x4 O[D::ND];
 #pragma unroll
@@ -543,7 +538,7 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
             for (int r = 0; r < 4; ++r)
               if (k + 4 * fg + r >= left) s4[r] = -INFINITY;
           }
-          weigh<MASK>(s4, g4, m4, l4, d4);
+          weigh(s4, g4, m4, l4, d4);
           Z[kb] = g4;
         }
         const typename D::TFrag zf = pair_frag<T>(Z[0], Z[1]);

@@ -12,9 +12,6 @@ import math
 import pytest
 import torch
 
-import nsw
-from nsw import ops
-
 from test_gpu_position_attention import DTYPES, U, case, check, pairs, run
 
 pytestmark = pytest.mark.gpu
@@ -50,7 +47,25 @@ def reference(t, far):
     far_off = torch.where(p > 0, z - top, 0.0).abs()
     f = 2 * (e + e.amax(-1, keepdim=True)) + 8 * U * (1 + far_off) + (L + 8) * U
     flat = lambda x: x.transpose(1, 2).reshape(Bw, L, -1)
-    out = {"o": (flat(p @ v), flat((p * (f + h + L * U)) @ v.abs()))}
+    o, do = p @ v, t["do"].double().view(Bw, L, heads, hd).transpose(1, 2)
+    to = (p * (f + h + L * U)) @ v.abs()
+    out = {"o": (flat(o), flat(to))}
+    stored = to + (o.abs() + to) * (h / 4 if h else U)
+    dp, D = do @ v.mT, (do * o).sum(-1, keepdim=True)
+    err = hd * U * (do.abs() @ v.abs().mT) + (do.abs() * (stored + hd * U * o.abs())).sum(-1, keepdim=True)
+    dz = p * (dp - D)
+    if L == 1:
+        dz, err = dz * 0, err * 0
+    tz = p * err + f * dz.abs()
+    wide = tz + (h + L * U) * (dz.abs() + tz)
+    sc = abs(t["scale"])
+    dq = (t["scale"] * dz @ k, sc * wide @ k.abs())
+    dk = (t["scale"] * dz.mT @ q, sc * wide.mT @ q.abs())
+    dv = (p.mT @ do, (p * (f + h + L * U)).mT @ do.abs())
+    out["dqkv"] = tuple(torch.cat([flat(x[i]) for x in (dq, dk, dv)], -1) for i in (0, 1))
+    add = lambda x: torch.zeros(rel.shape, dtype=torch.float64).index_add_(0, t["buckets"].long()[idx].reshape(-1),
+                                                                          x.sum(0).reshape(heads, L * L).T)
+    out["dtable"] = (add(dz), add(tz + (64 + Bw * L) * U * (dz.abs() + tz)))
     return out, top[..., 0] * math.log2(math.e), total[..., 0].log2(), f.amax(-1)
 
 
@@ -68,7 +83,18 @@ def test_forward(device, dtype, extent, which, far):
         t = far_case(dtype, 3, extent, 2, hd, far, which)
         got = run(t, device)
         want, top, total, f = reference(t, far)
-        check(got, want, dtype)
+        check(got, {"o": want["o"]}, dtype)
         stats = got["stats"].double().cpu()
         assert ((stats[..., 0] - top).abs() <= 8 * U * top.abs() + f).all()
         assert ((stats[..., 1] - total).abs() <= 2 * f + 4 * U * total).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extent", EXTENTS)
+@pytest.mark.parametrize("which", ["all", "causal"])
+@pytest.mark.parametrize("far", FAR)
+def test_gradients(device, dtype, extent, which, far):
+    """Probabilities formed again from statistics whose maximum is far from zero."""
+    for hd in (32, 64):
+        t = far_case(dtype, 3, extent, 2, hd, far, which)
+        check(run(t, device), reference(t, far)[0], dtype)

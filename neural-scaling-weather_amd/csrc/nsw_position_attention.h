@@ -69,11 +69,13 @@ __device__ __forceinline__ void logits(f32x4& s, float zs, const f32x4& bias) {
   for (int r = 0; r < 4; ++r) s[r] = fmaf(s[r], zs, bias[r]);
 }
 
-// A mask value times log2 e: the lowest floats stay finite, so that a row of them is uniform, as
-// in fp32 on the formula.
-__device__ __forceinline__ float mask_units(float m) {
-  const float v = m * LOG2E;
-  return v == -INFINITY && m != -INFINITY ? -3.402823466e38f : v;
+// A value of a mask or table times log2 e: finite ones stay finite (2.36e38 and what lies beyond
+// become the largest float), so that a row of the lowest or the highest floats is uniform, as in
+// fp32 on the formula.
+__device__ __forceinline__ float in_units(float x) {
+  constexpr float MOST = 3.402823466e38f;
+  const float v = x * LOG2E;
+  return fabsf(x) <= MOST ? __builtin_amdgcn_fmed3f(v, -MOST, MOST) : v;
 }
 
 // ------------------------------------------------------------- fragments ---
@@ -223,7 +225,7 @@ template <typename T>
 __device__ __forceinline__ void load_rel(const Args& a, int head, float* rel) {
   for (int r = (int)threadIdx.x; r < a.R; r += (int)blockDim.x) {
     const int b = a.buckets[r];
-    rel[r] = (unsigned)b < (unsigned)a.nb ? to_f32(((const T*)a.table)[(int64_t)b * a.heads + head]) * LOG2E : 0.f;
+    rel[r] = (unsigned)b < (unsigned)a.nb ? in_units(to_f32(((const T*)a.table)[(int64_t)b * a.heads + head])) : 0.f;
   }
 }
 

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
       for (int kb = 0; kb < NKB; ++kb) {
         const f32x4 m4 = mask.get4(query, 16 * kb + 4 * fg);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[kb][r] += mask_units(m4[r]);
+        for (int r = 0; r < 4; ++r) S[kb][r] += in_units(m4[r]);
       }
     }
     float mx = S[0][0];
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void forward_kernel(Args a) {
           if constexpr (MASK) {
             const f32x4 m4 = mask.get4(query, k0 + 16 * kb + 4 * fg);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[kb][r] += mask_units(m4[r]);
+            for (int r = 0; r < 4; ++r) S[kb][r] += in_units(m4[r]);
           }
           if (decltype(tail)::value && 16 * kb + 16 > left) {
 #pragma unroll

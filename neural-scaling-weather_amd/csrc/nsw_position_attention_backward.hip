@@ -218,7 +218,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              P[qb][r] += mask_units(mask.get(QT * step + 16 * qb + 4 * fg + r, key));
+              P[qb][r] += in_units(mask.get(QT * step + 16 * qb + 4 * fg + r, key));
             }
           }
           if (16 * wave + 16 > L) {
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
           logits(P[qb][b], zs, B[b]);
           if constexpr (MASK) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) P[qb][b][r] += mask_units(M[b][r]);
+            for (int r = 0; r < 4; ++r) P[qb][b][r] += in_units(M[b][r]);
           }
           if (kw + 16 * b + 16 > L) {
             if (key >= L) P[qb][b] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
           if constexpr (MASK) {
             const f32x4 x = mask.get4(query, k0 + k + 4 * fg);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s4[r] += mask_units(x[r]);
+            for (int r = 0; r < 4; ++r) s4[r] += in_units(x[r]);
           }
           if (decltype(tail)::value && k + 16 > left) {
 #pragma unroll

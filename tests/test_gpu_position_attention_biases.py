@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from test_gpu_position_attention import DTYPES, U, case, check, pairs, run
+from test_gpu_position_attention import reference as masked_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,28 @@ def test_gradients(device, dtype, extent, which, far):
     for hd in (32, 64):
         t = far_case(dtype, 3, extent, 2, hd, far, which)
         check(run(t, device), reference(t, far)[0], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extent", EXTENTS)
+@pytest.mark.parametrize("which", ["all", "causal"])
+@pytest.mark.parametrize("far", ["lowest", "highest", -2.4e38, 2.4e38])
+def test_the_largest_table_values(device, dtype, extent, which, far):
+    """Finite values whose product with log2 e is not: they stay what they are among others, and uniform by themselves."""
+    far = {"lowest": torch.finfo(dtype).min, "highest": torch.finfo(dtype).max}.get(far, far)
+    t = far_case(dtype, 3, extent, 2, 32, far, which)
+    check(run(t, device), reference(t, far)[0], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extent", [e for e in EXTENTS if math.prod(e) > 1])
+@pytest.mark.parametrize("high", [torch.finfo(torch.float32).max, 2.4e38])
+def test_the_largest_mask_values(device, dtype, extent, high):
+    """The keys that a mask lifts above all others share a row's weight."""
+    t = case(dtype, 4, extent, 2, 32, seed=21)
+    L = math.prod(extent)
+    m = torch.zeros(2, L, L)
+    m[0, L // 2, :L // 2 + 1] = high
+    m[1, :, L // 3] = high
+    m[1, L - 1] = -math.inf
+    check(run(t, device, mask=m), masked_reference(t, m), dtype)

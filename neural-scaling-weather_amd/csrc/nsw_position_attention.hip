@@ -148,6 +148,11 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
         const f32x4 m4 = mask.get4(query, 16 * kb + 4 * fg);
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[kb][r] += in_units(m4[r]);
+        if (16 * kb + 16 > L) {                                    // past the window the next query's values were read
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * kb + 4 * fg + r >= L) S[kb][r] = -INFINITY;
+        }
       }
     }
     float mx = S[0][0];

@@ -342,7 +342,7 @@ int launch_long(Args a, hipStream_t st) {
 template <typename T, int HD, int NKB>
 int launch_whole(Args a, hipStream_t st) {
   typedef Whole<T, HD, NKB> X;
-  const int64_t all = 256 * (16 / NKB);                            // as many as run at once
+  const int64_t all = 256 * (16 / NKB);                            // four waves to a SIMD, where the LDS holds as many
   const int64_t want = std::max<int64_t>(1, all / a.heads), each = (a.Bw + want - 1) / want;
   a.NP = (int)((a.Bw + each - 1) / each);
   const dim3 grid((unsigned)(a.NP * a.heads)), block(64 * NKB);

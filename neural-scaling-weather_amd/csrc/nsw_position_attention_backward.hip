@@ -649,14 +649,14 @@ int waves_of(int L) {
 // 16-key blocks of a wave of keys_kernel.
 template <typename T, int HD> constexpr int KEY_BLOCKS = HD * (int)sizeof(T) >= 256 ? 1 : 2;
 
-// Workgroups that share a head's windows: as many as run at once in all (windows_kernel: four
-// waves to a SIMD or one workgroup to a compute unit; keys_kernel: two workgroups), each with the
-// same number of windows as near as can be.  keys_kernel: at most 2 GiB of sums, too.
+// Workgroups that share a head's windows, one at least: in all 256 times four of 4 waves, two of 8
+// or one of 12 (windows_kernel; where the LDS holds fewer, from 128-byte rows on, the others
+// then follow) or two (keys_kernel), each with the same number of windows as near as can be.
+// Their sums of dz: 1 GiB at most, or heads L^2 floats where that is more.
 void set_parts(Args& a, int waves, int keys) {
   a.nqc = waves ? 1 : (a.L + keys - 1) / keys;
   const int64_t all = waves ? 256 * (16 / waves) : 512;
-  int64_t want = std::max<int64_t>(1, all / ((int64_t)a.heads * a.nqc));
-  if (!waves) want = std::max<int64_t>(1, std::min<int64_t>(want, (2LL << 30) / ((int64_t)a.heads * a.L * a.L * 4)));
+  const int64_t want = std::max<int64_t>(1, all / ((int64_t)a.heads * a.nqc));
   const int64_t Bw = std::max<int64_t>(a.Bw, 1), each = (Bw + want - 1) / want;
   a.NP = (int)((Bw + each - 1) / each);
 }

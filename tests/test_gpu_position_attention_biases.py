@@ -24,6 +24,8 @@ def far_case(dtype, Bw, extent, heads, hd, far, which, seed=20):
     t = case(dtype, Bw, extent, heads, hd, seed=seed)
     middle = t["table"].shape[0] // 2
     t["qkv"][..., :2 * heads * hd] *= 0.25
+    if abs(far) < 1e8:                          # half a step is less than a product: none at all
+        t["qkv"][..., :heads * hd] = 0
     t["table"][:None if which == "all" else middle + 1] = far
     return t
 
@@ -70,7 +72,7 @@ def reference(t, far):
     return out, top[..., 0] * math.log2(math.e), total[..., 0].log2(), f.amax(-1)
 
 
-FAR = [-1e8, -1e10, -1e30, -1e38, 1e10, 1e30]
+FAR = [-1e4, -1e6, 1e6, -1e8, -1e10, -1e30, -1e38, 1e10, 1e30]
 EXTENTS = [(1, 1, 1), (1, 3, 5), (1, 1, 70), (1, 9, 18), (1, 12, 16), (2, 9, 18)]
 
 

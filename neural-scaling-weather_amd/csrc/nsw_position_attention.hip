@@ -10,7 +10,7 @@
 // hold a row's logits with all keys; longer ones through forward_kernel, which steps over key
 // tiles with the running maximum m and sum of each row, so any length goes (180 x 360 x 1024 of
 // 9 x 18 windows, bf16: 142 us against 210 when this was chosen, 105 for the bytes at a copy's
-// rate; 155 with the lost bits in the statistics).
+// rate; 147 with the lost bits in the statistics).
 // S^T = K Q^T puts a query on a lane, whose probabilities are then the right operand of
 // O^T = V^T P^T as they lie.  Logits in units of log2 e (the factor is in the scale and in the
 // bias's LDS copy), so that a probability is one subtraction and exp2.  fp32 statistics and sums; bf16: probabilities
@@ -44,6 +44,7 @@ template <typename T, int HD, int NKB> struct Whole {
   static constexpr size_t KV = (size_t)2 * KEYS * Dim<T, HD>::STR * sizeof(T);
   static constexpr int BUFS = 2 * KV <= (128 << 10) ? 2 : 1;
   static constexpr size_t LDS = BUFS * KV + 2 * KEYS * sizeof(int);
+  static constexpr int END = NKB <= 4 ? 0 : NKB <= 8 ? 4 : NKB <= 11 ? 8 : 11;   // first block in which a window may end (launch_hd)
 };
 
 // Windows of up to 16 NKB tokens of one head in turn.  A wave owns 16 queries and holds their
@@ -51,13 +52,13 @@ template <typename T, int HD, int NKB> struct Whole {
 // and, as the pairs are the same in every window, their biases too.  Logits are whole before the
 // maximum is taken from them, so that the difference at the maximum is exactly 0 however large
 // a bias is (products that start from the biases over the scale, a probability one multiply-add:
-// infinite or 0 at biases of 1e10, and no faster, 154 us against 155).  k and v lie in LDS, loaded
+// infinite or 0 at biases of 1e10, and no faster, 154 us against 147).  k and v lie in LDS, loaded
 // while the window before is computed, in a second buffer where it fits (one barrier a window).
 // Four waves with three blocks of queries each, biases looked up: 185 us where this took 142.
-// 6,400 windows of 162 tokens and one head in 155 us: 572 MB at 3.7 TB/s (a copy: 5.1), vector
-// instructions 53 us of issue, matrix units 24, three waves a SIMD.  (The shift is added to whole
+// 6,400 windows of 162 tokens and one head in 147 us: 572 MB at 3.9 TB/s (a copy: 5.1), vector
+// instructions 56 us of issue, matrix units 24, three waves a SIMD.  The shift is added to whole
 // logits: added to the biases, two sets of them live at once, and the registers that go to
-// memory make it 275 us.)
+// memory make it 275 us.
 template <typename T, int HD, int NKB, bool MASK>
 __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) {
   typedef Dim<T, HD> D;
@@ -131,6 +132,9 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
 #pragma unroll
       for (int s = 0; s < D::NS; ++s) S[kb] = mma(row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg), q[s], S[kb]);
       logits(S[kb], zs, bias[kb]);
+      // block after block, which the registers hold (180 x 360 x 1024: 147 us, 160 in the compiler's order; with a
+      // mask its own order is the faster one, 274 against 305)
+      if constexpr (!MASK) __builtin_amdgcn_sched_barrier(0);
     }
     if (shifted) {
       const int qc = info_of(a, query, true);
@@ -148,12 +152,15 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
         const f32x4 m4 = mask.get4(query, 16 * kb + 4 * fg);
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[kb][r] += in_units(m4[r]);
-        if (16 * kb + 16 > L) {                                    // past the window the next query's values were read
+      }
+      // past the window the next query's values were read
+#pragma unroll
+      for (int kb = X::END; kb < NKB; ++kb)
+        if (16 * kb < L && 16 * kb + 16 > L) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (16 * kb + 4 * fg + r >= L) S[kb][r] = -INFINITY;
         }
-      }
     }
     float mx = S[0][0];
 #pragma unroll
@@ -353,7 +360,9 @@ int launch_whole(Args a, hipStream_t st) {
 }
 
 // Longest window of whole_kernel, in blocks of 64 tokens: what the LDS holds of k and v and the
-// registers of twelve waves of a row.
+// registers of twelve waves of a row.  Beyond 128 tokens 11 blocks of 16 where they suffice: what 12
+// need of registers goes to memory (400 windows of 162 tokens and 16 heads: head dim 64 147 us
+// against 163, 16 75 against 79, fp32 32 285 against 284, with a mask 342 against 430).
 template <typename T, int HD> constexpr int MOST_WHOLE = HD * (int)sizeof(T) >= 512 ? 1 : HD * (int)sizeof(T) >= 256 ? 2 : 3;
 
 template <typename T, int HD>

@@ -549,11 +549,11 @@ int nsw_group_norm_backward(const void* dy, const void* x, const float* stats, c
  * [Bw, num_heads, L, 2] fp32 receives each row's maximum m of z log2(e) and log2 of its sum of
  * 2^(z log2(e) - m); in bf16 [Bw, num_heads, L, 2 + ceil(hd / 8)], behind them 4 bits for each value
  * of o, the sixteenths of a step that its rounding lost, for the gradients.  k and v have to be
- * finite also where they are masked.  Finite table and mask values stay finite (of 2.36e38 and more: as that;
- * a sum of both past the largest float is infinite, as in fp32).  bf16: fp32 logits and sums, probabilities rounded to bf16 for the
- * product with v and their sum.  Head dims 4, 8, 16, 32, 64, 128; C a multiple of 8 below 2^18;
- * a window's rows of qkv below 2 GiB; Bw * num_heads below 2^31, and times ceil(L / 128) below
- * 2^23 where L > 64; qkv, o, stats 16-byte aligned. */
+ * finite also where they are masked.  Finite table and mask values stay finite (of 2.36e38 and
+ * more: as that; a sum of both past the largest float is infinite, as in fp32).  bf16: fp32 logits
+ * and sums, probabilities rounded to bf16 for the product with v and their sum.  Head dims 4, 8,
+ * 16, 32, 64, 128; C a multiple of 8 below 2^18; a window's rows of qkv below 2 GiB; Bw * num_heads
+ * below 2^31, and times ceil(L / 128) below 2^23 where L > 64; qkv, o, stats 16-byte aligned. */
 int nsw_position_attention(const void* qkv, const void* table, const int32_t* buckets, const float* mask,
                            int64_t nW_mask, void* o, float* stats, int64_t Bw, int64_t L, int64_t C,
                            int64_t num_heads, float scale, int64_t num_buckets, int64_t T, int64_t ws0, int64_t ws1,

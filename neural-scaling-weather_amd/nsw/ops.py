@@ -688,7 +688,8 @@ def position_attention(qkv: torch.Tensor, num_heads: int, scale: float, table: t
     buckets [(2T-1)(2A-1)(2W-1)] int32 (at most 8192), table [buckets, num_heads] in
     qkv's dtype.  ``mask`` [nW, L, L] or ``geometry`` as window_attention; a row whose
     mask leaves nothing gives zeros (k and v have to be finite also where they are masked, as
-    for the formula).  stats [Bw, num_heads, L, position_stats_width] fp32 for
+    for the formula).  Finite table and mask values may be as large as they go: a row of the lowest
+    alone is uniform, as in fp32.  stats [Bw, num_heads, L, position_stats_width] fp32 for
     position_attention_backward: each row's maximum m of z log2(e), log2 of its sum of
     2^(z log2(e) - m); bf16: then the bits that o's rounding lost."""
     what = "position_attention"

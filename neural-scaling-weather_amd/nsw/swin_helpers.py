@@ -307,7 +307,9 @@ def position_buckets(extent: Tuple[int, int, int], num_buckets: Optional[int] = 
     ``num_buckets`` each displacement has its own.  With it every axis of more than
     one token has that many (even, at least 4): half for either sign, half of those for
     the distances 0, 1, 2, ... one by one, the rest in steps that grow with the
-    logarithm of the distance up to ``max_distance``, the last for all beyond."""
+    logarithm of the distance up to ``max_distance``, the last for all beyond.  A displacement
+    is the query's place less the key's, and the second half is for the positive ones: a table
+    learned with the key's less the query's has its halves the other way round."""
     if num_buckets is not None and (num_buckets < 4 or num_buckets % 2):
         raise ValueError(f"position_buckets: num_buckets must be even and at least 4, got {num_buckets}")
     axes, sizes = [], []

@@ -10,11 +10,12 @@ and enqueue HIP kernels on the current stream, so they also run under CUDA
 graph capture.  Ops that write into a caller's tensor (``out=``) are not
 registered; their callers keep the ``nsw.ops`` functions.
 
-``linear`` (without GELU), ``gated_linear`` and ``residual_norm`` have
-gradients (``linear_backward``, ``gated_linear_backward``,
-``residual_norm_backward``); the others are forward only, and so are the modules
-that pack their parameters (attention, the blocks, the patch embedding): a
-backward pass to those parameters raises.
+``linear`` (without GELU), ``gated_linear``, ``residual_norm``, ``group_norm`` and
+``position_attention`` have gradients (``linear_backward``, ``gated_linear_backward``,
+``residual_norm_backward``, ``group_norm_backward``, ``position_attention_backward``),
+and so have the window maps (each the other); the others are forward only, and so are
+the modules that pack their parameters (``WindowMultiHeadAttention``, the blocks, the
+patch embedding): a backward pass to those parameters raises.
 
 The block parameters travel as one list in the field order of
 ``nsw_block_params`` (``BLOCK_PARAMS``), None for absent fields; shapes,

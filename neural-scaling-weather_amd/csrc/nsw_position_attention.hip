@@ -141,9 +141,7 @@ __global__ __launch_bounds__(64 * NKB, (NKB + 3) / 4) void whole_kernel(Args a) 
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
         const int4 k = *reinterpret_cast<const int4*>(kinfo + X::KEYS + 16 * kb + 4 * fg);
-        const int kn[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[kb][r] += ((qc ^ kn[r]) >> 30 ? -100.f * LOG2E : 0.f);
+        add_shift(S[kb], {qc, qc, qc, qc}, {k.x, k.y, k.z, k.w});
       }
     }
     if constexpr (MASK) {
@@ -274,6 +272,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void forward_kernel(Args a) {
 #pragma unroll
           for (int s = 0; s < D::NS; ++s) S[kb] = mma(row_frag<T, HD>(Ks + (16 * kb + fr) * D::STR, s, fg), q[s], S[kb]);
           logits(S[kb], zs, bias);
+          if (decltype(shift)::value) add_shift(S[kb], {qinfo, qinfo, qinfo, qinfo}, kn);
           if constexpr (MASK) {
             const f32x4 m4 = mask.get4(query, k0 + 16 * kb + 4 * fg);
 #pragma unroll

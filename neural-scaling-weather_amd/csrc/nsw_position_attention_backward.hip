@@ -210,12 +210,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void windows_kernel(Args a) 
             Z[qb] = mma(row_frag<T, HD>(Gs + (16 * qb + fr) * D::STR, s, fg), vf, Z[qb]);
           }
         }
+        logits(P[0], zs, B[0]);
+        logits(P[1], zs, B[1]);
+        if (shifted) {                                             // one branch (one a block: 180 x 360 x 1024 20 us more)
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) {
+            const int4 qi = *reinterpret_cast<const int4*>(r0 + 16 * qb + 4 * fg);
+            add_shift(P[qb], {qi.x, qi.y, qi.z, qi.w}, {kinfo, kinfo, kinfo, kinfo});
+            asm volatile("" : "+v"(P[qb]));
+          }
+        }
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
           const f32x4 m4 = *reinterpret_cast<const f32x4*>(r0 + QT + 16 * qb + 4 * fg);
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(r0 + 2 * QT + 16 * qb + 4 * fg);
           const f32x4 d4 = *reinterpret_cast<const f32x4*>(r0 + 3 * QT + 16 * qb + 4 * fg);
-          logits(P[qb], zs, B[qb]);
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -399,6 +408,7 @@ __global__ __launch_bounds__(NT, HD * (int)sizeof(T) >= 512 ? 1 : 2) void keys_k
         for (int b = 0; b < KB; ++b) {
           const int key = kw + 16 * b + fr;
           logits(P[qb][b], zs, B[b]);
+          if (shifted) add_shift(P[qb][b], {qi.x, qi.y, qi.z, qi.w}, {kinfo[b], kinfo[b], kinfo[b], kinfo[b]});
           if constexpr (MASK) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) P[qb][b][r] += in_units(M[b][r]);
@@ -529,6 +539,7 @@ __global__ __launch_bounds__(64 * WQ, HD * (int)sizeof(T) <= 128 ? 4 : 2) void q
             g4 = mma(row_frag<T, HD>(Vs + (k + fr) * D::STR, s, fg), g[s], g4);
           }
           logits(s4, zs, bias);
+          if (decltype(shift)::value) add_shift(s4, {qinfo, qinfo, qinfo, qinfo}, kn);
           if constexpr (MASK) {
             const f32x4 x = mask.get4(query, k0 + k + 4 * fg);
 #pragma unroll

@@ -126,3 +126,29 @@ def test_the_largest_mask_values(device, dtype, extent, high):
     m[1, :, L // 3] = high
     m[1, L - 1] = -math.inf
     check(run(t, device, mask=m), masked_reference(t, m), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extent,kind", [(e, k) for e in [(1, 3, 5), (1, 9, 18), (2, 9, 18), (1, 1, 700)]
+                                         for k in ["none", "shift", "mask"] if k != "shift" or e[1] > 1])
+@pytest.mark.parametrize("hd", [16, 64, 128])
+def test_probabilities_add_up_whatever_the_logits(device, dtype, extent, kind, hd):
+    """With ones for the gradient of o, dv summed over the keys is the sum of all probabilities: L, if the backward pass
+    forms each logit as the forward pass did.  Logits of 1e7 and more, whose fp32 steps change a probability by any factor.
+
+    A probability's exponent z - m - l: z - m is exact at the maximum and off by u |z - m| elsewhere, where p < 1 makes p
+    |z - m| at most 1/e a term; l, log2 of a sum of L terms, by (L + 8) u and a step of up to 2^-20; the sum over keys by
+    L u: (3 L + 64) u of L in all, and 16 u for l's step.  bf16: p and dv are rounded by 2^-8 each."""
+    T, A, W = extent
+    L, C = math.prod(extent), 2 * hd
+    tol = (3 * L + 80) * U + (2 * 2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+    g = torch.Generator().manual_seed(25)
+    how = {"none": {}, "shift": dict(geometry=(3 * A, 2 * W, (A, W), (A // 2, W // 2), T)),
+           "mask": dict(mask=torch.randn(2, L, L, generator=g))}[kind]
+    for factor in (1.0, 30.0, 300.0, 3000.0):
+        for std in (0.5, 1e6):
+            t = case(dtype, 6, extent, 2, hd, seed=26, std=std)
+            t["qkv"][..., :2 * C] *= factor
+            t["do"] = torch.ones_like(t["do"])
+            total = run(t, device, **how)["dqkv"][..., 2 * C:].double().sum(1) / L
+            assert ((total - 1).abs() <= tol).all(), (factor, std, (total - 1).abs().max().item(), tol)

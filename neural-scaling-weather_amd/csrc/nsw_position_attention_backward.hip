@@ -81,7 +81,7 @@ template <typename T, int HD, int WAVES> struct Windows {
   static constexpr size_t LDS = TILES + 2 * 4 * QT * sizeof(float);
 };
 
-// 180 x 360 x 1024 of 9 x 18 windows, 16 heads, bf16: 465-485 us, 1.3 GB at 2.8 TB/s, five
+// 180 x 360 x 1024 of 9 x 18 windows, 16 heads, bf16: 470-500 us, 1.3 GB at 2.8 TB/s, five
 // products at 0.22 PFLOP/s.  One workgroup of twelve waves a compute unit; vector instructions
 // 120 us of issue, matrix units 56, the rest LDS instructions (106 thousand a compute unit in 1.1
 // million cycles: every wave reads the tile of q and do twice, for 16 keys; bank conflicts are 5%
